@@ -42,6 +42,8 @@ enum {
   TTKV_ERR_BAD_BLOCK = 2,    /* a block id outside [0, num_blocks) inside a request's used prefix */
   TTKV_ERR_BAD_SLOT = 4,     /* slot_mapping entry past the cache (PAD entries, < 0, are skipped) */
   TTKV_ERR_SEQ_LEN = 8,      /* seq_lens[r] (or a query count) beyond what the call was sized for (clamped), or a continuation with seq_len < q_len */
+  TTKV_ERR_BAD_POSITION = 16, /* a rotary position outside [0, max_position) */
+  TTKV_ERR_NO_BLOCK = 32,    /* a step needs more blocks than its free list holds */
 };
 
 /* One layer's allocation. Mirrors TTKLayout(H, d, r1, qbits, res_k, res_bits, v_lanes, v_bits)
@@ -313,6 +315,115 @@ int ttkv_container_v_out(int32_t H, int32_t num_heads, int32_t d, int32_t B, int
                          const float* p, int64_t p_head_stride, int64_t p_batch_stride,
                          const uint8_t* v_bitmap, const uint8_t* v_packed, const float* v_scale,
                          int32_t v_pb, int32_t v_bits, float* out, ttkv_stream_t stream);
+
+/* ---- The 4-bit cache: rotated keys and values as 4-bit codes with a 16-bit scale per 32 dims, for
+ * layers and models that the compressed store above does not serve (it rotates the key of row t by
+ * position t, so positions with several axes are outside it, and it needs a calibrated layout and a
+ * fitted decoder). No counterpart in the reference. d == 128.
+ *
+ * A group of 32 dims x of a token's key or value row is stored as
+ *   lo = min(0, min x), hi = max(0, max x)                 (x clamped to +-32640 first)
+ *   s  = (hi - lo) / 15 rounded up to 7 significant bits, at least 2^-14
+ *   z  = rint(-lo / s) in [0, 15],  c = clamp(rint(x / s) + z, 0, 15),  value = (c - z) * s
+ * (exact in fp16), with the parameter fp16 bits of s | z (s's low four bits are zero); a group that
+ * holds a NaN or an infinity has the parameter 0x7e00 and reads back as NaN.
+ *
+ * Page: slot s of block b, b * block_size + offset, at 144 * H bytes per slot (slot_stride, a
+ * multiple of 16, may be larger); block sizes are multiples of 16. Sixteen slots from a multiple of
+ * 16 make a tile of H records of 2,304 bytes at page + (s / 16) * 16 * slot_stride + h * 2304:
+ *      0  key codes, dword (qd * 16 + u) * 4 + g of token u: dims 32 g + 8 qd + j at bit
+ *         4 (j / 2) + 16 (j % 2), j = 0..7
+ *   1024  value codes, dword ((q4 * 16 + n) * 2 + pair) * 2 + quad: token 4 q4 + 2 pair in its low
+ *         half, the next one in its high half, dims 32 (2 quad + gg) + 2 n + b at bit 4 (2 gg + b)
+ *   2048  key parameters, 16 bits each at u * 4 + g
+ *   2176  value parameters, 16 bits each at (q4 * 4 + g) * 4 + u % 4 */
+
+/* A step's block tables, slot map and positions from its requests' lengths, one launch.
+ * Request r has computed_lens[r] = c tokens stored and query_lens[r] = n new ones; it holds the
+ * first ceil(c / block_size) entries of its block_table row and gets ceil((c + n) / block_size) in
+ * all: its fresh ones are the next ids of free_blocks in order, request by request, and are written
+ * into the table (other entries are left alone). Writes
+ *   query_start_loc [num_reqs + 1]   prefix sums of n
+ *   seq_lens        [num_reqs]       c + n
+ *   slot_mapping    [num_tokens]     int64 slot of every new token, -1 past the last
+ *   positions       [num_tokens]     int64 c, c + 1, ...; 0 past the last
+ *   blocks_used     [1]              ids taken from free_blocks
+ * num_tokens is the padded token count the outputs are sized for. Conditions only the device sees:
+ * more tokens than num_tokens, a request longer than its row of max_blocks, or a negative length
+ * (taken as 0): TTKV_ERR_SEQ_LEN, the tokens without a place get slot -1; a free list that is too
+ * short: TTKV_ERR_NO_BLOCK, -1 for the missing ids and their slots; an id outside [0, num_blocks):
+ * TTKV_ERR_BAD_BLOCK, slot -1. At most 8,000 requests. Lengths saturate at 2^30 - 1. */
+int ttkv_step_plan(const int32_t* computed_lens, const int32_t* query_lens, int32_t num_reqs,
+                   int32_t* block_table, int64_t bt_row_stride, int32_t max_blocks,
+                   const int32_t* free_blocks, int32_t num_free, int32_t block_size,
+                   int64_t num_blocks, int32_t num_tokens, int32_t* query_start_loc,
+                   int32_t* seq_lens, int64_t* slot_mapping, int64_t* positions,
+                   int32_t* blocks_used, int32_t* error_word, ttkv_stream_t stream);
+
+/* Rotary positions with one to four axes (an image's tokens have a time, a row and a column).
+ * query [N, num_heads, d] and key [N, H, d] (same dtype; either may be absent with 0 heads) are
+ * rotated into query_out / key_out (which may be the inputs themselves): for j < half =
+ * rotary_dim / 2, with (cos, sin) of frequency j at the token's position on j's axis,
+ *   y[j] = x[j] cos - x[j + half] sin,   y[j + half] = x[j + half] cos + x[j] sin;
+ * dims past rotary_dim are copied. positions: int64, axis a of token i at a * axis_stride + i.
+ * sections [axes] (host memory) add up to half: frequencies in a row, sections[0] of axis 0 first;
+ * or, interleaved, j belongs to axis a = j % axes where j < axes * sections[a], else to axis 0.
+ * cos_sin_cache [max_position, rotary_dim] fp32: cos in columns [0, half), sin in [half, 2 half).
+ * Products and sums in 32 bits, rounded once. A token with a position outside the table sets
+ * TTKV_ERR_BAD_POSITION and its rows become NaN. */
+int ttkv_rotary_axes(const void* query, const void* key, void* query_out, void* key_out,
+                     int32_t dtype, int32_t num_tokens, int32_t num_heads, int32_t H, int32_t d,
+                     int64_t q_row_stride, int64_t k_row_stride, int64_t q_out_row_stride,
+                     int64_t k_out_row_stride, const int64_t* positions, int64_t axis_stride,
+                     int32_t axes, const int32_t* sections, int32_t interleaved,
+                     const float* cos_sin_cache, int64_t max_position, int32_t rotary_dim,
+                     int32_t* error_word, ttkv_stream_t stream);
+
+/* Quantise key / value [N, H, d] (fp32, fp16 or bf16; rotated keys) into their slots of the 4-bit
+ * cache. slot_mapping as for ttkv_write_paged: entries < 0 are padded tokens (skipped), entries
+ * past the cache set TTKV_ERR_BAD_SLOT; the slots of one call are distinct. key_out / value_out
+ * (optional, fp16 [N, H, d]) receive the values that the slots then stand for; rows of skipped
+ * tokens are left alone. Bytes are an exact function of the inputs. */
+int ttkv_nibble_write_paged(int32_t H, int32_t d, const void* key, int32_t k_dtype,
+                            int64_t k_row_stride, const void* value, int32_t v_dtype,
+                            int64_t v_row_stride, const int64_t* slot_mapping, int32_t num_tokens,
+                            uint8_t* page, int64_t n_slots, int64_t slot_stride, void* key_out,
+                            void* value_out, int32_t* error_word, ttkv_stream_t stream);
+
+/* Attention of one query per request over the 4-bit cache, the whole batch in one call; arguments
+ * as for ttkv_decode_paged, query and out fp16 or bf16, up to 16 query heads per KV head.
+ *   out[p] = sum_t softmax_t(scale * q[p] . K[t]) * V[t],  t < seq_lens[r]
+ * An empty request's rows are 0. A block id outside the cache sets TTKV_ERR_BAD_BLOCK and makes its
+ * request's rows NaN. Keys and values enter the products exactly; the query is taken as fp16, and
+ * the softmax weight is rounded to fp16 once. */
+int64_t ttkv_nibble_decode_workspace_bytes(int32_t H, int32_t num_heads, int32_t num_reqs,
+                                           int32_t max_seq_len);
+int ttkv_nibble_decode_paged(int32_t H, int32_t num_heads, int32_t d, float scale,
+                             const void* query, int32_t q_dtype, int64_t q_row_stride,
+                             const uint8_t* page, int64_t n_slots, int64_t slot_stride,
+                             int32_t block_size, const int32_t* block_table,
+                             int64_t bt_row_stride, int32_t max_blocks, const int32_t* seq_lens,
+                             const int32_t* query_start_loc, int32_t num_reqs,
+                             int32_t max_seq_len, void* out, int32_t out_dtype,
+                             int64_t out_row_stride, void* workspace, int64_t workspace_bytes,
+                             int32_t* error_word, ttkv_stream_t stream);
+
+/* Causal attention of chunks of queries over the 4-bit cache: request r's Q queries sit at the end
+ * of its n = seq_lens[r] stored keys (their own included; a first chunk has n = Q), query j sees
+ * keys t <= n - Q + j. Arguments as for ttkv_prefill_paged, limits and precision as above. A request
+ * with n < Q sets TTKV_ERR_SEQ_LEN and its rows become NaN. */
+int64_t ttkv_nibble_prefill_workspace_bytes(int32_t H, int32_t num_heads, int32_t num_reqs,
+                                            int32_t max_q_len, int32_t max_seq_len);
+int ttkv_nibble_prefill_paged(int32_t H, int32_t num_heads, int32_t d, float scale,
+                              const void* query, int32_t q_dtype, int64_t q_row_stride,
+                              const uint8_t* page, int64_t n_slots, int64_t slot_stride,
+                              int32_t block_size, const int32_t* block_table,
+                              int64_t bt_row_stride, int32_t max_blocks, const int32_t* seq_lens,
+                              const int32_t* query_start_loc, const int32_t* req_index,
+                              int32_t num_reqs, int32_t max_q_len, int32_t max_seq_len, void* out,
+                              int32_t out_dtype, int64_t out_row_stride, void* workspace,
+                              int64_t workspace_bytes, int32_t* error_word,
+                              ttkv_stream_t stream);
 
 /* Message for the last nonzero return on this thread. */
 const char* ttkv_last_error(void);

@@ -236,4 +236,86 @@ int ttkv_container_v_out(int32_t H, int32_t num_heads, int32_t d, int32_t B, int
                          v_packed, v_scale, v_pb, v_bits, out, (hipStream_t)stream);
 }
 
+int ttkv_step_plan(const int32_t* computed_lens, const int32_t* query_lens, int32_t num_reqs,
+                   int32_t* block_table, int64_t bt_row_stride, int32_t max_blocks,
+                   const int32_t* free_blocks, int32_t num_free, int32_t block_size,
+                   int64_t num_blocks, int32_t num_tokens, int32_t* query_start_loc,
+                   int32_t* seq_lens, int64_t* slot_mapping, int64_t* positions,
+                   int32_t* blocks_used, int32_t* error_word, ttkv_stream_t stream) {
+  return step_plan(computed_lens, query_lens, num_reqs, block_table, bt_row_stride, max_blocks,
+                   free_blocks, num_free, block_size, num_blocks, num_tokens, query_start_loc,
+                   seq_lens, slot_mapping, positions, blocks_used, error_word,
+                   (hipStream_t)stream);
+}
+
+int ttkv_rotary_axes(const void* query, const void* key, void* query_out, void* key_out,
+                     int32_t dtype, int32_t num_tokens, int32_t num_heads, int32_t H, int32_t d,
+                     int64_t q_row_stride, int64_t k_row_stride, int64_t q_out_row_stride,
+                     int64_t k_out_row_stride, const int64_t* positions, int64_t axis_stride,
+                     int32_t axes, const int32_t* sections, int32_t interleaved,
+                     const float* cos_sin_cache, int64_t max_position, int32_t rotary_dim,
+                     int32_t* error_word, ttkv_stream_t stream) {
+  return rotary_axes(query, key, query_out, key_out, dtype, num_tokens, num_heads, H, d,
+                     q_row_stride, k_row_stride, q_out_row_stride, k_out_row_stride, positions,
+                     axis_stride, axes, sections, interleaved, cos_sin_cache, max_position,
+                     rotary_dim, error_word, (hipStream_t)stream);
+}
+
+int ttkv_nibble_write_paged(int32_t H, int32_t d, const void* key, int32_t k_dtype,
+                            int64_t k_row_stride, const void* value, int32_t v_dtype,
+                            int64_t v_row_stride, const int64_t* slot_mapping, int32_t num_tokens,
+                            uint8_t* page, int64_t n_slots, int64_t slot_stride, void* key_out,
+                            void* value_out, int32_t* error_word, ttkv_stream_t stream) {
+  return nibble_write_paged(H, d, key, k_dtype, k_row_stride, value, v_dtype, v_row_stride,
+                            slot_mapping, num_tokens, page, n_slots, slot_stride, key_out,
+                            value_out, error_word, (hipStream_t)stream);
+}
+
+int64_t ttkv_nibble_decode_workspace_bytes(int32_t H, int32_t num_heads, int32_t num_reqs,
+                                           int32_t max_seq_len) {
+  if (H <= 0 || num_heads <= 0 || num_heads % H || num_reqs < 0 || max_seq_len < 0) return -1;
+  return nibble_decode_workspace_bytes(H, num_heads, num_reqs, max_seq_len);
+}
+
+int ttkv_nibble_decode_paged(int32_t H, int32_t num_heads, int32_t d, float scale,
+                             const void* query, int32_t q_dtype, int64_t q_row_stride,
+                             const uint8_t* page, int64_t n_slots, int64_t slot_stride,
+                             int32_t block_size, const int32_t* block_table,
+                             int64_t bt_row_stride, int32_t max_blocks, const int32_t* seq_lens,
+                             const int32_t* query_start_loc, int32_t num_reqs,
+                             int32_t max_seq_len, void* out, int32_t out_dtype,
+                             int64_t out_row_stride, void* workspace, int64_t workspace_bytes,
+                             int32_t* error_word, ttkv_stream_t stream) {
+  return nibble_decode_paged(H, num_heads, d, scale, query, q_dtype, q_row_stride, page, n_slots,
+                             slot_stride, block_size, block_table, bt_row_stride, max_blocks,
+                             seq_lens, query_start_loc, num_reqs, max_seq_len, out, out_dtype,
+                             out_row_stride, workspace, workspace_bytes, error_word,
+                             (hipStream_t)stream);
+}
+
+int64_t ttkv_nibble_prefill_workspace_bytes(int32_t H, int32_t num_heads, int32_t num_reqs,
+                                            int32_t max_q_len, int32_t max_seq_len) {
+  if (H <= 0 || num_heads <= 0 || num_heads % H || num_reqs < 0 || max_q_len < 0 ||
+      max_seq_len < 0)
+    return -1;
+  return nibble_prefill_workspace_bytes(H, num_heads, num_reqs, max_q_len, max_seq_len);
+}
+
+int ttkv_nibble_prefill_paged(int32_t H, int32_t num_heads, int32_t d, float scale,
+                              const void* query, int32_t q_dtype, int64_t q_row_stride,
+                              const uint8_t* page, int64_t n_slots, int64_t slot_stride,
+                              int32_t block_size, const int32_t* block_table,
+                              int64_t bt_row_stride, int32_t max_blocks, const int32_t* seq_lens,
+                              const int32_t* query_start_loc, const int32_t* req_index,
+                              int32_t num_reqs, int32_t max_q_len, int32_t max_seq_len, void* out,
+                              int32_t out_dtype, int64_t out_row_stride, void* workspace,
+                              int64_t workspace_bytes, int32_t* error_word,
+                              ttkv_stream_t stream) {
+  return nibble_prefill_paged(H, num_heads, d, scale, query, q_dtype, q_row_stride, page, n_slots,
+                              slot_stride, block_size, block_table, bt_row_stride, max_blocks,
+                              seq_lens, query_start_loc, req_index, num_reqs, max_q_len,
+                              max_seq_len, out, out_dtype, out_row_stride, workspace,
+                              workspace_bytes, error_word, (hipStream_t)stream);
+}
+
 }  // extern "C"

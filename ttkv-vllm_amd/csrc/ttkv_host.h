@@ -123,3 +123,36 @@ int container_v_out(int H, int HQ, int d, int B, int n, const float* p, int64_t 
                     int64_t p_batch_stride, const uint8_t* bm, const uint8_t* pk, const float* rs,
                     int pb, int bits, float* o, hipStream_t st);
 }  // namespace ttkv
+
+namespace ttkv {
+int step_plan(const int32_t* computed, const int32_t* qlens, int R, int32_t* bt,
+              int64_t bt_row_stride, int W, const int32_t* free_ids, int F, int bs,
+              int64_t num_blocks, int T, int32_t* qsl, int32_t* seq, int64_t* slots, int64_t* pos,
+              int32_t* used, int32_t* err, hipStream_t st);
+int rotary_axes(const void* q, const void* k, void* qo, void* ko, int dtype, int N, int HQ, int H,
+                int d, int64_t q_stride, int64_t k_stride, int64_t qo_stride, int64_t ko_stride,
+                const int64_t* pos, int64_t pos_stride, int axes, const int32_t* sections,
+                int interleaved, const float* cs, int64_t max_pos, int rot, int32_t* err,
+                hipStream_t st);
+// A 4-bit cache's page: geometry, alignment, whole tiles.
+int nibble_check_page(int H, int d, const uint8_t* page, int64_t n_slots, int64_t slot_stride);
+int nibble_write_paged(int H, int d, const void* key, int k_dtype, int64_t k_row_stride,
+                       const void* val, int v_dtype, int64_t v_row_stride, const int64_t* slots,
+                       int num_tokens, uint8_t* page, int64_t n_slots, int64_t slot_stride,
+                       void* k_out, void* v_out, int32_t* err, hipStream_t st);
+int64_t nibble_decode_workspace_bytes(int H, int HQ, int num_reqs, int max_seq);
+int nibble_decode_paged(int H, int HQ, int d, float scale, const void* q, int q_dtype,
+                        int64_t q_row_stride, const uint8_t* page, int64_t n_slots,
+                        int64_t slot_stride, int bs, const int32_t* bt, int64_t bt_row_stride,
+                        int max_blocks, const int32_t* seq_lens, const int32_t* qsl, int num_reqs,
+                        int max_seq, void* out, int out_dtype, int64_t out_row_stride, void* ws,
+                        int64_t ws_bytes, int32_t* err, hipStream_t st);
+int64_t nibble_prefill_workspace_bytes(int H, int HQ, int num_reqs, int max_q, int max_seq);
+int nibble_prefill_paged(int H, int HQ, int d, float scale, const void* q, int q_dtype,
+                         int64_t q_row_stride, const uint8_t* page, int64_t n_slots,
+                         int64_t slot_stride, int bs, const int32_t* bt, int64_t bt_row_stride,
+                         int max_blocks, const int32_t* seq_lens, const int32_t* qsl,
+                         const int32_t* req_index, int num_reqs, int max_q, int max_seq,
+                         void* out, int out_dtype, int64_t out_row_stride, void* ws,
+                         int64_t ws_bytes, int32_t* err, hipStream_t st);
+}  // namespace ttkv

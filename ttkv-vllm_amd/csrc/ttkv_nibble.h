@@ -1,0 +1,44 @@
+// The 4-bit cache: 16-bit codes-and-scale records of rotated keys and values, one record per tile
+// of 16 slots and KV head.
+//
+// A group of 32 dims of a token's key (or value) row x is stored as 32 codes of 4 bits and one
+// 16-bit parameter:
+//   lo = min(0, min x), hi = max(0, max x)            (x clamped to +-32640 first)
+//   s  = (hi - lo) / 15 rounded up to 7 significant bits, at least 2^-14
+//   z  = rint(-lo / s) in [0, 15],  c = clamp(rint(x / s) + z, 0, 15),  value = (c - z) * s
+// s is an fp16 number whose low four mantissa bits are zero; the parameter holds z there. c - z has
+// 4 bits and s 7, so a value is exact in fp16: the reads feed it to the matrix units unrounded. A
+// group that holds a NaN or an infinity has the parameter 0x7e00 (s = NaN) and reads back as NaN.
+//
+// The slots of a block are taken 16 at a time (the block size is a multiple of 16); such a tile's
+// bytes are its slots' bytes together, H records of 2,304 bytes (144 bytes per slot and head).
+// Within a record the codes lie as the read's matrix operands want them, a lane's share of the
+// tile in 16 consecutive bytes:
+//      0  key codes: dword (qd * 16 + u) * 4 + g holds token u's dims 32 g + 8 qd + j (j = 0..7) at
+//         bits 4 (j / 2) + 16 (j % 2): a shift and a mask give two consecutive dims as 16-bit halves
+//   1024  value codes: dword ((q4 * 16 + n) * 2 + pair) * 2 + quad holds, in its low half, token
+//         4 q4 + 2 pair and, in its high half, the next one: each dims 32 (2 quad + gg) + 2 n + b at
+//         bits 4 (2 gg + b): the same shift and mask give two tokens of one dim
+//   2048  key parameters, u * 4 + g
+//   2176  value parameters, (q4 * 4 + g) * 4 + u % 4
+#pragma once
+
+#include "ttkv_device.h"
+
+namespace ttkv {
+
+constexpr int kNibTile = 16;       // slots per tile
+constexpr int kNibGroup = 32;      // dims per parameter
+constexpr int kNibRecord = 2304;   // bytes of a tile's record of one head
+constexpr int kNibSlot = kNibRecord / kNibTile;  // bytes per slot and head
+constexpr int kNibV = 1024;        // record offsets: value codes,
+constexpr int kNibKp = 2048;       // key parameters,
+constexpr int kNibVp = 2176;       // value parameters
+constexpr float kNibMax = 32640.f;       // values are clamped to this: 7.5 steps of the largest scale
+constexpr float kNibMinScale = 0x1p-14f; // the smallest normal fp16
+
+// Scale and zero code of a parameter.
+__device__ __forceinline__ float nib_scale(uint32_t p) { return f16_bits_to_float(p & 0xfff0u); }
+__device__ __forceinline__ float nib_zero(uint32_t p) { return (float)(p & 15u); }
+
+}  // namespace ttkv

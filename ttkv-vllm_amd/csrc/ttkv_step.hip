@@ -1,0 +1,292 @@
+// A serving step's bookkeeping: block tables, slot map and positions from the requests' lengths
+// (step_plan), and rotary positions with one to four axes (rotary_axes). gfx950 / CDNA4.
+#include <math.h>
+
+#include "ttkv_device.h"
+#include "ttkv_host.h"
+
+namespace ttkv {
+
+// ------------------------------------------------------------------------------- step plan
+// One launch. Request r has c stored and n new tokens: it holds have = ceil(c / bs) blocks and needs
+// ceil((c + n) / bs); its fresh ones come from the free list at the sum of the requests' before it.
+// Every workgroup forms the two prefix sums (new tokens, fresh blocks) over all requests in LDS (a
+// few thousand integers from L2, cheaper than a second launch that waits for a first) and then
+// takes its share of the tokens, finding each one's request by bisection. A token of a fresh block
+// reads its block id from the free list and not from the table, which other workgroups are writing.
+constexpr int kPlanThreads = 256;
+constexpr int kPlanTokens = 4;        // tokens per thread the grid is sized for
+constexpr int kPlanMaxReqs = 8000;    // two prefix arrays within 64 KB of LDS
+constexpr int kPlanCap = (1 << 30) - 1;  // lengths and their sums saturate here
+
+struct PlanArgs {
+  const int32_t* computed;
+  const int32_t* qlens;
+  int R;
+  int32_t* bt;
+  int64_t bt_row_stride;
+  int W;
+  const int32_t* free_ids;
+  int F;
+  int bs;
+  int64_t num_blocks;
+  int T;
+  int32_t* qsl;
+  int32_t* seq;
+  int64_t* slots;
+  int64_t* pos;
+  int32_t* used;
+  int32_t* err;
+};
+
+__device__ __forceinline__ int sat_add(int a, int b) { return min(a + b, kPlanCap); }
+__device__ __forceinline__ int plan_len(int v) { return min(max(v, 0), kPlanCap); }
+__device__ __forceinline__ int div_up(int a, int b) { return a / b + (a % b != 0); }
+
+// Last index r in [0, n) with v[r] <= x; v ascends and v[0] = 0 <= x.
+__device__ __forceinline__ int last_not_above(const int* v, int n, int x) {
+  int lo = 0, hi = n;
+  while (hi - lo > 1) {
+    const int m = (lo + hi) >> 1;
+    if (v[m] <= x) lo = m;
+    else hi = m;
+  }
+  return lo;
+}
+
+__global__ __launch_bounds__(kPlanThreads) void step_plan_kernel(PlanArgs a) {
+  extern __shared__ int sh[];
+  int* qstart = sh;             // [R] first token of each request
+  int* fstart = sh + a.R;       // [R] its first fresh block in the free list
+  __shared__ int wsum[2][kPlanThreads / 64];
+  const int tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
+  const int per = (a.R + kPlanThreads - 1) / kPlanThreads;
+  const int r0 = min(tid * per, a.R), r1 = min(r0 + per, a.R);
+  int sq = 0, sf = 0, bits = 0;
+  for (int r = r0; r < r1; ++r) {
+    const int cr = a.computed[r], nr = a.qlens[r];
+    const int c = plan_len(cr), n = plan_len(nr);
+    if (c != cr || n != nr) bits |= TTKV_ERR_SEQ_LEN;
+    const int s = sat_add(c, n);
+    const int have = min(div_up(c, a.bs), a.W), need = min(div_up(s, a.bs), a.W);
+    if (div_up(s, a.bs) > a.W) bits |= TTKV_ERR_SEQ_LEN;
+    qstart[r] = sq;
+    fstart[r] = sf;
+    sq = sat_add(sq, n);
+    sf = sat_add(sf, need - have);
+  }
+  // inclusive scans of the threads' sums over the workgroup
+  int iq = sq, jf = sf;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const int tq = __shfl_up(iq, o), tf = __shfl_up(jf, o);
+    if (lane >= o) {
+      iq = sat_add(iq, tq);
+      jf = sat_add(jf, tf);
+    }
+  }
+  if (lane == 63) {
+    wsum[0][wv] = iq;
+    wsum[1][wv] = jf;
+  }
+  __syncthreads();
+  int bq = 0, bf = 0, total = 0, fresh = 0;
+  for (int w = 0; w < kPlanThreads / 64; ++w) {
+    if (w < wv) {
+      bq = sat_add(bq, wsum[0][w]);
+      bf = sat_add(bf, wsum[1][w]);
+    }
+    total = sat_add(total, wsum[0][w]);
+    fresh = sat_add(fresh, wsum[1][w]);
+  }
+  const int uq = __shfl_up(iq, 1), uf = __shfl_up(jf, 1);
+  bq = sat_add(bq, lane ? uq : 0);
+  bf = sat_add(bf, lane ? uf : 0);
+  for (int r = r0; r < r1; ++r) {
+    qstart[r] = sat_add(qstart[r], bq);
+    fstart[r] = sat_add(fstart[r], bf);
+  }
+  __syncthreads();
+  const int gid = blockIdx.x * kPlanThreads + tid;
+  const int step = gridDim.x * kPlanThreads;
+  if (total > a.T) bits |= TTKV_ERR_SEQ_LEN;
+  if (fresh > a.F) bits |= TTKV_ERR_NO_BLOCK;
+  for (int r = gid; r < a.R; r += step) {
+    a.qsl[r] = min(qstart[r], a.T);
+    a.seq[r] = sat_add(plan_len(a.computed[r]), plan_len(a.qlens[r]));
+  }
+  if (gid == 0) {
+    a.qsl[a.R] = min(total, a.T);
+    *a.used = min(fresh, a.F);
+  }
+  for (int f = gid; f < fresh; f += step) {
+    const int r = last_not_above(fstart, a.R, f);
+    const int col = div_up(plan_len(a.computed[r]), a.bs) + f - fstart[r];
+    const int id = f < a.F ? a.free_ids[f] : -1;
+    a.bt[(int64_t)r * a.bt_row_stride + col] = id;
+  }
+  for (int i = gid; i < a.T; i += step) {
+    int64_t slot = -1, pos = 0;
+    if (i < total) {
+      const int r = last_not_above(qstart, a.R, i);
+      const int c = plan_len(a.computed[r]);
+      const int p = sat_add(c, i - qstart[r]);
+      const int have = div_up(c, a.bs), col = p / a.bs;
+      pos = p;
+      if (col < a.W) {
+        int id = -1;
+        if (col < have) {
+          id = a.bt[(int64_t)r * a.bt_row_stride + col];
+        } else {
+          const int f = fstart[r] + col - have;
+          if (f < a.F) id = a.free_ids[f];
+        }
+        if (id >= 0 && id < a.num_blocks)
+          slot = (int64_t)id * a.bs + p % a.bs;
+        else if (col < have || fstart[r] + col - have < a.F)
+          bits |= TTKV_ERR_BAD_BLOCK;
+      }
+    }
+    a.slots[i] = slot;
+    a.pos[i] = pos;
+  }
+  if (bits) atomicOr(a.err, bits);
+}
+
+int step_plan(const int32_t* computed, const int32_t* qlens, int R, int32_t* bt,
+              int64_t bt_row_stride, int W, const int32_t* free_ids, int F, int bs,
+              int64_t num_blocks, int T, int32_t* qsl, int32_t* seq, int64_t* slots, int64_t* pos,
+              int32_t* used, int32_t* err, hipStream_t st) {
+  if (R < 0 || T < 0 || F < 0 || W < 0 || num_blocks < 0)
+    return host_fail(TTKV_E_INVALID, "negative count");
+  if (R > kPlanMaxReqs)
+    return host_fail(TTKV_E_UNSUPPORTED, "step_plan takes at most 8000 requests");
+  if (bs <= 0) return host_fail(TTKV_E_INVALID, "block_size must be positive");
+  if (bt_row_stride < W) return host_fail(TTKV_E_INVALID, "block table rows overlap");
+  if (T > kPlanCap || num_blocks > 0x7fffffff)
+    return host_fail(TTKV_E_INVALID, "too many tokens or blocks for one call");
+  if (!qsl || !used || !err || (R && (!computed || !qlens || !seq)) || (R && W && !bt) ||
+      (F && !free_ids) || (T && (!slots || !pos)))
+    return host_fail(TTKV_E_INVALID, "null pointer argument");
+  PlanArgs a{computed, qlens, R, bt,  bt_row_stride, W,     free_ids, F,   bs,
+             num_blocks, T,   qsl, seq, slots, pos, used, err};
+  const int grid = std::max(1, (T + kPlanThreads * kPlanTokens - 1) / (kPlanThreads * kPlanTokens));
+  hipLaunchKernelGGL(step_plan_kernel, dim3(grid), dim3(kPlanThreads), (size_t)R * 8, st, a);
+  const hipError_t e = hipGetLastError();
+  if (e != hipSuccess)
+    return host_fail(TTKV_E_LAUNCH, std::string("step plan launch: ") + hipGetErrorString(e));
+  return TTKV_OK;
+}
+
+// ----------------------------------------------------------------------------- rotary axes
+// y[j] = x[j] cos - x[j + half] sin,  y[j + half] = x[j + half] cos + x[j] sin for j < half =
+// rot / 2, the angle row taken at the token's position on frequency j's axis; dims past rot are
+// copied. Products and sums in 32 bits, rounded once to the row's type.
+constexpr int kRotAxes = 4;
+
+struct RotArgs {
+  const void* q;
+  const void* k;
+  void* qo;
+  void* ko;
+  int dtype, HQ, H, d, half, N;
+  int64_t q_stride, k_stride, qo_stride, ko_stride;
+  const int64_t* pos;
+  int64_t pos_stride;  // between axes
+  int axes, interleaved;
+  int sec[kRotAxes];
+  const float* cs;
+  int64_t max_pos;
+  int32_t* err;
+};
+
+__device__ __forceinline__ int rot_axis(const RotArgs& a, int j) {
+  if (a.interleaved) {
+    const int ax = j % a.axes;
+    int n = a.sec[0];
+#pragma unroll
+    for (int i = 1; i < kRotAxes; ++i) n = ax == i ? a.sec[i] : n;
+    return j < a.axes * n ? ax : 0;
+  }
+  int ax = 0, end = a.sec[0];
+#pragma unroll
+  for (int i = 1; i < kRotAxes; ++i) {
+    if (i < a.axes && j >= end) ax = i;
+    end += a.sec[i];
+  }
+  return ax;
+}
+
+__global__ __launch_bounds__(256) void rotary_axes_kernel(RotArgs a) {
+  const int64_t tok = blockIdx.x;
+  int64_t p[kRotAxes];
+  bool ok = true;
+  for (int i = 0; i < kRotAxes; ++i) {
+    p[i] = i < a.axes ? a.pos[i * a.pos_stride + tok] : 0;
+    if (p[i] < 0 || p[i] >= a.max_pos) {
+      ok = false;
+      p[i] = 0;
+    }
+  }
+  if (!ok && threadIdx.x == 0) atomicOr(a.err, TTKV_ERR_BAD_POSITION);
+  const int per = a.half + (a.d - 2 * a.half);  // pairs, then the dims that are copied
+  for (int i = threadIdx.x; i < (a.HQ + a.H) * per; i += 256) {
+    const int head = i / per, j = i % per;
+    const bool is_q = head < a.HQ;
+    const void* src = is_q ? a.q : a.k;
+    void* dst = is_q ? a.qo : a.ko;
+    const int64_t hd = (int64_t)(is_q ? head : head - a.HQ) * a.d;
+    const int64_t from = tok * (is_q ? a.q_stride : a.k_stride) + hd;
+    const int64_t to = tok * (is_q ? a.qo_stride : a.ko_stride) + hd;
+    if (j >= a.half) {
+      const int x = j + a.half;
+      store_act(dst, a.dtype, to + x, ok ? load_act(src, a.dtype, from + x) : NAN);
+      continue;
+    }
+    const int64_t row = p[rot_axis(a, j)] * (2 * a.half);
+    const float c = ok ? a.cs[row + j] : NAN, s = a.cs[row + j + a.half];
+    const float x = load_act(src, a.dtype, from + j), y = load_act(src, a.dtype, from + j + a.half);
+    store_act(dst, a.dtype, to + j, x * c - y * s);
+    store_act(dst, a.dtype, to + j + a.half, y * c + x * s);
+  }
+}
+
+int rotary_axes(const void* q, const void* k, void* qo, void* ko, int dtype, int N, int HQ, int H,
+                int d, int64_t q_stride, int64_t k_stride, int64_t qo_stride, int64_t ko_stride,
+                const int64_t* pos, int64_t pos_stride, int axes, const int32_t* sections,
+                int interleaved, const float* cs, int64_t max_pos, int rot, int32_t* err,
+                hipStream_t st) {
+  if (dtype != TTKV_DTYPE_F32 && dtype != TTKV_DTYPE_F16 && dtype != TTKV_DTYPE_BF16)
+    return host_fail(TTKV_E_INVALID, "dtype must be fp32, fp16 or bf16");
+  if (N < 0 || HQ < 0 || H < 0 || d <= 0) return host_fail(TTKV_E_INVALID, "negative count");
+  if (rot <= 0 || rot % 2 || rot > d)
+    return host_fail(TTKV_E_INVALID, "the rotary dims must be even and at most the head dim");
+  if (axes < 1 || axes > kRotAxes) return host_fail(TTKV_E_INVALID, "one to four axes");
+  if (!sections) return host_fail(TTKV_E_INVALID, "null sections");
+  int sum = 0;
+  for (int i = 0; i < axes; ++i) {
+    if (sections[i] < 0) return host_fail(TTKV_E_INVALID, "negative section");
+    sum += sections[i];
+    if (interleaved && i && sections[i] && i + axes * (sections[i] - 1) >= rot / 2)
+      return host_fail(TTKV_E_INVALID, "an interleaved section runs past the frequencies");
+  }
+  if (sum != rot / 2)
+    return host_fail(TTKV_E_INVALID, "the sections must add up to half the rotary dims");
+  if (max_pos <= 0) return host_fail(TTKV_E_INVALID, "empty cos_sin_cache");
+  if (N == 0 || HQ + H == 0) return TTKV_OK;
+  if ((HQ && (!q || !qo)) || (H && (!k || !ko)) || !pos || !cs || !err)
+    return host_fail(TTKV_E_INVALID, "null pointer argument");
+  RotArgs a{q,        k,        qo,         ko,   dtype,      HQ,   H,           d, rot / 2, N,
+            q_stride, k_stride, qo_stride, ko_stride, pos, pos_stride, axes, interleaved != 0};
+  for (int i = 0; i < axes; ++i) a.sec[i] = sections[i];
+  a.cs = cs;
+  a.max_pos = max_pos;
+  a.err = err;
+  hipLaunchKernelGGL(rotary_axes_kernel, dim3(N), dim3(256), 0, st, a);
+  const hipError_t e = hipGetLastError();
+  if (e != hipSuccess)
+    return host_fail(TTKV_E_LAUNCH, std::string("rotary launch: ") + hipGetErrorString(e));
+  return TTKV_OK;
+}
+
+}  // namespace ttkv

@@ -23,6 +23,8 @@ ERR_NO_DECODER = 1
 ERR_BAD_BLOCK = 2
 ERR_BAD_SLOT = 4
 ERR_SEQ_LEN = 8
+ERR_BAD_POSITION = 16
+ERR_NO_BLOCK = 32
 
 
 class Layout(ctypes.Structure):
@@ -169,6 +171,47 @@ def lib():
         P, P, P, I32, I32,            # v_bitmap, v_packed, v_scale, v_pb, v_bits
         P, P,                         # out, stream
     ]
+    L.ttkv_step_plan.restype = ctypes.c_int
+    L.ttkv_step_plan.argtypes = [
+        P, P, I32, P, I64, I32,       # computed_lens, query_lens, num_reqs, block_table, stride, max_blocks
+        P, I32, I32, I64, I32,        # free_blocks, num_free, block_size, num_blocks, num_tokens
+        P, P, P, P, P, P, P,          # query_start_loc, seq_lens, slot_mapping, positions, blocks_used, error_word, stream
+    ]
+    L.ttkv_rotary_axes.restype = ctypes.c_int
+    L.ttkv_rotary_axes.argtypes = [
+        P, P, P, P, I32,              # query, key, query_out, key_out, dtype
+        I32, I32, I32, I32,           # num_tokens, num_heads, H, d
+        I64, I64, I64, I64,           # row strides: query, key, query_out, key_out
+        P, I64, I32, P, I32,          # positions, axis_stride, axes, sections, interleaved
+        P, I64, I32, P, P,            # cos_sin_cache, max_position, rotary_dim, error_word, stream
+    ]
+    L.ttkv_nibble_write_paged.restype = ctypes.c_int
+    L.ttkv_nibble_write_paged.argtypes = [
+        I32, I32, P, I32, I64,        # H, d, key, k_dtype, k_row_stride
+        P, I32, I64, P, I32,          # value, v_dtype, v_row_stride, slot_mapping, num_tokens
+        P, I64, I64, P, P, P, P,      # page, n_slots, slot_stride, key_out, value_out, error_word, stream
+    ]
+    L.ttkv_nibble_decode_workspace_bytes.restype = I64
+    L.ttkv_nibble_decode_workspace_bytes.argtypes = [I32, I32, I32, I32]
+    L.ttkv_nibble_decode_paged.restype = ctypes.c_int
+    L.ttkv_nibble_decode_paged.argtypes = [
+        I32, I32, I32, F32, P, I32, I64,  # H, num_heads, d, scale, query, q_dtype, q_row_stride
+        P, I64, I64, I32,             # page, n_slots, slot_stride, block_size
+        P, I64, I32, P, P, I32, I32,  # block_table, stride, max_blocks, seq_lens, qsl, num_reqs, max_seq_len
+        P, I32, I64,                  # out, out_dtype, out_row_stride
+        P, I64, P, P,                 # workspace, workspace_bytes, error_word, stream
+    ]
+    L.ttkv_nibble_prefill_workspace_bytes.restype = I64
+    L.ttkv_nibble_prefill_workspace_bytes.argtypes = [I32, I32, I32, I32, I32]
+    L.ttkv_nibble_prefill_paged.restype = ctypes.c_int
+    L.ttkv_nibble_prefill_paged.argtypes = [
+        I32, I32, I32, F32, P, I32, I64,  # H, num_heads, d, scale, query, q_dtype, q_row_stride
+        P, I64, I64, I32,             # page, n_slots, slot_stride, block_size
+        P, I64, I32, P, P, P,         # block_table, stride, max_blocks, seq_lens, qsl, req_index
+        I32, I32, I32,                # num_reqs, max_q_len, max_seq_len
+        P, I32, I64,                  # out, out_dtype, out_row_stride
+        P, I64, P, P,                 # workspace, workspace_bytes, error_word, stream
+    ]
     for name in EXPORTS:
         getattr(L, name)  # every declared symbol must resolve
     _LIB = L
@@ -181,7 +224,10 @@ EXPORTS = ("ttkv_last_error", "ttkv_decoder_ranks", "ttkv_blob_bytes",
            "ttkv_write_paged", "ttkv_prefill_workspace_bytes", "ttkv_prefill_paged", "ttkv_multi_scores_paged", "ttkv_multi_scores_workspace_bytes",
            "ttkv_dense_workspace_bytes",
            "ttkv_dense_decode_paged", "ttkv_write_workspace_bytes", "ttkv_container_krt",
-           "ttkv_container_v_out")
+           "ttkv_container_v_out", "ttkv_step_plan", "ttkv_rotary_axes",
+           "ttkv_nibble_write_paged", "ttkv_nibble_decode_workspace_bytes",
+           "ttkv_nibble_decode_paged", "ttkv_nibble_prefill_workspace_bytes",
+           "ttkv_nibble_prefill_paged")
 
 
 def check(rc: int, what: str) -> None:

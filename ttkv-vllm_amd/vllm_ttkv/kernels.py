@@ -6,11 +6,16 @@ must live on a HIP device; there is no CPU path.
 """
 from __future__ import annotations
 
+import ctypes
+import functools
+from typing import NamedTuple
+
 import torch
 
 from . import _hip
 from .decoder_pool import DecoderPool, decoder_ranks
 from .layout import TTKLayout
+from .nibble import NibbleLayout
 
 
 def _need_device(*ts):
@@ -384,3 +389,318 @@ def dense_decode_paged(query: torch.Tensor, k_cache: torch.Tensor, v_cache: torc
         workspace.data_ptr(), workspace.numel(), _hip.stream_ptr(query.device))
     _hip.check(rc, "ttkv_dense_decode_paged")
     return out
+
+
+# ---------------------------------------------------------------- the 4-bit cache
+def _on_device(fn):
+    """Run a wrapper with its first tensor argument's device current: a launch goes to the current
+    device, whatever device its stream belongs to. (The guard costs more than the checks, so it is
+    taken only where the device differs.)"""
+    @functools.wraps(fn)
+    def call(*args, **kw):
+        dev = next((a.device for a in args if isinstance(a, torch.Tensor)), None)
+        if dev is None or dev.type != "cuda" or dev.index == torch.cuda.current_device():
+            return fn(*args, **kw)
+        with torch.cuda.device(dev):
+            return fn(*args, **kw)
+    return call
+
+
+def _one_device(first, *ts):
+    """Refuse host tensors and tensors of another device than the first."""
+    dev = first.device
+    if dev.type != "cuda":
+        _need_device(first)
+    for t in ts:
+        if t is not None and t.device != dev:
+            _need_device(t)
+            raise ValueError(f"tensors on {dev} and {t.device} in one call")
+
+
+def _error_word(error_word, device):
+    if error_word is None:
+        return torch.zeros(1, dtype=torch.int32, device=device)
+    if error_word.dtype != torch.int32 or error_word.numel() < 1:
+        raise ValueError("error_word must be an int32 tensor")
+    return error_word
+
+
+def _rows(t, heads, d, what):
+    """Check [N, heads, d] rows, contiguous within a token."""
+    if t.dim() != 3 or t.shape[1] != heads or t.shape[2] != d:
+        raise ValueError(f"{what} must be [N, {heads}, {d}], got {tuple(t.shape)}")
+    if t.numel() and (t.stride(2) != 1 or (heads > 1 and t.stride(1) != d)):
+        raise ValueError(f"{what} must be contiguous within a token ([heads, {d}] rows)")
+
+
+class StepPlan(NamedTuple):
+    """A step's addresses (`step_plan`)."""
+    query_start_loc: torch.Tensor   # [R + 1] int32
+    seq_lens: torch.Tensor          # [R] int32, this step's tokens included
+    slot_mapping: torch.Tensor      # [num_tokens] int64, -1 past the last token
+    positions: torch.Tensor         # [num_tokens] int64, 0 past the last token
+    blocks_used: torch.Tensor       # [1] int32, ids taken from the free list
+
+
+def _plan_out(t, n, dtype, device, name):
+    if t is None:
+        return torch.empty(n, dtype=dtype, device=device)
+    if t.dtype != dtype or t.numel() != n or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous {dtype} tensor of {n}")
+    return t
+
+
+@_on_device
+def step_plan(computed_lens: torch.Tensor, query_lens: torch.Tensor, block_table: torch.Tensor,
+              free_blocks: torch.Tensor, block_size: int, num_blocks: int, num_tokens: int,
+              query_start_loc: torch.Tensor | None = None, seq_lens: torch.Tensor | None = None,
+              slot_mapping: torch.Tensor | None = None, positions: torch.Tensor | None = None,
+              blocks_used: torch.Tensor | None = None,
+              error_word: torch.Tensor | None = None) -> StepPlan:
+    """Block tables, slot map and positions of a step, from its requests' lengths, in one launch
+    with nothing read back. See `ttkv_step_plan` in include/ttkv_hip.h.
+
+    computed_lens / query_lens [R] int32: tokens stored before the step and new in it;
+    block_table [R, max_blocks] int32, updated in place; free_blocks [F] int32, taken from the
+    front; num_tokens: the (padded) token count of the outputs, at least the sum of query_lens."""
+    _one_device(computed_lens, query_lens, block_table, free_blocks, query_start_loc, seq_lens,
+                slot_mapping, positions, blocks_used, error_word)
+    _i32(computed_lens, "computed_lens")
+    _i32(query_lens, "query_lens")
+    _i32(free_blocks, "free_blocks")
+    R, dev = computed_lens.numel(), computed_lens.device
+    if query_lens.numel() != R:
+        raise ValueError(f"{R} computed lengths and {query_lens.numel()} query lengths")
+    if block_table.dtype != torch.int32 or block_table.dim() != 2 or block_table.shape[0] != R \
+            or (block_table.shape[1] > 1 and block_table.stride(1) != 1):
+        raise ValueError(f"block_table must be int32 [{R}, max_blocks] with contiguous rows")
+    n = int(num_tokens)
+    plan = StepPlan(_plan_out(query_start_loc, R + 1, torch.int32, dev, "query_start_loc"),
+                    _plan_out(seq_lens, R, torch.int32, dev, "seq_lens"),
+                    _plan_out(slot_mapping, n, torch.int64, dev, "slot_mapping"),
+                    _plan_out(positions, n, torch.int64, dev, "positions"),
+                    _plan_out(blocks_used, 1, torch.int32, dev, "blocks_used"))
+    err = _error_word(error_word, dev)
+    W = block_table.shape[1]
+    rc = _hip.lib().ttkv_step_plan(
+        computed_lens.data_ptr(), query_lens.data_ptr(), R, block_table.data_ptr(),
+        block_table.stride(0) if R > 1 else W, W, free_blocks.data_ptr(), free_blocks.numel(),
+        int(block_size), int(num_blocks), n, plan.query_start_loc.data_ptr(),
+        plan.seq_lens.data_ptr(), plan.slot_mapping.data_ptr(), plan.positions.data_ptr(),
+        plan.blocks_used.data_ptr(), err.data_ptr(), _hip.stream_ptr(dev))
+    _hip.check(rc, "ttkv_step_plan")
+    return plan
+
+
+@functools.lru_cache(maxsize=64)
+def _c_sections(sections: tuple) -> ctypes.Array:
+    return (ctypes.c_int32 * len(sections))(*sections)
+
+
+@_on_device
+def rotary_axes(query: torch.Tensor, key: torch.Tensor | None, positions: torch.Tensor,
+                cos_sin_cache: torch.Tensor, sections, interleaved: bool = False,
+                query_out: torch.Tensor | None = None, key_out: torch.Tensor | None = None,
+                error_word: torch.Tensor | None = None):
+    """Rotate query [N, HQ, d] and key [N, H, d] by positions of one to four axes; returns
+    (query_out, key_out), which may be the inputs. See `ttkv_rotary_axes` in include/ttkv_hip.h.
+
+    positions [axes, N] (or [N] for one axis) int64; sections: how many of the rotary_dim / 2
+    frequencies each axis has, in a row, or dealt in turn where `interleaved`; cos_sin_cache
+    [max_pos, rotary_dim] fp32 (vLLM layout)."""
+    _one_device(query, key, positions, cos_sin_cache, query_out, key_out, error_word)
+    if query.dim() != 3:
+        raise ValueError(f"query must be [N, heads, d], got {tuple(query.shape)}")
+    N, HQ, d = query.shape
+    sections = tuple(int(s) for s in sections)
+    if positions.dtype != torch.int64 or positions.shape[-1] != N \
+            or positions.numel() != len(sections) * N:
+        raise ValueError(f"positions must be int64 [{len(sections)}, {N}], got "
+                         f"{positions.dtype} {tuple(positions.shape)}")
+    if N > 1 and positions.stride(-1) != 1:
+        raise ValueError("an axis's positions must be contiguous")
+    if cos_sin_cache.dtype != torch.float32 or cos_sin_cache.dim() != 2 \
+            or not cos_sin_cache.is_contiguous():
+        raise ValueError("cos_sin_cache must be contiguous fp32 [max_pos, rotary_dim]")
+    if query.dtype not in _hip.DTYPE_CODE:
+        raise ValueError("query dtype must be fp32, fp16 or bf16")
+    query_out = torch.empty_like(query) if query_out is None else query_out
+    H = 0
+    if key is not None:
+        H = key.shape[1] if key.dim() == 3 else 0
+        key_out = torch.empty_like(key) if key_out is None else key_out
+    for t, heads, what in ((query, HQ, "query"), (query_out, HQ, "query_out"), (key, H, "key"),
+                           (key_out, H, "key_out")):
+        if t is None:
+            continue
+        _rows(t, heads, d, what)
+        if t.shape[0] != N or t.dtype != query.dtype:
+            raise ValueError(f"{what} must have the query's {N} tokens and dtype")
+    err = _error_word(error_word, query.device)
+    rc = _hip.lib().ttkv_rotary_axes(
+        query.data_ptr(), _hip.ptr(key), query_out.data_ptr(), _hip.ptr(key_out),
+        _hip.DTYPE_CODE[query.dtype], N, HQ, H, d, query.stride(0),
+        0 if key is None else key.stride(0), query_out.stride(0),
+        0 if key is None else key_out.stride(0), positions.data_ptr(),
+        positions.stride(0) if positions.dim() == 2 else N, len(sections), _c_sections(sections),
+        int(bool(interleaved)), cos_sin_cache.data_ptr(), cos_sin_cache.shape[0],
+        cos_sin_cache.shape[1], err.data_ptr(), _hip.stream_ptr(query.device))
+    _hip.check(rc, "ttkv_rotary_axes")
+    return query_out, key_out
+
+
+@_on_device
+def nibble_write_paged(lay: NibbleLayout, key: torch.Tensor, value: torch.Tensor,
+                       slot_mapping: torch.Tensor, page: torch.Tensor,
+                       key_out: torch.Tensor | None = None,
+                       value_out: torch.Tensor | None = None,
+                       error_word: torch.Tensor | None = None) -> None:
+    """Quantise key / value [N, H, d] (rotated keys) into their slots of a 4-bit cache.
+
+    page: the layer's cache, its last dim one slot (`lay.compressed_bytes_per_token()` bytes or
+    more); slot_mapping [>= N] int64, -1 for padded tokens; key_out / value_out (optional, fp16
+    [N, H, d], contiguous) receive what the slots then stand for. See `ttkv_nibble_write_paged`."""
+    _one_device(key, value, slot_mapping, page, key_out, value_out, error_word)
+    N = key.shape[0]
+    for t, what in ((key, "key"), (value, "value")):
+        _rows(t, lay.H, lay.d, what)
+        if t.shape[0] != N:
+            raise ValueError(f"{N} keys and {t.shape[0]} values")
+        if t.dtype not in _hip.DTYPE_CODE:
+            raise ValueError(f"{what} dtype must be fp32, fp16 or bf16")
+    for t, what in ((key_out, "key_out"), (value_out, "value_out")):
+        if t is not None and (t.shape != key.shape or t.dtype != torch.float16
+                              or not t.is_contiguous()):
+            raise ValueError(f"{what} must be contiguous fp16 [{N}, {lay.H}, {lay.d}]")
+    if slot_mapping.dtype != torch.int64 or slot_mapping.numel() < N \
+            or not slot_mapping.is_contiguous():
+        raise ValueError("slot_mapping must be contiguous int64 with one id per token")
+    if not page.is_contiguous():
+        raise ValueError("the cache page must be contiguous")
+    page_ptr, n_slots, slot_bytes = _page_args(page, lay.compressed_bytes_per_token())
+    err = _error_word(error_word, key.device)
+    rc = _hip.lib().ttkv_nibble_write_paged(
+        lay.H, lay.d, key.data_ptr(), _hip.DTYPE_CODE[key.dtype], key.stride(0), value.data_ptr(),
+        _hip.DTYPE_CODE[value.dtype], value.stride(0), slot_mapping.data_ptr(), N, page_ptr,
+        n_slots, slot_bytes, _hip.ptr(key_out), _hip.ptr(value_out), err.data_ptr(),
+        _hip.stream_ptr(key.device))
+    _hip.check(rc, "ttkv_nibble_write_paged")
+
+
+def _nibble_read(lay, query, page, block_table, seq_lens, query_start_loc, out):
+    """Checks shared by the 4-bit reads; returns (page pointer, slots, bytes per slot, out)."""
+    _rows(query, query.shape[1] if query.dim() == 3 else 0, lay.d, "query")
+    if out is None:
+        out = torch.empty_like(query)
+    _one_device(query, page, block_table, seq_lens, query_start_loc, out)
+    _rows(out, query.shape[1], lay.d, "out")
+    if out.shape[0] != query.shape[0]:
+        raise ValueError("out must match query's shape")
+    for t, what in ((query, "query"), (out, "out")):
+        if t.dtype not in (torch.float16, torch.bfloat16):
+            raise ValueError(f"{what} dtype must be fp16 or bf16")
+    if block_table.dtype != torch.int32 or block_table.dim() != 2 \
+            or (block_table.shape[1] > 1 and block_table.stride(1) != 1):
+        raise ValueError("block_table must be int32 [requests, max_blocks] with contiguous rows")
+    _i32(seq_lens, "seq_lens")
+    _i32(query_start_loc, "query_start_loc")
+    if not page.is_contiguous():
+        raise ValueError("the cache page must be contiguous")
+    return *_page_args(page, lay.compressed_bytes_per_token()), out
+
+
+def nibble_decode_workspace(lay: NibbleLayout, num_heads: int, num_reqs: int, max_seq_len: int,
+                            device) -> torch.Tensor:
+    """A zero-filled workspace for `nibble_decode_paged` over this batch shape; its first 64 KiB
+    (counters) are left zero by every call, so a buffer this large serves later calls too."""
+    n = _hip.lib().ttkv_nibble_decode_workspace_bytes(lay.H, num_heads, num_reqs, max_seq_len)
+    if n < 0:
+        raise ValueError("invalid head count or batch for the decode workspace")
+    return torch.zeros(max(int(n), 256), dtype=torch.uint8, device=device)
+
+
+@_on_device
+def _nibble_decode(query, lay, page, block_size, block_table, seq_lens, query_start_loc,
+                   max_seq_len, scale, out, workspace, error_word):
+    page_ptr, n_slots, slot_bytes, out = _nibble_read(lay, query, page, block_table, seq_lens,
+                                                      query_start_loc, out)
+    B, HQ, dev = seq_lens.numel(), query.shape[1], query.device
+    if block_table.shape[0] < B or query_start_loc.numel() < B:
+        raise ValueError(f"{B} sequence lengths need as many block table rows and query rows")
+    if workspace is None:
+        workspace = nibble_decode_workspace(lay, HQ, B, max_seq_len, dev)
+    err = _error_word(error_word, dev)
+    _one_device(query, workspace, err)
+    rc = _hip.lib().ttkv_nibble_decode_paged(
+        lay.H, HQ, lay.d, float(scale), query.data_ptr(), _hip.DTYPE_CODE[query.dtype],
+        query.stride(0), page_ptr, n_slots, slot_bytes, int(block_size), block_table.data_ptr(),
+        block_table.stride(0), block_table.shape[1], seq_lens.data_ptr(),
+        query_start_loc.data_ptr(), B, int(max_seq_len), out.data_ptr(),
+        _hip.DTYPE_CODE[out.dtype], out.stride(0), workspace.data_ptr(), workspace.numel(),
+        err.data_ptr(), _hip.stream_ptr(dev))
+    _hip.check(rc, "ttkv_nibble_decode_paged")
+    return out
+
+
+def nibble_decode_paged(lay: NibbleLayout, query: torch.Tensor, page: torch.Tensor,
+                        block_size: int, block_table: torch.Tensor, seq_lens: torch.Tensor,
+                        query_start_loc: torch.Tensor, max_seq_len: int, scale: float,
+                        out: torch.Tensor | None = None, workspace: torch.Tensor | None = None,
+                        error_word: torch.Tensor | None = None) -> torch.Tensor:
+    """Attention of one query per request (row query_start_loc[r] of query [N, HQ, d], rotated)
+    over its seq_lens[r] stored tokens of a 4-bit cache. See `ttkv_nibble_decode_paged` in
+    include/ttkv_hip.h. Returns `out` [N, HQ, d] with the decode rows written."""
+    return _nibble_decode(query, lay, page, block_size, block_table, seq_lens, query_start_loc,
+                          max_seq_len, scale, out, workspace, error_word)
+
+
+def nibble_prefill_workspace(lay: NibbleLayout, num_heads: int, num_reqs: int, max_q_len: int,
+                             max_seq_len: int, device) -> torch.Tensor:
+    """A zero-filled workspace for `nibble_prefill_paged` over this batch shape."""
+    n = _hip.lib().ttkv_nibble_prefill_workspace_bytes(lay.H, num_heads, num_reqs, max_q_len,
+                                                       max_seq_len)
+    if n < 0:
+        raise ValueError("invalid head count or batch for the prefill workspace")
+    return torch.zeros(max(int(n), 256), dtype=torch.uint8, device=device)
+
+
+@_on_device
+def _nibble_prefill(query, lay, page, block_size, block_table, seq_lens, query_start_loc,
+                    max_q_len, max_seq_len, scale, req_index, out, workspace, error_word):
+    page_ptr, n_slots, slot_bytes, out = _nibble_read(lay, query, page, block_table, seq_lens,
+                                                      query_start_loc, out)
+    B, HQ, dev = seq_lens.numel(), query.shape[1], query.device
+    if block_table.shape[0] < B or query_start_loc.numel() < B + 1:
+        raise ValueError(f"{B} sequence lengths need as many block table rows and one more "
+                         f"query start")
+    if req_index is not None:
+        _i32(req_index, "req_index")
+        _one_device(query, req_index)
+        B = req_index.numel()
+    if workspace is None:
+        workspace = nibble_prefill_workspace(lay, HQ, B, max_q_len, max_seq_len, dev)
+    err = _error_word(error_word, dev)
+    _one_device(query, workspace, err)
+    rc = _hip.lib().ttkv_nibble_prefill_paged(
+        lay.H, HQ, lay.d, float(scale), query.data_ptr(), _hip.DTYPE_CODE[query.dtype],
+        query.stride(0), page_ptr, n_slots, slot_bytes, int(block_size), block_table.data_ptr(),
+        block_table.stride(0), block_table.shape[1], seq_lens.data_ptr(),
+        query_start_loc.data_ptr(), _hip.ptr(req_index), B, int(max_q_len), int(max_seq_len),
+        out.data_ptr(), _hip.DTYPE_CODE[out.dtype], out.stride(0), workspace.data_ptr(),
+        workspace.numel(), err.data_ptr(), _hip.stream_ptr(dev))
+    _hip.check(rc, "ttkv_nibble_prefill_paged")
+    return out
+
+
+def nibble_prefill_paged(lay: NibbleLayout, query: torch.Tensor, page: torch.Tensor,
+                         block_size: int, block_table: torch.Tensor, seq_lens: torch.Tensor,
+                         query_start_loc: torch.Tensor, max_q_len: int, max_seq_len: int,
+                         scale: float, req_index: torch.Tensor | None = None,
+                         out: torch.Tensor | None = None, workspace: torch.Tensor | None = None,
+                         error_word: torch.Tensor | None = None) -> torch.Tensor:
+    """Causal attention of chunks of queries (rows query_start_loc[r] .. [r + 1] of query
+    [N, HQ, d], rotated) over their requests' stored tokens of a 4-bit cache, the chunk's own
+    included. `req_index` picks the batch rows to process (default: all). See
+    `ttkv_nibble_prefill_paged` in include/ttkv_hip.h."""
+    return _nibble_prefill(query, lay, page, block_size, block_table, seq_lens, query_start_loc,
+                           max_q_len, max_seq_len, scale, req_index, out, workspace, error_word)
