@@ -136,6 +136,12 @@ int rotary_axes(const void* q, const void* k, void* qo, void* ko, int dtype, int
                 hipStream_t st);
 // A 4-bit cache's page: geometry, alignment, whole tiles.
 int nibble_check_page(int H, int d, const uint8_t* page, int64_t n_slots, int64_t slot_stride);
+// The 4-bit reads' arguments.
+int nibble_check_read(int H, int HQ, int d, const void* q, int q_dtype, int64_t q_row_stride,
+                      const uint8_t* page, int64_t n_slots, int64_t slot_stride, int bs,
+                      const int32_t* bt, int max_blocks, const int32_t* seq_lens,
+                      const int32_t* qsl, int num_reqs, int max_seq, const void* out,
+                      int out_dtype, int64_t out_row_stride, const int32_t* err);
 int nibble_write_paged(int H, int d, const void* key, int k_dtype, int64_t k_row_stride,
                        const void* val, int v_dtype, int64_t v_row_stride, const int64_t* slots,
                        int num_tokens, uint8_t* page, int64_t n_slots, int64_t slot_stride,

@@ -37,8 +37,18 @@ constexpr int kNibVp = 2176;       // value parameters
 constexpr float kNibMax = 32640.f;       // values are clamped to this: 7.5 steps of the largest scale
 constexpr float kNibMinScale = 0x1p-14f; // the smallest normal fp16
 
-// Scale and zero code of a parameter.
-__device__ __forceinline__ float nib_scale(uint32_t p) { return f16_bits_to_float(p & 0xfff0u); }
-__device__ __forceinline__ float nib_zero(uint32_t p) { return (float)(p & 15u); }
+// (c - z) * s of two codes as an fp16 pair, exactly: the codes' nibbles at bit 4 m of x's halves,
+// biased by 1024 (one unit in fp16's last place there), z likewise in zb = nib_bias(parameters),
+// s = nib_scales(parameters). The difference has 4 bits and s 7, so neither operation rounds.
+__device__ __forceinline__ half2v nib_bias(uint32_t p2) {
+  return __builtin_bit_cast(half2v, (p2 & 0x000f000fu) | 0x64006400u);
+}
+__device__ __forceinline__ half2v nib_scales(uint32_t p2) {
+  return __builtin_bit_cast(half2v, p2 & 0xfff0fff0u);
+}
+__device__ __forceinline__ half2v nib_pair(uint32_t x, int m, half2v zb, half2v s) {
+  const half2v c = __builtin_bit_cast(half2v, ((x >> (4 * m)) & 0x000f000fu) | 0x64006400u);
+  return (c - zb) * s;
+}
 
 }  // namespace ttkv

@@ -28,6 +28,9 @@ struct NibAttendArgs {
   int32_t* err;
 };
 
+__device__ __forceinline__ float nib_scale(uint32_t p) { return f16_bits_to_float(p & 0xfff0u); }
+__device__ __forceinline__ float nib_zero(uint32_t p) { return (float)(p & 15u); }
+
 // One wave per (request, query, query head): lane l owns dims 2 l and 2 l + 1.
 __global__ __launch_bounds__(64) void nibble_attend_kernel(NibAttendArgs a) {
   const int lane = threadIdx.x;
@@ -82,7 +85,7 @@ __global__ __launch_bounds__(64) void nibble_attend_kernel(NibAttendArgs a) {
   store_act(a.out, a.out_dtype, to + 1, ob * inv);
 }
 
-static int nibble_attend_check(int H, int HQ, int d, const void* q, int q_dtype,
+int nibble_check_read(int H, int HQ, int d, const void* q, int q_dtype,
                                int64_t q_row_stride, const uint8_t* page, int64_t n_slots,
                                int64_t slot_stride, int bs, const int32_t* bt, int max_blocks,
                                const int32_t* seq_lens, const int32_t* qsl, int num_reqs,
@@ -98,6 +101,8 @@ static int nibble_attend_check(int H, int HQ, int d, const void* q, int q_dtype,
   if (bs <= 0 || bs % kNibTile || n_slots % bs)
     return host_fail(TTKV_E_INVALID, "the block size must be a multiple of 16 that divides the "
                                      "page's slots");
+  if (n_slots / kNibTile > 0x7fffffff)
+    return host_fail(TTKV_E_UNSUPPORTED, "more than 2^31 tiles of 16 slots");
   if (num_reqs < 0 || max_seq < 0 || max_blocks < 0)
     return host_fail(TTKV_E_INVALID, "negative count");
   if ((int64_t)max_blocks * bs < max_seq)
@@ -125,29 +130,8 @@ static int nibble_attend(int H, int HQ, float scale, const void* q, int q_dtype,
   return TTKV_OK;
 }
 
-int64_t nibble_decode_workspace_bytes(int H, int HQ, int num_reqs, int max_seq) { return 256; }
 int64_t nibble_prefill_workspace_bytes(int H, int HQ, int num_reqs, int max_q, int max_seq) {
   return 256;
-}
-
-int nibble_decode_paged(int H, int HQ, int d, float scale, const void* q, int q_dtype,
-                        int64_t q_row_stride, const uint8_t* page, int64_t n_slots,
-                        int64_t slot_stride, int bs, const int32_t* bt, int64_t bt_row_stride,
-                        int max_blocks, const int32_t* seq_lens, const int32_t* qsl, int num_reqs,
-                        int max_seq, void* out, int out_dtype, int64_t out_row_stride, void* ws,
-                        int64_t ws_bytes, int32_t* err, hipStream_t st) {
-  if (int rc = nibble_attend_check(H, HQ, d, q, q_dtype, q_row_stride, page, n_slots, slot_stride,
-                                   bs, bt, max_blocks, seq_lens, qsl, num_reqs, max_seq, out,
-                                   out_dtype, out_row_stride, err))
-    return rc;
-  const int64_t need = nibble_decode_workspace_bytes(H, HQ, num_reqs, max_seq);
-  if (!ws || ws_bytes < need || (uintptr_t)ws % 256)
-    return host_fail(TTKV_E_WORKSPACE, "decode workspace needs " + std::to_string(need) +
-                                           " bytes, 256-aligned");
-  if (num_reqs == 0) return TTKV_OK;
-  return nibble_attend(H, HQ, scale, q, q_dtype, q_row_stride, page, n_slots, slot_stride, bs, bt,
-                       bt_row_stride, seq_lens, qsl, nullptr, num_reqs, 1, max_seq, true, out,
-                       out_dtype, out_row_stride, err, st);
 }
 
 int nibble_prefill_paged(int H, int HQ, int d, float scale, const void* q, int q_dtype,
@@ -157,7 +141,7 @@ int nibble_prefill_paged(int H, int HQ, int d, float scale, const void* q, int q
                          const int32_t* req_index, int num_reqs, int max_q, int max_seq,
                          void* out, int out_dtype, int64_t out_row_stride, void* ws,
                          int64_t ws_bytes, int32_t* err, hipStream_t st) {
-  if (int rc = nibble_attend_check(H, HQ, d, q, q_dtype, q_row_stride, page, n_slots, slot_stride,
+  if (int rc = nibble_check_read(H, HQ, d, q, q_dtype, q_row_stride, page, n_slots, slot_stride,
                                    bs, bt, max_blocks, seq_lens, qsl, num_reqs, max_seq, out,
                                    out_dtype, out_row_stride, err))
     return rc;
