@@ -38,17 +38,66 @@ constexpr float kNibMax = 32640.f;       // values are clamped to this: 7.5 step
 constexpr float kNibMinScale = 0x1p-14f; // the smallest normal fp16
 
 // (c - z) * s of two codes as an fp16 pair, exactly: the codes' nibbles at bit 4 m of x's halves,
-// biased by 1024 (one unit in fp16's last place there), z likewise in zb = nib_bias(parameters),
+// biased by 1024 (one unit in fp16's last place there), z likewise in zb = nib_biased(parameters),
 // s = nib_scales(parameters). The difference has 4 bits and s 7, so neither operation rounds.
-__device__ __forceinline__ half2v nib_bias(uint32_t p2) {
-  return __builtin_bit_cast(half2v, (p2 & 0x000f000fu) | 0x64006400u);
+// The masks come in registers (one scalar, one vector: an instruction takes one constant from
+// outside the vector registers), so each is a single v_and_or_b32.
+struct NibMasks {
+  uint32_t nib, one;  // 0x000f000f (uniform), 0x64006400 (in a vector register)
+};
+__device__ __forceinline__ NibMasks nib_masks() {
+  NibMasks k{0x000f000fu, 0x64006400u};
+  asm("" : "+s"(k.nib), "+v"(k.one));
+  return k;
+}
+__device__ __forceinline__ half2v nib_biased(uint32_t x, const NibMasks& k) {
+  return __builtin_bit_cast(half2v, (x & k.nib) | k.one);
 }
 __device__ __forceinline__ half2v nib_scales(uint32_t p2) {
   return __builtin_bit_cast(half2v, p2 & 0xfff0fff0u);
 }
-__device__ __forceinline__ half2v nib_pair(uint32_t x, int m, half2v zb, half2v s) {
-  const half2v c = __builtin_bit_cast(half2v, ((x >> (4 * m)) & 0x000f000fu) | 0x64006400u);
-  return (c - zb) * s;
+__device__ __forceinline__ half2v nib_pair(uint32_t x, int m, half2v zb, half2v s,
+                                           const NibMasks& k) {
+  return (nib_biased(x >> (4 * m), k) - zb) * s;
+}
+
+// A query row's share of a lane, the operand of the score products: dims 32 g + 8 q4 + (0..7) as
+// qf[g], lanes q4 = 0..3 of one row together. qs: what a product's result is multiplied by, never
+// negative (the query takes the scale's sign, so the largest product is the largest score).
+// bf16 comes to fp16 at a power of two per row that brings its largest value to [1, 2): exact but for
+// values below 2^-14 of the largest, which keep an error of at most 2^-25 of it. `on`: false for
+// columns without a row, which are 0.
+template <int QDT>
+__device__ __forceinline__ void nib_load_query(const uint16_t* row, int q4, float scale_log2,
+                                               bool on, half8 qf[4], float& qs) {
+  u32x4 raw[4];
+#pragma unroll
+  for (int g = 0; g < 4; ++g) raw[g] = *gbl((const u32x4*)(row + 32 * g + 8 * q4));
+  qs = fabsf(scale_log2);
+  if constexpr (QDT == TTKV_DTYPE_F16) {
+#pragma unroll
+    for (int g = 0; g < 4; ++g) qf[g] = __builtin_bit_cast(half8, raw[g]);
+  } else {
+    float x[32], mx = 0.f;
+#pragma unroll
+    for (int i = 0; i < 32; ++i) {
+      const uint32_t w = raw[i >> 3][(i & 7) >> 1];
+      x[i] = bf16_bits_to_float(i & 1 ? w >> 16 : w & 0xffffu);
+      mx = fmaxf(mx, fabsf(x[i]));
+    }
+    mx = cross_row_max(mx);
+    const int e = mx > 0.f && mx < INFINITY ? ilogbf(mx) : 0;
+#pragma unroll
+    for (int i = 0; i < 32; ++i) qf[i >> 3][i & 7] = (_Float16)ldexpf(x[i], -e);
+    qs = ldexpf(qs, e);
+  }
+  const bool none = qs == 0.f || !on;  // (a scale of 0 must not meet a masked score)
+  if (none) qs = 1.f;
+#pragma unroll
+  for (int g = 0; g < 4; ++g) {
+    if (scale_log2 < 0.f) qf[g] = -qf[g];
+    if (none) qf[g] = half8{};
+  }
 }
 
 }  // namespace ttkv

@@ -145,45 +145,21 @@ __global__ __launch_bounds__(kNDThreads, 2) void nibble_decode_kernel(NibDecodeA
 
   // The query, column `col`, as the B operand of the four score products: dims 32 g + 8 q4 ...
   half8 qf[4];
-  float qs = a.scale_log2;
-  {
-    u32x4 raw[4];
-    const uint16_t* qp = a.q + row * a.q_row_stride + (int64_t)(h * G + min(col, G - 1)) * kD;
-#pragma unroll
-    for (int g = 0; g < 4; ++g) raw[g] = *gbl((const u32x4*)(qp + 32 * g + 8 * q4));
-    if constexpr (QDT == TTKV_DTYPE_F16) {
-#pragma unroll
-      for (int g = 0; g < 4; ++g) qf[g] = __builtin_bit_cast(half8, raw[g]);
-    } else {
-      // bf16 to fp16 at a power of two per row that brings its largest value to [1, 2): exact but
-      // for values below 2^-14 of the largest, which keep an error of at most 2^-25 of it
-      float x[32], mx = 0.f;
-#pragma unroll
-      for (int i = 0; i < 32; ++i) {
-        const uint32_t w = raw[i >> 3][(i & 7) >> 1];
-        x[i] = bf16_bits_to_float(i & 1 ? w >> 16 : w & 0xffffu);
-        mx = fmaxf(mx, fabsf(x[i]));
-      }
-      mx = cross_row_max(mx);
-      const int e = mx > 0.f && mx < INFINITY ? ilogbf(mx) : 0;
-#pragma unroll
-      for (int i = 0; i < 32; ++i) qf[i >> 3][i & 7] = (_Float16)ldexpf(x[i], -e);
-      qs = ldexpf(qs, e);
-    }
-    if (col >= G) {
-#pragma unroll
-      for (int g = 0; g < 4; ++g) qf[g] = half8{};
-    }
-  }
+  float qs;
+  nib_load_query<QDT>(a.q + row * a.q_row_stride + (int64_t)(h * G + min(col, G - 1)) * kD, q4,
+                      a.scale_log2, col < G, qf, qs);
 
   const int steps = (n + kNDStep - 1) / kNDStep;
-  const int s0 = P.c * P.C, s1 = min(s0 + P.C, steps);
+  // the request's steps in equal parts
+  const int s0 = (int)((int64_t)steps * P.c / P.n_chunks);
+  const int s1 = (int)((int64_t)steps * (P.c + 1) / P.n_chunks);
   float4v acc[8];  // [group][dim of the pair]: dims 32 g + 8 q4 + 2 i + b of the column's query
 #pragma unroll
   for (int i = 0; i < 8; ++i) acc[i] = float4v{};
   float m = -INFINITY, l = 0.f;
   bool bad = false;
 
+  const NibMasks masks = nib_masks();
   const uint8_t* base = a.page + (int64_t)h * kNibRecord;
   const int32_t* bt = a.bt + (int64_t)r * a.bt_row_stride;
   // tile ids of this wave's next 64 steps, one step per lane (-1: a block outside the cache)
@@ -201,9 +177,9 @@ __global__ __launch_bounds__(kNDThreads, 2) void nibble_decode_kernel(NibDecodeA
     for (int t = 0; t < 2; ++t) {
       const int id = __builtin_amdgcn_readlane(t ? tid1 : tid0, k);
       const uint8_t* rec = base + (int64_t)max(id, 0) * a.tile_stride;
-      x.k[t] = *gbl((const u32x4*)(rec + 16 * lane));
+      x.k[t] = __builtin_nontemporal_load(gbl((const u32x4*)(rec + 16 * lane)));
       x.kp[t] = *gbl((const u32x2v*)(rec + kNibKp + 8 * col));
-      x.v[t] = *gbl((const u32x4*)(rec + kNibV + 16 * lane));
+      x.v[t] = __builtin_nontemporal_load(gbl((const u32x4*)(rec + kNibV + 16 * lane)));
       x.vp[t][0] = *gbl((const u32x4*)(rec + kNibVp + 32 * q4));
       x.vp[t][1] = *gbl((const u32x4*)(rec + kNibVp + 32 * q4 + 16));
       bad |= id < 0;
@@ -216,12 +192,12 @@ __global__ __launch_bounds__(kNDThreads, 2) void nibble_decode_kernel(NibDecodeA
       sc[t] = float4v{};
 #pragma unroll
       for (int g = 0; g < 4; ++g) {
-        const half2v zz = nib_bias(x.kp[t][g >> 1]), sg = nib_scales(x.kp[t][g >> 1]);
+        const half2v zz = nib_biased(x.kp[t][g >> 1], masks), sg = nib_scales(x.kp[t][g >> 1]);
         const half2v zb = {zz[g & 1], zz[g & 1]}, ss = {sg[g & 1], sg[g & 1]};
         half8 kf;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          const half2v v = nib_pair(x.k[t][g], j, zb, ss);
+          const half2v v = nib_pair(x.k[t][g], j, zb, ss, masks);
           kf[2 * j] = v[0];
           kf[2 * j + 1] = v[1];
         }
@@ -246,9 +222,9 @@ __global__ __launch_bounds__(kNDThreads, 2) void nibble_decode_kernel(NibDecodeA
     for (int t = 0; t < 2; ++t)
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        sc[t][i] *= qs;
         mt = fmaxf(mt, sc[t][i]);
       }
+    mt *= qs;
     if (__builtin_amdgcn_ballot_w64(mt > m + kNDLazy)) {
       const float mn = fmaxf(m, cross_row_max(mt));
       const float f = m == -INFINITY ? 0.f : exp2f(m - mn);
@@ -261,10 +237,13 @@ __global__ __launch_bounds__(kNDThreads, 2) void nibble_decode_kernel(NibDecodeA
 #pragma unroll
     for (int t = 0; t < 2; ++t)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float p = fast_exp2(sc[t][i] - m);
-        l += p;
-        pf[4 * t + i] = (_Float16)p;  // the one rounding on the way to the output
+      for (int i = 0; i < 4; i += 2) {
+        // the one rounding on the way to the output; the sum takes the rounded weights
+        const half2v p = {(_Float16)fast_exp2(fmaf(sc[t][i], qs, -m)),
+                          (_Float16)fast_exp2(fmaf(sc[t][i + 1], qs, -m))};
+        l = __builtin_amdgcn_fdot2(p, half2v{(_Float16)1.f, (_Float16)1.f}, l, false);
+        pf[4 * t + i] = p[0];
+        pf[4 * t + i + 1] = p[1];
       }
 #pragma unroll
     for (int quad = 0; quad < 2; ++quad)
@@ -277,10 +256,10 @@ __global__ __launch_bounds__(kNDThreads, 2) void nibble_decode_kernel(NibDecodeA
 #pragma unroll
           for (int pair = 0; pair < 2; ++pair) {
             const uint32_t p2 = x.vp[t][g >> 1][2 * (g & 1) + pair];
-            const half2v zb = nib_bias(p2), ss = nib_scales(p2);
+            const half2v zb = nib_biased(p2, masks), ss = nib_scales(p2);
 #pragma unroll
             for (int b = 0; b < 2; ++b) {
-              const half2v v = nib_pair(x.v[t][2 * pair + quad], 2 * gg + b, zb, ss);
+              const half2v v = nib_pair(x.v[t][2 * pair + quad], 2 * gg + b, zb, ss, masks);
               vf[b][4 * t + 2 * pair] = v[0];
               vf[b][4 * t + 2 * pair + 1] = v[1];
             }
@@ -408,7 +387,9 @@ __global__ __launch_bounds__(kNDThreads, 2) void nibble_decode_kernel(NibDecodeA
   }
 }
 
-// Resident workgroups of the kernel: the plan's item target.
+// The plan's item target: two workgroups per CU. A third would fit, but shorter chunks pay their
+// prologue and join more often (8 x 14,402 tokens: 31.2 us at two per CU, 32.8 at three, 36.2 at
+// four; 61 requests of 70 to 2,900: 33.4, 35.0, 34.6).
 static int nd_target() {
   static int slots = 0;
   if (!slots) {
@@ -417,7 +398,7 @@ static int nd_target() {
             &per_cu, nibble_decode_kernel<TTKV_DTYPE_F16>, kNDThreads, 0) != hipSuccess ||
         per_cu < 1)
       per_cu = 2;
-    slots = per_cu * device_cu_count();
+    slots = std::min(per_cu, 2) * device_cu_count();
   }
   return slots;
 }

@@ -1,0 +1,664 @@
+// Attention of chunks of queries over the 4-bit cache (format: ttkv_nibble.h), causal. gfx950 / CDNA4.
+//
+// Flash attention. The rows of a (request, KV head) are its (query, query head) pairs, row = j G + p,
+// so the G heads of a KV head share every key read. A workgroup of 8 waves holds 128, 256 or 384 of
+// them (NG = 1 to 3 groups of 16 per wave) and walks a part of the request's keys in tiles of 64:
+//   dequantise  waves 0..3 the tile's keys, waves 4..7 its values, 16 code bytes per thread, exactly
+//               (ttkv_nibble.h) to fp16 in LDS: keys [token][dim], values transposed [dim][token] in
+//               the order of the products' operands. Once per tile and 128 NG rows.
+//   S^T = K Q^T on v_mfma_f32_16x16x32_f16, 32 tokens at a time: a key fragment read from LDS serves
+//               the wave's NG groups. Lane column = row, so a row's softmax state is a lane's own.
+//   softmax     as in the decode kernel: the maximum moves when a score exceeds it by 8, weights are
+//               rounded to fp16 once and their sum is of the rounded ones.
+//   O^T += V^T P^T: the scores' layout is the weights' operand layout as it stands.
+// One barrier per tile (two tile buffers); the next tile's codes are in flight in registers. Waves
+// 0..3 compute before they dequantise and waves 4..7 after, so that the two waves of a SIMD are
+// out of step and one's matrix products run under the other's vector work.
+//
+// The keys of a row block are split over several workgroups where the batch has too few row blocks
+// to fill the chip; the last to arrive joins the parts' unnormalised results. The split comes from a
+// plan that every workgroup computes alike from the lengths on the device.
+#include <math.h>
+
+#include "ttkv_host.h"
+#include "ttkv_nibble.h"
+
+namespace ttkv {
+
+constexpr int kNPThreads = 512;
+constexpr int kNPWaves = 8;
+constexpr int kNPTile = 64;        // keys per tile
+constexpr int kNPPlanLanes = 4;    // requests per lane in the plan: 256 per launch
+constexpr int kNPMaxSplit = 32;
+constexpr int kNPMinTiles = 4;     // keys per part, in tiles
+constexpr float kNPLazy = 8.f;     // log2 of the largest softmax weight before a rescale
+constexpr float kNPNone = -1e30f;  // a maximum before the first visible key
+constexpr int64_t kNPPartRows = 128000;  // rows of partial results a launch may leave: 66.6 MB
+constexpr int kNPKBytes = kNPTile * kD * 2;
+constexpr int kNPSmem = 4 * kNPKBytes;   // two buffers of keys and values
+
+struct NibPrefillArgs {
+  int H, G;
+  float scale_log2;
+  const uint16_t* q;
+  int64_t q_row_stride;
+  const uint8_t* page;
+  int64_t tile_stride;
+  int num_blocks, tpb;
+  const int32_t* bt;
+  int64_t bt_row_stride;
+  const int32_t* seq_lens;
+  const int32_t* qsl;
+  const int32_t* req_index;
+  int num_reqs, max_q, max_seq;
+  void* out;
+  int out_dtype;
+  int64_t out_row_stride;
+  int* ws_cnt;
+  float* ws_o;   // [part rows][kD]
+  float* ws_ml;  // [part rows][2]
+  int64_t part_rows;
+  int target;
+  int32_t* err;
+};
+
+struct NibPrefillPlan {
+  int r, h, rb, sp, ns;  // batch row, KV head, row block, key part and how many
+  int n, Q, rows;        // keys, the chunk's queries, rows processed
+  int cnt;               // the row block's counter
+  int64_t part;          // first part row of the (request, head)
+  bool none;
+};
+
+__device__ __forceinline__ int np_incl_scan(int v) {
+  const int lane = threadIdx.x & 63;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const int t = __shfl_up(v, o);
+    v += lane >= o ? t : 0;
+  }
+  return v;
+}
+
+__device__ __forceinline__ int np_parts(int tiles, int C) {
+  return min((tiles + C - 1) / C, kNPMaxSplit);
+}
+
+// Parts of at least C tiles: the shortest that spread the batch's tiles over the target's workgroups
+// and whose partial results fit the workspace.
+template <int RW>
+__device__ __forceinline__ NibPrefillPlan np_plan(const NibPrefillArgs& a, int item) {
+  const int lane = threadIdx.x & 63;
+  int idx[kNPPlanLanes], n[kNPPlanLanes], Q[kNPPlanLanes], rows[kNPPlanLanes], tiles[kNPPlanLanes];
+  float work = 0.f;
+#pragma unroll
+  for (int i = 0; i < kNPPlanLanes; ++i) {
+    const int r = lane + 64 * i;
+    const bool on = r < a.num_reqs;
+    idx[i] = on ? (a.req_index ? a.req_index[r] : r) : 0;
+    n[i] = on ? a.seq_lens[idx[i]] : 0;
+    Q[i] = on ? a.qsl[idx[i] + 1] - a.qsl[idx[i]] : 0;
+    const int nn = min(max(n[i], 0), a.max_seq);
+    rows[i] = min(max(Q[i], 0), a.max_q) * a.G;
+    tiles[i] = nn < Q[i] ? 1 : (nn + kNPTile - 1) / kNPTile;
+    work += (float)((rows[i] + RW - 1) / RW) * (float)tiles[i];
+  }
+  work = wave_sum(work) * (float)a.H;
+  int C = max(kNPMinTiles, (int)ceilf(work / (float)a.target));
+  while (true) {
+    float need = 0.f;
+#pragma unroll
+    for (int i = 0; i < kNPPlanLanes; ++i) {
+      const int ns = np_parts(tiles[i], C);
+      need += ns > 1 ? (float)rows[i] * (float)ns : 0.f;
+    }
+    need = wave_sum(need) * (float)a.H;
+    if (need <= (float)a.part_rows) break;
+    C += (C >> 2) + 1;
+  }
+  NibPrefillPlan P{};
+  P.none = true;
+  P.h = item % a.H;
+  const int it = item / a.H;
+  int carry = 0, blocks = 0, prows = 0;
+#pragma unroll
+  for (int i = 0; i < kNPPlanLanes; ++i) {
+    if (64 * i >= a.num_reqs) break;
+    const int rb = (rows[i] + RW - 1) / RW, ns = np_parts(tiles[i], C), items = rb * ns;
+    const int pr = ns > 1 ? rows[i] * ns : 0;
+    const int incl = np_incl_scan(items), ex = carry + incl - items;
+    const int bincl = np_incl_scan(rb), pincl = np_incl_scan(pr);
+    const uint64_t hit = __builtin_amdgcn_ballot_w64(items > 0 && ex <= it && it < ex + items);
+    if (hit) {
+      const int ln = __builtin_ctzll(hit);
+      const int local = it - __builtin_amdgcn_readlane(ex, ln);
+      const int nrb = __builtin_amdgcn_readlane(rb, ln);
+      P.none = false;
+      P.r = __builtin_amdgcn_readlane(idx[i], ln);
+      P.n = __builtin_amdgcn_readlane(n[i], ln);
+      P.Q = __builtin_amdgcn_readlane(Q[i], ln);
+      P.rows = __builtin_amdgcn_readlane(rows[i], ln);
+      P.ns = __builtin_amdgcn_readlane(ns, ln);
+      P.rb = nrb - 1 - local / P.ns;  // the last rows see the most keys: first
+      P.sp = local % P.ns;
+      P.cnt = (blocks + __builtin_amdgcn_readlane(bincl - rb, ln) + P.rb) * a.H + P.h;
+      P.part = (int64_t)(prows + __builtin_amdgcn_readlane(pincl - pr, ln)) * a.H +
+               (int64_t)P.h * P.ns * P.rows;
+    }
+    carry += __builtin_amdgcn_readlane(incl, 63);
+    blocks += __builtin_amdgcn_readlane(bincl, 63);
+    prows += __builtin_amdgcn_readlane(pincl, 63);
+  }
+  return P;
+}
+
+// Tile buffers, 16-byte chunks exchanged by their row so that a fragment's 16 rows lie in distinct
+// banks: keys [token][16 chunks of 8 dims], values [dim][8 chunks of 8 token slots].
+__device__ __forceinline__ int np_k_at(int token, int chunk) {
+  return token * kD + ((chunk ^ (token & 15)) << 3);
+}
+__device__ __forceinline__ int np_v_at(int dim, int chunk) {
+  return dim * kNPTile + ((chunk ^ (dim & 7)) << 3);
+}
+// Barrier for LDS alone: global loads stay in flight across it.
+__device__ __forceinline__ void np_barrier() {
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
+__device__ __forceinline__ float2v ld_agent2(const float* p) {
+  return __builtin_bit_cast(float2v, __hip_atomic_load((const uint64_t*)p, __ATOMIC_RELAXED,
+                                                       __HIP_MEMORY_SCOPE_AGENT));
+}
+
+template <int QDT, int NG>
+__global__ __launch_bounds__(kNPThreads, 2) void nibble_prefill_kernel(NibPrefillArgs a) {
+  constexpr int RW = kNPWaves * 16 * NG;
+  extern __shared__ __align__(16) unsigned char smem[];
+  __shared__ uint32_t nan_sh[2][kNPTile / 4];  // per token of a masked tile: its groups that are NaN
+  __shared__ int bad_sh, last_sh;
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wv = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const NibPrefillPlan P = np_plan<RW>(a, blockIdx.x);
+  if (P.none) return;
+  const int G = a.G, h = P.h;
+  const int n = min(max(P.n, 0), a.max_seq);
+  const int64_t q0 = a.qsl[P.r];
+  const int nrow = min(RW, P.rows - P.rb * RW);
+  if (tid == 0 && h == 0 && P.sp == 0 && P.rb == 0 &&
+      (P.n > a.max_seq || P.Q > a.max_q || n < P.Q))
+    atomicOr(a.err, TTKV_ERR_SEQ_LEN);
+  if (n < P.Q) {  // fewer keys than queries
+    for (int e = tid; e < nrow * kD; e += kNPThreads) {
+      const int row = P.rb * RW + e / kD;
+      store_act(a.out, a.out_dtype,
+                (q0 + row / G) * a.out_row_stride + (int64_t)(h * G + row % G) * kD + e % kD, NAN);
+    }
+    return;
+  }
+  const int col = lane & 15, q4 = lane >> 4;
+  const int row0 = P.rb * RW + wv * 16 * NG;  // the wave's first row
+  const bool active = row0 < P.rows;
+  const int p0 = n - P.Q;  // position of query 0
+  const int see_min = p0 + row0 / G, see_max = p0 + min(row0 + 16 * NG - 1, P.rows - 1) / G;
+
+  half8 qf[NG][4];
+  float qs[NG], m[NG], l[NG];
+  int lim[NG];  // last key the lane's row sees
+  float4v acc[NG][8];
+#pragma unroll
+  for (int gr = 0; gr < NG; ++gr) {
+    const int row = min(row0 + 16 * gr + col, P.rows - 1);
+    lim[gr] = p0 + row / G;
+    nib_load_query<QDT>(a.q + (q0 + row / G) * a.q_row_stride + (int64_t)(h * G + row % G) * kD,
+                        q4, a.scale_log2, true, qf[gr], qs[gr]);
+    m[gr] = kNPNone;
+    l[gr] = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) acc[gr][i] = float4v{};
+  }
+
+  // the block's tiles and this part of them
+  const int tiles = (p0 + (P.rb * RW + nrow - 1) / G) / kNPTile + 1;
+  const int t0 = (int)((int64_t)tiles * P.sp / P.ns), t1 = (int)((int64_t)tiles * (P.sp + 1) / P.ns);
+  const int wg_see = p0 + P.rb * RW / G;  // last key that every row of the block sees
+  const uint8_t* base = a.page + (int64_t)h * kNibRecord;
+  const int32_t* bt = a.bt + (int64_t)P.r * a.bt_row_stride;
+  const NibMasks masks = nib_masks();
+  const bool values = wv >= 4;
+  const int tt = wv & 3;  // this wave's record of a tile
+  const int last_rec = (n - 1) / kNibTile;
+  bool bad = false;
+  int ids = 0;
+  auto fetch_ids = [&](int t) {  // record ids of the next 64 tiles, one per lane (-1: bad block)
+    const int rec = min(4 * (t + lane) + tt, last_rec);
+    const int b = rec / a.tpb, id = bt[b];
+    ids = (uint32_t)id < (uint32_t)a.num_blocks ? id * a.tpb + rec - b * a.tpb : -1;
+  };
+  u32x4 code;
+  u32x4 par[2];
+  int ids_at = t0;
+  auto load = [&](int t) {
+    if (t >= t1) return;
+    if (t - ids_at >= 64) {
+      ids_at = t;
+      fetch_ids(t);
+    }
+    const int id = __builtin_amdgcn_readlane(ids, t - ids_at);
+    bad |= id < 0;
+    const uint8_t* rec = base + (int64_t)max(id, 0) * a.tile_stride;
+    if (values) {
+      code = *gbl((const u32x4*)(rec + kNibV + 16 * lane));
+      par[0] = *gbl((const u32x4*)(rec + kNibVp + 32 * q4));
+      par[1] = *gbl((const u32x4*)(rec + kNibVp + 32 * q4 + 16));
+    } else {
+      code = *gbl((const u32x4*)(rec + 16 * lane));
+      const u32x2v kp = *gbl((const u32x2v*)(rec + kNibKp + 8 * col));
+      par[0][0] = kp[0];
+      par[0][1] = kp[1];
+    }
+  };
+  auto dequant_keys = [&](int t) {
+    if (t >= t1) return;
+    _Float16* kb = (_Float16*)smem + (t & 1) * (2 * kNPTile * kD);
+    const int token = 16 * tt + col;
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const half2v zz = nib_biased(par[0][g >> 1], masks), sg = nib_scales(par[0][g >> 1]);
+      const half2v zb = {zz[g & 1], zz[g & 1]}, ss = {sg[g & 1], sg[g & 1]};
+      half8 o;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const half2v v = nib_pair(code[g], j, zb, ss, masks);
+        o[2 * j] = v[0];
+        o[2 * j + 1] = v[1];
+      }
+      *(half8*)(kb + np_k_at(token, 4 * g + q4)) = o;
+    }
+  };
+  auto dequant_values = [&](int t) {
+    if (t >= t1) return;
+    _Float16* vb = (_Float16*)smem + (t & 1) * (2 * kNPTile * kD) + kNPTile * kD;
+    const int tok = t * kNPTile + 16 * tt + 4 * q4;  // the lane's four tokens
+    if ((t + 1) * kNPTile - 1 > wg_see) {
+      // Some row does not see all of this tile. A weight of 0 must not meet a NaN: values past the
+      // last key become 0, and a group that is NaN becomes 0 too and is noted for the rows that see it.
+      uint32_t note = 0;
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          const int at = 2 * (g & 1) + (i >> 1);
+          const uint32_t w = par[g >> 1][at], p = i & 1 ? w >> 16 : w & 0xffffu;
+          const bool nan = (p & 0x7c00u) == 0x7c00u;
+          if (tok + i >= n || nan) {
+            par[g >> 1][at] = w & (i & 1 ? 0x0000ffffu : 0xffff0000u);
+            note |= tok + i < n ? 1u << (8 * i + g) : 0u;
+          }
+        }
+      if (col == 0) nan_sh[t & 1][4 * tt + q4] = note;
+    }
+    const int slot = (tt >> 1) * 4 + q4, half = tt & 1;
+#pragma unroll
+    for (int quad = 0; quad < 2; ++quad)
+#pragma unroll
+      for (int gg = 0; gg < 2; ++gg) {
+        const int g = 2 * quad + gg;
+        half4 o[2];
+#pragma unroll
+        for (int pair = 0; pair < 2; ++pair) {
+          const uint32_t p2 = par[g >> 1][2 * (g & 1) + pair];
+          const half2v zb = nib_biased(p2, masks), ss = nib_scales(p2);
+#pragma unroll
+          for (int b = 0; b < 2; ++b) {
+            const half2v v = nib_pair(code[2 * pair + quad], 2 * gg + b, zb, ss, masks);
+            o[b][2 * pair] = v[0];
+            o[b][2 * pair + 1] = v[1];
+          }
+        }
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {
+          const int dim = 32 * g + 2 * col + b;
+          *(half4*)(vb + np_v_at(dim, slot) + 4 * half) = o[b];
+        }
+      }
+  };
+  auto compute = [&](int t) {
+    if (!active || t * kNPTile > see_max) return;
+    const _Float16* kb = (const _Float16*)smem + (t & 1) * (2 * kNPTile * kD);
+    const _Float16* vb = kb + kNPTile * kD;
+    const bool masked = (t + 1) * kNPTile - 1 > see_min;
+#pragma unroll
+    for (int ks = 0; ks < 2; ++ks) {
+      float4v sc[NG][2];
+#pragma unroll
+      for (int tg = 0; tg < 2; ++tg) {
+#pragma unroll
+        for (int gr = 0; gr < NG; ++gr) sc[gr][tg] = float4v{};
+#pragma unroll
+        for (int s = 0; s < 4; ++s) {
+          const half8 kf = *(const half8*)(kb + np_k_at(32 * ks + 16 * tg + col, 4 * s + q4));
+#pragma unroll
+          for (int gr = 0; gr < NG; ++gr)
+            sc[gr][tg] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qf[gr][s], sc[gr][tg], 0, 0, 0);
+        }
+      }
+      half8 pf[NG];
+#pragma unroll
+      for (int gr = 0; gr < NG; ++gr) {
+        if (masked) {
+          const int tok = t * kNPTile + 32 * ks + 4 * q4;
+#pragma unroll
+          for (int tg = 0; tg < 2; ++tg)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              if (tok + 16 * tg + i > lim[gr]) sc[gr][tg][i] = -INFINITY;
+        }
+        float mt = -INFINITY;
+#pragma unroll
+        for (int tg = 0; tg < 2; ++tg)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) mt = fmaxf(mt, sc[gr][tg][i]);
+        mt *= qs[gr];
+        if (__builtin_amdgcn_ballot_w64(mt > m[gr] + kNPLazy)) {
+          const float mn = fmaxf(m[gr], cross_row_max(mt));
+          const float f = exp2f(m[gr] - mn);
+          m[gr] = mn;
+          l[gr] *= f;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) acc[gr][i] *= f;
+        }
+#pragma unroll
+        for (int tg = 0; tg < 2; ++tg)
+#pragma unroll
+          for (int i = 0; i < 4; i += 2) {
+            // the one rounding on the way to the output; the sum takes the rounded weights
+            const half2v p = {(_Float16)fast_exp2(fmaf(sc[gr][tg][i], qs[gr], -m[gr])),
+                              (_Float16)fast_exp2(fmaf(sc[gr][tg][i + 1], qs[gr], -m[gr]))};
+            l[gr] = __builtin_amdgcn_fdot2(p, half2v{(_Float16)1.f, (_Float16)1.f}, l[gr], false);
+            pf[gr][4 * tg + i] = p[0];
+            pf[gr][4 * tg + i + 1] = p[1];
+          }
+      }
+#pragma unroll
+      for (int db = 0; db < 8; ++db) {
+        const half8 vf = *(const half8*)(vb + np_v_at(16 * db + col, 4 * ks + q4));
+#pragma unroll
+        for (int gr = 0; gr < NG; ++gr)
+          acc[gr][db] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, pf[gr], acc[gr][db], 0, 0, 0);
+      }
+    }
+    if ((t + 1) * kNPTile - 1 > wg_see) {  // NaN groups of a tile with masked keys
+      const uint32_t mine = nan_sh[t & 1][lane & 15];
+      if (__builtin_amdgcn_ballot_w64(mine != 0)) {
+        for (int k = 0; k < kNPTile; ++k) {
+          const uint32_t note = (nan_sh[t & 1][k >> 2] >> (8 * (k & 3))) & 15u;
+          if (!note) continue;
+#pragma unroll
+          for (int gr = 0; gr < NG; ++gr)
+#pragma unroll
+            for (int db = 0; db < 8; ++db)
+              if ((note >> (db >> 1) & 1) && t * kNPTile + k <= lim[gr]) acc[gr][db] += NAN;
+        }
+      }
+    }
+  };
+
+  if (tid == 0) bad_sh = 0;
+  if (t0 < t1) {
+    fetch_ids(t0);
+    load(t0);
+    if (!values) {
+      dequant_keys(t0);
+      load(t0 + 1);
+    }
+    // The value waves enter the loop half a turn early: they dequantise tile t + 1 (at t = t0 - 1 the
+    // first tile) before they compute tile t, the key waves after it.
+    for (int t = t0 - 1; t < t1; ++t) {
+      if (values) {
+        dequant_values(t + 1);
+        load(t + 2);
+      }
+      if (t >= t0) compute(t);
+      if (!values && t >= t0) {
+        dequant_keys(t + 1);
+        load(t + 2);
+      }
+      np_barrier();
+    }
+  } else {
+    np_barrier();
+  }
+  if (bad) {
+    bad_sh = 1;
+    if (lane == 0) atomicOr(a.err, TTKV_ERR_BAD_BLOCK);
+  }
+  __syncthreads();
+  const bool nan_rows = bad_sh != 0;
+#pragma unroll
+  for (int gr = 0; gr < NG; ++gr) l[gr] = nan_rows ? NAN : cross_row_sum(l[gr]);
+
+  if (P.ns == 1) {
+    if (!active) return;
+#pragma unroll
+    for (int gr = 0; gr < NG; ++gr) {
+      const int row = row0 + 16 * gr + col;
+      if (row >= P.rows) continue;
+      const float inv = 1.f / l[gr];
+      const int64_t at = (q0 + row / G) * a.out_row_stride + (int64_t)(h * G + row % G) * kD;
+#pragma unroll
+      for (int db = 0; db < 8; ++db)
+        store_act4(a.out, a.out_dtype, at + 16 * db + 4 * q4, acc[gr][db] * inv, true);
+    }
+    return;
+  }
+  if (active) {
+#pragma unroll
+    for (int gr = 0; gr < NG; ++gr) {
+      const int row = row0 + 16 * gr + col;
+      if (row >= P.rows) continue;
+      const int64_t pr = P.part + (int64_t)P.sp * P.rows + row;
+#pragma unroll
+      for (int db = 0; db < 8; ++db)
+        store_agent16(a.ws_o + pr * kD + 16 * db + 4 * q4, acc[gr][db]);
+      if (q4 == 0) store_agent8(a.ws_ml + 2 * pr, float2v{m[gr], l[gr]});
+    }
+  }
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  __syncthreads();
+  if (tid == 0) {
+    int* cnt = a.ws_cnt + P.cnt;
+    const int prev = arrive(cnt);
+    last_sh = prev == P.ns - 1;
+    if (last_sh) __hip_atomic_store(cnt, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  }
+  __syncthreads();
+  if (!last_sh) return;
+  // ---- the row block's parts joined: each row's weights, then the sums
+  float* wgt = (float*)smem;  // [parts][RW]
+  const int64_t first = P.part + P.rb * RW;
+  for (int row = tid; row < nrow; row += kNPThreads) {
+    float mm = kNPNone, ll = 0.f;
+    for (int s = 0; s < P.ns; ++s) {
+      const float2v ml = ld_agent2(a.ws_ml + 2 * (first + (int64_t)s * P.rows + row));
+      const float mn = fmaxf(mm, ml[0]);
+      ll = ll * exp2f(mm - mn) + ml[1] * exp2f(ml[0] - mn);
+      mm = mn;
+      wgt[s * RW + row] = ml[0];
+    }
+    const float inv = 1.f / ll;
+    for (int s = 0; s < P.ns; ++s) wgt[s * RW + row] = exp2f(wgt[s * RW + row] - mm) * inv;
+  }
+  __syncthreads();
+  for (int e = tid; e < nrow * (kD / 4); e += kNPThreads) {
+    const int row = e / (kD / 4), d = 4 * (e % (kD / 4));
+    float4v o = {};
+#pragma unroll 4
+    for (int s = 0; s < P.ns; ++s) {
+      const float* po = a.ws_o + (first + (int64_t)s * P.rows + row) * kD + d;
+      const float2v x = ld_agent2(po), y = ld_agent2(po + 2);
+      o += float4v{x[0], x[1], y[0], y[1]} * wgt[s * RW + row];
+    }
+    const int rr = P.rb * RW + row;
+    store_act4(a.out, a.out_dtype,
+               (q0 + rr / G) * a.out_row_stride + (int64_t)(h * G + rr % G) * kD + d, o, true);
+  }
+}
+
+int nibble_check_read(int H, int HQ, int d, const void* q, int q_dtype,
+                               int64_t q_row_stride, const uint8_t* page, int64_t n_slots,
+                               int64_t slot_stride, int bs, const int32_t* bt, int max_blocks,
+                               const int32_t* seq_lens, const int32_t* qsl, int num_reqs,
+                               int max_seq, const void* out, int out_dtype,
+                               int64_t out_row_stride, const int32_t* err) {
+  if (int rc = nibble_check_page(H, d, page, n_slots, slot_stride)) return rc;
+  if (HQ <= 0 || HQ % H) return host_fail(TTKV_E_INVALID, "num_heads is not a multiple of H");
+  if (HQ / H > 16)
+    return host_fail(TTKV_E_UNSUPPORTED, "more than 16 query heads per KV head");
+  for (int dt : {q_dtype, out_dtype})
+    if (dt != TTKV_DTYPE_F16 && dt != TTKV_DTYPE_BF16)
+      return host_fail(TTKV_E_INVALID, "query / out dtype must be fp16 or bf16");
+  if (bs <= 0 || bs % kNibTile || n_slots % bs)
+    return host_fail(TTKV_E_INVALID, "the block size must be a multiple of 16 that divides the "
+                                     "page's slots");
+  if (n_slots / kNibTile > 0x7fffffff)
+    return host_fail(TTKV_E_UNSUPPORTED, "more than 2^31 tiles of 16 slots");
+  if (num_reqs < 0 || max_seq < 0 || max_blocks < 0)
+    return host_fail(TTKV_E_INVALID, "negative count");
+  if ((int64_t)max_blocks * bs < max_seq)
+    return host_fail(TTKV_E_INVALID, "max_seq_len needs more blocks than the block table holds");
+  if (num_reqs && (!q || !bt || !seq_lens || !qsl || !out || !err))
+    return host_fail(TTKV_E_INVALID, "null pointer argument");
+  if (((uintptr_t)q | (uintptr_t)out) % 16 || q_row_stride % 8 || out_row_stride % 8)
+    return host_fail(TTKV_E_INVALID, "query / out rows must be 16-byte aligned");
+  return TTKV_OK;
+}
+
+// Groups of 16 rows per wave for chunks of at most `rows` rows: a wave's key and value fragments
+// serve all of its groups, so three are the fastest per row, unless fewer leave less of a block empty.
+static int np_groups(int64_t rows) {
+  static const double cost[] = {0, 1.6, 1.15, 1.0};  // per row held
+  int best = 3;
+  double least = 0;
+  for (int ng = 3; ng >= 1; --ng) {
+    const int64_t rw = kNPWaves * 16 * ng;
+    const double c = (double)((rows + rw - 1) / rw * rw) * cost[ng];
+    if (ng == 3 || c < least) {
+      best = ng;
+      least = c;
+    }
+  }
+  return best;
+}
+
+// Requests per launch: the plan's lanes and a counter per row block and head; with no room for one
+// request's counters, its keys are not split.
+struct NibPrefillSlice {
+  int ng, reqs;
+  int64_t blocks;  // row blocks of a launch, at most
+  bool split;
+};
+static NibPrefillSlice np_slice(int H, int HQ, int num_reqs, int max_q) {
+  NibPrefillSlice s{};
+  s.ng = np_groups((int64_t)max_q * (HQ / H));
+  const int64_t rw = kNPWaves * 16 * s.ng;
+  const int64_t per = ((int64_t)max_q * (HQ / H) + rw - 1) / rw * H;  // row blocks of one request
+  s.split = per <= kMaxCounters;
+  s.reqs = std::min(num_reqs, kNPPlanLanes * 64);
+  if (s.split) s.reqs = (int)std::min<int64_t>(s.reqs, std::max<int64_t>(1, kMaxCounters / std::max<int64_t>(per, 1)));
+  s.reqs = std::max(1, s.reqs);
+  s.blocks = per * s.reqs;
+  return s;
+}
+
+static int64_t np_part_rows(int HQ, int reqs, int max_q, int max_seq) {
+  const int64_t tiles = (max_seq + kNPTile - 1) / kNPTile;
+  const int64_t parts = std::min<int64_t>(kNPMaxSplit, (tiles + kNPMinTiles - 1) / kNPMinTiles);
+  return parts <= 1 ? 0 : std::min(kNPPartRows, parts * reqs * max_q * HQ);
+}
+
+int64_t nibble_prefill_workspace_bytes(int H, int HQ, int num_reqs, int max_q, int max_seq) {
+  if (num_reqs == 0 || max_q == 0) return 256;
+  const NibPrefillSlice s = np_slice(H, HQ, num_reqs, max_q);
+  return kCounterBytes + (s.split ? np_part_rows(HQ, s.reqs, max_q, max_seq) * (kD + 2) * 4 : 0);
+}
+
+template <int QDT, int NG>
+static int np_launch(const NibPrefillArgs& a, unsigned grid, hipStream_t st) {
+  if (int rc = raise_smem_limit((const void*)nibble_prefill_kernel<QDT, NG>, kNPSmem)) return rc;
+  hipLaunchKernelGGL((nibble_prefill_kernel<QDT, NG>), dim3(grid), dim3(kNPThreads), kNPSmem, st, a);
+  const hipError_t e = hipGetLastError();
+  if (e != hipSuccess)
+    return host_fail(TTKV_E_LAUNCH, std::string("nibble prefill launch: ") + hipGetErrorString(e));
+  return TTKV_OK;
+}
+
+int nibble_prefill_paged(int H, int HQ, int d, float scale, const void* q, int q_dtype,
+                         int64_t q_row_stride, const uint8_t* page, int64_t n_slots,
+                         int64_t slot_stride, int bs, const int32_t* bt, int64_t bt_row_stride,
+                         int max_blocks, const int32_t* seq_lens, const int32_t* qsl,
+                         const int32_t* req_index, int num_reqs, int max_q, int max_seq,
+                         void* out, int out_dtype, int64_t out_row_stride, void* ws,
+                         int64_t ws_bytes, int32_t* err, hipStream_t st) {
+  if (int rc = nibble_check_read(H, HQ, d, q, q_dtype, q_row_stride, page, n_slots, slot_stride,
+                                 bs, bt, max_blocks, seq_lens, qsl, num_reqs, max_seq, out,
+                                 out_dtype, out_row_stride, err))
+    return rc;
+  if (max_q < 0) return host_fail(TTKV_E_INVALID, "negative max_q_len");
+  if (max_q > max_seq) return host_fail(TTKV_E_INVALID, "max_q_len is longer than max_seq_len");
+  const int64_t need = nibble_prefill_workspace_bytes(H, HQ, num_reqs, max_q, max_seq);
+  if (!ws || ws_bytes < need || (uintptr_t)ws % 256)
+    return host_fail(TTKV_E_WORKSPACE, "prefill workspace needs " + std::to_string(need) +
+                                           " bytes, 256-aligned");
+  if (num_reqs == 0 || max_q == 0) return TTKV_OK;
+  const NibPrefillSlice s = np_slice(H, HQ, num_reqs, max_q);
+  const int64_t items = s.blocks + (s.split ? device_cu_count() + 8 : 0);
+  if (items > 0x7fffffff) return host_fail(TTKV_E_INVALID, "too many queries for one call");
+  NibPrefillArgs a{};
+  a.H = H;
+  a.G = HQ / H;
+  a.scale_log2 = scale * 1.4426950408889634f;
+  a.q = (const uint16_t*)q;
+  a.q_row_stride = q_row_stride;
+  a.page = page;
+  a.tile_stride = kNibTile * slot_stride;
+  a.num_blocks = (int)(n_slots / bs);
+  a.tpb = bs / kNibTile;
+  a.bt = bt;
+  a.bt_row_stride = bt_row_stride;
+  a.seq_lens = seq_lens;
+  a.qsl = qsl;
+  a.max_q = max_q;
+  a.max_seq = max_seq;
+  a.out = out;
+  a.out_dtype = out_dtype;
+  a.out_row_stride = out_row_stride;
+  a.part_rows = s.split ? np_part_rows(HQ, s.reqs, max_q, max_seq) : 0;
+  a.ws_cnt = (int*)ws;
+  a.ws_o = (float*)((char*)ws + kCounterBytes);
+  a.ws_ml = a.ws_o + a.part_rows * kD;
+  a.target = device_cu_count();  // a workgroup fills a CU
+  a.err = err;
+  for (int r0 = 0; r0 < num_reqs; r0 += s.reqs) {
+    a.num_reqs = std::min(s.reqs, num_reqs - r0);
+    if (req_index) {
+      a.req_index = req_index + r0;
+    } else {
+      a.seq_lens = seq_lens + r0;
+      a.qsl = qsl + r0;
+      a.bt = bt + (int64_t)r0 * bt_row_stride;
+    }
+    const unsigned grid = (unsigned)items;
+    const bool f16 = q_dtype == TTKV_DTYPE_F16;
+    int rc = TTKV_OK;
+    switch (s.ng) {
+      case 1: rc = f16 ? np_launch<TTKV_DTYPE_F16, 1>(a, grid, st) : np_launch<TTKV_DTYPE_BF16, 1>(a, grid, st); break;
+      case 2: rc = f16 ? np_launch<TTKV_DTYPE_F16, 2>(a, grid, st) : np_launch<TTKV_DTYPE_BF16, 2>(a, grid, st); break;
+      default: rc = f16 ? np_launch<TTKV_DTYPE_F16, 3>(a, grid, st) : np_launch<TTKV_DTYPE_BF16, 3>(a, grid, st); break;
+    }
+    if (rc != TTKV_OK) return rc;
+  }
+  return TTKV_OK;
+}
+
+}  // namespace ttkv
