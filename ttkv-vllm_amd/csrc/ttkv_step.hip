@@ -217,10 +217,11 @@ __device__ __forceinline__ int rot_axis(const RotArgs& a, int j) {
   return ax;
 }
 
-__global__ __launch_bounds__(256) void rotary_axes_kernel(RotArgs a) {
-  const int64_t tok = blockIdx.x;
-  int64_t p[kRotAxes];
+// The token's position on each axis; false where one is outside the table.
+__device__ __forceinline__ bool rot_positions(const RotArgs& a, int64_t tok,
+                                              int64_t p[kRotAxes]) {
   bool ok = true;
+#pragma unroll
   for (int i = 0; i < kRotAxes; ++i) {
     p[i] = i < a.axes ? a.pos[i * a.pos_stride + tok] : 0;
     if (p[i] < 0 || p[i] >= a.max_pos) {
@@ -229,6 +230,131 @@ __global__ __launch_bounds__(256) void rotary_axes_kernel(RotArgs a) {
     }
   }
   if (!ok && threadIdx.x == 0) atomicOr(a.err, TTKV_ERR_BAD_POSITION);
+  return ok;
+}
+
+// Eight consecutive elements of a 16-byte aligned row piece, in registers and as floats.
+template <int DT>
+struct Rot8 {
+  u32x4 raw[DT == TTKV_DTYPE_F32 ? 2 : 1];
+};
+template <int DT>
+__device__ __forceinline__ Rot8<DT> rot_load8(const void* p, int64_t i) {
+  Rot8<DT> x;
+  const char* at = (const char*)p + i * (DT == TTKV_DTYPE_F32 ? 4 : 2);
+#pragma unroll
+  for (int j = 0; j < (DT == TTKV_DTYPE_F32 ? 2 : 1); ++j) x.raw[j] = *gbl((const u32x4*)at + j);
+  return x;
+}
+template <int DT>
+__device__ __forceinline__ float rot_get(const Rot8<DT>& x, int i) {
+  if constexpr (DT == TTKV_DTYPE_F32) {
+    const uint32_t w = x.raw[i >> 2][i & 3];  // (by value: a bit cast of an element reads the first)
+    return __builtin_bit_cast(float, w);
+  }
+  const uint32_t w = x.raw[0][i >> 1], b = i & 1 ? w >> 16 : w & 0xffffu;
+  return DT == TTKV_DTYPE_F16 ? f16_bits_to_float(b) : bf16_bits_to_float(b);
+}
+template <int DT>
+__device__ __forceinline__ void rot_store8(void* p, int64_t i, const float v[8]) {
+  store_act4(p, DT, i, float4v{v[0], v[1], v[2], v[3]}, true);
+  store_act4(p, DT, i + 4, float4v{v[4], v[5], v[6], v[7]}, true);
+}
+
+// One wave per token. Lane j first looks up frequency j's cosine and sine (one load each, whatever
+// the axes) and leaves them in LDS; then the lanes take (head, 8 frequencies) pairs of 16-byte pieces,
+// four heads' loads in flight at a time, the first four asked for before the lookup. Bound by memory:
+// every query and key byte read and written once.
+constexpr int kRotHalf = 128;  // frequencies the LDS holds
+constexpr int kRotBatch = 4;
+template <int DT>
+__global__ __launch_bounds__(64) void rotary_rows_kernel(RotArgs a) {
+  __shared__ float cs[2][kRotHalf];
+  const int64_t tok = blockIdx.x;
+  const int lane = threadIdx.x;
+  const int nch = a.half >> 3, slots = 64 / nch, heads = a.HQ + a.H;
+  const int slot = lane / nch, j0 = (lane - slot * nch) * 8;
+  const bool on = slot < slots;
+  auto place = [&](int head, bool out, int64_t& at) -> const void* {
+    const bool is_q = head < a.HQ;
+    const int64_t stride = out ? (is_q ? a.qo_stride : a.ko_stride)
+                               : (is_q ? a.q_stride : a.k_stride);
+    at = tok * stride + (int64_t)(is_q ? head : head - a.HQ) * a.d;
+    return out ? (is_q ? a.qo : a.ko) : (is_q ? a.q : a.k);
+  };
+  Rot8<DT> x[kRotBatch], y[kRotBatch];
+  auto fetch = [&](int h0) {
+#pragma unroll
+    for (int b = 0; b < kRotBatch; ++b) {
+      const int head = h0 + b * slots + slot;
+      if (on && head < heads) {
+        int64_t at;
+        const void* src = place(head, false, at);
+        x[b] = rot_load8<DT>(src, at + j0);
+        y[b] = rot_load8<DT>(src, at + j0 + a.half);
+      }
+    }
+  };
+  fetch(0);
+  int64_t p[kRotAxes];
+  const bool ok = rot_positions(a, tok, p);
+  for (int j = lane; j < a.half; j += 64) {
+    const int ax = rot_axis(a, j);
+    int64_t q = p[0];
+#pragma unroll
+    for (int i = 1; i < kRotAxes; ++i) q = ax == i ? p[i] : q;
+    const float* row = a.cs + q * (2 * a.half) + j;
+    const float c = *gbl(row), s = *gbl(row + a.half);
+    cs[0][j] = ok ? c : NAN;
+    cs[1][j] = ok ? s : NAN;
+  }
+  __syncthreads();
+  float c[8], s[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    c[i] = cs[0][j0 + i];
+    s[i] = cs[1][j0 + i];
+  }
+  for (int h0 = 0; h0 < heads; h0 += kRotBatch * slots) {
+#pragma unroll
+    for (int b = 0; b < kRotBatch; ++b) {
+      const int head = h0 + b * slots + slot;
+      if (on && head < heads) {
+        int64_t at;
+        void* dst = const_cast<void*>(place(head, true, at));
+        float u[8], v[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const float xi = rot_get<DT>(x[b], i), yi = rot_get<DT>(y[b], i);
+          u[i] = xi * c[i] - yi * s[i];
+          v[i] = yi * c[i] + xi * s[i];
+        }
+        rot_store8<DT>(dst, at + j0, u);
+        rot_store8<DT>(dst, at + j0 + a.half, v);
+      }
+    }
+    fetch(h0 + kRotBatch * slots);
+  }
+  const int rest = (a.d - 2 * a.half) >> 3;  // pieces that are copied
+  for (int i = lane; i < heads * rest; i += 64) {
+    const int head = i / rest, x0 = 2 * a.half + (i - head * rest) * 8;
+    int64_t from, to;
+    const void* src = place(head, false, from);
+    void* dst = const_cast<void*>(place(head, true, to));
+    const Rot8<DT> z = rot_load8<DT>(src, from + x0);
+    float v[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v[k] = ok ? rot_get<DT>(z, k) : NAN;
+    rot_store8<DT>(dst, to + x0, v);
+  }
+}
+
+// Rows whose pieces of 8 are not 16-byte aligned, or longer than the wave kernel's table: one pair
+// per thread.
+__global__ __launch_bounds__(256) void rotary_axes_kernel(RotArgs a) {
+  const int64_t tok = blockIdx.x;
+  int64_t p[kRotAxes];
+  const bool ok = rot_positions(a, tok, p);
   const int per = a.half + (a.d - 2 * a.half);  // pairs, then the dims that are copied
   for (int i = threadIdx.x; i < (a.HQ + a.H) * per; i += 256) {
     const int head = i / per, j = i % per;
@@ -282,7 +408,18 @@ int rotary_axes(const void* q, const void* k, void* qo, void* ko, int dtype, int
   a.cs = cs;
   a.max_pos = max_pos;
   a.err = err;
-  hipLaunchKernelGGL(rotary_axes_kernel, dim3(N), dim3(256), 0, st, a);
+  const int64_t eb = dtype == TTKV_DTYPE_F32 ? 4 : 2;
+  bool rows = rot % 16 == 0 && d % 8 == 0 && rot / 2 <= kRotHalf;
+  for (const void* p : {q, k, (const void*)qo, (const void*)ko}) rows &= (uintptr_t)p % 16 == 0;
+  for (int64_t s : {q_stride, k_stride, qo_stride, ko_stride}) rows &= s * eb % 16 == 0;
+  if (!rows)
+    hipLaunchKernelGGL(rotary_axes_kernel, dim3(N), dim3(256), 0, st, a);
+  else if (dtype == TTKV_DTYPE_F32)
+    hipLaunchKernelGGL(rotary_rows_kernel<TTKV_DTYPE_F32>, dim3(N), dim3(64), 0, st, a);
+  else if (dtype == TTKV_DTYPE_F16)
+    hipLaunchKernelGGL(rotary_rows_kernel<TTKV_DTYPE_F16>, dim3(N), dim3(64), 0, st, a);
+  else
+    hipLaunchKernelGGL(rotary_rows_kernel<TTKV_DTYPE_BF16>, dim3(N), dim3(64), 0, st, a);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess)
     return host_fail(TTKV_E_LAUNCH, std::string("rotary launch: ") + hipGetErrorString(e));
