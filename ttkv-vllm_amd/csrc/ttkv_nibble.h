@@ -100,4 +100,22 @@ __device__ __forceinline__ void nib_load_query(const uint16_t* row, int q4, floa
   }
 }
 
+// Inclusive prefix sum over the wave's lanes (all active), on DPP: within rows of 16, then the rows.
+__device__ __forceinline__ int nib_scan(int v) {
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, false);  // row_shr 1, 2, 4, 8
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false);  // last lane of rows 0, 2 to 1, 3
+  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false);  // of row 1 to rows 2 and 3
+  return v;
+}
+
+// Two floats of another workgroup's partial result (see ld_agent).
+__device__ __forceinline__ float2v ld_agent2(const float* p) {
+  const uint64_t w =
+      __hip_atomic_load((const uint64_t*)p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  return __builtin_bit_cast(float2v, w);
+}
+
 }  // namespace ttkv

@@ -61,16 +61,6 @@ struct NibDecodePlan {
   bool none;
 };
 
-__device__ __forceinline__ int nd_incl_scan(int v) {
-  const int lane = threadIdx.x & 63;
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const int t = __shfl_up(v, o);
-    v += lane >= o ? t : 0;
-  }
-  return v;
-}
-
 __device__ __forceinline__ NibDecodePlan nd_plan(const NibDecodeArgs& a, int item) {
   const int lane = threadIdx.x & 63;
   int n[kNDPlanLanes], st[kNDPlanLanes], total = 0;
@@ -99,7 +89,7 @@ __device__ __forceinline__ NibDecodePlan nd_plan(const NibDecodeArgs& a, int ite
     if (64 * i >= a.num_reqs) break;
     const int r = lane + 64 * i;
     const int nch = r < a.num_reqs ? max(1, (st[i] + P.C - 1) / P.C) : 0;
-    const int incl = nd_incl_scan(nch), ex = carry + incl - nch;
+    const int incl = nib_scan(nch), ex = carry + incl - nch;
     const uint64_t hit = __builtin_amdgcn_ballot_w64(nch > 0 && ex <= it && it < ex + nch);
     if (hit) {
       const int ln = __builtin_ctzll(hit);
@@ -359,7 +349,8 @@ __global__ __launch_bounds__(kNDThreads, 2) void nibble_decode_kernel(NibDecodeA
     for (int c0 = 0; c0 < P.n_chunks; c0 += 64) {
       const int nb = min(64, P.n_chunks - c0);
       const float* pl = pp + (c0 + min(lane, nb - 1)) * cstride + kD;
-      const float mc = lane < nb ? ld_agent(pl) : -INFINITY, lc = ld_agent(pl + 1);
+      const float2v ml = ld_agent2(pl);
+      const float mc = lane < nb ? ml[0] : -INFINITY, lc = ml[1];
       const float mn = fmaxf(mm, wave_max(mc));
       const float keep = mm == -INFINITY ? 0.f : exp2f(mm - mn);
       const float wc = lane < nb ? exp2f(mc - mn) : 0.f;
@@ -370,7 +361,7 @@ __global__ __launch_bounds__(kNDThreads, 2) void nibble_decode_kernel(NibDecodeA
 #pragma unroll
         for (int u = 0; u < 8; ++u) {
           const float* po = pp + (c0 + min(j + u, nb - 1)) * cstride + 2 * lane;
-          x[u] = float2v{ld_agent(po), ld_agent(po + 1)};
+          x[u] = ld_agent2(po);
         }
 #pragma unroll
         for (int u = 0; u < 8; ++u) {

@@ -35,7 +35,10 @@ constexpr float kNPLazy = 8.f;     // log2 of the largest softmax weight before 
 constexpr float kNPNone = -1e30f;  // a maximum before the first visible key
 constexpr int64_t kNPPartRows = 128000;  // rows of partial results a launch may leave: 66.6 MB
 constexpr int kNPKBytes = kNPTile * kD * 2;
-constexpr int kNPSmem = 4 * kNPKBytes;   // two buffers of keys and values
+// Two buffers of keys and values; the join's maxima and sums of every part and row.
+constexpr int np_smem(int ng) {
+  return std::max(4 * kNPKBytes, kNPMaxSplit * kNPWaves * 16 * ng * 8);
+}
 
 struct NibPrefillArgs {
   int H, G;
@@ -69,16 +72,6 @@ struct NibPrefillPlan {
   int64_t part;          // first part row of the (request, head)
   bool none;
 };
-
-__device__ __forceinline__ int np_incl_scan(int v) {
-  const int lane = threadIdx.x & 63;
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const int t = __shfl_up(v, o);
-    v += lane >= o ? t : 0;
-  }
-  return v;
-}
 
 __device__ __forceinline__ int np_parts(int tiles, int C) {
   return min((tiles + C - 1) / C, kNPMaxSplit);
@@ -126,8 +119,8 @@ __device__ __forceinline__ NibPrefillPlan np_plan(const NibPrefillArgs& a, int i
     if (64 * i >= a.num_reqs) break;
     const int rb = (rows[i] + RW - 1) / RW, ns = np_parts(tiles[i], C), items = rb * ns;
     const int pr = ns > 1 ? rows[i] * ns : 0;
-    const int incl = np_incl_scan(items), ex = carry + incl - items;
-    const int bincl = np_incl_scan(rb), pincl = np_incl_scan(pr);
+    const int incl = nib_scan(items), ex = carry + incl - items;
+    const int bincl = nib_scan(rb), pincl = nib_scan(pr);
     const uint64_t hit = __builtin_amdgcn_ballot_w64(items > 0 && ex <= it && it < ex + items);
     if (hit) {
       const int ln = __builtin_ctzll(hit);
@@ -166,11 +159,6 @@ __device__ __forceinline__ void np_barrier() {
   __builtin_amdgcn_s_barrier();
   asm volatile("" ::: "memory");
 }
-__device__ __forceinline__ float2v ld_agent2(const float* p) {
-  return __builtin_bit_cast(float2v, __hip_atomic_load((const uint64_t*)p, __ATOMIC_RELAXED,
-                                                       __HIP_MEMORY_SCOPE_AGENT));
-}
-
 template <int QDT, int NG>
 __global__ __launch_bounds__(kNPThreads, 2) void nibble_prefill_kernel(NibPrefillArgs a) {
   constexpr int RW = kNPWaves * 16 * NG;
@@ -474,30 +462,47 @@ __global__ __launch_bounds__(kNPThreads, 2) void nibble_prefill_kernel(NibPrefil
   }
   __syncthreads();
   if (!last_sh) return;
-  // ---- the row block's parts joined: each row's weights, then the sums
-  float* wgt = (float*)smem;  // [parts][RW]
+  // ---- the row block's parts joined: every part's maxima and sums to LDS in one round trip, the
+  // rows' weights from them, then the weighted sums, eight parts' loads in flight
+  float2v* ml = (float2v*)smem;  // [parts][nrow]
   const int64_t first = P.part + P.rb * RW;
-  for (int row = tid; row < nrow; row += kNPThreads) {
-    float mm = kNPNone, ll = 0.f;
-    for (int s = 0; s < P.ns; ++s) {
-      const float2v ml = ld_agent2(a.ws_ml + 2 * (first + (int64_t)s * P.rows + row));
-      const float mn = fmaxf(mm, ml[0]);
-      ll = ll * exp2f(mm - mn) + ml[1] * exp2f(ml[0] - mn);
-      mm = mn;
-      wgt[s * RW + row] = ml[0];
-    }
-    const float inv = 1.f / ll;
-    for (int s = 0; s < P.ns; ++s) wgt[s * RW + row] = exp2f(wgt[s * RW + row] - mm) * inv;
+  for (int e = tid; e < P.ns * nrow; e += kNPThreads) {
+    const int s = e / nrow;
+    ml[e] = ld_agent2(a.ws_ml + 2 * (first + (int64_t)s * P.rows + (e - s * nrow)));
   }
   __syncthreads();
+  for (int row = tid; row < nrow; row += kNPThreads) {
+    float mm = kNPNone, ll = 0.f;
+    for (int s = 0; s < P.ns; ++s) mm = fmaxf(mm, ml[s * nrow + row][0]);
+    for (int s = 0; s < P.ns; ++s) {
+      const float2v x = ml[s * nrow + row];
+      const float w = exp2f(x[0] - mm);
+      ll += x[1] * w;
+      ml[s * nrow + row][0] = w;
+    }
+    const float inv = 1.f / ll;
+    for (int s = 0; s < P.ns; ++s) ml[s * nrow + row][0] *= inv;
+  }
+  __syncthreads();
+#pragma unroll 2
   for (int e = tid; e < nrow * (kD / 4); e += kNPThreads) {
     const int row = e / (kD / 4), d = 4 * (e % (kD / 4));
     float4v o = {};
-#pragma unroll 4
-    for (int s = 0; s < P.ns; ++s) {
-      const float* po = a.ws_o + (first + (int64_t)s * P.rows + row) * kD + d;
-      const float2v x = ld_agent2(po), y = ld_agent2(po + 2);
-      o += float4v{x[0], x[1], y[0], y[1]} * wgt[s * RW + row];
+    const float* po = a.ws_o + (first + row) * kD + d;
+    const int64_t between = (int64_t)P.rows * kD;  // from a part to the next
+    for (int s0 = 0; s0 < P.ns; s0 += 4) {
+      float2v x[4][2];
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (s0 + i < P.ns) {
+          x[i][0] = ld_agent2(po + (s0 + i) * between);
+          x[i][1] = ld_agent2(po + (s0 + i) * between + 2);
+        }
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (s0 + i < P.ns)
+          o += float4v{x[i][0][0], x[i][0][1], x[i][1][0], x[i][1][1]} *
+               ml[(s0 + i) * nrow + row][0];
     }
     const int rr = P.rb * RW + row;
     store_act4(a.out, a.out_dtype,
@@ -585,8 +590,8 @@ int64_t nibble_prefill_workspace_bytes(int H, int HQ, int num_reqs, int max_q, i
 
 template <int QDT, int NG>
 static int np_launch(const NibPrefillArgs& a, unsigned grid, hipStream_t st) {
-  if (int rc = raise_smem_limit((const void*)nibble_prefill_kernel<QDT, NG>, kNPSmem)) return rc;
-  hipLaunchKernelGGL((nibble_prefill_kernel<QDT, NG>), dim3(grid), dim3(kNPThreads), kNPSmem, st, a);
+  if (int rc = raise_smem_limit((const void*)nibble_prefill_kernel<QDT, NG>, np_smem(NG))) return rc;
+  hipLaunchKernelGGL((nibble_prefill_kernel<QDT, NG>), dim3(grid), dim3(kNPThreads), np_smem(NG), st, a);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess)
     return host_fail(TTKV_E_LAUNCH, std::string("nibble prefill launch: ") + hipGetErrorString(e));

@@ -392,29 +392,37 @@ def dense_decode_paged(query: torch.Tensor, k_cache: torch.Tensor, v_cache: torc
 
 
 # ---------------------------------------------------------------- the 4-bit cache
-def _on_device(fn):
-    """Run a wrapper with its first tensor argument's device current: a launch goes to the current
-    device, whatever device its stream belongs to. (The guard costs more than the checks, so it is
-    taken only where the device differs.)"""
-    @functools.wraps(fn)
-    def call(*args, **kw):
-        dev = next((a.device for a in args if isinstance(a, torch.Tensor)), None)
-        if dev is None or dev.type != "cuda" or dev.index == torch.cuda.current_device():
-            return fn(*args, **kw)
-        with torch.cuda.device(dev):
-            return fn(*args, **kw)
-    return call
+_current_device = torch._C._cuda_getDevice if hasattr(torch._C, "_cuda_getDevice") \
+    else torch.cuda.current_device
 
 
-def _one_device(first, *ts):
-    """Refuse host tensors and tensors of another device than the first."""
-    dev = first.device
-    if dev.type != "cuda":
+def _on_device(index: int, fn, *args) -> int:
+    """Call a launching C entry with device `index` current: a launch goes to the current device,
+    whatever device its stream belongs to. (The guard costs more than the checks, so it is taken only
+    where the device differs.)"""
+    if index == _current_device():
+        return fn(*args)
+    with torch.cuda.device(index):
+        return fn(*args)
+
+
+def _one_device(first, *ts) -> int:
+    """Refuse host tensors and tensors of another device than the first; returns its index."""
+    index = first.get_device()
+    if index < 0:
         _need_device(first)
     for t in ts:
-        if t is not None and t.device != dev:
+        if t is not None and t.get_device() != index:
             _need_device(t)
-            raise ValueError(f"tensors on {dev} and {t.device} in one call")
+            raise ValueError(f"tensors on {first.device} and {t.device} in one call")
+    return index
+
+
+def _stream(index: int) -> int:
+    """The current stream of device `index`."""
+    if _hip._raw_stream is not None:
+        return _hip._raw_stream(index)
+    return torch.cuda.current_stream(index).cuda_stream
 
 
 def _error_word(error_word, device):
@@ -427,9 +435,11 @@ def _error_word(error_word, device):
 
 def _rows(t, heads, d, what):
     """Check [N, heads, d] rows, contiguous within a token."""
-    if t.dim() != 3 or t.shape[1] != heads or t.shape[2] != d:
-        raise ValueError(f"{what} must be [N, {heads}, {d}], got {tuple(t.shape)}")
-    if t.numel() and (t.stride(2) != 1 or (heads > 1 and t.stride(1) != d)):
+    shape = t.shape
+    if len(shape) != 3 or shape[1] != heads or shape[2] != d:
+        raise ValueError(f"{what} must be [N, {heads}, {d}], got {tuple(shape)}")
+    if not t.is_contiguous() and t.numel() and (t.stride(2) != 1
+                                                or (heads > 1 and t.stride(1) != d)):
         raise ValueError(f"{what} must be contiguous within a token ([heads, {d}] rows)")
 
 
@@ -450,7 +460,6 @@ def _plan_out(t, n, dtype, device, name):
     return t
 
 
-@_on_device
 def step_plan(computed_lens: torch.Tensor, query_lens: torch.Tensor, block_table: torch.Tensor,
               free_blocks: torch.Tensor, block_size: int, num_blocks: int, num_tokens: int,
               query_start_loc: torch.Tensor | None = None, seq_lens: torch.Tensor | None = None,
@@ -463,8 +472,8 @@ def step_plan(computed_lens: torch.Tensor, query_lens: torch.Tensor, block_table
     computed_lens / query_lens [R] int32: tokens stored before the step and new in it;
     block_table [R, max_blocks] int32, updated in place; free_blocks [F] int32, taken from the
     front; num_tokens: the (padded) token count of the outputs, at least the sum of query_lens."""
-    _one_device(computed_lens, query_lens, block_table, free_blocks, query_start_loc, seq_lens,
-                slot_mapping, positions, blocks_used, error_word)
+    index = _one_device(computed_lens, query_lens, block_table, free_blocks, query_start_loc,
+                        seq_lens, slot_mapping, positions, blocks_used, error_word)
     _i32(computed_lens, "computed_lens")
     _i32(query_lens, "query_lens")
     _i32(free_blocks, "free_blocks")
@@ -482,12 +491,12 @@ def step_plan(computed_lens: torch.Tensor, query_lens: torch.Tensor, block_table
                     _plan_out(blocks_used, 1, torch.int32, dev, "blocks_used"))
     err = _error_word(error_word, dev)
     W = block_table.shape[1]
-    rc = _hip.lib().ttkv_step_plan(
-        computed_lens.data_ptr(), query_lens.data_ptr(), R, block_table.data_ptr(),
+    rc = _on_device(
+        index, _hip.lib().ttkv_step_plan, computed_lens.data_ptr(), query_lens.data_ptr(), R, block_table.data_ptr(),
         block_table.stride(0) if R > 1 else W, W, free_blocks.data_ptr(), free_blocks.numel(),
         int(block_size), int(num_blocks), n, plan.query_start_loc.data_ptr(),
         plan.seq_lens.data_ptr(), plan.slot_mapping.data_ptr(), plan.positions.data_ptr(),
-        plan.blocks_used.data_ptr(), err.data_ptr(), _hip.stream_ptr(dev))
+        plan.blocks_used.data_ptr(), err.data_ptr(), _stream(index))
     _hip.check(rc, "ttkv_step_plan")
     return plan
 
@@ -497,7 +506,6 @@ def _c_sections(sections: tuple) -> ctypes.Array:
     return (ctypes.c_int32 * len(sections))(*sections)
 
 
-@_on_device
 def rotary_axes(query: torch.Tensor, key: torch.Tensor | None, positions: torch.Tensor,
                 cos_sin_cache: torch.Tensor, sections, interleaved: bool = False,
                 query_out: torch.Tensor | None = None, key_out: torch.Tensor | None = None,
@@ -508,11 +516,11 @@ def rotary_axes(query: torch.Tensor, key: torch.Tensor | None, positions: torch.
     positions [axes, N] (or [N] for one axis) int64; sections: how many of the rotary_dim / 2
     frequencies each axis has, in a row, or dealt in turn where `interleaved`; cos_sin_cache
     [max_pos, rotary_dim] fp32 (vLLM layout)."""
-    _one_device(query, key, positions, cos_sin_cache, query_out, key_out, error_word)
+    index = _one_device(query, key, positions, cos_sin_cache, query_out, key_out, error_word)
     if query.dim() != 3:
         raise ValueError(f"query must be [N, heads, d], got {tuple(query.shape)}")
     N, HQ, d = query.shape
-    sections = tuple(int(s) for s in sections)
+    sections = tuple(sections)
     if positions.dtype != torch.int64 or positions.shape[-1] != N \
             or positions.numel() != len(sections) * N:
         raise ValueError(f"positions must be int64 [{len(sections)}, {N}], got "
@@ -537,19 +545,18 @@ def rotary_axes(query: torch.Tensor, key: torch.Tensor | None, positions: torch.
         if t.shape[0] != N or t.dtype != query.dtype:
             raise ValueError(f"{what} must have the query's {N} tokens and dtype")
     err = _error_word(error_word, query.device)
-    rc = _hip.lib().ttkv_rotary_axes(
-        query.data_ptr(), _hip.ptr(key), query_out.data_ptr(), _hip.ptr(key_out),
+    rc = _on_device(
+        index, _hip.lib().ttkv_rotary_axes, query.data_ptr(), _hip.ptr(key), query_out.data_ptr(), _hip.ptr(key_out),
         _hip.DTYPE_CODE[query.dtype], N, HQ, H, d, query.stride(0),
         0 if key is None else key.stride(0), query_out.stride(0),
         0 if key is None else key_out.stride(0), positions.data_ptr(),
         positions.stride(0) if positions.dim() == 2 else N, len(sections), _c_sections(sections),
         int(bool(interleaved)), cos_sin_cache.data_ptr(), cos_sin_cache.shape[0],
-        cos_sin_cache.shape[1], err.data_ptr(), _hip.stream_ptr(query.device))
+        cos_sin_cache.shape[1], err.data_ptr(), _stream(index))
     _hip.check(rc, "ttkv_rotary_axes")
     return query_out, key_out
 
 
-@_on_device
 def nibble_write_paged(lay: NibbleLayout, key: torch.Tensor, value: torch.Tensor,
                        slot_mapping: torch.Tensor, page: torch.Tensor,
                        key_out: torch.Tensor | None = None,
@@ -560,7 +567,7 @@ def nibble_write_paged(lay: NibbleLayout, key: torch.Tensor, value: torch.Tensor
     page: the layer's cache, its last dim one slot (`lay.compressed_bytes_per_token()` bytes or
     more); slot_mapping [>= N] int64, -1 for padded tokens; key_out / value_out (optional, fp16
     [N, H, d], contiguous) receive what the slots then stand for. See `ttkv_nibble_write_paged`."""
-    _one_device(key, value, slot_mapping, page, key_out, value_out, error_word)
+    index = _one_device(key, value, slot_mapping, page, key_out, value_out, error_word)
     N = key.shape[0]
     for t, what in ((key, "key"), (value, "value")):
         _rows(t, lay.H, lay.d, what)
@@ -579,20 +586,21 @@ def nibble_write_paged(lay: NibbleLayout, key: torch.Tensor, value: torch.Tensor
         raise ValueError("the cache page must be contiguous")
     page_ptr, n_slots, slot_bytes = _page_args(page, lay.compressed_bytes_per_token())
     err = _error_word(error_word, key.device)
-    rc = _hip.lib().ttkv_nibble_write_paged(
-        lay.H, lay.d, key.data_ptr(), _hip.DTYPE_CODE[key.dtype], key.stride(0), value.data_ptr(),
+    rc = _on_device(
+        index, _hip.lib().ttkv_nibble_write_paged, lay.H, lay.d, key.data_ptr(), _hip.DTYPE_CODE[key.dtype], key.stride(0), value.data_ptr(),
         _hip.DTYPE_CODE[value.dtype], value.stride(0), slot_mapping.data_ptr(), N, page_ptr,
         n_slots, slot_bytes, _hip.ptr(key_out), _hip.ptr(value_out), err.data_ptr(),
-        _hip.stream_ptr(key.device))
+        _stream(index))
     _hip.check(rc, "ttkv_nibble_write_paged")
 
 
 def _nibble_read(lay, query, page, block_table, seq_lens, query_start_loc, out):
-    """Checks shared by the 4-bit reads; returns (page pointer, slots, bytes per slot, out)."""
+    """Checks shared by the 4-bit reads; returns (page pointer, slots, bytes per slot, out,
+    device index)."""
     _rows(query, query.shape[1] if query.dim() == 3 else 0, lay.d, "query")
     if out is None:
         out = torch.empty_like(query)
-    _one_device(query, page, block_table, seq_lens, query_start_loc, out)
+    index = _one_device(query, page, block_table, seq_lens, query_start_loc, out)
     _rows(out, query.shape[1], lay.d, "out")
     if out.shape[0] != query.shape[0]:
         raise ValueError("out must match query's shape")
@@ -606,7 +614,7 @@ def _nibble_read(lay, query, page, block_table, seq_lens, query_start_loc, out):
     _i32(query_start_loc, "query_start_loc")
     if not page.is_contiguous():
         raise ValueError("the cache page must be contiguous")
-    return *_page_args(page, lay.compressed_bytes_per_token()), out
+    return *_page_args(page, lay.compressed_bytes_per_token()), out, index
 
 
 def nibble_decode_workspace(lay: NibbleLayout, num_heads: int, num_reqs: int, max_seq_len: int,
@@ -619,29 +627,6 @@ def nibble_decode_workspace(lay: NibbleLayout, num_heads: int, num_reqs: int, ma
     return torch.zeros(max(int(n), 256), dtype=torch.uint8, device=device)
 
 
-@_on_device
-def _nibble_decode(query, lay, page, block_size, block_table, seq_lens, query_start_loc,
-                   max_seq_len, scale, out, workspace, error_word):
-    page_ptr, n_slots, slot_bytes, out = _nibble_read(lay, query, page, block_table, seq_lens,
-                                                      query_start_loc, out)
-    B, HQ, dev = seq_lens.numel(), query.shape[1], query.device
-    if block_table.shape[0] < B or query_start_loc.numel() < B:
-        raise ValueError(f"{B} sequence lengths need as many block table rows and query rows")
-    if workspace is None:
-        workspace = nibble_decode_workspace(lay, HQ, B, max_seq_len, dev)
-    err = _error_word(error_word, dev)
-    _one_device(query, workspace, err)
-    rc = _hip.lib().ttkv_nibble_decode_paged(
-        lay.H, HQ, lay.d, float(scale), query.data_ptr(), _hip.DTYPE_CODE[query.dtype],
-        query.stride(0), page_ptr, n_slots, slot_bytes, int(block_size), block_table.data_ptr(),
-        block_table.stride(0), block_table.shape[1], seq_lens.data_ptr(),
-        query_start_loc.data_ptr(), B, int(max_seq_len), out.data_ptr(),
-        _hip.DTYPE_CODE[out.dtype], out.stride(0), workspace.data_ptr(), workspace.numel(),
-        err.data_ptr(), _hip.stream_ptr(dev))
-    _hip.check(rc, "ttkv_nibble_decode_paged")
-    return out
-
-
 def nibble_decode_paged(lay: NibbleLayout, query: torch.Tensor, page: torch.Tensor,
                         block_size: int, block_table: torch.Tensor, seq_lens: torch.Tensor,
                         query_start_loc: torch.Tensor, max_seq_len: int, scale: float,
@@ -650,8 +635,25 @@ def nibble_decode_paged(lay: NibbleLayout, query: torch.Tensor, page: torch.Tens
     """Attention of one query per request (row query_start_loc[r] of query [N, HQ, d], rotated)
     over its seq_lens[r] stored tokens of a 4-bit cache. See `ttkv_nibble_decode_paged` in
     include/ttkv_hip.h. Returns `out` [N, HQ, d] with the decode rows written."""
-    return _nibble_decode(query, lay, page, block_size, block_table, seq_lens, query_start_loc,
-                          max_seq_len, scale, out, workspace, error_word)
+    page_ptr, n_slots, slot_bytes, out, index = _nibble_read(lay, query, page, block_table,
+                                                             seq_lens, query_start_loc, out)
+    B, HQ, dev = seq_lens.numel(), query.shape[1], query.device
+    if block_table.shape[0] < B or query_start_loc.numel() < B:
+        raise ValueError(f"{B} sequence lengths need as many block table rows and query rows")
+    if workspace is None:
+        workspace = nibble_decode_workspace(lay, HQ, B, max_seq_len, dev)
+    err = _error_word(error_word, dev)
+    _one_device(query, workspace, err)
+    rc = _on_device(
+        index, _hip.lib().ttkv_nibble_decode_paged, lay.H, HQ, lay.d, float(scale),
+        query.data_ptr(), _hip.DTYPE_CODE[query.dtype], query.stride(0), page_ptr, n_slots,
+        slot_bytes, int(block_size), block_table.data_ptr(), block_table.stride(0),
+        block_table.shape[1], seq_lens.data_ptr(),
+        query_start_loc.data_ptr(), B, int(max_seq_len), out.data_ptr(),
+        _hip.DTYPE_CODE[out.dtype], out.stride(0), workspace.data_ptr(), workspace.numel(),
+        err.data_ptr(), _stream(index))
+    _hip.check(rc, "ttkv_nibble_decode_paged")
+    return out
 
 
 def nibble_prefill_workspace(lay: NibbleLayout, num_heads: int, num_reqs: int, max_q_len: int,
@@ -664,11 +666,18 @@ def nibble_prefill_workspace(lay: NibbleLayout, num_heads: int, num_reqs: int, m
     return torch.zeros(max(int(n), 256), dtype=torch.uint8, device=device)
 
 
-@_on_device
-def _nibble_prefill(query, lay, page, block_size, block_table, seq_lens, query_start_loc,
-                    max_q_len, max_seq_len, scale, req_index, out, workspace, error_word):
-    page_ptr, n_slots, slot_bytes, out = _nibble_read(lay, query, page, block_table, seq_lens,
-                                                      query_start_loc, out)
+def nibble_prefill_paged(lay: NibbleLayout, query: torch.Tensor, page: torch.Tensor,
+                         block_size: int, block_table: torch.Tensor, seq_lens: torch.Tensor,
+                         query_start_loc: torch.Tensor, max_q_len: int, max_seq_len: int,
+                         scale: float, req_index: torch.Tensor | None = None,
+                         out: torch.Tensor | None = None, workspace: torch.Tensor | None = None,
+                         error_word: torch.Tensor | None = None) -> torch.Tensor:
+    """Causal attention of chunks of queries (rows query_start_loc[r] .. [r + 1] of query
+    [N, HQ, d], rotated) over their requests' stored tokens of a 4-bit cache, the chunk's own
+    included. `req_index` picks the batch rows to process (default: all). See
+    `ttkv_nibble_prefill_paged` in include/ttkv_hip.h."""
+    page_ptr, n_slots, slot_bytes, out, index = _nibble_read(lay, query, page, block_table,
+                                                             seq_lens, query_start_loc, out)
     B, HQ, dev = seq_lens.numel(), query.shape[1], query.device
     if block_table.shape[0] < B or query_start_loc.numel() < B + 1:
         raise ValueError(f"{B} sequence lengths need as many block table rows and one more "
@@ -681,26 +690,13 @@ def _nibble_prefill(query, lay, page, block_size, block_table, seq_lens, query_s
         workspace = nibble_prefill_workspace(lay, HQ, B, max_q_len, max_seq_len, dev)
     err = _error_word(error_word, dev)
     _one_device(query, workspace, err)
-    rc = _hip.lib().ttkv_nibble_prefill_paged(
-        lay.H, HQ, lay.d, float(scale), query.data_ptr(), _hip.DTYPE_CODE[query.dtype],
-        query.stride(0), page_ptr, n_slots, slot_bytes, int(block_size), block_table.data_ptr(),
-        block_table.stride(0), block_table.shape[1], seq_lens.data_ptr(),
+    rc = _on_device(
+        index, _hip.lib().ttkv_nibble_prefill_paged, lay.H, HQ, lay.d, float(scale),
+        query.data_ptr(), _hip.DTYPE_CODE[query.dtype], query.stride(0), page_ptr, n_slots,
+        slot_bytes, int(block_size), block_table.data_ptr(), block_table.stride(0),
+        block_table.shape[1], seq_lens.data_ptr(),
         query_start_loc.data_ptr(), _hip.ptr(req_index), B, int(max_q_len), int(max_seq_len),
         out.data_ptr(), _hip.DTYPE_CODE[out.dtype], out.stride(0), workspace.data_ptr(),
-        workspace.numel(), err.data_ptr(), _hip.stream_ptr(dev))
+        workspace.numel(), err.data_ptr(), _stream(index))
     _hip.check(rc, "ttkv_nibble_prefill_paged")
     return out
-
-
-def nibble_prefill_paged(lay: NibbleLayout, query: torch.Tensor, page: torch.Tensor,
-                         block_size: int, block_table: torch.Tensor, seq_lens: torch.Tensor,
-                         query_start_loc: torch.Tensor, max_q_len: int, max_seq_len: int,
-                         scale: float, req_index: torch.Tensor | None = None,
-                         out: torch.Tensor | None = None, workspace: torch.Tensor | None = None,
-                         error_word: torch.Tensor | None = None) -> torch.Tensor:
-    """Causal attention of chunks of queries (rows query_start_loc[r] .. [r + 1] of query
-    [N, HQ, d], rotated) over their requests' stored tokens of a 4-bit cache, the chunk's own
-    included. `req_index` picks the batch rows to process (default: all). See
-    `ttkv_nibble_prefill_paged` in include/ttkv_hip.h."""
-    return _nibble_prefill(query, lay, page, block_size, block_table, seq_lens, query_start_loc,
-                           max_q_len, max_seq_len, scale, req_index, out, workspace, error_word)
