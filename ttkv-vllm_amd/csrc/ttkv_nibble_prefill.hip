@@ -145,13 +145,19 @@ __device__ __forceinline__ NibPrefillPlan np_plan(const NibPrefillArgs& a, int i
   return P;
 }
 
-// Tile buffers, 16-byte chunks exchanged by their row so that a fragment's 16 rows lie in distinct
-// banks: keys [token][16 chunks of 8 dims], values [dim][8 chunks of 8 token slots].
-__device__ __forceinline__ int np_k_at(int token, int chunk) {
-  return token * kD + ((chunk ^ (token & 15)) << 3);
+// Tile buffers, by byte address: keys [token][16 chunks of 8 dims], 256 bytes a token, then values
+// [dim][8 chunks of 8 token slots], 128 bytes a dim. A row's 16-byte chunks are exchanged by XOR with
+// the row's number, so that a fragment's 16 rows lie in distinct banks; chunk 4 s + q4 of the row is
+// then the address of chunk q4 with s << 6 exchanged in. Addresses are formed from the tile's buffer
+// each time, since kept ones spill the matrix operands.
+constexpr uint32_t kNPBuf = 2 * kNPKBytes;  // bytes of a tile
+template <typename T>
+__device__ __forceinline__ T np_get(uint32_t at) {
+  return *(const __attribute__((address_space(3))) T*)(uintptr_t)at;
 }
-__device__ __forceinline__ int np_v_at(int dim, int chunk) {
-  return dim * kNPTile + ((chunk ^ (dim & 7)) << 3);
+template <typename T>
+__device__ __forceinline__ void np_put(uint32_t at, T v) {
+  *(__attribute__((address_space(3))) T*)(uintptr_t)at = v;
 }
 // Barrier for LDS alone: global loads stay in flight across it.
 __device__ __forceinline__ void np_barrier() {
@@ -162,7 +168,7 @@ __device__ __forceinline__ void np_barrier() {
 template <int QDT, int NG>
 __global__ __launch_bounds__(kNPThreads, 2) void nibble_prefill_kernel(NibPrefillArgs a) {
   constexpr int RW = kNPWaves * 16 * NG;
-  extern __shared__ __align__(16) unsigned char smem[];
+  extern __shared__ __align__(1024) unsigned char smem[];  // (the XORs above count on whole rows)
   __shared__ uint32_t nan_sh[2][kNPTile / 4];  // per token of a masked tile: its groups that are NaN
   __shared__ int bad_sh, last_sh;
   const int tid = threadIdx.x, lane = tid & 63;
@@ -213,6 +219,8 @@ __global__ __launch_bounds__(kNPThreads, 2) void nibble_prefill_kernel(NibPrefil
   const uint8_t* base = a.page + (int64_t)h * kNibRecord;
   const int32_t* bt = a.bt + (int64_t)P.r * a.bt_row_stride;
   const NibMasks masks = nib_masks();
+  const uint32_t smem_at = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) unsigned char*)smem;
+  const uint32_t krow = smem_at + col * 256 + ((q4 ^ col) << 4);  // token col, chunk q4
   const bool values = wv >= 4;
   const int tt = wv & 3;  // this wave's record of a tile
   const int last_rec = (n - 1) / kNibTile;
@@ -248,8 +256,7 @@ __global__ __launch_bounds__(kNPThreads, 2) void nibble_prefill_kernel(NibPrefil
   };
   auto dequant_keys = [&](int t) {
     if (t >= t1) return;
-    _Float16* kb = (_Float16*)smem + (t & 1) * (2 * kNPTile * kD);
-    const int token = 16 * tt + col;
+    const uint32_t at = krow + (t & 1) * kNPBuf + tt * (16 * 256);
 #pragma unroll
     for (int g = 0; g < 4; ++g) {
       const half2v zz = nib_biased(par[0][g >> 1], masks), sg = nib_scales(par[0][g >> 1]);
@@ -261,12 +268,11 @@ __global__ __launch_bounds__(kNPThreads, 2) void nibble_prefill_kernel(NibPrefil
         o[2 * j] = v[0];
         o[2 * j + 1] = v[1];
       }
-      *(half8*)(kb + np_k_at(token, 4 * g + q4)) = o;
+      np_put(at ^ (g << 6), o);
     }
   };
   auto dequant_values = [&](int t) {
     if (t >= t1) return;
-    _Float16* vb = (_Float16*)smem + (t & 1) * (2 * kNPTile * kD) + kNPTile * kD;
     const int tok = t * kNPTile + 16 * tt + 4 * q4;  // the lane's four tokens
     if ((t + 1) * kNPTile - 1 > wg_see) {
       // Some row does not see all of this tile. A weight of 0 must not meet a NaN: values past the
@@ -286,7 +292,14 @@ __global__ __launch_bounds__(kNPThreads, 2) void nibble_prefill_kernel(NibPrefil
         }
       if (col == 0) nan_sh[t & 1][4 * tt + q4] = note;
     }
-    const int slot = (tt >> 1) * 4 + q4, half = tt & 1;
+    // chunk 4 (tt / 2) + q4 of dim 2 col + b, its half tt % 2
+    const uint32_t vb = smem_at + (t & 1) * kNPBuf + kNPKBytes + 8 * (tt & 1);
+    uint32_t at[2];
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+      const int dim = 2 * col + b;
+      at[b] = vb + dim * 128 + (((4 * (tt >> 1) + q4) ^ (dim & 7)) << 4);
+    }
 #pragma unroll
     for (int quad = 0; quad < 2; ++quad)
 #pragma unroll
@@ -305,57 +318,77 @@ __global__ __launch_bounds__(kNPThreads, 2) void nibble_prefill_kernel(NibPrefil
           }
         }
 #pragma unroll
-        for (int b = 0; b < 2; ++b) {
-          const int dim = 32 * g + 2 * col + b;
-          *(half4*)(vb + np_v_at(dim, slot) + 4 * half) = o[b];
-        }
+        for (int b = 0; b < 2; ++b) np_put(at[b] + 32 * 128 * g, o[b]);
       }
   };
   auto compute = [&](int t) {
     if (!active || t * kNPTile > see_max) return;
-    const _Float16* kb = (const _Float16*)smem + (t & 1) * (2 * kNPTile * kD);
-    const _Float16* vb = kb + kNPTile * kD;
+    const uint32_t kb = krow + (t & 1) * kNPBuf;
+    const uint32_t vb = smem_at + (t & 1) * kNPBuf + kNPKBytes + col * 128 + ((q4 ^ (col & 7)) << 4);
     const bool masked = (t + 1) * kNPTile - 1 > see_min;
+    // Fragments are asked for a few products ahead (rings of four and three, the order pinned by the
+    // scheduling barriers): with their loads next to their use, every third product waited for LDS.
+    auto key_frag = [&](int ks, int f) {  // f: tokens 16 (f / 4), dims 32 (f % 4)
+      return np_get<half8>((kb ^ ((f & 3) << 6)) + (32 * ks + 16 * (f >> 2)) * 256);
+    };
+    auto value_frag = [&](int ks, int db) {
+      return np_get<half8>((vb ^ (ks << 6)) + 16 * 128 * db);
+    };
+    half8 kf[4], vf[3];
+#pragma unroll
+    for (int f = 0; f < 4; ++f) kf[f] = key_frag(0, f);
 #pragma unroll
     for (int ks = 0; ks < 2; ++ks) {
       float4v sc[NG][2];
 #pragma unroll
-      for (int tg = 0; tg < 2; ++tg) {
+      for (int gr = 0; gr < NG; ++gr) sc[gr][0] = sc[gr][1] = float4v{};
+      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int gr = 0; gr < NG; ++gr) sc[gr][tg] = float4v{};
+      for (int f = 0; f < 8; ++f) {
 #pragma unroll
-        for (int s = 0; s < 4; ++s) {
-          const half8 kf = *(const half8*)(kb + np_k_at(32 * ks + 16 * tg + col, 4 * s + q4));
-#pragma unroll
-          for (int gr = 0; gr < NG; ++gr)
-            sc[gr][tg] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qf[gr][s], sc[gr][tg], 0, 0, 0);
-        }
+        for (int gr = 0; gr < NG; ++gr)
+          sc[gr][f >> 2] =
+              __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[f & 3], qf[gr][f & 3], sc[gr][f >> 2], 0, 0, 0);
+        if (f < 4) kf[f & 3] = key_frag(ks, f + 4);
+        else if (f < 7) vf[f - 4] = value_frag(ks, f - 4);
+        __builtin_amdgcn_sched_barrier(0);
       }
-      half8 pf[NG];
+      if (masked) {
+        const int tok = t * kNPTile + 32 * ks + 4 * q4;
 #pragma unroll
-      for (int gr = 0; gr < NG; ++gr) {
-        if (masked) {
-          const int tok = t * kNPTile + 32 * ks + 4 * q4;
+        for (int gr = 0; gr < NG; ++gr)
 #pragma unroll
           for (int tg = 0; tg < 2; ++tg)
 #pragma unroll
             for (int i = 0; i < 4; ++i)
               if (tok + 16 * tg + i > lim[gr]) sc[gr][tg][i] = -INFINITY;
-        }
-        float mt = -INFINITY;
+      }
+      float mt[NG];
+      bool more = false;
+#pragma unroll
+      for (int gr = 0; gr < NG; ++gr) {
+        mt[gr] = -INFINITY;
 #pragma unroll
         for (int tg = 0; tg < 2; ++tg)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) mt = fmaxf(mt, sc[gr][tg][i]);
-        mt *= qs[gr];
-        if (__builtin_amdgcn_ballot_w64(mt > m[gr] + kNPLazy)) {
-          const float mn = fmaxf(m[gr], cross_row_max(mt));
+          for (int i = 0; i < 4; ++i) mt[gr] = fmaxf(mt[gr], sc[gr][tg][i]);
+        mt[gr] *= qs[gr];
+        more |= mt[gr] > m[gr] + kNPLazy;
+      }
+      if (__builtin_amdgcn_ballot_w64(more)) {
+#pragma unroll
+        for (int gr = 0; gr < NG; ++gr) {
+          const float mn = fmaxf(m[gr], cross_row_max(mt[gr]));
           const float f = exp2f(m[gr] - mn);
           m[gr] = mn;
           l[gr] *= f;
 #pragma unroll
           for (int i = 0; i < 8; ++i) acc[gr][i] *= f;
         }
+      }
+      half8 pf[NG];
+#pragma unroll
+      for (int gr = 0; gr < NG; ++gr)
 #pragma unroll
         for (int tg = 0; tg < 2; ++tg)
 #pragma unroll
@@ -367,13 +400,16 @@ __global__ __launch_bounds__(kNPThreads, 2) void nibble_prefill_kernel(NibPrefil
             pf[gr][4 * tg + i] = p[0];
             pf[gr][4 * tg + i + 1] = p[1];
           }
-      }
+      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int db = 0; db < 8; ++db) {
-        const half8 vf = *(const half8*)(vb + np_v_at(16 * db + col, 4 * ks + q4));
 #pragma unroll
         for (int gr = 0; gr < NG; ++gr)
-          acc[gr][db] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, pf[gr], acc[gr][db], 0, 0, 0);
+          acc[gr][db] =
+              __builtin_amdgcn_mfma_f32_16x16x32_f16(vf[db % 3], pf[gr], acc[gr][db], 0, 0, 0);
+        if (db < 5) vf[db % 3] = value_frag(ks, db + 3);
+        if (db >= 4 && ks == 0) kf[db - 4] = key_frag(1, db - 4);
+        __builtin_amdgcn_sched_barrier(0);
       }
     }
     if ((t + 1) * kNPTile - 1 > wg_see) {  // NaN groups of a tile with masked keys
