@@ -343,6 +343,7 @@ __global__ __launch_bounds__(kNPThreads, 2) void nibble_prefill_kernel(NibPrefil
 #pragma unroll
       for (int gr = 0; gr < NG; ++gr) sc[gr][0] = sc[gr][1] = float4v{};
       __builtin_amdgcn_sched_barrier(0);
+      __builtin_amdgcn_s_setprio(1);
 #pragma unroll
       for (int f = 0; f < 8; ++f) {
 #pragma unroll
@@ -353,6 +354,7 @@ __global__ __launch_bounds__(kNPThreads, 2) void nibble_prefill_kernel(NibPrefil
         else if (f < 7) vf[f - 4] = value_frag(ks, f - 4);
         __builtin_amdgcn_sched_barrier(0);
       }
+      __builtin_amdgcn_s_setprio(0);
       if (masked) {
         const int tok = t * kNPTile + 32 * ks + 4 * q4;
 #pragma unroll
@@ -401,6 +403,7 @@ __global__ __launch_bounds__(kNPThreads, 2) void nibble_prefill_kernel(NibPrefil
             pf[gr][4 * tg + i + 1] = p[1];
           }
       __builtin_amdgcn_sched_barrier(0);
+      __builtin_amdgcn_s_setprio(1);
 #pragma unroll
       for (int db = 0; db < 8; ++db) {
 #pragma unroll
@@ -411,6 +414,7 @@ __global__ __launch_bounds__(kNPThreads, 2) void nibble_prefill_kernel(NibPrefil
         if (db >= 4 && ks == 0) kf[db - 4] = key_frag(1, db - 4);
         __builtin_amdgcn_sched_barrier(0);
       }
+      __builtin_amdgcn_s_setprio(0);
     }
     if ((t + 1) * kNPTile - 1 > wg_see) {  // NaN groups of a tile with masked keys
       const uint32_t mine = nan_sh[t & 1][lane & 15];
