@@ -118,4 +118,13 @@ __device__ __forceinline__ float2v ld_agent2(const float* p) {
   return __builtin_bit_cast(float2v, w);
 }
 
+// Four floats of other workgroups' partial results, at byte `at` of `bytes` from a wave-uniform base:
+// one 16-byte load of the cache policy of an agent-scope load (sc1). ld_agent's atomic loads are of
+// 8 bytes at most; a join is bound by how much it has in flight.
+__device__ __forceinline__ float4v ld_agent16(const float* base, uint32_t bytes, uint32_t at) {
+  const auto rsrc = __builtin_amdgcn_make_buffer_rsrc((void*)base, 0, (int)bytes, 0x00027000);
+  const auto w = __builtin_amdgcn_raw_buffer_load_b128(rsrc, (int)at, 0, 16);
+  return __builtin_bit_cast(float4v, w);
+}
+
 }  // namespace ttkv

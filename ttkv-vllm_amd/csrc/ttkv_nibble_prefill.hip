@@ -528,21 +528,17 @@ __global__ __launch_bounds__(kNPThreads, 2) void nibble_prefill_kernel(NibPrefil
   for (int e = tid; e < nrow * (kD / 4); e += kNPThreads) {
     const int row = e / (kD / 4), d = 4 * (e % (kD / 4));
     float4v o = {};
-    const float* po = a.ws_o + (first + row) * kD + d;
-    const int64_t between = (int64_t)P.rows * kD;  // from a part to the next
-    for (int s0 = 0; s0 < P.ns; s0 += 4) {
-      float2v x[4][2];
+    const uint32_t at = (uint32_t)(row * kD + d) * 4;
+    const uint32_t between = (uint32_t)P.rows * (kD * 4);  // from a part to the next
+    for (int s0 = 0; s0 < P.ns; s0 += 8) {
+      float4v x[8];
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (s0 + i < P.ns) {
-          x[i][0] = ld_agent2(po + (s0 + i) * between);
-          x[i][1] = ld_agent2(po + (s0 + i) * between + 2);
-        }
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
+      for (int i = 0; i < 8; ++i)
         if (s0 + i < P.ns)
-          o += float4v{x[i][0][0], x[i][0][1], x[i][1][0], x[i][1][1]} *
-               ml[(s0 + i) * nrow + row][0];
+          x[i] = ld_agent16(a.ws_o + first * kD, between * (uint32_t)P.ns, at + (s0 + i) * between);
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (s0 + i < P.ns) o += x[i] * ml[(s0 + i) * nrow + row][0];
     }
     const int rr = P.rb * RW + row;
     store_act4(a.out, a.out_dtype,
