@@ -16,8 +16,11 @@
 // out of step and one's matrix products run under the other's vector work.
 //
 // The keys of a row block are split over several workgroups where the batch has too few row blocks
-// to fill the chip; the last to arrive joins the parts' unnormalised results. The split comes from a
-// plan that every workgroup computes alike from the lengths on the device.
+// to fill the chip: the split comes from a plan that every workgroup computes alike from the lengths
+// on the device. The parts' unnormalised results are joined by a second launch, 32 rows per workgroup
+// (a row block's last part cannot join them itself in good time: one CU draws about 45 GB/s from what
+// other XCDs wrote, and 384 rows of four parts are 0.8 MB; 1 x 512 queries with their own keys: 24 us
+// for the join by the last part's workgroup).
 #include <math.h>
 
 #include "ttkv_host.h"
@@ -35,10 +38,7 @@ constexpr float kNPLazy = 8.f;     // log2 of the largest softmax weight before 
 constexpr float kNPNone = -1e30f;  // a maximum before the first visible key
 constexpr int64_t kNPPartRows = 128000;  // rows of partial results a launch may leave: 66.6 MB
 constexpr int kNPKBytes = kNPTile * kD * 2;
-// Two buffers of keys and values; the join's maxima and sums of every part and row.
-constexpr int np_smem(int ng) {
-  return std::max(4 * kNPKBytes, kNPMaxSplit * kNPWaves * 16 * ng * 8);
-}
+constexpr int kNPSmem = 4 * kNPKBytes;  // two buffers of keys and values
 
 struct NibPrefillArgs {
   int H, G;
@@ -57,7 +57,8 @@ struct NibPrefillArgs {
   void* out;
   int out_dtype;
   int64_t out_row_stride;
-  int* ws_cnt;
+  uint8_t* ws_flag;       // [row blocks][RW / 32]: a piece that the join has to take
+  struct NibPrefillJoin* ws_join;  // [row blocks]
   float* ws_o;   // [part rows][kD]
   float* ws_ml;  // [part rows][2]
   int64_t part_rows;
@@ -65,10 +66,19 @@ struct NibPrefillArgs {
   int32_t* err;
 };
 
+// A row block whose keys were split: what its join needs.
+struct NibPrefillJoin {
+  int64_t part, q0;  // its first part row, the chunk's first query row
+  int ns, rows;      // parts, and rows between them
+  int row0, nrow, h;
+};
+constexpr int kNPJoinRows = 32;     // rows per workgroup of the join
+constexpr int kNPJoinThreads = 256;
+
 struct NibPrefillPlan {
   int r, h, rb, sp, ns;  // batch row, KV head, row block, key part and how many
   int n, Q, rows;        // keys, the chunk's queries, rows processed
-  int cnt;               // the row block's counter
+  int block;             // the row block's number in the launch
   int64_t part;          // first part row of the (request, head)
   bool none;
 };
@@ -134,7 +144,7 @@ __device__ __forceinline__ NibPrefillPlan np_plan(const NibPrefillArgs& a, int i
       P.ns = __builtin_amdgcn_readlane(ns, ln);
       P.rb = nrb - 1 - local / P.ns;  // the last rows see the most keys: first
       P.sp = local % P.ns;
-      P.cnt = (blocks + __builtin_amdgcn_readlane(bincl - rb, ln) + P.rb) * a.H + P.h;
+      P.block = (blocks + __builtin_amdgcn_readlane(bincl - rb, ln) + P.rb) * a.H + P.h;
       P.part = (int64_t)(prows + __builtin_amdgcn_readlane(pincl - pr, ln)) * a.H +
                (int64_t)P.h * P.ns * P.rows;
     }
@@ -170,7 +180,7 @@ __global__ __launch_bounds__(kNPThreads, 2) void nibble_prefill_kernel(NibPrefil
   constexpr int RW = kNPWaves * 16 * NG;
   extern __shared__ __align__(1024) unsigned char smem[];  // (the XORs above count on whole rows)
   __shared__ uint32_t nan_sh[2][kNPTile / 4];  // per token of a masked tile: its groups that are NaN
-  __shared__ int bad_sh, last_sh;
+  __shared__ int bad_sh;
   const int tid = threadIdx.x, lane = tid & 63;
   const int wv = __builtin_amdgcn_readfirstlane(tid >> 6);
   const NibPrefillPlan P = np_plan<RW>(a, blockIdx.x);
@@ -488,61 +498,87 @@ __global__ __launch_bounds__(kNPThreads, 2) void nibble_prefill_kernel(NibPrefil
       const int64_t pr = P.part + (int64_t)P.sp * P.rows + row;
 #pragma unroll
       for (int db = 0; db < 8; ++db)
-        store_agent16(a.ws_o + pr * kD + 16 * db + 4 * q4, acc[gr][db]);
-      if (q4 == 0) store_agent8(a.ws_ml + 2 * pr, float2v{m[gr], l[gr]});
+        *gblw((float4v*)(a.ws_o + pr * kD + 16 * db + 4 * q4)) = acc[gr][db];
+      if (q4 == 0) *gblw((float2v*)(a.ws_ml + 2 * pr)) = float2v{m[gr], l[gr]};
     }
   }
-  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-  __syncthreads();
-  if (tid == 0) {
-    int* cnt = a.ws_cnt + P.cnt;
-    const int prev = arrive(cnt);
-    last_sh = prev == P.ns - 1;
-    if (last_sh) __hip_atomic_store(cnt, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  if (P.sp == 0) {
+    if (tid == 0)
+      a.ws_join[P.block] = NibPrefillJoin{P.part + P.rb * RW, q0, P.ns, P.rows, P.rb * RW, nrow, h};
+    constexpr int PIECES = RW / kNPJoinRows;
+    if (tid < PIECES && tid * kNPJoinRows < nrow) a.ws_flag[P.block * PIECES + tid] = 1;
+  }
+}
+
+// Joins the parts of 32 rows: out = sum_s w_s o_s / sum_s w_s l_s, w_s = 2^(m_s - max m). Its flag is
+// set by the attention launch and cleared here, so the flags are zero between calls.
+template <int RW>
+__global__ __launch_bounds__(kNPJoinThreads) void nibble_join_kernel(NibPrefillArgs a) {
+  constexpr int PIECES = RW / kNPJoinRows;
+  __shared__ float2v wgt[kNPMaxSplit][kNPJoinRows];  // weight, sum
+  __shared__ float inv_sh[kNPJoinRows];
+  const int tid = threadIdx.x;
+  const int block = blockIdx.x / PIECES, piece = blockIdx.x % PIECES;
+  uint8_t* flag = a.ws_flag + blockIdx.x;
+  const uint8_t on = *flag;
+  const NibPrefillJoin J = a.ws_join[block];  // (meaningless without the flag)
+  if (!on) return;
+  const int r0 = piece * kNPJoinRows, nr = min(kNPJoinRows, J.nrow - r0);
+  const int64_t first = J.part + r0;
+  constexpr int UNITS = kNPJoinRows * kD / 4 / kNPJoinThreads;  // four floats each
+  auto load = [&](int u, int s) {
+    const int e = tid + u * kNPJoinThreads, row = min(e / (kD / 4), nr - 1);
+    return *gbl((const float4v*)(a.ws_o + (first + (int64_t)s * J.rows + row) * kD +
+                                 4 * (e % (kD / 4))));
+  };
+  constexpr int AHEAD = 2;  // parts in flight
+  float4v x[AHEAD][UNITS];
+#pragma unroll
+  for (int k = 0; k < AHEAD; ++k)
+    if (k < J.ns)
+#pragma unroll
+      for (int u = 0; u < UNITS; ++u) x[k][u] = load(u, k);
+  for (int e = tid; e < J.ns * kNPJoinRows; e += kNPJoinThreads) {
+    const int s = e / kNPJoinRows, row = min(e % kNPJoinRows, nr - 1);
+    wgt[s][e % kNPJoinRows] =
+        *gbl((const float2v*)(a.ws_ml + 2 * (first + (int64_t)s * J.rows + row)));
   }
   __syncthreads();
-  if (!last_sh) return;
-  // ---- the row block's parts joined: every part's maxima and sums to LDS in one round trip, the
-  // rows' weights from them, then the weighted sums, eight parts' loads in flight
-  float2v* ml = (float2v*)smem;  // [parts][nrow]
-  const int64_t first = P.part + P.rb * RW;
-  for (int e = tid; e < P.ns * nrow; e += kNPThreads) {
-    const int s = e / nrow;
-    ml[e] = ld_agent2(a.ws_ml + 2 * (first + (int64_t)s * P.rows + (e - s * nrow)));
-  }
-  __syncthreads();
-  for (int row = tid; row < nrow; row += kNPThreads) {
+  if (tid == 0) *flag = 0;
+  if (tid < kNPJoinRows) {
     float mm = kNPNone, ll = 0.f;
-    for (int s = 0; s < P.ns; ++s) mm = fmaxf(mm, ml[s * nrow + row][0]);
-    for (int s = 0; s < P.ns; ++s) {
-      const float2v x = ml[s * nrow + row];
-      const float w = exp2f(x[0] - mm);
-      ll += x[1] * w;
-      ml[s * nrow + row][0] = w;
+    for (int s = 0; s < J.ns; ++s) mm = fmaxf(mm, wgt[s][tid][0]);
+    for (int s = 0; s < J.ns; ++s) {
+      const float w = exp2f(wgt[s][tid][0] - mm);
+      ll += w * wgt[s][tid][1];
+      wgt[s][tid][0] = w;
     }
-    const float inv = 1.f / ll;
-    for (int s = 0; s < P.ns; ++s) ml[s * nrow + row][0] *= inv;
+    inv_sh[tid] = 1.f / ll;
   }
   __syncthreads();
-#pragma unroll 2
-  for (int e = tid; e < nrow * (kD / 4); e += kNPThreads) {
-    const int row = e / (kD / 4), d = 4 * (e % (kD / 4));
-    float4v o = {};
-    const uint32_t at = (uint32_t)(row * kD + d) * 4;
-    const uint32_t between = (uint32_t)P.rows * (kD * 4);  // from a part to the next
-    for (int s0 = 0; s0 < P.ns; s0 += 8) {
-      float4v x[8];
+  float4v o[UNITS];
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
-        if (s0 + i < P.ns)
-          x[i] = ld_agent16(a.ws_o + first * kD, between * (uint32_t)P.ns, at + (s0 + i) * between);
+  for (int u = 0; u < UNITS; ++u) o[u] = float4v{};
+  for (int s = 0; s < J.ns; s += AHEAD) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
-        if (s0 + i < P.ns) o += x[i] * ml[(s0 + i) * nrow + row][0];
+    for (int k = 0; k < AHEAD; ++k) {
+      if (s + k >= J.ns) break;
+#pragma unroll
+      for (int u = 0; u < UNITS; ++u) {
+        o[u] += x[k][u] * wgt[s + k][(tid + u * kNPJoinThreads) / (kD / 4)][0];
+        if (s + k + AHEAD < J.ns) x[k][u] = load(u, s + k + AHEAD);
+      }
     }
-    const int rr = P.rb * RW + row;
+  }
+#pragma unroll
+  for (int u = 0; u < UNITS; ++u) {
+    const int e = tid + u * kNPJoinThreads, row = e / (kD / 4);
+    if (row >= nr) break;
+    const int rr = J.row0 + r0 + row;
     store_act4(a.out, a.out_dtype,
-               (q0 + rr / G) * a.out_row_stride + (int64_t)(h * G + rr % G) * kD + d, o, true);
+               (J.q0 + rr / a.G) * a.out_row_stride + (int64_t)(J.h * a.G + rr % a.G) * kD +
+                   4 * (e % (kD / 4)),
+               o[u] * inv_sh[row], true);
   }
 }
 
@@ -592,42 +628,56 @@ static int np_groups(int64_t rows) {
   return best;
 }
 
-// Requests per launch: the plan's lanes and a counter per row block and head; with no room for one
-// request's counters, its keys are not split.
+// Requests per launch: the plan's lanes and a flag per 32 rows of every row block and head; with no
+// room for one request's flags, its keys are not split.
 struct NibPrefillSlice {
   int ng, reqs;
   int64_t blocks;  // row blocks of a launch, at most
   bool split;
 };
-static NibPrefillSlice np_slice(int H, int HQ, int num_reqs, int max_q) {
+// Parts of a request at most.
+static int64_t np_max_parts(int max_seq) {
+  const int64_t tiles = (max_seq + kNPTile - 1) / kNPTile;
+  return std::min<int64_t>(kNPMaxSplit, (tiles + kNPMinTiles - 1) / kNPMinTiles);
+}
+
+static NibPrefillSlice np_slice(int H, int HQ, int num_reqs, int max_q, int max_seq) {
   NibPrefillSlice s{};
   s.ng = np_groups((int64_t)max_q * (HQ / H));
   const int64_t rw = kNPWaves * 16 * s.ng;
   const int64_t per = ((int64_t)max_q * (HQ / H) + rw - 1) / rw * H;  // row blocks of one request
-  s.split = per <= kMaxCounters;
+  const int64_t flags = kCounterBytes / (rw / kNPJoinRows);  // row blocks the flags serve
+  s.split = per <= flags && np_max_parts(max_seq) > 1;
   s.reqs = std::min(num_reqs, kNPPlanLanes * 64);
-  if (s.split) s.reqs = (int)std::min<int64_t>(s.reqs, std::max<int64_t>(1, kMaxCounters / std::max<int64_t>(per, 1)));
-  s.reqs = std::max(1, s.reqs);
+  if (s.split) s.reqs = (int)std::min<int64_t>(s.reqs, flags / per);
   s.blocks = per * s.reqs;
   return s;
 }
 
 static int64_t np_part_rows(int HQ, int reqs, int max_q, int max_seq) {
-  const int64_t tiles = (max_seq + kNPTile - 1) / kNPTile;
-  const int64_t parts = std::min<int64_t>(kNPMaxSplit, (tiles + kNPMinTiles - 1) / kNPMinTiles);
-  return parts <= 1 ? 0 : std::min(kNPPartRows, parts * reqs * max_q * HQ);
+  return std::min(kNPPartRows, np_max_parts(max_seq) * reqs * max_q * HQ);
+}
+
+static int64_t np_join_bytes(const NibPrefillSlice& s) {
+  return (s.blocks * (int64_t)sizeof(NibPrefillJoin) + 255) / 256 * 256;
 }
 
 int64_t nibble_prefill_workspace_bytes(int H, int HQ, int num_reqs, int max_q, int max_seq) {
   if (num_reqs == 0 || max_q == 0) return 256;
-  const NibPrefillSlice s = np_slice(H, HQ, num_reqs, max_q);
-  return kCounterBytes + (s.split ? np_part_rows(HQ, s.reqs, max_q, max_seq) * (kD + 2) * 4 : 0);
+  const NibPrefillSlice s = np_slice(H, HQ, num_reqs, max_q, max_seq);
+  if (!s.split) return 256;
+  return kCounterBytes + np_join_bytes(s) + np_part_rows(HQ, s.reqs, max_q, max_seq) * (kD + 2) * 4;
 }
 
 template <int QDT, int NG>
-static int np_launch(const NibPrefillArgs& a, unsigned grid, hipStream_t st) {
-  if (int rc = raise_smem_limit((const void*)nibble_prefill_kernel<QDT, NG>, np_smem(NG))) return rc;
-  hipLaunchKernelGGL((nibble_prefill_kernel<QDT, NG>), dim3(grid), dim3(kNPThreads), np_smem(NG), st, a);
+static int np_launch(const NibPrefillArgs& a, unsigned grid, unsigned blocks, hipStream_t st) {
+  if (int rc = raise_smem_limit((const void*)nibble_prefill_kernel<QDT, NG>, kNPSmem)) return rc;
+  hipLaunchKernelGGL((nibble_prefill_kernel<QDT, NG>), dim3(grid), dim3(kNPThreads), kNPSmem, st, a);
+  if (a.part_rows) {
+    constexpr int RW = kNPWaves * 16 * NG;
+    hipLaunchKernelGGL((nibble_join_kernel<RW>), dim3(blocks * (RW / kNPJoinRows)),
+                       dim3(kNPJoinThreads), 0, st, a);
+  }
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess)
     return host_fail(TTKV_E_LAUNCH, std::string("nibble prefill launch: ") + hipGetErrorString(e));
@@ -652,7 +702,7 @@ int nibble_prefill_paged(int H, int HQ, int d, float scale, const void* q, int q
     return host_fail(TTKV_E_WORKSPACE, "prefill workspace needs " + std::to_string(need) +
                                            " bytes, 256-aligned");
   if (num_reqs == 0 || max_q == 0) return TTKV_OK;
-  const NibPrefillSlice s = np_slice(H, HQ, num_reqs, max_q);
+  const NibPrefillSlice s = np_slice(H, HQ, num_reqs, max_q, max_seq);
   const int64_t items = s.blocks + (s.split ? device_cu_count() + 8 : 0);
   if (items > 0x7fffffff) return host_fail(TTKV_E_INVALID, "too many queries for one call");
   NibPrefillArgs a{};
@@ -675,8 +725,9 @@ int nibble_prefill_paged(int H, int HQ, int d, float scale, const void* q, int q
   a.out_dtype = out_dtype;
   a.out_row_stride = out_row_stride;
   a.part_rows = s.split ? np_part_rows(HQ, s.reqs, max_q, max_seq) : 0;
-  a.ws_cnt = (int*)ws;
-  a.ws_o = (float*)((char*)ws + kCounterBytes);
+  a.ws_flag = (uint8_t*)ws;
+  a.ws_join = (NibPrefillJoin*)((char*)ws + kCounterBytes);
+  a.ws_o = (float*)((char*)ws + kCounterBytes + np_join_bytes(s));
   a.ws_ml = a.ws_o + a.part_rows * kD;
   a.target = device_cu_count();  // a workgroup fills a CU
   a.err = err;
@@ -693,9 +744,9 @@ int nibble_prefill_paged(int H, int HQ, int d, float scale, const void* q, int q
     const bool f16 = q_dtype == TTKV_DTYPE_F16;
     int rc = TTKV_OK;
     switch (s.ng) {
-      case 1: rc = f16 ? np_launch<TTKV_DTYPE_F16, 1>(a, grid, st) : np_launch<TTKV_DTYPE_BF16, 1>(a, grid, st); break;
-      case 2: rc = f16 ? np_launch<TTKV_DTYPE_F16, 2>(a, grid, st) : np_launch<TTKV_DTYPE_BF16, 2>(a, grid, st); break;
-      default: rc = f16 ? np_launch<TTKV_DTYPE_F16, 3>(a, grid, st) : np_launch<TTKV_DTYPE_BF16, 3>(a, grid, st); break;
+      case 1: rc = f16 ? np_launch<TTKV_DTYPE_F16, 1>(a, grid, (unsigned)s.blocks, st) : np_launch<TTKV_DTYPE_BF16, 1>(a, grid, (unsigned)s.blocks, st); break;
+      case 2: rc = f16 ? np_launch<TTKV_DTYPE_F16, 2>(a, grid, (unsigned)s.blocks, st) : np_launch<TTKV_DTYPE_BF16, 2>(a, grid, (unsigned)s.blocks, st); break;
+      default: rc = f16 ? np_launch<TTKV_DTYPE_F16, 3>(a, grid, (unsigned)s.blocks, st) : np_launch<TTKV_DTYPE_BF16, 3>(a, grid, (unsigned)s.blocks, st); break;
     }
     if (rc != TTKV_OK) return rc;
   }
