@@ -424,6 +424,96 @@ def test_prefill_large_and_small_values():
         _close(out, q, *st.kv(0), scale, scale)
 
 
+@pytest.mark.parametrize("H,HQ,n,Q,at", [(1, 4, 300, 100, 230), (1, 4, 70, 70, 3), (1, 2, 90, 8, 85),
+                                         (1, 16, 33, 1, 20), (1, 3, 640, 130, 575)])
+@pytest.mark.parametrize("what", ["value", "key"])
+def test_prefill_nan_stays_behind(H, HQ, n, Q, at, what):
+    """A NaN in a token's value (one group) or key reaches the queries that see the token and no
+    query before it, in the same tile or not."""
+    st = Store([n], H, seed=n, dtype=torch.float16)
+    k, v = st.k.clone(), st.v.clone()
+    (v if what == "value" else k)[at, 0, 37] = float("nan")
+    kernels.nibble_write_paged(st.lay, k.cuda(), v.cuda(), st.slots.cuda(), st.page)
+    q = torch.randn(Q, HQ, D, generator=_gen(n)).half()
+    out, err, _ = _prefill(st, q.cuda(), [Q])
+    assert err == 0
+    clear = max(0, min(Q, at - (n - Q)))         # queries before the token
+    K, V = st.kv(0)
+    if clear:
+        _close(out[:clear], q[:clear], K[:n - Q + clear], V[:n - Q + clear], SCALE, "before")
+    rest = out[clear:]
+    if what == "key":
+        assert bool(torch.isnan(rest).all())
+    else:
+        nan = torch.isnan(rest)
+        assert bool(nan[..., 32:64].all()) and not bool(nan[..., :32].any() or nan[..., 64:].any())
+
+
+@pytest.mark.parametrize("scale", [0.0, -SCALE, 2.0])
+def test_scales_of_any_sign(scale):
+    """Zero (a plain mean), negative, and large enough that one key takes nearly all."""
+    for dtype in (torch.float16, torch.bfloat16):
+        st = Store([333, 40], 2, seed=14, dtype=dtype)
+        q = torch.randn(2, 8, D, generator=_gen(14)).to(dtype)
+        qsl = torch.arange(3, dtype=torch.int32, device="cuda")
+        out = kernels.nibble_decode_paged(st.lay, q.cuda(), st.page, 16, st.bt, st.seq, qsl, 333,
+                                          scale)
+        for r in range(2):
+            _close(out[r:r + 1], q[r:r + 1], *st.kv(r), scale, r)
+        q = torch.randn(70, 8, D, generator=_gen(15)).to(dtype)
+        out = kernels.nibble_prefill_paged(st.lay, q.cuda(), st.page, 16, st.bt, st.seq,
+                                           _i32([0, 40, 70]), 40, 333, scale)
+        for r, s in ((0, slice(0, 40)), (1, slice(40, 70))):
+            _close(out[s], q[s], *st.kv(r), scale, r)
+
+
+def test_prefill_many_requests_and_long_splits():
+    """More requests than a launch's plan holds, with chunks of both kernels; one long request whose
+    keys are split many times."""
+    g = _gen(16)
+    for most in (3, 40):
+        counts = [int(x) for x in torch.randint(0, most + 1, (300,), generator=g)]
+        lens = [c + int(x) for c, x in zip(counts, torch.randint(0, 150, (300,), generator=g))]
+        st = Store(lens, 1, seed=most)
+        q = torch.randn(sum(counts), 4, D, generator=g).half()
+        out, err, qsl = _prefill(st, q.cuda(), counts, max_q=most)
+        assert err == 0
+        for r in range(0, 300, 7):
+            s = slice(qsl[r], qsl[r + 1])
+            if counts[r]:
+                _close(out[s], q[s], *st.kv(r), SCALE, r)
+    for Q in (2, 33):
+        st = Store([20011], 1, seed=17)
+        q = torch.randn(Q, 5, D, generator=g).half()
+        out, err, _ = _prefill(st, q.cuda(), [Q])
+        again, _, _ = _prefill(st, q.cuda(), [Q])
+        assert err == 0 and torch.equal(out, again)
+        _close(out, q, *st.kv(0), SCALE, Q)
+
+
+def test_prefill_workspace_serves_other_shapes():
+    """One workspace for prefill calls of different shapes and for decode calls in turn."""
+    shapes = [([5000, 300], 2, 8, [70, 20]), ([900, 64, 30], 1, 4, [3, 1, 2]), ([1200], 4, 12, [400])]
+    ws = torch.zeros(max(
+        [kernels.nibble_prefill_workspace(NibbleLayout(H), HQ, len(l), max(c), max(l), "cpu").numel()
+         for l, H, HQ, c in shapes]
+        + [kernels.nibble_decode_workspace(NibbleLayout(2), 8, 3, 2000, "cpu").numel()]),
+        dtype=torch.uint8, device="cuda")
+    for lens, H, HQ, counts in shapes * 2:
+        st = Store(lens, H, seed=len(lens))
+        q = torch.randn(sum(counts), HQ, D, generator=_gen(3)).half()
+        out, err, qsl = _prefill(st, q.cuda(), counts, workspace=ws)
+        assert err == 0
+        for r in range(len(lens)):
+            s = slice(qsl[r], qsl[r + 1])
+            _close(out[s], q[s], *st.kv(r), SCALE, (lens[r], H))
+        st, dq, qd, _ = _decode_args(50)
+        out, err = _decode(st, dq, workspace=ws)
+        assert err == 0
+        for r in range(3):
+            _close(out[r:r + 1], dq[r:r + 1].cpu(), *st.kv(r), SCALE, r)
+
+
 def test_prefill_and_decode_agree_on_one_query():
     st = Store([777, 20], 2, seed=13)
     q = torch.randn(2, 8, D, generator=_gen(13)).half()

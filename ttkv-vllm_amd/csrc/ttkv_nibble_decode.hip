@@ -1,22 +1,23 @@
-// Decode attention over the 4-bit cache (format: ttkv_nibble.h): one query per request. gfx950 / CDNA4.
+// Decode attention over the 4-bit cache (format: ttkv_nibble.h): one query per request, and short
+// chunks of queries. gfx950 / CDNA4.
 //
-// Work item = (request, KV head, chunk of the request's 32-token steps), one workgroup of 4 waves
-// that take the chunk's steps in turn. The chunk length comes from a plan that every workgroup
-// computes alike from the batch's lengths: the shortest that spreads the batch's steps over the
-// resident workgroups, so a ragged batch fills the chip by its total work. Items of a (request,
-// head) leave unnormalised partials in the workspace; the last to arrive joins them.
+// The rows of a (request, KV head) are its query heads, or (chunk) its (query, query head) pairs, row
+// = j G + p, 16 at most. Work item = (request, chunk of its 32-token steps, KV head), one workgroup of 4 waves that take the chunk's steps in turn. The chunk length comes from a plan
+// that every workgroup computes alike from the batch's lengths: the shortest that spreads the batch's
+// steps over the resident workgroups, so a ragged batch fills the chip by its total work. Items of a
+// (request, head) leave unnormalised partials in the workspace; the last to arrive joins them.
 //
 // One step of a wave, two tiles of 16 tokens:
-//   S^T [token, query] = K Q^T, four v_mfma_f32_16x16x32_f16 per tile: a lane's 16 key code bytes are
-//     its A operand of all four (token lane % 16, 8 dims of each group of 32), unpacked by a shift and
-//     a mask per pair and dequantised exactly in packed fp16; the query is the B operand, held in
-//     registers. The 16 columns are the G query heads (the rest are zero).
-//   softmax in the result's own registers: lane column = query, 8 tokens of it; the running maximum
+//   S^T [token, row] = K Q^T, four v_mfma_f32_16x16x32_f16 per tile: a lane's 16 key code
+//     bytes are its A operand of all four (token lane % 16, 8 dims of each group of 32), unpacked by a
+//     shift and a mask per pair and dequantised exactly in packed fp16; the queries are the B operand,
+//     held in registers. Columns without a row are zero.
+//   softmax in the result's own registers: lane column = row, 8 tokens of it; the running maximum
 //     moves only when a score exceeds it by 8 (weights stay below 2^8), so most steps need no
 //     exchange between lanes, and the sum stays per lane until the end.
-//   O^T [dim, query] += V^T P^T, eight MFMAs: the scores' layout is the B operand's as it stands, and
-//     a lane's 16 value code bytes per tile are its A operand of all eight (a dim pair of each group,
-//     four tokens). The result's column is the query again, so the rescale is a factor of the lane's.
+//   O^T [dim, row] += V^T P^T, eight MFMAs: the scores' layout is the B operand's as it
+//     stands, and a lane's 16 value code bytes per tile are its A operand of all eight (a dim pair of
+//     each group, four tokens). The result's column is the row again, so the rescale is a lane's factor.
 // Bytes per step 4,608; the two register sets keep the next step's loads in flight.
 #include <math.h>
 
@@ -30,7 +31,8 @@ constexpr int kNDWaves = 4;
 constexpr int kNDStep = 2 * kNibTile;  // tokens per wave step
 constexpr int kNDPlanLanes = 4;        // requests per lane in the plan: 256 per launch
 constexpr float kNDLazy = 8.f;         // log2 of the largest softmax weight before a rescale
-constexpr int kNDPart = kD + 2;        // floats of a partial row: o, max, sum
+constexpr float kNDNone = -1e30f;      // a maximum before the first visible key
+constexpr int kNDRows = 16;            // rows per KV head: a matrix product's columns
 
 struct NibDecodeArgs {
   int H, G;
@@ -45,62 +47,79 @@ struct NibDecodeArgs {
   int64_t bt_row_stride;
   const int32_t* seq_lens;
   const int32_t* qsl;
-  int num_reqs, max_seq;
+  const int32_t* req_index;  // chunks
+  int num_reqs, max_q, max_seq;
   void* out;
   int out_dtype;
   int64_t out_row_stride;
   int* ws_cnt;
-  float* ws_part;
+  float* ws_o;        // [split items][part_rows][kD]
+  float* ws_ml;       // [split items][part_rows][2]
+  uint32_t o_bytes;   // size of ws_o
+  int part_rows;      // rows of an item's partials
   int target;
   int32_t* err;
 };
 
-// Item -> (request, chunk, head); `steps`: 32-token steps of the request, C of them per chunk.
 struct NibDecodePlan {
-  int C, r, c, h, n, n_chunks, first;
+  int r, c, h;          // batch row, chunk, KV head
+  int n, Q, rows, nch;  // keys, queries, rows, chunks
+  int part, block;      // the request's first split item and its number, both before the head
   bool none;
 };
 
+template <bool CHUNK>
 __device__ __forceinline__ NibDecodePlan nd_plan(const NibDecodeArgs& a, int item) {
   const int lane = threadIdx.x & 63;
-  int n[kNDPlanLanes], st[kNDPlanLanes], total = 0;
+  int idx[kNDPlanLanes], n[kNDPlanLanes], Q[kNDPlanLanes], st[kNDPlanLanes];
+  int total = 0;
 #pragma unroll
   for (int i = 0; i < kNDPlanLanes; ++i) {
     const int r = lane + 64 * i;
-    n[i] = r < a.num_reqs ? a.seq_lens[r] : 0;
+    const bool on = r < a.num_reqs;
+    idx[i] = CHUNK && a.req_index && on ? a.req_index[r] : on ? r : 0;
+    n[i] = on ? a.seq_lens[idx[i]] : 0;
+    Q[i] = on ? (CHUNK ? a.qsl[idx[i] + 1] - a.qsl[idx[i]] : 1) : 0;
   }
 #pragma unroll
   for (int i = 0; i < kNDPlanLanes; ++i) {
-    st[i] = (min(max(n[i], 0), a.max_seq) + kNDStep - 1) / kNDStep;
+    const int nn = min(max(n[i], 0), a.max_seq);
+    st[i] = (nn + kNDStep - 1) / kNDStep;
+    if (CHUNK && nn < Q[i]) st[i] = 1;
+    if (Q[i] <= 0) st[i] = 0;
     total += st[i];
   }
   total = wave_sum_i(total);
-  NibDecodePlan P{};
   // whole rounds of the four waves
   const int64_t all = (int64_t)total * a.H;
   const int64_t per = (all + a.target - 1) / a.target;
-  P.C = max(1, (int)((per + kNDWaves - 1) / kNDWaves)) * kNDWaves;
+  const int C = max(1, (int)((per + kNDWaves - 1) / kNDWaves)) * kNDWaves;
+  NibDecodePlan P{};
   P.h = item % a.H;
-  const int it = item / a.H;  // among (request, chunk)
-  int carry = 0;
+  const int it = item / a.H;
+  int carry = 0, parts = 0;
   P.none = true;
 #pragma unroll
   for (int i = 0; i < kNDPlanLanes; ++i) {
     if (64 * i >= a.num_reqs) break;
-    const int r = lane + 64 * i;
-    const int nch = r < a.num_reqs ? max(1, (st[i] + P.C - 1) / P.C) : 0;
+    const int nch = Q[i] > 0 ? max(1, (st[i] + C - 1) / C) : 0, split = nch > 1 ? nch : 0;
     const int incl = nib_scan(nch), ex = carry + incl - nch;
+    const int pincl = nib_scan(split);
     const uint64_t hit = __builtin_amdgcn_ballot_w64(nch > 0 && ex <= it && it < ex + nch);
     if (hit) {
       const int ln = __builtin_ctzll(hit);
       P.none = false;
-      P.r = 64 * i + ln;
-      P.first = __builtin_amdgcn_readlane(ex, ln);
-      P.c = it - P.first;
+      P.r = __builtin_amdgcn_readlane(idx[i], ln);
       P.n = __builtin_amdgcn_readlane(n[i], ln);
-      P.n_chunks = __builtin_amdgcn_readlane(nch, ln);
+      P.Q = __builtin_amdgcn_readlane(Q[i], ln);
+      P.nch = __builtin_amdgcn_readlane(nch, ln);
+      P.c = it - __builtin_amdgcn_readlane(ex, ln);
+      P.rows = CHUNK ? min(max(P.Q, 0), a.max_q) * a.G : a.G;
+      P.part = parts + __builtin_amdgcn_readlane(pincl - split, ln);
+      P.block = 64 * i + ln;
     }
     carry += __builtin_amdgcn_readlane(incl, 63);
+    parts += __builtin_amdgcn_readlane(pincl, 63);
   }
   return P;
 }
@@ -113,45 +132,54 @@ struct NibStep {
   u32x4 vp[2][2];
 };
 
-template <int QDT>
+template <int QDT, bool CHUNK>
 __global__ __launch_bounds__(kNDThreads, 2) void nibble_decode_kernel(NibDecodeArgs a) {
-  __shared__ float red_o[kNDWaves][16][kD];
-  __shared__ float red_m[kNDWaves][16], red_l[kNDWaves][16];
+  __shared__ float red_o[kNDWaves][kNDRows][kD];
+  __shared__ float red_m[kNDWaves][kNDRows], red_l[kNDWaves][kNDRows];
   __shared__ int last_sh;
   const int tid = threadIdx.x, lane = tid & 63;
   const int wv = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const NibDecodePlan P = nd_plan(a, blockIdx.x);
+  const NibDecodePlan P = nd_plan<CHUNK>(a, blockIdx.x);
   if (P.none) return;
-  const int r = P.r, h = P.h, G = a.G;
+  const int h = P.h, G = a.G;
   const int n = min(max(P.n, 0), a.max_seq);
-  if (P.n > a.max_seq && P.c == 0 && h == 0 && tid == 0) atomicOr(a.err, TTKV_ERR_SEQ_LEN);
-  const int64_t row = a.qsl[r];
-  if (n == 0) {  // no keys: the attention is 0
-    for (int i = tid; i < G * kD; i += kNDThreads)
-      store_act(a.out, a.out_dtype, row * a.out_row_stride + (int64_t)h * G * kD + i, 0.f);
+  const int p0 = CHUNK ? n - P.Q : n - 1;  // position of query 0
+  if (tid == 0 && h == 0 && P.c == 0 &&
+      (P.n > a.max_seq || (CHUNK && (P.Q > a.max_q || p0 < 0))))
+    atomicOr(a.err, TTKV_ERR_SEQ_LEN);
+  const int64_t q0 = a.qsl[P.r];
+  const int nrow = P.rows;
+  // row `row` in the query and the output
+  auto row_at = [&](int row, int64_t stride) -> int64_t {
+    const int j = CHUNK ? row / G : 0;
+    return (q0 + j) * stride + (int64_t)(h * G + row - j * G) * kD;
+  };
+  if (CHUNK ? p0 < 0 : n == 0) {  // fewer keys than queries; an empty request's attention is 0
+    for (int i = tid; i < nrow * kD; i += kNDThreads)
+      store_act(a.out, a.out_dtype, row_at(i / kD, a.out_row_stride) + i % kD, CHUNK ? NAN : 0.f);
     return;
   }
   const int col = lane & 15, q4 = lane >> 4;
 
-  // The query, column `col`, as the B operand of the four score products: dims 32 g + 8 q4 ...
+  // The queries, row `col`, as the B operand of the four score products
   half8 qf[4];
-  float qs;
-  nib_load_query<QDT>(a.q + row * a.q_row_stride + (int64_t)(h * G + min(col, G - 1)) * kD, q4,
-                      a.scale_log2, col < G, qf, qs);
-
-  const int steps = (n + kNDStep - 1) / kNDStep;
-  // the request's steps in equal parts
-  const int s0 = (int)((int64_t)steps * P.c / P.n_chunks);
-  const int s1 = (int)((int64_t)steps * (P.c + 1) / P.n_chunks);
-  float4v acc[8];  // [group][dim of the pair]: dims 32 g + 8 q4 + 2 i + b of the column's query
+  float qs, m = kNDNone, l = 0.f;
+  nib_load_query<QDT>(a.q + row_at(min(col, nrow - 1), a.q_row_stride), q4, a.scale_log2,
+                      col < nrow, qf, qs);
+  const int lim = CHUNK ? p0 + min(col, nrow - 1) / G : p0;  // last key the lane's row sees
+  float4v acc[8];  // [group][dim of the pair]: dims 32 g + 8 q4 + 2 i + b of the lane's row
 #pragma unroll
   for (int i = 0; i < 8; ++i) acc[i] = float4v{};
-  float m = -INFINITY, l = 0.f;
+
+  const int steps = (CHUNK ? p0 + (nrow - 1) / G : p0) / kNDStep + 1;
+  // the steps in equal parts
+  const int s0 = (int)((int64_t)steps * P.c / P.nch);
+  const int s1 = (int)((int64_t)steps * (P.c + 1) / P.nch);
   bool bad = false;
 
   const NibMasks masks = nib_masks();
   const uint8_t* base = a.page + (int64_t)h * kNibRecord;
-  const int32_t* bt = a.bt + (int64_t)r * a.bt_row_stride;
+  const int32_t* bt = a.bt + (int64_t)P.r * a.bt_row_stride;
   // tile ids of this wave's next 64 steps, one step per lane (-1: a block outside the cache)
   int tid0 = 0, tid1 = 0;
   auto fetch_ids = [&](int s) {
@@ -195,29 +223,37 @@ __global__ __launch_bounds__(kNDThreads, 2) void nibble_decode_kernel(NibDecodeA
       }
     }
     const int tok = s * kNDStep + 4 * q4;
-    if ((s + 1) * kNDStep > n) {  // the last step: no score and no value past the last token
+    uint32_t note = 0;  // bit 16 t + 4 i + g: that group of the lane's token is NaN
+    if ((s + 1) * kNDStep - 1 > p0) {
+      // Some row does not see all of this step: no score past its last key. A weight of 0 must not
+      // meet a NaN: values past the last key become 0, and in a chunk a group that is NaN becomes 0
+      // too and is noted for the rows that see it.
 #pragma unroll
       for (int t = 0; t < 2; ++t)
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-          if (tok + 16 * t + i >= n) {
-            sc[t][i] = -INFINITY;
-            const uint32_t keep = i & 1 ? 0x0000ffffu : 0xffff0000u;
+        for (int i = 0; i < 4; ++i) {
+          const int tk = tok + 16 * t + i;
+          if (tk > lim) sc[t][i] = -INFINITY;
+          const uint32_t keep = i & 1 ? 0x0000ffffu : 0xffff0000u;
 #pragma unroll
-            for (int g = 0; g < 4; ++g) x.vp[t][g >> 1][2 * (g & 1) + (i >> 1)] &= keep;
+          for (int g = 0; g < 4; ++g) {
+            const int at = 2 * (g & 1) + (i >> 1);
+            const uint32_t w = x.vp[t][g >> 1][at], p = i & 1 ? w >> 16 : w & 0xffffu;
+            const bool nan = CHUNK && (p & 0x7c00u) == 0x7c00u;
+            if (tk >= n || nan) x.vp[t][g >> 1][at] = w & keep;
+            if (CHUNK && nan && tk < n) note |= 1u << (16 * t + 4 * i + g);
           }
+        }
     }
     float mt = -INFINITY;
 #pragma unroll
     for (int t = 0; t < 2; ++t)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        mt = fmaxf(mt, sc[t][i]);
-      }
+      for (int i = 0; i < 4; ++i) mt = fmaxf(mt, sc[t][i]);
     mt *= qs;
     if (__builtin_amdgcn_ballot_w64(mt > m + kNDLazy)) {
       const float mn = fmaxf(m, cross_row_max(mt));
-      const float f = m == -INFINITY ? 0.f : exp2f(m - mn);
+      const float f = exp2f(m - mn);
       m = mn;
       l *= f;
 #pragma unroll
@@ -258,6 +294,16 @@ __global__ __launch_bounds__(kNDThreads, 2) void nibble_decode_kernel(NibDecodeA
         for (int b = 0; b < 2; ++b)
           acc[2 * g + b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf[b], pf, acc[2 * g + b], 0, 0, 0);
       }
+    if (CHUNK && __builtin_amdgcn_ballot_w64(note != 0)) {
+      for (int k = 0; k < kNDStep; ++k) {  // token 16 t + 4 q + i
+        const int of = __builtin_amdgcn_readlane((int)note, 16 * ((k >> 2) & 3));
+        const int groups = (of >> (16 * (k >> 4) + 4 * (k & 3))) & 15;
+        if (!groups) continue;
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          if ((groups >> (i >> 1) & 1) && s * kNDStep + k <= lim) acc[i] += NAN;
+      }
+    }
   };
 
   for (int s = s0 + wv; s < s1;) {
@@ -278,11 +324,8 @@ __global__ __launch_bounds__(kNDThreads, 2) void nibble_decode_kernel(NibDecodeA
     }
     s += kNDWaves * 64;
   }
-  if (bad) {
-    l = NAN;
-    if (lane == 0) atomicOr(a.err, TTKV_ERR_BAD_BLOCK);
-  }
-  l = cross_row_sum(l);
+  if (bad && lane == 0) atomicOr(a.err, TTKV_ERR_BAD_BLOCK);
+  l = bad ? NAN : cross_row_sum(l);
 
   // ---- the four waves' results, joined in LDS
   if (q4 == 0) {
@@ -290,11 +333,11 @@ __global__ __launch_bounds__(kNDThreads, 2) void nibble_decode_kernel(NibDecodeA
     red_l[wv][col] = l;
   }
   __syncthreads();
-  float M = -INFINITY;
+  float M = kNDNone;
 #pragma unroll
   for (int w = 0; w < kNDWaves; ++w) M = fmaxf(M, red_m[w][col]);
-  const float f = m == -INFINITY ? 0.f : exp2f(m - M);
-  if (col < G) {
+  const float f = exp2f(m - M);
+  if (col < nrow) {
 #pragma unroll
     for (int g = 0; g < 4; ++g)
 #pragma unroll
@@ -304,112 +347,215 @@ __global__ __launch_bounds__(kNDThreads, 2) void nibble_decode_kernel(NibDecodeA
       }
   }
   __syncthreads();
-  const int64_t orow = row * a.out_row_stride + (int64_t)h * G * kD;
-  const int64_t item = ((int64_t)P.first + P.c) * a.H + h;
-  float* part = a.ws_part + item * G * kNDPart;
-  for (int e = 2 * tid; e < G * kD; e += 2 * kNDThreads) {  // (a wave covers one row)
+  const int PR = a.part_rows;
+  const int64_t part = ((int64_t)P.part + P.c) * a.H + h;  // (where the request is split)
+  for (int e = 4 * tid; e < nrow * kD; e += 4 * kNDThreads) {
     const int p = e / kD, d = e % kD;
-    float mm = -INFINITY, ll = 0.f;
-    float2v o = {};
+    float mm = kNDNone, ll = 0.f;
+    float4v o = {};
 #pragma unroll
     for (int w = 0; w < kNDWaves; ++w) mm = fmaxf(mm, red_m[w][p]);
 #pragma unroll
-    for (int w = 0; w < kNDWaves; ++w) {
-      ll += red_m[w][p] == -INFINITY && red_l[w][p] == 0.f ? 0.f
-                                                           : red_l[w][p] * exp2f(red_m[w][p] - mm);
-      o += *(const float2v*)&red_o[w][p][d];
-    }
-    if (P.n_chunks == 1) {
-      const float inv = 1.f / ll;
-      store_act(a.out, a.out_dtype, orow + e, o[0] * inv);
-      store_act(a.out, a.out_dtype, orow + e + 1, o[1] * inv);
+    for (int w = 0; w < kNDWaves; ++w) ll += red_l[w][p] * exp2f(red_m[w][p] - mm);
+#pragma unroll
+    for (int w = 0; w < kNDWaves; ++w) o += *(const float4v*)&red_o[w][p][d];
+    if (P.nch == 1) {
+      store_act4(a.out, a.out_dtype, row_at(p, a.out_row_stride) + d, o * (1.f / ll), true);
     } else {
-      store_agent8(part + p * kNDPart + d, o);
-      if (d == 0) store_agent8(part + p * kNDPart + kD, float2v{mm, ll});
+      store_agent16(a.ws_o + (part * PR + p) * kD + d, o);
+      if (d == 0) store_agent8(a.ws_ml + (part * PR + p) * 2, float2v{mm, ll});
     }
   }
-  if (P.n_chunks == 1) return;
+  if (P.nch == 1) return;
 
   // ---- the last workgroup of a (request, head) joins its chunks' partials
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   __syncthreads();
   if (tid == 0) {
-    int* cnt = a.ws_cnt + r * a.H + h;
+    int* cnt = a.ws_cnt + P.block * a.H + h;
     const int prev = arrive(cnt);
-    last_sh = prev == P.n_chunks - 1;
+    last_sh = prev == P.nch - 1;
     if (last_sh) __hip_atomic_store(cnt, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
   }
   __syncthreads();
   if (!last_sh) return;
-  const int64_t cstride = (int64_t)a.H * G * kNDPart;
-  for (int p = wv; p < G; p += kNDWaves) {
-    const float* pp = a.ws_part + ((int64_t)P.first * a.H + h) * G * kNDPart + p * kNDPart;
-    float mm = -INFINITY, ll = 0.f;
-    float2v o = {};
-    for (int c0 = 0; c0 < P.n_chunks; c0 += 64) {
-      const int nb = min(64, P.n_chunks - c0);
-      const float* pl = pp + (c0 + min(lane, nb - 1)) * cstride + kD;
-      const float2v ml = ld_agent2(pl);
-      const float mc = lane < nb ? ml[0] : -INFINITY, lc = ml[1];
-      const float mn = fmaxf(mm, wave_max(mc));
-      const float keep = mm == -INFINITY ? 0.f : exp2f(mm - mn);
-      const float wc = lane < nb ? exp2f(mc - mn) : 0.f;
-      ll = ll * keep + wave_sum(lane < nb ? lc * wc : 0.f);
-      o *= keep;
-      for (int j = 0; j < nb; j += 8) {
-        float2v x[8];
+  // Half a wave takes a row, a lane four dims of it; lane % 32 first holds a chunk's maximum and sum.
+  // All of a wave's rows are under way together.
+  constexpr int ROWS = kNDRows / (2 * kNDWaves);  // per half wave
+  const int c32 = lane & 31, lead = lane & 32;
+  const int64_t part0 = (int64_t)P.part * a.H + h;
+  float mm[ROWS], ll[ROWS];
+  float4v o[ROWS];
+  int row[ROWS];
 #pragma unroll
-        for (int u = 0; u < 8; ++u) {
-          const float* po = pp + (c0 + min(j + u, nb - 1)) * cstride + 2 * lane;
-          x[u] = ld_agent2(po);
-        }
+  for (int k = 0; k < ROWS; ++k) {
+    row[k] = min(2 * (wv + kNDWaves * k) + (lane >> 5), nrow - 1);
+    mm[k] = kNDNone;
+    ll[k] = 0.f;
+    o[k] = float4v{};
+  }
+  constexpr int AHEAD = 8;  // chunks of every row in flight
+  for (int c0 = 0; c0 < P.nch; c0 += 32) {
+    const int nb = min(32, P.nch - c0);
+    float4v x[ROWS][AHEAD];
+    auto fetch = [&](int j) {
 #pragma unroll
-        for (int u = 0; u < 8; ++u) {
-          const float w = __builtin_bit_cast(
-              float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, wc), min(j + u, 63)));
-          if (j + u < nb) o += x[u] * w;
-        }
-      }
-      mm = mn;
+      for (int k = 0; k < ROWS; ++k)
+        if (2 * (wv + kNDWaves * k) < nrow)
+#pragma unroll
+          for (int u = 0; u < AHEAD; ++u)
+            if (j + u < nb)
+              x[k][u] = ld_agent16(
+                  a.ws_o, a.o_bytes,
+                  (uint32_t)((((part0 + (int64_t)(c0 + j + u) * a.H) * PR + row[k]) * kD + 4 * c32) * 4));
+    };
+    float2v ml[ROWS];
+    float wc[ROWS];
+#pragma unroll
+    for (int k = 0; k < ROWS; ++k)
+      ml[k] = ld_agent2(a.ws_ml + ((part0 + (int64_t)(c0 + min(c32, nb - 1)) * a.H) * PR + row[k]) * 2);
+    fetch(0);  // (a round trip that the weights' does not come before)
+#pragma unroll
+    for (int k = 0; k < ROWS; ++k) {
+      float x0, x1;
+      swap16(row_max(c32 < nb ? ml[k][0] : kNDNone), x0, x1);
+      const float mn = fmaxf(mm[k], fmaxf(x0, x1));
+      const float keep = exp2f(mm[k] - mn);
+      wc[k] = c32 < nb ? exp2f(ml[k][0] - mn) : 0.f;
+      swap16(row_sum(c32 < nb ? ml[k][1] * wc[k] : 0.f), x0, x1);
+      ll[k] = ll[k] * keep + x0 + x1;
+      o[k] *= keep;
+      mm[k] = mn;
     }
-    const float inv = 1.f / ll;
-    store_act(a.out, a.out_dtype, orow + p * kD + 2 * lane, o[0] * inv);
-    store_act(a.out, a.out_dtype, orow + p * kD + 2 * lane + 1, o[1] * inv);
+    for (int j = 0; j < nb; j += AHEAD) {
+      if (j) fetch(j);
+#pragma unroll
+      for (int u = 0; u < AHEAD; ++u)
+        if (j + u < nb)
+#pragma unroll
+          for (int k = 0; k < ROWS; ++k) {
+            const float w = __shfl(wc[k], lead + j + u);
+            if (2 * (wv + kNDWaves * k) < nrow) o[k] += x[k][u] * w;
+          }
+    }
+  }
+#pragma unroll
+  for (int k = 0; k < ROWS; ++k) {
+    const int r = 2 * (wv + kNDWaves * k) + (lane >> 5);
+    if (r < nrow)
+      store_act4(a.out, a.out_dtype, row_at(r, a.out_row_stride) + 4 * c32, o[k] * (1.f / ll[k]), true);
   }
 }
 
-// The plan's item target: two workgroups per CU. A third would fit, but shorter chunks pay their
-// prologue and join more often (8 x 14,402 tokens: 31.2 us at two per CU, 32.8 at three, 36.2 at
-// four; 61 requests of 70 to 2,900: 33.4, 35.0, 34.6).
-static int nd_target() {
-  static int slots = 0;
-  if (!slots) {
-    int per_cu = 0;
-    if (hipOccupancyMaxActiveBlocksPerMultiprocessor(
-            &per_cu, nibble_decode_kernel<TTKV_DTYPE_F16>, kNDThreads, 0) != hipSuccess ||
-        per_cu < 1)
-      per_cu = 2;
-    slots = std::min(per_cu, 2) * device_cu_count();
-  }
-  return slots;
-}
+// The plan's item target: two workgroups per CU. A third would fit beside them, but shorter chunks
+// pay their prologue and join more often (8 x 14,402 tokens: 31.2 us at two per CU, 32.8 at three, 36.2
+// at four; 61 requests of 70 to 2,900: 33.4, 35.0, 34.6).
+static int nd_target() { return 2 * device_cu_count(); }
 
 // Requests per launch: the plan's lanes, and a counter per (request, head).
 static int nd_slice(int H, int num_reqs) {
   return std::max(1, std::min({num_reqs, kNDPlanLanes * 64, kMaxCounters / H}));
 }
 
-// Items a launch of nr requests can plan: the target's share and a rounding per (request, head),
-// and never more than one per round of the four waves.
-static int64_t nd_max_items(int H, int nr, int max_seq) {
+// Chunks of a request at most: whole rounds of the four waves.
+static int64_t nd_max_chunks(int max_seq) {
   const int64_t round = kNDStep * kNDWaves;
-  const int64_t most = std::max<int64_t>(1, (max_seq + round - 1) / round);
-  return std::min((int64_t)nd_target() + (int64_t)nr * H, (int64_t)nr * H * most);
+  return std::max<int64_t>(1, (max_seq + round - 1) / round);
+}
+
+// Items of split requests, at most. A chunk has at least total / target steps, and a split request of
+// st steps has less than st / C + 1 < 2 st / C chunks: less than 2 target of them in all.
+static int64_t nd_parts(int H, int nr, int max_seq) {
+  const int64_t most = nd_max_chunks(max_seq);
+  return most <= 1 ? 0 : std::min<int64_t>(2 * nd_target(), (int64_t)nr * H * most);
+}
+
+static int64_t nd_workspace(int H, int num_reqs, int max_seq, int rows) {
+  if (num_reqs == 0 || H > kMaxCounters) return 256;
+  return kCounterBytes + nd_parts(H, nd_slice(H, num_reqs), max_seq) * rows * (kD + 2) * 4;
 }
 
 int64_t nibble_decode_workspace_bytes(int H, int HQ, int num_reqs, int max_seq) {
-  if (num_reqs == 0) return 256;
-  return kCounterBytes + nd_max_items(H, nd_slice(H, num_reqs), max_seq) * (HQ / H) * kNDPart * 4;
+  return nd_workspace(H, num_reqs, max_seq, HQ / H);
+}
+
+// Chunks of at most 16 rows take this kernel: it reads every key for 16 rows, the prefill kernel for 128,
+// but without tiles in LDS or a second launch (3 chunks of 4 queries and 4 heads per KV head over
+// 3,000 keys: 16.2 us here, 19.6 there; of 8, in two groups of rows here: 24.3 and 22.2).
+bool nibble_short_applies(int H, int HQ, int max_q) {
+  return (int64_t)max_q * (HQ / H) <= kNDRows && H <= kMaxCounters;
+}
+
+int64_t nibble_short_workspace_bytes(int H, int HQ, int num_reqs, int max_q, int max_seq) {
+  return nd_workspace(H, num_reqs, max_seq, max_q * (HQ / H));
+}
+
+template <bool CHUNK>
+static int nd_launch(const NibDecodeArgs& a, unsigned grid, int q_dtype, hipStream_t st) {
+  if (q_dtype == TTKV_DTYPE_F16)
+    hipLaunchKernelGGL((nibble_decode_kernel<TTKV_DTYPE_F16, CHUNK>), dim3(grid),
+                       dim3(kNDThreads), 0, st, a);
+  else
+    hipLaunchKernelGGL((nibble_decode_kernel<TTKV_DTYPE_BF16, CHUNK>), dim3(grid),
+                       dim3(kNDThreads), 0, st, a);
+  const hipError_t e = hipGetLastError();
+  if (e != hipSuccess)
+    return host_fail(TTKV_E_LAUNCH, std::string("nibble decode launch: ") + hipGetErrorString(e));
+  return TTKV_OK;
+}
+
+// The arguments have been checked. max_q == 0: decode.
+int nibble_decode_launch(int H, int HQ, float scale, const void* q, int q_dtype,
+                         int64_t q_row_stride, const uint8_t* page, int64_t n_slots,
+                         int64_t slot_stride, int bs, const int32_t* bt, int64_t bt_row_stride,
+                         const int32_t* seq_lens, const int32_t* qsl, const int32_t* req_index,
+                         int num_reqs, int max_q, int max_seq, void* out, int out_dtype,
+                         int64_t out_row_stride, void* ws, int32_t* err, hipStream_t st) {
+  const int slice = nd_slice(H, num_reqs);
+  const int64_t parts = nd_parts(H, slice, max_seq);
+  NibDecodeArgs a{};
+  a.H = H;
+  a.G = HQ / H;
+  a.scale_log2 = scale * 1.4426950408889634f;
+  a.q = (const uint16_t*)q;
+  a.q_row_stride = q_row_stride;
+  a.page = page;
+  a.tile_stride = kNibTile * slot_stride;
+  a.num_blocks = (int)(n_slots / bs);
+  a.tpb = bs / kNibTile;
+  a.bt = bt;
+  a.bt_row_stride = bt_row_stride;
+  a.seq_lens = seq_lens;
+  a.qsl = qsl;
+  a.max_q = max_q;
+  a.max_seq = max_seq;
+  a.out = out;
+  a.out_dtype = out_dtype;
+  a.out_row_stride = out_row_stride;
+  a.part_rows = a.G * std::max(max_q, 1);
+  a.ws_cnt = (int*)ws;
+  a.ws_o = (float*)((char*)ws + kCounterBytes);
+  a.ws_ml = a.ws_o + parts * a.part_rows * kD;
+  a.o_bytes = (uint32_t)(parts * a.part_rows * kD * 4);
+  a.target = nd_target();
+  a.err = err;
+  for (int r0 = 0; r0 < num_reqs; r0 += slice) {
+    a.num_reqs = std::min(slice, num_reqs - r0);
+    if (req_index) {
+      a.req_index = req_index + r0;
+    } else {
+      a.seq_lens = seq_lens + r0;
+      a.qsl = qsl + r0;
+      a.bt = bt + (int64_t)r0 * bt_row_stride;
+    }
+    // an item per (request, head), and what the split ones have more
+    const int64_t pairs = (int64_t)a.num_reqs * H;
+    const unsigned grid = (unsigned)std::min(pairs + nd_target(), pairs * nd_max_chunks(max_seq));
+    const int rc = max_q > 0 ? nd_launch<true>(a, grid, q_dtype, st)
+                             : nd_launch<false>(a, grid, q_dtype, st);
+    if (rc != TTKV_OK) return rc;
+  }
+  return TTKV_OK;
 }
 
 int nibble_decode_paged(int H, int HQ, int d, float scale, const void* q, int q_dtype,
@@ -427,42 +573,10 @@ int nibble_decode_paged(int H, int HQ, int d, float scale, const void* q, int q_
   if (!ws || ws_bytes < need || (uintptr_t)ws % 256)
     return host_fail(TTKV_E_WORKSPACE, "decode workspace needs " + std::to_string(need) +
                                            " bytes, 256-aligned");
-  const int slice = nd_slice(H, num_reqs);
-  for (int r0 = 0; r0 < num_reqs; r0 += slice) {
-    const int nr = std::min(slice, num_reqs - r0);
-    NibDecodeArgs a{};
-    a.H = H;
-    a.G = HQ / H;
-    a.scale_log2 = scale * 1.4426950408889634f;
-    a.q = (const uint16_t*)q;
-    a.q_row_stride = q_row_stride;
-    a.page = page;
-    a.tile_stride = kNibTile * slot_stride;
-    a.num_blocks = (int)(n_slots / bs);
-    a.tpb = bs / kNibTile;
-    a.bt = bt + (int64_t)r0 * bt_row_stride;
-    a.bt_row_stride = bt_row_stride;
-    a.seq_lens = seq_lens + r0;
-    a.qsl = qsl + r0;
-    a.num_reqs = nr;
-    a.max_seq = max_seq;
-    a.out = out;
-    a.out_dtype = out_dtype;
-    a.out_row_stride = out_row_stride;
-    a.ws_cnt = (int*)ws;
-    a.ws_part = (float*)((char*)ws + kCounterBytes);
-    a.target = nd_target();
-    a.err = err;
-    const dim3 grid((unsigned)nd_max_items(H, nr, max_seq));
-    if (q_dtype == TTKV_DTYPE_F16)
-      hipLaunchKernelGGL((nibble_decode_kernel<TTKV_DTYPE_F16>), grid, dim3(kNDThreads), 0, st, a);
-    else
-      hipLaunchKernelGGL((nibble_decode_kernel<TTKV_DTYPE_BF16>), grid, dim3(kNDThreads), 0, st, a);
-    const hipError_t e = hipGetLastError();
-    if (e != hipSuccess)
-      return host_fail(TTKV_E_LAUNCH, std::string("nibble decode launch: ") + hipGetErrorString(e));
-  }
-  return TTKV_OK;
+  if (num_reqs == 0) return TTKV_OK;
+  return nibble_decode_launch(H, HQ, scale, q, q_dtype, q_row_stride, page, n_slots, slot_stride,
+                              bs, bt, bt_row_stride, seq_lens, qsl, nullptr, num_reqs, 0, max_seq,
+                              out, out_dtype, out_row_stride, ws, err, st);
 }
 
 }  // namespace ttkv

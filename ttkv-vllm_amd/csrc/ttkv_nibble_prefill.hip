@@ -511,7 +511,9 @@ __global__ __launch_bounds__(kNPThreads, 2) void nibble_prefill_kernel(NibPrefil
 }
 
 // Joins the parts of 32 rows: out = sum_s w_s o_s / sum_s w_s l_s, w_s = 2^(m_s - max m). Its flag is
-// set by the attention launch and cleared here, so the flags are zero between calls.
+// set by the attention launch and cleared here, so the flags are zero between calls. A chain of round
+// trips to memory (flag, sums, parts), so parts are asked for B at a time, without a branch between them
+// (past one the compiler waits for all that is in flight), the first before the sums are there.
 template <int RW>
 __global__ __launch_bounds__(kNPJoinThreads) void nibble_join_kernel(NibPrefillArgs a) {
   constexpr int PIECES = RW / kNPJoinRows;
@@ -526,60 +528,69 @@ __global__ __launch_bounds__(kNPJoinThreads) void nibble_join_kernel(NibPrefillA
   const int r0 = piece * kNPJoinRows, nr = min(kNPJoinRows, J.nrow - r0);
   const int64_t first = J.part + r0;
   constexpr int UNITS = kNPJoinRows * kD / 4 / kNPJoinThreads;  // four floats each
-  auto load = [&](int u, int s) {
-    const int e = tid + u * kNPJoinThreads, row = min(e / (kD / 4), nr - 1);
-    return *gbl((const float4v*)(a.ws_o + (first + (int64_t)s * J.rows + row) * kD +
-                                 4 * (e % (kD / 4))));
-  };
-  constexpr int AHEAD = 2;  // parts in flight
-  float4v x[AHEAD][UNITS];
+  const int d = 4 * (tid % (kD / 4));
+  auto join = [&](auto b_c) {
+    constexpr int B = decltype(b_c)::value;
+    float4v x[B][UNITS], o[UNITS];
+    auto fetch = [&](int s0) {
 #pragma unroll
-  for (int k = 0; k < AHEAD; ++k)
-    if (k < J.ns)
+      for (int k = 0; k < B; ++k)
 #pragma unroll
-      for (int u = 0; u < UNITS; ++u) x[k][u] = load(u, k);
-  for (int e = tid; e < J.ns * kNPJoinRows; e += kNPJoinThreads) {
-    const int s = e / kNPJoinRows, row = min(e % kNPJoinRows, nr - 1);
-    wgt[s][e % kNPJoinRows] =
-        *gbl((const float2v*)(a.ws_ml + 2 * (first + (int64_t)s * J.rows + row)));
-  }
-  __syncthreads();
-  if (tid == 0) *flag = 0;
-  if (tid < kNPJoinRows) {
-    float mm = kNPNone, ll = 0.f;
-    for (int s = 0; s < J.ns; ++s) mm = fmaxf(mm, wgt[s][tid][0]);
-    for (int s = 0; s < J.ns; ++s) {
-      const float w = exp2f(wgt[s][tid][0] - mm);
-      ll += w * wgt[s][tid][1];
-      wgt[s][tid][0] = w;
+        for (int u = 0; u < UNITS; ++u) {
+          const int row = min((tid + u * kNPJoinThreads) / (kD / 4), nr - 1);
+          x[k][u] = *gbl((const float4v*)(
+              a.ws_o + (first + (int64_t)min(s0 + k, J.ns - 1) * J.rows + row) * kD + d));
+        }
+    };
+    fetch(0);
+    for (int e = tid; e < J.ns * kNPJoinRows; e += kNPJoinThreads) {
+      const int s = e / kNPJoinRows, row = min(e % kNPJoinRows, nr - 1);
+      wgt[s][e % kNPJoinRows] =
+          *gbl((const float2v*)(a.ws_ml + 2 * (first + (int64_t)s * J.rows + row)));
     }
-    inv_sh[tid] = 1.f / ll;
-  }
-  __syncthreads();
-  float4v o[UNITS];
+    __syncthreads();
+    if (tid == 0) *flag = 0;
+    if (tid < kNPJoinRows) {
+      float mm = kNPNone, ll = 0.f;
+#pragma unroll 8
+      for (int s = 0; s < J.ns; ++s) mm = fmaxf(mm, wgt[s][tid][0]);
+#pragma unroll 8
+      for (int s = 0; s < J.ns; ++s) {
+        const float2v ml = wgt[s][tid];
+        const float w = exp2f(ml[0] - mm);
+        ll += w * ml[1];
+        wgt[s][tid][0] = w;
+      }
+      inv_sh[tid] = 1.f / ll;
+    }
+    __syncthreads();
 #pragma unroll
-  for (int u = 0; u < UNITS; ++u) o[u] = float4v{};
-  for (int s = 0; s < J.ns; s += AHEAD) {
+    for (int u = 0; u < UNITS; ++u) o[u] = float4v{};
+    for (int s0 = 0; s0 < J.ns; s0 += B) {
+      if (s0) fetch(s0);
 #pragma unroll
-    for (int k = 0; k < AHEAD; ++k) {
-      if (s + k >= J.ns) break;
+      for (int k = 0; k < B; ++k) {
+        const int s = min(s0 + k, J.ns - 1);
 #pragma unroll
-      for (int u = 0; u < UNITS; ++u) {
-        o[u] += x[k][u] * wgt[s + k][(tid + u * kNPJoinThreads) / (kD / 4)][0];
-        if (s + k + AHEAD < J.ns) x[k][u] = load(u, s + k + AHEAD);
+        for (int u = 0; u < UNITS; ++u) {
+          const float w = wgt[s][(tid + u * kNPJoinThreads) / (kD / 4)][0];
+          o[u] += x[k][u] * (s0 + k < J.ns ? w : 0.f);
+        }
       }
     }
-  }
 #pragma unroll
-  for (int u = 0; u < UNITS; ++u) {
-    const int e = tid + u * kNPJoinThreads, row = e / (kD / 4);
-    if (row >= nr) break;
-    const int rr = J.row0 + r0 + row;
-    store_act4(a.out, a.out_dtype,
-               (J.q0 + rr / a.G) * a.out_row_stride + (int64_t)(J.h * a.G + rr % a.G) * kD +
-                   4 * (e % (kD / 4)),
-               o[u] * inv_sh[row], true);
-  }
+    for (int u = 0; u < UNITS; ++u) {
+      const int row = (tid + u * kNPJoinThreads) / (kD / 4);
+      if (row >= nr) break;
+      const int rr = J.row0 + r0 + row;
+      store_act4(a.out, a.out_dtype,
+                 (J.q0 + rr / a.G) * a.out_row_stride + (int64_t)(J.h * a.G + rr % a.G) * kD + d,
+                 o[u] * inv_sh[row], true);
+    }
+  };
+  if (J.ns == 2) join(std::integral_constant<int, 2>{});
+  else if (J.ns <= 4) join(std::integral_constant<int, 4>{});
+  else join(std::integral_constant<int, 8>{});
 }
 
 int nibble_check_read(int H, int HQ, int d, const void* q, int q_dtype,
@@ -600,6 +611,8 @@ int nibble_check_read(int H, int HQ, int d, const void* q, int q_dtype,
                                      "page's slots");
   if (n_slots / kNibTile > 0x7fffffff)
     return host_fail(TTKV_E_UNSUPPORTED, "more than 2^31 tiles of 16 slots");
+  if (max_seq > (1 << 26))
+    return host_fail(TTKV_E_UNSUPPORTED, "max_seq_len beyond 2^26");
   if (num_reqs < 0 || max_seq < 0 || max_blocks < 0)
     return host_fail(TTKV_E_INVALID, "negative count");
   if ((int64_t)max_blocks * bs < max_seq)
@@ -664,6 +677,8 @@ static int64_t np_join_bytes(const NibPrefillSlice& s) {
 
 int64_t nibble_prefill_workspace_bytes(int H, int HQ, int num_reqs, int max_q, int max_seq) {
   if (num_reqs == 0 || max_q == 0) return 256;
+  if (nibble_short_applies(H, HQ, max_q))
+    return nibble_short_workspace_bytes(H, HQ, num_reqs, max_q, max_seq);
   const NibPrefillSlice s = np_slice(H, HQ, num_reqs, max_q, max_seq);
   if (!s.split) return 256;
   return kCounterBytes + np_join_bytes(s) + np_part_rows(HQ, s.reqs, max_q, max_seq) * (kD + 2) * 4;
@@ -702,6 +717,10 @@ int nibble_prefill_paged(int H, int HQ, int d, float scale, const void* q, int q
     return host_fail(TTKV_E_WORKSPACE, "prefill workspace needs " + std::to_string(need) +
                                            " bytes, 256-aligned");
   if (num_reqs == 0 || max_q == 0) return TTKV_OK;
+  if (nibble_short_applies(H, HQ, max_q))
+    return nibble_decode_launch(H, HQ, scale, q, q_dtype, q_row_stride, page, n_slots, slot_stride,
+                                bs, bt, bt_row_stride, seq_lens, qsl, req_index, num_reqs, max_q,
+                                max_seq, out, out_dtype, out_row_stride, ws, err, st);
   const NibPrefillSlice s = np_slice(H, HQ, num_reqs, max_q, max_seq);
   const int64_t items = s.blocks + (s.split ? device_cu_count() + 8 : 0);
   if (items > 0x7fffffff) return host_fail(TTKV_E_INVALID, "too many queries for one call");
