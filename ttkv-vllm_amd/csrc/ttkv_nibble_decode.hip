@@ -2,10 +2,11 @@
 // chunks of queries. gfx950 / CDNA4.
 //
 // The rows of a (request, KV head) are its query heads, or (chunk) its (query, query head) pairs, row
-// = j G + p, 16 at most. Work item = (request, chunk of its 32-token steps, KV head), one workgroup of 4 waves that take the chunk's steps in turn. The chunk length comes from a plan
+// = j G + p. Work item = (request, block of 16 rows, chunk of the block's 32-token steps, KV head),
+// one workgroup of 4 waves that take the chunk's steps in turn. The chunk length comes from a plan
 // that every workgroup computes alike from the batch's lengths: the shortest that spreads the batch's
 // steps over the resident workgroups, so a ragged batch fills the chip by its total work. Items of a
-// (request, head) leave unnormalised partials in the workspace; the last to arrive joins them.
+// (block, head) leave unnormalised partials in the workspace; the last to arrive joins them.
 //
 // One step of a wave, two tiles of 16 tokens:
 //   S^T [token, row] = K Q^T, four v_mfma_f32_16x16x32_f16 per tile: a lane's 16 key code
@@ -30,9 +31,11 @@ constexpr int kNDThreads = 256;
 constexpr int kNDWaves = 4;
 constexpr int kNDStep = 2 * kNibTile;  // tokens per wave step
 constexpr int kNDPlanLanes = 4;        // requests per lane in the plan: 256 per launch
+constexpr int kNDShortRows = 256;      // rows of a chunk that may come here
+constexpr int64_t kNDShortWork = 130000;  // and steps of its blocks, times the blocks
 constexpr float kNDLazy = 8.f;         // log2 of the largest softmax weight before a rescale
 constexpr float kNDNone = -1e30f;      // a maximum before the first visible key
-constexpr int kNDRows = 16;            // rows per KV head: a matrix product's columns
+constexpr int kNDRows = 16;            // rows of a block: a matrix product's columns
 
 struct NibDecodeArgs {
   int H, G;
@@ -62,16 +65,16 @@ struct NibDecodeArgs {
 };
 
 struct NibDecodePlan {
-  int r, c, h;          // batch row, chunk, KV head
-  int n, Q, rows, nch;  // keys, queries, rows, chunks
-  int part, block;      // the request's first split item and its number, both before the head
+  int r, rb, c, h;      // batch row, row block, chunk, KV head
+  int n, Q, rows, nch;  // keys, queries, rows of all blocks, the block's chunks
+  int part, block;      // the block's first split item and its number, both before the head
   bool none;
 };
 
 template <bool CHUNK>
 __device__ __forceinline__ NibDecodePlan nd_plan(const NibDecodeArgs& a, int item) {
   const int lane = threadIdx.x & 63;
-  int idx[kNDPlanLanes], n[kNDPlanLanes], Q[kNDPlanLanes], st[kNDPlanLanes];
+  int idx[kNDPlanLanes], n[kNDPlanLanes], Q[kNDPlanLanes], st[kNDPlanLanes], rb[kNDPlanLanes];
   int total = 0;
 #pragma unroll
   for (int i = 0; i < kNDPlanLanes; ++i) {
@@ -86,8 +89,8 @@ __device__ __forceinline__ NibDecodePlan nd_plan(const NibDecodeArgs& a, int ite
     const int nn = min(max(n[i], 0), a.max_seq);
     st[i] = (nn + kNDStep - 1) / kNDStep;
     if (CHUNK && nn < Q[i]) st[i] = 1;
-    if (Q[i] <= 0) st[i] = 0;
-    total += st[i];
+    rb[i] = CHUNK ? (min(max(Q[i], 0), a.max_q) * a.G + kNDRows - 1) / kNDRows : Q[i];
+    total += st[i] * rb[i];
   }
   total = wave_sum_i(total);
   // whole rounds of the four waves
@@ -97,15 +100,16 @@ __device__ __forceinline__ NibDecodePlan nd_plan(const NibDecodeArgs& a, int ite
   NibDecodePlan P{};
   P.h = item % a.H;
   const int it = item / a.H;
-  int carry = 0, parts = 0;
+  int carry = 0, blocks = 0, parts = 0;
   P.none = true;
 #pragma unroll
   for (int i = 0; i < kNDPlanLanes; ++i) {
     if (64 * i >= a.num_reqs) break;
-    const int nch = Q[i] > 0 ? max(1, (st[i] + C - 1) / C) : 0, split = nch > 1 ? nch : 0;
-    const int incl = nib_scan(nch), ex = carry + incl - nch;
-    const int pincl = nib_scan(split);
-    const uint64_t hit = __builtin_amdgcn_ballot_w64(nch > 0 && ex <= it && it < ex + nch);
+    const int nch = max(1, (st[i] + C - 1) / C), items = rb[i] * nch;
+    const int split = nch > 1 ? items : 0;
+    const int incl = nib_scan(items), ex = carry + incl - items;
+    const int bincl = CHUNK ? nib_scan(rb[i]) : 0, pincl = nib_scan(split);
+    const uint64_t hit = __builtin_amdgcn_ballot_w64(items > 0 && ex <= it && it < ex + items);
     if (hit) {
       const int ln = __builtin_ctzll(hit);
       P.none = false;
@@ -113,13 +117,16 @@ __device__ __forceinline__ NibDecodePlan nd_plan(const NibDecodeArgs& a, int ite
       P.n = __builtin_amdgcn_readlane(n[i], ln);
       P.Q = __builtin_amdgcn_readlane(Q[i], ln);
       P.nch = __builtin_amdgcn_readlane(nch, ln);
-      P.c = it - __builtin_amdgcn_readlane(ex, ln);
+      const int local = it - __builtin_amdgcn_readlane(ex, ln);
+      P.rb = CHUNK ? local / P.nch : 0;
+      P.c = local - P.rb * P.nch;
       P.rows = CHUNK ? min(max(P.Q, 0), a.max_q) * a.G : a.G;
-      P.part = parts + __builtin_amdgcn_readlane(pincl - split, ln);
-      P.block = 64 * i + ln;
+      P.part = parts + __builtin_amdgcn_readlane(pincl - split, ln) + P.rb * P.nch;
+      P.block = CHUNK ? blocks + __builtin_amdgcn_readlane(bincl - rb[i], ln) + P.rb : 64 * i + ln;
     }
     carry += __builtin_amdgcn_readlane(incl, 63);
     parts += __builtin_amdgcn_readlane(pincl, 63);
+    if (CHUNK) blocks += __builtin_amdgcn_readlane(bincl, 63);
   }
   return P;
 }
@@ -144,14 +151,14 @@ __global__ __launch_bounds__(kNDThreads, 2) void nibble_decode_kernel(NibDecodeA
   const int h = P.h, G = a.G;
   const int n = min(max(P.n, 0), a.max_seq);
   const int p0 = CHUNK ? n - P.Q : n - 1;  // position of query 0
-  if (tid == 0 && h == 0 && P.c == 0 &&
+  if (tid == 0 && h == 0 && P.c == 0 && P.rb == 0 &&
       (P.n > a.max_seq || (CHUNK && (P.Q > a.max_q || p0 < 0))))
     atomicOr(a.err, TTKV_ERR_SEQ_LEN);
   const int64_t q0 = a.qsl[P.r];
-  const int nrow = P.rows;
-  // row `row` in the query and the output
-  auto row_at = [&](int row, int64_t stride) -> int64_t {
-    const int j = CHUNK ? row / G : 0;
+  const int row0 = P.rb * kNDRows, nrow = min(kNDRows, P.rows - row0);  // the block's rows
+  // row `r` of the block in the query and the output
+  auto row_at = [&](int r, int64_t stride) -> int64_t {
+    const int row = row0 + r, j = CHUNK ? row / G : 0;
     return (q0 + j) * stride + (int64_t)(h * G + row - j * G) * kD;
   };
   if (CHUNK ? p0 < 0 : n == 0) {  // fewer keys than queries; an empty request's attention is 0
@@ -166,13 +173,14 @@ __global__ __launch_bounds__(kNDThreads, 2) void nibble_decode_kernel(NibDecodeA
   float qs, m = kNDNone, l = 0.f;
   nib_load_query<QDT>(a.q + row_at(min(col, nrow - 1), a.q_row_stride), q4, a.scale_log2,
                       col < nrow, qf, qs);
-  const int lim = CHUNK ? p0 + min(col, nrow - 1) / G : p0;  // last key the lane's row sees
+  const int lim = CHUNK ? p0 + (row0 + min(col, nrow - 1)) / G : p0;  // last key the lane's row sees
+  const int see_min = CHUNK ? p0 + row0 / G : p0;                     // and every row
   float4v acc[8];  // [group][dim of the pair]: dims 32 g + 8 q4 + 2 i + b of the lane's row
 #pragma unroll
   for (int i = 0; i < 8; ++i) acc[i] = float4v{};
 
-  const int steps = (CHUNK ? p0 + (nrow - 1) / G : p0) / kNDStep + 1;
-  // the steps in equal parts
+  const int steps = (CHUNK ? p0 + (row0 + nrow - 1) / G : p0) / kNDStep + 1;
+  // the block's steps in equal parts
   const int s0 = (int)((int64_t)steps * P.c / P.nch);
   const int s1 = (int)((int64_t)steps * (P.c + 1) / P.nch);
   bool bad = false;
@@ -224,7 +232,7 @@ __global__ __launch_bounds__(kNDThreads, 2) void nibble_decode_kernel(NibDecodeA
     }
     const int tok = s * kNDStep + 4 * q4;
     uint32_t note = 0;  // bit 16 t + 4 i + g: that group of the lane's token is NaN
-    if ((s + 1) * kNDStep - 1 > p0) {
+    if ((s + 1) * kNDStep - 1 > see_min) {
       // Some row does not see all of this step: no score past its last key. A weight of 0 must not
       // meet a NaN: values past the last key become 0, and in a chunk a group that is NaN becomes 0
       // too and is noted for the rows that see it.
@@ -348,7 +356,7 @@ __global__ __launch_bounds__(kNDThreads, 2) void nibble_decode_kernel(NibDecodeA
   }
   __syncthreads();
   const int PR = a.part_rows;
-  const int64_t part = ((int64_t)P.part + P.c) * a.H + h;  // (where the request is split)
+  const int64_t part = ((int64_t)P.part + P.c) * a.H + h;  // (where the block is split)
   for (int e = 4 * tid; e < nrow * kD; e += 4 * kNDThreads) {
     const int p = e / kD, d = e % kD;
     float mm = kNDNone, ll = 0.f;
@@ -368,7 +376,7 @@ __global__ __launch_bounds__(kNDThreads, 2) void nibble_decode_kernel(NibDecodeA
   }
   if (P.nch == 1) return;
 
-  // ---- the last workgroup of a (request, head) joins its chunks' partials
+  // ---- the last workgroup of a (block, head) joins its chunks' partials
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   __syncthreads();
   if (tid == 0) {
@@ -452,38 +460,48 @@ __global__ __launch_bounds__(kNDThreads, 2) void nibble_decode_kernel(NibDecodeA
 // at four; 61 requests of 70 to 2,900: 33.4, 35.0, 34.6).
 static int nd_target() { return 2 * device_cu_count(); }
 
-// Requests per launch: the plan's lanes, and a counter per (request, head).
-static int nd_slice(int H, int num_reqs) {
-  return std::max(1, std::min({num_reqs, kNDPlanLanes * 64, kMaxCounters / H}));
+// Requests per launch, of `blocks` row blocks each: the plan's lanes, and a counter per (block, head).
+static int nd_slice(int H, int blocks, int num_reqs) {
+  return std::max(1, std::min({num_reqs, kNDPlanLanes * 64, kMaxCounters / (H * blocks)}));
 }
 
-// Chunks of a request at most: whole rounds of the four waves.
+// Chunks of a block at most: whole rounds of the four waves.
 static int64_t nd_max_chunks(int max_seq) {
   const int64_t round = kNDStep * kNDWaves;
   return std::max<int64_t>(1, (max_seq + round - 1) / round);
 }
 
-// Items of split requests, at most. A chunk has at least total / target steps, and a split request of
-// st steps has less than st / C + 1 < 2 st / C chunks: less than 2 target of them in all.
-static int64_t nd_parts(int H, int nr, int max_seq) {
+// Items of split blocks, at most, of `pairs` (block, head) pairs. A chunk has at least total / target
+// steps, and a split block of st steps has less than st / C + 1 < 2 st / C chunks: less than 2 target of
+// them in all.
+static int64_t nd_parts(int64_t pairs, int max_seq) {
   const int64_t most = nd_max_chunks(max_seq);
-  return most <= 1 ? 0 : std::min<int64_t>(2 * nd_target(), (int64_t)nr * H * most);
+  return most <= 1 ? 0 : std::min<int64_t>(2 * nd_target(), pairs * most);
 }
+
+static int nd_blocks(int rows) { return (rows + kNDRows - 1) / kNDRows; }
 
 static int64_t nd_workspace(int H, int num_reqs, int max_seq, int rows) {
   if (num_reqs == 0 || H > kMaxCounters) return 256;
-  return kCounterBytes + nd_parts(H, nd_slice(H, num_reqs), max_seq) * rows * (kD + 2) * 4;
+  const int64_t pairs = (int64_t)nd_slice(H, nd_blocks(rows), num_reqs) * H * nd_blocks(rows);
+  return kCounterBytes + nd_parts(pairs, max_seq) * std::min(rows, kNDRows) * (kD + 2) * 4;
 }
 
 int64_t nibble_decode_workspace_bytes(int H, int HQ, int num_reqs, int max_seq) {
   return nd_workspace(H, num_reqs, max_seq, HQ / H);
 }
 
-// Chunks of at most 16 rows take this kernel: it reads every key for 16 rows, the prefill kernel for 128,
-// but without tiles in LDS or a second launch (3 chunks of 4 queries and 4 heads per KV head over
-// 3,000 keys: 16.2 us here, 19.6 there; of 8, in two groups of rows here: 24.3 and 22.2).
-bool nibble_short_applies(int H, int HQ, int max_q) {
-  return (int64_t)max_q * (HQ / H) <= kNDRows && H <= kMaxCounters;
+// Chunks of at most 16 rows take this kernel, and short ones while the whole call is short: it reads
+// and dequantises a key for 16 rows, the prefill kernel for 128 to 384, but it has no tiles in LDS, no
+// second launch and a smaller join. Both measured at four query heads and eight KV heads, here and
+// there: 1 x 64 queries over 500 keys 14.8 and 23.7 us, 1 x 32 over 4,000 19.4 and 25.7, 3 x 16 over
+// 3,000 20.3 and 24.0, 16 x 8 over 6,000 51.3 and 65.6; 8 x 16 over 3,000 32.0 and 30.6, 3 x 32 over
+// 3,000 34.0 and 28.8, 8 x 32 over 3,000 48.2 and 38.0. The limit on steps times blocks parts these.
+bool nibble_short_applies(int H, int HQ, int num_reqs, int max_q, int max_seq) {
+  const int64_t rows = (int64_t)max_q * (HQ / H);
+  if (rows > kNDShortRows || H * nd_blocks((int)rows) > kMaxCounters) return false;
+  const int64_t blocks = nd_blocks((int)rows), steps = (max_seq + kNDStep - 1) / kNDStep;
+  return blocks == 1 || num_reqs * H * steps * blocks * blocks <= kNDShortWork;
 }
 
 int64_t nibble_short_workspace_bytes(int H, int HQ, int num_reqs, int max_q, int max_seq) {
@@ -511,8 +529,9 @@ int nibble_decode_launch(int H, int HQ, float scale, const void* q, int q_dtype,
                          const int32_t* seq_lens, const int32_t* qsl, const int32_t* req_index,
                          int num_reqs, int max_q, int max_seq, void* out, int out_dtype,
                          int64_t out_row_stride, void* ws, int32_t* err, hipStream_t st) {
-  const int slice = nd_slice(H, num_reqs);
-  const int64_t parts = nd_parts(H, slice, max_seq);
+  const int rows = HQ / H * std::max(max_q, 1), blocks = nd_blocks(rows);
+  const int slice = nd_slice(H, blocks, num_reqs);
+  const int64_t parts = nd_parts((int64_t)slice * H * blocks, max_seq);
   NibDecodeArgs a{};
   a.H = H;
   a.G = HQ / H;
@@ -532,7 +551,7 @@ int nibble_decode_launch(int H, int HQ, float scale, const void* q, int q_dtype,
   a.out = out;
   a.out_dtype = out_dtype;
   a.out_row_stride = out_row_stride;
-  a.part_rows = a.G * std::max(max_q, 1);
+  a.part_rows = std::min(rows, kNDRows);
   a.ws_cnt = (int*)ws;
   a.ws_o = (float*)((char*)ws + kCounterBytes);
   a.ws_ml = a.ws_o + parts * a.part_rows * kD;
@@ -548,8 +567,8 @@ int nibble_decode_launch(int H, int HQ, float scale, const void* q, int q_dtype,
       a.qsl = qsl + r0;
       a.bt = bt + (int64_t)r0 * bt_row_stride;
     }
-    // an item per (request, head), and what the split ones have more
-    const int64_t pairs = (int64_t)a.num_reqs * H;
+    // an item per (block, head), and what the split ones have more
+    const int64_t pairs = (int64_t)a.num_reqs * H * blocks;
     const unsigned grid = (unsigned)std::min(pairs + nd_target(), pairs * nd_max_chunks(max_seq));
     const int rc = max_q > 0 ? nd_launch<true>(a, grid, q_dtype, st)
                              : nd_launch<false>(a, grid, q_dtype, st);

@@ -677,7 +677,7 @@ static int64_t np_join_bytes(const NibPrefillSlice& s) {
 
 int64_t nibble_prefill_workspace_bytes(int H, int HQ, int num_reqs, int max_q, int max_seq) {
   if (num_reqs == 0 || max_q == 0) return 256;
-  if (nibble_short_applies(H, HQ, max_q))
+  if (nibble_short_applies(H, HQ, num_reqs, max_q, max_seq))
     return nibble_short_workspace_bytes(H, HQ, num_reqs, max_q, max_seq);
   const NibPrefillSlice s = np_slice(H, HQ, num_reqs, max_q, max_seq);
   if (!s.split) return 256;
@@ -717,7 +717,7 @@ int nibble_prefill_paged(int H, int HQ, int d, float scale, const void* q, int q
     return host_fail(TTKV_E_WORKSPACE, "prefill workspace needs " + std::to_string(need) +
                                            " bytes, 256-aligned");
   if (num_reqs == 0 || max_q == 0) return TTKV_OK;
-  if (nibble_short_applies(H, HQ, max_q))
+  if (nibble_short_applies(H, HQ, num_reqs, max_q, max_seq))
     return nibble_decode_launch(H, HQ, scale, q, q_dtype, q_row_stride, page, n_slots, slot_stride,
                                 bs, bt, bt_row_stride, seq_lens, qsl, req_index, num_reqs, max_q,
                                 max_seq, out, out_dtype, out_row_stride, ws, err, st);
