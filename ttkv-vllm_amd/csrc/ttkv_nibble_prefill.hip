@@ -33,7 +33,8 @@ constexpr int kNPWaves = 8;
 constexpr int kNPTile = 64;        // keys per tile
 constexpr int kNPPlanLanes = 4;    // requests per lane in the plan: 256 per launch
 constexpr int kNPMaxSplit = 32;
-constexpr int kNPMinTiles = 4;     // keys per part, in tiles
+constexpr int kNPMinTiles = 4;     // keys per part, in tiles (batches that are not searched)
+constexpr int kNPSearch = 16;      // requests up to which the plan searches for the number of parts
 constexpr float kNPLazy = 8.f;     // log2 of the largest softmax weight before a rescale
 constexpr float kNPNone = -1e30f;  // a maximum before the first visible key
 constexpr int64_t kNPPartRows = 128000;  // rows of partial results a launch may leave: 66.6 MB
@@ -62,7 +63,7 @@ struct NibPrefillArgs {
   float* ws_o;   // [part rows][kD]
   float* ws_ml;  // [part rows][2]
   int64_t part_rows;
-  int target;
+  int target, grid;
   int32_t* err;
 };
 
@@ -83,17 +84,48 @@ struct NibPrefillPlan {
   bool none;
 };
 
+// Parts of a request's tiles, C of them each but for rounding (a reciprocal: near a whole quotient it may
+// be one off, alike for every workgroup, and the parts are cut equal from their number; 1 for C >= tiles).
 __device__ __forceinline__ int np_parts(int tiles, int C) {
-  return min((tiles + C - 1) / C, kNPMaxSplit);
+  return min(max(1, (int)((float)(tiles + C - 1) * __builtin_amdgcn_rcpf((float)C))), kNPMaxSplit);
 }
 
-// Parts of at least C tiles: the shortest that spread the batch's tiles over the target's workgroups
-// and whose partial results fit the workspace.
+// Tiles per part of `parts` parts of T tiles, rounded up or one more.
+__device__ __forceinline__ int np_each(int T, int parts) {
+  return max(1, (int)((float)T * __builtin_amdgcn_rcpf((float)parts) + 0.999f));
+}
+
+// An estimate of a launch's time in us, from what these kernels measured: a tile of a row block takes
+// 2.0, 2.3 and 3.4 us with one, two and three groups of rows per wave (8 x 384 rows over 6,000 and
+// 12,000 keys) and a block 5 us beside its tiles (4 x 1,432 rows over 180 keys, 8 heads); the items, of
+// `load` tiles in all, take whole rounds of the CUs, and no less than the longest; a split costs its join
+// and, per partial row, 520 bytes written and read.
+__host__ __device__ inline float np_cost(int ng, float longest, float load, float items, float cus,
+                                         float need) {
+  const float tile = ng == 1 ? 2.0f : ng == 2 ? 2.3f : 3.4f;
+#ifdef __HIP_DEVICE_COMPILE__
+  const float rounds = ceilf(items * __builtin_amdgcn_rcpf(cus)), each = load * __builtin_amdgcn_rcpf(items);
+#else
+  const float rounds = ceilf(items / cus), each = load / items;
+#endif
+  return 5.f * rounds + tile * fmaxf(longest, rounds * each) + (need > 0.f ? 5.f + 1.5e-4f * need : 0.f);
+}
+// Tiles that a row block of a chunk of Q queries over T tiles has on average.
+__host__ __device__ inline float np_mean_tiles(int T, int Q) {
+  const float less = (float)Q / (2 * kNPTile);
+  return (float)T - (less < 0.5f * T ? less : 0.5f * T);
+}
+
+// Parts of at least C tiles. For few requests every number of parts of the longest one, from 1 to 32, is
+// priced, one per lane; many requests have row blocks enough, and get the shortest parts that spread
+// their tiles over the target's workgroups. Either way the partial results have to fit the workspace,
+// and the items the grid.
 template <int RW>
 __device__ __forceinline__ NibPrefillPlan np_plan(const NibPrefillArgs& a, int item) {
+  constexpr int NG = RW / (16 * kNPWaves);
   const int lane = threadIdx.x & 63;
   int idx[kNPPlanLanes], n[kNPPlanLanes], Q[kNPPlanLanes], rows[kNPPlanLanes], tiles[kNPPlanLanes];
-  float work = 0.f;
+  float work = 0.f;  // tiles of all row blocks
 #pragma unroll
   for (int i = 0; i < kNPPlanLanes; ++i) {
     const int r = lane + 64 * i;
@@ -104,10 +136,32 @@ __device__ __forceinline__ NibPrefillPlan np_plan(const NibPrefillArgs& a, int i
     const int nn = min(max(n[i], 0), a.max_seq);
     rows[i] = min(max(Q[i], 0), a.max_q) * a.G;
     tiles[i] = nn < Q[i] ? 1 : (nn + kNPTile - 1) / kNPTile;
-    work += (float)((rows[i] + RW - 1) / RW) * (float)tiles[i];
+    work += (float)((rows[i] + RW - 1) / RW) * np_mean_tiles(tiles[i], Q[i]);
   }
   work = wave_sum(work) * (float)a.H;
-  int C = max(kNPMinTiles, (int)ceilf(work / (float)a.target));
+  int C;
+  if (a.num_reqs <= kNPSearch) {
+    const int most = wave_max_i(rows[0] > 0 ? tiles[0] : 1);
+    const int parts = (lane & (kNPMaxSplit - 1)) + 1, c = np_each(most, parts);
+    float longest = 0.f, items = 0.f, need = 0.f;
+    for (int r = 0; r < a.num_reqs; ++r) {
+      const int T = __builtin_amdgcn_readlane(tiles[0], r), rw = __builtin_amdgcn_readlane(rows[0], r);
+      if (rw <= 0) continue;
+      const int ns = np_parts(T, c);
+      longest = fmaxf(longest, (float)T * __builtin_amdgcn_rcpf((float)ns));
+      items += (float)((rw + RW - 1) / RW * ns);
+      need += ns > 1 ? (float)rw * (float)ns : 0.f;
+    }
+    items *= (float)a.H;
+    need *= (float)a.H;
+    const bool fits = need <= (float)a.part_rows && items <= (float)a.grid;  // (one part always does)
+    const float us = np_cost(NG, longest, work, fmaxf(items, 1.f), (float)a.target, need);
+    const int price = fits ? (int)fminf(us * 16.f, 3e7f) : 0x3ffffff;  // sixteenths
+    const int best = -wave_max_i(-(price * 32 + parts - 1)) & 31;
+    C = np_each(most, best + 1);
+  } else {
+    C = max(kNPMinTiles, (int)ceilf(work / (float)a.target));
+  }
   while (true) {
     float need = 0.f;
 #pragma unroll
@@ -624,23 +678,6 @@ int nibble_check_read(int H, int HQ, int d, const void* q, int q_dtype,
   return TTKV_OK;
 }
 
-// Groups of 16 rows per wave for chunks of at most `rows` rows: a wave's key and value fragments
-// serve all of its groups, so three are the fastest per row, unless fewer leave less of a block empty.
-static int np_groups(int64_t rows) {
-  static const double cost[] = {0, 1.6, 1.15, 1.0};  // per row held
-  int best = 3;
-  double least = 0;
-  for (int ng = 3; ng >= 1; --ng) {
-    const int64_t rw = kNPWaves * 16 * ng;
-    const double c = (double)((rows + rw - 1) / rw * rw) * cost[ng];
-    if (ng == 3 || c < least) {
-      best = ng;
-      least = c;
-    }
-  }
-  return best;
-}
-
 // Requests per launch: the plan's lanes and a flag per 32 rows of every row block and head; with no
 // room for one request's flags, its keys are not split.
 struct NibPrefillSlice {
@@ -651,20 +688,38 @@ struct NibPrefillSlice {
 // Parts of a request at most.
 static int64_t np_max_parts(int max_seq) {
   const int64_t tiles = (max_seq + kNPTile - 1) / kNPTile;
-  return std::min<int64_t>(kNPMaxSplit, (tiles + kNPMinTiles - 1) / kNPMinTiles);
+  return std::min<int64_t>(kNPMaxSplit, tiles);
 }
 
 static NibPrefillSlice np_slice(int H, int HQ, int num_reqs, int max_q, int max_seq) {
-  NibPrefillSlice s{};
-  s.ng = np_groups((int64_t)max_q * (HQ / H));
-  const int64_t rw = kNPWaves * 16 * s.ng;
-  const int64_t per = ((int64_t)max_q * (HQ / H) + rw - 1) / rw * H;  // row blocks of one request
-  const int64_t flags = kCounterBytes / (rw / kNPJoinRows);  // row blocks the flags serve
-  s.split = per <= flags && np_max_parts(max_seq) > 1;
-  s.reqs = std::min(num_reqs, kNPPlanLanes * 64);
-  if (s.split) s.reqs = (int)std::min<int64_t>(s.reqs, flags / per);
-  s.blocks = per * s.reqs;
-  return s;
+  const int64_t rows = (int64_t)max_q * (HQ / H), cus = device_cu_count();
+  const int T = (max_seq + kNPTile - 1) / kNPTile;
+  NibPrefillSlice best{};
+  float least = 0.f;
+  for (int ng = 3; ng >= 1; --ng) {
+    NibPrefillSlice s{};
+    s.ng = ng;
+    const int64_t rw = kNPWaves * 16 * ng;
+    const int64_t per = (rows + rw - 1) / rw * H;              // row blocks of one request
+    const int64_t flags = kCounterBytes / (rw / kNPJoinRows);  // row blocks the flags serve
+    s.split = per <= flags && np_max_parts(max_seq) > 1;
+    s.reqs = std::min(num_reqs, kNPPlanLanes * 64);
+    if (s.split) s.reqs = (int)std::min<int64_t>(s.reqs, flags / per);
+    s.blocks = per * s.reqs;
+    // the plan's search with every request at its longest
+    const float load = (float)(per * num_reqs) * np_mean_tiles(T, max_q);
+    for (int k = 1; k <= (s.split ? np_max_parts(max_seq) : 1); ++k) {
+      const int64_t need = k > 1 ? rows * H * num_reqs * k : 0;
+      if (k > 1 && (need > kNPPartRows || per * num_reqs * (k - 1) > cus)) break;
+      const float us = np_cost(ng, (float)((T + k - 1) / k), load, (float)(per * num_reqs * k), (float)cus,
+                               (float)need);
+      if (best.ng == 0 || us < least) {
+        best = s;
+        least = us;
+      }
+    }
+  }
+  return best;
 }
 
 static int64_t np_part_rows(int HQ, int reqs, int max_q, int max_seq) {
@@ -722,7 +777,8 @@ int nibble_prefill_paged(int H, int HQ, int d, float scale, const void* q, int q
                                 bs, bt, bt_row_stride, seq_lens, qsl, req_index, num_reqs, max_q,
                                 max_seq, out, out_dtype, out_row_stride, ws, err, st);
   const NibPrefillSlice s = np_slice(H, HQ, num_reqs, max_q, max_seq);
-  const int64_t items = s.blocks + (s.split ? device_cu_count() + 8 : 0);
+  const int64_t items =
+      s.split ? std::min(s.blocks + device_cu_count() + 8, s.blocks * np_max_parts(max_seq)) : s.blocks;
   if (items > 0x7fffffff) return host_fail(TTKV_E_INVALID, "too many queries for one call");
   NibPrefillArgs a{};
   a.H = H;
@@ -749,6 +805,7 @@ int nibble_prefill_paged(int H, int HQ, int d, float scale, const void* q, int q
   a.ws_o = (float*)((char*)ws + kCounterBytes + np_join_bytes(s));
   a.ws_ml = a.ws_o + a.part_rows * kD;
   a.target = device_cu_count();  // a workgroup fills a CU
+  a.grid = (int)items;
   a.err = err;
   for (int r0 = 0; r0 < num_reqs; r0 += s.reqs) {
     a.num_reqs = std::min(s.reqs, num_reqs - r0);
