@@ -491,6 +491,24 @@ def test_prefill_many_requests_and_long_splits():
         _close(out, q, *st.kv(0), SCALE, Q)
 
 
+@pytest.mark.parametrize("H,HQ,lens,counts", [
+    (2, 2, [700] * 17, [700] * 17), (1, 2, [1500] * 18, [1500] * 18), (2, 2, [2001] * 20, [900] * 20),
+    (1, 2, [5000] + [70] * 15, [300] + [70] * 15), (1, 2, [5000] + [70] * 39, [300] + [70] * 39),
+    (2, 4, [64, 65] * 8, [64, 63] * 8), (1, 4, [9000], [130])])
+def test_prefill_batches_write_every_row(H, HQ, lens, counts):
+    """Prompts of many row blocks each, and one long among short: every row is written, by whatever
+    rows per block and key parts the plan takes."""
+    st = Store(lens, H, seed=20)
+    q = torch.randn(sum(counts), HQ, D, generator=_gen(21)).half()
+    out = torch.full((sum(counts), HQ, D), float("nan"), dtype=torch.float16, device="cuda")
+    _, err, qsl = _prefill(st, q.cuda(), counts, out=out)
+    assert err == 0
+    assert not bool(torch.isnan(out).any())
+    for r in (0, len(lens) // 2, len(lens) - 1):
+        s = slice(qsl[r], qsl[r + 1])
+        _close(out[s], q[s], *st.kv(r), SCALE, r)
+
+
 def test_prefill_workspace_serves_other_shapes():
     """One workspace for prefill calls of different shapes and for decode calls in turn."""
     shapes = [([5000, 300], 2, 8, [70, 20]), ([900, 64, 30], 1, 4, [3, 1, 2]), ([1200], 4, 12, [400])]

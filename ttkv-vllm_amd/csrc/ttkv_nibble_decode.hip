@@ -501,7 +501,7 @@ bool nibble_short_applies(int H, int HQ, int num_reqs, int max_q, int max_seq) {
   const int64_t rows = (int64_t)max_q * (HQ / H);
   if (rows > kNDShortRows || H * nd_blocks((int)rows) > kMaxCounters) return false;
   const int64_t blocks = nd_blocks((int)rows), steps = (max_seq + kNDStep - 1) / kNDStep;
-  return blocks == 1 || num_reqs * H * steps * blocks * blocks <= kNDShortWork;
+  return blocks == 1 || (int64_t)num_reqs * H * steps * blocks * blocks <= kNDShortWork;
 }
 
 int64_t nibble_short_workspace_bytes(int H, int HQ, int num_reqs, int max_q, int max_seq) {

@@ -125,7 +125,7 @@ __device__ __forceinline__ NibPrefillPlan np_plan(const NibPrefillArgs& a, int i
   constexpr int NG = RW / (16 * kNPWaves);
   const int lane = threadIdx.x & 63;
   int idx[kNPPlanLanes], n[kNPPlanLanes], Q[kNPPlanLanes], rows[kNPPlanLanes], tiles[kNPPlanLanes];
-  float work = 0.f;  // tiles of all row blocks
+  float work = 0.f, most_work = 0.f;  // tiles of all row blocks: that they see, and of their requests
 #pragma unroll
   for (int i = 0; i < kNPPlanLanes; ++i) {
     const int r = lane + 64 * i;
@@ -137,6 +137,7 @@ __device__ __forceinline__ NibPrefillPlan np_plan(const NibPrefillArgs& a, int i
     rows[i] = min(max(Q[i], 0), a.max_q) * a.G;
     tiles[i] = nn < Q[i] ? 1 : (nn + kNPTile - 1) / kNPTile;
     work += (float)((rows[i] + RW - 1) / RW) * np_mean_tiles(tiles[i], Q[i]);
+    most_work += (float)((rows[i] + RW - 1) / RW) * (float)tiles[i];
   }
   work = wave_sum(work) * (float)a.H;
   int C;
@@ -160,7 +161,8 @@ __device__ __forceinline__ NibPrefillPlan np_plan(const NibPrefillArgs& a, int i
     const int best = -wave_max_i(-(price * 32 + parts - 1)) & 31;
     C = np_each(most, best + 1);
   } else {
-    C = max(kNPMinTiles, (int)ceilf(work / (float)a.target));
+    // at most work / C items beside one per row block: within the grid
+    C = max(kNPMinTiles, (int)ceilf(wave_sum(most_work) * (float)a.H / (float)a.target));
   }
   while (true) {
     float need = 0.f;
