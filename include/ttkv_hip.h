@@ -394,8 +394,14 @@ int ttkv_nibble_write_paged(int32_t H, int32_t d, const void* key, int32_t k_dty
  * as for ttkv_decode_paged, query and out fp16 or bf16, up to 16 query heads per KV head.
  *   out[p] = sum_t softmax_t(scale * q[p] . K[t]) * V[t],  t < seq_lens[r]
  * An empty request's rows are 0. A block id outside the cache sets TTKV_ERR_BAD_BLOCK and makes its
- * request's rows NaN. Keys and values enter the products exactly; the query is taken as fp16, and
- * the softmax weight is rounded to fp16 once. */
+ * request's rows NaN. Keys and values enter the products exactly; the query is taken as fp16 (bf16
+ * at a power of two per row), and the softmax weight is rounded to fp16 once. `out` may be the query.
+ * max_seq_len at most 2^26 and at most the tokens that max_blocks hold; the page at most 2^31 tiles.
+ *
+ * Workspace, of this call and the next: 256-byte aligned, its first 64 KiB zero before its first call
+ * and left zero by every call. Its size grows with every argument, so one buffer for the largest batch
+ * serves the others, and one of the larger size serves both calls, in stream order; calls that may
+ * overlap take one each. Results do not depend on what it held, and repeat bit for bit. */
 int64_t ttkv_nibble_decode_workspace_bytes(int32_t H, int32_t num_heads, int32_t num_reqs,
                                            int32_t max_seq_len);
 int ttkv_nibble_decode_paged(int32_t H, int32_t num_heads, int32_t d, float scale,
@@ -411,7 +417,9 @@ int ttkv_nibble_decode_paged(int32_t H, int32_t num_heads, int32_t d, float scal
 /* Causal attention of chunks of queries over the 4-bit cache: request r's Q queries sit at the end
  * of its n = seq_lens[r] stored keys (their own included; a first chunk has n = Q), query j sees
  * keys t <= n - Q + j. Arguments as for ttkv_prefill_paged, limits and precision as above. A request
- * with n < Q sets TTKV_ERR_SEQ_LEN and its rows become NaN. */
+ * with n < Q sets TTKV_ERR_SEQ_LEN and its rows become NaN; one with Q > max_q_len or n > max_seq_len
+ * sets it and has its first max_q_len queries, or its first max_seq_len keys, taken. Of a request with
+ * a block id outside the cache, the rows that see the block become NaN, and others of it may. */
 int64_t ttkv_nibble_prefill_workspace_bytes(int32_t H, int32_t num_heads, int32_t num_reqs,
                                             int32_t max_q_len, int32_t max_seq_len);
 int ttkv_nibble_prefill_paged(int32_t H, int32_t num_heads, int32_t d, float scale,

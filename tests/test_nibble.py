@@ -190,6 +190,24 @@ def test_workspace_sizes():
     assert 0 < small <= L.ttkv_nibble_decode_workspace_bytes(8, 24, 64, 16000)
 
 
+def test_a_workspace_for_the_largest_batch_serves_smaller_ones():
+    L, g = _hip.lib(), torch.Generator().manual_seed(3)
+
+    def draw(most):
+        return int(2 ** (float(torch.rand(1, generator=g)) * most))
+
+    for _ in range(300):
+        H, G = draw(4), min(draw(5), 16)
+        R, q, n = draw(9), draw(12), draw(15)
+        q = min(q, n)
+        r2, q2, n2 = R + draw(4) - 1, q + draw(8) - 1, n + draw(13)
+        assert L.ttkv_nibble_decode_workspace_bytes(H, H * G, R, n) \
+            <= L.ttkv_nibble_decode_workspace_bytes(H, H * G, r2, n2)
+        a = L.ttkv_nibble_prefill_workspace_bytes(H, H * G, R, q, n)
+        assert 256 <= a <= L.ttkv_nibble_prefill_workspace_bytes(H, H * G, r2, q2, max(n2, q2))
+        assert a <= 64 << 20
+
+
 def _rotary(sections=(16, 24, 24), **kw):
     a = dict(q=16, k=16, qo=16, ko=16, dt=1, N=4, HQ=24, H=8, d=128, qs=24 * 128, ks=1024,
              qos=24 * 128, kos=1024, pos=16, ps=4, axes=len(sections),
@@ -234,6 +252,10 @@ def test_plan_refusals():
     _refused(_plan(free=0), 1, "null")
     _refused(_plan(slots=0), 1, "null")
     _refused(_plan(used=0), 1, "null")
+    out = dict(qsl=32, seq=48, used=64)
+    for name in out:
+        for at in ("c", "n"):
+            _refused(_plan(**{**out, "c": 80, "n": 96, at: out[name]}), 1, "length inputs")
 
 
 # --------------------------------------------------------------------------- wrapper refusals

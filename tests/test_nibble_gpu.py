@@ -532,6 +532,22 @@ def test_prefill_workspace_serves_other_shapes():
             _close(out[r:r + 1], dq[r:r + 1].cpu(), *st.kv(r), SCALE, r)
 
 
+@pytest.mark.parametrize("lens,counts", [([300, 5000], [300, 40]), ([5000, 90], [9, 3]),
+                                         ([700], [128]), ([20000, 1], [1, 1])])
+def test_the_output_may_be_the_query(lens, counts):
+    st = Store(lens, 2, seed=30)
+    q = torch.randn(sum(counts), 8, D, generator=_gen(31)).half()
+    want, err, qsl = _prefill(st, q.cuda(), counts)
+    got = q.cuda()
+    _prefill(st, got, counts, out=got)
+    assert err == 0 and torch.equal(got, want)
+    if counts == [1] * len(counts):
+        want, _ = _decode(st, q.cuda())
+        got = q.cuda()
+        _decode(st, got, out=got)
+        assert torch.equal(got, want)
+
+
 def test_prefill_and_decode_agree_on_one_query():
     st = Store([777, 20], 2, seed=13)
     q = torch.randn(2, 8, D, generator=_gen(13)).half()

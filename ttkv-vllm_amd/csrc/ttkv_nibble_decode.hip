@@ -504,8 +504,11 @@ bool nibble_short_applies(int H, int HQ, int num_reqs, int max_q, int max_seq) {
   return blocks == 1 || (int64_t)num_reqs * H * steps * blocks * blocks <= kNDShortWork;
 }
 
-int64_t nibble_short_workspace_bytes(int H, int HQ, int num_reqs, int max_q, int max_seq) {
-  return nd_workspace(H, num_reqs, max_seq, max_q * (HQ / H));
+// Bytes of partial results of such a chunk call at most, growing with every argument.
+int64_t nibble_short_part_bytes(int H, int HQ, int num_reqs, int max_q, int max_seq) {
+  const int rows = (int)std::min<int64_t>((int64_t)max_q * (HQ / H), kNDShortRows);
+  const int64_t pairs = std::min<int64_t>((int64_t)num_reqs * H * nd_blocks(rows), kMaxCounters);
+  return nd_parts(pairs, max_seq) * std::min(rows, kNDRows) * (kD + 2) * 4;
 }
 
 template <bool CHUNK>

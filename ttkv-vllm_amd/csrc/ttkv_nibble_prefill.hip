@@ -37,7 +37,7 @@ constexpr int kNPMinTiles = 4;     // keys per part, in tiles (batches that are 
 constexpr int kNPSearch = 16;      // requests up to which the plan searches for the number of parts
 constexpr float kNPLazy = 8.f;     // log2 of the largest softmax weight before a rescale
 constexpr float kNPNone = -1e30f;  // a maximum before the first visible key
-constexpr int64_t kNPPartRows = 128000;  // rows of partial results a launch may leave: 66.6 MB
+constexpr int64_t kNPPartRows = 127000;  // rows of partial results a launch may leave: 66.0 MB
 constexpr int kNPKBytes = kNPTile * kD * 2;
 constexpr int kNPSmem = 4 * kNPKBytes;  // two buffers of keys and values
 
@@ -725,20 +725,24 @@ static NibPrefillSlice np_slice(int H, int HQ, int num_reqs, int max_q, int max_
 }
 
 static int64_t np_part_rows(int HQ, int reqs, int max_q, int max_seq) {
-  return std::min(kNPPartRows, np_max_parts(max_seq) * reqs * max_q * HQ);
+  return std::min(kNPPartRows, np_max_parts(max_seq) * reqs * std::min<int64_t>(max_q, kNPPartRows) * HQ);
 }
 
 static int64_t np_join_bytes(const NibPrefillSlice& s) {
   return (s.blocks * (int64_t)sizeof(NibPrefillJoin) + 255) / 256 * 256;
 }
 
+// An upper bound that grows with every argument, so that a workspace for the largest batch serves the
+// others: a join record for every row block that the flags can serve, of 128 rows each, and the parts of
+// either kernel.
 int64_t nibble_prefill_workspace_bytes(int H, int HQ, int num_reqs, int max_q, int max_seq) {
   if (num_reqs == 0 || max_q == 0) return 256;
-  if (nibble_short_applies(H, HQ, num_reqs, max_q, max_seq))
-    return nibble_short_workspace_bytes(H, HQ, num_reqs, max_q, max_seq);
-  const NibPrefillSlice s = np_slice(H, HQ, num_reqs, max_q, max_seq);
-  if (!s.split) return 256;
-  return kCounterBytes + np_join_bytes(s) + np_part_rows(HQ, s.reqs, max_q, max_seq) * (kD + 2) * 4;
+  const int64_t rows = (int64_t)max_q * (HQ / H), rw = kNPWaves * 16;
+  const int64_t blocks = std::min<int64_t>(kCounterBytes / (rw / kNPJoinRows),
+                                           std::min<int64_t>((rows + rw - 1) / rw, kCounterBytes) * H * num_reqs);
+  const int64_t joins = (blocks * (int64_t)sizeof(NibPrefillJoin) + 255) / 256 * 256;
+  const int64_t parts = np_part_rows(HQ, num_reqs, max_q, max_seq) * (kD + 2) * 4;
+  return kCounterBytes + std::max(joins + parts, nibble_short_part_bytes(H, HQ, num_reqs, max_q, max_seq));
 }
 
 template <int QDT, int NG>

@@ -168,6 +168,10 @@ int step_plan(const int32_t* computed, const int32_t* qlens, int R, int32_t* bt,
   if (!qsl || !used || !err || (R && (!computed || !qlens || !seq)) || (R && W && !bt) ||
       (F && !free_ids) || (T && (!slots || !pos)))
     return host_fail(TTKV_E_INVALID, "null pointer argument");
+  // every workgroup reads the lengths while others write
+  for (const int32_t* out : {(const int32_t*)qsl, (const int32_t*)seq, (const int32_t*)used})
+    if (out && (out == computed || out == qlens))
+      return host_fail(TTKV_E_INVALID, "an output is one of the length inputs");
   PlanArgs a{computed, qlens, R, bt,  bt_row_stride, W,     free_ids, F,   bs,
              num_blocks, T,   qsl, seq, slots, pos, used, err};
   const int grid = std::max(1, (T + kPlanThreads * kPlanTokens - 1) / (kPlanThreads * kPlanTokens));

@@ -617,14 +617,22 @@ def _nibble_read(lay, query, page, block_table, seq_lens, query_start_loc, out):
     return *_page_args(page, lay.compressed_bytes_per_token()), out, index
 
 
+def _nibble_workspace(n: int, device) -> torch.Tensor:
+    ws = torch.empty(max(n, 256), dtype=torch.uint8, device=device)
+    ws[:65536].zero_()
+    return ws
+
+
 def nibble_decode_workspace(lay: NibbleLayout, num_heads: int, num_reqs: int, max_seq_len: int,
                             device) -> torch.Tensor:
-    """A zero-filled workspace for `nibble_decode_paged` over this batch shape; its first 64 KiB
-    (counters) are left zero by every call, so a buffer this large serves later calls too."""
+    """A workspace for `nibble_decode_paged` over batches of up to this shape. Its first 64 KiB
+    (counters) are zero, and every call of either 4-bit read leaves them so: one buffer of the
+    larger size serves both, call after call in stream order. Calls that may overlap, on two
+    streams, take one each."""
     n = _hip.lib().ttkv_nibble_decode_workspace_bytes(lay.H, num_heads, num_reqs, max_seq_len)
     if n < 0:
         raise ValueError("invalid head count or batch for the decode workspace")
-    return torch.zeros(max(int(n), 256), dtype=torch.uint8, device=device)
+    return _nibble_workspace(int(n), device)
 
 
 def nibble_decode_paged(lay: NibbleLayout, query: torch.Tensor, page: torch.Tensor,
@@ -658,12 +666,13 @@ def nibble_decode_paged(lay: NibbleLayout, query: torch.Tensor, page: torch.Tens
 
 def nibble_prefill_workspace(lay: NibbleLayout, num_heads: int, num_reqs: int, max_q_len: int,
                              max_seq_len: int, device) -> torch.Tensor:
-    """A zero-filled workspace for `nibble_prefill_paged` over this batch shape."""
+    """A workspace for `nibble_prefill_paged` over batches of up to this shape (see
+    `nibble_decode_workspace`)."""
     n = _hip.lib().ttkv_nibble_prefill_workspace_bytes(lay.H, num_heads, num_reqs, max_q_len,
                                                        max_seq_len)
     if n < 0:
         raise ValueError("invalid head count or batch for the prefill workspace")
-    return torch.zeros(max(int(n), 256), dtype=torch.uint8, device=device)
+    return _nibble_workspace(int(n), device)
 
 
 def nibble_prefill_paged(lay: NibbleLayout, query: torch.Tensor, page: torch.Tensor,
