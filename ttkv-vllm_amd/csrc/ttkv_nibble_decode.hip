@@ -31,6 +31,7 @@ constexpr int kNDThreads = 256;
 constexpr int kNDWaves = 4;
 constexpr int kNDStep = 2 * kNibTile;  // tokens per wave step
 constexpr int kNDPlanLanes = 4;        // requests per lane in the plan: 256 per launch
+constexpr int kNDClasses = 8;          // of chunk lengths, for the items' order
 constexpr int kNDShortRows = 256;      // rows of a chunk that may come here
 constexpr int64_t kNDShortWork = 130000;  // and steps of its blocks, times the blocks
 constexpr float kNDLazy = 8.f;         // log2 of the largest softmax weight before a rescale
@@ -100,33 +101,49 @@ __device__ __forceinline__ NibDecodePlan nd_plan(const NibDecodeArgs& a, int ite
   NibDecodePlan P{};
   P.h = item % a.H;
   const int it = item / a.H;
-  int carry = 0, blocks = 0, parts = 0;
   P.none = true;
+  // Long chunks first: the short ones fill the gaps that they leave at the end (61 requests of 70 to
+  // 2,900 tokens: 30.2 us in the batch's order, 28.3 so). Classes by the chunk's eighth of C, in the
+  // batch's order within each.
+  int nch[kNDPlanLanes], cls[kNDPlanLanes], bex[kNDPlanLanes], pex[kNDPlanLanes];
+  int blocks = 0, parts = 0;
 #pragma unroll
   for (int i = 0; i < kNDPlanLanes; ++i) {
     if (64 * i >= a.num_reqs) break;
-    const int nch = max(1, (st[i] + C - 1) / C), items = rb[i] * nch;
-    const int split = nch > 1 ? items : 0;
-    const int incl = nib_scan(items), ex = carry + incl - items;
+    nch[i] = max(1, (st[i] + C - 1) / C);
+    cls[i] = kNDClasses - 1 - min(kNDClasses - 1, (st[i] * kNDClasses - 1) / (nch[i] * C));
+    const int split = nch[i] > 1 ? rb[i] * nch[i] : 0;
     const int bincl = CHUNK ? nib_scan(rb[i]) : 0, pincl = nib_scan(split);
-    const uint64_t hit = __builtin_amdgcn_ballot_w64(items > 0 && ex <= it && it < ex + items);
-    if (hit) {
-      const int ln = __builtin_ctzll(hit);
-      P.none = false;
-      P.r = __builtin_amdgcn_readlane(idx[i], ln);
-      P.n = __builtin_amdgcn_readlane(n[i], ln);
-      P.Q = __builtin_amdgcn_readlane(Q[i], ln);
-      P.nch = __builtin_amdgcn_readlane(nch, ln);
-      const int local = it - __builtin_amdgcn_readlane(ex, ln);
-      P.rb = CHUNK ? local / P.nch : 0;
-      P.c = local - P.rb * P.nch;
-      P.rows = CHUNK ? min(max(P.Q, 0), a.max_q) * a.G : a.G;
-      P.part = parts + __builtin_amdgcn_readlane(pincl - split, ln) + P.rb * P.nch;
-      P.block = CHUNK ? blocks + __builtin_amdgcn_readlane(bincl - rb[i], ln) + P.rb : 64 * i + ln;
-    }
-    carry += __builtin_amdgcn_readlane(incl, 63);
+    bex[i] = CHUNK ? blocks + bincl - rb[i] : 64 * i + lane;
+    pex[i] = parts + pincl - split;
     parts += __builtin_amdgcn_readlane(pincl, 63);
     if (CHUNK) blocks += __builtin_amdgcn_readlane(bincl, 63);
+  }
+  int carry = 0;
+  for (int k = 0; k < kNDClasses && P.none; ++k) {
+#pragma unroll
+    for (int i = 0; i < kNDPlanLanes; ++i) {
+      if (64 * i >= a.num_reqs) break;
+      const int items = cls[i] == k ? rb[i] * nch[i] : 0;
+      if (!__builtin_amdgcn_ballot_w64(items > 0)) continue;
+      const int incl = nib_scan(items), ex = carry + incl - items;
+      const uint64_t hit = __builtin_amdgcn_ballot_w64(items > 0 && ex <= it && it < ex + items);
+      if (hit) {
+        const int ln = __builtin_ctzll(hit);
+        P.none = false;
+        P.r = __builtin_amdgcn_readlane(idx[i], ln);
+        P.n = __builtin_amdgcn_readlane(n[i], ln);
+        P.Q = __builtin_amdgcn_readlane(Q[i], ln);
+        P.nch = __builtin_amdgcn_readlane(nch[i], ln);
+        const int local = it - __builtin_amdgcn_readlane(ex, ln);
+        P.rb = CHUNK ? local / P.nch : 0;
+        P.c = local - P.rb * P.nch;
+        P.rows = CHUNK ? min(max(P.Q, 0), a.max_q) * a.G : a.G;
+        P.part = __builtin_amdgcn_readlane(pex[i], ln) + P.rb * P.nch;
+        P.block = __builtin_amdgcn_readlane(bex[i], ln) + P.rb;
+      }
+      carry += __builtin_amdgcn_readlane(incl, 63);
+    }
   }
   return P;
 }
