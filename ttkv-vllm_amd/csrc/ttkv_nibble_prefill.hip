@@ -35,7 +35,7 @@ constexpr int kNPPlanLanes = 4;    // requests per lane in the plan: 256 per lau
 constexpr int kNPMaxSplit = 32;
 constexpr int kNPMinTiles = 4;     // keys per part, in tiles (batches that are not searched)
 constexpr int kNPSearch = 16;      // requests up to which the plan searches for the number of parts
-constexpr float kNPLazy = 8.f;     // log2 of the largest softmax weight before a rescale
+constexpr float kNPMost = 2048.f;  // a lane's sum of eight softmax weights before a rescale
 constexpr float kNPNone = -1e30f;  // a maximum before the first visible key
 constexpr int64_t kNPPartRows = 127000;  // rows of partial results a launch may leave: 66.0 MB
 constexpr int kNPKBytes = kNPTile * kD * 2;
@@ -431,32 +431,12 @@ __global__ __launch_bounds__(kNPThreads, 2) void nibble_prefill_kernel(NibPrefil
             for (int i = 0; i < 4; ++i)
               if (tok + 16 * tg + i > lim[gr]) sc[gr][tg][i] = -INFINITY;
       }
-      float mt[NG];
-      bool more = false;
-#pragma unroll
-      for (int gr = 0; gr < NG; ++gr) {
-        mt[gr] = -INFINITY;
-#pragma unroll
-        for (int tg = 0; tg < 2; ++tg)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) mt[gr] = fmaxf(mt[gr], sc[gr][tg][i]);
-        mt[gr] *= qs[gr];
-        more |= mt[gr] > m[gr] + kNPLazy;
-      }
-      if (__builtin_amdgcn_ballot_w64(more)) {
-#pragma unroll
-        for (int gr = 0; gr < NG; ++gr) {
-          const float mn = fmaxf(m[gr], cross_row_max(mt[gr]));
-          const float f = exp2f(m[gr] - mn);
-          m[gr] = mn;
-          l[gr] *= f;
-#pragma unroll
-          for (int i = 0; i < 8; ++i) acc[gr][i] *= f;
-        }
-      }
+      // Weights against the maximum as it stands. It has to move only where a lane's sum of eight
+      // exceeds 2^11 (or is NaN): the scores' own maximum is taken in that case alone.
       half8 pf[NG];
-#pragma unroll
-      for (int gr = 0; gr < NG; ++gr)
+      float sum[NG];
+      auto weights = [&](int gr) {
+        sum[gr] = 0.f;
 #pragma unroll
         for (int tg = 0; tg < 2; ++tg)
 #pragma unroll
@@ -464,10 +444,36 @@ __global__ __launch_bounds__(kNPThreads, 2) void nibble_prefill_kernel(NibPrefil
             // the one rounding on the way to the output; the sum takes the rounded weights
             const half2v p = {(_Float16)fast_exp2(fmaf(sc[gr][tg][i], qs[gr], -m[gr])),
                               (_Float16)fast_exp2(fmaf(sc[gr][tg][i + 1], qs[gr], -m[gr]))};
-            l[gr] = __builtin_amdgcn_fdot2(p, half2v{(_Float16)1.f, (_Float16)1.f}, l[gr], false);
+            sum[gr] = __builtin_amdgcn_fdot2(p, half2v{(_Float16)1.f, (_Float16)1.f}, sum[gr], false);
             pf[gr][4 * tg + i] = p[0];
             pf[gr][4 * tg + i + 1] = p[1];
           }
+      };
+      bool fits = true;
+#pragma unroll
+      for (int gr = 0; gr < NG; ++gr) {
+        weights(gr);
+        fits &= sum[gr] <= kNPMost;
+      }
+      if (__builtin_amdgcn_ballot_w64(!fits)) {
+#pragma unroll
+        for (int gr = 0; gr < NG; ++gr) {
+          float mt = -INFINITY;
+#pragma unroll
+          for (int tg = 0; tg < 2; ++tg)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) mt = fmaxf(mt, sc[gr][tg][i]);
+          const float mn = fmaxf(m[gr], cross_row_max(mt * qs[gr]));
+          const float f = exp2f(m[gr] - mn);
+          m[gr] = mn;
+          l[gr] *= f;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) acc[gr][i] *= f;
+          weights(gr);
+        }
+      }
+#pragma unroll
+      for (int gr = 0; gr < NG; ++gr) l[gr] += sum[gr];
       __builtin_amdgcn_sched_barrier(0);
       __builtin_amdgcn_s_setprio(1);
 #pragma unroll
