@@ -67,12 +67,19 @@ __device__ __forceinline__ half2v nib_pair(uint32_t x, int m, half2v zb, half2v 
 // bf16 comes to fp16 at a power of two per row that brings its largest value to [1, 2): exact but for
 // values below 2^-14 of the largest, which keep an error of at most 2^-25 of it. `on`: false for
 // columns without a row, which are 0.
-template <int QDT>
-__device__ __forceinline__ void nib_load_query(const uint16_t* row, int q4, float scale_log2,
-                                               bool on, half8 qf[4], float& qs) {
+struct NibRow {
   u32x4 raw[4];
+};
+__device__ __forceinline__ NibRow nib_load_row(const uint16_t* row, int q4) {
+  NibRow x;
 #pragma unroll
-  for (int g = 0; g < 4; ++g) raw[g] = *gbl((const u32x4*)(row + 32 * g + 8 * q4));
+  for (int g = 0; g < 4; ++g) x.raw[g] = *gbl((const u32x4*)(row + 32 * g + 8 * q4));
+  return x;
+}
+template <int QDT>
+__device__ __forceinline__ void nib_query(const NibRow& in, float scale_log2, bool on, half8 qf[4],
+                                          float& qs) {
+  const auto& raw = in.raw;
   qs = fabsf(scale_log2);
   if constexpr (QDT == TTKV_DTYPE_F16) {
 #pragma unroll
@@ -80,15 +87,20 @@ __device__ __forceinline__ void nib_load_query(const uint16_t* row, int q4, floa
   } else {
     float x[32], mx = 0.f;
 #pragma unroll
-    for (int i = 0; i < 32; ++i) {
+    for (int i = 0; i < 32; i += 2) {
       const uint32_t w = raw[i >> 3][(i & 7) >> 1];
-      x[i] = bf16_bits_to_float(i & 1 ? w >> 16 : w & 0xffffu);
-      mx = fmaxf(mx, fabsf(x[i]));
+      x[i] = bf16_bits_to_float(w & 0xffffu);
+      x[i + 1] = bf16_bits_to_float(w >> 16);
+      mx = fmaxf(fmaxf(mx, fabsf(x[i])), fabsf(x[i + 1]));
     }
     mx = cross_row_max(mx);
     const int e = mx > 0.f && mx < INFINITY ? ilogbf(mx) : 0;
 #pragma unroll
-    for (int i = 0; i < 32; ++i) qf[i >> 3][i & 7] = (_Float16)ldexpf(x[i], -e);
+    for (int i = 0; i < 32; i += 2) {
+      const half2v p = {(_Float16)ldexpf(x[i], -e), (_Float16)ldexpf(x[i + 1], -e)};
+      qf[i >> 3][i & 7] = p[0];
+      qf[i >> 3][(i & 7) + 1] = p[1];
+    }
     qs = ldexpf(qs, e);
   }
   const bool none = qs == 0.f || !on;  // (a scale of 0 must not meet a masked score)

@@ -188,8 +188,8 @@ __global__ __launch_bounds__(kNDThreads, 2) void nibble_decode_kernel(NibDecodeA
   // The queries, row `col`, as the B operand of the four score products
   half8 qf[4];
   float qs, m = kNDNone, l = 0.f;
-  nib_load_query<QDT>(a.q + row_at(min(col, nrow - 1), a.q_row_stride), q4, a.scale_log2,
-                      col < nrow, qf, qs);
+  const NibRow qrow = nib_load_row(a.q + row_at(min(col, nrow - 1), a.q_row_stride), q4);
+  nib_query<QDT>(qrow, a.scale_log2, col < nrow, qf, qs);
   const int lim = CHUNK ? p0 + (row0 + min(col, nrow - 1)) / G : p0;  // last key the lane's row sees
   const int see_min = CHUNK ? p0 + row0 / G : p0;                     // and every row
   float4v acc[8];  // [group][dim of the pair]: dims 32 g + 8 q4 + 2 i + b of the lane's row

@@ -55,6 +55,7 @@ struct NibPrefillArgs {
   const int32_t* qsl;
   const int32_t* req_index;
   int num_reqs, max_q, max_seq;
+  uint32_t g_mul, g_shift;  // row / G = (2 row g_mul / 2^32) >> g_shift
   void* out;
   int out_dtype;
   int64_t out_row_stride;
@@ -80,14 +81,14 @@ struct NibPrefillPlan {
   int r, h, rb, sp, ns;  // batch row, KV head, row block, key part and how many
   int n, Q, rows;        // keys, the chunk's queries, rows processed
   int block;             // the row block's number in the launch
-  int64_t part;          // first part row of the (request, head)
+  int64_t part, q0;      // first part row of the (request, head), the chunk's first query row
   bool none;
 };
 
 // Parts of a request's tiles, C of them each but for rounding (a reciprocal: near a whole quotient it may
 // be one off, alike for every workgroup, and the parts are cut equal from their number; 1 for C >= tiles).
-__device__ __forceinline__ int np_parts(int tiles, int C) {
-  return min(max(1, (int)((float)(tiles + C - 1) * __builtin_amdgcn_rcpf((float)C))), kNPMaxSplit);
+__device__ __forceinline__ int np_parts(int tiles, int C, float by_C) {
+  return min(max(1, (int)((float)(tiles + C - 1) * by_C)), kNPMaxSplit);
 }
 
 // Tiles per part of `parts` parts of T tiles, rounded up or one more.
@@ -124,35 +125,56 @@ template <int RW>
 __device__ __forceinline__ NibPrefillPlan np_plan(const NibPrefillArgs& a, int item) {
   constexpr int NG = RW / (16 * kNPWaves);
   const int lane = threadIdx.x & 63;
-  int idx[kNPPlanLanes], n[kNPPlanLanes], Q[kNPPlanLanes], rows[kNPPlanLanes], tiles[kNPPlanLanes];
-  float work = 0.f, most_work = 0.f;  // tiles of all row blocks: that they see, and of their requests
+  int idx[kNPPlanLanes], n[kNPPlanLanes], q0[kNPPlanLanes], Q[kNPPlanLanes];
+  int rows[kNPPlanLanes], tiles[kNPPlanLanes];
 #pragma unroll
   for (int i = 0; i < kNPPlanLanes; ++i) {
+    idx[i] = n[i] = q0[i] = Q[i] = 0;
+    if (64 * i >= a.num_reqs) continue;
     const int r = lane + 64 * i;
     const bool on = r < a.num_reqs;
     idx[i] = on ? (a.req_index ? a.req_index[r] : r) : 0;
     n[i] = on ? a.seq_lens[idx[i]] : 0;
-    Q[i] = on ? a.qsl[idx[i] + 1] - a.qsl[idx[i]] : 0;
+    q0[i] = on ? a.qsl[idx[i]] : 0;
+    Q[i] = on ? a.qsl[idx[i] + 1] - q0[i] : 0;
+  }
+  float work = 0.f, most_work = 0.f;  // tiles of all row blocks: that they see, and of their requests
+#pragma unroll
+  for (int i = 0; i < kNPPlanLanes; ++i) {
+    rows[i] = tiles[i] = 0;
+    if (64 * i >= a.num_reqs) continue;
     const int nn = min(max(n[i], 0), a.max_seq);
     rows[i] = min(max(Q[i], 0), a.max_q) * a.G;
     tiles[i] = nn < Q[i] ? 1 : (nn + kNPTile - 1) / kNPTile;
     work += (float)((rows[i] + RW - 1) / RW) * np_mean_tiles(tiles[i], Q[i]);
     most_work += (float)((rows[i] + RW - 1) / RW) * (float)tiles[i];
   }
-  work = wave_sum(work) * (float)a.H;
   int C;
   if (a.num_reqs <= kNPSearch) {
     const int most = wave_max_i(rows[0] > 0 ? tiles[0] : 1);
     const int parts = (lane & (kNPMaxSplit - 1)) + 1, c = np_each(most, parts);
     float longest = 0.f, items = 0.f, need = 0.f;
-    for (int r = 0; r < a.num_reqs; ++r) {
-      const int T = __builtin_amdgcn_readlane(tiles[0], r), rw = __builtin_amdgcn_readlane(rows[0], r);
-      if (rw <= 0) continue;
-      const int ns = np_parts(T, c);
-      longest = fmaxf(longest, (float)T * __builtin_amdgcn_rcpf((float)ns));
-      items += (float)((rw + RW - 1) / RW * ns);
-      need += ns > 1 ? (float)rw * (float)ns : 0.f;
+    const float by_c = __builtin_amdgcn_rcpf((float)c);
+    const int blocks = (rows[0] + RW - 1) / RW;
+    work = wave_sum(work) * (float)a.H;
+    // a half wave takes every other request, four of them at a time (lanes past the last hold none)
+    for (int r = 0; r < a.num_reqs; r += 8) {
+#pragma unroll
+      for (int k = r; k < r + 8; k += 2) {
+        auto of = [&](int v) {
+          const int even = __builtin_amdgcn_readlane(v, k), odd = __builtin_amdgcn_readlane(v, k + 1);
+          return lane < 32 ? even : odd;
+        };
+        const int T = of(tiles[0]), rw = of(rows[0]);
+        const float ns = (float)np_parts(T, c, by_c);
+        longest = fmaxf(longest, rw > 0 ? (float)T * __builtin_amdgcn_rcpf(ns) : 0.f);
+        items += (float)of(blocks) * ns;
+        need += ns > 1.f ? (float)rw * ns : 0.f;
+      }
     }
+    longest = fmaxf(longest, __shfl_xor(longest, 32));
+    items += __shfl_xor(items, 32);
+    need += __shfl_xor(need, 32);
     items *= (float)a.H;
     need *= (float)a.H;
     const bool fits = need <= (float)a.part_rows && items <= (float)a.grid;  // (one part always does)
@@ -163,27 +185,28 @@ __device__ __forceinline__ NibPrefillPlan np_plan(const NibPrefillArgs& a, int i
   } else {
     // at most work / C items beside one per row block: within the grid
     C = max(kNPMinTiles, (int)ceilf(wave_sum(most_work) * (float)a.H / (float)a.target));
-  }
-  while (true) {
-    float need = 0.f;
+    while (true) {
+      float need = 0.f;
 #pragma unroll
-    for (int i = 0; i < kNPPlanLanes; ++i) {
-      const int ns = np_parts(tiles[i], C);
-      need += ns > 1 ? (float)rows[i] * (float)ns : 0.f;
+      for (int i = 0; i < kNPPlanLanes; ++i) {
+        const int ns = np_parts(tiles[i], C, __builtin_amdgcn_rcpf((float)C));
+        need += ns > 1 ? (float)rows[i] * (float)ns : 0.f;
+      }
+      need = wave_sum(need) * (float)a.H;
+      if (need <= (float)a.part_rows) break;
+      C += (C >> 2) + 1;
     }
-    need = wave_sum(need) * (float)a.H;
-    if (need <= (float)a.part_rows) break;
-    C += (C >> 2) + 1;
   }
   NibPrefillPlan P{};
   P.none = true;
   P.h = item % a.H;
   const int it = item / a.H;
   int carry = 0, blocks = 0, prows = 0;
+  const float by_C = __builtin_amdgcn_rcpf((float)C);
 #pragma unroll
   for (int i = 0; i < kNPPlanLanes; ++i) {
     if (64 * i >= a.num_reqs) break;
-    const int rb = (rows[i] + RW - 1) / RW, ns = np_parts(tiles[i], C), items = rb * ns;
+    const int rb = (rows[i] + RW - 1) / RW, ns = np_parts(tiles[i], C, by_C), items = rb * ns;
     const int pr = ns > 1 ? rows[i] * ns : 0;
     const int incl = nib_scan(items), ex = carry + incl - items;
     const int bincl = nib_scan(rb), pincl = nib_scan(pr);
@@ -196,6 +219,7 @@ __device__ __forceinline__ NibPrefillPlan np_plan(const NibPrefillArgs& a, int i
       P.r = __builtin_amdgcn_readlane(idx[i], ln);
       P.n = __builtin_amdgcn_readlane(n[i], ln);
       P.Q = __builtin_amdgcn_readlane(Q[i], ln);
+      P.q0 = __builtin_amdgcn_readlane(q0[i], ln);
       P.rows = __builtin_amdgcn_readlane(rows[i], ln);
       P.ns = __builtin_amdgcn_readlane(ns, ln);
       P.rb = nrb - 1 - local / P.ns;  // the last rows see the most keys: first
@@ -231,6 +255,17 @@ __device__ __forceinline__ void np_barrier() {
   __builtin_amdgcn_s_barrier();
   asm volatile("" ::: "memory");
 }
+// row / G for rows below 2^31, with g_mul = ceil(2^(31 + g_shift) / G) and 2^g_shift >= G: row times
+// what the rounding adds is below 2^(31 + g_shift).
+__device__ __forceinline__ int np_by_g(const NibPrefillArgs& a, int row) {
+  return (int)(__umulhi(2u * (uint32_t)row, a.g_mul) >> a.g_shift);
+}
+// Row `row` of a chunk that begins at query row q0, KV head h, in the query or the output.
+__device__ __forceinline__ int64_t np_row_at(const NibPrefillArgs& a, int64_t q0, int h, int row,
+                                             int64_t stride) {
+  const int j = np_by_g(a, row);
+  return (q0 + j) * stride + (int64_t)(h * a.G + row - j * a.G) * kD;
+}
 template <int QDT, int NG>
 __global__ __launch_bounds__(kNPThreads, 2) void nibble_prefill_kernel(NibPrefillArgs a) {
   constexpr int RW = kNPWaves * 16 * NG;
@@ -241,9 +276,9 @@ __global__ __launch_bounds__(kNPThreads, 2) void nibble_prefill_kernel(NibPrefil
   const int wv = __builtin_amdgcn_readfirstlane(tid >> 6);
   const NibPrefillPlan P = np_plan<RW>(a, blockIdx.x);
   if (P.none) return;
-  const int G = a.G, h = P.h;
+  const int h = P.h;
   const int n = min(max(P.n, 0), a.max_seq);
-  const int64_t q0 = a.qsl[P.r];
+  const int64_t q0 = P.q0;
   const int nrow = min(RW, P.rows - P.rb * RW);
   if (tid == 0 && h == 0 && P.sp == 0 && P.rb == 0 &&
       (P.n > a.max_seq || P.Q > a.max_q || n < P.Q))
@@ -252,7 +287,7 @@ __global__ __launch_bounds__(kNPThreads, 2) void nibble_prefill_kernel(NibPrefil
     for (int e = tid; e < nrow * kD; e += kNPThreads) {
       const int row = P.rb * RW + e / kD;
       store_act(a.out, a.out_dtype,
-                (q0 + row / G) * a.out_row_stride + (int64_t)(h * G + row % G) * kD + e % kD, NAN);
+                np_row_at(a, q0, h, row, a.out_row_stride) + e % kD, NAN);
     }
     return;
   }
@@ -260,28 +295,13 @@ __global__ __launch_bounds__(kNPThreads, 2) void nibble_prefill_kernel(NibPrefil
   const int row0 = P.rb * RW + wv * 16 * NG;  // the wave's first row
   const bool active = row0 < P.rows;
   const int p0 = n - P.Q;  // position of query 0
-  const int see_min = p0 + row0 / G, see_max = p0 + min(row0 + 16 * NG - 1, P.rows - 1) / G;
-
-  half8 qf[NG][4];
-  float qs[NG], m[NG], l[NG];
-  int lim[NG];  // last key the lane's row sees
-  float4v acc[NG][8];
-#pragma unroll
-  for (int gr = 0; gr < NG; ++gr) {
-    const int row = min(row0 + 16 * gr + col, P.rows - 1);
-    lim[gr] = p0 + row / G;
-    nib_load_query<QDT>(a.q + (q0 + row / G) * a.q_row_stride + (int64_t)(h * G + row % G) * kD,
-                        q4, a.scale_log2, true, qf[gr], qs[gr]);
-    m[gr] = kNPNone;
-    l[gr] = 0.f;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) acc[gr][i] = float4v{};
-  }
+  const int see_min = p0 + np_by_g(a, row0),
+            see_max = p0 + np_by_g(a, min(row0 + 16 * NG - 1, P.rows - 1));
 
   // the block's tiles and this part of them
-  const int tiles = (p0 + (P.rb * RW + nrow - 1) / G) / kNPTile + 1;
+  const int tiles = (p0 + np_by_g(a, P.rb * RW + nrow - 1)) / kNPTile + 1;
   const int t0 = (int)((int64_t)tiles * P.sp / P.ns), t1 = (int)((int64_t)tiles * (P.sp + 1) / P.ns);
-  const int wg_see = p0 + P.rb * RW / G;  // last key that every row of the block sees
+  const int wg_see = p0 + np_by_g(a, P.rb * RW);  // last key that every row of the block sees
   const uint8_t* base = a.page + (int64_t)h * kNibRecord;
   const int32_t* bt = a.bt + (int64_t)P.r * a.bt_row_stride;
   const NibMasks masks = nib_masks();
@@ -320,6 +340,28 @@ __global__ __launch_bounds__(kNPThreads, 2) void nibble_prefill_kernel(NibPrefil
       par[0][1] = kp[1];
     }
   };
+  if (t0 < t1) fetch_ids(t0);
+  // The query rows are asked for behind the first tile's record ids, and wait behind its codes.
+  NibRow qrow[NG];
+  int lim[NG];  // last key the lane's row sees
+#pragma unroll
+  for (int gr = 0; gr < NG; ++gr) {
+    const int row = min(row0 + 16 * gr + col, P.rows - 1);
+    lim[gr] = p0 + np_by_g(a, row);
+    qrow[gr] = nib_load_row(a.q + np_row_at(a, q0, h, row, a.q_row_stride), q4);
+  }
+  load(t0);
+  half8 qf[NG][4];
+  float qs[NG], m[NG], l[NG];
+  float4v acc[NG][8];
+#pragma unroll
+  for (int gr = 0; gr < NG; ++gr) {
+    nib_query<QDT>(qrow[gr], a.scale_log2, true, qf[gr], qs[gr]);
+    m[gr] = kNPNone;
+    l[gr] = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) acc[gr][i] = float4v{};
+  }
   auto dequant_keys = [&](int t) {
     if (t >= t1) return;
     const uint32_t at = krow + (t & 1) * kNPBuf + tt * (16 * 256);
@@ -506,8 +548,6 @@ __global__ __launch_bounds__(kNPThreads, 2) void nibble_prefill_kernel(NibPrefil
 
   if (tid == 0) bad_sh = 0;
   if (t0 < t1) {
-    fetch_ids(t0);
-    load(t0);
     if (!values) {
       dequant_keys(t0);
       load(t0 + 1);
@@ -545,7 +585,7 @@ __global__ __launch_bounds__(kNPThreads, 2) void nibble_prefill_kernel(NibPrefil
       const int row = row0 + 16 * gr + col;
       if (row >= P.rows) continue;
       const float inv = 1.f / l[gr];
-      const int64_t at = (q0 + row / G) * a.out_row_stride + (int64_t)(h * G + row % G) * kD;
+      const int64_t at = np_row_at(a, q0, h, row, a.out_row_stride);
 #pragma unroll
       for (int db = 0; db < 8; ++db)
         store_act4(a.out, a.out_dtype, at + 16 * db + 4 * q4, acc[gr][db] * inv, true);
@@ -646,7 +686,7 @@ __global__ __launch_bounds__(kNPJoinThreads) void nibble_join_kernel(NibPrefillA
       if (row >= nr) break;
       const int rr = J.row0 + r0 + row;
       store_act4(a.out, a.out_dtype,
-                 (J.q0 + rr / a.G) * a.out_row_stride + (int64_t)(J.h * a.G + rr % a.G) * kD + d,
+                 np_row_at(a, J.q0, J.h, rr, a.out_row_stride) + d,
                  o[u] * inv_sh[row], true);
     }
   };
@@ -795,6 +835,8 @@ int nibble_prefill_paged(int H, int HQ, int d, float scale, const void* q, int q
   NibPrefillArgs a{};
   a.H = H;
   a.G = HQ / H;
+  while ((1 << a.g_shift) < a.G) ++a.g_shift;
+  a.g_mul = (uint32_t)(((1ull << (31 + a.g_shift)) + a.G - 1) / a.G);
   a.scale_log2 = scale * 1.4426950408889634f;
   a.q = (const uint16_t*)q;
   a.q_row_stride = q_row_stride;
