@@ -13,9 +13,9 @@
 //     bytes are its A operand of all four (token lane % 16, 8 dims of each group of 32), unpacked by a
 //     shift and a mask per pair and dequantised exactly in packed fp16; the queries are the B operand,
 //     held in registers. Columns without a row are zero.
-//   softmax in the result's own registers: lane column = row, 8 tokens of it; the running maximum
-//     moves only when a score exceeds it by 8 (weights stay below 2^8), so most steps need no
-//     exchange between lanes, and the sum stays per lane until the end.
+//   softmax in the result's own registers: lane column = row, 8 tokens of it. Weights are taken against
+//     the maximum as it stands, which moves only when a lane's eight sum to more than 2^11, so most
+//     steps need no maximum and no exchange between lanes; the sum stays per lane until the end.
 //   O^T [dim, row] += V^T P^T, eight MFMAs: the scores' layout is the B operand's as it
 //     stands, and a lane's 16 value code bytes per tile are its A operand of all eight (a dim pair of
 //     each group, four tokens). The result's column is the row again, so the rescale is a lane's factor.
@@ -34,7 +34,7 @@ constexpr int kNDPlanLanes = 4;        // requests per lane in the plan: 256 per
 constexpr int kNDClasses = 8;          // of chunk lengths, for the items' order
 constexpr int kNDShortRows = 256;      // rows of a chunk that may come here
 constexpr int64_t kNDShortWork = 130000;  // and steps of its blocks, times the blocks
-constexpr float kNDLazy = 8.f;         // log2 of the largest softmax weight before a rescale
+constexpr float kNDMost = 2048.f;      // a lane's sum of eight softmax weights before a rescale
 constexpr float kNDNone = -1e30f;      // a maximum before the first visible key
 constexpr int kNDRows = 16;            // rows of a block: a matrix product's columns
 
@@ -270,32 +270,40 @@ __global__ __launch_bounds__(kNDThreads, 2) void nibble_decode_kernel(NibDecodeA
           }
         }
     }
-    float mt = -INFINITY;
+    // Weights against the maximum as it stands. It has to move only where a lane's sum of eight
+    // exceeds 2^11 (or is NaN): the scores' own maximum is taken in that case alone.
+    half8 pf;
+    float sum;
+    auto weights = [&]() {
+      sum = 0.f;
 #pragma unroll
-    for (int t = 0; t < 2; ++t)
+      for (int t = 0; t < 2; ++t)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) mt = fmaxf(mt, sc[t][i]);
-    mt *= qs;
-    if (__builtin_amdgcn_ballot_w64(mt > m + kNDLazy)) {
-      const float mn = fmaxf(m, cross_row_max(mt));
+        for (int i = 0; i < 4; i += 2) {
+          // the one rounding on the way to the output; the sum takes the rounded weights
+          const half2v p = {(_Float16)fast_exp2(fmaf(sc[t][i], qs, -m)),
+                            (_Float16)fast_exp2(fmaf(sc[t][i + 1], qs, -m))};
+          sum = __builtin_amdgcn_fdot2(p, half2v{(_Float16)1.f, (_Float16)1.f}, sum, false);
+          pf[4 * t + i] = p[0];
+          pf[4 * t + i + 1] = p[1];
+        }
+    };
+    weights();
+    if (__builtin_amdgcn_ballot_w64(!(sum <= kNDMost))) {
+      float mt = -INFINITY;
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) mt = fmaxf(mt, sc[t][i]);
+      const float mn = fmaxf(m, cross_row_max(mt * qs));
       const float f = exp2f(m - mn);
       m = mn;
       l *= f;
 #pragma unroll
       for (int i = 0; i < 8; ++i) acc[i] *= f;
+      weights();
     }
-    half8 pf;
-#pragma unroll
-    for (int t = 0; t < 2; ++t)
-#pragma unroll
-      for (int i = 0; i < 4; i += 2) {
-        // the one rounding on the way to the output; the sum takes the rounded weights
-        const half2v p = {(_Float16)fast_exp2(fmaf(sc[t][i], qs, -m)),
-                          (_Float16)fast_exp2(fmaf(sc[t][i + 1], qs, -m))};
-        l = __builtin_amdgcn_fdot2(p, half2v{(_Float16)1.f, (_Float16)1.f}, l, false);
-        pf[4 * t + i] = p[0];
-        pf[4 * t + i + 1] = p[1];
-      }
+    l += sum;
 #pragma unroll
     for (int quad = 0; quad < 2; ++quad)
 #pragma unroll

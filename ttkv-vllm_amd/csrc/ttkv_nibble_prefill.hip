@@ -8,8 +8,8 @@
 //               the order of the products' operands. Once per tile and 128 NG rows.
 //   S^T = K Q^T on v_mfma_f32_16x16x32_f16, 32 tokens at a time: a key fragment read from LDS serves
 //               the wave's NG groups. Lane column = row, so a row's softmax state is a lane's own.
-//   softmax     as in the decode kernel: the maximum moves when a score exceeds it by 8, weights are
-//               rounded to fp16 once and their sum is of the rounded ones.
+//   softmax     as in the decode kernel: weights against a maximum that moves seldom, rounded to fp16
+//               once, and their sum is of the rounded ones.
 //   O^T += V^T P^T: the scores' layout is the weights' operand layout as it stands.
 // One barrier per tile (two tile buffers); the next tile's codes are in flight in registers. Waves
 // 0..3 compute before they dequantise and waves 4..7 after, so that the two waves of a SIMD are
@@ -97,13 +97,13 @@ __device__ __forceinline__ int np_each(int T, int parts) {
 }
 
 // An estimate of a launch's time in us, from what these kernels measured: a tile of a row block takes
-// 2.0, 2.3 and 3.4 us with one, two and three groups of rows per wave (8 x 384 rows over 6,000 and
-// 12,000 keys) and a block 5 us beside its tiles (4 x 1,432 rows over 180 keys, 8 heads); the items, of
+// 1.55, 2.05 and 3.0 us with one, two and three groups of rows per wave (16 x 384 rows over 24,000 and
+// 48,000 keys) and a block 5 us beside its tiles (4 x 1,432 rows over 180 keys, 8 heads); the items, of
 // `load` tiles in all, take whole rounds of the CUs, and no less than the longest; a split costs its join
 // and, per partial row, 520 bytes written and read.
 __host__ __device__ inline float np_cost(int ng, float longest, float load, float items, float cus,
                                          float need) {
-  const float tile = ng == 1 ? 2.0f : ng == 2 ? 2.3f : 3.4f;
+  const float tile = ng == 1 ? 1.55f : ng == 2 ? 2.05f : 3.0f;
 #ifdef __HIP_DEVICE_COMPILE__
   const float rounds = ceilf(items * __builtin_amdgcn_rcpf(cus)), each = load * __builtin_amdgcn_rcpf(items);
 #else
