@@ -69,13 +69,15 @@ def page_bytes(page: torch.Tensor, blob: int) -> torch.Tensor:
 def _page_args(page: torch.Tensor, blob: int) -> tuple[int, int, int]:
     """(pointer, slots, bytes per slot) of a paged cache, as `page_bytes` views it (the same
     refusals, without making the views)."""
-    if page.dim() < 2 or not page.is_contiguous():
+    shape = page.shape
+    if len(shape) < 2 or not page.is_contiguous():
         flat = page_bytes(page, blob)
         return flat.data_ptr(), flat.shape[0], flat.stride(0)
-    row = page.shape[-1] * page.element_size()
+    last = shape[-1]
+    row = last * page.element_size()
     if row < blob:
         raise ValueError(f"the cache row is {row} bytes but the layout needs {blob}")
-    return page.data_ptr(), page.numel() // max(page.shape[-1], 1), row
+    return page.data_ptr(), page.numel() // (last or 1), row
 
 
 def decode_workspace(lay: TTKLayout, num_heads: int, num_reqs: int, max_seq_len: int,
@@ -452,9 +454,19 @@ class StepPlan(NamedTuple):
     blocks_used: torch.Tensor       # [1] int32, ids taken from the free list
 
 
-def _plan_out(t, n, dtype, device, name):
+def _table(block_table, want, rows=None):
+    """(max_blocks, row stride) of a block table; `rows`: how many it must have."""
+    shape = block_table.shape
+    if block_table.dtype != torch.int32 or len(shape) != 2 \
+            or (rows is not None and shape[0] != rows) \
+            or (not block_table.is_contiguous() and shape[1] > 1 and block_table.stride(1) != 1):
+        raise ValueError(f"block_table must be int32 {want} with contiguous rows")
+    return shape[1], block_table.stride(0)
+
+
+def _plan_out(t, n, dtype, like, name):
     if t is None:
-        return torch.empty(n, dtype=dtype, device=device)
+        return like.new_empty(n, dtype=dtype)
     if t.dtype != dtype or t.numel() != n or not t.is_contiguous():
         raise ValueError(f"{name} must be a contiguous {dtype} tensor of {n}")
     return t
@@ -477,23 +489,20 @@ def step_plan(computed_lens: torch.Tensor, query_lens: torch.Tensor, block_table
     _i32(computed_lens, "computed_lens")
     _i32(query_lens, "query_lens")
     _i32(free_blocks, "free_blocks")
-    R, dev = computed_lens.numel(), computed_lens.device
+    R = computed_lens.numel()
     if query_lens.numel() != R:
         raise ValueError(f"{R} computed lengths and {query_lens.numel()} query lengths")
-    if block_table.dtype != torch.int32 or block_table.dim() != 2 or block_table.shape[0] != R \
-            or (block_table.shape[1] > 1 and block_table.stride(1) != 1):
-        raise ValueError(f"block_table must be int32 [{R}, max_blocks] with contiguous rows")
+    W, stride = _table(block_table, f"[{R}, max_blocks]", R)
     n = int(num_tokens)
-    plan = StepPlan(_plan_out(query_start_loc, R + 1, torch.int32, dev, "query_start_loc"),
-                    _plan_out(seq_lens, R, torch.int32, dev, "seq_lens"),
-                    _plan_out(slot_mapping, n, torch.int64, dev, "slot_mapping"),
-                    _plan_out(positions, n, torch.int64, dev, "positions"),
-                    _plan_out(blocks_used, 1, torch.int32, dev, "blocks_used"))
-    err = _error_word(error_word, dev)
-    W = block_table.shape[1]
+    plan = StepPlan(_plan_out(query_start_loc, R + 1, torch.int32, computed_lens, "query_start_loc"),
+                    _plan_out(seq_lens, R, torch.int32, computed_lens, "seq_lens"),
+                    _plan_out(slot_mapping, n, torch.int64, computed_lens, "slot_mapping"),
+                    _plan_out(positions, n, torch.int64, computed_lens, "positions"),
+                    _plan_out(blocks_used, 1, torch.int32, computed_lens, "blocks_used"))
+    err = _error_word(error_word, computed_lens.device)
     rc = _on_device(
         index, _hip.lib().ttkv_step_plan, computed_lens.data_ptr(), query_lens.data_ptr(), R, block_table.data_ptr(),
-        block_table.stride(0) if R > 1 else W, W, free_blocks.data_ptr(), free_blocks.numel(),
+        stride if R > 1 else W, W, free_blocks.data_ptr(), free_blocks.numel(),
         int(block_size), int(num_blocks), n, plan.query_start_loc.data_ptr(),
         plan.seq_lens.data_ptr(), plan.slot_mapping.data_ptr(), plan.positions.data_ptr(),
         plan.blocks_used.data_ptr(), err.data_ptr(), _stream(index))
@@ -537,17 +546,19 @@ def rotary_axes(query: torch.Tensor, key: torch.Tensor | None, positions: torch.
     if key is not None:
         H = key.shape[1] if key.dim() == 3 else 0
         key_out = torch.empty_like(key) if key_out is None else key_out
+    dtype = query.dtype
     for t, heads, what in ((query, HQ, "query"), (query_out, HQ, "query_out"), (key, H, "key"),
                            (key_out, H, "key_out")):
         if t is None:
             continue
         _rows(t, heads, d, what)
-        if t.shape[0] != N or t.dtype != query.dtype:
+        if t.shape[0] != N or t.dtype != dtype:
             raise ValueError(f"{what} must have the query's {N} tokens and dtype")
     err = _error_word(error_word, query.device)
     rc = _on_device(
-        index, _hip.lib().ttkv_rotary_axes, query.data_ptr(), _hip.ptr(key), query_out.data_ptr(), _hip.ptr(key_out),
-        _hip.DTYPE_CODE[query.dtype], N, HQ, H, d, query.stride(0),
+        index, _hip.lib().ttkv_rotary_axes, query.data_ptr(), _hip.ptr(key),
+        query_out.data_ptr(), _hip.ptr(key_out), _hip.DTYPE_CODE[dtype], N, HQ, H, d,
+        query.stride(0),
         0 if key is None else key.stride(0), query_out.stride(0),
         0 if key is None else key_out.stride(0), positions.data_ptr(),
         positions.stride(0) if positions.dim() == 2 else N, len(sections), _c_sections(sections),
@@ -568,15 +579,17 @@ def nibble_write_paged(lay: NibbleLayout, key: torch.Tensor, value: torch.Tensor
     more); slot_mapping [>= N] int64, -1 for padded tokens; key_out / value_out (optional, fp16
     [N, H, d], contiguous) receive what the slots then stand for. See `ttkv_nibble_write_paged`."""
     index = _one_device(key, value, slot_mapping, page, key_out, value_out, error_word)
-    N = key.shape[0]
-    for t, what in ((key, "key"), (value, "value")):
-        _rows(t, lay.H, lay.d, what)
-        if t.shape[0] != N:
-            raise ValueError(f"{N} keys and {t.shape[0]} values")
-        if t.dtype not in _hip.DTYPE_CODE:
-            raise ValueError(f"{what} dtype must be fp32, fp16 or bf16")
+    shape = key.shape
+    _rows(key, lay.H, lay.d, "key")
+    _rows(value, lay.H, lay.d, "value")
+    N = shape[0]
+    if value.shape[0] != N:
+        raise ValueError(f"{N} keys and {value.shape[0]} values")
+    k_code, v_code = _hip.DTYPE_CODE.get(key.dtype), _hip.DTYPE_CODE.get(value.dtype)
+    if k_code is None or v_code is None:
+        raise ValueError("key / value dtype must be fp32, fp16 or bf16")
     for t, what in ((key_out, "key_out"), (value_out, "value_out")):
-        if t is not None and (t.shape != key.shape or t.dtype != torch.float16
+        if t is not None and (t.shape != shape or t.dtype != torch.float16
                               or not t.is_contiguous()):
             raise ValueError(f"{what} must be contiguous fp16 [{N}, {lay.H}, {lay.d}]")
     if slot_mapping.dtype != torch.int64 or slot_mapping.numel() < N \
@@ -584,37 +597,41 @@ def nibble_write_paged(lay: NibbleLayout, key: torch.Tensor, value: torch.Tensor
         raise ValueError("slot_mapping must be contiguous int64 with one id per token")
     if not page.is_contiguous():
         raise ValueError("the cache page must be contiguous")
-    page_ptr, n_slots, slot_bytes = _page_args(page, lay.compressed_bytes_per_token())
     err = _error_word(error_word, key.device)
     rc = _on_device(
-        index, _hip.lib().ttkv_nibble_write_paged, lay.H, lay.d, key.data_ptr(), _hip.DTYPE_CODE[key.dtype], key.stride(0), value.data_ptr(),
-        _hip.DTYPE_CODE[value.dtype], value.stride(0), slot_mapping.data_ptr(), N, page_ptr,
-        n_slots, slot_bytes, _hip.ptr(key_out), _hip.ptr(value_out), err.data_ptr(),
-        _stream(index))
+        index, _hip.lib().ttkv_nibble_write_paged, lay.H, lay.d, key.data_ptr(), k_code,
+        key.stride(0), value.data_ptr(), v_code, value.stride(0), slot_mapping.data_ptr(), N,
+        *_page_args(page, lay.compressed_bytes_per_token()), _hip.ptr(key_out),
+        _hip.ptr(value_out), err.data_ptr(), _stream(index))
     _hip.check(rc, "ttkv_nibble_write_paged")
 
 
+_NIBBLE_DTYPES = {t: _hip.DTYPE_CODE[t] for t in (torch.float16, torch.bfloat16)}
+
+
 def _nibble_read(lay, query, page, block_table, seq_lens, query_start_loc, out):
-    """Checks shared by the 4-bit reads; returns (page pointer, slots, bytes per slot, out,
-    device index)."""
-    _rows(query, query.shape[1] if query.dim() == 3 else 0, lay.d, "query")
+    """Checks shared by the 4-bit reads; returns (out, what the C entries take of query and page, of
+    the block table and of out)."""
+    shape = query.shape
+    _rows(query, shape[1] if len(shape) == 3 else 0, lay.d, "query")
     if out is None:
         out = torch.empty_like(query)
-    index = _one_device(query, page, block_table, seq_lens, query_start_loc, out)
-    _rows(out, query.shape[1], lay.d, "out")
-    if out.shape[0] != query.shape[0]:
-        raise ValueError("out must match query's shape")
-    for t, what in ((query, "query"), (out, "out")):
-        if t.dtype not in (torch.float16, torch.bfloat16):
-            raise ValueError(f"{what} dtype must be fp16 or bf16")
-    if block_table.dtype != torch.int32 or block_table.dim() != 2 \
-            or (block_table.shape[1] > 1 and block_table.stride(1) != 1):
-        raise ValueError("block_table must be int32 [requests, max_blocks] with contiguous rows")
+    elif out.shape != shape or not out.is_contiguous():
+        _rows(out, shape[1], lay.d, "out")
+        if out.shape[0] != shape[0]:
+            raise ValueError("out must match query's shape")
+    q_code, out_code = _NIBBLE_DTYPES.get(query.dtype), _NIBBLE_DTYPES.get(out.dtype)
+    if q_code is None or out_code is None:
+        raise ValueError(f"{'out' if q_code else 'query'} dtype must be fp16 or bf16")
+    table = _table(block_table, "[requests, max_blocks]")
     _i32(seq_lens, "seq_lens")
     _i32(query_start_loc, "query_start_loc")
     if not page.is_contiguous():
         raise ValueError("the cache page must be contiguous")
-    return *_page_args(page, lay.compressed_bytes_per_token()), out, index
+    return (out, (query.data_ptr(), q_code, query.stride(0),
+                  *_page_args(page, lay.compressed_bytes_per_token())),
+            (block_table.data_ptr(), table[1], table[0]),
+            (out.data_ptr(), out_code, out.stride(0)))
 
 
 def _nibble_workspace(n: int, device) -> torch.Tensor:
@@ -643,23 +660,21 @@ def nibble_decode_paged(lay: NibbleLayout, query: torch.Tensor, page: torch.Tens
     """Attention of one query per request (row query_start_loc[r] of query [N, HQ, d], rotated)
     over its seq_lens[r] stored tokens of a 4-bit cache. See `ttkv_nibble_decode_paged` in
     include/ttkv_hip.h. Returns `out` [N, HQ, d] with the decode rows written."""
-    page_ptr, n_slots, slot_bytes, out, index = _nibble_read(lay, query, page, block_table,
-                                                             seq_lens, query_start_loc, out)
-    B, HQ, dev = seq_lens.numel(), query.shape[1], query.device
+    index = _one_device(query, page, block_table, seq_lens, query_start_loc, out, workspace,
+                        error_word)
+    out, q_args, bt_args, out_args = _nibble_read(lay, query, page, block_table, seq_lens,
+                                                  query_start_loc, out)
+    B, HQ = seq_lens.numel(), query.shape[1]
     if block_table.shape[0] < B or query_start_loc.numel() < B:
         raise ValueError(f"{B} sequence lengths need as many block table rows and query rows")
     if workspace is None:
-        workspace = nibble_decode_workspace(lay, HQ, B, max_seq_len, dev)
-    err = _error_word(error_word, dev)
-    _one_device(query, workspace, err)
+        workspace = nibble_decode_workspace(lay, HQ, B, max_seq_len, query.device)
+    err = _error_word(error_word, query.device)
     rc = _on_device(
-        index, _hip.lib().ttkv_nibble_decode_paged, lay.H, HQ, lay.d, float(scale),
-        query.data_ptr(), _hip.DTYPE_CODE[query.dtype], query.stride(0), page_ptr, n_slots,
-        slot_bytes, int(block_size), block_table.data_ptr(), block_table.stride(0),
-        block_table.shape[1], seq_lens.data_ptr(),
-        query_start_loc.data_ptr(), B, int(max_seq_len), out.data_ptr(),
-        _hip.DTYPE_CODE[out.dtype], out.stride(0), workspace.data_ptr(), workspace.numel(),
-        err.data_ptr(), _stream(index))
+        index, _hip.lib().ttkv_nibble_decode_paged, lay.H, HQ, lay.d, float(scale), *q_args,
+        int(block_size), *bt_args, seq_lens.data_ptr(), query_start_loc.data_ptr(), B,
+        int(max_seq_len), *out_args, workspace.data_ptr(), workspace.numel(), err.data_ptr(),
+        _stream(index))
     _hip.check(rc, "ttkv_nibble_decode_paged")
     return out
 
@@ -685,27 +700,24 @@ def nibble_prefill_paged(lay: NibbleLayout, query: torch.Tensor, page: torch.Ten
     [N, HQ, d], rotated) over their requests' stored tokens of a 4-bit cache, the chunk's own
     included. `req_index` picks the batch rows to process (default: all). See
     `ttkv_nibble_prefill_paged` in include/ttkv_hip.h."""
-    page_ptr, n_slots, slot_bytes, out, index = _nibble_read(lay, query, page, block_table,
-                                                             seq_lens, query_start_loc, out)
-    B, HQ, dev = seq_lens.numel(), query.shape[1], query.device
+    index = _one_device(query, page, block_table, seq_lens, query_start_loc, req_index, out,
+                        workspace, error_word)
+    out, q_args, bt_args, out_args = _nibble_read(lay, query, page, block_table, seq_lens,
+                                                  query_start_loc, out)
+    B, HQ = seq_lens.numel(), query.shape[1]
     if block_table.shape[0] < B or query_start_loc.numel() < B + 1:
         raise ValueError(f"{B} sequence lengths need as many block table rows and one more "
                          f"query start")
     if req_index is not None:
         _i32(req_index, "req_index")
-        _one_device(query, req_index)
         B = req_index.numel()
     if workspace is None:
-        workspace = nibble_prefill_workspace(lay, HQ, B, max_q_len, max_seq_len, dev)
-    err = _error_word(error_word, dev)
-    _one_device(query, workspace, err)
+        workspace = nibble_prefill_workspace(lay, HQ, B, max_q_len, max_seq_len, query.device)
+    err = _error_word(error_word, query.device)
     rc = _on_device(
-        index, _hip.lib().ttkv_nibble_prefill_paged, lay.H, HQ, lay.d, float(scale),
-        query.data_ptr(), _hip.DTYPE_CODE[query.dtype], query.stride(0), page_ptr, n_slots,
-        slot_bytes, int(block_size), block_table.data_ptr(), block_table.stride(0),
-        block_table.shape[1], seq_lens.data_ptr(),
-        query_start_loc.data_ptr(), _hip.ptr(req_index), B, int(max_q_len), int(max_seq_len),
-        out.data_ptr(), _hip.DTYPE_CODE[out.dtype], out.stride(0), workspace.data_ptr(),
-        workspace.numel(), err.data_ptr(), _stream(index))
+        index, _hip.lib().ttkv_nibble_prefill_paged, lay.H, HQ, lay.d, float(scale), *q_args,
+        int(block_size), *bt_args, seq_lens.data_ptr(), query_start_loc.data_ptr(),
+        _hip.ptr(req_index), B, int(max_q_len), int(max_seq_len), *out_args,
+        workspace.data_ptr(), workspace.numel(), err.data_ptr(), _stream(index))
     _hip.check(rc, "ttkv_nibble_prefill_paged")
     return out
