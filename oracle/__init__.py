@@ -18,6 +18,9 @@ Modules
   coef_modes -- fp16 and 4-bit (group-32) coefficient fields: this build's own storage modes,
               not the reference's (parity unpinned against it; pinned by closed forms, brute
               force and round trips in tests/test_coef_modes.py)
+  nibble   -- the 4-bit cache's format (places of every code, write and read) and plain attention
+              over it in 64 bits: not the reference's (pinned by exact fractions and round trips in
+              tests/test_nibble.py)
 
 Pinning (what each part is checked against; see `tests/test_oracle_*.py`):
   * layout geometry: closed-form table of byte offsets (safe/tight/campaign4x) and the
