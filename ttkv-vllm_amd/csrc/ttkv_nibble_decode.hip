@@ -33,7 +33,9 @@ constexpr int kNDStep = 2 * kNibTile;  // tokens per wave step
 constexpr int kNDPlanLanes = 4;        // requests per lane in the plan: 256 per launch
 constexpr int kNDClasses = 8;          // of chunk lengths, for the items' order
 constexpr int kNDShortRows = 256;      // rows of a chunk that may come here
-constexpr int64_t kNDShortWork = 130000;  // and steps of its blocks, times the blocks
+constexpr int64_t kNDShortWork = 17000;  // and steps of all its blocks,
+constexpr int64_t kNDFewWork = 24000;    // where they are few
+constexpr int kNDLongSteps = 32;       // steps from which a second round of items is worth it
 constexpr float kNDMost = 2048.f;      // a lane's sum of eight softmax weights before a rescale
 constexpr float kNDNone = -1e30f;      // a maximum before the first visible key
 constexpr int kNDRows = 16;            // rows of a block: a matrix product's columns
@@ -97,7 +99,22 @@ __device__ __forceinline__ NibDecodePlan nd_plan(const NibDecodeArgs& a, int ite
   // whole rounds of the four waves
   const int64_t all = (int64_t)total * a.H;
   const int64_t per = (all + a.target - 1) / a.target;
-  const int C = max(1, (int)((per + kNDWaves - 1) / kNDWaves)) * kNDWaves;
+  int C = max(1, (int)((per + kNDWaves - 1) / kNDWaves)) * kNDWaves;
+  if (CHUNK) {
+    // Two workgroups of chunks fill a CU (decode: three): longer chunks rather than a second round of
+    // them, where the batch has not more blocks anyway (6 x 32 queries over 600 keys: 27.5 us, 17.0 so).
+    int whole = 0;
+#pragma unroll
+    for (int i = 0; i < kNDPlanLanes; ++i) whole += rb[i];
+    whole = wave_sum_i(whole);
+    while ((int64_t)whole * a.H <= a.target) {
+      int items = 0;
+#pragma unroll
+      for (int i = 0; i < kNDPlanLanes; ++i) items += rb[i] * max(1, (st[i] + C - 1) / C);
+      if ((int64_t)wave_sum_i(items) * a.H <= a.target) break;
+      C += max(1, C / (16 * kNDWaves)) * kNDWaves;
+    }
+  }
   NibDecodePlan P{};
   P.h = item % a.H;
   const int it = item / a.H;
@@ -516,17 +533,24 @@ int64_t nibble_decode_workspace_bytes(int H, int HQ, int num_reqs, int max_seq) 
   return nd_workspace(H, num_reqs, max_seq, HQ / H);
 }
 
-// Chunks of at most 16 rows take this kernel, and short ones while the whole call is short: it reads
+// Chunks of at most 16 rows take this kernel, and longer ones while the whole call is short: it reads
 // and dequantises a key for 16 rows, the prefill kernel for 128 to 384, but it has no tiles in LDS, no
-// second launch and a smaller join. Both measured at four query heads and eight KV heads, here and
-// there: 1 x 64 queries over 500 keys 14.8 and 23.7 us, 1 x 32 over 4,000 19.4 and 25.7, 3 x 16 over
-// 3,000 20.3 and 24.0, 16 x 8 over 6,000 51.3 and 65.6; 8 x 16 over 3,000 32.0 and 30.6, 3 x 32 over
-// 3,000 34.0 and 28.8, 8 x 32 over 3,000 48.2 and 38.0. The limit on steps times blocks parts these.
+// second launch and a smaller join. A call's items before any split are its (block, head) pairs, its
+// work their steps. Measured here and there (us, four query heads and eight KV heads):
+//   two blocks: one round of items, or long ones   30 x 8 queries over 100 keys 11.5, 13.5;
+//     16 x 8 over 6,000 48.4, 61.3; 60 x 8 over 1,500 51.8, 61.9; but 60 x 8 over 300 26.4, 24.4
+//   more, one round of items, 24,000 steps of few of them   1 x 32 over 12,000 29.8, 35.2; 1 x 64 over
+//     5,000 26.8, 28.2; 1 x 64 over 6,000 30.3, 30.3; 2 x 20 over 14,000 38.7, 37.2
+//   or 17,000 of many   4 x 60 over 300 15.4, 18.1; 20 x 12 over 900 21.7, 34.0; 4 x 32 over 2,000 23.7,
+//     24.5; 4 x 32 over 2,500 26.3, 25.6; 5 x 20 over 4,000 35.3, 30.6; two rounds: 30 x 16 over 300 25.6, 16.0
 bool nibble_short_applies(int H, int HQ, int num_reqs, int max_q, int max_seq) {
   const int64_t rows = (int64_t)max_q * (HQ / H);
   if (rows > kNDShortRows || H * nd_blocks((int)rows) > kMaxCounters) return false;
   const int64_t blocks = nd_blocks((int)rows), steps = (max_seq + kNDStep - 1) / kNDStep;
-  return blocks == 1 || (int64_t)num_reqs * H * steps * blocks * blocks <= kNDShortWork;
+  const int64_t items = (int64_t)num_reqs * H * blocks;
+  if (blocks == 1) return true;
+  if (blocks == 2) return items <= nd_target() || steps >= kNDLongSteps;
+  return items <= nd_target() && items * steps <= (items <= nd_target() / 4 ? kNDFewWork : kNDShortWork);
 }
 
 // Bytes of partial results of such a chunk call at most, growing with every argument.
