@@ -19,7 +19,10 @@
 //   O^T [dim, row] += V^T P^T, eight MFMAs: the scores' layout is the B operand's as it
 //     stands, and a lane's 16 value code bytes per tile are its A operand of all eight (a dim pair of
 //     each group, four tokens). The result's column is the row again, so the rescale is a lane's factor.
-// Bytes per step 4,608; the two register sets keep the next step's loads in flight.
+// Bytes per step 4,608; the two register sets keep the next step's loads in flight. Bound by memory: 8 x
+// 14,402 tokens of 8 heads, 133 MB, 30.6 us, 4.35 TB/s (a copy reaches 4.8); the loads alone took 26 us
+// of a profiled 33. 61 requests of 70 to 2,900 tokens 28.3 us for 98 MB; one of 1,082 tokens 9 us, the
+// chain of plan, block ids, codes, hand-off and join.
 #include <math.h>
 
 #include "ttkv_host.h"
@@ -498,8 +501,8 @@ __global__ __launch_bounds__(kNDThreads, 2) void nibble_decode_kernel(NibDecodeA
 }
 
 // The plan's item target: two workgroups per CU. A third would fit beside them, but shorter chunks
-// pay their prologue and join more often (8 x 14,402 tokens: 31.2 us at two per CU, 32.8 at three, 36.2
-// at four; 61 requests of 70 to 2,900: 33.4, 35.0, 34.6).
+// pay their prologue and join more often (8 x 14,402 tokens: 30.7 us at two per CU, 35.7 at two and a
+// half, 32.8 at three; 61 requests of 70 to 2,900: 28.6, 28.2, 31.0).
 static int nd_target() { return 2 * device_cu_count(); }
 
 // Requests per launch, of `blocks` row blocks each: the plan's lanes, and a counter per (block, head).

@@ -15,6 +15,11 @@
 // 0..3 compute before they dequantise and waves 4..7 after, so that the two waves of a SIMD are
 // out of step and one's matrix products run under the other's vector work.
 //
+// Bound by instruction issue: per tile of 384 rows a SIMD's two waves have 192 products of 16 cycles and
+// about 750 vector instructions (softmax, dequantisation) that take 4 cycles each beside them; 5,900
+// cycles in all, with the clock near 1.95 GHz when every CU works. 1 x 2,048 queries of 32 heads over 12,345
+// keys: 274 us, 1,040 TFLOP/s (a large library product 1,250); 4 x 256 of 24 heads over 7,656: 106 us.
+//
 // The keys of a row block are split over several workgroups where the batch has too few row blocks
 // to fill the chip: the split comes from a plan that every workgroup computes alike from the lengths
 // on the device. The parts' unnormalised results are joined by a second launch, 32 rows per workgroup

@@ -10,6 +10,10 @@
 // x - q s, is within 1e-6, and exact on a border: there the corrected value differs from a number
 // that fp32 holds by less than q 2^-44 before it is rounded. 32-bit inputs are divided in 64 bits.
 // The scale's range and its quotient by 15 are taken in 64 bits for every type.
+//
+// Bound by the instructions of the quantisation, about 300 per wave: 2,048 tokens of 8 heads in bf16, 15
+// MB with the stored values returned, 7.5 us (a row over 32 lanes and library divisions: 13); a few
+// tokens are one chain of round trips, 3.3 us.
 #include <math.h>
 
 #include "ttkv_host.h"
