@@ -249,7 +249,8 @@ __device__ __forceinline__ Rot8<DT> rot_load8(const void* p, int64_t i) {
   Rot8<DT> x;
   const char* at = (const char*)p + i * (DT == TTKV_DTYPE_F32 ? 4 : 2);
 #pragma unroll
-  for (int j = 0; j < (DT == TTKV_DTYPE_F32 ? 2 : 1); ++j) x.raw[j] = *gbl((const u32x4*)at + j);
+  for (int j = 0; j < (DT == TTKV_DTYPE_F32 ? 2 : 1); ++j)
+    x.raw[j] = __builtin_nontemporal_load(gbl((const u32x4*)at + j));
   return x;
 }
 template <int DT>
@@ -263,15 +264,29 @@ __device__ __forceinline__ float rot_get(const Rot8<DT>& x, int i) {
 }
 template <int DT>
 __device__ __forceinline__ void rot_store8(void* p, int64_t i, const float v[8]) {
-  store_act4(p, DT, i, float4v{v[0], v[1], v[2], v[3]}, true);
-  store_act4(p, DT, i + 4, float4v{v[4], v[5], v[6], v[7]}, true);
+  if constexpr (DT == TTKV_DTYPE_F32) {
+    store_act4(p, DT, i, float4v{v[0], v[1], v[2], v[3]}, true);
+    store_act4(p, DT, i + 4, float4v{v[4], v[5], v[6], v[7]}, true);
+  } else {
+    u32x4 w;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const float lo = v[2 * k], hi = v[2 * k + 1];
+      if constexpr (DT == TTKV_DTYPE_F16)
+        w[k] = __builtin_bit_cast(uint32_t, half2v{(_Float16)lo, (_Float16)hi});
+      else
+        w[k] = (uint32_t)float_to_bf16_bits(lo) | ((uint32_t)float_to_bf16_bits(hi) << 16);
+    }
+    *gblw((u32x4*)((uint16_t*)p + i)) = w;
+  }
 }
 
 // One wave per token. Lane j first looks up frequency j's cosine and sine (one load each, whatever
 // the axes) and leaves them in LDS; then the lanes take (head, 8 frequencies) pairs of 16-byte pieces,
 // four heads' loads in flight at a time, the first four asked for before the lookup. Bound by memory:
-// every query and key byte read and written once. 8,192 tokens of 40 heads in bf16, 171 MB: 41.5 us,
-// 4.1 TB/s (a copy reaches 4.8; the kernel below, a pair per thread, 116 us).
+// every query and key byte read and written once. 8,192 tokens of 40 heads in bf16, 171 MB: 37.3 us,
+// 4.6 TB/s (a copy reaches 4.8; loads that stay in the cache 41.3, the kernel below, a pair per thread,
+// 116).
 constexpr int kRotHalf = 128;  // frequencies the LDS holds
 constexpr int kRotBatch = 4;
 template <int DT>
