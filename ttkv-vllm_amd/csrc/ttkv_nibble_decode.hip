@@ -241,10 +241,10 @@ __global__ __launch_bounds__(kNDThreads, 2) void nibble_decode_kernel(NibDecodeA
       const int id = __builtin_amdgcn_readlane(t ? tid1 : tid0, k);
       const uint8_t* rec = base + (int64_t)max(id, 0) * a.tile_stride;
       x.k[t] = __builtin_nontemporal_load(gbl((const u32x4*)(rec + 16 * lane)));
-      x.kp[t] = *gbl((const u32x2v*)(rec + kNibKp + 8 * col));
+      x.kp[t] = __builtin_nontemporal_load(gbl((const u32x2v*)(rec + kNibKp + 8 * col)));
       x.v[t] = __builtin_nontemporal_load(gbl((const u32x4*)(rec + kNibV + 16 * lane)));
-      x.vp[t][0] = *gbl((const u32x4*)(rec + kNibVp + 32 * q4));
-      x.vp[t][1] = *gbl((const u32x4*)(rec + kNibVp + 32 * q4 + 16));
+      x.vp[t][0] = __builtin_nontemporal_load(gbl((const u32x4*)(rec + kNibVp + 32 * q4)));
+      x.vp[t][1] = __builtin_nontemporal_load(gbl((const u32x4*)(rec + kNibVp + 32 * q4 + 16)));
       bad |= id < 0;
     }
   };
