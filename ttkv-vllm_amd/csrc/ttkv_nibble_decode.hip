@@ -81,7 +81,7 @@ template <bool CHUNK>
 __device__ __forceinline__ NibDecodePlan nd_plan(const NibDecodeArgs& a, int item) {
   const int lane = threadIdx.x & 63;
   int idx[kNDPlanLanes], n[kNDPlanLanes], Q[kNDPlanLanes], st[kNDPlanLanes], rb[kNDPlanLanes];
-  int total = 0;
+  int total = 0, longest = 0;
 #pragma unroll
   for (int i = 0; i < kNDPlanLanes; ++i) {
     const int r = lane + 64 * i;
@@ -97,12 +97,17 @@ __device__ __forceinline__ NibDecodePlan nd_plan(const NibDecodeArgs& a, int ite
     if (CHUNK && nn < Q[i]) st[i] = 1;
     rb[i] = CHUNK ? (min(max(Q[i], 0), a.max_q) * a.G + kNDRows - 1) / kNDRows : Q[i];
     total += st[i] * rb[i];
+    longest = max(longest, st[i]);
   }
   total = wave_sum_i(total);
   // whole rounds of the four waves
   const int64_t all = (int64_t)total * a.H;
   const int64_t per = (all + a.target - 1) / a.target;
   int C = max(1, (int)((per + kNDWaves - 1) / kNDWaves)) * kNDWaves;
+  // A chunk's step costs the request about 0.2 us and a chunk about as much in the join: where the
+  // batch would fill the chip with shorter ones, the root of the steps, rounded down for 16 rows, whose
+  // steps cost more (1 x 14,000 tokens of 8 heads: 21.1 us, 16.6 so; of 2 heads 28.9, 16.7).
+  C = max(C, (int)(sqrtf((float)wave_max_i(longest)) / kNDWaves + (CHUNK ? 0.25f : 0.75f)) * kNDWaves);
   if (CHUNK) {
     // Two workgroups of chunks fill a CU (decode: three): longer chunks rather than a second round of
     // them, where the batch has not more blocks anyway (6 x 32 queries over 600 keys: 27.5 us, 17.0 so).
