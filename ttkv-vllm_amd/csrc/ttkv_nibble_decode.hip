@@ -73,37 +73,51 @@ struct NibDecodeArgs {
 struct NibDecodePlan {
   int r, rb, c, h;      // batch row, row block, chunk, KV head
   int n, Q, rows, nch;  // keys, queries, rows of all blocks, the block's chunks
+  int q0;               // the request's first row of the query
   int part, block;      // the block's first split item and its number, both before the head
   bool none;
 };
 
+// Chunks of at most C steps, by 1 / C to an ulp: never more than the quotient rounded up, and one less
+// only where it is whole, alike for every workgroup (the chunks are cut equal from their number).
+__device__ __forceinline__ int nd_chunks(int steps, int C, float by_C) {
+  return max(1, (int)((float)(steps + C - 1) * by_C));
+}
+
 template <bool CHUNK>
 __device__ __forceinline__ NibDecodePlan nd_plan(const NibDecodeArgs& a, int item) {
   const int lane = threadIdx.x & 63;
-  int idx[kNDPlanLanes], n[kNDPlanLanes], Q[kNDPlanLanes], st[kNDPlanLanes], rb[kNDPlanLanes];
-  int total = 0, longest = 0;
+  int idx[kNDPlanLanes], n[kNDPlanLanes], q0[kNDPlanLanes], Q[kNDPlanLanes];
+  int st[kNDPlanLanes], rb[kNDPlanLanes];
+  int total = 0, longest = 0, whole = 0;
 #pragma unroll
   for (int i = 0; i < kNDPlanLanes; ++i) {
+    idx[i] = n[i] = q0[i] = Q[i] = st[i] = rb[i] = 0;
+    if (64 * i >= a.num_reqs) continue;
     const int r = lane + 64 * i;
     const bool on = r < a.num_reqs;
     idx[i] = CHUNK && a.req_index && on ? a.req_index[r] : on ? r : 0;
     n[i] = on ? a.seq_lens[idx[i]] : 0;
-    Q[i] = on ? (CHUNK ? a.qsl[idx[i] + 1] - a.qsl[idx[i]] : 1) : 0;
+    q0[i] = on ? a.qsl[idx[i]] : 0;
+    Q[i] = on ? (CHUNK ? a.qsl[idx[i] + 1] - q0[i] : 1) : 0;
   }
 #pragma unroll
   for (int i = 0; i < kNDPlanLanes; ++i) {
+    if (64 * i >= a.num_reqs) continue;
     const int nn = min(max(n[i], 0), a.max_seq);
     st[i] = (nn + kNDStep - 1) / kNDStep;
     if (CHUNK && nn < Q[i]) st[i] = 1;
     rb[i] = CHUNK ? (min(max(Q[i], 0), a.max_q) * a.G + kNDRows - 1) / kNDRows : Q[i];
     total += st[i] * rb[i];
     longest = max(longest, st[i]);
+    whole += rb[i];
   }
   total = wave_sum_i(total);
   // whole rounds of the four waves
   const int64_t all = (int64_t)total * a.H;
-  const int64_t per = (all + a.target - 1) / a.target;
-  int C = max(1, (int)((per + kNDWaves - 1) / kNDWaves)) * kNDWaves;
+  const int per = all < 0x40000000 ? (int)((uint32_t)all + a.target - 1) / a.target
+                                   : (int)fminf((float)all / (float)a.target * 1.00001f, 1e8f) + 1;
+  int C = max(1, (per + kNDWaves - 1) / kNDWaves) * kNDWaves;
   // A chunk's step costs the request about 0.2 us and a chunk about as much in the join: where the
   // batch would fill the chip with shorter ones, the root of the steps, rounded down for 16 rows, whose
   // steps cost more (1 x 14,000 tokens of 8 heads: 21.1 us, 16.6 so; of 2 heads 28.9, 16.7).
@@ -111,14 +125,13 @@ __device__ __forceinline__ NibDecodePlan nd_plan(const NibDecodeArgs& a, int ite
   if (CHUNK) {
     // Two workgroups of chunks fill a CU (decode: three): longer chunks rather than a second round of
     // them, where the batch has not more blocks anyway (6 x 32 queries over 600 keys: 27.5 us, 17.0 so).
-    int whole = 0;
-#pragma unroll
-    for (int i = 0; i < kNDPlanLanes; ++i) whole += rb[i];
     whole = wave_sum_i(whole);
     while ((int64_t)whole * a.H <= a.target) {
       int items = 0;
+      const float by_C = __builtin_amdgcn_rcpf((float)C);
 #pragma unroll
-      for (int i = 0; i < kNDPlanLanes; ++i) items += rb[i] * max(1, (st[i] + C - 1) / C);
+      for (int i = 0; i < kNDPlanLanes; ++i)
+        if (64 * i < a.num_reqs) items += rb[i] * nd_chunks(st[i], C, by_C);
       if ((int64_t)wave_sum_i(items) * a.H <= a.target) break;
       C += max(1, C / (16 * kNDWaves)) * kNDWaves;
     }
@@ -132,11 +145,13 @@ __device__ __forceinline__ NibDecodePlan nd_plan(const NibDecodeArgs& a, int ite
   // batch's order within each.
   int nch[kNDPlanLanes], cls[kNDPlanLanes], bex[kNDPlanLanes], pex[kNDPlanLanes];
   int blocks = 0, parts = 0;
+  const float by_C = __builtin_amdgcn_rcpf((float)C);
 #pragma unroll
   for (int i = 0; i < kNDPlanLanes; ++i) {
     if (64 * i >= a.num_reqs) break;
-    nch[i] = max(1, (st[i] + C - 1) / C);
-    cls[i] = kNDClasses - 1 - min(kNDClasses - 1, (st[i] * kNDClasses - 1) / (nch[i] * C));
+    nch[i] = nd_chunks(st[i], C, by_C);
+    const float eighths = (float)st[i] * __builtin_amdgcn_rcpf((float)nch[i]) * by_C * kNDClasses;
+    cls[i] = kNDClasses - 1 - min(kNDClasses - 1, (int)eighths);
     const int split = nch[i] > 1 ? rb[i] * nch[i] : 0;
     const int bincl = CHUNK ? nib_scan(rb[i]) : 0, pincl = nib_scan(split);
     bex[i] = CHUNK ? blocks + bincl - rb[i] : 64 * i + lane;
@@ -159,6 +174,7 @@ __device__ __forceinline__ NibDecodePlan nd_plan(const NibDecodeArgs& a, int ite
         P.r = __builtin_amdgcn_readlane(idx[i], ln);
         P.n = __builtin_amdgcn_readlane(n[i], ln);
         P.Q = __builtin_amdgcn_readlane(Q[i], ln);
+        P.q0 = __builtin_amdgcn_readlane(q0[i], ln);
         P.nch = __builtin_amdgcn_readlane(nch[i], ln);
         const int local = it - __builtin_amdgcn_readlane(ex, ln);
         P.rb = CHUNK ? local / P.nch : 0;
@@ -196,7 +212,7 @@ __global__ __launch_bounds__(kNDThreads, 2) void nibble_decode_kernel(NibDecodeA
   if (tid == 0 && h == 0 && P.c == 0 && P.rb == 0 &&
       (P.n > a.max_seq || (CHUNK && (P.Q > a.max_q || p0 < 0))))
     atomicOr(a.err, TTKV_ERR_SEQ_LEN);
-  const int64_t q0 = a.qsl[P.r];
+  const int64_t q0 = P.q0;
   const int row0 = P.rb * kNDRows, nrow = min(kNDRows, P.rows - row0);  // the block's rows
   // row `r` of the block in the query and the output
   auto row_at = [&](int r, int64_t stride) -> int64_t {
