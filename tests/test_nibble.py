@@ -206,6 +206,8 @@ def test_a_workspace_for_the_largest_batch_serves_smaller_ones():
         a = L.ttkv_nibble_prefill_workspace_bytes(H, H * G, R, q, n)
         assert 256 <= a <= L.ttkv_nibble_prefill_workspace_bytes(H, H * G, r2, q2, max(n2, q2))
         assert a <= 64 << 20
+    big = 2 ** 31 - 1
+    assert 0 < L.ttkv_nibble_prefill_workspace_bytes(16384, 16384, big, big, big) <= 64 << 20
 
 
 def _rotary(sections=(16, 24, 24), **kw):

@@ -383,6 +383,18 @@ def test_prefill_picked_rows_and_empty_chunks():
     assert bool((out[20:21] == 5).all())
 
 
+@pytest.mark.parametrize("lens,counts", [([300, 4000], [20, 3]), ([300, 4000], [200, 90])])
+def test_prefill_of_a_row_picked_twice(lens, counts):
+    st = Store(lens, 2, seed=33)
+    q = torch.randn(sum(counts), 8, D, generator=_gen(34)).half().cuda()
+    want, err, qsl = _prefill(st, q, counts)
+    got, err2, _ = _prefill(st, q, counts, req_index=_i32([1, 0, 1]))
+    assert err == 0 and err2 == 0
+    for r in range(2):
+        s = slice(qsl[r], qsl[r + 1])
+        _close(got[s], q[s].cpu(), *st.kv(r), SCALE, r)
+
+
 def test_prefill_refuses_on_the_device():
     """Fewer keys than queries, a block outside the cache, a count past max_q_len."""
     lens, counts = [100, 30, 200, 64], [10, 31, 20, 12]
@@ -841,3 +853,40 @@ def test_captured_step_replays():
         free.copy_(torch.cat([free[taken:], free[:taken]]))
         st, qq, _, _ = _decode_args(40 + t, lens=(100, 50))
         _decode(st, qq)
+
+
+def test_captured_prefill_replays():
+    """Chunks in a graph, with lengths that change on the device between the replays and eager calls of
+    both reads on the same workspace."""
+    st = Store([2000, 700], 2, seed=36)
+    qsl = _i32([0, 200, 290])
+    q = torch.zeros(290, 8, D, dtype=torch.float16, device="cuda")
+    seq = st.seq.clone()
+    ws = kernels.nibble_prefill_workspace(st.lay, 8, 2, 200, 2000, "cuda")
+    other = kernels.nibble_prefill_workspace(st.lay, 8, 2, 200, 2000, "cuda")
+    err, g = _err(), _gen(37)
+
+    def call(w):
+        return kernels.nibble_prefill_paged(st.lay, q, st.page, st.block, st.bt, seq, qsl, 200, 2000,
+                                            SCALE, workspace=w, error_word=err)
+
+    call(ws)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = call(ws)
+    for lens in ([2000, 700], [200, 90], [1111, 699], [2000, 90]):
+        q.copy_(torch.randn(290, 8, D, generator=g))
+        seq.copy_(_i32(lens))
+        out.fill_(9)
+        graph.replay()
+        torch.cuda.synchronize()
+        got = out.clone()
+        assert torch.equal(got, call(other)) and int(err) == 0
+        for r, s in ((0, slice(0, 200)), (1, slice(200, 290))):
+            K, V = st.kv(r)
+            _close(got[s], q[s].cpu(), K[:lens[r]], V[:lens[r]], SCALE, (lens, r))
+        assert torch.equal(call(ws), got)
+        kernels.nibble_decode_paged(st.lay, q, st.page, st.block, st.bt, seq, qsl[:2], 2000, SCALE,
+                                    workspace=ws, error_word=err)
+        assert not bool(ws[:65536].any())

@@ -569,7 +569,7 @@ int64_t nibble_decode_workspace_bytes(int H, int HQ, int num_reqs, int max_seq) 
 //     24.5; 4 x 32 over 2,500 26.3, 25.6; 5 x 20 over 4,000 35.3, 30.6; two rounds: 30 x 16 over 300 25.6, 16.0
 bool nibble_short_applies(int H, int HQ, int num_reqs, int max_q, int max_seq) {
   const int64_t rows = (int64_t)max_q * (HQ / H);
-  if (rows > kNDShortRows || H * nd_blocks((int)rows) > kMaxCounters) return false;
+  if (rows > kNDShortRows || (int64_t)H * nd_blocks((int)rows) > kMaxCounters) return false;
   const int64_t blocks = nd_blocks((int)rows), steps = (max_seq + kNDStep - 1) / kNDStep;
   const int64_t items = (int64_t)num_reqs * H * blocks;
   if (blocks == 1) return true;
@@ -580,7 +580,8 @@ bool nibble_short_applies(int H, int HQ, int num_reqs, int max_q, int max_seq) {
 // Bytes of partial results of such a chunk call at most, growing with every argument.
 int64_t nibble_short_part_bytes(int H, int HQ, int num_reqs, int max_q, int max_seq) {
   const int rows = (int)std::min<int64_t>((int64_t)max_q * (HQ / H), kNDShortRows);
-  const int64_t pairs = std::min<int64_t>((int64_t)num_reqs * H * nd_blocks(rows), kMaxCounters);
+  const int64_t pairs = std::min<int64_t>(
+      std::min<int64_t>(num_reqs, kMaxCounters) * std::min(H, kMaxCounters) * nd_blocks(rows), kMaxCounters);
   return nd_parts(pairs, max_seq) * std::min(rows, kNDRows) * (kD + 2) * 4;
 }
 

@@ -776,7 +776,8 @@ static NibPrefillSlice np_slice(int H, int HQ, int num_reqs, int max_q, int max_
 }
 
 static int64_t np_part_rows(int HQ, int reqs, int max_q, int max_seq) {
-  return std::min(kNPPartRows, np_max_parts(max_seq) * reqs * std::min<int64_t>(max_q, kNPPartRows) * HQ);
+  return std::min(kNPPartRows, np_max_parts(max_seq) * std::min<int64_t>(reqs, kNPPartRows) *
+                                   std::min<int64_t>(max_q, kNPPartRows) * HQ);
 }
 
 static int64_t np_join_bytes(const NibPrefillSlice& s) {
@@ -789,8 +790,9 @@ static int64_t np_join_bytes(const NibPrefillSlice& s) {
 int64_t nibble_prefill_workspace_bytes(int H, int HQ, int num_reqs, int max_q, int max_seq) {
   if (num_reqs == 0 || max_q == 0) return 256;
   const int64_t rows = (int64_t)max_q * (HQ / H), rw = kNPWaves * 16;
-  const int64_t blocks = std::min<int64_t>(kCounterBytes / (rw / kNPJoinRows),
-                                           std::min<int64_t>((rows + rw - 1) / rw, kCounterBytes) * H * num_reqs);
+  int64_t blocks = 1;
+  for (int64_t x : {(rows + rw - 1) / rw, (int64_t)H, (int64_t)num_reqs})
+    blocks = std::min(blocks * std::min(x, kCounterBytes), kCounterBytes / (rw / kNPJoinRows));
   const int64_t joins = (blocks * (int64_t)sizeof(NibPrefillJoin) + 255) / 256 * 256;
   const int64_t parts = np_part_rows(HQ, num_reqs, max_q, max_seq) * (kD + 2) * 4;
   return kCounterBytes + std::max(joins + parts, nibble_short_part_bytes(H, HQ, num_reqs, max_q, max_seq));
