@@ -20,8 +20,8 @@
 //     stands, and a lane's 16 value code bytes per tile are its A operand of all eight (a dim pair of
 //     each group, four tokens). The result's column is the row again, so the rescale is a lane's factor.
 // Bytes per step 4,608; the two register sets keep the next step's loads in flight. Bound by memory: 8 x
-// 14,402 tokens of 8 heads, 133 MB, 30.6 us, 4.35 TB/s (a copy reaches 4.8); the loads alone took 26 us
-// of a profiled 33. 61 requests of 70 to 2,900 tokens 28.3 us for 98 MB; one of 1,082 tokens 9 us, the
+// 14,402 tokens of 8 heads, 133 MB, 30.2 us, 4.4 TB/s (a copy reaches 4.8); the loads alone took 26 us
+// of a profiled 33. 61 requests of 70 to 2,900 tokens 27.8 us for 98 MB; one of 1,082 tokens 9 us, the
 // chain of plan, block ids, codes, hand-off and join.
 #include <math.h>
 
