@@ -25,6 +25,8 @@
 // chain of plan, block ids, codes, hand-off and join.
 #include <math.h>
 
+#include <type_traits>
+
 #include "ttkv_host.h"
 #include "ttkv_nibble.h"
 
@@ -454,71 +456,95 @@ __global__ __launch_bounds__(kNDThreads, 2) void nibble_decode_kernel(NibDecodeA
   __syncthreads();
   if (!last_sh) return;
   // Half a wave takes a row, a lane four dims of it; lane % 32 first holds a chunk's maximum and sum.
-  // All of a wave's rows are under way together.
+  // All of a wave's rows are under way together. With four rows or less and more chunks than a half wave
+  // has in flight, 2, 4 or 8 of them share a row's chunks and are joined in LDS (1 x 60,000 tokens of one
+  // head: 22.2 us, 18.9 so; 4 x 9,000 of 8: 20.7, 19.7).
   constexpr int ROWS = kNDRows / (2 * kNDWaves);  // per half wave
   const int c32 = lane & 31, lead = lane & 32;
   const int64_t part0 = (int64_t)P.part * a.H + h;
-  float mm[ROWS], ll[ROWS];
-  float4v o[ROWS];
-  int row[ROWS];
-#pragma unroll
-  for (int k = 0; k < ROWS; ++k) {
-    row[k] = min(2 * (wv + kNDWaves * k) + (lane >> 5), nrow - 1);
-    mm[k] = kNDNone;
-    ll[k] = 0.f;
-    o[k] = float4v{};
-  }
   constexpr int AHEAD = 8;  // chunks of every row in flight
-  for (int c0 = 0; c0 < P.nch; c0 += 32) {
-    const int nb = min(32, P.nch - c0);
-    float4v x[ROWS][AHEAD];
-    auto fetch = [&](int j) {
+  // log2 of the half waves per row
+  const int share = min(nrow > 4 ? 0 : nrow > 2 ? 1 : nrow > 1 ? 2 : 3,
+                        P.nch <= AHEAD ? 0 : P.nch <= 2 * AHEAD ? 1 : P.nch <= 4 * AHEAD ? 2 : 3);
+  auto join = [&](auto shared_c) {
+    constexpr bool SHARED = decltype(shared_c)::value;
+    constexpr int K = SHARED ? 1 : ROWS;
+    const int half = 2 * wv + (lane >> 5), sh = SHARED ? share : 0;
+    const int sub = SHARED ? half & ((1 << share) - 1) : 0;
+    // by half waves or, unshared, by waves (one of whose rows may be the last one again)
+    auto on = [&](int k) { return SHARED ? half >> sh < nrow : 2 * (wv + kNDWaves * k) < nrow; };
+    float mm[K], ll[K];
+    float4v o[K];
+    int row[K];
 #pragma unroll
-      for (int k = 0; k < ROWS; ++k)
-        if (2 * (wv + kNDWaves * k) < nrow)
-#pragma unroll
-          for (int u = 0; u < AHEAD; ++u)
-            if (j + u < nb)
-              x[k][u] = ld_agent16(
-                  a.ws_o, a.o_bytes,
-                  (uint32_t)((((part0 + (int64_t)(c0 + j + u) * a.H) * PR + row[k]) * kD + 4 * c32) * 4));
-    };
-    float2v ml[ROWS];
-    float wc[ROWS];
-#pragma unroll
-    for (int k = 0; k < ROWS; ++k)
-      ml[k] = ld_agent2(a.ws_ml + ((part0 + (int64_t)(c0 + min(c32, nb - 1)) * a.H) * PR + row[k]) * 2);
-    fetch(0);  // (a round trip that the weights' does not come before)
-#pragma unroll
-    for (int k = 0; k < ROWS; ++k) {
-      float x0, x1;
-      swap16(row_max(c32 < nb ? ml[k][0] : kNDNone), x0, x1);
-      const float mn = fmaxf(mm[k], fmaxf(x0, x1));
-      const float keep = exp2f(mm[k] - mn);
-      wc[k] = c32 < nb ? exp2f(ml[k][0] - mn) : 0.f;
-      swap16(row_sum(c32 < nb ? ml[k][1] * wc[k] : 0.f), x0, x1);
-      ll[k] = ll[k] * keep + x0 + x1;
-      o[k] *= keep;
-      mm[k] = mn;
+    for (int k = 0; k < K; ++k) {
+      row[k] = min((half >> sh) + 2 * kNDWaves * k, nrow - 1);
+      mm[k] = kNDNone;
+      ll[k] = 0.f;
+      o[k] = float4v{};
     }
-    for (int j = 0; j < nb; j += AHEAD) {
-      if (j) fetch(j);
+    for (int c0 = 0; c0 < P.nch; c0 += 32) {
+      const int nb = min(32, P.nch - c0);
+      float4v x[K][AHEAD];
+      auto fetch = [&](int j) {  // chunks j + sub, j + sub + 2^sh, ...
 #pragma unroll
-      for (int u = 0; u < AHEAD; ++u)
-        if (j + u < nb)
+        for (int k = 0; k < K; ++k)
+          if (on(k))
 #pragma unroll
-          for (int k = 0; k < ROWS; ++k) {
-            const float w = __shfl(wc[k], lead + j + u);
-            if (2 * (wv + kNDWaves * k) < nrow) o[k] += x[k][u] * w;
-          }
+            for (int u = 0; u < AHEAD; ++u) {
+              const int c = j + sub + (u << sh);
+              if (c < nb)
+                x[k][u] = ld_agent16(
+                    a.ws_o, a.o_bytes,
+                    (uint32_t)((((part0 + (int64_t)(c0 + c) * a.H) * PR + row[k]) * kD + 4 * c32) * 4));
+            }
+      };
+      float2v ml[K];
+      float wc[K];
+#pragma unroll
+      for (int k = 0; k < K; ++k)
+        ml[k] = ld_agent2(a.ws_ml + ((part0 + (int64_t)(c0 + min(c32, nb - 1)) * a.H) * PR + row[k]) * 2);
+      fetch(0);  // (a round trip that the weights' does not come before)
+#pragma unroll
+      for (int k = 0; k < K; ++k) {
+        float x0, x1;
+        swap16(row_max(c32 < nb ? ml[k][0] : kNDNone), x0, x1);
+        const float mn = fmaxf(mm[k], fmaxf(x0, x1));
+        const float keep = exp2f(mm[k] - mn);
+        wc[k] = c32 < nb ? exp2f(ml[k][0] - mn) : 0.f;
+        swap16(row_sum(c32 < nb ? ml[k][1] * wc[k] : 0.f), x0, x1);
+        ll[k] = ll[k] * keep + x0 + x1;
+        o[k] *= keep;
+        mm[k] = mn;
+      }
+      for (int j = 0; j < nb; j += AHEAD << sh) {
+        if (j) fetch(j);
+#pragma unroll
+        for (int u = 0; u < AHEAD; ++u) {
+          const int c = j + sub + (u << sh);
+          if (SHARED || c < nb)
+#pragma unroll
+            for (int k = 0; k < K; ++k) {
+              const float w = __shfl(wc[k], lead + (c & 31));
+              if (on(k) && c < nb) o[k] += x[k][u] * w;
+            }
+        }
+      }
     }
-  }
+    if (SHARED) {
+      float* sums = &red_o[0][0][0];  // [half wave][kD]
+      *(float4v*)(sums + half * kD + 4 * c32) = o[0];
+      __syncthreads();
+      if (sub) return;
+      for (int u = 1; u < 1 << sh; ++u) o[0] += *(const float4v*)(sums + (half + u) * kD + 4 * c32);
+    }
 #pragma unroll
-  for (int k = 0; k < ROWS; ++k) {
-    const int r = 2 * (wv + kNDWaves * k) + (lane >> 5);
-    if (r < nrow)
-      store_act4(a.out, a.out_dtype, row_at(r, a.out_row_stride) + 4 * c32, o[k] * (1.f / ll[k]), true);
-  }
+    for (int k = 0; k < K; ++k)
+      if ((half >> sh) + 2 * kNDWaves * k < nrow)
+        store_act4(a.out, a.out_dtype, row_at(row[k], a.out_row_stride) + 4 * c32, o[k] * (1.f / ll[k]), true);
+  };
+  if (share) join(std::true_type{});
+  else join(std::false_type{});
 }
 
 // The plan's item target: two workgroups per CU. A third would fit beside them, but shorter chunks
