@@ -521,6 +521,40 @@ def test_prefill_batches_write_every_row(H, HQ, lens, counts):
         _close(out[s], q[s], *st.kv(r), SCALE, r)
 
 
+@pytest.mark.parametrize("R,H,HQ,most,longest", [
+    (70, 4, 16, 7, 300), (33, 8, 24, 10, 90), (300, 1, 5, 5, 70), (140, 2, 4, 16, 33), (3, 8, 32, 8, 26000)])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_prefill_of_many_short_chunks(R, H, HQ, most, longest, dtype):
+    """Chunks of 17 to 32 rows per KV head in batches large enough for two groups of 16 rows to share a
+    block, ragged, and a NaN in a value that only the queries at or after it may see."""
+    g = _gen(R + most)
+    counts = [most] + [int(torch.randint(0, most + 1, (1,), generator=g)) for _ in range(R - 1)]
+    lens = [longest] + [c + int(torch.randint(0, longest - most, (1,), generator=g)) for c in counts[1:]]
+    st = Store(lens, H, seed=40, dtype=dtype)
+    q = torch.randn(sum(counts), HQ, D, generator=g).to(dtype)
+    out = torch.full((sum(counts), HQ, D), float("nan"), dtype=dtype, device="cuda")
+    _, err, qsl = _prefill(st, q.cuda(), counts, out=out)
+    assert err == 0 and not bool(torch.isnan(out).any())
+    for r in {0, 1, R // 2, R - 1}:
+        s = slice(qsl[r], qsl[r + 1])
+        if counts[r]:
+            _close(out[s], q[s], *st.kv(r), SCALE, (r, lens[r], counts[r]))
+    k, v = st.k.clone(), st.v.clone()
+    at = lens[0] - most + 2                       # seen by the queries from 2 on
+    v[at, 0, 40] = float("nan")
+    page = st.page.clone()
+    kernels.nibble_write_paged(st.lay, k.cuda(), v.cuda(), st.slots.cuda(), page)
+    bad = kernels.nibble_prefill_paged(st.lay, q.cuda(), page, st.block, st.bt, st.seq, _i32(qsl), most,
+                                       max(lens), SCALE)
+    G = HQ // H
+    nan = torch.isnan(bad[:most, :G])
+    assert bool(nan[2:, :, 32:64].all()) and not bool(nan[:2].any())
+    assert not bool(nan[:, :, :32].any()) and not bool(nan[:, :, 64:].any())
+    nan = torch.isnan(bad)
+    nan[:most, :G] = False
+    assert not bool(nan.any())
+
+
 def test_prefill_workspace_serves_other_shapes():
     """One workspace for prefill calls of different shapes and for decode calls in turn."""
     shapes = [([5000, 300], 2, 8, [70, 20]), ([900, 64, 30], 1, 4, [3, 1, 2]), ([1200], 4, 12, [400])]

@@ -40,7 +40,7 @@ constexpr int kNDClasses = 8;          // of chunk lengths, for the items' order
 constexpr int kNDShortRows = 256;      // rows of a chunk that may come here
 constexpr int64_t kNDShortWork = 17000;  // and steps of all its blocks,
 constexpr int64_t kNDFewWork = 24000;    // where they are few
-constexpr int kNDLongSteps = 32;       // steps from which a second round of items is worth it
+constexpr int64_t kNDWideWork = 36000;   // from which two groups of 16 rows share a block
 constexpr float kNDMost = 2048.f;      // a lane's sum of eight softmax weights before a rescale
 constexpr float kNDNone = -1e30f;      // a maximum before the first visible key
 constexpr int kNDRows = 16;            // rows of a block: a matrix product's columns
@@ -86,7 +86,8 @@ __device__ __forceinline__ int nd_chunks(int steps, int C, float by_C) {
   return max(1, (int)((float)(steps + C - 1) * by_C));
 }
 
-template <bool CHUNK>
+// RB: rows of a block.
+template <bool CHUNK, int RB>
 __device__ __forceinline__ NibDecodePlan nd_plan(const NibDecodeArgs& a, int item) {
   const int lane = threadIdx.x & 63;
   int idx[kNDPlanLanes], n[kNDPlanLanes], q0[kNDPlanLanes], Q[kNDPlanLanes];
@@ -109,7 +110,7 @@ __device__ __forceinline__ NibDecodePlan nd_plan(const NibDecodeArgs& a, int ite
     const int nn = min(max(n[i], 0), a.max_seq);
     st[i] = (nn + kNDStep - 1) / kNDStep;
     if (CHUNK && nn < Q[i]) st[i] = 1;
-    rb[i] = CHUNK ? (min(max(Q[i], 0), a.max_q) * a.G + kNDRows - 1) / kNDRows : Q[i];
+    rb[i] = CHUNK ? (min(max(Q[i], 0), a.max_q) * a.G + RB - 1) / RB : Q[i];
     total += st[i] * rb[i];
     longest = max(longest, st[i]);
     whole += rb[i];
@@ -199,14 +200,17 @@ struct NibStep {
   u32x4 vp[2][2];
 };
 
-template <int QDT, bool CHUNK>
+// RG: groups of 16 rows that a block has, one column of a product each.
+template <int QDT, bool CHUNK, int RG>
 __global__ __launch_bounds__(kNDThreads, 2) void nibble_decode_kernel(NibDecodeArgs a) {
-  __shared__ float red_o[kNDWaves][kNDRows][kD];
-  __shared__ float red_m[kNDWaves][kNDRows], red_l[kNDWaves][kNDRows];
+  constexpr int RB = kNDRows * RG;
+  extern __shared__ __align__(16) float red_all[];  // [waves][RB][kD]: the waves' results, then the join's
+  float(*red_o)[RB][kD] = (float(*)[RB][kD])red_all;
+  __shared__ float red_m[kNDWaves][RB], red_l[kNDWaves][RB];
   __shared__ int last_sh;
   const int tid = threadIdx.x, lane = tid & 63;
   const int wv = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const NibDecodePlan P = nd_plan<CHUNK>(a, blockIdx.x);
+  const NibDecodePlan P = nd_plan<CHUNK, RB>(a, blockIdx.x);
   if (P.none) return;
   const int h = P.h, G = a.G;
   const int n = min(max(P.n, 0), a.max_seq);
@@ -215,7 +219,7 @@ __global__ __launch_bounds__(kNDThreads, 2) void nibble_decode_kernel(NibDecodeA
       (P.n > a.max_seq || (CHUNK && (P.Q > a.max_q || p0 < 0))))
     atomicOr(a.err, TTKV_ERR_SEQ_LEN);
   const int64_t q0 = P.q0;
-  const int row0 = P.rb * kNDRows, nrow = min(kNDRows, P.rows - row0);  // the block's rows
+  const int row0 = P.rb * RB, nrow = min(RB, P.rows - row0);  // the block's rows
   // row `r` of the block in the query and the output
   auto row_at = [&](int r, int64_t stride) -> int64_t {
     const int row = row0 + r, j = CHUNK ? row / G : 0;
@@ -228,16 +232,25 @@ __global__ __launch_bounds__(kNDThreads, 2) void nibble_decode_kernel(NibDecodeA
   }
   const int col = lane & 15, q4 = lane >> 4;
 
-  // The queries, row `col`, as the B operand of the four score products
-  half8 qf[4];
-  float qs, m = kNDNone, l = 0.f;
-  const NibRow qrow = nib_load_row(a.q + row_at(min(col, nrow - 1), a.q_row_stride), q4);
-  nib_query<QDT>(qrow, a.scale_log2, col < nrow, qf, qs);
-  const int lim = CHUNK ? p0 + (row0 + min(col, nrow - 1)) / G : p0;  // last key the lane's row sees
-  const int see_min = CHUNK ? p0 + row0 / G : p0;                     // and every row
-  float4v acc[8];  // [group][dim of the pair]: dims 32 g + 8 q4 + 2 i + b of the lane's row
+  // The queries, row 16 r + `col` of group r, as the B operand of the four score products
+  half8 qf[RG][4];
+  float qs[RG], m[RG], l[RG];
+  int lim[RG];  // last key the lane's row sees
 #pragma unroll
-  for (int i = 0; i < 8; ++i) acc[i] = float4v{};
+  for (int r = 0; r < RG; ++r) {
+    const int row = min(kNDRows * r + col, nrow - 1);
+    const NibRow qrow = nib_load_row(a.q + row_at(row, a.q_row_stride), q4);
+    nib_query<QDT>(qrow, a.scale_log2, kNDRows * r + col < nrow, qf[r], qs[r]);
+    m[r] = kNDNone;
+    l[r] = 0.f;
+    lim[r] = CHUNK ? p0 + (row0 + row) / G : p0;
+  }
+  const int see_min = CHUNK ? p0 + row0 / G : p0;                     // and every row
+  float4v acc[RG][8];  // [group][dim of the pair]: dims 32 g + 8 q4 + 2 i + b of the lane's rows
+#pragma unroll
+  for (int r = 0; r < RG; ++r)
+#pragma unroll
+    for (int i = 0; i < 8; ++i) acc[r][i] = float4v{};
 
   const int steps = (CHUNK ? p0 + (row0 + nrow - 1) / G : p0) / kNDStep + 1;
   // the block's steps in equal parts
@@ -272,10 +285,11 @@ __global__ __launch_bounds__(kNDThreads, 2) void nibble_decode_kernel(NibDecodeA
     }
   };
   auto step = [&](int s, NibStep& x) {
-    float4v sc[2];
+    float4v sc[RG][2];
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
-      sc[t] = float4v{};
+#pragma unroll
+      for (int r = 0; r < RG; ++r) sc[r][t] = float4v{};
 #pragma unroll
       for (int g = 0; g < 4; ++g) {
         const half2v zz = nib_biased(x.kp[t][g >> 1], masks), sg = nib_scales(x.kp[t][g >> 1]);
@@ -287,7 +301,9 @@ __global__ __launch_bounds__(kNDThreads, 2) void nibble_decode_kernel(NibDecodeA
           kf[2 * j] = v[0];
           kf[2 * j + 1] = v[1];
         }
-        sc[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qf[g], sc[t], 0, 0, 0);
+#pragma unroll
+        for (int r = 0; r < RG; ++r)
+          sc[r][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qf[r][g], sc[r][t], 0, 0, 0);
       }
     }
     const int tok = s * kNDStep + 4 * q4;
@@ -301,7 +317,9 @@ __global__ __launch_bounds__(kNDThreads, 2) void nibble_decode_kernel(NibDecodeA
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const int tk = tok + 16 * t + i;
-          if (tk > lim) sc[t][i] = -INFINITY;
+#pragma unroll
+          for (int r = 0; r < RG; ++r)
+            if (tk > lim[r]) sc[r][t][i] = -INFINITY;
           const uint32_t keep = i & 1 ? 0x0000ffffu : 0xffff0000u;
 #pragma unroll
           for (int g = 0; g < 4; ++g) {
@@ -315,38 +333,47 @@ __global__ __launch_bounds__(kNDThreads, 2) void nibble_decode_kernel(NibDecodeA
     }
     // Weights against the maximum as it stands. It has to move only where a lane's sum of eight
     // exceeds 2^11 (or is NaN): the scores' own maximum is taken in that case alone.
-    half8 pf;
-    float sum;
-    auto weights = [&]() {
-      sum = 0.f;
+    half8 pf[RG];
+    float sum[RG];
+    auto weights = [&](int r) {
+      sum[r] = 0.f;
 #pragma unroll
       for (int t = 0; t < 2; ++t)
 #pragma unroll
         for (int i = 0; i < 4; i += 2) {
           // the one rounding on the way to the output; the sum takes the rounded weights
-          const half2v p = {(_Float16)fast_exp2(fmaf(sc[t][i], qs, -m)),
-                            (_Float16)fast_exp2(fmaf(sc[t][i + 1], qs, -m))};
-          sum = __builtin_amdgcn_fdot2(p, half2v{(_Float16)1.f, (_Float16)1.f}, sum, false);
-          pf[4 * t + i] = p[0];
-          pf[4 * t + i + 1] = p[1];
+          const half2v p = {(_Float16)fast_exp2(fmaf(sc[r][t][i], qs[r], -m[r])),
+                            (_Float16)fast_exp2(fmaf(sc[r][t][i + 1], qs[r], -m[r]))};
+          sum[r] = __builtin_amdgcn_fdot2(p, half2v{(_Float16)1.f, (_Float16)1.f}, sum[r], false);
+          pf[r][4 * t + i] = p[0];
+          pf[r][4 * t + i + 1] = p[1];
         }
     };
-    weights();
-    if (__builtin_amdgcn_ballot_w64(!(sum <= kNDMost))) {
-      float mt = -INFINITY;
+    bool fits = true;
 #pragma unroll
-      for (int t = 0; t < 2; ++t)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) mt = fmaxf(mt, sc[t][i]);
-      const float mn = fmaxf(m, cross_row_max(mt * qs));
-      const float f = exp2f(m - mn);
-      m = mn;
-      l *= f;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) acc[i] *= f;
-      weights();
+    for (int r = 0; r < RG; ++r) {
+      weights(r);
+      fits &= sum[r] <= kNDMost;
     }
-    l += sum;
+    if (__builtin_amdgcn_ballot_w64(!fits)) {
+#pragma unroll
+      for (int r = 0; r < RG; ++r) {
+        float mt = -INFINITY;
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) mt = fmaxf(mt, sc[r][t][i]);
+        const float mn = fmaxf(m[r], cross_row_max(mt * qs[r]));
+        const float f = exp2f(m[r] - mn);
+        m[r] = mn;
+        l[r] *= f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) acc[r][i] *= f;
+        weights(r);
+      }
+    }
+#pragma unroll
+    for (int r = 0; r < RG; ++r) l[r] += sum[r];
 #pragma unroll
     for (int quad = 0; quad < 2; ++quad)
 #pragma unroll
@@ -368,7 +395,10 @@ __global__ __launch_bounds__(kNDThreads, 2) void nibble_decode_kernel(NibDecodeA
           }
 #pragma unroll
         for (int b = 0; b < 2; ++b)
-          acc[2 * g + b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf[b], pf, acc[2 * g + b], 0, 0, 0);
+#pragma unroll
+          for (int r = 0; r < RG; ++r)
+            acc[r][2 * g + b] =
+                __builtin_amdgcn_mfma_f32_16x16x32_f16(vf[b], pf[r], acc[r][2 * g + b], 0, 0, 0);
       }
     if (CHUNK && __builtin_amdgcn_ballot_w64(note != 0)) {
       for (int k = 0; k < kNDStep; ++k) {  // token 16 t + 4 q + i
@@ -376,8 +406,10 @@ __global__ __launch_bounds__(kNDThreads, 2) void nibble_decode_kernel(NibDecodeA
         const int groups = (of >> (16 * (k >> 4) + 4 * (k & 3))) & 15;
         if (!groups) continue;
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-          if ((groups >> (i >> 1) & 1) && s * kNDStep + k <= lim) acc[i] += NAN;
+        for (int r = 0; r < RG; ++r)
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            if ((groups >> (i >> 1) & 1) && s * kNDStep + k <= lim[r]) acc[r][i] += NAN;
       }
     }
   };
@@ -401,26 +433,34 @@ __global__ __launch_bounds__(kNDThreads, 2) void nibble_decode_kernel(NibDecodeA
     s += kNDWaves * 64;
   }
   if (bad && lane == 0) atomicOr(a.err, TTKV_ERR_BAD_BLOCK);
-  l = bad ? NAN : cross_row_sum(l);
+#pragma unroll
+  for (int r = 0; r < RG; ++r) l[r] = bad ? NAN : cross_row_sum(l[r]);
 
   // ---- the four waves' results, joined in LDS
   if (q4 == 0) {
-    red_m[wv][col] = m;
-    red_l[wv][col] = l;
+#pragma unroll
+    for (int r = 0; r < RG; ++r) {
+      red_m[wv][kNDRows * r + col] = m[r];
+      red_l[wv][kNDRows * r + col] = l[r];
+    }
   }
   __syncthreads();
-  float M = kNDNone;
 #pragma unroll
-  for (int w = 0; w < kNDWaves; ++w) M = fmaxf(M, red_m[w][col]);
-  const float f = exp2f(m - M);
-  if (col < nrow) {
+  for (int r = 0; r < RG; ++r) {
+    const int row = kNDRows * r + col;
+    float M = kNDNone;
 #pragma unroll
-    for (int g = 0; g < 4; ++g)
+    for (int w = 0; w < kNDWaves; ++w) M = fmaxf(M, red_m[w][row]);
+    const float f = exp2f(m[r] - M);
+    if (row < nrow) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float2v o = {acc[2 * g][i] * f, acc[2 * g + 1][i] * f};
-        *(float2v*)&red_o[wv][col][32 * g + 8 * q4 + 2 * i] = o;
-      }
+      for (int g = 0; g < 4; ++g)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float2v o = {acc[r][2 * g][i] * f, acc[r][2 * g + 1][i] * f};
+          *(float2v*)&red_o[wv][row][32 * g + 8 * q4 + 2 * i] = o;
+        }
+    }
   }
   __syncthreads();
   const int PR = a.part_rows;
@@ -459,7 +499,7 @@ __global__ __launch_bounds__(kNDThreads, 2) void nibble_decode_kernel(NibDecodeA
   // All of a wave's rows are under way together. With four rows or less and more chunks than a half wave
   // has in flight, 2, 4 or 8 of them share a row's chunks and are joined in LDS (1 x 60,000 tokens of one
   // head: 22.2 us, 18.9 so; 4 x 9,000 of 8: 20.7, 19.7).
-  constexpr int ROWS = kNDRows / (2 * kNDWaves);  // per half wave
+  constexpr int ROWS = RB / (2 * kNDWaves);  // per half wave
   const int c32 = lane & 31, lead = lane & 32;
   const int64_t part0 = (int64_t)P.part * a.H + h;
   // log2 of the half waves per row
@@ -470,7 +510,7 @@ __global__ __launch_bounds__(kNDThreads, 2) void nibble_decode_kernel(NibDecodeA
     constexpr int K = decltype(rows_c)::value;
     // chunks of every row in flight (one row: 8 heads per KV head, 2 x 12,000 tokens: 20.4 us with 8, 19.3;
     // shared, 4 x 9,000: 18.6 with 8, 19.1)
-    constexpr int AHEAD = K == 1 && !SHARED ? 16 : 8;
+    constexpr int AHEAD = K == 1 && !SHARED ? 16 : K == 4 ? 4 : 8;
     const int half = 2 * wv + (lane >> 5), sh = SHARED ? share : 0;
     const int sub = SHARED ? half & ((1 << share) - 1) : 0;
     // by half waves or, unshared, by waves (one of whose rows may be the last one again)
@@ -534,7 +574,7 @@ __global__ __launch_bounds__(kNDThreads, 2) void nibble_decode_kernel(NibDecodeA
       }
     }
     if (SHARED) {
-      float* sums = &red_o[0][0][0];  // [half wave][kD]
+      float* sums = red_all;  // [half wave][kD]
       *(float4v*)(sums + half * kD + 4 * c32) = o[0];
       __syncthreads();
       if (sub) return;
@@ -574,35 +614,44 @@ static int64_t nd_parts(int64_t pairs, int max_seq) {
   return most <= 1 ? 0 : std::min<int64_t>(2 * nd_target(), pairs * most);
 }
 
-static int nd_blocks(int rows) { return (rows + kNDRows - 1) / kNDRows; }
+static int nd_blocks(int rows, int groups) {
+  return (rows + kNDRows * groups - 1) / (kNDRows * groups);
+}
 
-static int64_t nd_workspace(int H, int num_reqs, int max_seq, int rows) {
-  if (num_reqs == 0 || H > kMaxCounters) return 256;
-  const int64_t pairs = (int64_t)nd_slice(H, nd_blocks(rows), num_reqs) * H * nd_blocks(rows);
-  return kCounterBytes + nd_parts(pairs, max_seq) * std::min(rows, kNDRows) * (kD + 2) * 4;
+// Groups of 16 rows per block: one, or two where a chunk has 17 to 32 rows and the call is large; both
+// of a block's groups share the dequantised keys and values, but a small call waits longer for its
+// larger join (us, with one and two: 60 x 8 queries of four heads per KV head over 1,500 keys 49.5, 35.5;
+// 16 x 8 over 6,000 48.0, 40.0; 60 x 8 over 300 26.4, 18.5; 4 x 8 over 14,000 33.3, 34.6; 30 x 8 over 100
+// 11.2, 12.3. Longer chunks gain less: 16 x 16 over 2,000 32.3 in the prefill kernel, 30.2).
+static int nd_groups(int H, int num_reqs, int rows, int max_seq) {
+  if (rows <= kNDRows || rows > 2 * kNDRows) return 1;
+  const int64_t items = (int64_t)num_reqs * H * 2, steps = (max_seq + kNDStep - 1) / kNDStep;
+  return items > nd_target() || items * steps > kNDWideWork ? 2 : 1;
 }
 
 int64_t nibble_decode_workspace_bytes(int H, int HQ, int num_reqs, int max_seq) {
-  return nd_workspace(H, num_reqs, max_seq, HQ / H);
+  if (num_reqs == 0 || H > kMaxCounters) return 256;
+  const int64_t pairs = (int64_t)nd_slice(H, 1, num_reqs) * H;
+  return kCounterBytes + nd_parts(pairs, max_seq) * (HQ / H) * (kD + 2) * 4;
 }
 
-// Chunks of at most 16 rows take this kernel, and longer ones while the whole call is short: it reads
+// Chunks of at most 32 rows take this kernel, and longer ones while the whole call is short: it reads
 // and dequantises a key for 16 rows, the prefill kernel for 128 to 384, but it has no tiles in LDS, no
 // second launch and a smaller join. A call's items before any split are its (block, head) pairs, its
 // work their steps. Measured here and there (us, four query heads and eight KV heads):
-//   two blocks: one round of items, or long ones   30 x 8 queries over 100 keys 11.5, 13.5;
-//     16 x 8 over 6,000 48.4, 61.3; 60 x 8 over 1,500 51.8, 61.9; but 60 x 8 over 300 26.4, 24.4
+//   two blocks   30 x 8 queries over 100 keys 11.5, 13.5; 16 x 8 over 6,000 40.0, 61.3; 60 x 8 over 300
+//     18.5, 24.3
 //   more, one round of items, 24,000 steps of few of them   1 x 32 over 12,000 29.8, 35.2; 1 x 64 over
 //     5,000 26.8, 28.2; 1 x 64 over 6,000 30.3, 30.3; 2 x 20 over 14,000 38.7, 37.2
 //   or 17,000 of many   4 x 60 over 300 15.4, 18.1; 20 x 12 over 900 21.7, 34.0; 4 x 32 over 2,000 23.7,
 //     24.5; 4 x 32 over 2,500 26.3, 25.6; 5 x 20 over 4,000 35.3, 30.6; two rounds: 30 x 16 over 300 25.6, 16.0
 bool nibble_short_applies(int H, int HQ, int num_reqs, int max_q, int max_seq) {
   const int64_t rows = (int64_t)max_q * (HQ / H);
-  if (rows > kNDShortRows || (int64_t)H * nd_blocks((int)rows) > kMaxCounters) return false;
-  const int64_t blocks = nd_blocks((int)rows), steps = (max_seq + kNDStep - 1) / kNDStep;
+  if (rows > kNDShortRows) return false;
+  const int64_t blocks = nd_blocks((int)rows, 1), steps = (max_seq + kNDStep - 1) / kNDStep;
+  if (H * blocks > kMaxCounters) return false;
+  if (blocks <= 2) return true;
   const int64_t items = (int64_t)num_reqs * H * blocks;
-  if (blocks == 1) return true;
-  if (blocks == 2) return items <= nd_target() || steps >= kNDLongSteps;
   return items <= nd_target() && items * steps <= (items <= nd_target() / 4 ? kNDFewWork : kNDShortWork);
 }
 
@@ -610,18 +659,18 @@ bool nibble_short_applies(int H, int HQ, int num_reqs, int max_q, int max_seq) {
 int64_t nibble_short_part_bytes(int H, int HQ, int num_reqs, int max_q, int max_seq) {
   const int rows = (int)std::min<int64_t>((int64_t)max_q * (HQ / H), kNDShortRows);
   const int64_t pairs = std::min<int64_t>(
-      std::min<int64_t>(num_reqs, kMaxCounters) * std::min(H, kMaxCounters) * nd_blocks(rows), kMaxCounters);
-  return nd_parts(pairs, max_seq) * std::min(rows, kNDRows) * (kD + 2) * 4;
+      std::min<int64_t>(num_reqs, kMaxCounters) * std::min(H, kMaxCounters) * nd_blocks(rows, 1), kMaxCounters);
+  return nd_parts(pairs, max_seq) * std::min(rows, 2 * kNDRows) * (kD + 2) * 4;
 }
 
-template <bool CHUNK>
+template <bool CHUNK, int RG>
 static int nd_launch(const NibDecodeArgs& a, unsigned grid, int q_dtype, hipStream_t st) {
-  if (q_dtype == TTKV_DTYPE_F16)
-    hipLaunchKernelGGL((nibble_decode_kernel<TTKV_DTYPE_F16, CHUNK>), dim3(grid),
-                       dim3(kNDThreads), 0, st, a);
-  else
-    hipLaunchKernelGGL((nibble_decode_kernel<TTKV_DTYPE_BF16, CHUNK>), dim3(grid),
-                       dim3(kNDThreads), 0, st, a);
+  constexpr int smem = kNDWaves * kNDRows * RG * kD * 4;
+  auto kernel = q_dtype == TTKV_DTYPE_F16 ? nibble_decode_kernel<TTKV_DTYPE_F16, CHUNK, RG>
+                                          : nibble_decode_kernel<TTKV_DTYPE_BF16, CHUNK, RG>;
+  if (RG > 1)
+    if (int rc = raise_smem_limit((const void*)kernel, smem)) return rc;
+  hipLaunchKernelGGL(kernel, dim3(grid), dim3(kNDThreads), smem, st, a);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess)
     return host_fail(TTKV_E_LAUNCH, std::string("nibble decode launch: ") + hipGetErrorString(e));
@@ -635,7 +684,8 @@ int nibble_decode_launch(int H, int HQ, float scale, const void* q, int q_dtype,
                          const int32_t* seq_lens, const int32_t* qsl, const int32_t* req_index,
                          int num_reqs, int max_q, int max_seq, void* out, int out_dtype,
                          int64_t out_row_stride, void* ws, int32_t* err, hipStream_t st) {
-  const int rows = HQ / H * std::max(max_q, 1), blocks = nd_blocks(rows);
+  const int rows = HQ / H * std::max(max_q, 1), groups = nd_groups(H, num_reqs, rows, max_seq);
+  const int blocks = nd_blocks(rows, groups);
   const int slice = nd_slice(H, blocks, num_reqs);
   const int64_t parts = nd_parts((int64_t)slice * H * blocks, max_seq);
   NibDecodeArgs a{};
@@ -657,7 +707,7 @@ int nibble_decode_launch(int H, int HQ, float scale, const void* q, int q_dtype,
   a.out = out;
   a.out_dtype = out_dtype;
   a.out_row_stride = out_row_stride;
-  a.part_rows = std::min(rows, kNDRows);
+  a.part_rows = std::min(rows, kNDRows * groups);
   a.ws_cnt = (int*)ws;
   a.ws_o = (float*)((char*)ws + kCounterBytes);
   a.ws_ml = a.ws_o + parts * a.part_rows * kD;
@@ -676,8 +726,9 @@ int nibble_decode_launch(int H, int HQ, float scale, const void* q, int q_dtype,
     // an item per (block, head), and what the split ones have more
     const int64_t pairs = (int64_t)a.num_reqs * H * blocks;
     const unsigned grid = (unsigned)std::min(pairs + nd_target(), pairs * nd_max_chunks(max_seq));
-    const int rc = max_q > 0 ? nd_launch<true>(a, grid, q_dtype, st)
-                             : nd_launch<false>(a, grid, q_dtype, st);
+    const int rc = max_q == 0    ? nd_launch<false, 1>(a, grid, q_dtype, st)
+                   : groups == 1 ? nd_launch<true, 1>(a, grid, q_dtype, st)
+                                 : nd_launch<true, 2>(a, grid, q_dtype, st);
     if (rc != TTKV_OK) return rc;
   }
   return TTKV_OK;
