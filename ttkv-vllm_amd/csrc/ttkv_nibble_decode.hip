@@ -2,14 +2,15 @@
 // chunks of queries. gfx950 / CDNA4.
 //
 // The rows of a (request, KV head) are its query heads, or (chunk) its (query, query head) pairs, row
-// = j G + p. Work item = (request, block of 16 rows, chunk of the block's 32-token steps, KV head),
+// = j G + p. Work item = (request, block of 16 rows or of two groups of 16, chunk of the block's
+// 32-token steps, KV head),
 // one workgroup of 4 waves that take the chunk's steps in turn. The chunk length comes from a plan
 // that every workgroup computes alike from the batch's lengths: the shortest that spreads the batch's
 // steps over the resident workgroups, so a ragged batch fills the chip by its total work. Items of a
 // (block, head) leave unnormalised partials in the workspace; the last to arrive joins them.
 //
 // One step of a wave, two tiles of 16 tokens:
-//   S^T [token, row] = K Q^T, four v_mfma_f32_16x16x32_f16 per tile: a lane's 16 key code
+//   S^T [token, row] = K Q^T, four v_mfma_f32_16x16x32_f16 per tile and group of rows: a lane's 16 key code
 //     bytes are its A operand of all four (token lane % 16, 8 dims of each group of 32), unpacked by a
 //     shift and a mask per pair and dequantised exactly in packed fp16; the queries are the B operand,
 //     held in registers. Columns without a row are zero.
