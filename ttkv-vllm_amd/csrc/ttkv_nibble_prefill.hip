@@ -749,6 +749,7 @@ static NibPrefillSlice np_slice(int H, int HQ, int num_reqs, int max_q, int max_
   const int T = (max_seq + kNPTile - 1) / kNPTile;
   NibPrefillSlice best{};
   float least = 0.f;
+  int parts = 1;
   for (int ng = 3; ng >= 1; --ng) {
     NibPrefillSlice s{};
     s.ng = ng;
@@ -769,9 +770,13 @@ static NibPrefillSlice np_slice(int H, int HQ, int num_reqs, int max_q, int max_
       if (best.ng == 0 || us < least) {
         best = s;
         least = us;
+        parts = k;
       }
     }
   }
+  // One request whose keys need no split at its longest: no second launch (1 x 256 over 256: 20.2
+  // us, 18.7 so).
+  if (num_reqs == 1 && parts == 1) best.split = false;
   return best;
 }
 
