@@ -578,6 +578,26 @@ def test_prefill_workspace_serves_other_shapes():
             _close(out[r:r + 1], dq[r:r + 1].cpu(), *st.kv(r), SCALE, r)
 
 
+def test_the_largest_length_a_call_may_name():
+    """max_seq_len of 2^26, as a captured server would have it, over short requests."""
+    most = 1 << 26
+    st = Store([400, 90], 2, seed=41)
+    table = torch.full((2, most // 16), -1, dtype=torch.int32, device="cuda")
+    table[:, :st.bt.shape[1]] = st.bt
+    st.bt = table
+    for counts in ([1, 1], [5, 9], [300, 90]):
+        q = torch.randn(sum(counts), 8, D, generator=_gen(42)).half()
+        out, err, qsl = _prefill(st, q.cuda(), counts, max_seq=most, max_q=max(counts) + 3)
+        assert err == 0
+        for r in range(2):
+            s = slice(qsl[r], qsl[r + 1])
+            _close(out[s], q[s], *st.kv(r), SCALE, (counts, r))
+    out, err = _decode(st, q[:2].cuda(), max_seq=most)
+    assert err == 0
+    for r in range(2):
+        _close(out[r:r + 1], q[r:r + 1], *st.kv(r), SCALE, r)
+
+
 @pytest.mark.parametrize("lens,counts", [([300, 5000], [300, 40]), ([5000, 90], [9, 3]),
                                          ([700], [128]), ([20000, 1], [1, 1])])
 def test_the_output_may_be_the_query(lens, counts):
