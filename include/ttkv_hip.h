@@ -393,7 +393,12 @@ int ttkv_nibble_write_paged(int32_t H, int32_t d, const void* key, int32_t k_dty
 /* Attention of one query per request over the 4-bit cache, the whole batch in one call; arguments
  * as for ttkv_decode_paged, query and out fp16 or bf16, up to 16 query heads per KV head.
  *   out[p] = sum_t softmax_t(scale * q[p] . K[t]) * V[t],  t < seq_lens[r]
- * An empty request's rows are 0. A block id outside the cache sets TTKV_ERR_BAD_BLOCK and makes its
+ * A request whose start equals the next one's (ttkv_step_plan's for query_lens[r] == 0: it waits) has
+ * no query in the call: it is skipped, and its start's row is the next request's alone. Of num_reqs
+ * starts, as ttkv_nibble_decode_paged takes them, the last always has a query;
+ * ttkv_nibble_decode_starts_paged takes num_starts, num_reqs + 1 where the last may wait too. Rows that
+ * are not skipped are distinct. An empty request's row (seq_lens[r] == 0) is 0.
+ * A block id outside the cache sets TTKV_ERR_BAD_BLOCK and makes its
  * request's rows NaN. Keys and values enter the products exactly; the query is taken as fp16 (bf16
  * at a power of two per row), and the softmax weight is rounded to fp16 once. `out` may be the query.
  * max_seq_len at most 2^26 and at most the tokens that max_blocks hold; the page at most 2^31 tiles.
@@ -413,6 +418,16 @@ int ttkv_nibble_decode_paged(int32_t H, int32_t num_heads, int32_t d, float scal
                              int32_t max_seq_len, void* out, int32_t out_dtype,
                              int64_t out_row_stride, void* workspace, int64_t workspace_bytes,
                              int32_t* error_word, ttkv_stream_t stream);
+int ttkv_nibble_decode_starts_paged(int32_t H, int32_t num_heads, int32_t d, float scale,
+                                    const void* query, int32_t q_dtype, int64_t q_row_stride,
+                                    const uint8_t* page, int64_t n_slots, int64_t slot_stride,
+                                    int32_t block_size, const int32_t* block_table,
+                                    int64_t bt_row_stride, int32_t max_blocks,
+                                    const int32_t* seq_lens, const int32_t* query_start_loc,
+                                    int32_t num_starts, int32_t num_reqs, int32_t max_seq_len,
+                                    void* out, int32_t out_dtype, int64_t out_row_stride,
+                                    void* workspace, int64_t workspace_bytes, int32_t* error_word,
+                                    ttkv_stream_t stream);
 
 /* Causal attention of chunks of queries over the 4-bit cache: request r's Q queries sit at the end
  * of its n = seq_lens[r] stored keys (their own included; a first chunk has n = Q), query j sees

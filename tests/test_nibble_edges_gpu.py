@@ -1,0 +1,88 @@
+"""The 4-bit cache's operators at calls that their documentation allows and that go wrong easily:
+requests without a query. Helpers and tolerances are test_nibble_gpu's."""
+import pytest
+import torch
+
+from test_nibble_gpu import D, SCALE, Store, _close, _err, _gen, _i32
+from vllm_ttkv import kernels
+
+pytestmark = pytest.mark.gpu
+
+
+# ----------------------------------------------------------------- requests without a query
+def _starts(counts):
+    at = [0]
+    for c in counts:
+        at.append(at[-1] + c)
+    return at
+
+
+def _guarded(rows, heads, dtype=torch.float16, fill=9.0):
+    """(output rows, the buffer around them with a row before and three behind)."""
+    buf = torch.full((rows + 4, heads, D), fill, dtype=dtype, device="cuda")
+    return buf[1:rows + 1], buf
+
+
+@pytest.mark.parametrize("counts", [[1, 0, 1], [1, 1, 0], [0, 0, 1], [0, 1, 0, 0], [1, 0, 0, 1, 0]])
+@pytest.mark.parametrize("longest", [60, 9000])
+def test_decode_skips_requests_that_wait(counts, longest):
+    """A request with tokens stored and no query this step writes no row, neither the next request's
+    nor one past the output."""
+    lens = [longest - 7 * r for r in range(len(counts))]
+    st = Store(lens, 2, seed=longest)
+    n, qsl = sum(counts), _starts(counts)
+    q = torch.randn(n, 8, D, generator=_gen(50)).half()
+    out, buf = _guarded(n, 8)
+    err = _err()
+    kernels.nibble_decode_paged(st.lay, q.cuda(), st.page, 16, st.bt, st.seq, _i32(qsl), longest,
+                                SCALE, out=out, error_word=err)
+    assert int(err) == 0
+    for r, c in enumerate(counts):
+        if c:
+            _close(out[qsl[r]:qsl[r] + 1], q[qsl[r]:qsl[r] + 1], *st.kv(r), SCALE, r)
+    assert bool((buf[0] == 9).all()) and bool((buf[n + 1:] == 9).all())
+
+
+def test_decode_skips_among_many_requests():
+    """More requests than a launch's plan holds, waiting ones on both sides of its border; a batch
+    in which all wait."""
+    g = _gen(51)
+    counts = [int(x) for x in torch.randint(0, 2, (300,), generator=g)]
+    counts[254:258], counts[-1] = [1, 0, 0, 1], 0
+    lens = [int(x) for x in torch.randint(1, 300, (300,), generator=g)]
+    st = Store(lens, 1, seed=51)
+    n, qsl = sum(counts), _starts(counts)
+    q = torch.randn(n, 4, D, generator=g).half()
+    out, buf = _guarded(n, 4)
+    err = _err()
+    kernels.nibble_decode_paged(st.lay, q.cuda(), st.page, 16, st.bt, st.seq, _i32(qsl), max(lens),
+                                SCALE, out=out, error_word=err)
+    assert int(err) == 0
+    for r, c in enumerate(counts):
+        if c:
+            _close(out[qsl[r]:qsl[r] + 1], q[qsl[r]:qsl[r] + 1], *st.kv(r), SCALE, r)
+    assert bool((buf[0] == 9).all()) and bool((buf[n + 1:] == 9).all())
+    out, buf = _guarded(2, 4)
+    kernels.nibble_decode_paged(st.lay, q[:2].cuda(), st.page, 16, st.bt[:3], st.seq[:3],
+                                _i32([0, 0, 0, 0]), max(lens), SCALE, out=out, error_word=err)
+    assert int(err) == 0 and bool((buf == 9).all())
+
+
+def test_decode_of_a_planned_step_with_waiting_requests():
+    """The plan's own starts, a padded batch whose last requests are empty: their rows, which are
+    the padding's, stay as they were."""
+    lens = [40, 700, 33]
+    st = Store(lens, 2, seed=52)
+    err = _err()
+    bt = torch.cat([st.bt, torch.full_like(st.bt, -1)])
+    computed, query = _i32([39, 700, 32, 0, 0, 0]), _i32([1, 0, 1, 0, 0, 0])
+    fresh = st.bt[2, 2:3].clone()        # request 2's new token, its 33rd, opens a block
+    p = kernels.step_plan(computed, query, bt, fresh, 16, st.blocks, 4, error_word=err)
+    q = torch.randn(4, 8, D, generator=_gen(52)).half()
+    out, buf = _guarded(4, 8)
+    kernels.nibble_decode_paged(st.lay, q.cuda(), st.page, 16, bt, p.seq_lens, p.query_start_loc,
+                                700, SCALE, out=out, error_word=err)
+    assert int(err) == 0
+    for row, r in ((0, 0), (1, 2)):
+        _close(out[row:row + 1], q[row:row + 1], *st.kv(r), SCALE, r)
+    assert bool((buf[0] == 9).all()) and bool((buf[3:] == 9).all())

@@ -288,8 +288,25 @@ int ttkv_nibble_decode_paged(int32_t H, int32_t num_heads, int32_t d, float scal
                              int32_t* error_word, ttkv_stream_t stream) {
   return nibble_decode_paged(H, num_heads, d, scale, query, q_dtype, q_row_stride, page, n_slots,
                              slot_stride, block_size, block_table, bt_row_stride, max_blocks,
-                             seq_lens, query_start_loc, num_reqs, max_seq_len, out, out_dtype,
-                             out_row_stride, workspace, workspace_bytes, error_word,
+                             seq_lens, query_start_loc, num_reqs, num_reqs, max_seq_len, out,
+                             out_dtype, out_row_stride, workspace, workspace_bytes, error_word,
+                             (hipStream_t)stream);
+}
+
+int ttkv_nibble_decode_starts_paged(int32_t H, int32_t num_heads, int32_t d, float scale,
+                                    const void* query, int32_t q_dtype, int64_t q_row_stride,
+                                    const uint8_t* page, int64_t n_slots, int64_t slot_stride,
+                                    int32_t block_size, const int32_t* block_table,
+                                    int64_t bt_row_stride, int32_t max_blocks,
+                                    const int32_t* seq_lens, const int32_t* query_start_loc,
+                                    int32_t num_starts, int32_t num_reqs, int32_t max_seq_len,
+                                    void* out, int32_t out_dtype, int64_t out_row_stride,
+                                    void* workspace, int64_t workspace_bytes, int32_t* error_word,
+                                    ttkv_stream_t stream) {
+  return nibble_decode_paged(H, num_heads, d, scale, query, q_dtype, q_row_stride, page, n_slots,
+                             slot_stride, block_size, block_table, bt_row_stride, max_blocks,
+                             seq_lens, query_start_loc, num_starts, num_reqs, max_seq_len, out,
+                             out_dtype, out_row_stride, workspace, workspace_bytes, error_word,
                              (hipStream_t)stream);
 }
 

@@ -150,18 +150,19 @@ int64_t nibble_decode_workspace_bytes(int H, int HQ, int num_reqs, int max_seq);
 int nibble_decode_paged(int H, int HQ, int d, float scale, const void* q, int q_dtype,
                         int64_t q_row_stride, const uint8_t* page, int64_t n_slots,
                         int64_t slot_stride, int bs, const int32_t* bt, int64_t bt_row_stride,
-                        int max_blocks, const int32_t* seq_lens, const int32_t* qsl, int num_reqs,
-                        int max_seq, void* out, int out_dtype, int64_t out_row_stride, void* ws,
-                        int64_t ws_bytes, int32_t* err, hipStream_t st);
+                        int max_blocks, const int32_t* seq_lens, const int32_t* qsl, int num_starts,
+                        int num_reqs, int max_seq, void* out, int out_dtype, int64_t out_row_stride,
+                        void* ws, int64_t ws_bytes, int32_t* err, hipStream_t st);
 // Short chunks of queries, on the decode kernel.
 bool nibble_short_applies(int H, int HQ, int num_reqs, int max_q, int max_seq);
 int64_t nibble_short_part_bytes(int H, int HQ, int num_reqs, int max_q, int max_seq);
 int nibble_decode_launch(int H, int HQ, float scale, const void* q, int q_dtype,
                          int64_t q_row_stride, const uint8_t* page, int64_t n_slots,
                          int64_t slot_stride, int bs, const int32_t* bt, int64_t bt_row_stride,
-                         const int32_t* seq_lens, const int32_t* qsl, const int32_t* req_index,
-                         int num_reqs, int max_q, int max_seq, void* out, int out_dtype,
-                         int64_t out_row_stride, void* ws, int32_t* err, hipStream_t st);
+                         const int32_t* seq_lens, const int32_t* qsl, int num_starts,
+                         const int32_t* req_index, int num_reqs, int max_q, int max_seq, void* out,
+                         int out_dtype, int64_t out_row_stride, void* ws, int32_t* err,
+                         hipStream_t st);
 int64_t nibble_prefill_workspace_bytes(int H, int HQ, int num_reqs, int max_q, int max_seq);
 int nibble_prefill_paged(int H, int HQ, int d, float scale, const void* q, int q_dtype,
                          int64_t q_row_stride, const uint8_t* page, int64_t n_slots,

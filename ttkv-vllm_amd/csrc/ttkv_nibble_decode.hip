@@ -61,6 +61,7 @@ struct NibDecodeArgs {
   const int32_t* qsl;
   const int32_t* req_index;  // chunks
   int num_reqs, max_q, max_seq;
+  int num_starts;  // entries of qsl (decode)
   void* out;
   int out_dtype;
   int64_t out_row_stride;
@@ -103,13 +104,14 @@ __device__ __forceinline__ NibDecodePlan nd_plan(const NibDecodeArgs& a, int ite
     idx[i] = CHUNK && a.req_index && on ? a.req_index[r] : on ? r : 0;
     n[i] = on ? a.seq_lens[idx[i]] : 0;
     q0[i] = on ? a.qsl[idx[i]] : 0;
-    Q[i] = on ? (CHUNK ? a.qsl[idx[i] + 1] - q0[i] : 1) : 0;
+    // decode: no query where the next request's row is the same one
+    Q[i] = !on ? 0 : CHUNK ? a.qsl[idx[i] + 1] - q0[i] : r + 1 >= a.num_starts || a.qsl[r + 1] != q0[i];
   }
 #pragma unroll
   for (int i = 0; i < kNDPlanLanes; ++i) {
     if (64 * i >= a.num_reqs) continue;
     const int nn = min(max(n[i], 0), a.max_seq);
-    st[i] = (nn + kNDStep - 1) / kNDStep;
+    st[i] = Q[i] != 0 ? (nn + kNDStep - 1) / kNDStep : 0;
     if (CHUNK && nn < Q[i]) st[i] = 1;
     rb[i] = CHUNK ? (min(max(Q[i], 0), a.max_q) * a.G + RB - 1) / RB : Q[i];
     total += st[i] * rb[i];
@@ -678,13 +680,14 @@ static int nd_launch(const NibDecodeArgs& a, unsigned grid, int q_dtype, hipStre
   return TTKV_OK;
 }
 
-// The arguments have been checked. max_q == 0: decode.
+// The arguments have been checked. max_q == 0: decode, of num_starts entries in qsl.
 int nibble_decode_launch(int H, int HQ, float scale, const void* q, int q_dtype,
                          int64_t q_row_stride, const uint8_t* page, int64_t n_slots,
                          int64_t slot_stride, int bs, const int32_t* bt, int64_t bt_row_stride,
-                         const int32_t* seq_lens, const int32_t* qsl, const int32_t* req_index,
-                         int num_reqs, int max_q, int max_seq, void* out, int out_dtype,
-                         int64_t out_row_stride, void* ws, int32_t* err, hipStream_t st) {
+                         const int32_t* seq_lens, const int32_t* qsl, int num_starts,
+                         const int32_t* req_index, int num_reqs, int max_q, int max_seq, void* out,
+                         int out_dtype, int64_t out_row_stride, void* ws, int32_t* err,
+                         hipStream_t st) {
   const int rows = HQ / H * std::max(max_q, 1), groups = nd_groups(H, num_reqs, rows, max_seq);
   const int blocks = nd_blocks(rows, groups);
   const int slice = nd_slice(H, blocks, num_reqs);
@@ -717,6 +720,7 @@ int nibble_decode_launch(int H, int HQ, float scale, const void* q, int q_dtype,
   a.err = err;
   for (int r0 = 0; r0 < num_reqs; r0 += slice) {
     a.num_reqs = std::min(slice, num_reqs - r0);
+    a.num_starts = num_starts - r0;
     if (req_index) {
       a.req_index = req_index + r0;
     } else {
@@ -738,21 +742,22 @@ int nibble_decode_launch(int H, int HQ, float scale, const void* q, int q_dtype,
 int nibble_decode_paged(int H, int HQ, int d, float scale, const void* q, int q_dtype,
                         int64_t q_row_stride, const uint8_t* page, int64_t n_slots,
                         int64_t slot_stride, int bs, const int32_t* bt, int64_t bt_row_stride,
-                        int max_blocks, const int32_t* seq_lens, const int32_t* qsl, int num_reqs,
-                        int max_seq, void* out, int out_dtype, int64_t out_row_stride, void* ws,
+                        int max_blocks, const int32_t* seq_lens, const int32_t* qsl, int num_starts,
+                        int num_reqs, int max_seq, void* out, int out_dtype, int64_t out_row_stride, void* ws,
                         int64_t ws_bytes, int32_t* err, hipStream_t st) {
   if (int rc = nibble_check_read(H, HQ, d, q, q_dtype, q_row_stride, page, n_slots, slot_stride,
                                  bs, bt, max_blocks, seq_lens, qsl, num_reqs, max_seq, out,
                                  out_dtype, out_row_stride, err))
     return rc;
   if (H > kMaxCounters) return host_fail(TTKV_E_UNSUPPORTED, "too many KV heads");
+  if (num_starts < num_reqs) return host_fail(TTKV_E_INVALID, "fewer query starts than requests");
   const int64_t need = nibble_decode_workspace_bytes(H, HQ, num_reqs, max_seq);
   if (!ws || ws_bytes < need || (uintptr_t)ws % 256)
     return host_fail(TTKV_E_WORKSPACE, "decode workspace needs " + std::to_string(need) +
                                            " bytes, 256-aligned");
   if (num_reqs == 0) return TTKV_OK;
   return nibble_decode_launch(H, HQ, scale, q, q_dtype, q_row_stride, page, n_slots, slot_stride,
-                              bs, bt, bt_row_stride, seq_lens, qsl, nullptr, num_reqs, 0, max_seq,
+                              bs, bt, bt_row_stride, seq_lens, qsl, num_starts, nullptr, num_reqs, 0, max_seq,
                               out, out_dtype, out_row_stride, ws, err, st);
 }
 

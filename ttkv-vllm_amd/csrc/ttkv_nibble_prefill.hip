@@ -838,7 +838,7 @@ int nibble_prefill_paged(int H, int HQ, int d, float scale, const void* q, int q
   if (num_reqs == 0 || max_q == 0) return TTKV_OK;
   if (nibble_short_applies(H, HQ, num_reqs, max_q, max_seq))
     return nibble_decode_launch(H, HQ, scale, q, q_dtype, q_row_stride, page, n_slots, slot_stride,
-                                bs, bt, bt_row_stride, seq_lens, qsl, req_index, num_reqs, max_q,
+                                bs, bt, bt_row_stride, seq_lens, qsl, 0, req_index, num_reqs, max_q,
                                 max_seq, out, out_dtype, out_row_stride, ws, err, st);
   const NibPrefillSlice s = np_slice(H, HQ, num_reqs, max_q, max_seq);
   const int64_t items =

@@ -201,6 +201,14 @@ def lib():
         P, I32, I64,                  # out, out_dtype, out_row_stride
         P, I64, P, P,                 # workspace, workspace_bytes, error_word, stream
     ]
+    L.ttkv_nibble_decode_starts_paged.restype = ctypes.c_int
+    L.ttkv_nibble_decode_starts_paged.argtypes = [
+        I32, I32, I32, F32, P, I32, I64,  # H, num_heads, d, scale, query, q_dtype, q_row_stride
+        P, I64, I64, I32,             # page, n_slots, slot_stride, block_size
+        P, I64, I32, P, P, I32,       # block_table, stride, max_blocks, seq_lens, qsl, num_starts
+        I32, I32, P, I32, I64,        # num_reqs, max_seq_len, out, out_dtype, out_row_stride
+        P, I64, P, P,                 # workspace, workspace_bytes, error_word, stream
+    ]
     L.ttkv_nibble_prefill_workspace_bytes.restype = I64
     L.ttkv_nibble_prefill_workspace_bytes.argtypes = [I32, I32, I32, I32, I32]
     L.ttkv_nibble_prefill_paged.restype = ctypes.c_int
@@ -226,8 +234,8 @@ EXPORTS = ("ttkv_last_error", "ttkv_decoder_ranks", "ttkv_blob_bytes",
            "ttkv_dense_decode_paged", "ttkv_write_workspace_bytes", "ttkv_container_krt",
            "ttkv_container_v_out", "ttkv_step_plan", "ttkv_rotary_axes",
            "ttkv_nibble_write_paged", "ttkv_nibble_decode_workspace_bytes",
-           "ttkv_nibble_decode_paged", "ttkv_nibble_prefill_workspace_bytes",
-           "ttkv_nibble_prefill_paged")
+           "ttkv_nibble_decode_paged", "ttkv_nibble_decode_starts_paged",
+           "ttkv_nibble_prefill_workspace_bytes", "ttkv_nibble_prefill_paged")
 
 
 def check(rc: int, what: str) -> None:

@@ -659,7 +659,10 @@ def nibble_decode_paged(lay: NibbleLayout, query: torch.Tensor, page: torch.Tens
                         error_word: torch.Tensor | None = None) -> torch.Tensor:
     """Attention of one query per request (row query_start_loc[r] of query [N, HQ, d], rotated)
     over its seq_lens[r] stored tokens of a 4-bit cache. See `ttkv_nibble_decode_paged` in
-    include/ttkv_hip.h. Returns `out` [N, HQ, d] with the decode rows written."""
+    include/ttkv_hip.h. Returns `out` [N, HQ, d] with the decode rows written.
+
+    query_start_loc [B] or, as `step_plan` writes it, [B + 1]: a request whose entry equals the next
+    one has no query in this step and is skipped."""
     index = _one_device(query, page, block_table, seq_lens, query_start_loc, out, workspace,
                         error_word)
     out, q_args, bt_args, out_args = _nibble_read(lay, query, page, block_table, seq_lens,
@@ -671,8 +674,9 @@ def nibble_decode_paged(lay: NibbleLayout, query: torch.Tensor, page: torch.Tens
         workspace = nibble_decode_workspace(lay, HQ, B, max_seq_len, query.device)
     err = _error_word(error_word, query.device)
     rc = _on_device(
-        index, _hip.lib().ttkv_nibble_decode_paged, lay.H, HQ, lay.d, float(scale), *q_args,
-        int(block_size), *bt_args, seq_lens.data_ptr(), query_start_loc.data_ptr(), B,
+        index, _hip.lib().ttkv_nibble_decode_starts_paged, lay.H, HQ, lay.d, float(scale), *q_args,
+        int(block_size), *bt_args, seq_lens.data_ptr(), query_start_loc.data_ptr(),
+        min(query_start_loc.numel(), B + 1), B,
         int(max_seq_len), *out_args, workspace.data_ptr(), workspace.numel(), err.data_ptr(),
         _stream(index))
     _hip.check(rc, "ttkv_nibble_decode_paged")
