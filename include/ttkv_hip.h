@@ -352,7 +352,9 @@ int ttkv_container_v_out(int32_t H, int32_t num_heads, int32_t d, int32_t B, int
  * more tokens than num_tokens, a request longer than its row of max_blocks, or a negative length
  * (taken as 0): TTKV_ERR_SEQ_LEN, the tokens without a place get slot -1; a free list that is too
  * short: TTKV_ERR_NO_BLOCK, -1 for the missing ids and their slots; an id outside [0, num_blocks):
- * TTKV_ERR_BAD_BLOCK, slot -1. At most 8,000 requests. Lengths saturate at 2^30 - 1. */
+ * TTKV_ERR_BAD_BLOCK, slot -1. At most 8,000 requests. Lengths saturate at 2^30 - 1.
+ * Outputs and the table overlap neither the inputs nor one another (TTKV_E_INVALID): the lengths and
+ * the free list are read while they are written. */
 int ttkv_step_plan(const int32_t* computed_lens, const int32_t* query_lens, int32_t num_reqs,
                    int32_t* block_table, int64_t bt_row_stride, int32_t max_blocks,
                    const int32_t* free_blocks, int32_t num_free, int32_t block_size,

@@ -17,3 +17,33 @@ def test_decode_starts_refusals():
     _refused(call(0, 1), 1, "query starts")
     _refused(call(-1, 1), 1, "query starts")
     assert call(0, 0) == 0 and call(1, 0) == 0                      # nothing to do
+
+
+# ------------------------------------------------------- a plan's outputs and what it reads
+def _plan(**kw):
+    """Two requests, a table of two rows of 4 at a stride of 8, 6 free ids, 9 tokens, apart from
+    one another; a call that is not refused would launch, so each one here is."""
+    a = dict(c=0x1000, n=0x2000, R=2, bt=0x3000, bts=8, W=4, free=0x4000, F=6, bs=16, blocks=8, T=9,
+             qsl=0x5000, seq=0x6000, slots=0x7000, pos=0x8000, used=0x9000, err=0xa000)
+    a.update(kw)
+    return _hip.lib().ttkv_step_plan(*a.values(), None)
+
+
+def test_plan_refuses_outputs_that_lie_in_its_inputs():
+    size = dict(qsl=12, seq=8, used=4, slots=72, pos=72)
+    for name, n in size.items():
+        for at, length in ((0x1000, 8), (0x2000, 8)):               # the lengths, at any offset
+            for off in range(-n + 4, length, 4):
+                _refused(_plan(**{name: at + off}), 1, "length inputs")
+        for off in range(-n + 4, 24, 4):
+            _refused(_plan(**{name: 0x4000 + off}), 1, "free list")
+        for row in (0x3000, 0x3020):
+            for off in range(-n + 4, 16, 4):
+                _refused(_plan(**{name: row + off}), 1, "block table")
+    _refused(_plan(c=0x300c), 1, "length inputs")
+    _refused(_plan(n=0x3020), 1, "length inputs")
+    _refused(_plan(free=0x301c), 1, "free list")
+    _refused(_plan(pos=0x7040), 1, "overlap")
+    _refused(_plan(seq=0x5008), 1, "overlap")
+    # query_lens as the tail of the buffer that the starts go to
+    _refused(_plan(n=0x5004), 1, "length inputs")

@@ -1,5 +1,5 @@
 """The 4-bit cache's operators at calls that their documentation allows and that go wrong easily:
-requests without a query. Helpers and tolerances are test_nibble_gpu's."""
+requests without a query, a plan's tensors within one buffer. Helpers and tolerances are test_nibble_gpu's."""
 import pytest
 import torch
 
@@ -86,3 +86,35 @@ def test_decode_of_a_planned_step_with_waiting_requests():
     for row, r in ((0, 0), (1, 2)):
         _close(out[row:row + 1], q[row:row + 1], *st.kv(r), SCALE, r)
     assert bool((buf[0] == 9).all()) and bool((buf[3:] == 9).all())
+
+
+# ----------------------------------------------------------- a plan's tensors within one buffer
+def test_plan_of_tensors_that_touch():
+    """Lengths, free list and outputs side by side in one buffer, the lengths between the table's
+    rows: the same plan as of tensors of their own. Starts into whose tail the query lengths are a
+    view are refused."""
+    R, W, block, blocks, T = 3, 4, 16, 20, 30
+    c, n, free = [20, 0, 33], [5, 17, 2], [11, 12, 13, 14]
+    table = torch.full((R, W + R), -1, dtype=torch.int32, device="cuda")
+    table[0, :2], table[2, :3] = _i32([3, 4]), _i32([5, 6, 7])
+    own = table[:, :W].contiguous()
+    want = kernels.step_plan(_i32(c), _i32(n), own, _i32(free), block, blocks, T)
+    flat = torch.zeros(64, dtype=torch.int32, device="cuda")
+    table[1, W:W + R] = _i32(c)                     # in the gap behind row 1
+    computed, query, ids = table[1, W:W + R], flat[:R], flat[R:R + 4]
+    query.copy_(_i32(n))
+    ids.copy_(_i32(free))
+    wide = torch.zeros(2 * T, dtype=torch.int64, device="cuda")
+    err = _err()
+    got = kernels.step_plan(computed, query, table[:, :W], ids, block, blocks, T,
+                            query_start_loc=flat[7:11], seq_lens=flat[11:14], blocks_used=flat[14:15],
+                            slot_mapping=wide[:T], positions=wide[T:], error_word=err)
+    assert int(err) == 0
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)
+    assert torch.equal(table[:, :W], own)
+    assert table[1, W:].tolist() == c and flat[:7].tolist() == n + free
+    starts = torch.zeros(R + 1, dtype=torch.int32, device="cuda")
+    for kw in (dict(query_start_loc=starts), dict(seq_lens=starts[:R]), dict(blocks_used=starts[2:3])):
+        with pytest.raises(RuntimeError, match="length inputs"):
+            kernels.step_plan(_i32(c), starts[1:], own, _i32(free), block, blocks, T, **kw)

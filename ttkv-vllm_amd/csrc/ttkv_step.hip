@@ -170,10 +170,36 @@ int step_plan(const int32_t* computed, const int32_t* qlens, int R, int32_t* bt,
   if (!qsl || !used || !err || (R && (!computed || !qlens || !seq)) || (R && W && !bt) ||
       (F && !free_ids) || (T && (!slots || !pos)))
     return host_fail(TTKV_E_INVALID, "null pointer argument");
-  // every workgroup reads the lengths while others write
-  for (const int32_t* out : {(const int32_t*)qsl, (const int32_t*)seq, (const int32_t*)used})
-    if (out && (out == computed || out == qlens))
-      return host_fail(TTKV_E_INVALID, "an output is one of the length inputs");
+  // Every workgroup reads the lengths and the free list while others write, so no output may lie in
+  // them, nor in another output. Ranges in bytes; the table's rows may have gaps between them.
+  struct Range {
+    uintptr_t at, end;
+    bool meets(const Range& o) const { return at < o.end && o.at < end; }
+  };
+  auto range = [](const void* p, int64_t bytes) { return Range{(uintptr_t)p, (uintptr_t)p + (uintptr_t)bytes}; };
+  const Range outs[] = {range(qsl, ((int64_t)R + 1) * 4), range(seq, (int64_t)R * 4), range(used, 4),
+                        range(slots, (int64_t)T * 8), range(pos, (int64_t)T * 8)};
+  const Range lens[] = {range(computed, (int64_t)R * 4), range(qlens, (int64_t)R * 4)};
+  const Range ids = range(free_ids, (int64_t)F * 4);
+  auto in_table = [&](const Range& x) {
+    const uintptr_t t0 = (uintptr_t)bt;
+    if (!R || !W || x.at >= x.end || x.end <= t0) return false;
+    const uint64_t row = (uint64_t)bt_row_stride * 4, from = x.at > t0 ? x.at - t0 : 0, to = x.end - t0;
+    if (from / row >= (uint64_t)R) return false;
+    return from % row < (uint64_t)W * 4 || (from / row + 1 < (uint64_t)R && to > (from / row + 1) * row);
+  };
+  for (const Range& x : outs)
+    if (x.meets(lens[0]) || x.meets(lens[1]))
+      return host_fail(TTKV_E_INVALID, "an output lies in one of the length inputs");
+  if (in_table(lens[0]) || in_table(lens[1]))
+    return host_fail(TTKV_E_INVALID, "the block table holds one of the length inputs");
+  if (in_table(ids)) return host_fail(TTKV_E_INVALID, "the free list lies in the block table");
+  for (const Range& x : outs) {
+    if (x.meets(ids)) return host_fail(TTKV_E_INVALID, "an output lies in the free list");
+    if (in_table(x)) return host_fail(TTKV_E_INVALID, "an output lies in the block table");
+    for (const Range& y : outs)
+      if (&x != &y && x.meets(y)) return host_fail(TTKV_E_INVALID, "two outputs overlap");
+  }
   PlanArgs a{computed, qlens, R, bt,  bt_row_stride, W,     free_ids, F,   bs,
              num_blocks, T,   qsl, seq, slots, pos, used, err};
   const int grid = std::max(1, (T + kPlanThreads * kPlanTokens - 1) / (kPlanThreads * kPlanTokens));
