@@ -1,5 +1,6 @@
 """The 4-bit cache's operators at calls that their documentation allows and that go wrong easily:
-requests without a query, a plan's tensors within one buffer. Helpers and tolerances are test_nibble_gpu's."""
+requests without a query, a plan's tensors within one buffer,
+positions of other shapes. Helpers and tolerances are test_nibble_gpu's."""
 import pytest
 import torch
 
@@ -118,3 +119,28 @@ def test_plan_of_tensors_that_touch():
     for kw in (dict(query_start_loc=starts), dict(seq_lens=starts[:R]), dict(blocks_used=starts[2:3])):
         with pytest.raises(RuntimeError, match="length inputs"):
             kernels.step_plan(_i32(c), starts[1:], own, _i32(free), block, blocks, T, **kw)
+
+
+# ------------------------------------------------------------------- positions of other shapes
+def test_rotary_positions_of_other_shapes():
+    """Positions of three dims are taken where they are contiguous and refused where they are not
+    (only a matrix's axis stride is passed on); a broadcast or strided matrix, and one token."""
+    g, N = _gen(60), 6
+    cs = torch.randn(50, D, generator=g).cuda()
+    q = torch.randn(N, 4, D, generator=g).half().cuda()
+    sections = (16, 24, 24)
+    pos = torch.randint(0, 50, (3, N), generator=g).cuda()
+
+    def turn(p, x=q):
+        return kernels.rotary_axes(x, None, p, cs, sections)[0]
+    want = turn(pos)
+    assert torch.equal(turn(pos.reshape(3, 1, N)), want)
+    wide = torch.zeros(3, 40, dtype=torch.int64, device="cuda")
+    wide[:, 3:3 + N] = pos
+    assert torch.equal(turn(wide[:, 3:3 + N]), want)
+    assert torch.equal(turn(pos[:1].expand(3, N)), turn(pos[:1].repeat(3, 1)))
+    assert torch.equal(turn(pos[:, 2:3], q[2:3]), want[2:3])
+    for bad in (pos[:1].reshape(1, 1, N).expand(3, 1, N), wide[:, 3:3 + N].unsqueeze(1),
+                pos.t().contiguous().t(), torch.zeros((), dtype=torch.int64, device="cuda")):
+        with pytest.raises(ValueError, match="positions"):
+            turn(bad)

@@ -530,11 +530,12 @@ def rotary_axes(query: torch.Tensor, key: torch.Tensor | None, positions: torch.
         raise ValueError(f"query must be [N, heads, d], got {tuple(query.shape)}")
     N, HQ, d = query.shape
     sections = tuple(sections)
-    if positions.dtype != torch.int64 or positions.shape[-1] != N \
+    if positions.dtype != torch.int64 or positions.shape[-1:] != (N,) \
             or positions.numel() != len(sections) * N:
         raise ValueError(f"positions must be int64 [{len(sections)}, {N}], got "
                          f"{positions.dtype} {tuple(positions.shape)}")
-    if N > 1 and positions.stride(-1) != 1:
+    if (N > 1 and positions.stride(-1) != 1) or (positions.dim() > 2
+                                                 and not positions.is_contiguous()):
         raise ValueError("an axis's positions must be contiguous")
     if cos_sin_cache.dtype != torch.float32 or cos_sin_cache.dim() != 2 \
             or not cos_sin_cache.is_contiguous():
