@@ -364,8 +364,9 @@ int ttkv_step_plan(const int32_t* computed_lens, const int32_t* query_lens, int3
 
 /* Rotary positions with one to four axes (an image's tokens have a time, a row and a column).
  * query [N, num_heads, d] and key [N, H, d] (same dtype; either may be absent with 0 heads) are
- * rotated into query_out / key_out (which may be the inputs themselves): for j < half =
- * rotary_dim / 2, with (cos, sin) of frequency j at the token's position on j's axis,
+ * rotated into query_out / key_out (query_out may be query, and key_out key, at the same stride;
+ * otherwise outputs overlap nothing): for j < half = rotary_dim / 2, with (cos, sin) of frequency j
+ * at the token's position on j's axis,
  *   y[j] = x[j] cos - x[j + half] sin,   y[j + half] = x[j + half] cos + x[j] sin;
  * dims past rotary_dim are copied. positions: int64, axis a of token i at a * axis_stride + i.
  * sections [axes] (host memory) add up to half: frequencies in a row, sections[0] of axis 0 first;

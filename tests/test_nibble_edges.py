@@ -1,5 +1,7 @@
 """The 4-bit cache's entry points on the CPU: refusals that go with their edge cases (nothing is
 launched)."""
+import ctypes
+
 from vllm_ttkv import _hip
 
 
@@ -47,3 +49,30 @@ def test_plan_refuses_outputs_that_lie_in_its_inputs():
     _refused(_plan(seq=0x5008), 1, "overlap")
     # query_lens as the tail of the buffer that the starts go to
     _refused(_plan(n=0x5004), 1, "length inputs")
+
+
+# ------------------------------------------------------------------ rotary outputs and inputs
+def _rotary(**kw):
+    """Four tokens, four query and two key heads of 8 dims in fp16, inside rows of 8 heads (128 bytes
+    a token): queries at 0, keys at 64, values behind; outputs apart unless named."""
+    a = dict(q=0x10000, k=0x10040, qo=0x20000, ko=0x30000, dt=1, N=4, HQ=4, H=2, d=8, qs=64, ks=64,
+             qos=32, kos=16, pos=16, ps=4, axes=1, sec=(ctypes.c_int32 * 1)(4), inter=0, cs=16,
+             max_pos=64, rot=8, err=16)
+    a.update(kw)
+    return _hip.lib().ttkv_rotary_axes(*a.values(), None)
+
+
+def test_rotary_refuses_outputs_that_overlap():
+    q, k, row = 0x10000, 0x10040, 128
+    for off in (-48, -16, 16, 48):                                  # shifted in place
+        _refused(_rotary(qo=q + off, qos=64), 1, "without being it")
+    for rows in (-3, -1, 1, 3):                                     # by whole rows
+        _refused(_rotary(qo=q + rows * row, qos=64), 1, "without being it")
+        _refused(_rotary(ko=k + rows * row, kos=64), 1, "without being it")
+    _refused(_rotary(qo=q, qos=32), 1, "without being it")          # packed at the same place
+    _refused(_rotary(ko=q + 16, kos=64), 1, "overlaps the other")   # key_out in the queries
+    _refused(_rotary(qo=k, qos=64), 1, "overlaps the other")
+    _refused(_rotary(qo=k - 16, qos=64, N=1), 1, "without being it")
+    _refused(_rotary(qo=q, qos=64, ko=q, kos=64), 1, "overlaps the other")
+    _refused(_rotary(qo=0x20000, ko=0x20000, qos=32, kos=32), 1, "overlaps the other")
+    _refused(_rotary(qo=0x20000, ko=0x20030 + 128, qos=64, kos=64), 1, "overlaps the other")

@@ -144,3 +144,20 @@ def test_rotary_positions_of_other_shapes():
                 pos.t().contiguous().t(), torch.zeros((), dtype=torch.int64, device="cuda")):
         with pytest.raises(ValueError, match="positions"):
             turn(bad)
+
+
+def test_rotary_outputs_beside_inputs():
+    """Outputs in the same rows as the inputs, behind them or in place, one of each: the same values."""
+    g, N = _gen(61), 9
+    cs = torch.randn(50, D, generator=g).cuda()
+    pos = torch.randint(0, 50, (3, N), generator=g).cuda()
+    rows = torch.randn(N, 12 * D, generator=g).half().cuda()
+    part = lambda a, n: rows[:, a * D:(a + n) * D].unflatten(1, (n, D))  # noqa: E731
+    q, k = part(0, 4), part(4, 2)
+    want = kernels.rotary_axes(q.contiguous(), k.contiguous(), pos, cs, (16, 24, 24))
+    before = rows[:, 4 * D:6 * D].clone()
+    got = kernels.rotary_axes(q, k, pos, cs, (16, 24, 24), query_out=q, key_out=part(7, 2))
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    assert torch.equal(rows[:, 4 * D:6 * D], before)
+    got = kernels.rotary_axes(part(0, 4), k, pos, cs, (16, 24, 24), query_out=part(8, 4), key_out=k)
+    assert torch.equal(got[1], want[1])

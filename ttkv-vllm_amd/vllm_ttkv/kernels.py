@@ -520,7 +520,7 @@ def rotary_axes(query: torch.Tensor, key: torch.Tensor | None, positions: torch.
                 query_out: torch.Tensor | None = None, key_out: torch.Tensor | None = None,
                 error_word: torch.Tensor | None = None):
     """Rotate query [N, HQ, d] and key [N, H, d] by positions of one to four axes; returns
-    (query_out, key_out), which may be the inputs. See `ttkv_rotary_axes` in include/ttkv_hip.h.
+    (query_out, key_out), each of which may be its input. See `ttkv_rotary_axes` in include/ttkv_hip.h.
 
     positions [axes, N] (or [N] for one axis) int64; sections: how many of the rotary_dim / 2
     frequencies each axis has, in a row, or dealt in turn where `interleaved`; cos_sin_cache
