@@ -1,10 +1,11 @@
 """The 4-bit cache's operators at calls that their documentation allows and that go wrong easily:
 requests without a query, a plan's tensors within one buffer,
-positions of other shapes. Helpers and tolerances are test_nibble_gpu's."""
+positions of other shapes, outputs that lie in inputs, scores of any size. Helpers and tolerances are test_nibble_gpu's."""
 import pytest
 import torch
 
-from test_nibble_gpu import D, SCALE, Store, _close, _err, _gen, _i32
+from oracle import nibble as on
+from test_nibble_gpu import D, HALF, SCALE, Store, _close, _err, _gen, _i32
 from vllm_ttkv import kernels
 
 pytestmark = pytest.mark.gpu
@@ -161,3 +162,49 @@ def test_rotary_outputs_beside_inputs():
     assert torch.equal(rows[:, 4 * D:6 * D], before)
     got = kernels.rotary_axes(part(0, 4), k, pos, cs, (16, 24, 24), query_out=part(8, 4), key_out=k)
     assert torch.equal(got[1], want[1])
+
+
+# ------------------------------------------------------------------------------- large scores
+def _levels(n, seed):
+    """A store of n tokens of one KV head whose keys are one channel of seven levels, 8 % apart or
+    more (the stored ones), and random values; the levels as stored and the values."""
+    st = Store([n], 1, seed=seed)
+    level = torch.randint(1, 8, (n,), generator=_gen(seed)).half()
+    k = torch.zeros(n, 1, D).half()
+    k[:, 0, 0] = level
+    kernels.nibble_write_paged(st.lay, k.cuda(), st.v.cuda(), st.slots.cuda(), st.page)
+    return st, on.values(k)[:, 0, 0], on.values(st.v)[:, 0]
+
+
+def _winners(level, V, sign, sees):
+    """The mean of the values of the largest (smallest) level among the first `sees` tokens."""
+    lv = level[:sees] * sign
+    return V[:sees][lv == lv.max()].mean(0)
+
+
+@pytest.mark.parametrize("n,Q", [(70, 1), (9000, 1), (500, 7), (6000, 5), (100, 100), (3000, 130)])
+@pytest.mark.parametrize("dtype,peak,scale", [
+    (torch.bfloat16, 2.0 ** 12, 1.0), (torch.bfloat16, 2.0 ** 24, 1.0), (torch.bfloat16, 2.0 ** 29, 1.0),
+    (torch.bfloat16, 2.0 ** 31, 1.3), (torch.bfloat16, 2.0 ** 60, 0.7), (torch.bfloat16, 2.0 ** 101, 1.1),
+    (torch.bfloat16, 2.0 ** 122, 1.0), (torch.float16, 60000.0, 1e4), (torch.float16, 60000.0, 3e25)])
+def test_scores_far_beyond_the_weights_range(n, Q, dtype, peak, scale):
+    """Scores of up to 2^125, of either sign: neighbours are 2^8 or more apart, so a row is the mean
+    of the values of its largest keys, whose scores are equal. Equal weights leave the roundings of
+    the mean's sum (n additions of 2^-24) and of the output: half + 2^-24 n of the largest value."""
+    st, level, V = _levels(n, n)
+    q = torch.zeros(Q, 4, D)
+    q[:, :2, 0], q[:, 2:, 0] = peak, -peak
+    err = _err()
+    if Q == 1:
+        out = kernels.nibble_decode_paged(st.lay, q.to(dtype).cuda(), st.page, 16, st.bt, st.seq,
+                                          _i32([0, 1]), n, scale, error_word=err)
+    else:
+        out = kernels.nibble_prefill_paged(st.lay, q.to(dtype).cuda(), st.page, 16, st.bt, st.seq,
+                                           _i32([0, Q]), Q, n, scale, error_word=err)
+    assert int(err) == 0
+    got = out.cpu().double()
+    for j in {0, Q // 2, Q - 1}:
+        for p, sign in ((0, 1), (1, 1), (2, -1), (3, -1)):
+            want = _winners(level, V, sign, n - Q + j + 1)
+            tol = HALF[dtype] * want.abs() + 2.0 ** -24 * n * V.abs().max()
+            assert bool(((got[j, p] - want).abs() <= tol).all()), (j, p, got[j, p, :3], want[:3])

@@ -112,6 +112,20 @@ __device__ __forceinline__ void nib_query(const NibRow& in, float scale_log2, bo
   }
 }
 
+// Softmax weights are 2^(score * qs - m), m a running maximum. Formed in one fma, the exponent of a key
+// whose score is the maximum is what the rounding of m left over, 2^-25 |m| at most: a common factor of
+// the row's weights, but one that leaves fp16 where |m| is about 2^29. Rows of |m| above kNibFar take the
+// product rounded by itself: equal scores then weigh the same and the largest exactly 1, whatever their
+// size. A maximum before the first visible key is the lowest float.
+constexpr float kNibFar = 4096.f;
+constexpr float kNibNone = -3.402823466e38f;
+__device__ __forceinline__ bool nib_far(float m) { return fabsf(m) > kNibFar && m > kNibNone; }
+__device__ __forceinline__ float nib_apart(float score, float qs, float m) {
+#pragma clang fp contract(off)
+  const float p = score * qs;
+  return p - m;
+}
+
 // Inclusive prefix sum over the wave's lanes (all active), on DPP: within rows of 16, then the rows.
 __device__ __forceinline__ int nib_scan(int v) {
   v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, false);  // row_shr 1, 2, 4, 8

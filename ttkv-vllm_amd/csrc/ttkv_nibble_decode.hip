@@ -43,7 +43,6 @@ constexpr int64_t kNDShortWork = 17000;  // and steps of all its blocks,
 constexpr int64_t kNDFewWork = 24000;    // where they are few
 constexpr int64_t kNDWideWork = 36000;   // from which two groups of 16 rows share a block
 constexpr float kNDMost = 2048.f;      // a lane's sum of eight softmax weights before a rescale
-constexpr float kNDNone = -1e30f;      // a maximum before the first visible key
 constexpr int kNDRows = 16;            // rows of a block: a matrix product's columns
 
 struct NibDecodeArgs {
@@ -244,7 +243,7 @@ __global__ __launch_bounds__(kNDThreads, 2) void nibble_decode_kernel(NibDecodeA
     const int row = min(kNDRows * r + col, nrow - 1);
     const NibRow qrow = nib_load_row(a.q + row_at(row, a.q_row_stride), q4);
     nib_query<QDT>(qrow, a.scale_log2, kNDRows * r + col < nrow, qf[r], qs[r]);
-    m[r] = kNDNone;
+    m[r] = kNibNone;
     l[r] = 0.f;
     lim[r] = CHUNK ? p0 + (row0 + row) / G : p0;
   }
@@ -260,6 +259,7 @@ __global__ __launch_bounds__(kNDThreads, 2) void nibble_decode_kernel(NibDecodeA
   const int s0 = (int)((int64_t)steps * P.c / P.nch);
   const int s1 = (int)((int64_t)steps * (P.c + 1) / P.nch);
   bool bad = false;
+  float most = kNDMost;  // below every sum from the wave's first far maximum on
 
   const NibMasks masks = nib_masks();
   const uint8_t* base = a.page + (int64_t)h * kNibRecord;
@@ -335,18 +335,23 @@ __global__ __launch_bounds__(kNDThreads, 2) void nibble_decode_kernel(NibDecodeA
         }
     }
     // Weights against the maximum as it stands. It has to move only where a lane's sum of eight
-    // exceeds 2^11 (or is NaN): the scores' own maximum is taken in that case alone.
+    // exceeds 2^11 (or is NaN), and the scores' own maximum is taken in that case alone, or where a row
+    // of the wave has a far one.
     half8 pf[RG];
     float sum[RG];
-    auto weights = [&](int r) {
+    auto weights = [&](int r, bool apart) {
       sum[r] = 0.f;
+      auto exponent = [&](float s) {
+        const float e = fmaf(s, qs[r], -m[r]);
+        return apart ? nib_apart(s, qs[r], m[r]) : e;
+      };
 #pragma unroll
       for (int t = 0; t < 2; ++t)
 #pragma unroll
         for (int i = 0; i < 4; i += 2) {
           // the one rounding on the way to the output; the sum takes the rounded weights
-          const half2v p = {(_Float16)fast_exp2(fmaf(sc[r][t][i], qs[r], -m[r])),
-                            (_Float16)fast_exp2(fmaf(sc[r][t][i + 1], qs[r], -m[r]))};
+          const half2v p = {(_Float16)fast_exp2(exponent(sc[r][t][i])),
+                            (_Float16)fast_exp2(exponent(sc[r][t][i + 1]))};
           sum[r] = __builtin_amdgcn_fdot2(p, half2v{(_Float16)1.f, (_Float16)1.f}, sum[r], false);
           pf[r][4 * t + i] = p[0];
           pf[r][4 * t + i + 1] = p[1];
@@ -355,8 +360,8 @@ __global__ __launch_bounds__(kNDThreads, 2) void nibble_decode_kernel(NibDecodeA
     bool fits = true;
 #pragma unroll
     for (int r = 0; r < RG; ++r) {
-      weights(r);
-      fits &= sum[r] <= kNDMost;
+      weights(r, false);
+      fits &= sum[r] <= most;
     }
     if (__builtin_amdgcn_ballot_w64(!fits)) {
 #pragma unroll
@@ -372,7 +377,8 @@ __global__ __launch_bounds__(kNDThreads, 2) void nibble_decode_kernel(NibDecodeA
         l[r] *= f;
 #pragma unroll
         for (int i = 0; i < 8; ++i) acc[r][i] *= f;
-        weights(r);
+        weights(r, nib_far(mn));
+        if (__builtin_amdgcn_ballot_w64(nib_far(mn))) most = -1.f;
       }
     }
 #pragma unroll
@@ -451,7 +457,7 @@ __global__ __launch_bounds__(kNDThreads, 2) void nibble_decode_kernel(NibDecodeA
 #pragma unroll
   for (int r = 0; r < RG; ++r) {
     const int row = kNDRows * r + col;
-    float M = kNDNone;
+    float M = kNibNone;
 #pragma unroll
     for (int w = 0; w < kNDWaves; ++w) M = fmaxf(M, red_m[w][row]);
     const float f = exp2f(m[r] - M);
@@ -470,7 +476,7 @@ __global__ __launch_bounds__(kNDThreads, 2) void nibble_decode_kernel(NibDecodeA
   const int64_t part = ((int64_t)P.part + P.c) * a.H + h;  // (where the block is split)
   for (int e = 4 * tid; e < nrow * kD; e += 4 * kNDThreads) {
     const int p = e / kD, d = e % kD;
-    float mm = kNDNone, ll = 0.f;
+    float mm = kNibNone, ll = 0.f;
     float4v o = {};
 #pragma unroll
     for (int w = 0; w < kNDWaves; ++w) mm = fmaxf(mm, red_m[w][p]);
@@ -524,7 +530,7 @@ __global__ __launch_bounds__(kNDThreads, 2) void nibble_decode_kernel(NibDecodeA
 #pragma unroll
     for (int k = 0; k < K; ++k) {
       row[k] = min((half >> sh) + 2 * kNDWaves * k, nrow - 1);
-      mm[k] = kNDNone;
+      mm[k] = kNibNone;
       ll[k] = 0.f;
       o[k] = float4v{};
     }
@@ -553,7 +559,7 @@ __global__ __launch_bounds__(kNDThreads, 2) void nibble_decode_kernel(NibDecodeA
 #pragma unroll
       for (int k = 0; k < K; ++k) {
         float x0, x1;
-        swap16(row_max(c32 < nb ? ml[k][0] : kNDNone), x0, x1);
+        swap16(row_max(c32 < nb ? ml[k][0] : kNibNone), x0, x1);
         const float mn = fmaxf(mm[k], fmaxf(x0, x1));
         const float keep = exp2f(mm[k] - mn);
         wc[k] = c32 < nb ? exp2f(ml[k][0] - mn) : 0.f;

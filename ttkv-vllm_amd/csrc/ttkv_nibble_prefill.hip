@@ -41,7 +41,6 @@ constexpr int kNPMaxSplit = 32;
 constexpr int kNPMinTiles = 4;     // keys per part, in tiles (batches that are not searched)
 constexpr int kNPSearch = 16;      // requests up to which the plan searches for the number of parts
 constexpr float kNPMost = 2048.f;  // a lane's sum of eight softmax weights before a rescale
-constexpr float kNPNone = -1e30f;  // a maximum before the first visible key
 constexpr int64_t kNPPartRows = 127000;  // rows of partial results a launch may leave: 66.0 MB
 constexpr int kNPKBytes = kNPTile * kD * 2;
 constexpr int kNPSmem = 4 * kNPKBytes;  // two buffers of keys and values
@@ -316,6 +315,7 @@ __global__ __launch_bounds__(kNPThreads, 2) void nibble_prefill_kernel(NibPrefil
   const int tt = wv & 3;  // this wave's record of a tile
   const int last_rec = (n - 1) / kNibTile;
   bool bad = false;
+  float most = kNPMost;  // below every sum from the wave's first far maximum on
   int ids = 0;
   auto fetch_ids = [&](int t) {  // record ids of the next 64 tiles, one per lane (-1: bad block)
     const int rec = min(4 * (t + lane) + tt, last_rec);
@@ -362,7 +362,7 @@ __global__ __launch_bounds__(kNPThreads, 2) void nibble_prefill_kernel(NibPrefil
 #pragma unroll
   for (int gr = 0; gr < NG; ++gr) {
     nib_query<QDT>(qrow[gr], a.scale_log2, true, qf[gr], qs[gr]);
-    m[gr] = kNPNone;
+    m[gr] = kNibNone;
     l[gr] = 0.f;
 #pragma unroll
     for (int i = 0; i < 8; ++i) acc[gr][i] = float4v{};
@@ -479,18 +479,23 @@ __global__ __launch_bounds__(kNPThreads, 2) void nibble_prefill_kernel(NibPrefil
               if (tok + 16 * tg + i > lim[gr]) sc[gr][tg][i] = -INFINITY;
       }
       // Weights against the maximum as it stands. It has to move only where a lane's sum of eight
-      // exceeds 2^11 (or is NaN): the scores' own maximum is taken in that case alone.
+      // exceeds 2^11 (or is NaN), and the scores' own maximum is taken in that case alone, or where a
+      // row of the wave has a far one.
       half8 pf[NG];
       float sum[NG];
-      auto weights = [&](int gr) {
+      auto weights = [&](int gr, bool apart) {
         sum[gr] = 0.f;
+        auto exponent = [&](float s) {
+          const float e = fmaf(s, qs[gr], -m[gr]);
+          return apart ? nib_apart(s, qs[gr], m[gr]) : e;
+        };
 #pragma unroll
         for (int tg = 0; tg < 2; ++tg)
 #pragma unroll
           for (int i = 0; i < 4; i += 2) {
             // the one rounding on the way to the output; the sum takes the rounded weights
-            const half2v p = {(_Float16)fast_exp2(fmaf(sc[gr][tg][i], qs[gr], -m[gr])),
-                              (_Float16)fast_exp2(fmaf(sc[gr][tg][i + 1], qs[gr], -m[gr]))};
+            const half2v p = {(_Float16)fast_exp2(exponent(sc[gr][tg][i])),
+                              (_Float16)fast_exp2(exponent(sc[gr][tg][i + 1]))};
             sum[gr] = __builtin_amdgcn_fdot2(p, half2v{(_Float16)1.f, (_Float16)1.f}, sum[gr], false);
             pf[gr][4 * tg + i] = p[0];
             pf[gr][4 * tg + i + 1] = p[1];
@@ -499,8 +504,8 @@ __global__ __launch_bounds__(kNPThreads, 2) void nibble_prefill_kernel(NibPrefil
       bool fits = true;
 #pragma unroll
       for (int gr = 0; gr < NG; ++gr) {
-        weights(gr);
-        fits &= sum[gr] <= kNPMost;
+        weights(gr, false);
+        fits &= sum[gr] <= most;
       }
       if (__builtin_amdgcn_ballot_w64(!fits)) {
 #pragma unroll
@@ -516,7 +521,8 @@ __global__ __launch_bounds__(kNPThreads, 2) void nibble_prefill_kernel(NibPrefil
           l[gr] *= f;
 #pragma unroll
           for (int i = 0; i < 8; ++i) acc[gr][i] *= f;
-          weights(gr);
+          weights(gr, nib_far(mn));
+          if (__builtin_amdgcn_ballot_w64(nib_far(mn))) most = -1.f;
         }
       }
 #pragma unroll
@@ -658,7 +664,7 @@ __global__ __launch_bounds__(kNPJoinThreads) void nibble_join_kernel(NibPrefillA
     __syncthreads();
     if (tid == 0) *flag = 0;
     if (tid < kNPJoinRows) {
-      float mm = kNPNone, ll = 0.f;
+      float mm = kNibNone, ll = 0.f;
 #pragma unroll 8
       for (int s = 0; s < J.ns; ++s) mm = fmaxf(mm, wgt[s][tid][0]);
 #pragma unroll 8
