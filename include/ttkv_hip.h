@@ -403,7 +403,8 @@ int ttkv_nibble_write_paged(int32_t H, int32_t d, const void* key, int32_t k_dty
  * are not skipped are distinct. An empty request's row (seq_lens[r] == 0) is 0.
  * A block id outside the cache sets TTKV_ERR_BAD_BLOCK and makes its
  * request's rows NaN. Keys and values enter the products exactly; the query is taken as fp16 (bf16
- * at a power of two per row), and the softmax weight is rounded to fp16 once. `out` may be the query.
+ * at a power of two per row), and the softmax weight is rounded to fp16 once: to 2^-11 of itself down to
+ * 2^-18 of the row's largest, below that to 2^-29 of the largest. `out` may be the query.
  * max_seq_len at most 2^26 and at most the tokens that max_blocks hold; the page at most 2^31 tiles.
  *
  * Workspace, of this call and the next: 256-byte aligned, its first 64 KiB zero before its first call

@@ -1,12 +1,14 @@
 """The 4-bit cache's operators at calls that their documentation allows and that go wrong easily:
 requests without a query, a plan's tensors within one buffer,
-positions of other shapes, outputs that lie in inputs, scores of any size. Helpers and tolerances are test_nibble_gpu's."""
+positions of other shapes, outputs that lie in inputs, scores of any size,
+small weights in numbers. Helpers and tolerances are test_nibble_gpu's."""
 import pytest
 import torch
 
 from oracle import nibble as on
 from test_nibble_gpu import D, HALF, SCALE, Store, _close, _err, _gen, _i32
 from vllm_ttkv import kernels
+from vllm_ttkv.nibble import NibbleLayout
 
 pytestmark = pytest.mark.gpu
 
@@ -208,3 +210,54 @@ def test_scores_far_beyond_the_weights_range(n, Q, dtype, peak, scale):
             want = _winners(level, V, sign, n - Q + j + 1)
             tol = HALF[dtype] * want.abs() + 2.0 ** -24 * n * V.abs().max()
             assert bool(((got[j, p] - want).abs() <= tol).all()), (j, p, got[j, p, :3], want[:3])
+
+
+# ------------------------------------------------------------------ small weights in numbers
+def _far_key(n, at, H=2):
+    """n tokens whose scores are 0 but for token `at`'s, which is the query's first element; its
+    value is 0, the others' are in [1, 2): the output is the sum of the small weights."""
+    g = _gen(n + at)
+    k, v = torch.zeros(n, H, D), 1 + torch.rand(n, H, D, generator=g)
+    k[at, :, 0], v[at] = 1, 0
+    k, v = k.half(), v.half()
+    lay = NibbleLayout(H)
+    blocks = -(-n // 16)
+    page = torch.full((blocks, 16, 144 * H), 255, dtype=torch.uint8, device="cuda")
+    ids = torch.randperm(blocks, generator=g).to(torch.int32)
+    kernels.nibble_write_paged(lay, k.cuda(), v.cuda(), on.table_slots(ids, n, 16).cuda(), page)
+    return lay, page, ids.cuda(), on.values(k), on.values(v)
+
+
+@pytest.mark.parametrize("bits", [15.5, 18.6, 20.4, 22.3, 26.0])
+@pytest.mark.parametrize("kind,B,n,Q,at", [
+    ("decode", 300, 600, 1, 0), ("decode", 300, 600, 1, 599), ("decode", 2, 9000, 1, 4500),
+    ("chunk", 300, 600, 4, 1), ("flash", 20, 2000, 400, 0), ("flash", 20, 2000, 400, 1200),
+    ("flash", 1, 5000, 200, 0)])
+def test_many_small_weights_beside_a_large_one(kind, B, n, Q, at, bits):
+    """Weights of 2^-15 to 2^-26 of the largest: each is rounded to half a step of fp16, 2^-11 of it
+    while it is a normal number and 2^-25 below that, where the largest weight is 2^8 (decode and
+    short chunks) or 2^4 (long ones): 2^-33 and 2^-29 of the largest. Requests share one table."""
+    least = 2.0 ** (-29 if kind == "flash" else -33)
+    lay, page, ids, K, V = _far_key(n, at)
+    scale = 0.6931471805599453
+    H, G = 2, 4 if kind != "flash" else 8
+    q = torch.zeros(Q, H * G, D).half()
+    q[..., 0] = bits
+    all_q = q.repeat(B, 1, 1).cuda()
+    bt = ids.repeat(B, 1).contiguous()
+    seq, qsl, err = _i32([n] * B), _i32([Q * r for r in range(B + 1)]), _err()
+    if kind == "decode":
+        out = kernels.nibble_decode_paged(lay, all_q, page, 16, bt, seq, qsl, n, scale,
+                                          error_word=err)
+    else:
+        out = kernels.nibble_prefill_paged(lay, all_q, page, 16, bt, seq, qsl, Q, n, scale,
+                                           error_word=err)
+    assert int(err) == 0
+    for r in {0, B // 2, B - 1}:
+        for j in {0, Q // 2, Q - 1}:
+            sees = n - Q + j + 1
+            want, spread, score = on.attend(q[j:j + 1], K[:sees], V[:sees], scale)
+            tol = 1.05 * (2.0 ** -11 * want.abs() + (2.0 ** -11 + 2.0 ** -16 * score + 2.0 ** -20)
+                          * spread + sees * least * V.abs().max()) + 2.0 ** -25
+            e = (out[r * Q + j].cpu().double() - want[0]).abs()
+            assert bool((e <= tol[0]).all()), (r, j, float((e / tol[0]).max()))

@@ -120,6 +120,14 @@ __device__ __forceinline__ void nib_query(const NibRow& in, float scale_log2, bo
 constexpr float kNibFar = 4096.f;
 constexpr float kNibNone = -3.402823466e38f;
 __device__ __forceinline__ bool nib_far(float m) { return fabsf(m) > kNibFar && m > kNibNone; }
+// Other rows have m the maximum less `lift`: weights down to 2^-(14 + lift) of the largest are normal
+// fp16 numbers, and smaller ones are rounded to 2^-(25 + lift) of it. (With m the maximum itself 2,000
+// tokens at 2^-20.6 beside one came out 2.8 % off, at 2^-26 as nothing.) m has to move once a key's weight
+// is 2^(16 - lift) times the largest of when it last moved.
+constexpr float kNibMost = 8 * 65504.f;  // a lane's sum of eight weights; beyond it one is infinite
+__device__ __forceinline__ float nib_max(float m, float scores, float lift) {
+  return fmaxf(m, nib_far(scores) ? scores : scores - lift);
+}
 __device__ __forceinline__ float nib_apart(float score, float qs, float m) {
 #pragma clang fp contract(off)
   const float p = score * qs;

@@ -15,7 +15,7 @@
 //     shift and a mask per pair and dequantised exactly in packed fp16; the queries are the B operand,
 //     held in registers. Columns without a row are zero.
 //   softmax in the result's own registers: lane column = row, 8 tokens of it. Weights are taken against
-//     the maximum as it stands, which moves only when a lane's eight sum to more than 2^11, so most
+//     the maximum as it stands, which moves only when a weight leaves fp16 (2^8 growth), so most
 //     steps need no maximum and no exchange between lanes; the sum stays per lane until the end.
 //   O^T [dim, row] += V^T P^T, eight MFMAs: the scores' layout is the B operand's as it
 //     stands, and a lane's 16 value code bytes per tile are its A operand of all eight (a dim pair of
@@ -42,8 +42,8 @@ constexpr int kNDShortRows = 256;      // rows of a chunk that may come here
 constexpr int64_t kNDShortWork = 17000;  // and steps of all its blocks,
 constexpr int64_t kNDFewWork = 24000;    // where they are few
 constexpr int64_t kNDWideWork = 36000;   // from which two groups of 16 rows share a block
-constexpr float kNDMost = 2048.f;      // a lane's sum of eight softmax weights before a rescale
 constexpr int kNDRows = 16;            // rows of a block: a matrix product's columns
+constexpr float kNDLift = 8.f;         // of the weights (nib_max)
 
 struct NibDecodeArgs {
   int H, G;
@@ -259,7 +259,7 @@ __global__ __launch_bounds__(kNDThreads, 2) void nibble_decode_kernel(NibDecodeA
   const int s0 = (int)((int64_t)steps * P.c / P.nch);
   const int s1 = (int)((int64_t)steps * (P.c + 1) / P.nch);
   bool bad = false;
-  float most = kNDMost;  // below every sum from the wave's first far maximum on
+  float most = kNibMost;  // below every sum from the wave's first far maximum on
 
   const NibMasks masks = nib_masks();
   const uint8_t* base = a.page + (int64_t)h * kNibRecord;
@@ -334,8 +334,8 @@ __global__ __launch_bounds__(kNDThreads, 2) void nibble_decode_kernel(NibDecodeA
           }
         }
     }
-    // Weights against the maximum as it stands. It has to move only where a lane's sum of eight
-    // exceeds 2^11 (or is NaN), and the scores' own maximum is taken in that case alone, or where a row
+    // Weights against the maximum as it stands. It has to move only where a weight leaves fp16 and so
+    // makes its lane's sum of eight infinite (or NaN), and the scores' own maximum is taken in that case alone, or where a row
     // of the wave has a far one.
     half8 pf[RG];
     float sum[RG];
@@ -371,7 +371,7 @@ __global__ __launch_bounds__(kNDThreads, 2) void nibble_decode_kernel(NibDecodeA
         for (int t = 0; t < 2; ++t)
 #pragma unroll
           for (int i = 0; i < 4; ++i) mt = fmaxf(mt, sc[r][t][i]);
-        const float mn = fmaxf(m[r], cross_row_max(mt * qs[r]));
+        const float mn = nib_max(m[r], cross_row_max(mt * qs[r]), kNDLift);
         const float f = exp2f(m[r] - mn);
         m[r] = mn;
         l[r] *= f;

@@ -40,7 +40,10 @@ constexpr int kNPPlanLanes = 4;    // requests per lane in the plan: 256 per lau
 constexpr int kNPMaxSplit = 32;
 constexpr int kNPMinTiles = 4;     // keys per part, in tiles (batches that are not searched)
 constexpr int kNPSearch = 16;      // requests up to which the plan searches for the number of parts
-constexpr float kNPMost = 2048.f;  // a lane's sum of eight softmax weights before a rescale
+// Lift of the weights (nib_max): a wave moves its maxima when any of its 48 rows has to. 1 x 2,048 over
+// 12,345 and 4 x 256 over 7,656 took 270.4 and 105.9 us with 0 or 4, 274.5 and 107.7 with 6, 277.7 and 110.2
+// with 8 (decode, bound by memory, 8 in the same time).
+constexpr float kNPLift = 4.f;
 constexpr int64_t kNPPartRows = 127000;  // rows of partial results a launch may leave: 66.0 MB
 constexpr int kNPKBytes = kNPTile * kD * 2;
 constexpr int kNPSmem = 4 * kNPKBytes;  // two buffers of keys and values
@@ -315,7 +318,7 @@ __global__ __launch_bounds__(kNPThreads, 2) void nibble_prefill_kernel(NibPrefil
   const int tt = wv & 3;  // this wave's record of a tile
   const int last_rec = (n - 1) / kNibTile;
   bool bad = false;
-  float most = kNPMost;  // below every sum from the wave's first far maximum on
+  float most = kNibMost;  // below every sum from the wave's first far maximum on
   int ids = 0;
   auto fetch_ids = [&](int t) {  // record ids of the next 64 tiles, one per lane (-1: bad block)
     const int rec = min(4 * (t + lane) + tt, last_rec);
@@ -478,8 +481,8 @@ __global__ __launch_bounds__(kNPThreads, 2) void nibble_prefill_kernel(NibPrefil
             for (int i = 0; i < 4; ++i)
               if (tok + 16 * tg + i > lim[gr]) sc[gr][tg][i] = -INFINITY;
       }
-      // Weights against the maximum as it stands. It has to move only where a lane's sum of eight
-      // exceeds 2^11 (or is NaN), and the scores' own maximum is taken in that case alone, or where a
+      // Weights against the maximum as it stands. It has to move only where a weight leaves fp16 and so
+      // makes its lane's sum of eight infinite (or NaN), and the scores' own maximum is taken in that case alone, or where a
       // row of the wave has a far one.
       half8 pf[NG];
       float sum[NG];
@@ -515,7 +518,7 @@ __global__ __launch_bounds__(kNPThreads, 2) void nibble_prefill_kernel(NibPrefil
           for (int tg = 0; tg < 2; ++tg)
 #pragma unroll
             for (int i = 0; i < 4; ++i) mt = fmaxf(mt, sc[gr][tg][i]);
-          const float mn = fmaxf(m[gr], cross_row_max(mt * qs[gr]));
+          const float mn = nib_max(m[gr], cross_row_max(mt * qs[gr]), kNPLift);
           const float f = exp2f(m[gr] - mn);
           m[gr] = mn;
           l[gr] *= f;
