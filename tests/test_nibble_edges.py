@@ -2,6 +2,8 @@
 launched)."""
 import ctypes
 
+import torch
+
 from vllm_ttkv import _hip
 
 
@@ -76,3 +78,26 @@ def test_rotary_refuses_outputs_that_overlap():
     _refused(_rotary(qo=q, qos=64, ko=q, kos=64), 1, "overlaps the other")
     _refused(_rotary(qo=0x20000, ko=0x20000, qos=32, kos=32), 1, "overlaps the other")
     _refused(_rotary(qo=0x20000, ko=0x20030 + 128, qos=64, kos=64), 1, "overlaps the other")
+
+
+# ----------------------------------------------------------------------------- workspace sizes
+def test_workspaces_grow_with_every_argument():
+    """With the KV heads and with the query heads too: one buffer serves layers of unlike heads."""
+    L, g = _hip.lib(), torch.Generator().manual_seed(5)
+
+    def draw(most):
+        return int(2 ** (float(torch.rand(1, generator=g)) * most))
+
+    for _ in range(400):
+        HQ, R, n = 12 * draw(4), draw(9), draw(17)
+        q = min(draw(12), n)
+        heads = [h for h in range(1, HQ + 1) if HQ % h == 0 and HQ // h <= 16]
+        decode = [L.ttkv_nibble_decode_workspace_bytes(h, HQ, R, n) for h in heads]
+        prefill = [L.ttkv_nibble_prefill_workspace_bytes(h, HQ, R, q, n) for h in heads]
+        assert decode == sorted(decode) and prefill == sorted(prefill) and decode[0] >= 65536
+        h = heads[draw(3) % len(heads)]
+        for k in (h, 2 * h, 5 * h):                                 # more query heads
+            assert L.ttkv_nibble_decode_workspace_bytes(h, HQ, R, n) \
+                <= L.ttkv_nibble_decode_workspace_bytes(h, HQ + k, R, n)
+            assert L.ttkv_nibble_prefill_workspace_bytes(h, HQ, R, q, n) \
+                <= L.ttkv_nibble_prefill_workspace_bytes(h, HQ + k, R, q, n)

@@ -1,7 +1,7 @@
 """The 4-bit cache's operators at calls that their documentation allows and that go wrong easily:
 requests without a query, a plan's tensors within one buffer,
 positions of other shapes, outputs that lie in inputs, scores of any size,
-small weights in numbers. Helpers and tolerances are test_nibble_gpu's."""
+small weights in numbers, layers of unlike heads. Helpers and tolerances are test_nibble_gpu's."""
 import pytest
 import torch
 
@@ -261,3 +261,29 @@ def test_many_small_weights_beside_a_large_one(kind, B, n, Q, at, bits):
                           * spread + sees * least * V.abs().max()) + 2.0 ** -25
             e = (out[r * Q + j].cpu().double() - want[0]).abs()
             assert bool((e <= tol[0]).all()), (r, j, float((e / tol[0]).max()))
+
+
+# ---------------------------------------------------------- a workspace for layers of unlike heads
+def test_one_workspace_for_layers_of_unlike_heads():
+    """Sixteen query heads over 16, 4, 2 and 1 KV heads on the buffer of the first's size."""
+    lens, HQ = [5000, 300, 40], 16
+    for counts in ([1, 1, 1], [9, 2, 5], [150, 300, 40]):
+        lay, most = NibbleLayout(16), max(counts)
+        ws = torch.zeros(max(kernels.nibble_prefill_workspace(lay, HQ, 3, most, 5000, "cpu").numel(),
+                             kernels.nibble_decode_workspace(lay, HQ, 3, 5000, "cpu").numel()),
+                         dtype=torch.uint8, device="cuda")
+        for H in (16, 4, 1, 2):
+            st = Store(lens, H, seed=70 + H)
+            q = torch.randn(sum(counts), HQ, D, generator=_gen(71)).half()
+            qsl, err = _starts(counts), _err()
+            args = (st.lay, q.cuda(), st.page, 16, st.bt, st.seq, _i32(qsl))
+            outs = [kernels.nibble_prefill_paged(*args, most, 5000, SCALE, workspace=ws,
+                                                 error_word=err)]
+            if most == 1:
+                outs.append(kernels.nibble_decode_paged(*args, 5000, SCALE, workspace=ws,
+                                                        error_word=err))
+            assert int(err) == 0
+            for out in outs:
+                for r in range(3):
+                    s = slice(qsl[r], qsl[r + 1])
+                    _close(out[s], q[s], *st.kv(r), SCALE, (H, counts, r))

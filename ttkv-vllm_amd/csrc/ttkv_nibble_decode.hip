@@ -638,10 +638,14 @@ static int nd_groups(int H, int num_reqs, int rows, int max_seq) {
   return items > nd_target() || items * steps > kNDWideWork ? 2 : 1;
 }
 
+// Rows of a (request, KV head) per query position at most, whatever the KV heads: the sizes below grow
+// with every argument, so that layers of unlike heads share a workspace.
+static int nd_most_rows(int HQ) { return std::min(HQ, 16); }
+
 int64_t nibble_decode_workspace_bytes(int H, int HQ, int num_reqs, int max_seq) {
-  if (num_reqs == 0 || H > kMaxCounters) return 256;
+  if (num_reqs == 0) return 256;
   const int64_t pairs = (int64_t)nd_slice(H, 1, num_reqs) * H;
-  return kCounterBytes + nd_parts(pairs, max_seq) * (HQ / H) * (kD + 2) * 4;
+  return kCounterBytes + nd_parts(pairs, max_seq) * nd_most_rows(HQ) * (kD + 2) * 4;
 }
 
 // Chunks of at most 32 rows take this kernel, and longer ones while the whole call is short: it reads
@@ -666,7 +670,7 @@ bool nibble_short_applies(int H, int HQ, int num_reqs, int max_q, int max_seq) {
 
 // Bytes of partial results of such a chunk call at most, growing with every argument.
 int64_t nibble_short_part_bytes(int H, int HQ, int num_reqs, int max_q, int max_seq) {
-  const int rows = (int)std::min<int64_t>((int64_t)max_q * (HQ / H), kNDShortRows);
+  const int rows = (int)std::min<int64_t>((int64_t)max_q * nd_most_rows(HQ), kNDShortRows);
   const int64_t pairs = std::min<int64_t>(
       std::min<int64_t>(num_reqs, kMaxCounters) * std::min(H, kMaxCounters) * nd_blocks(rows, 1), kMaxCounters);
   return nd_parts(pairs, max_seq) * std::min(rows, 2 * kNDRows) * (kD + 2) * 4;

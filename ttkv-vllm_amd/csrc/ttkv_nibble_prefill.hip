@@ -799,14 +799,14 @@ static int64_t np_join_bytes(const NibPrefillSlice& s) {
 }
 
 // An upper bound that grows with every argument, so that a workspace for the largest batch serves the
-// others: a join record for every row block that the flags can serve, of 128 rows each, and the parts of
-// either kernel.
+// others: a join record for every row block that the flags can serve, of 128 rows each (a request has
+// max_q HQ / 128 of them and, for what its heads round up, less than H more), and the parts of either
+// kernel.
 int64_t nibble_prefill_workspace_bytes(int H, int HQ, int num_reqs, int max_q, int max_seq) {
   if (num_reqs == 0 || max_q == 0) return 256;
-  const int64_t rows = (int64_t)max_q * (HQ / H), rw = kNPWaves * 16;
-  int64_t blocks = 1;
-  for (int64_t x : {(rows + rw - 1) / rw, (int64_t)H, (int64_t)num_reqs})
-    blocks = std::min(blocks * std::min(x, kCounterBytes), kCounterBytes / (rw / kNPJoinRows));
+  const int64_t rw = kNPWaves * 16, most = kCounterBytes / (rw / kNPJoinRows);
+  const int64_t per = std::min((int64_t)max_q * HQ / rw + H, most);
+  const int64_t blocks = std::min(per * std::min<int64_t>(num_reqs, most), most);
   const int64_t joins = (blocks * (int64_t)sizeof(NibPrefillJoin) + 255) / 256 * 256;
   const int64_t parts = np_part_rows(HQ, num_reqs, max_q, max_seq) * (kD + 2) * 4;
   return kCounterBytes + std::max(joins + parts, nibble_short_part_bytes(H, HQ, num_reqs, max_q, max_seq));
