@@ -1,7 +1,8 @@
 """The 4-bit cache's operators at calls that their documentation allows and that go wrong easily:
 requests without a query, a plan's tensors within one buffer,
 positions of other shapes, outputs that lie in inputs, scores of any size,
-small weights in numbers, layers of unlike heads. Helpers and tolerances are test_nibble_gpu's."""
+small weights in numbers, layers of unlike heads, steps without
+tokens. Helpers and tolerances are test_nibble_gpu's."""
 import pytest
 import torch
 
@@ -287,3 +288,30 @@ def test_one_workspace_for_layers_of_unlike_heads():
                 for r in range(3):
                     s = slice(qsl[r], qsl[r + 1])
                     _close(out[s], q[s], *st.kv(r), SCALE, (H, counts, r))
+
+
+# ------------------------------------------------------------------------ a step without tokens
+def test_a_step_without_tokens():
+    """Every request waits and nothing is padded: plan, rotation, write and both reads take a step of
+    no tokens."""
+    st = Store([40, 700], 2, seed=80)
+    lay, H, HQ = st.lay, 2, 8
+    page, cs = st.page.clone(), torch.randn(50, D).cuda()
+
+    def step():
+        err = _err()
+        p = kernels.step_plan(st.seq, _i32([0, 0]), st.bt, _i32([0]), 16, st.blocks, 0, error_word=err)
+        q, k = (torch.zeros(0, h, D, dtype=torch.float16, device="cuda") for h in (HQ, H))
+        pos = torch.zeros(3, 0, dtype=torch.int64, device="cuda")
+        qr, kr = kernels.rotary_axes(q, k, pos, cs, (16, 24, 24), error_word=err)
+        kernels.nibble_write_paged(lay, kr, k, p.slot_mapping, st.page, error_word=err)
+        args = (lay, qr, st.page, 16, st.bt, p.seq_lens, p.query_start_loc)
+        outs = [kernels.nibble_decode_paged(*args, 700, SCALE, error_word=err),
+                kernels.nibble_prefill_paged(*args, 0, 700, SCALE, error_word=err),
+                kernels.nibble_prefill_paged(*args, 64, 700, SCALE, error_word=err),
+                kernels.nibble_prefill_paged(*args, 300, 700, SCALE, req_index=_i32([1]),
+                                             error_word=err)]
+        assert int(err) == 0 and all(tuple(o.shape) == (0, HQ, D) for o in outs)
+        assert p.query_start_loc.tolist() == [0, 0, 0] and p.seq_lens.tolist() == [40, 700]
+    step()
+    assert torch.equal(st.page, page)

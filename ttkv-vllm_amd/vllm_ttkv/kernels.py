@@ -671,6 +671,8 @@ def nibble_decode_paged(lay: NibbleLayout, query: torch.Tensor, page: torch.Tens
     B, HQ = seq_lens.numel(), query.shape[1]
     if block_table.shape[0] < B or query_start_loc.numel() < B:
         raise ValueError(f"{B} sequence lengths need as many block table rows and query rows")
+    if query.shape[0] == 0:                     # every request waits
+        return out
     if workspace is None:
         workspace = nibble_decode_workspace(lay, HQ, B, max_seq_len, query.device)
     err = _error_word(error_word, query.device)
@@ -713,6 +715,8 @@ def nibble_prefill_paged(lay: NibbleLayout, query: torch.Tensor, page: torch.Ten
     if block_table.shape[0] < B or query_start_loc.numel() < B + 1:
         raise ValueError(f"{B} sequence lengths need as many block table rows and one more "
                          f"query start")
+    if query.shape[0] == 0:
+        return out
     if req_index is not None:
         _i32(req_index, "req_index")
         B = req_index.numel()
