@@ -435,7 +435,9 @@ int ttkv_nibble_decode_starts_paged(int32_t H, int32_t num_heads, int32_t d, flo
 
 /* Causal attention of chunks of queries over the 4-bit cache: request r's Q queries sit at the end
  * of its n = seq_lens[r] stored keys (their own included; a first chunk has n = Q), query j sees
- * keys t <= n - Q + j. Arguments as for ttkv_prefill_paged, limits and precision as above. A request
+ * keys t <= n - Q + j. Arguments as for ttkv_prefill_paged, limits and precision as above (where `out` is
+ * the query, req_index names no row twice). Every request is sized by max_q_len: give a step's single
+ * queries and its long chunks a call each, by req_index. A request
  * with n < Q sets TTKV_ERR_SEQ_LEN and its rows become NaN; one with Q > max_q_len or n > max_seq_len
  * sets it and has its first max_q_len queries, or its first max_seq_len keys, taken. Of a request with
  * a block id outside the cache, the rows that see the block become NaN, and others of it may. */

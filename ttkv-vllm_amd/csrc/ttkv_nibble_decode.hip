@@ -21,8 +21,8 @@
 //     stands, and a lane's 16 value code bytes per tile are its A operand of all eight (a dim pair of
 //     each group, four tokens). The result's column is the row again, so the rescale is a lane's factor.
 // Bytes per step 4,608; the two register sets keep the next step's loads in flight. Bound by memory: 8 x
-// 14,402 tokens of 8 heads, 133 MB, 30.2 us, 4.4 TB/s (a copy reaches 4.8); the loads alone took 26 us
-// of a profiled 33. 61 requests of 70 to 2,900 tokens 27.8 us for 98 MB; one of 1,082 tokens 9 us, the
+// 14,402 tokens of 8 heads, 133 MB, 30.2 to 33 us by card, 4.4 TB/s at best (a copy reaches 4.8); the
+// loads alone took 26 us of a profiled 33. 61 requests of 70 to 2,900 tokens 27.6 us for 98 MB; one of 1,082 tokens 9 us, the
 // chain of plan, block ids, codes, hand-off and join.
 #include <math.h>
 
@@ -349,7 +349,8 @@ __global__ __launch_bounds__(kNDThreads, 2) void nibble_decode_kernel(NibDecodeA
       for (int t = 0; t < 2; ++t)
 #pragma unroll
         for (int i = 0; i < 4; i += 2) {
-          // the one rounding on the way to the output; the sum takes the rounded weights
+          // the one rounding on the way to the output, to the value product's 16-bit operand (low parts
+          // in a second product would double it); the sum takes the rounded weights
           const half2v p = {(_Float16)fast_exp2(exponent(sc[r][t][i])),
                             (_Float16)fast_exp2(exponent(sc[r][t][i + 1]))};
           sum[r] = __builtin_amdgcn_fdot2(p, half2v{(_Float16)1.f, (_Float16)1.f}, sum[r], false);
@@ -600,7 +601,7 @@ __global__ __launch_bounds__(kNDThreads, 2) void nibble_decode_kernel(NibDecodeA
 }
 
 // The plan's item target: two workgroups per CU. A third would fit beside them, but shorter chunks
-// pay their prologue and join more often (8 x 14,402 tokens: 30.7 us at two per CU, 35.7 at two and a
+// pay their prologue and join more often (8 x 14,402 tokens on one card: 30.7 us at two per CU, 35.7 at two and a
 // half, 32.8 at three; 61 requests of 70 to 2,900: 28.6, 28.2, 31.0).
 static int nd_target() { return 2 * device_cu_count(); }
 

@@ -18,7 +18,8 @@
 // Bound by instruction issue: per tile of 384 rows a SIMD's two waves have 192 products of 16 cycles and
 // about 750 vector instructions (softmax, dequantisation) that take 4 cycles each beside them; 5,900
 // cycles in all, with the clock near 1.95 GHz when every CU works. 1 x 2,048 queries of 32 heads over 12,345
-// keys: 274 us, 1,040 TFLOP/s (a large library product 1,250); 4 x 256 of 24 heads over 7,656: 106 us.
+// keys: 270 to 283 us by card, 1,050 TFLOP/s at best (a large library product 1,250); 4 x 256 of 24 heads
+// over 7,656: 105 to 111.
 //
 // The keys of a row block are split over several workgroups where the batch has too few row blocks
 // to fill the chip: the split comes from a plan that every workgroup computes alike from the lengths
@@ -44,7 +45,9 @@ constexpr int kNPSearch = 16;      // requests up to which the plan searches for
 // 12,345 and 4 x 256 over 7,656 took 270.4 and 105.9 us with 0 or 4, 274.5 and 107.7 with 6, 277.7 and 110.2
 // with 8 (decode, bound by memory, 8 in the same time).
 constexpr float kNPLift = 4.f;
-constexpr int64_t kNPPartRows = 127000;  // rows of partial results a launch may leave: 66.0 MB
+// Rows of partial results a launch may leave, 66.0 MB: a workspace stays below 64 MiB, and calls that
+// would leave more have row blocks enough to fill the chip with fewer parts.
+constexpr int64_t kNPPartRows = 127000;
 constexpr int kNPKBytes = kNPTile * kD * 2;
 constexpr int kNPSmem = 4 * kNPKBytes;  // two buffers of keys and values
 
@@ -105,7 +108,7 @@ __device__ __forceinline__ int np_each(int T, int parts) {
 
 // An estimate of a launch's time in us, from what these kernels measured: a tile of a row block takes
 // 1.55, 2.05 and 3.0 us with one, two and three groups of rows per wave (16 x 384 rows over 24,000 and
-// 48,000 keys) and a block 5 us beside its tiles (4 x 1,432 rows over 180 keys, 8 heads); the items, of
+// 48,000 keys; eight KV heads, 256 CUs) and a block 5 us beside its tiles (4 x 1,432 rows over 180 keys, 8 heads); the items, of
 // `load` tiles in all, take whole rounds of the CUs, and no less than the longest; a split costs its join
 // and, per partial row, 520 bytes written and read.
 __host__ __device__ inline float np_cost(int ng, float longest, float load, float items, float cus,
@@ -496,7 +499,8 @@ __global__ __launch_bounds__(kNPThreads, 2) void nibble_prefill_kernel(NibPrefil
         for (int tg = 0; tg < 2; ++tg)
 #pragma unroll
           for (int i = 0; i < 4; i += 2) {
-            // the one rounding on the way to the output; the sum takes the rounded weights
+            // the one rounding on the way to the output, to the value product's 16-bit operand (low
+            // parts in a second product would double it); the sum takes the rounded weights
             const half2v p = {(_Float16)fast_exp2(exponent(sc[gr][tg][i])),
                               (_Float16)fast_exp2(exponent(sc[gr][tg][i + 1]))};
             sum[gr] = __builtin_amdgcn_fdot2(p, half2v{(_Float16)1.f, (_Float16)1.f}, sum[gr], false);

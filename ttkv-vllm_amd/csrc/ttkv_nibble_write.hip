@@ -11,9 +11,9 @@
 // that fp32 holds by less than q 2^-44 before it is rounded. 32-bit inputs are divided in 64 bits.
 // The scale's range and its quotient by 15 are taken in 64 bits for every type.
 //
-// Bound by the instructions of the quantisation, about 300 per wave: 2,048 tokens of 8 heads in bf16, 15
-// MB with the stored values returned, 7.5 us (a row over 32 lanes and library divisions: 13); a few
-// tokens are one chain of round trips, 3.3 us.
+// Bound by the instructions of the quantisation, 306 per wave: 2,048 tokens of 8 heads in bf16, 19 MB with
+// the stored values returned, 7.6 us with vector issue at 90 % (a row over 32 lanes and library divisions:
+// 13; fp32 9.4, fp16 with bf16 9.7); a few tokens are one chain of round trips, 3.5 us.
 #include <math.h>
 
 #include "ttkv_host.h"

@@ -14,8 +14,9 @@ namespace ttkv {
 // few thousand integers from L2, cheaper than a second launch that waits for a first) and then
 // takes its share of the tokens, finding each one's request by bisection. A token of a fresh block
 // reads its block id from the free list and not from the table, which other workgroups are writing.
-// Bound by the chain of dependent reads: 3 us for 8 single tokens, 8 for 256 requests of up to 120
-// (the scan over the workgroup, then seven steps of bisection in LDS); a few KB move.
+// Bound by the chain of dependent reads: 3 us for 8 single tokens, 8.7 for 256 requests of up to 120
+// (the scan over the workgroup, then for each of a thread's four tokens eight steps of bisection in LDS
+// and two reads); a few KB move.
 constexpr int kPlanThreads = 256;
 constexpr int kPlanTokens = 4;        // tokens per thread the grid is sized for
 constexpr int kPlanMaxReqs = 8000;    // two prefix arrays within 64 KB of LDS
@@ -310,9 +311,9 @@ __device__ __forceinline__ void rot_store8(void* p, int64_t i, const float v[8])
 // One wave per token. Lane j first looks up frequency j's cosine and sine (one load each, whatever
 // the axes) and leaves them in LDS; then the lanes take (head, 8 frequencies) pairs of 16-byte pieces,
 // four heads' loads in flight at a time, the first four asked for before the lookup. Bound by memory:
-// every query and key byte read and written once. 8,192 tokens of 40 heads in bf16, 171 MB: 37.3 us,
+// every query and key byte read and written once. 8,192 tokens of 40 heads in bf16, 171 MB: 36.9 us,
 // 4.6 TB/s (a copy reaches 4.8; loads that stay in the cache 41.3, the kernel below, a pair per thread,
-// 116).
+// 90).
 constexpr int kRotHalf = 128;  // frequencies the LDS holds
 constexpr int kRotBatch = 4;
 template <int DT>
@@ -398,7 +399,7 @@ __global__ __launch_bounds__(64) void rotary_rows_kernel(RotArgs a) {
 }
 
 // Rows whose pieces of 8 are not 16-byte aligned, or longer than the wave kernel's table: one pair
-// per thread.
+// per thread. 8,192 tokens of 40 heads in bf16 90 us, where aligned rows on the same card take 39.
 __global__ __launch_bounds__(256) void rotary_axes_kernel(RotArgs a) {
   const int64_t tok = blockIdx.x;
   int64_t p[kRotAxes];
