@@ -323,7 +323,7 @@ int ttkv_container_v_out(int32_t H, int32_t num_heads, int32_t d, int32_t B, int
  *
  * A group of 32 dims x of a token's key or value row is stored as
  *   lo = min(0, min x), hi = max(0, max x)                 (x clamped to +-32640 first)
- *   s  = (hi - lo) / 15 rounded up to 7 significant bits, at least 2^-14
+ *   s  = (hi - lo) / 15, in 64 bits, rounded up to 7 significant bits, at least 2^-14
  *   z  = rint(-lo / s) in [0, 15],  c = clamp(rint(x / s) + z, 0, 15),  value = (c - z) * s
  * (exact in fp16), with the parameter fp16 bits of s | z (s's low four bits are zero); a group that
  * holds a NaN or an infinity has the parameter 0x7e00 and reads back as NaN.

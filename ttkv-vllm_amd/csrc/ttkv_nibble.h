@@ -4,7 +4,7 @@
 // A group of 32 dims of a token's key (or value) row x is stored as 32 codes of 4 bits and one
 // 16-bit parameter:
 //   lo = min(0, min x), hi = max(0, max x)            (x clamped to +-32640 first)
-//   s  = (hi - lo) / 15 rounded up to 7 significant bits, at least 2^-14
+//   s  = (hi - lo) / 15, in 64 bits, rounded up to 7 significant bits, at least 2^-14
 //   z  = rint(-lo / s) in [0, 15],  c = clamp(rint(x / s) + z, 0, 15),  value = (c - z) * s
 // s is an fp16 number whose low four mantissa bits are zero; the parameter holds z there. c - z has
 // 4 bits and s 7, so a value is exact in fp16: the reads feed it to the matrix units unrounded. A

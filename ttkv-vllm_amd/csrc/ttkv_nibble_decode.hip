@@ -22,8 +22,8 @@
 //     each group, four tokens). The result's column is the row again, so the rescale is a lane's factor.
 // Bytes per step 4,608; the two register sets keep the next step's loads in flight. Bound by memory: 8 x
 // 14,402 tokens of 8 heads, 133 MB, 30.2 to 33 us by card, 4.4 TB/s at best (a copy reaches 4.8); the
-// loads alone took 26 us of a profiled 33. 61 requests of 70 to 2,900 tokens 27.6 us for 98 MB; one of 1,082 tokens 9 us, the
-// chain of plan, block ids, codes, hand-off and join.
+// loads alone took 26 us of a profiled 33. 61 requests of 70 to 2,900 tokens 27.6 us for 98 MB; one of
+// 1,082 tokens 9 us, the chain of plan, block ids, codes, hand-off and join.
 #include <math.h>
 
 #include <type_traits>
@@ -335,8 +335,8 @@ __global__ __launch_bounds__(kNDThreads, 2) void nibble_decode_kernel(NibDecodeA
         }
     }
     // Weights against the maximum as it stands. It has to move only where a weight leaves fp16 and so
-    // makes its lane's sum of eight infinite (or NaN), and the scores' own maximum is taken in that case alone, or where a row
-    // of the wave has a far one.
+    // makes its lane's sum of eight infinite (or NaN): the scores' own maximum is taken in that case
+    // alone, or where a row of the wave has a far one.
     half8 pf[RG];
     float sum[RG];
     auto weights = [&](int r, bool apart) {
@@ -601,8 +601,8 @@ __global__ __launch_bounds__(kNDThreads, 2) void nibble_decode_kernel(NibDecodeA
 }
 
 // The plan's item target: two workgroups per CU. A third would fit beside them, but shorter chunks
-// pay their prologue and join more often (8 x 14,402 tokens on one card: 30.7 us at two per CU, 35.7 at two and a
-// half, 32.8 at three; 61 requests of 70 to 2,900: 28.6, 28.2, 31.0).
+// pay their prologue and join more often (8 x 14,402 tokens on one card: 30.7 us at two per CU, 35.7 at
+// two and a half, 32.8 at three; 61 requests of 70 to 2,900: 28.6, 28.2, 31.0).
 static int nd_target() { return 2 * device_cu_count(); }
 
 // Requests per launch, of `blocks` row blocks each: the plan's lanes, and a counter per (block, head).

@@ -108,9 +108,9 @@ __device__ __forceinline__ int np_each(int T, int parts) {
 
 // An estimate of a launch's time in us, from what these kernels measured: a tile of a row block takes
 // 1.55, 2.05 and 3.0 us with one, two and three groups of rows per wave (16 x 384 rows over 24,000 and
-// 48,000 keys; eight KV heads, 256 CUs) and a block 5 us beside its tiles (4 x 1,432 rows over 180 keys, 8 heads); the items, of
-// `load` tiles in all, take whole rounds of the CUs, and no less than the longest; a split costs its join
-// and, per partial row, 520 bytes written and read.
+// 48,000 keys; eight KV heads, 256 CUs) and a block 5 us beside its tiles (4 x 1,432 rows over 180 keys,
+// 8 heads); the items, of `load` tiles in all, take whole rounds of the CUs, and no less than the longest;
+// a split costs its join and, per partial row, 520 bytes written and read.
 __host__ __device__ inline float np_cost(int ng, float longest, float load, float items, float cus,
                                          float need) {
   const float tile = ng == 1 ? 1.55f : ng == 2 ? 2.05f : 3.0f;
@@ -484,9 +484,9 @@ __global__ __launch_bounds__(kNPThreads, 2) void nibble_prefill_kernel(NibPrefil
             for (int i = 0; i < 4; ++i)
               if (tok + 16 * tg + i > lim[gr]) sc[gr][tg][i] = -INFINITY;
       }
-      // Weights against the maximum as it stands. It has to move only where a weight leaves fp16 and so
-      // makes its lane's sum of eight infinite (or NaN), and the scores' own maximum is taken in that case alone, or where a
-      // row of the wave has a far one.
+      // Weights against the maximum as it stands. It has to move only where a weight leaves fp16 and
+      // so makes its lane's sum of eight infinite (or NaN): the scores' own maximum is taken in that
+      // case alone, or where a row of the wave has a far one.
       half8 pf[NG];
       float sum[NG];
       auto weights = [&](int gr, bool apart) {
