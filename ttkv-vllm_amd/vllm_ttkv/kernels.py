@@ -662,8 +662,8 @@ def nibble_decode_paged(lay: NibbleLayout, query: torch.Tensor, page: torch.Tens
     over its seq_lens[r] stored tokens of a 4-bit cache. See `ttkv_nibble_decode_paged` in
     include/ttkv_hip.h. Returns `out` [N, HQ, d] with the decode rows written.
 
-    query_start_loc [B] or, as `step_plan` writes it, [B + 1]: a request whose entry equals the next
-    one has no query in this step and is skipped."""
+    query_start_loc [B] or, as `step_plan` writes it, [B + 1] (of a longer one its first B + 1): a
+    request whose entry equals the next one has no query in this step and is skipped."""
     index = _one_device(query, page, block_table, seq_lens, query_start_loc, out, workspace,
                         error_word)
     out, q_args, bt_args, out_args = _nibble_read(lay, query, page, block_table, seq_lens,
