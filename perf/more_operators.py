@@ -353,7 +353,7 @@ def _quantise(x):
     """Codes [..., d] as bytes, and the bytes of their groups' powers of two, of x [..., d]."""
     t = x.double().reshape(*x.shape[:-1], -1, 32)
     m, e = torch.frexp(t.abs().amax(-1))            # 448 = 0.875 * 2^9
-    byte = (e + 127 - 9 + (m > 0.875)).clamp(min=127 - 117)
+    byte = torch.where(m == 0, 0, e + 127 - 9 + (m > 0.875)).clamp(min=127 - 117)
     code = (t * _two(254 - byte)[..., None]).float().to(torch.float8_e4m3fn)
     return code.view(torch.uint8).reshape(x.shape), byte.to(torch.uint8)
 
@@ -478,7 +478,7 @@ def _exact_codes(x):
     """(code values, powers of two) of x in 64 bits, by the grid of each value's own exponent."""
     g = x.double().reshape(*x.shape[:-1], -1, 32)
     top = g.abs().amax(-1)
-    e = (torch.frexp(top)[1] - 9).clamp(min=-117)
+    e = torch.where(top == 0, -117, torch.frexp(top)[1] - 9).clamp(min=-117)
     e = e + (top > 448 * _exact_power(e)).int()
     y = g / _exact_power(e)[..., None]
     step = _exact_power((torch.frexp(y)[1] - 1).clamp(min=-6) - 3)
