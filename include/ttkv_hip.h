@@ -42,7 +42,7 @@ enum {
   TTKV_ERR_BAD_BLOCK = 2,    /* a block id outside [0, num_blocks) inside a request's used prefix */
   TTKV_ERR_BAD_SLOT = 4,     /* slot_mapping entry past the cache (PAD entries, < 0, are skipped) */
   TTKV_ERR_SEQ_LEN = 8,      /* seq_lens[r] (or a query count) beyond what the call was sized for (clamped), or a continuation with seq_len < q_len */
-  TTKV_ERR_BAD_POSITION = 16, /* a rotary position outside [0, max_position) */
+  TTKV_ERR_BAD_POSITION = 16, /* a rotary position outside [0, max_position), or [0, 2^31) without a table */
   TTKV_ERR_NO_BLOCK = 32,    /* a step needs more blocks than its free list holds */
 };
 
@@ -453,6 +453,106 @@ int ttkv_nibble_prefill_paged(int32_t H, int32_t num_heads, int32_t d, float sca
                               int32_t out_dtype, int64_t out_row_stride, void* workspace,
                               int64_t workspace_bytes, int32_t* error_word,
                               ttkv_stream_t stream);
+
+/* Rotary positions without a table of angles, for contexts that a table does not reach and for models
+ * whose pairs are adjacent elements. query [N, num_heads, d] and key [N, H, d] (same dtype; either may
+ * be absent with 0 heads) are rotated into query_out / key_out (which may be query and key at the same
+ * strides; otherwise outputs overlap nothing): for j < rotary_dim / 2, with the angle
+ * 2 pi positions[i] turns[j] of token i and (cos, sin) both times `amplitude`,
+ *   y[u] = x[u] cos - x[v] sin,   y[v] = x[v] cos + x[u] sin
+ * of the pair (u, v) = (j, j + rotary_dim / 2) or, adjacent, (2 j, 2 j + 1); dims past rotary_dim are
+ * copied. turns [rotary_dim / 2] fp64 (device memory): revolutions per position, so scaled frequencies of
+ * any rule. Angles are formed in 64 bits, products and sums in 32, rounded once. rotary_dim even, at
+ * most 1,024. A position outside [0, 2^31) sets TTKV_ERR_BAD_POSITION and its rows become NaN. */
+int ttkv_rotary_scaled(const void* query, const void* key, void* query_out, void* key_out,
+                       int32_t dtype, int32_t num_tokens, int32_t num_heads, int32_t H, int32_t d,
+                       int64_t q_row_stride, int64_t k_row_stride, int64_t q_out_row_stride,
+                       int64_t k_out_row_stride, const int64_t* positions, const double* turns,
+                       int32_t rotary_dim, float amplitude, int32_t adjacent, int32_t* error_word,
+                       ttkv_stream_t stream);
+
+/* ---- The 8-bit cache: rotated keys and values as e4m3 codes with a power of two per 32 dims, for layers
+ * that 4 bits do not serve, heads of 64, 128 or 256 dims, sliding windows and attention sinks. No
+ * counterpart in the reference.
+ *
+ * A group of 32 dims x of a token's key or value row is stored as
+ *   2^e the smallest power of two with max |x| <= 448 * 2^e, e >= -117   (x clamped to +-1.75 * 2^127)
+ *   code = e4m3(x / 2^e), to the nearest, ties to even;  byte = e + 127;  value = code * 2^e
+ * (exact in bf16); a group that holds a NaN or an infinity reads back as NaN.
+ *
+ * Page: slot s of block b, b * block_size + offset, at 33 d H / 16 bytes per slot (slot_stride may be
+ * larger); block sizes are multiples of 16. Sixteen slots from a multiple of 16 make a tile of H records
+ * of 33 d bytes at page + (s / 16) * 16 * slot_stride + h * 33 * d. With P = max(1, d / 128), N = d / 16:
+ *      0  key codes, token u, dim x = q (d / 4) + 16 p + c (c < 16) at ((p * 4 + q) * 16 + u) * 16 + c
+ *   16 d  value codes, token u = 4 q + i, dim x = N n + e (e < N): with b = N i + e, at
+ *         (b / 16 * 64 + 16 q + n) * 16 + b % 16
+ *   32 d  key bytes, group g of token u at (g / P * 16 + u) * P + g % P
+ *   32 d + d / 2  value bytes, g * 16 + u */
+
+/* Quantise key / value [N, H, d] (fp32, fp16 or bf16) into their slots of the 8-bit cache. With
+ * rotary_dim > 0 the keys are rotated on the way as ttkv_rotary_scaled rotates them (not rounded in
+ * between), and query [N, num_heads, d] (q_dtype; 0 heads: none) is rotated into query_out, which may be
+ * the query at its stride and otherwise overlaps nothing; with rotary_dim == 0 the keys come rotated and
+ * there are no queries. slot_mapping as for ttkv_write_paged: entries < 0 are padded tokens (not stored;
+ * their queries are rotated and their positions looked at all the same), entries past the cache set
+ * TTKV_ERR_BAD_SLOT; the slots of one call are distinct. key_out / value_out (optional, bf16 [N, H, d])
+ * receive the values that the slots then stand for; rows of tokens that are not stored are left alone.
+ * A position outside [0, 2^31) sets TTKV_ERR_BAD_POSITION; its key is stored as NaN. */
+int ttkv_octet_write_paged(int32_t H, int32_t d, const void* key, int32_t k_dtype,
+                           int64_t k_row_stride, const void* value, int32_t v_dtype,
+                           int64_t v_row_stride, const int64_t* slot_mapping, int32_t num_tokens,
+                           uint8_t* page, int64_t n_slots, int64_t slot_stride, void* key_out,
+                           void* value_out, const int64_t* positions, const double* turns,
+                           int32_t rotary_dim, float amplitude, int32_t adjacent, const void* query,
+                           int32_t q_dtype, int64_t q_row_stride, int32_t num_heads, void* query_out,
+                           int64_t q_out_row_stride, int32_t* error_word, ttkv_stream_t stream);
+
+/* Stored keys and values back as rows, for dense attention over a stored prefix or another worker's
+ * cache. Rows row_start_loc[r] .. [r + 1] - 1 of key_out / value_out [num_rows, H, d] (fp32, fp16 or
+ * bf16; the stored value rounded once, exact in bf16) receive request r's tokens first[r], first[r] + 1,
+ * ... (first null: from 0). Rows that no request has are left alone. A token outside [0, max_seq_len) or
+ * a row outside [0, num_rows) sets TTKV_ERR_SEQ_LEN, a block id outside the cache TTKV_ERR_BAD_BLOCK;
+ * such a token's row becomes NaN, such a row is not written. */
+int ttkv_octet_read_paged(int32_t H, int32_t d, const uint8_t* page, int64_t n_slots,
+                          int64_t slot_stride, int32_t block_size, const int32_t* block_table,
+                          int64_t bt_row_stride, int32_t max_blocks, const int32_t* row_start_loc,
+                          const int32_t* first, int32_t num_reqs, int32_t max_seq_len,
+                          int32_t num_rows, void* key_out, int64_t k_out_row_stride,
+                          void* value_out, int64_t v_out_row_stride, int32_t out_dtype,
+                          int32_t* error_word, ttkv_stream_t stream);
+
+/* Attention of new tokens over the 8-bit cache, the whole batch in one call: request r's Q =
+ * query_start_loc[r + 1] - query_start_loc[r] queries (0: it waits; at most max_q_len, at most 16) sit at
+ * the end of its n = seq_lens[r] stored keys, their own included. Query j, at position p = n - Q + j, sees
+ * the keys t <= p and, with a window > 0, t > p - window:
+ *   out[j] = sum_t softmax_t(scale * q[j] . K[t]) * V[t]
+ * With sinks [num_heads] fp32 the softmax has one more term, exp(sinks[head]), that carries no value; lse
+ * [num_tokens, num_heads] fp32 (optional) receives the logarithm of the softmax's sum, by which results
+ * over parts of a context are joined. query and out [num_tokens, num_heads, d] fp16 or bf16, up to 16
+ * query heads per KV head; `out` may be the query. Rows that no request has are left alone.
+ * A request with n == 0 has rows of 0 and an lse of -infinity, or the sink. One with 0 < n < Q sets
+ * TTKV_ERR_SEQ_LEN and its rows become NaN; one with Q > max_q_len or n > max_seq_len sets it and has its
+ * first max_q_len queries, or its first max_seq_len keys, taken; rows outside [0, num_tokens) set it and
+ * are not taken. A block id outside the cache sets TTKV_ERR_BAD_BLOCK; rows that see the block become NaN,
+ * and others of the request may. Keys, values and queries enter the products exactly, sums are in 32
+ * bits; a score beyond fp32 makes its row NaN.
+ * max_seq_len at most 2^26 and at most the tokens that max_blocks hold; the page at most 2^31 tiles.
+ *
+ * Workspace: as for the 4-bit reads, and one buffer may serve them all, in stream order: 256-byte
+ * aligned, its first 64 KiB zero before its first call and left zero by every call; the size grows with
+ * every argument but H, whose largest counts. Results do not depend on what it held, and repeat bit for bit. */
+int64_t ttkv_octet_decode_workspace_bytes(int32_t H, int32_t num_heads, int32_t d,
+                                          int32_t num_reqs, int32_t max_q_len,
+                                          int32_t max_seq_len);
+int ttkv_octet_decode_paged(int32_t H, int32_t num_heads, int32_t d, float scale,
+                            const void* query, int32_t q_dtype, int64_t q_row_stride,
+                            int32_t num_tokens, const uint8_t* page, int64_t n_slots,
+                            int64_t slot_stride, int32_t block_size, const int32_t* block_table,
+                            int64_t bt_row_stride, int32_t max_blocks, const int32_t* seq_lens,
+                            const int32_t* query_start_loc, int32_t num_reqs, int32_t max_q_len,
+                            int32_t max_seq_len, int32_t window, const float* sinks, void* out,
+                            int32_t out_dtype, int64_t out_row_stride, float* lse, void* workspace,
+                            int64_t workspace_bytes, int32_t* error_word, ttkv_stream_t stream);
 
 /* Message for the last nonzero return on this thread. */
 const char* ttkv_last_error(void);

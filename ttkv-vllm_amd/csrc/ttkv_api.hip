@@ -53,6 +53,70 @@ using namespace ttkv;
 
 extern "C" {
 
+int ttkv_rotary_scaled(const void* query, const void* key, void* query_out, void* key_out,
+                       int32_t dtype, int32_t num_tokens, int32_t num_heads, int32_t H, int32_t d,
+                       int64_t q_row_stride, int64_t k_row_stride, int64_t q_out_row_stride,
+                       int64_t k_out_row_stride, const int64_t* positions, const double* turns,
+                       int32_t rotary_dim, float amplitude, int32_t adjacent, int32_t* error_word,
+                       ttkv_stream_t stream) {
+  return rotary_scaled(query, key, query_out, key_out, dtype, num_tokens, num_heads, H, d,
+                       q_row_stride, k_row_stride, q_out_row_stride, k_out_row_stride, positions,
+                       turns, rotary_dim, amplitude, adjacent, error_word, (hipStream_t)stream);
+}
+
+int ttkv_octet_write_paged(int32_t H, int32_t d, const void* key, int32_t k_dtype,
+                           int64_t k_row_stride, const void* value, int32_t v_dtype,
+                           int64_t v_row_stride, const int64_t* slot_mapping, int32_t num_tokens,
+                           uint8_t* page, int64_t n_slots, int64_t slot_stride, void* key_out,
+                           void* value_out, const int64_t* positions, const double* turns,
+                           int32_t rotary_dim, float amplitude, int32_t adjacent, const void* query,
+                           int32_t q_dtype, int64_t q_row_stride, int32_t num_heads, void* query_out,
+                           int64_t q_out_row_stride, int32_t* error_word, ttkv_stream_t stream) {
+  return octet_write_paged(H, d, key, k_dtype, k_row_stride, value, v_dtype, v_row_stride,
+                           slot_mapping, num_tokens, page, n_slots, slot_stride, key_out, value_out,
+                           positions, turns, rotary_dim, amplitude, adjacent, query, q_dtype,
+                           q_row_stride, num_heads, query_out, q_out_row_stride, error_word,
+                           (hipStream_t)stream);
+}
+
+int ttkv_octet_read_paged(int32_t H, int32_t d, const uint8_t* page, int64_t n_slots,
+                          int64_t slot_stride, int32_t block_size, const int32_t* block_table,
+                          int64_t bt_row_stride, int32_t max_blocks, const int32_t* row_start_loc,
+                          const int32_t* first, int32_t num_reqs, int32_t max_seq_len,
+                          int32_t num_rows, void* key_out, int64_t k_out_row_stride,
+                          void* value_out, int64_t v_out_row_stride, int32_t out_dtype,
+                          int32_t* error_word, ttkv_stream_t stream) {
+  return octet_read_paged(H, d, page, n_slots, slot_stride, block_size, block_table, bt_row_stride,
+                          max_blocks, row_start_loc, first, num_reqs, max_seq_len, num_rows, key_out,
+                          k_out_row_stride, value_out, v_out_row_stride, out_dtype, error_word,
+                          (hipStream_t)stream);
+}
+
+int64_t ttkv_octet_decode_workspace_bytes(int32_t H, int32_t num_heads, int32_t d,
+                                          int32_t num_reqs, int32_t max_q_len,
+                                          int32_t max_seq_len) {
+  if (H <= 0 || num_heads <= 0 || num_heads % H || (d != 64 && d != 128 && d != 256) ||
+      num_reqs < 0 || max_q_len < 0 || max_seq_len < 0)
+    return -1;
+  return octet_decode_workspace_bytes(H, num_heads, d, num_reqs, max_q_len, max_seq_len);
+}
+
+int ttkv_octet_decode_paged(int32_t H, int32_t num_heads, int32_t d, float scale,
+                            const void* query, int32_t q_dtype, int64_t q_row_stride,
+                            int32_t num_tokens, const uint8_t* page, int64_t n_slots,
+                            int64_t slot_stride, int32_t block_size, const int32_t* block_table,
+                            int64_t bt_row_stride, int32_t max_blocks, const int32_t* seq_lens,
+                            const int32_t* query_start_loc, int32_t num_reqs, int32_t max_q_len,
+                            int32_t max_seq_len, int32_t window, const float* sinks, void* out,
+                            int32_t out_dtype, int64_t out_row_stride, float* lse, void* workspace,
+                            int64_t workspace_bytes, int32_t* error_word, ttkv_stream_t stream) {
+  return octet_decode_paged(H, num_heads, d, scale, query, q_dtype, q_row_stride, num_tokens, page,
+                            n_slots, slot_stride, block_size, block_table, bt_row_stride, max_blocks,
+                            seq_lens, query_start_loc, num_reqs, max_q_len, max_seq_len, window,
+                            sinks, out, out_dtype, out_row_stride, lse, workspace, workspace_bytes,
+                            error_word, (hipStream_t)stream);
+}
+
 const char* ttkv_last_error(void) { return t_err.c_str(); }
 
 int32_t ttkv_decoder_ranks(int32_t r1) { return r1 > 0 ? dec_ranks(r1) : -1; }

@@ -25,6 +25,20 @@ inline int check_dec_pool(const int8_t* dec_q, const float* dec_scale) {
   return TTKV_OK;
 }
 
+// Whether rows of `a` and of `b` share bytes: n rows each, of wa and wb bytes at strides sa and sb. Rows
+// of unlike strides are only looked at where they begin.
+inline bool rows_meet(const void* a, int64_t sa, int64_t wa, const void* b, int64_t sb, int64_t wb,
+                          int64_t n) {
+  if (!wa || !wb || !a || !b) return false;
+  const int64_t off = (int64_t)((uintptr_t)b - (uintptr_t)a);
+  auto meet = [&](int64_t o) { return o < wa && -o < wb; };
+  if (n == 1 || sa != sb || sa <= 0) return meet(off);
+  const int64_t k0 = -off / sa;  // row i + k of b lies nearest to row i of a
+  for (int64_t k = k0 - 1; k <= k0 + 1; ++k)
+    if (k > -n && k < n && meet(off + k * sa)) return true;
+  return false;
+}
+
 // Every workspace starts with a fixed region of arrival counters: zero before first use (a fresh
 // zero-filled buffer), left zero by every call. It sits at the same offset with the same size
 // whatever the call's shape, so one buffer can serve calls of any shape in turn: a call's data
@@ -171,4 +185,31 @@ int nibble_prefill_paged(int H, int HQ, int d, float scale, const void* q, int q
                          const int32_t* req_index, int num_reqs, int max_q, int max_seq,
                          void* out, int out_dtype, int64_t out_row_stride, void* ws,
                          int64_t ws_bytes, int32_t* err, hipStream_t st);
+}  // namespace ttkv
+
+namespace ttkv {
+int rotary_scaled(const void* q, const void* k, void* qo, void* ko, int dtype, int N, int HQ, int H, int d,
+                  int64_t q_stride, int64_t k_stride, int64_t qo_stride, int64_t ko_stride, const int64_t* pos,
+                  const double* turns, int rot, float amplitude, int adjacent, int32_t* err, hipStream_t st);
+// An 8-bit cache's page: geometry, alignment, whole tiles.
+int octet_check_page(int H, int d, const uint8_t* page, int64_t n_slots, int64_t slot_stride);
+// The block table that an 8-bit read goes by.
+int octet_check_table(int bs, int64_t n_slots, int num_reqs, int max_blocks, int max_seq);
+int octet_write_paged(int H, int d, const void* key, int k_dtype, int64_t k_row_stride, const void* val,
+                      int v_dtype, int64_t v_row_stride, const int64_t* slots, int num_tokens, uint8_t* page,
+                      int64_t n_slots, int64_t slot_stride, void* k_out, void* v_out, const int64_t* pos,
+                      const double* turns, int rot, float amplitude, int adjacent, const void* q, int q_dtype,
+                      int64_t q_stride, int HQ, void* qo, int64_t qo_stride, int32_t* err, hipStream_t st);
+int octet_read_paged(int H, int d, const uint8_t* page, int64_t n_slots, int64_t slot_stride, int bs,
+                     const int32_t* bt, int64_t bt_row_stride, int max_blocks, const int32_t* starts,
+                     const int32_t* first, int num_reqs, int max_seq, int num_rows, void* k_out,
+                     int64_t k_stride, void* v_out, int64_t v_stride, int out_dtype, int32_t* err,
+                     hipStream_t st);
+int64_t octet_decode_workspace_bytes(int H, int HQ, int d, int num_reqs, int max_q, int max_seq);
+int octet_decode_paged(int H, int HQ, int d, float scale, const void* q, int q_dtype, int64_t q_row_stride,
+                       int num_tokens, const uint8_t* page, int64_t n_slots, int64_t slot_stride, int bs,
+                       const int32_t* bt, int64_t bt_row_stride, int max_blocks, const int32_t* seq_lens,
+                       const int32_t* qsl, int num_reqs, int max_q, int max_seq, int window,
+                       const float* sinks, void* out, int out_dtype, int64_t out_row_stride, float* lse,
+                       void* ws, int64_t ws_bytes, int32_t* err, hipStream_t st);
 }  // namespace ttkv

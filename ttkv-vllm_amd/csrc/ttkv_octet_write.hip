@@ -1,0 +1,238 @@
+// Write of new keys and values into the 8-bit cache (format: ttkv_octet.h), the keys rotated on the way
+// where the call has positions, its queries with them; and the rotation by itself. gfx950 / CDNA4.
+//
+// A workgroup of 256 threads takes the keys and values of 1024 / d tokens of one head, 8 dims a thread:
+// a group of 32 dims is 4 neighbouring lanes. Tokens of one workgroup that follow each other in a tile
+// write whole 128-byte lines of its record.
+#include <math.h>
+
+#include "ttkv_host.h"
+#include "ttkv_octet.h"
+#include "ttkv_turn.h"
+
+namespace ttkv {
+
+struct OctWriteArgs {
+  const void* k;
+  const void* v;
+  int k_dtype, v_dtype;
+  int64_t k_row_stride, v_row_stride;
+  const int64_t* slots;
+  int num_tokens, H;
+  uint8_t* page;
+  int64_t n_slots, slot_stride;
+  uint16_t* k_out;
+  uint16_t* v_out;
+  int32_t* err;
+  int write_blocks;  // workgroups before those of the queries
+  TurnArgs turn;     // half == 0: keys come rotated
+};
+
+template <int D>
+__global__ __launch_bounds__(256) void octet_write_kernel(OctWriteArgs a) {
+  using F = Oct<D>;
+  constexpr int kTokens = 1024 / D, kLanes = D / 8;
+  __shared__ float2v cs[kTurnHalf];
+  __shared__ float xs[kTokens][D];
+  const int tid = threadIdx.x;
+  if ((int)blockIdx.x >= a.write_blocks) {
+    turn_token(a.turn, (int)blockIdx.x - a.write_blocks, tid, 256, cs);
+    return;
+  }
+  const int row = tid / kLanes, i = tid % kLanes, t = row % kTokens;  // dims 8 i .. 8 i + 7
+  const bool val = row >= kTokens;
+  const int h = (int)(blockIdx.x % (unsigned)a.H);
+  const int64_t tok0 = (int64_t)(blockIdx.x / (unsigned)a.H) * kTokens, tok = tok0 + t;
+  const bool on = tok < a.num_tokens;
+  const int64_t slot = on ? *gbl(a.slots + tok) : -1;  // negative: a padded token
+  if (slot >= a.n_slots && !val && i == 0) atomicOr(a.err, TTKV_ERR_BAD_SLOT);
+  const bool keep = slot >= 0 && slot < a.n_slots;
+  const void* src = val ? a.v : a.k;
+  const int dt = val ? a.v_dtype : a.k_dtype;
+  const int64_t stride = val ? a.v_row_stride : a.k_row_stride;
+  float x[8] = {};
+  if (keep) load_act_n<8>(src, dt, tok * stride + (int64_t)h * D + 8 * i, act_rows_aligned(src, dt, stride), x);
+  const int half = a.turn.half;
+  if (half) {
+    // every token's table in turn: half frequencies of kTokens tokens fit, kTokens * half <= 512
+    for (int n = 0; n < kTokens; ++n)
+      if (tok0 + n < a.num_tokens) {
+        const bool ok = turn_table(a.turn.pos, a.turn.turns, half, a.turn.amplitude, tok0 + n, tid, 256,
+                                   cs + n * half);
+        if (!ok && tid == 0 && h == 0) atomicOr(a.err, TTKV_ERR_BAD_POSITION);
+      }
+    if (!val)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) xs[t][8 * i + j] = x[j];
+    __syncthreads();
+    if (!val && keep) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const int e = 8 * i + j;
+        if (e < 2 * half) {
+          const int at = a.turn.adjacent ? e >> 1 : e < half ? e : e - half;
+          const bool first = a.turn.adjacent ? !(e & 1) : e < half;
+          const int mate = a.turn.adjacent ? e ^ 1 : first ? e + half : e - half;
+          const float2v w = cs[t * half + at];
+          x[j] = first ? x[j] * w[0] - xs[t][mate] * w[1] : x[j] * w[0] + xs[t][mate] * w[1];
+        } else if (cs[t * half][0] != cs[t * half][0]) {
+          x[j] = NAN;  // (a refused position)
+        }
+      }
+    }
+  }
+  if (!keep) return;
+  float odd = 0.f, top = 0.f;  // odd: NaN where a value is not finite
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    odd = fmaf(x[j], 0.f, odd);
+    x[j] = fminf(fmaxf(x[j], -kOctMax), kOctMax);
+    top = fmaxf(top, fabsf(x[j]));
+  }
+  for (int m = 1; m <= 2; m *= 2) {
+    odd += __shfl_xor(odd, m);
+    top = fmaxf(top, __shfl_xor(top, m));
+  }
+  const bool bad = odd != odd;
+  // 448 = 1.75 * 2^8: the exponent less 8, and one more where the mantissa is above 1.75
+  const uint32_t e = ((__builtin_bit_cast(uint32_t, top) + 0x1fffffu) >> 23) - 8;
+  const uint32_t byte = bad ? kOctNanByte : max((int)e, kOctMinByte);
+  const float by = oct_power(254 - byte);
+  uint32_t w[2];
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    int c = __builtin_amdgcn_cvt_pk_fp8_f32(x[4 * j] * by, x[4 * j + 1] * by, 0, false);
+    c = __builtin_amdgcn_cvt_pk_fp8_f32(x[4 * j + 2] * by, x[4 * j + 3] * by, c, true);
+    w[j] = bad ? kOctNanCode * 0x01010101u : (uint32_t)c;
+  }
+  uint16_t* outp = val ? a.v_out : a.k_out;
+  if (outp) {
+    const float p = oct_power(byte);
+    const bf16x2 o[4] = {oct_pair<false>(w[0], p), oct_pair<true>(w[0], p), oct_pair<false>(w[1], p),
+                         oct_pair<true>(w[1], p)};
+    *gblw((u32x4*)(outp + (tok * a.H + h) * D + 8 * i)) =
+        u32x4{__builtin_bit_cast(uint32_t, o[0]), __builtin_bit_cast(uint32_t, o[1]),
+              __builtin_bit_cast(uint32_t, o[2]), __builtin_bit_cast(uint32_t, o[3])};
+  }
+  uint8_t* rec = a.page + (slot >> 4) * (kOctTile * a.slot_stride) + (int64_t)h * F::kRecord;
+  const int u = (int)(slot & 15), g = i >> 2;
+  if (!val) {
+    *gblw((u32x2v*)(rec + F::key(u, 8 * i))) = u32x2v{w[0], w[1]};
+    if ((i & 3) == 0) *gblw(rec + F::key_power(u, g)) = (uint8_t)byte;
+  } else {
+    if constexpr (F::kDims >= 8) {
+      *gblw((u32x2v*)(rec + F::value(u, 8 * i))) = u32x2v{w[0], w[1]};
+    } else {
+      *gblw((uint32_t*)(rec + F::value(u, 8 * i))) = w[0];
+      *gblw((uint32_t*)(rec + F::value(u, 8 * i + 4))) = w[1];
+    }
+    if ((i & 3) == 0) *gblw(rec + F::value_power(u, g)) = (uint8_t)byte;
+  }
+}
+
+__global__ __launch_bounds__(256) void rotary_scaled_kernel(TurnArgs a) {
+  __shared__ float2v cs[kTurnHalf];
+  turn_token(a, blockIdx.x, threadIdx.x, 256, cs);
+}
+
+static bool act_dtype(int dt) {
+  return dt == TTKV_DTYPE_F32 || dt == TTKV_DTYPE_F16 || dt == TTKV_DTYPE_BF16;
+}
+
+// The rotation's own arguments; `limit`: dims of a row.
+static int turn_check(const int64_t* pos, const double* turns, int rot, int limit) {
+  if (rot <= 0 || rot % 2 || rot > limit)
+    return host_fail(TTKV_E_INVALID, "the rotary dims must be even and at most the head dim");
+  if (rot / 2 > kTurnHalf) return host_fail(TTKV_E_UNSUPPORTED, "more than 1024 rotary dims");
+  if (!pos || !turns) return host_fail(TTKV_E_INVALID, "null positions or turns");
+  if ((uintptr_t)turns % 8) return host_fail(TTKV_E_INVALID, "turns must be 8-byte aligned");
+  return TTKV_OK;
+}
+
+// A set's output may be its input, at its stride, or lie apart from it.
+static bool turn_clash(const void* x, int64_t xs, const void* y, int64_t ys, int64_t width, int64_t eb, int64_t n) {
+  return !(x == y && (xs == ys || n == 1)) && rows_meet(y, ys * eb, width, x, xs * eb, width, n);
+}
+
+int rotary_scaled(const void* q, const void* k, void* qo, void* ko, int dtype, int N, int HQ, int H, int d,
+                  int64_t q_stride, int64_t k_stride, int64_t qo_stride, int64_t ko_stride, const int64_t* pos,
+                  const double* turns, int rot, float amplitude, int adjacent, int32_t* err, hipStream_t st) {
+  if (!act_dtype(dtype)) return host_fail(TTKV_E_INVALID, "dtype must be fp32, fp16 or bf16");
+  if (N < 0 || HQ < 0 || H < 0 || d <= 0) return host_fail(TTKV_E_INVALID, "negative count");
+  if (N == 0 || HQ + H == 0) return TTKV_OK;
+  if (int rc = turn_check(pos, turns, rot, d)) return rc;
+  if ((HQ && (!q || !qo)) || (H && (!k || !ko)) || !err) return host_fail(TTKV_E_INVALID, "null pointer argument");
+  const int64_t eb = dtype == TTKV_DTYPE_F32 ? 4 : 2, qw = HQ ? (int64_t)HQ * d * eb : 0,
+                kw = H ? (int64_t)H * d * eb : 0;
+  if (turn_clash(q, q_stride, qo, qo_stride, qw, eb, N) || turn_clash(k, k_stride, ko, ko_stride, kw, eb, N))
+    return host_fail(TTKV_E_INVALID, "an output overlaps its input without being it");
+  if (rows_meet(qo, qo_stride * eb, qw, k, k_stride * eb, kw, N) ||
+      rows_meet(ko, ko_stride * eb, kw, q, q_stride * eb, qw, N) ||
+      rows_meet(qo, qo_stride * eb, qw, ko, ko_stride * eb, kw, N))
+    return host_fail(TTKV_E_INVALID, "one of query and key overlaps the other's output");
+  TurnArgs a{{q, k},  {qo, ko}, {HQ, H}, {q_stride, k_stride}, {qo_stride, ko_stride}, dtype, d,
+             rot / 2, adjacent, pos,     turns,                amplitude,              err};
+  hipLaunchKernelGGL(rotary_scaled_kernel, dim3(N), dim3(256), 0, st, a);
+  const hipError_t e = hipGetLastError();
+  if (e != hipSuccess)
+    return host_fail(TTKV_E_LAUNCH, std::string("scaled rotary launch: ") + hipGetErrorString(e));
+  return TTKV_OK;
+}
+
+int octet_check_page(int H, int d, const uint8_t* page, int64_t n_slots, int64_t slot_stride) {
+  if (d != 64 && d != 128 && d != 256) return host_fail(TTKV_E_UNSUPPORTED, "head dim must be 64, 128 or 256");
+  if (H <= 0) return host_fail(TTKV_E_INVALID, "H must be positive");
+  if (!page) return host_fail(TTKV_E_INVALID, "null page");
+  if (slot_stride < ((int64_t)33 * d * H + 15) / 16)
+    return host_fail(TTKV_E_INVALID, "slot stride is smaller than the slot (33 d H / 16 bytes)");
+  if ((uintptr_t)page % 16) return host_fail(TTKV_E_INVALID, "the page must be 16-byte aligned");
+  if (n_slots <= 0 || n_slots % kOctTile)
+    return host_fail(TTKV_E_INVALID, "the page must hold a positive multiple of 16 slots");
+  return TTKV_OK;
+}
+
+int octet_write_paged(int H, int d, const void* key, int k_dtype, int64_t k_row_stride, const void* val,
+                      int v_dtype, int64_t v_row_stride, const int64_t* slots, int num_tokens, uint8_t* page,
+                      int64_t n_slots, int64_t slot_stride, void* k_out, void* v_out, const int64_t* pos,
+                      const double* turns, int rot, float amplitude, int adjacent, const void* q, int q_dtype,
+                      int64_t q_stride, int HQ, void* qo, int64_t qo_stride, int32_t* err, hipStream_t st) {
+  if (int rc = octet_check_page(H, d, page, n_slots, slot_stride)) return rc;
+  if (!act_dtype(k_dtype) || !act_dtype(v_dtype))
+    return host_fail(TTKV_E_INVALID, "key / value dtype must be fp32, fp16 or bf16");
+  if (num_tokens < 0 || HQ < 0) return host_fail(TTKV_E_INVALID, "negative count");
+  if (rot < 0) return host_fail(TTKV_E_INVALID, "negative rotary dims");
+  if (HQ && !rot) return host_fail(TTKV_E_INVALID, "queries are taken to be rotated: they need rotary dims");
+  if (num_tokens == 0) return TTKV_OK;
+  if (!key || !val || !slots || !err) return host_fail(TTKV_E_INVALID, "null pointer argument");
+  if ((uintptr_t)k_out % 16 || (uintptr_t)v_out % 16)
+    return host_fail(TTKV_E_INVALID, "key_out / value_out must be 16-byte aligned");
+  if (rot)
+    if (int rc = turn_check(pos, turns, rot, d)) return rc;
+  if (HQ) {
+    if (!act_dtype(q_dtype)) return host_fail(TTKV_E_INVALID, "query dtype must be fp32, fp16 or bf16");
+    if (!q || !qo) return host_fail(TTKV_E_INVALID, "null pointer argument");
+    const int64_t eb = q_dtype == TTKV_DTYPE_F32 ? 4 : 2, qw = (int64_t)HQ * d * eb;
+    if (turn_clash(q, q_stride, qo, qo_stride, qw, eb, num_tokens))
+      return host_fail(TTKV_E_INVALID, "query_out overlaps the query without being it");
+    // (keys and values are read while queries are written)
+    const int64_t kb = k_dtype == TTKV_DTYPE_F32 ? 4 : 2, vb = v_dtype == TTKV_DTYPE_F32 ? 4 : 2;
+    if (rows_meet(qo, qo_stride * eb, qw, key, k_row_stride * kb, (int64_t)H * d * kb, num_tokens) ||
+        rows_meet(qo, qo_stride * eb, qw, val, v_row_stride * vb, (int64_t)H * d * vb, num_tokens))
+      return host_fail(TTKV_E_INVALID, "query_out overlaps the keys or values");
+  }
+  const int64_t tokens = 1024 / d, blocks = (num_tokens + tokens - 1) / tokens * H;
+  const int64_t grid = blocks + (HQ ? num_tokens : 0);
+  if (grid > 0x7fffffff) return host_fail(TTKV_E_INVALID, "too many tokens for one call");
+  OctWriteArgs a{key,  val,     k_dtype,     v_dtype,          k_row_stride,     v_row_stride, slots,      num_tokens, H,
+                 page, n_slots, slot_stride, (uint16_t*)k_out, (uint16_t*)v_out, err,          (int)blocks};
+  a.turn = TurnArgs{{q, nullptr},  {qo, nullptr}, {HQ, 0},     {q_stride, 0}, {qo_stride, 0}, q_dtype, d, rot / 2,
+                    adjacent != 0, pos,           turns,       amplitude,     err};
+  auto kernel = d == 64 ? octet_write_kernel<64> : d == 128 ? octet_write_kernel<128> : octet_write_kernel<256>;
+  hipLaunchKernelGGL(kernel, dim3((unsigned)grid), dim3(256), 0, st, a);
+  const hipError_t e = hipGetLastError();
+  if (e != hipSuccess)
+    return host_fail(TTKV_E_LAUNCH, std::string("octet write launch: ") + hipGetErrorString(e));
+  return TTKV_OK;
+}
+
+}  // namespace ttkv

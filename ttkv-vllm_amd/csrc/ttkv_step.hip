@@ -426,20 +426,6 @@ __global__ __launch_bounds__(256) void rotary_axes_kernel(RotArgs a) {
   }
 }
 
-// Whether rows of `a` and of `b` share bytes: n rows each, of wa and wb bytes at strides sa and sb. Rows
-// of unlike strides are only looked at where they begin.
-static bool rot_rows_meet(const void* a, int64_t sa, int64_t wa, const void* b, int64_t sb, int64_t wb,
-                          int64_t n) {
-  if (!wa || !wb || !a || !b) return false;
-  const int64_t off = (int64_t)((uintptr_t)b - (uintptr_t)a);
-  auto meet = [&](int64_t o) { return o < wa && -o < wb; };
-  if (n == 1 || sa != sb || sa <= 0) return meet(off);
-  const int64_t k0 = -off / sa;  // row i + k of b lies nearest to row i of a
-  for (int64_t k = k0 - 1; k <= k0 + 1; ++k)
-    if (k > -n && k < n && meet(off + k * sa)) return true;
-  return false;
-}
-
 int rotary_axes(const void* q, const void* k, void* qo, void* ko, int dtype, int N, int HQ, int H,
                 int d, int64_t q_stride, int64_t k_stride, int64_t qo_stride, int64_t ko_stride,
                 const int64_t* pos, int64_t pos_stride, int axes, const int32_t* sections,
@@ -468,11 +454,11 @@ int rotary_axes(const void* q, const void* k, void* qo, void* ko, int dtype, int
   // a row is written while others are still to be read: an output is its input as it stands, or apart
   const int64_t eb = dtype == TTKV_DTYPE_F32 ? 4 : 2, qw = (int64_t)HQ * d * eb, kw = (int64_t)H * d * eb;
   const int64_t qs = q_stride * eb, ks = k_stride * eb, qos = qo_stride * eb, kos = ko_stride * eb;
-  if ((!(qo == q && (qos == qs || N == 1)) && rot_rows_meet(qo, qos, qw, q, qs, qw, N)) ||
-      (!(ko == k && (kos == ks || N == 1)) && rot_rows_meet(ko, kos, kw, k, ks, kw, N)))
+  if ((!(qo == q && (qos == qs || N == 1)) && rows_meet(qo, qos, qw, q, qs, qw, N)) ||
+      (!(ko == k && (kos == ks || N == 1)) && rows_meet(ko, kos, kw, k, ks, kw, N)))
     return host_fail(TTKV_E_INVALID, "an output overlaps its input without being it");
-  if (rot_rows_meet(qo, qos, qw, k, ks, kw, N) || rot_rows_meet(ko, kos, kw, q, qs, qw, N) ||
-      rot_rows_meet(qo, qos, qw, ko, kos, kw, N))
+  if (rows_meet(qo, qos, qw, k, ks, kw, N) || rows_meet(ko, kos, kw, q, qs, qw, N) ||
+      rows_meet(qo, qos, qw, ko, kos, kw, N))
     return host_fail(TTKV_E_INVALID, "one of query and key overlaps the other's output");
   RotArgs a{q,        k,        qo,         ko,   dtype,      HQ,   H,           d, rot / 2, N,
             q_stride, k_stride, qo_stride, ko_stride, pos, pos_stride, axes, interleaved != 0};

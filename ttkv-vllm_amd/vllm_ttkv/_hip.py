@@ -220,6 +220,40 @@ def lib():
         P, I32, I64,                  # out, out_dtype, out_row_stride
         P, I64, P, P,                 # workspace, workspace_bytes, error_word, stream
     ]
+    L.ttkv_rotary_scaled.restype = ctypes.c_int
+    L.ttkv_rotary_scaled.argtypes = [
+        P, P, P, P, I32,              # query, key, query_out, key_out, dtype
+        I32, I32, I32, I32,           # num_tokens, num_heads, H, d
+        I64, I64, I64, I64,           # row strides: query, key, query_out, key_out
+        P, P, I32, F32, I32, P, P,    # positions, turns, rotary_dim, amplitude, adjacent, error_word, stream
+    ]
+    L.ttkv_octet_write_paged.restype = ctypes.c_int
+    L.ttkv_octet_write_paged.argtypes = [
+        I32, I32, P, I32, I64,        # H, d, key, k_dtype, k_row_stride
+        P, I32, I64, P, I32,          # value, v_dtype, v_row_stride, slot_mapping, num_tokens
+        P, I64, I64, P, P,            # page, n_slots, slot_stride, key_out, value_out
+        P, P, I32, F32, I32,          # positions, turns, rotary_dim, amplitude, adjacent
+        P, I32, I64, I32, P, I64,     # query, q_dtype, q_row_stride, num_heads, query_out, q_out_row_stride
+        P, P,                         # error_word, stream
+    ]
+    L.ttkv_octet_read_paged.restype = ctypes.c_int
+    L.ttkv_octet_read_paged.argtypes = [
+        I32, I32, P, I64, I64, I32,   # H, d, page, n_slots, slot_stride, block_size
+        P, I64, I32, P, P, I32, I32,  # block_table, stride, max_blocks, row_start_loc, first, num_reqs, max_seq_len
+        I32, P, I64, P, I64, I32,     # num_rows, key_out, stride, value_out, stride, out_dtype
+        P, P,                         # error_word, stream
+    ]
+    L.ttkv_octet_decode_workspace_bytes.restype = I64
+    L.ttkv_octet_decode_workspace_bytes.argtypes = [I32, I32, I32, I32, I32, I32]
+    L.ttkv_octet_decode_paged.restype = ctypes.c_int
+    L.ttkv_octet_decode_paged.argtypes = [
+        I32, I32, I32, F32, P, I32, I64, I32,  # H, num_heads, d, scale, query, q_dtype, q_row_stride, num_tokens
+        P, I64, I64, I32,             # page, n_slots, slot_stride, block_size
+        P, I64, I32, P, P, I32,       # block_table, stride, max_blocks, seq_lens, qsl, num_reqs
+        I32, I32, I32, P,             # max_q_len, max_seq_len, window, sinks
+        P, I32, I64, P,               # out, out_dtype, out_row_stride, lse
+        P, I64, P, P,                 # workspace, workspace_bytes, error_word, stream
+    ]
     for name in EXPORTS:
         getattr(L, name)  # every declared symbol must resolve
     _LIB = L
@@ -235,7 +269,9 @@ EXPORTS = ("ttkv_last_error", "ttkv_decoder_ranks", "ttkv_blob_bytes",
            "ttkv_container_v_out", "ttkv_step_plan", "ttkv_rotary_axes",
            "ttkv_nibble_write_paged", "ttkv_nibble_decode_workspace_bytes",
            "ttkv_nibble_decode_paged", "ttkv_nibble_decode_starts_paged",
-           "ttkv_nibble_prefill_workspace_bytes", "ttkv_nibble_prefill_paged")
+           "ttkv_nibble_prefill_workspace_bytes", "ttkv_nibble_prefill_paged",
+           "ttkv_rotary_scaled", "ttkv_octet_write_paged", "ttkv_octet_read_paged",
+           "ttkv_octet_decode_workspace_bytes", "ttkv_octet_decode_paged")
 
 
 def check(rc: int, what: str) -> None:

@@ -16,6 +16,8 @@ from . import _hip
 from .decoder_pool import DecoderPool, decoder_ranks
 from .layout import TTKLayout
 from .nibble import NibbleLayout
+from .octet import OctetLayout
+from .rope import Rotary
 
 
 def _need_device(*ts):
@@ -729,4 +731,221 @@ def nibble_prefill_paged(lay: NibbleLayout, query: torch.Tensor, page: torch.Ten
         _hip.ptr(req_index), B, int(max_q_len), int(max_seq_len), *out_args,
         workspace.data_ptr(), workspace.numel(), err.data_ptr(), _stream(index))
     _hip.check(rc, "ttkv_nibble_prefill_paged")
+    return out
+
+
+# ---------------------------------------------------------------- the 8-bit cache
+def _turns(rotary, d, device_index, positions, N):
+    """(positions, turns, rotary_dim, amplitude, adjacent) as the C entries take them."""
+    turns = rotary.turns
+    if turns.dtype != torch.float64 or turns.dim() != 1 or not turns.is_contiguous():
+        raise ValueError("rotary.turns must be a contiguous fp64 tensor, one per pair")
+    if turns.get_device() != device_index:
+        _need_device(turns)
+        raise ValueError(f"rotary.turns are on {turns.device}, the rows on device {device_index}")
+    rot = 2 * turns.numel()
+    if rot == 0 or rot > d:
+        raise ValueError(f"{turns.numel()} frequencies for heads of {d} dims")
+    if positions is None or positions.dtype != torch.int64 or positions.dim() != 1 \
+            or positions.numel() < N or not positions.is_contiguous():
+        raise ValueError(f"positions must be contiguous int64, one per token ({N})")
+    return positions.data_ptr(), turns.data_ptr(), rot, float(rotary.amplitude), \
+        int(bool(rotary.adjacent))
+
+
+def rotary_scaled(query: torch.Tensor, key: torch.Tensor | None, positions: torch.Tensor,
+                  rotary: Rotary, query_out: torch.Tensor | None = None,
+                  key_out: torch.Tensor | None = None, error_word: torch.Tensor | None = None):
+    """Rotate query [N, HQ, d] and key [N, H, d] by positions [N] int64, the angles formed from
+    `rotary`'s frequencies; returns (query_out, key_out), each of which may be its input. See
+    `ttkv_rotary_scaled` in include/ttkv_hip.h."""
+    index = _one_device(query, key, positions, query_out, key_out, error_word)
+    if query.dim() != 3:
+        raise ValueError(f"query must be [N, heads, d], got {tuple(query.shape)}")
+    N, HQ, d = query.shape
+    turned = _turns(rotary, d, index, positions, N)
+    if query.dtype not in _hip.DTYPE_CODE:
+        raise ValueError("query dtype must be fp32, fp16 or bf16")
+    query_out = torch.empty_like(query) if query_out is None else query_out
+    H = 0
+    if key is not None:
+        H = key.shape[1] if key.dim() == 3 else 0
+        key_out = torch.empty_like(key) if key_out is None else key_out
+    dtype = query.dtype
+    for t, heads, what in ((query, HQ, "query"), (query_out, HQ, "query_out"), (key, H, "key"),
+                           (key_out, H, "key_out")):
+        if t is None:
+            continue
+        _rows(t, heads, d, what)
+        if t.shape[0] != N or t.dtype != dtype:
+            raise ValueError(f"{what} must have the query's {N} tokens and dtype")
+    err = _error_word(error_word, query.device)
+    rc = _on_device(
+        index, _hip.lib().ttkv_rotary_scaled, query.data_ptr(), _hip.ptr(key),
+        query_out.data_ptr(), _hip.ptr(key_out), _hip.DTYPE_CODE[dtype], N, HQ, H, d,
+        query.stride(0), 0 if key is None else key.stride(0), query_out.stride(0),
+        0 if key is None else key_out.stride(0), *turned, err.data_ptr(), _stream(index))
+    _hip.check(rc, "ttkv_rotary_scaled")
+    return query_out, key_out
+
+
+def octet_write_paged(lay: OctetLayout, key: torch.Tensor, value: torch.Tensor,
+                      slot_mapping: torch.Tensor, page: torch.Tensor,
+                      rotary: Rotary | None = None, positions: torch.Tensor | None = None,
+                      query: torch.Tensor | None = None, query_out: torch.Tensor | None = None,
+                      key_out: torch.Tensor | None = None, value_out: torch.Tensor | None = None,
+                      error_word: torch.Tensor | None = None) -> torch.Tensor | None:
+    """Quantise key / value [N, H, d] into their slots of an 8-bit cache. With `rotary`, keys are
+    rotated by positions [>= N] int64 on the way, and query [N, HQ, d] into query_out (which may be
+    the query; allocated if absent); without, keys come rotated. Returns query_out.
+
+    page: the layer's cache, its last dim one slot (`lay.compressed_bytes_per_token()` bytes or
+    more); slot_mapping [>= N] int64, -1 for padded tokens; key_out / value_out (optional, bf16
+    [N, H, d], contiguous) receive what the slots then stand for. See `ttkv_octet_write_paged`."""
+    index = _one_device(key, value, slot_mapping, page, positions, query, query_out, key_out,
+                        value_out, error_word)
+    shape = key.shape
+    _rows(key, lay.H, lay.d, "key")
+    _rows(value, lay.H, lay.d, "value")
+    N = shape[0]
+    if value.shape[0] != N:
+        raise ValueError(f"{N} keys and {value.shape[0]} values")
+    k_code, v_code = _hip.DTYPE_CODE.get(key.dtype), _hip.DTYPE_CODE.get(value.dtype)
+    if k_code is None or v_code is None:
+        raise ValueError("key / value dtype must be fp32, fp16 or bf16")
+    for t, what in ((key_out, "key_out"), (value_out, "value_out")):
+        if t is not None and (t.shape != shape or t.dtype != torch.bfloat16
+                              or not t.is_contiguous()):
+            raise ValueError(f"{what} must be contiguous bf16 [{N}, {lay.H}, {lay.d}]")
+    if slot_mapping.dtype != torch.int64 or slot_mapping.numel() < N \
+            or not slot_mapping.is_contiguous():
+        raise ValueError("slot_mapping must be contiguous int64 with one id per token")
+    if not page.is_contiguous():
+        raise ValueError("the cache page must be contiguous")
+    turned, q_args = (0, 0, 0, 1.0, 0), (0, 0, 0, 0, 0, 0)
+    if rotary is not None:
+        turned = _turns(rotary, lay.d, index, positions, N)
+    elif query is not None:
+        raise ValueError("queries are taken to be rotated: they need `rotary`")
+    if query is not None:
+        HQ = query.shape[1] if query.dim() == 3 else 0
+        query_out = torch.empty_like(query) if query_out is None else query_out
+        q_code = _hip.DTYPE_CODE.get(query.dtype)
+        if q_code is None:
+            raise ValueError("query dtype must be fp32, fp16 or bf16")
+        for t, what in ((query, "query"), (query_out, "query_out")):
+            _rows(t, HQ, lay.d, what)
+            if t.shape[0] != N or t.dtype != query.dtype:
+                raise ValueError(f"{what} must have the {N} tokens and the query's dtype")
+        q_args = (query.data_ptr(), q_code, query.stride(0), HQ, query_out.data_ptr(),
+                  query_out.stride(0))
+    elif query_out is not None:
+        raise ValueError("query_out without a query")
+    err = _error_word(error_word, key.device)
+    rc = _on_device(
+        index, _hip.lib().ttkv_octet_write_paged, lay.H, lay.d, key.data_ptr(), k_code,
+        key.stride(0), value.data_ptr(), v_code, value.stride(0), slot_mapping.data_ptr(), N,
+        *_page_args(page, lay.compressed_bytes_per_token()), _hip.ptr(key_out),
+        _hip.ptr(value_out), *turned, *q_args, err.data_ptr(), _stream(index))
+    _hip.check(rc, "ttkv_octet_write_paged")
+    return query_out
+
+
+def octet_read_paged(lay: OctetLayout, page: torch.Tensor, block_size: int,
+                     block_table: torch.Tensor, row_start_loc: torch.Tensor, max_seq_len: int,
+                     first: torch.Tensor | None = None, num_rows: int | None = None,
+                     dtype: torch.dtype = torch.bfloat16, key_out: torch.Tensor | None = None,
+                     value_out: torch.Tensor | None = None,
+                     error_word: torch.Tensor | None = None):
+    """Stored keys and values of an 8-bit cache as rows: request r's tokens from first[r] (default 0)
+    go to rows row_start_loc[r] .. [r + 1] - 1 of key_out / value_out [rows, H, d] (allocated in
+    `dtype` with num_rows rows if absent). Returns (key_out, value_out). See
+    `ttkv_octet_read_paged` in include/ttkv_hip.h."""
+    index = _one_device(page, block_table, row_start_loc, first, key_out, value_out, error_word)
+    B = row_start_loc.numel() - 1
+    _i32(row_start_loc, "row_start_loc")
+    if B < 0:
+        raise ValueError("row_start_loc must have one entry more than there are requests")
+    if first is not None and _i32(first, "first").numel() < B:
+        raise ValueError(f"first must have an entry for each of {B} requests")
+    W, stride = _table(block_table, "[requests, max_blocks]")
+    if block_table.shape[0] < B:
+        raise ValueError(f"{B} requests need as many block table rows")
+    for t in (key_out, value_out):
+        if t is not None:
+            num_rows, dtype = t.shape[0], t.dtype
+    if num_rows is None:
+        raise ValueError("num_rows or an output must say how many rows there are")
+    key_out, value_out = (page.new_empty(num_rows, lay.H, lay.d, dtype=dtype) if t is None else t
+                          for t in (key_out, value_out))
+    code = _hip.DTYPE_CODE.get(dtype)
+    if code is None:
+        raise ValueError("key_out / value_out dtype must be fp32, fp16 or bf16")
+    for t, what in ((key_out, "key_out"), (value_out, "value_out")):
+        _rows(t, lay.H, lay.d, what)
+        if t.shape[0] != num_rows or t.dtype != dtype:
+            raise ValueError("key_out and value_out must have the same rows and dtype")
+    if not page.is_contiguous():
+        raise ValueError("the cache page must be contiguous")
+    err = _error_word(error_word, page.device)
+    rc = _on_device(
+        index, _hip.lib().ttkv_octet_read_paged, lay.H, lay.d,
+        *_page_args(page, lay.compressed_bytes_per_token()), int(block_size),
+        block_table.data_ptr(), stride, W, row_start_loc.data_ptr(), _hip.ptr(first), B,
+        int(max_seq_len), num_rows, key_out.data_ptr(), key_out.stride(0), value_out.data_ptr(),
+        value_out.stride(0), code, err.data_ptr(), _stream(index))
+    _hip.check(rc, "ttkv_octet_read_paged")
+    return key_out, value_out
+
+
+def octet_decode_workspace(lay: OctetLayout, num_heads: int, num_reqs: int, max_q_len: int,
+                           max_seq_len: int, device) -> torch.Tensor:
+    """A workspace for `octet_decode_paged` over batches of up to this shape (see
+    `nibble_decode_workspace`; one buffer may serve the reads of both caches, in stream order)."""
+    n = _hip.lib().ttkv_octet_decode_workspace_bytes(lay.H, num_heads, lay.d, num_reqs, max_q_len,
+                                                     max_seq_len)
+    if n < 0:
+        raise ValueError("invalid head count or batch for the decode workspace")
+    return _nibble_workspace(int(n), device)
+
+
+def octet_decode_paged(lay: OctetLayout, query: torch.Tensor, page: torch.Tensor, block_size: int,
+                       block_table: torch.Tensor, seq_lens: torch.Tensor,
+                       query_start_loc: torch.Tensor, max_q_len: int, max_seq_len: int,
+                       scale: float, window: int = 0, sinks: torch.Tensor | None = None,
+                       out: torch.Tensor | None = None, lse: torch.Tensor | None = None,
+                       workspace: torch.Tensor | None = None,
+                       error_word: torch.Tensor | None = None) -> torch.Tensor:
+    """Attention of each request's new tokens (rows query_start_loc[r] .. [r + 1] of query
+    [N, HQ, d], rotated; at most max_q_len <= 16) over its seq_lens[r] stored tokens of an 8-bit
+    cache, their own included. window: the last keys a query sees, itself among them (0: all);
+    sinks [HQ] fp32: one more logit per head; lse [N, HQ] fp32 (optional) receives the logarithm of
+    the softmax's sum. See `ttkv_octet_decode_paged` in include/ttkv_hip.h. Returns `out`
+    [N, HQ, d] with the requests' rows written."""
+    index = _one_device(query, page, block_table, seq_lens, query_start_loc, sinks, out, lse,
+                        workspace, error_word)
+    out, q_args, bt_args, out_args = _nibble_read(lay, query, page, block_table, seq_lens,
+                                                  query_start_loc, out)
+    N, HQ = query.shape[:2]
+    B = seq_lens.numel()
+    if block_table.shape[0] < B or query_start_loc.numel() < B + 1:
+        raise ValueError(f"{B} sequence lengths need as many block table rows and one more "
+                         f"query start")
+    if sinks is not None and (sinks.dtype != torch.float32 or sinks.shape != (HQ,)
+                              or not sinks.is_contiguous()):
+        raise ValueError(f"sinks must be contiguous fp32 [{HQ}]")
+    if lse is not None and (lse.dtype != torch.float32 or lse.shape != (N, HQ)
+                            or not lse.is_contiguous()):
+        raise ValueError(f"lse must be contiguous fp32 [{N}, {HQ}]")
+    if N == 0:                                  # every request waits
+        return out
+    if workspace is None:
+        workspace = octet_decode_workspace(lay, HQ, B, max_q_len, max_seq_len, query.device)
+    err = _error_word(error_word, query.device)
+    rc = _on_device(
+        index, _hip.lib().ttkv_octet_decode_paged, lay.H, HQ, lay.d, float(scale), *q_args[:3], N,
+        *q_args[3:], int(block_size), *bt_args, seq_lens.data_ptr(), query_start_loc.data_ptr(), B,
+        int(max_q_len), int(max_seq_len), min(int(window), 2 ** 31 - 1), _hip.ptr(sinks), *out_args, _hip.ptr(lse),
+        workspace.data_ptr(), workspace.numel(), err.data_ptr(), _stream(index))
+    _hip.check(rc, "ttkv_octet_decode_paged")
     return out
