@@ -1,101 +1,584 @@
 // Attention of new tokens over the 8-bit cache (format: ttkv_octet.h): one query per request, or a few
 // drafts. gfx950 / CDNA4.
+//
+// The rows of a (request, KV head) are its (query, query head) pairs, row = j G + p. Work item = (request,
+// block of 16 rows, chunk of the request's 32-token steps, KV head), one workgroup of 4 waves that take the
+// chunk's steps in turn. The chunk length comes from a plan that every workgroup computes alike from the
+// batch's lengths: the shortest that spreads the batch's steps over the resident workgroups, so a ragged
+// batch fills the chip by its total work. Items of a (block, head) leave unnormalised partials in the
+// workspace; the last to arrive joins them.
+//
+// One step of a wave, two tiles of 16 tokens:
+//   S^T [token, row] = K Q^T on v_mfma_f32_16x16x32_bf16: a lane's d / 4 key code bytes of a tile are its A
+//     operand of the d / 32 products (token lane % 16), made bf16 at their power of two by one instruction
+//     per pair, exactly; the queries are the B operand, held in registers (fp16 ones as two bf16 parts,
+//     exactly). Columns without a row are zero.
+//   softmax in the result's own registers: lane column = row, 8 tokens of it. Weights are taken against
+//     the maximum as it stands, which moves only when their sum is large, so most steps need no maximum
+//     and no exchange between lanes; the sum stays per lane until the end. bf16 has fp32's range, so no
+//     weight leaves it; two parts of a weight keep 16 bits of it.
+//   O^T [dim, row] += V^T P^T, a product per dim of a lane's d / 16 and weight part: the scores' layout is
+//     the B operand's as it stands. A lane holds dims of four tokens per tile; their bf16 pairs of two dims
+//     become pairs of two tokens by one byte permutation each. The result's column is the row again, so
+//     the rescale is a lane's factor.
 #include <math.h>
 
 #include "ttkv_host.h"
+#include "ttkv_nibble.h"
 #include "ttkv_octet.h"
 
 namespace ttkv {
 
 constexpr int kODMaxQ = 16;  // queries per request
+constexpr int kODThreads = 256;
+constexpr int kODWaves = 4;
+constexpr int kODStep = 2 * kOctTile;  // tokens per wave step
+constexpr int kODPlanLanes = 4;        // requests per lane in the plan: 256 per launch
+constexpr int kODRows = 16;            // rows of a block: a matrix product's columns
+constexpr float kODNone = -3.402823466e38f;  // the maximum before the first visible key
+constexpr float kODMost = 0x1p10f;     // a lane's sum of eight weights before the maximum moves
+constexpr float kLog2e = 1.4426950408889634f;
 
 struct OctDecodeArgs {
   int H, G;
-  float scale;
-  const void* q;
-  int q_dtype;
+  float scale_log2;
+  const uint16_t* q;
   int64_t q_row_stride;
   int num_tokens;
   const uint8_t* page;
   int64_t tile_stride;
-  int num_blocks, tpb;
+  int num_blocks;
+  int tpb;  // tiles per block
   const int32_t* bt;
   int64_t bt_row_stride;
   const int32_t* seq_lens;
   const int32_t* qsl;
-  int max_q, max_seq, window;
+  int num_reqs, max_q, max_seq;
+  int window;  // 0: none
   const float* sinks;
   void* out;
   int out_dtype;
   int64_t out_row_stride;
   float* lse;
+  int* ws_cnt;
+  float* ws_o;       // [split items][part_rows][D]
+  float* ws_ml;      // [split items][part_rows][2]
+  uint32_t o_bytes;  // size of ws_o
+  int part_rows;     // rows of an item's partials
+  int target;
   int32_t* err;
 };
 
-// One workgroup per (request, query, query head); a wave per key in turn, joined in LDS.
-template <int D>
-__global__ __launch_bounds__(256) void octet_decode_kernel(OctDecodeArgs a) {
-  using F = Oct<D>;
-  constexpr int N = D / 64;
-  __shared__ float sh[4][D + 2];
-  const int lane = threadIdx.x & 63, wv = threadIdx.x >> 6, HQ = a.H * a.G;
-  const int hq = (int)(blockIdx.x % (unsigned)HQ), h = hq / a.G;
-  const int j = (int)(blockIdx.x / (unsigned)HQ % (unsigned)a.max_q), r = (int)(blockIdx.x / (unsigned)HQ / (unsigned)a.max_q);
-  const int n = min(max(a.seq_lens[r], 0), a.max_seq), row0 = a.qsl[r], Q = a.qsl[r + 1] - row0;
-  const bool first = threadIdx.x == 0 && hq == 0 && j == 0;
-  if (first && (a.seq_lens[r] > a.max_seq || Q > a.max_q || (n > 0 && n < Q))) atomicOr(a.err, TTKV_ERR_SEQ_LEN);
-  if (j >= Q) return;
-  const int64_t row = (int64_t)row0 + j;
-  if (row < 0 || row >= a.num_tokens) {
-    if (threadIdx.x == 0 && hq == 0) atomicOr(a.err, TTKV_ERR_SEQ_LEN);
-    return;
+struct OctPlan {
+  int r, rb, c, h;   // batch row, row block, chunk, KV head
+  int n, Q, q0;      // keys, queries and the first one's row
+  int s0, steps;     // the request's steps: the first and how many
+  int nch;           // the block's chunks
+  int part, block;   // the block's first split item and its number, both before the head
+  bool none;
+};
+
+__device__ __forceinline__ OctPlan od_plan(const OctDecodeArgs& a, int item) {
+  const int lane = threadIdx.x & 63;
+  int n[kODPlanLanes], q0[kODPlanLanes], Q[kODPlanLanes], s0[kODPlanLanes], st[kODPlanLanes], rb[kODPlanLanes];
+  int total = 0;
+#pragma unroll
+  for (int i = 0; i < kODPlanLanes; ++i) {
+    n[i] = q0[i] = Q[i] = 0;
+    const int r = lane + 64 * i;
+    if (64 * i >= a.num_reqs || r >= a.num_reqs) continue;
+    n[i] = a.seq_lens[r];
+    q0[i] = a.qsl[r];
+    Q[i] = a.qsl[r + 1] - q0[i];
   }
-  const int at = n - Q + j, lo = a.window > 0 ? max(0, at - a.window + 1) : 0;
-  float q[N], o[N] = {}, m = -INFINITY, l = 0.f;
-  for (int k = 0; k < N; ++k) q[k] = load_act(a.q, a.q_dtype, row * a.q_row_stride + (int64_t)hq * D + lane * N + k);
-  bool bad = n > 0 && n < Q;
-  for (int t = lo + wv; t <= at; t += 4) {
-    const int tile = t / kOctTile, b = tile / a.tpb, u = t % kOctTile, id = a.bt[r * a.bt_row_stride + b];
-    if ((uint32_t)id >= (uint32_t)a.num_blocks) {
-      if (lane == 0) atomicOr(a.err, TTKV_ERR_BAD_BLOCK);
-      bad = true;
-      break;
+#pragma unroll
+  for (int i = 0; i < kODPlanLanes; ++i) {
+    const int nn = min(max(n[i], 0), a.max_seq), qq = min(max(Q[i], 0), a.max_q), p0 = nn - Q[i];
+    s0[i] = a.window && p0 >= a.window ? (p0 - a.window + 1) / kODStep : 0;
+    st[i] = p0 >= 0 && qq > 0 ? (p0 + qq - 1) / kODStep + 1 - s0[i] : 0;
+    rb[i] = (qq * a.G + kODRows - 1) / kODRows;
+    total += st[i] * rb[i];
+  }
+  // (a lane has less than 2^28 of them)
+  const int64_t all = ((int64_t)wave_sum_i(total >> 12) * 4096 + wave_sum_i(total & 4095)) * a.H;
+  // whole rounds of the four waves
+  const int per = all < 0x40000000 ? (int)(((uint32_t)all + a.target - 1) / a.target)
+                                   : (int)fminf((float)all / (float)a.target * 1.00001f, 1e8f) + 1;
+  const int C = max(1, (per + kODWaves - 1) / kODWaves) * kODWaves;
+  OctPlan P{};
+  P.h = item % a.H;
+  P.none = true;
+  const int it = item / a.H;
+  int carry = 0, blocks = 0, parts = 0;
+#pragma unroll
+  for (int i = 0; i < kODPlanLanes; ++i) {
+    if (64 * i >= a.num_reqs || !P.none) break;
+    const int nch = max(1, (st[i] + C - 1) / C), items = rb[i] * nch, split = nch > 1 ? items : 0;
+    const int incl = nib_scan(items), bincl = nib_scan(rb[i]), pincl = nib_scan(split);
+    const int ex = carry + incl - items;
+    const uint64_t hit = __builtin_amdgcn_ballot_w64(ex <= it && it < ex + items);
+    if (hit) {
+      const int ln = __builtin_ctzll(hit);
+      P.none = false;
+      P.r = 64 * i + ln;
+      P.n = __builtin_amdgcn_readlane(n[i], ln);
+      P.Q = __builtin_amdgcn_readlane(Q[i], ln);
+      P.q0 = __builtin_amdgcn_readlane(q0[i], ln);
+      P.s0 = __builtin_amdgcn_readlane(s0[i], ln);
+      P.steps = __builtin_amdgcn_readlane(st[i], ln);
+      P.nch = __builtin_amdgcn_readlane(nch, ln);
+      const int local = it - __builtin_amdgcn_readlane(ex, ln);
+      P.rb = local / P.nch;
+      P.c = local - P.rb * P.nch;
+      P.part = __builtin_amdgcn_readlane(parts + pincl - split, ln) + P.rb * P.nch;
+      P.block = __builtin_amdgcn_readlane(blocks + bincl - rb[i], ln) + P.rb;
     }
-    const uint8_t* rec = a.page + ((int64_t)id * a.tpb + tile - b * a.tpb) * a.tile_stride + (int64_t)h * F::kRecord;
-    float s = 0.f, v[N];
-    for (int k = 0; k < N; ++k) {
-      const int x = lane * N + k;
-      s = fmaf(q[k], (float)oct_pair<false>(rec[F::key(u, x)], oct_power(rec[F::key_power(u, x / 32)]))[0], s);
-      v[k] = (float)oct_pair<false>(rec[F::value(u, x)], oct_power(rec[F::value_power(u, x / 32)]))[0];
-    }
-    s = wave_sum(s) * a.scale;
-    const float mn = fmaxf(m, s), f = m == mn ? 1.f : expf(m - mn), p = expf(s - mn);
-    l = l * f + p;
-    for (int k = 0; k < N; ++k) o[k] = o[k] * f + p * v[k];
-    m = mn;
+    carry += __builtin_amdgcn_readlane(incl, 63);
+    blocks += __builtin_amdgcn_readlane(bincl, 63);
+    parts += __builtin_amdgcn_readlane(pincl, 63);
   }
-  if (bad) l = NAN;
-  for (int k = 0; k < N; ++k) sh[wv][lane * N + k] = o[k];
-  if (lane == 0) {
-    sh[wv][D] = m;
-    sh[wv][D + 1] = l;
-  }
-  __syncthreads();
-  float M = a.sinks ? a.sinks[hq] : -INFINITY;
-  for (int w = 0; w < 4; ++w) M = fmaxf(M, sh[w][D]);
-  float total = a.sinks && M > -INFINITY ? expf(a.sinks[hq] - M) : 0.f;
-  float x = 0.f;
-  for (int w = 0; w < 4; ++w) {
-    const float f = sh[w][D] == -INFINITY ? 0.f : expf(sh[w][D] - M);
-    total += sh[w][D + 1] != sh[w][D + 1] ? NAN : sh[w][D + 1] * f;
-    if (threadIdx.x < D) x += f == 0.f ? 0.f : sh[w][threadIdx.x] * f;
-  }
-  if (threadIdx.x < D)
-    store_act(a.out, a.out_dtype, row * a.out_row_stride + (int64_t)hq * D + threadIdx.x, total == 0.f ? 0.f : x / total);
-  if (a.lse && threadIdx.x == 0) a.lse[row * HQ + hq] = total == 0.f ? -INFINITY : M + logf(total);
+  return P;
 }
 
-int64_t octet_decode_workspace_bytes(int H, int HQ, int d, int num_reqs, int max_q, int max_seq) { return 256; }
+// One step's bytes of a lane: per tile its token's key codes and exponents, and its dims' value codes and
+// exponents of four tokens.
+template <int D>
+struct OctStep {
+  u32x4 k[2][D / 64], v[2][D / 64];
+  uint32_t kp[2], vp[2];
+};
+
+// Four tokens' values of one dim, and of the next, from the tokens' pairs of those dims.
+__device__ __forceinline__ uint32_t od_low(bf16x2 a, bf16x2 b) {
+  return __builtin_amdgcn_perm(__builtin_bit_cast(uint32_t, b), __builtin_bit_cast(uint32_t, a), 0x05040100u);
+}
+__device__ __forceinline__ uint32_t od_high(bf16x2 a, bf16x2 b) {
+  return __builtin_amdgcn_perm(__builtin_bit_cast(uint32_t, b), __builtin_bit_cast(uint32_t, a), 0x07060302u);
+}
+
+template <int D, int QDT, bool CHUNK>
+__global__ __launch_bounds__(kODThreads, D == 256 ? 1 : 2) void octet_decode_kernel(OctDecodeArgs a) {
+  using F = Oct<D>;
+  constexpr int N = F::kDims, KS = D / 32, PIECES = D / 64, PARTS = QDT == TTKV_DTYPE_F16 ? 2 : 1;
+  constexpr int RS = D + 4;  // floats of a row in LDS: the rows' columns start in different banks
+  extern __shared__ __align__(16) float red_all[];  // [waves][rows][RS]: the waves' results, then the join's
+  float(*red_o)[kODRows][RS] = (float(*)[kODRows][RS])red_all;
+  __shared__ float red_m[kODWaves][kODRows], red_l[kODWaves][kODRows];
+  __shared__ int last_sh;
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wv = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const OctPlan P = od_plan(a, blockIdx.x);
+  if (P.none) return;
+  const int h = P.h, G = a.G, HQ = a.H * a.G;
+  const int n = min(max(P.n, 0), a.max_seq), Q = min(P.Q, a.max_q);
+  const int p0 = n - P.Q;  // position of query 0
+  const int row0 = P.rb * kODRows, nrow = min(kODRows, Q * G - row0);  // the block's rows
+  const bool outside = P.q0 < 0 || (int64_t)P.q0 + Q > a.num_tokens;
+  if (tid == 0 && h == 0 && P.c == 0 && P.rb == 0 &&
+      (P.n > a.max_seq || P.Q > a.max_q || (n > 0 && p0 < 0) || outside))
+    atomicOr(a.err, TTKV_ERR_SEQ_LEN);
+  // row `r` of the block in the query and the output, and whether it has a place there
+  auto row_at = [&](int r, int64_t stride) -> int64_t {
+    const int row = row0 + r, j = CHUNK ? row / G : 0;
+    return ((int64_t)P.q0 + j) * stride + (int64_t)(h * G + row - j * G) * D;
+  };
+  auto has = [&](int r) {
+    const int64_t t = (int64_t)P.q0 + (CHUNK ? (row0 + r) / G : 0);
+    return !outside || (t >= 0 && t < a.num_tokens);
+  };
+  // The end of a row: the sink joins its sum. `o` of dims d .. d + 3, not yet divided by l.
+  auto finish = [&](int r, int d, float4v o, float m, float l) {
+    if (!has(r)) return;
+    const int row = row0 + r, j = CHUNK ? row / G : 0, hq = h * G + row - j * G;
+    if (a.sinks) {
+      const float s = a.sinks[hq] * kLog2e, mn = fmaxf(m, s), f = exp2f(m - mn);
+      l = l * f + exp2f(s - mn);
+      o *= f;
+      m = mn;
+    }
+    const float by = l == 0.f ? 0.f : 1.f / l;
+    store_act4(a.out, a.out_dtype, row_at(r, a.out_row_stride) + d, o * by, true);
+    if (a.lse && d == 0)
+      a.lse[((int64_t)P.q0 + j) * HQ + hq] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
+  };
+  if (p0 < 0) {  // an empty request's rows are 0; fewer keys than queries are refused
+    for (int i = tid; i < nrow * (D / 4); i += kODThreads)
+      finish(i / (D / 4), i % (D / 4) * 4, float4v{}, kODNone, n > 0 ? NAN : 0.f);
+    return;
+  }
+  const int col = lane & 15, q4 = lane >> 4;
+
+  // The queries, row `col`, as the B operand of the score products: dims q4 D / 4 + 8 s + (0..7)
+  bf16x8 qf[PARTS][KS];
+  const int my = min(col, nrow - 1);
+  {
+    const bool on = col < nrow && has(my);
+    const uint16_t* src = a.q + row_at(my, a.q_row_stride) + q4 * (D / 4);
+#pragma unroll
+    for (int s = 0; s < KS; ++s) {
+      u32x4 raw = {};
+      if (on) raw = *gbl((const u32x4*)(src + 8 * s));
+      if constexpr (QDT == TTKV_DTYPE_BF16) {
+        qf[0][s] = __builtin_bit_cast(bf16x8, raw);
+      } else {
+        const half8 x = __builtin_bit_cast(half8, raw);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {  // 11 bits are 8 and the 3 that they leave
+          const __bf16 hi = (__bf16)(float)x[j];
+          qf[0][s][j] = hi;
+          qf[PARTS - 1][s][j] = (__bf16)((float)x[j] - (float)hi);
+        }
+      }
+    }
+  }
+  const int lim = p0 + (CHUNK ? (row0 + my) / G : 0);  // last key the lane's row sees
+  const int low = a.window ? lim - a.window : -1;      // and the one before its first
+  const int see_all = p0 + (CHUNK ? row0 / G : 0);     // no row of the block sees less than to here
+  const int low_all = a.window ? p0 + (CHUNK ? (row0 + nrow - 1) / G : 0) - a.window : -1;  // and from behind here
+  float m = kODNone, l = 0.f;
+  float4v acc[N];  // [e][i]: dim (4 q4 + i) N + e of the lane's row
+#pragma unroll
+  for (int e = 0; e < N; ++e) acc[e] = float4v{};
+
+  // the block's steps in equal parts
+  const int s0 = P.s0 + (int)((int64_t)P.steps * P.c / P.nch);
+  const int s1 = P.s0 + (int)((int64_t)P.steps * (P.c + 1) / P.nch);
+  const int first_tile = a.window ? max(p0 - a.window + 1, 0) / kOctTile : 0;
+  bool bad = false;
+
+  const uint8_t* base = a.page + (int64_t)h * F::kRecord;
+  const int32_t* bt = a.bt + (int64_t)P.r * a.bt_row_stride;
+  // tile ids of this wave's next 64 steps, one step per lane (-1: a block outside the cache)
+  int tid0 = 0, tid1 = 0;
+  auto fetch_ids = [&](int s) {
+    const int mine = min(s + kODWaves * lane, s1 - 1);  // (past the chunk: its last step's again)
+    // (no tile outside the keys that some row sees: a window's past blocks may be gone)
+    const int t0 = max(2 * mine, first_tile), t1 = min(max(2 * mine + 1, first_tile), (n - 1) / kOctTile);
+    const int b0 = t0 / a.tpb, b1 = t1 / a.tpb;
+    const int i0 = bt[b0], i1 = bt[b1];
+    tid0 = (uint32_t)i0 < (uint32_t)a.num_blocks ? i0 * a.tpb + t0 - b0 * a.tpb : -1;
+    tid1 = (uint32_t)i1 < (uint32_t)a.num_blocks ? i1 * a.tpb + t1 - b1 * a.tpb : -1;
+  };
+  auto load = [&](int k, OctStep<D>& x) {  // the wave's k-th step since fetch_ids
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      const int id = __builtin_amdgcn_readlane(t ? tid1 : tid0, k);
+      const uint8_t* rec = base + (int64_t)max(id, 0) * a.tile_stride;
+#pragma unroll
+      for (int p = 0; p < PIECES; ++p)
+        x.k[t][p] = __builtin_nontemporal_load(gbl((const u32x4*)(rec + 1024 * p + 16 * lane)));
+      if constexpr (D == 256)
+        x.kp[t] = __builtin_nontemporal_load(gbl((const uint16_t*)(rec + F::kKp) + lane));
+      else
+        x.kp[t] = __builtin_nontemporal_load(gbl(rec + F::kKp + (D == 64 ? (lane >> 5) * 16 + col : lane)));
+#pragma unroll
+      for (int p = 0; p < PIECES; ++p)
+        x.v[t][p] = __builtin_nontemporal_load(gbl((const u32x4*)(rec + F::kV + 1024 * p + 16 * lane)));
+      x.vp[t] = __builtin_nontemporal_load(gbl((const uint32_t*)(rec + F::kVp + col * N / 32 * 16) + q4));
+      bad |= id < 0;
+    }
+  };
+  auto step = [&](int s, OctStep<D>& x) {
+    float4v sc[2];
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      sc[t] = float4v{};
+      const float pw[2] = {oct_power(x.kp[t] & 0xffu), oct_power(x.kp[t] >> 8)};
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) {
+        const float p = pw[D == 256 ? ks / 4 : 0];
+        bf16x8 kf;
+#pragma unroll
+        for (int w = 0; w < 2; ++w) {
+          const uint32_t c = x.k[t][ks / 2][ks % 2 * 2 + w];
+          const bf16x2 lo = oct_pair<false>(c, p), hi = oct_pair<true>(c, p);
+          kf[4 * w] = lo[0];
+          kf[4 * w + 1] = lo[1];
+          kf[4 * w + 2] = hi[0];
+          kf[4 * w + 3] = hi[1];
+        }
+#pragma unroll
+        for (int part = 0; part < PARTS; ++part)
+          sc[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, qf[part][ks], sc[t], 0, 0, 0);
+      }
+      sc[t] *= a.scale_log2;
+    }
+    const int tok = s * kODStep + 4 * q4;
+    uint32_t note = 0;  // bit 4 t + i: the lane's dims of that token are NaN
+    if ((s + 1) * kODStep - 1 > see_all || s * kODStep <= low_all) {
+      // Some row does not see all of this step: no score outside its keys. A weight of 0 must not meet a
+      // NaN: values that no row sees become 0, and with several queries a group that is NaN becomes 0
+      // too and is noted for the rows that see it.
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int tk = tok + 16 * t + i;
+          if (tk > lim || tk <= low) sc[t][i] = -INFINITY;
+          bool drop = CHUNK ? tk >= n || tk <= p0 - a.window : tk > lim || tk <= low;
+          if (CHUNK && !a.window) drop = tk >= n;
+          if constexpr (CHUNK) {
+            const uint32_t c = x.v[t][i * N / 16][i * N % 16 / 4] & 0x7fu;  // (a group is NaN as a whole)
+            if (!drop && c == kOctNanCode) {
+              note |= 1u << (4 * t + i);
+              drop = true;
+            }
+          }
+          if (drop) {
+#pragma unroll
+            for (int w = 0; w < N / 4; ++w) x.v[t][(i * N / 4 + w) / 4][(i * N / 4 + w) % 4] = 0;
+            x.vp[t] = (x.vp[t] & ~(0xffu << (8 * i))) | (127u << (8 * i));
+          }
+        }
+    }
+    // Weights against the maximum as it stands; it moves where a lane's sum of eight is large (or NaN). A
+    // score's product with the scale is rounded by itself, so that equal scores weigh the same.
+    float p[8], sum;
+    auto weights = [&]() {
+#pragma clang fp contract(off)
+      sum = 0.f;
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          p[4 * t + i] = fast_exp2(sc[t][i] - m);
+          sum += p[4 * t + i];
+        }
+    };
+    weights();
+    if (__builtin_amdgcn_ballot_w64(!(sum <= kODMost))) {
+      float mt = kODNone;
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) mt = fmaxf(mt, sc[t][i]);
+      const float mn = fmaxf(m, cross_row_max(mt)), f = exp2f(m - mn);
+      m = mn;
+      l *= f;
+#pragma unroll
+      for (int e = 0; e < N; ++e) acc[e] *= f;
+      weights();
+    }
+    l += sum;
+    bf16x8 ph, pl;  // 16 bits of each weight, in two parts
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      ph[i] = (__bf16)p[i];
+      pl[i] = (__bf16)(p[i] - (float)ph[i]);
+    }
+    float vp[2][4];
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) vp[t][i] = oct_power((x.vp[t] >> (8 * i)) & 0xffu);
+#pragma unroll
+    for (int e = 0; e < N; e += 2) {
+      u32x4 lo, hi;
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        bf16x2 pr[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int b = i * N + e;
+          const uint32_t c = x.v[t][b / 16][b % 16 / 4];
+          pr[i] = b & 2 ? oct_pair<true>(c, vp[t][i]) : oct_pair<false>(c, vp[t][i]);
+        }
+        lo[2 * t] = od_low(pr[0], pr[1]);
+        lo[2 * t + 1] = od_low(pr[2], pr[3]);
+        hi[2 * t] = od_high(pr[0], pr[1]);
+        hi[2 * t + 1] = od_high(pr[2], pr[3]);
+      }
+      const bf16x8 v0 = __builtin_bit_cast(bf16x8, lo), v1 = __builtin_bit_cast(bf16x8, hi);
+      acc[e] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v0, ph, acc[e], 0, 0, 0);
+      acc[e + 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v1, ph, acc[e + 1], 0, 0, 0);
+      acc[e] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v0, pl, acc[e], 0, 0, 0);
+      acc[e + 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v1, pl, acc[e + 1], 0, 0, 0);
+    }
+    if (CHUNK && __builtin_amdgcn_ballot_w64(note != 0)) {
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {  // tokens 16 (k / 4) + 4 (0..3) + k % 4, lanes' dims N lane % 16
+        const uint64_t of = __builtin_amdgcn_ballot_w64((note >> k) & 1);
+        if (!of) continue;
+        for (int b = 0; b < 4; ++b) {
+          const uint32_t lanes = (uint32_t)(of >> (16 * b)) & 0xffffu;
+          const int tk = s * kODStep + 16 * (k / 4) + 4 * b + k % 4;
+          if (tk > lim || tk <= low) continue;
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if ((lanes >> (4 * q4 + i)) & 1)
+#pragma unroll
+              for (int e = 0; e < N; ++e) acc[e][i] = NAN;
+        }
+      }
+    }
+  };
+
+  for (int s = s0 + wv; s < s1;) {
+    fetch_ids(s);
+    const int cnt = min(64, (s1 - s + kODWaves - 1) / kODWaves);  // steps of this wave in the set
+    OctStep<D> xa, xb;
+    load(0, xa);
+    int k = 0;
+    while (true) {
+      load(min(k + 1, cnt - 1), xb);
+      __builtin_amdgcn_sched_barrier(0);
+      step(s + kODWaves * k, xa);
+      if (++k >= cnt) break;
+      load(min(k + 1, cnt - 1), xa);
+      __builtin_amdgcn_sched_barrier(0);
+      step(s + kODWaves * k, xb);
+      if (++k >= cnt) break;
+    }
+    s += kODWaves * 64;
+  }
+  if (bad && lane == 0) atomicOr(a.err, TTKV_ERR_BAD_BLOCK);
+  l = bad ? NAN : cross_row_sum(l);
+
+  // ---- the four waves' results, joined in LDS
+  if (q4 == 0) {
+    red_m[wv][col] = m;
+    red_l[wv][col] = l;
+  }
+  __syncthreads();
+  {
+    float M = kODNone;
+#pragma unroll
+    for (int w = 0; w < kODWaves; ++w) M = fmaxf(M, red_m[w][col]);
+    const float f = exp2f(m - M);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int e = 0; e < N; e += 4)
+        *(float4v*)&red_o[wv][col][(4 * q4 + i) * N + e] =
+            float4v{acc[e][i] * f, acc[e + 1][i] * f, acc[e + 2][i] * f, acc[e + 3][i] * f};
+  }
+  __syncthreads();
+  const int PR = a.part_rows;
+  const int64_t part = ((int64_t)P.part + P.c) * a.H + h;  // (where the block is split)
+  for (int i = tid; i < nrow * (D / 4); i += kODThreads) {
+    const int r = i / (D / 4), d = i % (D / 4) * 4;
+    float mm = kODNone, ll = 0.f;
+    float4v o = {};
+#pragma unroll
+    for (int w = 0; w < kODWaves; ++w) mm = fmaxf(mm, red_m[w][r]);
+#pragma unroll
+    for (int w = 0; w < kODWaves; ++w) {
+      ll += red_l[w][r] * exp2f(red_m[w][r] - mm);
+      o += *(const float4v*)&red_o[w][r][d];
+    }
+    if (P.nch == 1) {
+      finish(r, d, o, mm, ll);
+    } else {
+      store_agent16(a.ws_o + (part * PR + r) * D + d, o);
+      if (d == 0) store_agent8(a.ws_ml + (part * PR + r) * 2, float2v{mm, ll});
+    }
+  }
+  if (P.nch == 1) return;
+
+  // ---- the last workgroup of a (block, head) joins its chunks' partials
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  __syncthreads();
+  if (tid == 0) {
+    int* cnt = a.ws_cnt + P.block * a.H + h;
+    const int prev = arrive(cnt);
+    last_sh = prev == P.nch - 1;
+    if (last_sh) __hip_atomic_store(cnt, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  }
+  __syncthreads();
+  if (!last_sh) return;
+  // d / 4 lanes take a row, four dims each, chunk after chunk with a running maximum; where rows are few,
+  // 2^share such teams take every 2^share-th chunk of a row and are joined in LDS.
+  constexpr int LPR = D / 4, TEAMS = kODThreads / LPR, AHEAD = 8;
+  const int team = tid / LPR, d4 = tid % LPR * 4;
+  int share = 0;
+  while (nrow << (share + 1) <= TEAMS && 2 << share <= P.nch) ++share;
+  const int64_t part0 = (int64_t)P.part * a.H + h;
+  const int sub = team & ((1 << share) - 1);
+  for (int r0 = 0; r0 < nrow; r0 += TEAMS >> share) {
+    const int r = r0 + (team >> share);
+    float mm = kODNone, ll = 0.f;
+    float4v o = {};
+    if (r < nrow)
+      for (int c0 = sub; c0 < P.nch; c0 += AHEAD << share) {
+        float4v x[AHEAD];
+        float2v ml[AHEAD];
+#pragma unroll
+        for (int u = 0; u < AHEAD; ++u) {
+          const int c = min(c0 + (u << share), P.nch - 1);
+          const int64_t at = (part0 + (int64_t)c * a.H) * PR + r;
+          ml[u] = ld_agent2(a.ws_ml + at * 2);
+          x[u] = ld_agent16(a.ws_o, a.o_bytes, (uint32_t)((at * D + d4) * 4));
+        }
+#pragma unroll
+        for (int u = 0; u < AHEAD; ++u)
+          if (c0 + (u << share) < P.nch) {
+            const float mn = fmaxf(mm, ml[u][0]), f = exp2f(mm - mn), g = exp2f(ml[u][0] - mn);
+            o = o * f + x[u] * g;
+            ll = ll * f + ml[u][1] * g;
+            mm = mn;
+          }
+      }
+    if (share) {  // (one round: rows << share fit the teams)
+      float* at = red_all + team * (D + 8);
+      *(float4v*)(at + d4) = o;
+      if (d4 == 0) {
+        at[D] = mm;
+        at[D + 1] = ll;
+      }
+      __syncthreads();
+      if (sub) return;
+      for (int u = 1; u < 1 << share; ++u) {
+        const float* y = at + u * (D + 8);
+        const float mn = fmaxf(mm, y[D]), f = exp2f(mm - mn), g = exp2f(y[D] - mn);
+        o = o * f + *(const float4v*)(y + d4) * g;
+        ll = ll * f + y[D + 1] * g;
+        mm = mn;
+      }
+    }
+    if (r < nrow) finish(r, d4, o, mm, ll);
+  }
+}
+
+// The plan's item target: workgroups that are resident.
+static int od_target(int d) { return (d == 256 ? 1 : 2) * device_cu_count(); }
+
+// Requests per launch, of `blocks` row blocks each: the plan's lanes, and a counter per (block, head).
+static int od_slice(int H, int blocks, int num_reqs) {
+  return std::max(1, std::min({num_reqs, kODPlanLanes * 64, kMaxCounters / (H * blocks)}));
+}
+
+// Items of split blocks, at most, of `pairs` (block, head) pairs. A chunk has at least total / target
+// steps, and a split block of st steps has less than st / C + 1 < 2 st / C chunks: less than 2 target of
+// them in all; and whole rounds of the four waves of a request.
+static int64_t od_max_chunks(int max_seq) {
+  const int64_t round = kODStep * kODWaves;
+  return std::max<int64_t>(1, (max_seq + round - 1) / round + 1);  // (a window's first step may be cut)
+}
+static int64_t od_parts(int d, int64_t pairs, int max_seq) {
+  return std::min<int64_t>(2 * od_target(d), pairs * od_max_chunks(max_seq));
+}
+
+int64_t octet_decode_workspace_bytes(int H, int HQ, int d, int num_reqs, int max_q, int max_seq) {
+  if (num_reqs == 0 || max_q == 0) return 256;
+  // (sizes that grow with every argument: layers of unlike heads share a workspace)
+  return kCounterBytes + (int64_t)2 * 2 * device_cu_count() * kODRows * (d + 2) * 4;
+}
+
+template <int D>
+static int od_launch(const OctDecodeArgs& a, unsigned grid, int q_dtype, bool chunk, hipStream_t st) {
+  constexpr int smem = kODWaves * kODRows * (D + 4) * 4;
+  auto kernel = q_dtype == TTKV_DTYPE_F16
+                    ? chunk ? octet_decode_kernel<D, TTKV_DTYPE_F16, true> : octet_decode_kernel<D, TTKV_DTYPE_F16, false>
+                : chunk ? octet_decode_kernel<D, TTKV_DTYPE_BF16, true>
+                        : octet_decode_kernel<D, TTKV_DTYPE_BF16, false>;
+  if (smem > 65536 - 4096)
+    if (int rc = raise_smem_limit((const void*)kernel, smem)) return rc;
+  hipLaunchKernelGGL(kernel, dim3(grid), dim3(kODThreads), smem, st, a);
+  const hipError_t e = hipGetLastError();
+  if (e != hipSuccess)
+    return host_fail(TTKV_E_LAUNCH, std::string("octet decode launch: ") + hipGetErrorString(e));
+  return TTKV_OK;
+}
 
 int octet_decode_paged(int H, int HQ, int d, float scale, const void* q, int q_dtype, int64_t q_row_stride,
                        int num_tokens, const uint8_t* page, int64_t n_slots, int64_t slot_stride, int bs,
@@ -112,6 +595,7 @@ int octet_decode_paged(int H, int HQ, int d, float scale, const void* q, int q_d
       return host_fail(TTKV_E_INVALID, "query / out dtype must be fp16 or bf16");
   if (num_tokens < 0 || max_q < 0) return host_fail(TTKV_E_INVALID, "negative count");
   if (max_q > kODMaxQ) return host_fail(TTKV_E_UNSUPPORTED, "more than 16 queries per request");
+  if (H > kMaxCounters / (kODMaxQ * 16 / kODRows)) return host_fail(TTKV_E_UNSUPPORTED, "too many KV heads");
   if (window < 0) return host_fail(TTKV_E_INVALID, "negative window");
   if (num_reqs && (!q || !bt || !seq_lens || !qsl || !out || !err))
     return host_fail(TTKV_E_INVALID, "null pointer argument");
@@ -122,16 +606,49 @@ int octet_decode_paged(int H, int HQ, int d, float scale, const void* q, int q_d
     return host_fail(TTKV_E_WORKSPACE, "decode workspace needs " + std::to_string(need) + " bytes, 256-aligned");
   if (num_reqs == 0 || num_tokens == 0 || max_q == 0) return TTKV_OK;
   if (window >= max_seq) window = 0;  // no window
-  OctDecodeArgs a{H,        HQ / H,     scale,          q,   q_dtype,       q_row_stride, num_tokens, page,
-                  kOctTile * slot_stride, (int)(n_slots / bs), bs / kOctTile, bt, bt_row_stride, seq_lens, qsl, max_q,
-                  max_seq,  window,     sinks,          out, out_dtype,     out_row_stride, lse,    err};
-  auto kernel = d == 64 ? octet_decode_kernel<64> : d == 128 ? octet_decode_kernel<128> : octet_decode_kernel<256>;
-  const int64_t grid = (int64_t)num_reqs * max_q * HQ;
-  if (grid > 0x7fffffff) return host_fail(TTKV_E_INVALID, "too many requests for one call");
-  hipLaunchKernelGGL(kernel, dim3((unsigned)grid), dim3(256), 0, st, a);
-  const hipError_t e = hipGetLastError();
-  if (e != hipSuccess)
-    return host_fail(TTKV_E_LAUNCH, std::string("octet decode launch: ") + hipGetErrorString(e));
+  const int rows = HQ / H * max_q, blocks = (rows + kODRows - 1) / kODRows;
+  const int slice = od_slice(H, blocks, num_reqs);
+  const int64_t parts = od_parts(d, (int64_t)slice * H * blocks, max_seq);
+  OctDecodeArgs a{};
+  a.H = H;
+  a.G = HQ / H;
+  a.scale_log2 = scale * kLog2e;
+  a.q = (const uint16_t*)q;
+  a.q_row_stride = q_row_stride;
+  a.num_tokens = num_tokens;
+  a.page = page;
+  a.tile_stride = kOctTile * slot_stride;
+  a.num_blocks = (int)(n_slots / bs);
+  a.tpb = bs / kOctTile;
+  a.bt_row_stride = bt_row_stride;
+  a.max_q = max_q;
+  a.max_seq = max_seq;
+  a.window = window;
+  a.sinks = sinks;
+  a.out = out;
+  a.out_dtype = out_dtype;
+  a.out_row_stride = out_row_stride;
+  a.lse = lse;
+  a.part_rows = std::min(rows, kODRows);
+  a.ws_cnt = (int*)ws;
+  a.ws_o = (float*)((char*)ws + kCounterBytes);
+  a.ws_ml = a.ws_o + parts * a.part_rows * d;
+  a.o_bytes = (uint32_t)(parts * a.part_rows * d * 4);
+  a.target = od_target(d);
+  a.err = err;
+  for (int r0 = 0; r0 < num_reqs; r0 += slice) {
+    a.num_reqs = std::min(slice, num_reqs - r0);
+    a.seq_lens = seq_lens + r0;
+    a.qsl = qsl + r0;
+    a.bt = bt + (int64_t)r0 * bt_row_stride;
+    // an item per (block, head), and what the split ones have more
+    const int64_t pairs = (int64_t)a.num_reqs * H * blocks;
+    const unsigned grid = (unsigned)std::min(pairs + a.target, pairs * od_max_chunks(max_seq));
+    const int rc = d == 64    ? od_launch<64>(a, grid, q_dtype, max_q > 1, st)
+                   : d == 128 ? od_launch<128>(a, grid, q_dtype, max_q > 1, st)
+                              : od_launch<256>(a, grid, q_dtype, max_q > 1, st);
+    if (rc != TTKV_OK) return rc;
+  }
   return TTKV_OK;
 }
 
