@@ -291,5 +291,46 @@ __device__ __forceinline__ void store_act4(void* p, int dt, int64_t i, float4v v
   }
 }
 
-}  // namespace ttkv
+// Eight consecutive elements of a 16-byte aligned row piece, in registers and as floats.
+template <int DT>
+struct Act8 {
+  u32x4 raw[DT == TTKV_DTYPE_F32 ? 2 : 1];
+};
+template <int DT>
+__device__ __forceinline__ Act8<DT> load_act8(const void* p, int64_t i) {
+  Act8<DT> x;
+  const char* at = (const char*)p + i * (DT == TTKV_DTYPE_F32 ? 4 : 2);
+#pragma unroll
+  for (int j = 0; j < (DT == TTKV_DTYPE_F32 ? 2 : 1); ++j)
+    x.raw[j] = __builtin_nontemporal_load(gbl((const u32x4*)at + j));
+  return x;
+}
+template <int DT>
+__device__ __forceinline__ float act8_get(const Act8<DT>& x, int i) {
+  if constexpr (DT == TTKV_DTYPE_F32) {
+    const uint32_t w = x.raw[i >> 2][i & 3];  // (by value: a bit cast of an element reads the first)
+    return __builtin_bit_cast(float, w);
+  }
+  const uint32_t w = x.raw[0][i >> 1], b = i & 1 ? w >> 16 : w & 0xffffu;
+  return DT == TTKV_DTYPE_F16 ? f16_bits_to_float(b) : bf16_bits_to_float(b);
+}
+template <int DT>
+__device__ __forceinline__ void store_act8(void* p, int64_t i, const float v[8]) {
+  if constexpr (DT == TTKV_DTYPE_F32) {
+    store_act4(p, DT, i, float4v{v[0], v[1], v[2], v[3]}, true);
+    store_act4(p, DT, i + 4, float4v{v[4], v[5], v[6], v[7]}, true);
+  } else {
+    u32x4 w;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const float lo = v[2 * k], hi = v[2 * k + 1];
+      if constexpr (DT == TTKV_DTYPE_F16)
+        w[k] = __builtin_bit_cast(uint32_t, half2v{(_Float16)lo, (_Float16)hi});
+      else
+        w[k] = (uint32_t)float_to_bf16_bits(lo) | ((uint32_t)float_to_bf16_bits(hi) << 16);
+    }
+    *gblw((u32x4*)((uint16_t*)p + i)) = w;
+  }
+}
 
+}  // namespace ttkv

@@ -1,13 +1,15 @@
 // Read of stored keys and values out of the 8-bit cache (format: ttkv_octet.h) as rows. gfx950 / CDNA4.
+// Bound by memory: every stored byte read and every row written once.
 #include <math.h>
 
 #include "ttkv_host.h"
+#include "ttkv_nibble.h"
 #include "ttkv_octet.h"
 
 namespace ttkv {
 
 struct OctReadArgs {
-  int H;
+  int H, num_reqs;
   const uint8_t* page;
   int64_t tile_stride;
   int num_blocks, tpb;  // tpb: tiles per block
@@ -23,45 +25,139 @@ struct OctReadArgs {
   int32_t* err;
 };
 
-// One workgroup per (request, KV head); a thread per 8 dims of a row.
-template <int D>
+// A request's rows that the outputs hold, and the tiles of their tokens.
+struct OctReadRows {
+  int64_t t0;      // token of row k is t0 + k, in row row0 + k
+  int row0, lo, hi;  // k in [lo, hi)
+  int tile, tiles;
+};
+__device__ __forceinline__ OctReadRows oct_read_rows(const OctReadArgs& a, int r, bool& clipped) {
+  OctReadRows x;
+  x.row0 = a.starts[r];
+  const int64_t rows = (int64_t)a.starts[r + 1] - x.row0;
+  x.t0 = a.first ? a.first[r] : 0;
+  x.lo = max(0, -x.row0);
+  x.hi = (int)min(rows, (int64_t)a.num_rows - x.row0);
+  clipped = rows < 0 || (rows > 0 && (x.lo > 0 || x.hi < rows));
+  x.tile = (int)((x.t0 + x.lo) >> 4);
+  x.tiles = x.hi > x.lo ? (int)((x.t0 + x.hi - 1) >> 4) - x.tile + 1 : 0;
+  return x;
+}
+
+// A wave per (tile, KV head): its lanes take 8 dims of a row each, d / 8 lanes a row, so that rows are
+// stored whole, and every load of the record is under way before the first is used.
+template <int D, int DT, bool VEC>
 __global__ __launch_bounds__(256) void octet_read_kernel(OctReadArgs a) {
   using F = Oct<D>;
-  constexpr int kLanes = D / 8;
-  const int h = (int)(blockIdx.x % (unsigned)a.H), r = (int)(blockIdx.x / (unsigned)a.H);
-  const int i = threadIdx.x % kLanes, x = 8 * i;
-  const int64_t row0 = a.starts[r], rows = (int64_t)a.starts[r + 1] - row0;
-  const int64_t t0 = a.first ? a.first[r] : 0;
-  for (int64_t k = threadIdx.x / kLanes; k < rows; k += 256 / kLanes) {
-    const int64_t row = row0 + k, t = t0 + k;
-    if (row < 0 || row >= a.num_rows) {
-      if (h == 0 && i == 0) atomicOr(a.err, TTKV_ERR_SEQ_LEN);
-      continue;
+  constexpr int kLanes = D / 8, kRows = 64 / kLanes, kRounds = 16 / kRows;
+  const int lane = threadIdx.x & 63;
+  const int i = lane % kLanes, x = 8 * i;
+  const int64_t waves = (int64_t)gridDim.x * 4;
+  for (int64_t item = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);; item += waves) {
+    const int64_t want = item / a.H;
+    const int h = (int)(item - want * a.H);
+    // the request whose tiles hold number `want`
+    int r = -1;
+    int64_t before = 0;
+    OctReadRows rq{};
+    for (int r0 = 0; r0 < a.num_reqs && r < 0; r0 += 64) {
+      bool clipped = false;
+      OctReadRows mine{};
+      if (r0 + lane < a.num_reqs) mine = oct_read_rows(a, r0 + lane, clipped);
+      if (clipped && item == 0) atomicOr(a.err, TTKV_ERR_SEQ_LEN);
+      const int incl = nib_scan(mine.tiles);
+      const int64_t at = want - before;
+      const uint64_t hit = __builtin_amdgcn_ballot_w64(at < incl && mine.tiles > 0);
+      if (hit) {
+        const int ln = __builtin_ctzll(hit);
+        r = r0 + ln;
+        rq.row0 = __builtin_amdgcn_readlane(mine.row0, ln);
+        rq.lo = __builtin_amdgcn_readlane(mine.lo, ln);
+        rq.hi = __builtin_amdgcn_readlane(mine.hi, ln);
+        rq.t0 = a.first ? a.first[r] : 0;
+        rq.tile = __builtin_amdgcn_readlane(mine.tile, ln) + (int)at - __builtin_amdgcn_readlane(incl - mine.tiles, ln);
+      }
+      before += __builtin_amdgcn_readlane(incl, 63);
+      if (item == 0 && r >= 0)  // (the requests behind the first hit are looked at for their rows, too)
+        for (int k = r0 + 64 + lane; k < a.num_reqs; k += 64) {
+          oct_read_rows(a, k, clipped);
+          if (clipped) atomicOr(a.err, TTKV_ERR_SEQ_LEN);
+        }
     }
-    float kv[2][8];
-    for (int j = 0; j < 8; ++j) kv[0][j] = kv[1][j] = NAN;
-    if (t < 0 || t >= a.max_seq) {
-      if (h == 0 && i == 0) atomicOr(a.err, TTKV_ERR_SEQ_LEN);
-    } else {
-      const int tile = (int)(t / kOctTile), b = tile / a.tpb, u = (int)(t % kOctTile);
-      const int id = a.bt[r * a.bt_row_stride + b];
+    if (r < 0) return;
+    const int64_t tok = (int64_t)rq.tile * 16;
+    // a token outside the call's lengths or a block outside the cache: NaN
+    const int b = rq.tile < 0 ? 0 : rq.tile / a.tpb;
+    int id = -1;
+    if (tok >= 0 && tok < a.max_seq) {
+      id = a.bt[r * a.bt_row_stride + b];
       if ((uint32_t)id >= (uint32_t)a.num_blocks) {
-        if (h == 0 && i == 0) atomicOr(a.err, TTKV_ERR_BAD_BLOCK);
+        id = -1;
+        if (lane == 0 && h == 0) atomicOr(a.err, TTKV_ERR_BAD_BLOCK);
+      }
+    }
+    const uint8_t* rec = a.page + ((int64_t)max(id, 0) * a.tpb + max(rq.tile, 0) - b * a.tpb) * a.tile_stride +
+                         (int64_t)h * F::kRecord;
+    u32x2v c[2][kRounds];
+    uint8_t pw[2][kRounds];
+#pragma unroll
+    for (int k = 0; k < kRounds; ++k) {
+      const int u = k * kRows + lane / kLanes;
+      c[0][k] = *gbl((const u32x2v*)(rec + F::key(u, x)));
+      pw[0][k] = *gbl(rec + F::key_power(u, x / 32));
+      if constexpr (D == 64) {
+        c[1][k][0] = *gbl((const uint32_t*)(rec + F::value(u, x)));
+        c[1][k][1] = *gbl((const uint32_t*)(rec + F::value(u, x + 4)));
       } else {
-        const uint8_t* rec =
-            a.page + ((int64_t)id * a.tpb + tile - b * a.tpb) * a.tile_stride + (int64_t)h * F::kRecord;
-        const float kp = oct_power(rec[F::key_power(u, x / 32)]), vp = oct_power(rec[F::value_power(u, x / 32)]);
-        for (int j = 0; j < 8; ++j) {
-          kv[0][j] = (float)oct_pair<false>(rec[F::key(u, x + j)], kp)[0];
-          kv[1][j] = (float)oct_pair<false>(rec[F::value(u, x + j)], vp)[0];
+        c[1][k] = *gbl((const u32x2v*)(rec + F::value(u, x)));
+      }
+      pw[1][k] = *gbl(rec + F::value_power(u, x / 32));
+    }
+#pragma unroll
+    for (int k = 0; k < kRounds; ++k) {
+      const int64_t t = tok + k * kRows + lane / kLanes, at = t - rq.t0;
+      if (at < rq.lo || at >= rq.hi) continue;
+      const bool in = t >= 0 && t < a.max_seq;
+      if (!in && h == 0 && i == 0) atomicOr(a.err, TTKV_ERR_SEQ_LEN);
+      const bool nan = id < 0 || !in;
+#pragma unroll
+      for (int kv = 0; kv < 2; ++kv) {
+        const float p = oct_power(pw[kv][k]);
+        bf16x2 o[4] = {oct_pair<false>(c[kv][k][0], p), oct_pair<true>(c[kv][k][0], p),
+                       oct_pair<false>(c[kv][k][1], p), oct_pair<true>(c[kv][k][1], p)};
+        const int64_t to = (rq.row0 + at) * (kv ? a.v_stride : a.k_stride) + (int64_t)h * D + x;
+        void* out = kv ? a.v_out : a.k_out;
+        if (VEC && DT == TTKV_DTYPE_BF16) {
+          u32x4 w;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) w[j] = nan ? 0x7fc07fc0u : __builtin_bit_cast(uint32_t, o[j]);
+          *gblw((u32x4*)((uint16_t*)out + to)) = w;
+        } else {
+          float f[8];
+#pragma unroll
+          for (int j = 0; j < 8; ++j) f[j] = nan ? NAN : (float)o[j >> 1][j & 1];
+          if (VEC) store_act8<DT>(out, to, f);
+          else
+#pragma unroll
+            for (int j = 0; j < 8; ++j) store_act(out, DT, to + j, f[j]);
         }
       }
     }
-    for (int j = 0; j < 8; ++j) {
-      store_act(a.k_out, a.out_dtype, row * a.k_stride + h * D + x + j, kv[0][j]);
-      store_act(a.v_out, a.out_dtype, row * a.v_stride + h * D + x + j, kv[1][j]);
-    }
   }
+}
+
+template <int D, int DT>
+static void oct_read_launch(const OctReadArgs& a, unsigned grid, bool vec, hipStream_t st) {
+  if (vec)
+    hipLaunchKernelGGL((octet_read_kernel<D, DT, true>), dim3(grid), dim3(256), 0, st, a);
+  else
+    hipLaunchKernelGGL((octet_read_kernel<D, DT, false>), dim3(grid), dim3(256), 0, st, a);
+}
+template <int D>
+static void oct_read_launch(const OctReadArgs& a, unsigned grid, bool vec, hipStream_t st) {
+  if (a.out_dtype == TTKV_DTYPE_F32) oct_read_launch<D, TTKV_DTYPE_F32>(a, grid, vec, st);
+  else if (a.out_dtype == TTKV_DTYPE_F16) oct_read_launch<D, TTKV_DTYPE_F16>(a, grid, vec, st);
+  else oct_read_launch<D, TTKV_DTYPE_BF16>(a, grid, vec, st);
 }
 
 int octet_check_table(int bs, int64_t n_slots, int num_reqs, int max_blocks, int max_seq) {
@@ -88,12 +184,18 @@ int octet_read_paged(int H, int d, const uint8_t* page, int64_t n_slots, int64_t
   if (num_rows < 0) return host_fail(TTKV_E_INVALID, "negative count");
   if (num_reqs == 0 || num_rows == 0) return TTKV_OK;
   if (!bt || !starts || !k_out || !v_out || !err) return host_fail(TTKV_E_INVALID, "null pointer argument");
-  if ((int64_t)num_reqs * H > 0x7fffffff) return host_fail(TTKV_E_INVALID, "too many requests for one call");
-  OctReadArgs a{H,     page,    kOctTile * slot_stride, (int)(n_slots / bs), bs / kOctTile, bt,       bt_row_stride,
-                starts, first,  max_seq,                num_rows,            k_out,         v_out,    k_stride,
-                v_stride, out_dtype, err};
-  auto kernel = d == 64 ? octet_read_kernel<64> : d == 128 ? octet_read_kernel<128> : octet_read_kernel<256>;
-  hipLaunchKernelGGL(kernel, dim3((unsigned)(num_reqs * H)), dim3(256), 0, st, a);
+  const int64_t eb = out_dtype == TTKV_DTYPE_F32 ? 4 : 2;
+  // wide stores where every row starts 16-byte aligned; else an element at a time
+  const bool vec = ((uintptr_t)k_out | (uintptr_t)v_out) % 16 == 0 && (k_stride * eb | v_stride * eb) % 16 == 0;
+  OctReadArgs a{H,     num_reqs, page,    kOctTile * slot_stride, (int)(n_slots / bs), bs / kOctTile, bt, bt_row_stride,
+                starts, first,   max_seq, num_rows,               k_out,               v_out,         k_stride, v_stride,
+                out_dtype, err};
+  // a wave per (tile, head), of rows that start anywhere in a tile; those beyond the grid in turn
+  const int64_t items = ((int64_t)num_rows / kOctTile + 2 * (int64_t)num_reqs) * H;
+  const unsigned grid = (unsigned)std::min<int64_t>((items + 3) / 4, 1 << 20);
+  if (d == 64) oct_read_launch<64>(a, grid, vec, st);
+  else if (d == 128) oct_read_launch<128>(a, grid, vec, st);
+  else oct_read_launch<256>(a, grid, vec, st);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess)
     return host_fail(TTKV_E_LAUNCH, std::string("octet read launch: ") + hipGetErrorString(e));

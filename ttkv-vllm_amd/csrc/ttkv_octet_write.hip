@@ -130,9 +130,21 @@ __global__ __launch_bounds__(256) void octet_write_kernel(OctWriteArgs a) {
   }
 }
 
+// A workgroup per token.
 __global__ __launch_bounds__(256) void rotary_scaled_kernel(TurnArgs a) {
   __shared__ float2v cs[kTurnHalf];
-  turn_token(a, blockIdx.x, threadIdx.x, 256, cs);
+  turn_token(a, blockIdx.x, threadIdx.x, (int)blockDim.x, cs);
+}
+
+// Whether rows go in pieces of 8 elements by a workgroup of `threads`: aligned, and pairs within them.
+static bool turn_pieces_apply(const TurnArgs& a, int threads) {
+  const int64_t eb = a.dtype == TTKV_DTYPE_F32 ? 4 : 2;
+  if (a.d % 8 || a.half % (a.adjacent ? 4 : 8) || a.half / (a.adjacent ? 4 : 8) > threads) return false;
+  for (int i = 0; i < 2; ++i)
+    if (a.heads[i] && (((uintptr_t)a.x[i] | (uintptr_t)a.y[i]) % 16 || a.x_stride[i] * eb % 16 ||
+                       a.y_stride[i] * eb % 16))
+      return false;
+  return true;
 }
 
 static bool act_dtype(int dt) {
@@ -171,8 +183,11 @@ int rotary_scaled(const void* q, const void* k, void* qo, void* ko, int dtype, i
       rows_meet(qo, qo_stride * eb, qw, ko, ko_stride * eb, kw, N))
     return host_fail(TTKV_E_INVALID, "one of query and key overlaps the other's output");
   TurnArgs a{{q, k},  {qo, ko}, {HQ, H}, {q_stride, k_stride}, {qo_stride, ko_stride}, dtype, d,
-             rot / 2, adjacent, pos,     turns,                amplitude,              err};
-  hipLaunchKernelGGL(rotary_scaled_kernel, dim3(N), dim3(256), 0, st, a);
+             rot / 2, adjacent != 0, 0, pos, turns,            amplitude,              err};
+  // a wave per token; four share the rows of a token where there are few
+  const int threads = N >= 4 * device_cu_count() ? 64 : 256;
+  a.pieces = turn_pieces_apply(a, threads);
+  hipLaunchKernelGGL(rotary_scaled_kernel, dim3(N), dim3(a.pieces ? threads : 256), 0, st, a);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess)
     return host_fail(TTKV_E_LAUNCH, std::string("scaled rotary launch: ") + hipGetErrorString(e));
@@ -226,7 +241,8 @@ int octet_write_paged(int H, int d, const void* key, int k_dtype, int64_t k_row_
   OctWriteArgs a{key,  val,     k_dtype,     v_dtype,          k_row_stride,     v_row_stride, slots,      num_tokens, H,
                  page, n_slots, slot_stride, (uint16_t*)k_out, (uint16_t*)v_out, err,          (int)blocks};
   a.turn = TurnArgs{{q, nullptr},  {qo, nullptr}, {HQ, 0},     {q_stride, 0}, {qo_stride, 0}, q_dtype, d, rot / 2,
-                    adjacent != 0, pos,           turns,       amplitude,     err};
+                    adjacent != 0, 0,             pos,         turns,         amplitude,       err};
+  a.turn.pieces = HQ && turn_pieces_apply(a.turn, 256);
   auto kernel = d == 64 ? octet_write_kernel<64> : d == 128 ? octet_write_kernel<128> : octet_write_kernel<256>;
   hipLaunchKernelGGL(kernel, dim3((unsigned)grid), dim3(256), 0, st, a);
   const hipError_t e = hipGetLastError();

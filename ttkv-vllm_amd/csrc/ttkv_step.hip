@@ -266,48 +266,6 @@ __device__ __forceinline__ bool rot_positions(const RotArgs& a, int64_t tok,
   return ok;
 }
 
-// Eight consecutive elements of a 16-byte aligned row piece, in registers and as floats.
-template <int DT>
-struct Rot8 {
-  u32x4 raw[DT == TTKV_DTYPE_F32 ? 2 : 1];
-};
-template <int DT>
-__device__ __forceinline__ Rot8<DT> rot_load8(const void* p, int64_t i) {
-  Rot8<DT> x;
-  const char* at = (const char*)p + i * (DT == TTKV_DTYPE_F32 ? 4 : 2);
-#pragma unroll
-  for (int j = 0; j < (DT == TTKV_DTYPE_F32 ? 2 : 1); ++j)
-    x.raw[j] = __builtin_nontemporal_load(gbl((const u32x4*)at + j));
-  return x;
-}
-template <int DT>
-__device__ __forceinline__ float rot_get(const Rot8<DT>& x, int i) {
-  if constexpr (DT == TTKV_DTYPE_F32) {
-    const uint32_t w = x.raw[i >> 2][i & 3];  // (by value: a bit cast of an element reads the first)
-    return __builtin_bit_cast(float, w);
-  }
-  const uint32_t w = x.raw[0][i >> 1], b = i & 1 ? w >> 16 : w & 0xffffu;
-  return DT == TTKV_DTYPE_F16 ? f16_bits_to_float(b) : bf16_bits_to_float(b);
-}
-template <int DT>
-__device__ __forceinline__ void rot_store8(void* p, int64_t i, const float v[8]) {
-  if constexpr (DT == TTKV_DTYPE_F32) {
-    store_act4(p, DT, i, float4v{v[0], v[1], v[2], v[3]}, true);
-    store_act4(p, DT, i + 4, float4v{v[4], v[5], v[6], v[7]}, true);
-  } else {
-    u32x4 w;
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const float lo = v[2 * k], hi = v[2 * k + 1];
-      if constexpr (DT == TTKV_DTYPE_F16)
-        w[k] = __builtin_bit_cast(uint32_t, half2v{(_Float16)lo, (_Float16)hi});
-      else
-        w[k] = (uint32_t)float_to_bf16_bits(lo) | ((uint32_t)float_to_bf16_bits(hi) << 16);
-    }
-    *gblw((u32x4*)((uint16_t*)p + i)) = w;
-  }
-}
-
 // One wave per token. Lane j first looks up frequency j's cosine and sine (one load each, whatever
 // the axes) and leaves them in LDS; then the lanes take (head, 8 frequencies) pairs of 16-byte pieces,
 // four heads' loads in flight at a time, the first four asked for before the lookup. Bound by memory:
@@ -331,7 +289,7 @@ __global__ __launch_bounds__(64) void rotary_rows_kernel(RotArgs a) {
     at = tok * stride + (int64_t)(is_q ? head : head - a.HQ) * a.d;
     return out ? (is_q ? a.qo : a.ko) : (is_q ? a.q : a.k);
   };
-  Rot8<DT> x[kRotBatch], y[kRotBatch];
+  Act8<DT> x[kRotBatch], y[kRotBatch];
   auto fetch = [&](int h0) {
 #pragma unroll
     for (int b = 0; b < kRotBatch; ++b) {
@@ -339,8 +297,8 @@ __global__ __launch_bounds__(64) void rotary_rows_kernel(RotArgs a) {
       if (on && head < heads) {
         int64_t at;
         const void* src = place(head, false, at);
-        x[b] = rot_load8<DT>(src, at + j0);
-        y[b] = rot_load8<DT>(src, at + j0 + a.half);
+        x[b] = load_act8<DT>(src, at + j0);
+        y[b] = load_act8<DT>(src, at + j0 + a.half);
       }
     }
   };
@@ -374,12 +332,12 @@ __global__ __launch_bounds__(64) void rotary_rows_kernel(RotArgs a) {
         float u[8], v[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          const float xi = rot_get<DT>(x[b], i), yi = rot_get<DT>(y[b], i);
+          const float xi = act8_get<DT>(x[b], i), yi = act8_get<DT>(y[b], i);
           u[i] = xi * c[i] - yi * s[i];
           v[i] = yi * c[i] + xi * s[i];
         }
-        rot_store8<DT>(dst, at + j0, u);
-        rot_store8<DT>(dst, at + j0 + a.half, v);
+        store_act8<DT>(dst, at + j0, u);
+        store_act8<DT>(dst, at + j0 + a.half, v);
       }
     }
     fetch(h0 + kRotBatch * slots);
@@ -390,11 +348,11 @@ __global__ __launch_bounds__(64) void rotary_rows_kernel(RotArgs a) {
     int64_t from, to;
     const void* src = place(head, false, from);
     void* dst = const_cast<void*>(place(head, true, to));
-    const Rot8<DT> z = rot_load8<DT>(src, from + x0);
+    const Act8<DT> z = load_act8<DT>(src, from + x0);
     float v[8];
 #pragma unroll
-    for (int k = 0; k < 8; ++k) v[k] = ok ? rot_get<DT>(z, k) : NAN;
-    rot_store8<DT>(dst, to + x0, v);
+    for (int k = 0; k < 8; ++k) v[k] = ok ? act8_get<DT>(z, k) : NAN;
+    store_act8<DT>(dst, to + x0, v);
   }
 }
 

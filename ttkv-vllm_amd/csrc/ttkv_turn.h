@@ -36,6 +36,7 @@ struct TurnArgs {
   int heads[2];
   int64_t x_stride[2], y_stride[2];
   int dtype, d, half, adjacent;
+  int pieces;  // rows go in pieces of 8 elements
   const int64_t* pos;
   const double* turns;
   float amplitude;
@@ -56,8 +57,98 @@ __device__ __forceinline__ bool turn_table(const int64_t* pos, const double* tur
   return ok;
 }
 
-// One token's rows, an element or a pair per thread.
+// One token's rows by the threads of a workgroup, in pieces of 8 elements: rows whose pieces are 16-byte
+// aligned, pairs that lie in one piece or in two. A thread keeps its piece's frequencies from head to head;
+// kTurnBatch heads' loads are in flight at a time, the first ones asked for before the angles are formed.
+constexpr int kTurnBatch = 4;
+template <int DT>
+__device__ __forceinline__ void turn_pieces(const TurnArgs& a, int64_t tok, int tid, int threads, float2v* cs) {
+  const bool adj = a.adjacent;
+  const int nch = adj ? a.half >> 2 : a.half >> 3;  // pieces (by halves: pairs of them) that are turned
+  const int slots = threads / nch, heads = a.heads[0] + a.heads[1];
+  const int slot = tid / nch, p = tid - slot * nch, mate = adj ? 0 : a.half;
+  const bool on = slot < slots;
+  auto place = [&](int head, bool out, int64_t& at) -> const void* {
+    const int set = head >= a.heads[0];
+    at = tok * (out ? a.y_stride : a.x_stride)[set] + (int64_t)(set ? head - a.heads[0] : head) * a.d;
+    return out ? a.y[set] : a.x[set];
+  };
+  Act8<DT> x[kTurnBatch], y[kTurnBatch];
+  auto fetch = [&](int h0) {
+#pragma unroll
+    for (int b = 0; b < kTurnBatch; ++b) {
+      const int head = h0 + b * slots + slot;
+      if (on && head < heads) {
+        int64_t at;
+        const void* src = place(head, false, at);
+        x[b] = load_act8<DT>(src, at + 8 * p);
+        if (!adj) y[b] = load_act8<DT>(src, at + 8 * p + mate);
+      }
+    }
+  };
+  fetch(0);
+  const bool ok = turn_table(a.pos, a.turns, a.half, a.amplitude, tok, tid, threads, cs);
+  if (!ok && tid == 0) atomicOr(a.err, TTKV_ERR_BAD_POSITION);
+  __syncthreads();
+  float c[8], s[8];  // (adjacent pairs: four)
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float2v w = cs[adj ? 4 * p + (i & 3) : on ? 8 * p + i : 0];
+    c[i] = w[0];
+    s[i] = w[1];
+  }
+  for (int h0 = 0; h0 < heads; h0 += kTurnBatch * slots) {
+#pragma unroll
+    for (int b = 0; b < kTurnBatch; ++b) {
+      const int head = h0 + b * slots + slot;
+      if (on && head < heads) {
+        int64_t at;
+        void* dst = const_cast<void*>(place(head, true, at));
+        float u[8], v[8];
+        if (adj) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float xi = act8_get<DT>(x[b], 2 * i), yi = act8_get<DT>(x[b], 2 * i + 1);
+            u[2 * i] = xi * c[i] - yi * s[i];
+            u[2 * i + 1] = yi * c[i] + xi * s[i];
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const float xi = act8_get<DT>(x[b], i), yi = act8_get<DT>(y[b], i);
+            u[i] = xi * c[i] - yi * s[i];
+            v[i] = yi * c[i] + xi * s[i];
+          }
+          store_act8<DT>(dst, at + 8 * p + mate, v);
+        }
+        store_act8<DT>(dst, at + 8 * p, u);
+      }
+    }
+    fetch(h0 + kTurnBatch * slots);
+  }
+  const int rest = (a.d - 2 * a.half) >> 3;  // pieces that are copied
+  for (int i = tid; i < heads * rest; i += threads) {
+    const int head = i / rest, x0 = 2 * a.half + (i - head * rest) * 8;
+    int64_t from, to;
+    const void* src = place(head, false, from);
+    void* dst = const_cast<void*>(place(head, true, to));
+    if (dst == src && from == to && ok) continue;  // in place
+    const Act8<DT> z = load_act8<DT>(src, from + x0);
+    float v[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v[k] = ok ? act8_get<DT>(z, k) : NAN;
+    store_act8<DT>(dst, to + x0, v);
+  }
+}
+
+// One token's rows, in pieces or an element or a pair per thread.
 __device__ __forceinline__ void turn_token(const TurnArgs& a, int64_t tok, int tid, int threads, float2v* cs) {
+  if (a.pieces) {
+    if (a.dtype == TTKV_DTYPE_BF16) turn_pieces<TTKV_DTYPE_BF16>(a, tok, tid, threads, cs);
+    else if (a.dtype == TTKV_DTYPE_F16) turn_pieces<TTKV_DTYPE_F16>(a, tok, tid, threads, cs);
+    else turn_pieces<TTKV_DTYPE_F32>(a, tok, tid, threads, cs);
+    return;
+  }
   const bool ok = turn_table(a.pos, a.turns, a.half, a.amplitude, tok, tid, threads, cs);
   if (!ok && tid == 0) atomicOr(a.err, TTKV_ERR_BAD_POSITION);
   __syncthreads();
