@@ -28,15 +28,22 @@ struct OctWriteArgs {
   TurnArgs turn;     // half == 0: keys come rotated
 };
 
-template <int D>
+// The lane's value by xor 1 (STEP 0) or 2 (STEP 1) within 4 lanes.
+template <int STEP>
+__device__ __forceinline__ float quad_xor(float v) {
+  const int w = __builtin_bit_cast(int, v);
+  return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, w, STEP ? 0x4E : 0xB1, 0xF, 0xF, false));
+}
+
+// DT: the type of keys and values, or -1 where they differ (then by the arguments).
+template <int D, int DT>
 __global__ __launch_bounds__(256) void octet_write_kernel(OctWriteArgs a) {
   using F = Oct<D>;
   constexpr int kTokens = 1024 / D, kLanes = D / 8;
-  __shared__ float2v cs[kTurnHalf];
-  __shared__ float xs[kTokens][D];
+  __shared__ __align__(16) float2v cs[kTurnHalf];
   const int tid = threadIdx.x;
   if ((int)blockIdx.x >= a.write_blocks) {
-    turn_token(a.turn, (int)blockIdx.x - a.write_blocks, tid, 256, cs);
+    turn_block(a.turn, (int)blockIdx.x - a.write_blocks, tid, cs);
     return;
   }
   const int row = tid / kLanes, i = tid % kLanes, t = row % kTokens;  // dims 8 i .. 8 i + 7
@@ -44,41 +51,68 @@ __global__ __launch_bounds__(256) void octet_write_kernel(OctWriteArgs a) {
   const int h = (int)(blockIdx.x % (unsigned)a.H);
   const int64_t tok0 = (int64_t)(blockIdx.x / (unsigned)a.H) * kTokens, tok = tok0 + t;
   const bool on = tok < a.num_tokens;
+  const void* src = val ? a.v : a.k;
+  const int dt = DT >= 0 ? DT : val ? a.v_dtype : a.k_dtype;
+  const int64_t stride = val ? a.v_row_stride : a.k_row_stride, at = tok * stride + (int64_t)h * D;
+  const bool vec = act_rows_aligned(src, dt, stride);
+  const int half = a.turn.half;
+  // a lane's dims and the others of their pairs, in a piece of 8 where the halves are made of such
+  const bool whole = a.turn.adjacent || half % 8 == 0, mated = !val && !a.turn.adjacent && whole && 8 * i < 2 * half;
+  const int mate = 8 * i < half ? 8 * i + half : 8 * i - half;
+  float x[8] = {}, y[8] = {};
+  if (on) {
+    load_act_n<8>(src, dt, at + 8 * i, vec, x);
+    if (mated) load_act_n<8>(src, dt, at + mate, vec, y);
+  }
   const int64_t slot = on ? *gbl(a.slots + tok) : -1;  // negative: a padded token
   if (slot >= a.n_slots && !val && i == 0) atomicOr(a.err, TTKV_ERR_BAD_SLOT);
   const bool keep = slot >= 0 && slot < a.n_slots;
-  const void* src = val ? a.v : a.k;
-  const int dt = val ? a.v_dtype : a.k_dtype;
-  const int64_t stride = val ? a.v_row_stride : a.k_row_stride;
-  float x[8] = {};
-  if (keep) load_act_n<8>(src, dt, tok * stride + (int64_t)h * D + 8 * i, act_rows_aligned(src, dt, stride), x);
-  const int half = a.turn.half;
   if (half) {
-    // every token's table in turn: half frequencies of kTokens tokens fit, kTokens * half <= 512
-    for (int n = 0; n < kTokens; ++n)
-      if (tok0 + n < a.num_tokens) {
-        const bool ok = turn_table(a.turn.pos, a.turn.turns, half, a.turn.amplitude, tok0 + n, tid, 256,
-                                   cs + n * half);
-        if (!ok && tid == 0 && h == 0) atomicOr(a.err, TTKV_ERR_BAD_POSITION);
-      }
-    if (!val)
-#pragma unroll
-      for (int j = 0; j < 8; ++j) xs[t][8 * i + j] = x[j];
+    for (int e = tid; e < kTokens * half; e += 256) {  // (kTokens * half <= 512)
+      const int n = e / half, j = e - n * half;
+      if (tok0 + n >= a.num_tokens) break;
+      const int64_t p = *gbl(a.turn.pos + tok0 + n);
+      cs[e] = turn_at(a.turn.turns, j, p, a.turn.amplitude);
+      if (j == 0 && h == 0 && !turn_place(p)) atomicOr(a.err, TTKV_ERR_BAD_POSITION);
+    }
     __syncthreads();
     if (!val && keep) {
+      const float2v* w = cs + t * half;
+      const bool refused = w[0][0] != w[0][0];
+      if (a.turn.adjacent) {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const int e = 8 * i + j;
-        if (e < 2 * half) {
-          const int at = a.turn.adjacent ? e >> 1 : e < half ? e : e - half;
-          const bool first = a.turn.adjacent ? !(e & 1) : e < half;
-          const int mate = a.turn.adjacent ? e ^ 1 : first ? e + half : e - half;
-          const float2v w = cs[t * half + at];
-          x[j] = first ? x[j] * w[0] - xs[t][mate] * w[1] : x[j] * w[0] + xs[t][mate] * w[1];
-        } else if (cs[t * half][0] != cs[t * half][0]) {
-          x[j] = NAN;  // (a refused position)
+        for (int j = 0; j < 8; j += 2)
+          if (8 * i + j < 2 * half) {
+            const float2v f = w[4 * i + j / 2];
+            const float u = x[j] * f[0] - x[j + 1] * f[1], v = x[j + 1] * f[0] + x[j] * f[1];
+            x[j] = u;
+            x[j + 1] = v;
+          }
+      } else if (whole) {
+        if (mated) {
+          const bool first = 8 * i < half;
+          const int j0 = first ? 8 * i : 8 * i - half;
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            const float2v f = w[j0 + j];
+            x[j] = first ? x[j] * f[0] - y[j] * f[1] : x[j] * f[0] + y[j] * f[1];
+          }
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const int e = 8 * i + j;
+          if (e < 2 * half) {
+            const bool first = e < half;
+            const float2v f = w[first ? e : e - half];
+            const float m = load_act(src, dt, at + (first ? e + half : e - half));
+            x[j] = first ? x[j] * f[0] - m * f[1] : x[j] * f[0] + m * f[1];
+          }
         }
       }
+      if (refused)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[j] = NAN;
     }
   }
   if (!keep) return;
@@ -89,10 +123,10 @@ __global__ __launch_bounds__(256) void octet_write_kernel(OctWriteArgs a) {
     x[j] = fminf(fmaxf(x[j], -kOctMax), kOctMax);
     top = fmaxf(top, fabsf(x[j]));
   }
-  for (int m = 1; m <= 2; m *= 2) {
-    odd += __shfl_xor(odd, m);
-    top = fmaxf(top, __shfl_xor(top, m));
-  }
+  odd += quad_xor<0>(odd);
+  odd += quad_xor<1>(odd);
+  top = fmaxf(top, quad_xor<0>(top));
+  top = fmaxf(top, quad_xor<1>(top));
   const bool bad = odd != odd;
   // 448 = 1.75 * 2^8: the exponent less 8, and one more where the mantissa is above 1.75
   const uint32_t e = ((__builtin_bit_cast(uint32_t, top) + 0x1fffffu) >> 23) - 8;
@@ -130,21 +164,24 @@ __global__ __launch_bounds__(256) void octet_write_kernel(OctWriteArgs a) {
   }
 }
 
-// A workgroup per token.
 __global__ __launch_bounds__(256) void rotary_scaled_kernel(TurnArgs a) {
-  __shared__ float2v cs[kTurnHalf];
-  turn_token(a, blockIdx.x, threadIdx.x, (int)blockDim.x, cs);
+  __shared__ __align__(16) float2v cs[kTurnHalf];
+  turn_block(a, blockIdx.x, threadIdx.x, cs);
 }
 
-// Whether rows go in pieces of 8 elements by a workgroup of `threads`: aligned, and pairs within them.
-static bool turn_pieces_apply(const TurnArgs& a, int threads) {
+// How rows go: in pieces of 8 elements where they are aligned and pairs lie in them, and then a wave per
+// token where there are many, four where there are few. Returns the workgroups.
+static int64_t turn_shape(TurnArgs& a) {
   const int64_t eb = a.dtype == TTKV_DTYPE_F32 ? 4 : 2;
-  if (a.d % 8 || a.half % (a.adjacent ? 4 : 8) || a.half / (a.adjacent ? 4 : 8) > threads) return false;
+  const int unit = a.adjacent ? 4 : 8;
+  bool pieces = a.d % (2 * unit) == 0 && a.half % unit == 0 && a.d / (2 * unit) <= 256;
   for (int i = 0; i < 2; ++i)
-    if (a.heads[i] && (((uintptr_t)a.x[i] | (uintptr_t)a.y[i]) % 16 || a.x_stride[i] * eb % 16 ||
-                       a.y_stride[i] * eb % 16))
-      return false;
-  return true;
+    if (a.heads[i])
+      pieces &= ((uintptr_t)a.x[i] | (uintptr_t)a.y[i]) % 16 == 0 && a.x_stride[i] * eb % 16 == 0 &&
+                a.y_stride[i] * eb % 16 == 0;
+  const bool waves = pieces && a.d / (2 * unit) <= 64 && 4 * a.half <= kTurnHalf && a.num_tokens >= 4 * device_cu_count();
+  a.pieces = !pieces ? kTurnElements : waves ? kTurnWaves : kTurnBlock;
+  return waves ? ((int64_t)a.num_tokens + 3) / 4 : a.num_tokens;
 }
 
 static bool act_dtype(int dt) {
@@ -182,12 +219,10 @@ int rotary_scaled(const void* q, const void* k, void* qo, void* ko, int dtype, i
       rows_meet(ko, ko_stride * eb, kw, q, q_stride * eb, qw, N) ||
       rows_meet(qo, qo_stride * eb, qw, ko, ko_stride * eb, kw, N))
     return host_fail(TTKV_E_INVALID, "one of query and key overlaps the other's output");
-  TurnArgs a{{q, k},  {qo, ko}, {HQ, H}, {q_stride, k_stride}, {qo_stride, ko_stride}, dtype, d,
-             rot / 2, adjacent != 0, 0, pos, turns,            amplitude,              err};
-  // a wave per token; four share the rows of a token where there are few
-  const int threads = N >= 4 * device_cu_count() ? 64 : 256;
-  a.pieces = turn_pieces_apply(a, threads);
-  hipLaunchKernelGGL(rotary_scaled_kernel, dim3(N), dim3(a.pieces ? threads : 256), 0, st, a);
+  TurnArgs a{{q, k}, {qo, ko}, {HQ, H}, {q_stride, k_stride}, {qo_stride, ko_stride}, dtype, d, rot / 2, adjacent != 0,
+             0,      N,        pos,     turns,                amplitude,              err};
+  const int64_t grid = turn_shape(a);
+  hipLaunchKernelGGL(rotary_scaled_kernel, dim3((unsigned)grid), dim3(256), 0, st, a);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess)
     return host_fail(TTKV_E_LAUNCH, std::string("scaled rotary launch: ") + hipGetErrorString(e));
@@ -204,6 +239,15 @@ int octet_check_page(int H, int d, const uint8_t* page, int64_t n_slots, int64_t
   if (n_slots <= 0 || n_slots % kOctTile)
     return host_fail(TTKV_E_INVALID, "the page must hold a positive multiple of 16 slots");
   return TTKV_OK;
+}
+
+template <int D>
+static void oct_write_launch(const OctWriteArgs& a, unsigned grid, int dt, hipStream_t st) {
+  auto kernel = dt == TTKV_DTYPE_F32    ? octet_write_kernel<D, TTKV_DTYPE_F32>
+                : dt == TTKV_DTYPE_F16  ? octet_write_kernel<D, TTKV_DTYPE_F16>
+                : dt == TTKV_DTYPE_BF16 ? octet_write_kernel<D, TTKV_DTYPE_BF16>
+                                        : octet_write_kernel<D, -1>;
+  hipLaunchKernelGGL(kernel, dim3(grid), dim3(256), 0, st, a);
 }
 
 int octet_write_paged(int H, int d, const void* key, int k_dtype, int64_t k_row_stride, const void* val,
@@ -236,15 +280,16 @@ int octet_write_paged(int H, int d, const void* key, int k_dtype, int64_t k_row_
       return host_fail(TTKV_E_INVALID, "query_out overlaps the keys or values");
   }
   const int64_t tokens = 1024 / d, blocks = (num_tokens + tokens - 1) / tokens * H;
-  const int64_t grid = blocks + (HQ ? num_tokens : 0);
-  if (grid > 0x7fffffff) return host_fail(TTKV_E_INVALID, "too many tokens for one call");
+  if (blocks > 0x3fffffff) return host_fail(TTKV_E_INVALID, "too many tokens for one call");
   OctWriteArgs a{key,  val,     k_dtype,     v_dtype,          k_row_stride,     v_row_stride, slots,      num_tokens, H,
                  page, n_slots, slot_stride, (uint16_t*)k_out, (uint16_t*)v_out, err,          (int)blocks};
-  a.turn = TurnArgs{{q, nullptr},  {qo, nullptr}, {HQ, 0},     {q_stride, 0}, {qo_stride, 0}, q_dtype, d, rot / 2,
-                    adjacent != 0, 0,             pos,         turns,         amplitude,       err};
-  a.turn.pieces = HQ && turn_pieces_apply(a.turn, 256);
-  auto kernel = d == 64 ? octet_write_kernel<64> : d == 128 ? octet_write_kernel<128> : octet_write_kernel<256>;
-  hipLaunchKernelGGL(kernel, dim3((unsigned)grid), dim3(256), 0, st, a);
+  a.turn = TurnArgs{{q, nullptr},  {qo, nullptr}, {HQ, 0}, {q_stride, 0}, {qo_stride, 0}, q_dtype, d, rot / 2,
+                    adjacent != 0, 0,             num_tokens, pos,        turns,          amplitude, err};
+  const int64_t grid = blocks + (HQ ? turn_shape(a.turn) : 0);
+  const int dt = k_dtype == v_dtype ? k_dtype : -1;
+  if (d == 64) oct_write_launch<64>(a, (unsigned)grid, dt, st);
+  else if (d == 128) oct_write_launch<128>(a, (unsigned)grid, dt, st);
+  else oct_write_launch<256>(a, (unsigned)grid, dt, st);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess)
     return host_fail(TTKV_E_LAUNCH, std::string("octet write launch: ") + hipGetErrorString(e));

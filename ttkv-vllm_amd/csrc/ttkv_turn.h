@@ -8,11 +8,14 @@
 // series of the sine and the cosine.
 #pragma once
 
+#include <type_traits>
+
 #include "ttkv_device.h"
 
 namespace ttkv {
 
 constexpr int kTurnHalf = 512;              // frequencies that the LDS holds
+constexpr int kTurnElements = 0, kTurnBlock = 1, kTurnWaves = 2;
 constexpr int64_t kTurnPositions = 1ll << 31;
 
 // Cosine and sine of t revolutions. Series up to x^10 and x^9 at |x| <= pi / 4: off by 5e-10 and 2e-9.
@@ -36,38 +39,48 @@ struct TurnArgs {
   int heads[2];
   int64_t x_stride[2], y_stride[2];
   int dtype, d, half, adjacent;
-  int pieces;  // rows go in pieces of 8 elements
+  int pieces;  // how rows go: an element at a time (0), in pieces of 8, by a workgroup or a wave per token
+  int num_tokens;
   const int64_t* pos;
   const double* turns;
   float amplitude;
   int32_t* err;
 };
 
-// Cosines and sines of token `tok` into cs[0 .. half), by the workgroup's threads; NaN where its
-// position is refused, which is returned. The caller synchronises before they are read.
-__device__ __forceinline__ bool turn_table(const int64_t* pos, const double* turns, int half, float amplitude,
-                                           int64_t tok, int tid, int threads, float2v* cs) {
-  const int64_t p = *gbl(pos + tok);
-  const bool ok = p >= 0 && p < kTurnPositions;
-  for (int j = tid; j < half; j += threads) {
-    float c, s;
-    turn_angle((double)p * *gbl(turns + j), c, s);
-    cs[j] = ok ? float2v{c * amplitude, s * amplitude} : float2v{NAN, NAN};
-  }
-  return ok;
+// Whether position p is taken.
+__device__ __forceinline__ bool turn_place(int64_t p) { return p >= 0 && p < kTurnPositions; }
+
+// Cosine and sine of frequency j at position p; NaN where that is refused.
+__device__ __forceinline__ float2v turn_at(const double* turns, int j, int64_t p, float amplitude) {
+  float c, s;
+  turn_angle((double)p * *gbl(turns + j), c, s);
+  return turn_place(p) ? float2v{c * amplitude, s * amplitude} : float2v{NAN, NAN};
 }
 
-// One token's rows by the threads of a workgroup, in pieces of 8 elements: rows whose pieces are 16-byte
-// aligned, pairs that lie in one piece or in two. A thread keeps its piece's frequencies from head to head;
-// kTurnBatch heads' loads are in flight at a time, the first ones asked for before the angles are formed.
+// What one thread of a team writes to LDS, the others read: a team of one wave, or the workgroup.
+template <bool WAVE>
+__device__ __forceinline__ void turn_sync() {
+  if constexpr (WAVE) {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+  } else {
+    __syncthreads();
+  }
+}
+
+// One token's rows in pieces of 8 elements: rows whose pieces are 16-byte aligned, pairs that lie in one
+// piece (adjacent) or in two. A thread keeps its piece's frequencies from head to head; kTurnBatch heads'
+// loads are in flight at a time, the first ones asked for before the angles are formed.
 constexpr int kTurnBatch = 4;
-template <int DT>
+template <int DT, bool ADJ, bool WAVE>
 __device__ __forceinline__ void turn_pieces(const TurnArgs& a, int64_t tok, int tid, int threads, float2v* cs) {
-  const bool adj = a.adjacent;
-  const int nch = adj ? a.half >> 2 : a.half >> 3;  // pieces (by halves: pairs of them) that are turned
-  const int slots = threads / nch, heads = a.heads[0] + a.heads[1];
-  const int slot = tid / nch, p = tid - slot * nch, mate = adj ? 0 : a.half;
-  const bool on = slot < slots;
+  constexpr int kFreqs = ADJ ? 4 : 8;  // of an item: a piece, or a pair of pieces
+  const int items = a.d / (ADJ ? 8 : 16), turned = a.half / kFreqs;
+  const int slots = threads / items, heads = a.heads[0] + a.heads[1];
+  const int slot = tid / items, p = tid - slot * items;
+  const bool copy = p >= turned;
+  const int e0 = ADJ ? 8 * p : copy ? 2 * a.half + 16 * (p - turned) : 8 * p, e1 = e0 + (copy ? 8 : a.half);
   auto place = [&](int head, bool out, int64_t& at) -> const void* {
     const int set = head >= a.heads[0];
     at = tok * (out ? a.y_stride : a.x_stride)[set] + (int64_t)(set ? head - a.heads[0] : head) * a.d;
@@ -78,22 +91,24 @@ __device__ __forceinline__ void turn_pieces(const TurnArgs& a, int64_t tok, int 
 #pragma unroll
     for (int b = 0; b < kTurnBatch; ++b) {
       const int head = h0 + b * slots + slot;
-      if (on && head < heads) {
+      if (slot < slots && head < heads) {
         int64_t at;
         const void* src = place(head, false, at);
-        x[b] = load_act8<DT>(src, at + 8 * p);
-        if (!adj) y[b] = load_act8<DT>(src, at + 8 * p + mate);
+        x[b] = load_act8<DT>(src, at + e0);
+        if (!ADJ) y[b] = load_act8<DT>(src, at + e1);
       }
     }
   };
   fetch(0);
-  const bool ok = turn_table(a.pos, a.turns, a.half, a.amplitude, tok, tid, threads, cs);
+  const int64_t pos = *gbl(a.pos + tok);
+  const bool ok = turn_place(pos);
+  for (int j = tid; j < a.half; j += threads) cs[j] = turn_at(a.turns, j, pos, a.amplitude);
   if (!ok && tid == 0) atomicOr(a.err, TTKV_ERR_BAD_POSITION);
-  __syncthreads();
-  float c[8], s[8];  // (adjacent pairs: four)
+  turn_sync<WAVE>();
+  float c[kFreqs], s[kFreqs];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const float2v w = cs[adj ? 4 * p + (i & 3) : on ? 8 * p + i : 0];
+  for (int i = 0; i < kFreqs; ++i) {
+    const float2v w = cs[copy || slot >= slots ? 0 : kFreqs * p + i];
     c[i] = w[0];
     s[i] = w[1];
   }
@@ -101,55 +116,46 @@ __device__ __forceinline__ void turn_pieces(const TurnArgs& a, int64_t tok, int 
 #pragma unroll
     for (int b = 0; b < kTurnBatch; ++b) {
       const int head = h0 + b * slots + slot;
-      if (on && head < heads) {
+      if (slot < slots && head < heads) {
         int64_t at;
         void* dst = const_cast<void*>(place(head, true, at));
         float u[8], v[8];
-        if (adj) {
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const float xi = act8_get<DT>(x[b], 2 * i), yi = act8_get<DT>(x[b], 2 * i + 1);
-            u[2 * i] = xi * c[i] - yi * s[i];
-            u[2 * i + 1] = yi * c[i] + xi * s[i];
+        for (int i = 0; i < 8; ++i) {
+          const float xi = act8_get<DT>(x[b], i), yi = ADJ ? act8_get<DT>(x[b], i ^ 1) : act8_get<DT>(y[b], i);
+          const float ci = c[ADJ ? i / 2 : i], si = s[ADJ ? i / 2 : i];
+          u[i] = ADJ && (i & 1) ? xi * ci + yi * si : xi * ci - yi * si;
+          v[i] = yi * ci + xi * si;
+          if (copy) {
+            u[i] = ok ? xi : NAN;
+            v[i] = ok ? yi : NAN;
           }
-        } else {
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const float xi = act8_get<DT>(x[b], i), yi = act8_get<DT>(y[b], i);
-            u[i] = xi * c[i] - yi * s[i];
-            v[i] = yi * c[i] + xi * s[i];
-          }
-          store_act8<DT>(dst, at + 8 * p + mate, v);
         }
-        store_act8<DT>(dst, at + 8 * p, u);
+        store_act8<DT>(dst, at + e0, u);
+        if (!ADJ) store_act8<DT>(dst, at + e1, v);
       }
     }
     fetch(h0 + kTurnBatch * slots);
   }
-  const int rest = (a.d - 2 * a.half) >> 3;  // pieces that are copied
-  for (int i = tid; i < heads * rest; i += threads) {
-    const int head = i / rest, x0 = 2 * a.half + (i - head * rest) * 8;
-    int64_t from, to;
-    const void* src = place(head, false, from);
-    void* dst = const_cast<void*>(place(head, true, to));
-    if (dst == src && from == to && ok) continue;  // in place
-    const Act8<DT> z = load_act8<DT>(src, from + x0);
-    float v[8];
-#pragma unroll
-    for (int k = 0; k < 8; ++k) v[k] = ok ? act8_get<DT>(z, k) : NAN;
-    store_act8<DT>(dst, to + x0, v);
-  }
 }
 
-// One token's rows, in pieces or an element or a pair per thread.
-__device__ __forceinline__ void turn_token(const TurnArgs& a, int64_t tok, int tid, int threads, float2v* cs) {
-  if (a.pieces) {
-    if (a.dtype == TTKV_DTYPE_BF16) turn_pieces<TTKV_DTYPE_BF16>(a, tok, tid, threads, cs);
-    else if (a.dtype == TTKV_DTYPE_F16) turn_pieces<TTKV_DTYPE_F16>(a, tok, tid, threads, cs);
-    else turn_pieces<TTKV_DTYPE_F32>(a, tok, tid, threads, cs);
-    return;
-  }
-  const bool ok = turn_table(a.pos, a.turns, a.half, a.amplitude, tok, tid, threads, cs);
+template <bool WAVE>
+__device__ __forceinline__ void turn_pieces(const TurnArgs& a, int64_t tok, int tid, int threads, float2v* cs) {
+  auto run = [&](auto dt) {
+    constexpr int DT = decltype(dt)::value;
+    if (a.adjacent) turn_pieces<DT, true, WAVE>(a, tok, tid, threads, cs);
+    else turn_pieces<DT, false, WAVE>(a, tok, tid, threads, cs);
+  };
+  if (a.dtype == TTKV_DTYPE_BF16) run(std::integral_constant<int, TTKV_DTYPE_BF16>{});
+  else if (a.dtype == TTKV_DTYPE_F16) run(std::integral_constant<int, TTKV_DTYPE_F16>{});
+  else run(std::integral_constant<int, TTKV_DTYPE_F32>{});
+}
+
+// One token's rows, an element or a pair per thread of the workgroup.
+__device__ __forceinline__ void turn_elements(const TurnArgs& a, int64_t tok, int tid, int threads, float2v* cs) {
+  const int64_t pos = *gbl(a.pos + tok);
+  const bool ok = turn_place(pos);
+  for (int j = tid; j < a.half; j += threads) cs[j] = turn_at(a.turns, j, pos, a.amplitude);
   if (!ok && tid == 0) atomicOr(a.err, TTKV_ERR_BAD_POSITION);
   __syncthreads();
   const int per = a.d - a.half;  // pairs, then the dims that are copied
@@ -167,6 +173,19 @@ __device__ __forceinline__ void turn_token(const TurnArgs& a, int64_t tok, int t
     const float c = cs[j][0], s = cs[j][1];
     store_act(a.y[set], a.dtype, to + u, x * c - y * s);
     store_act(a.y[set], a.dtype, to + v, y * c + x * s);
+  }
+}
+
+// The workgroups' tokens: `block`-th workgroup of 256 threads.
+__device__ __forceinline__ void turn_block(const TurnArgs& a, int64_t block, int tid, float2v* cs) {
+  if (a.pieces == kTurnWaves) {  // a wave per token
+    const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int64_t tok = 4 * block + w;
+    if (tok < a.num_tokens) turn_pieces<true>(a, tok, tid & 63, 64, cs + w * a.half);
+  } else if (a.pieces) {
+    turn_pieces<false>(a, block, tid, 256, cs);
+  } else {
+    turn_elements(a, block, tid, 256, cs);
   }
 }
 
