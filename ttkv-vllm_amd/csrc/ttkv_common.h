@@ -296,13 +296,13 @@ template <int DT>
 struct Act8 {
   u32x4 raw[DT == TTKV_DTYPE_F32 ? 2 : 1];
 };
-template <int DT>
+template <int DT, bool STREAM = true>  // STREAM: not kept in the caches
 __device__ __forceinline__ Act8<DT> load_act8(const void* p, int64_t i) {
   Act8<DT> x;
   const char* at = (const char*)p + i * (DT == TTKV_DTYPE_F32 ? 4 : 2);
 #pragma unroll
   for (int j = 0; j < (DT == TTKV_DTYPE_F32 ? 2 : 1); ++j)
-    x.raw[j] = __builtin_nontemporal_load(gbl((const u32x4*)at + j));
+    x.raw[j] = STREAM ? __builtin_nontemporal_load(gbl((const u32x4*)at + j)) : *gbl((const u32x4*)at + j);
   return x;
 }
 template <int DT>

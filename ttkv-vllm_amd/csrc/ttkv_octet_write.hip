@@ -36,14 +36,14 @@ __device__ __forceinline__ float quad_xor(float v) {
 }
 
 // DT: the type of keys and values, or -1 where they differ (then by the arguments).
-template <int D, int DT>
+template <int D, int DT, bool TURN>
 __global__ __launch_bounds__(256) void octet_write_kernel(OctWriteArgs a) {
   using F = Oct<D>;
   constexpr int kTokens = 1024 / D, kLanes = D / 8;
-  __shared__ __align__(16) float2v cs[kTurnHalf];
+  __shared__ __align__(16) float2v cs[TURN ? kTurnHalf : 1];
   const int tid = threadIdx.x;
-  if ((int)blockIdx.x >= a.write_blocks) {
-    turn_block(a.turn, (int)blockIdx.x - a.write_blocks, tid, cs);
+  if (TURN && (int)blockIdx.x >= a.write_blocks) {
+    turn_token<false>(a.turn, (int)blockIdx.x - a.write_blocks, tid, 256, cs);
     return;
   }
   const int row = tid / kLanes, i = tid % kLanes, t = row % kTokens;  // dims 8 i .. 8 i + 7
@@ -55,7 +55,7 @@ __global__ __launch_bounds__(256) void octet_write_kernel(OctWriteArgs a) {
   const int dt = DT >= 0 ? DT : val ? a.v_dtype : a.k_dtype;
   const int64_t stride = val ? a.v_row_stride : a.k_row_stride, at = tok * stride + (int64_t)h * D;
   const bool vec = act_rows_aligned(src, dt, stride);
-  const int half = a.turn.half;
+  const int half = TURN ? a.turn.half : 0;
   // a lane's dims and the others of their pairs, in a piece of 8 where the halves are made of such
   const bool whole = a.turn.adjacent || half % 8 == 0, mated = !val && !a.turn.adjacent && whole && 8 * i < 2 * half;
   const int mate = 8 * i < half ? 8 * i + half : 8 * i - half;
@@ -67,7 +67,7 @@ __global__ __launch_bounds__(256) void octet_write_kernel(OctWriteArgs a) {
   const int64_t slot = on ? *gbl(a.slots + tok) : -1;  // negative: a padded token
   if (slot >= a.n_slots && !val && i == 0) atomicOr(a.err, TTKV_ERR_BAD_SLOT);
   const bool keep = slot >= 0 && slot < a.n_slots;
-  if (half) {
+  if constexpr (TURN) {
     for (int e = tid; e < kTokens * half; e += 256) {  // (kTokens * half <= 512)
       const int n = e / half, j = e - n * half;
       if (tok0 + n >= a.num_tokens) break;
@@ -164,14 +164,19 @@ __global__ __launch_bounds__(256) void octet_write_kernel(OctWriteArgs a) {
   }
 }
 
+// A workgroup per token.
+template <bool STREAM>
 __global__ __launch_bounds__(256) void rotary_scaled_kernel(TurnArgs a) {
   __shared__ __align__(16) float2v cs[kTurnHalf];
-  turn_block(a, blockIdx.x, threadIdx.x, cs);
+  turn_token<STREAM>(a, blockIdx.x, threadIdx.x, 256, cs);
 }
 
-// How rows go: in pieces of 8 elements where they are aligned and pairs lie in them, and then a wave per
-// token where there are many, four where there are few. Returns the workgroups.
-static int64_t turn_shape(TurnArgs& a) {
+// Rows that are read and written past this go by loads that do not stay in the caches (bf16, 40 heads of
+// 128: 8,192 tokens, 168 MB, 36.0 us so and 37.5 with loads that stay; 4,096 tokens, 84 MB, 21.3 and 17.9).
+constexpr int64_t kTurnStream = 128 << 20;
+
+// Whether rows go in pieces of 8 elements: aligned, and pairs that lie in one or two of them.
+static bool turn_pieces_apply(const TurnArgs& a) {
   const int64_t eb = a.dtype == TTKV_DTYPE_F32 ? 4 : 2;
   const int unit = a.adjacent ? 4 : 8;
   bool pieces = a.d % (2 * unit) == 0 && a.half % unit == 0 && a.d / (2 * unit) <= 256;
@@ -179,9 +184,7 @@ static int64_t turn_shape(TurnArgs& a) {
     if (a.heads[i])
       pieces &= ((uintptr_t)a.x[i] | (uintptr_t)a.y[i]) % 16 == 0 && a.x_stride[i] * eb % 16 == 0 &&
                 a.y_stride[i] * eb % 16 == 0;
-  const bool waves = pieces && a.d / (2 * unit) <= 64 && 4 * a.half <= kTurnHalf && a.num_tokens >= 4 * device_cu_count();
-  a.pieces = !pieces ? kTurnElements : waves ? kTurnWaves : kTurnBlock;
-  return waves ? ((int64_t)a.num_tokens + 3) / 4 : a.num_tokens;
+  return pieces;
 }
 
 static bool act_dtype(int dt) {
@@ -220,9 +223,10 @@ int rotary_scaled(const void* q, const void* k, void* qo, void* ko, int dtype, i
       rows_meet(qo, qo_stride * eb, qw, ko, ko_stride * eb, kw, N))
     return host_fail(TTKV_E_INVALID, "one of query and key overlaps the other's output");
   TurnArgs a{{q, k}, {qo, ko}, {HQ, H}, {q_stride, k_stride}, {qo_stride, ko_stride}, dtype, d, rot / 2, adjacent != 0,
-             0,      N,        pos,     turns,                amplitude,              err};
-  const int64_t grid = turn_shape(a);
-  hipLaunchKernelGGL(rotary_scaled_kernel, dim3((unsigned)grid), dim3(256), 0, st, a);
+             0,      pos,      turns,   amplitude,            err};
+  a.pieces = turn_pieces_apply(a);
+  auto kernel = 2 * (qw + kw) * N > kTurnStream ? rotary_scaled_kernel<true> : rotary_scaled_kernel<false>;
+  hipLaunchKernelGGL(kernel, dim3(N), dim3(256), 0, st, a);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess)
     return host_fail(TTKV_E_LAUNCH, std::string("scaled rotary launch: ") + hipGetErrorString(e));
@@ -241,13 +245,18 @@ int octet_check_page(int H, int d, const uint8_t* page, int64_t n_slots, int64_t
   return TTKV_OK;
 }
 
+template <int D, bool TURN>
+static void oct_write_launch(const OctWriteArgs& a, unsigned grid, int dt, hipStream_t st) {
+  auto kernel = dt == TTKV_DTYPE_F32    ? octet_write_kernel<D, TTKV_DTYPE_F32, TURN>
+                : dt == TTKV_DTYPE_F16  ? octet_write_kernel<D, TTKV_DTYPE_F16, TURN>
+                : dt == TTKV_DTYPE_BF16 ? octet_write_kernel<D, TTKV_DTYPE_BF16, TURN>
+                                        : octet_write_kernel<D, -1, TURN>;
+  hipLaunchKernelGGL(kernel, dim3(grid), dim3(256), 0, st, a);
+}
 template <int D>
 static void oct_write_launch(const OctWriteArgs& a, unsigned grid, int dt, hipStream_t st) {
-  auto kernel = dt == TTKV_DTYPE_F32    ? octet_write_kernel<D, TTKV_DTYPE_F32>
-                : dt == TTKV_DTYPE_F16  ? octet_write_kernel<D, TTKV_DTYPE_F16>
-                : dt == TTKV_DTYPE_BF16 ? octet_write_kernel<D, TTKV_DTYPE_BF16>
-                                        : octet_write_kernel<D, -1>;
-  hipLaunchKernelGGL(kernel, dim3(grid), dim3(256), 0, st, a);
+  if (a.turn.half) oct_write_launch<D, true>(a, grid, dt, st);
+  else oct_write_launch<D, false>(a, grid, dt, st);
 }
 
 int octet_write_paged(int H, int d, const void* key, int k_dtype, int64_t k_row_stride, const void* val,
@@ -284,8 +293,9 @@ int octet_write_paged(int H, int d, const void* key, int k_dtype, int64_t k_row_
   OctWriteArgs a{key,  val,     k_dtype,     v_dtype,          k_row_stride,     v_row_stride, slots,      num_tokens, H,
                  page, n_slots, slot_stride, (uint16_t*)k_out, (uint16_t*)v_out, err,          (int)blocks};
   a.turn = TurnArgs{{q, nullptr},  {qo, nullptr}, {HQ, 0}, {q_stride, 0}, {qo_stride, 0}, q_dtype, d, rot / 2,
-                    adjacent != 0, 0,             num_tokens, pos,        turns,          amplitude, err};
-  const int64_t grid = blocks + (HQ ? turn_shape(a.turn) : 0);
+                    adjacent != 0, 0,             pos,     turns,         amplitude,      err};
+  a.turn.pieces = HQ && turn_pieces_apply(a.turn);
+  const int64_t grid = blocks + (HQ ? num_tokens : 0);  // those of the queries: a token each
   const int dt = k_dtype == v_dtype ? k_dtype : -1;
   if (d == 64) oct_write_launch<64>(a, (unsigned)grid, dt, st);
   else if (d == 128) oct_write_launch<128>(a, (unsigned)grid, dt, st);

@@ -15,7 +15,6 @@
 namespace ttkv {
 
 constexpr int kTurnHalf = 512;              // frequencies that the LDS holds
-constexpr int kTurnElements = 0, kTurnBlock = 1, kTurnWaves = 2;
 constexpr int64_t kTurnPositions = 1ll << 31;
 
 // Cosine and sine of t revolutions. Series up to x^10 and x^9 at |x| <= pi / 4: off by 5e-10 and 2e-9.
@@ -39,8 +38,7 @@ struct TurnArgs {
   int heads[2];
   int64_t x_stride[2], y_stride[2];
   int dtype, d, half, adjacent;
-  int pieces;  // how rows go: an element at a time (0), in pieces of 8, by a workgroup or a wave per token
-  int num_tokens;
+  int pieces;  // rows go in pieces of 8 elements
   const int64_t* pos;
   const double* turns;
   float amplitude;
@@ -57,23 +55,14 @@ __device__ __forceinline__ float2v turn_at(const double* turns, int j, int64_t p
   return turn_place(p) ? float2v{c * amplitude, s * amplitude} : float2v{NAN, NAN};
 }
 
-// What one thread of a team writes to LDS, the others read: a team of one wave, or the workgroup.
-template <bool WAVE>
-__device__ __forceinline__ void turn_sync() {
-  if constexpr (WAVE) {
-    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-  } else {
-    __syncthreads();
-  }
-}
-
 // One token's rows in pieces of 8 elements: rows whose pieces are 16-byte aligned, pairs that lie in one
 // piece (adjacent) or in two. A thread keeps its piece's frequencies from head to head; kTurnBatch heads'
-// loads are in flight at a time, the first ones asked for before the angles are formed.
-constexpr int kTurnBatch = 4;
-template <int DT, bool ADJ, bool WAVE>
+// loads are in flight at a time, the first ones asked for before the angles are formed. Two of them (four:
+// 8,192 tokens of 40 heads 38.1 us, 36.0 with two, whose fewer registers hold more tokens on a CU), and a
+// workgroup of four waves per token at every size (a wave per token: 38.1, 512 tokens 9.1 against 4.9 us).
+// STREAM: loads that do not stay in the caches, for rows of more bytes than those hold (kTurnStream).
+constexpr int kTurnBatch = 2;
+template <int DT, bool ADJ, bool STREAM>
 __device__ __forceinline__ void turn_pieces(const TurnArgs& a, int64_t tok, int tid, int threads, float2v* cs) {
   constexpr int kFreqs = ADJ ? 4 : 8;  // of an item: a piece, or a pair of pieces
   const int items = a.d / (ADJ ? 8 : 16), turned = a.half / kFreqs;
@@ -94,8 +83,8 @@ __device__ __forceinline__ void turn_pieces(const TurnArgs& a, int64_t tok, int 
       if (slot < slots && head < heads) {
         int64_t at;
         const void* src = place(head, false, at);
-        x[b] = load_act8<DT>(src, at + e0);
-        if (!ADJ) y[b] = load_act8<DT>(src, at + e1);
+        x[b] = load_act8<DT, STREAM>(src, at + e0);
+        if (!ADJ) y[b] = load_act8<DT, STREAM>(src, at + e1);
       }
     }
   };
@@ -104,7 +93,7 @@ __device__ __forceinline__ void turn_pieces(const TurnArgs& a, int64_t tok, int 
   const bool ok = turn_place(pos);
   for (int j = tid; j < a.half; j += threads) cs[j] = turn_at(a.turns, j, pos, a.amplitude);
   if (!ok && tid == 0) atomicOr(a.err, TTKV_ERR_BAD_POSITION);
-  turn_sync<WAVE>();
+  __syncthreads();
   float c[kFreqs], s[kFreqs];
 #pragma unroll
   for (int i = 0; i < kFreqs; ++i) {
@@ -139,12 +128,12 @@ __device__ __forceinline__ void turn_pieces(const TurnArgs& a, int64_t tok, int 
   }
 }
 
-template <bool WAVE>
+template <bool STREAM>
 __device__ __forceinline__ void turn_pieces(const TurnArgs& a, int64_t tok, int tid, int threads, float2v* cs) {
   auto run = [&](auto dt) {
     constexpr int DT = decltype(dt)::value;
-    if (a.adjacent) turn_pieces<DT, true, WAVE>(a, tok, tid, threads, cs);
-    else turn_pieces<DT, false, WAVE>(a, tok, tid, threads, cs);
+    if (a.adjacent) turn_pieces<DT, true, STREAM>(a, tok, tid, threads, cs);
+    else turn_pieces<DT, false, STREAM>(a, tok, tid, threads, cs);
   };
   if (a.dtype == TTKV_DTYPE_BF16) run(std::integral_constant<int, TTKV_DTYPE_BF16>{});
   else if (a.dtype == TTKV_DTYPE_F16) run(std::integral_constant<int, TTKV_DTYPE_F16>{});
@@ -176,17 +165,11 @@ __device__ __forceinline__ void turn_elements(const TurnArgs& a, int64_t tok, in
   }
 }
 
-// The workgroups' tokens: `block`-th workgroup of 256 threads.
-__device__ __forceinline__ void turn_block(const TurnArgs& a, int64_t block, int tid, float2v* cs) {
-  if (a.pieces == kTurnWaves) {  // a wave per token
-    const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int64_t tok = 4 * block + w;
-    if (tok < a.num_tokens) turn_pieces<true>(a, tok, tid & 63, 64, cs + w * a.half);
-  } else if (a.pieces) {
-    turn_pieces<false>(a, block, tid, 256, cs);
-  } else {
-    turn_elements(a, block, tid, 256, cs);
-  }
+// A token's rows by a workgroup.
+template <bool STREAM>
+__device__ __forceinline__ void turn_token(const TurnArgs& a, int64_t tok, int tid, int threads, float2v* cs) {
+  if (a.pieces) turn_pieces<STREAM>(a, tok, tid, threads, cs);
+  else turn_elements(a, tok, tid, threads, cs);
 }
 
 }  // namespace ttkv
