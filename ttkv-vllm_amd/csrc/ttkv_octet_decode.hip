@@ -30,13 +30,15 @@
 namespace ttkv {
 
 constexpr int kODMaxQ = 16;  // queries per request
-constexpr int kODThreads = 256;
-constexpr int kODWaves = 4;
 constexpr int kODStep = 2 * kOctTile;  // tokens per wave step
 constexpr int kODPlanLanes = 4;        // requests per lane in the plan: 256 per launch
+constexpr int kODClasses = 8;          // of chunk lengths, for the items' order
 constexpr int kODRows = 16;            // rows of a block: a matrix product's columns
 constexpr float kODNone = -3.402823466e38f;  // the maximum before the first visible key
 constexpr float kODMost = 0x1p10f;     // a lane's sum of eight weights before the maximum moves
+// What a chunk's join costs per row and dim against a step (1 x 14,000 tokens: 16.4 us with 6e-4, 14.1 so; 1 x
+// 60,000 of one KV head of eight query heads 70 without it, 19.4 so).
+constexpr float kODJoin = 9e-4f;
 constexpr float kLog2e = 1.4426950408889634f;
 
 struct OctDecodeArgs {
@@ -61,11 +63,15 @@ struct OctDecodeArgs {
   int64_t out_row_stride;
   float* lse;
   int* ws_cnt;
+  int cnt_stride;    // between counters: cache lines of their own where there is room (atomics on one line wait
+                     // for each other: 1 x 14,000 tokens 14.2 us side by side, 12.5 so)
   float* ws_o;       // [split items][part_rows][D]
   float* ws_ml;      // [split items][part_rows][2]
   uint32_t o_bytes;  // size of ws_o
   int part_rows;     // rows of an item's partials
-  int target;
+  float by_target;       // 1 / the items that the plan aims at
+  int resident;          // what the chip holds at once
+  float join;            // what a chunk's join costs against a step
   int32_t* err;
 };
 
@@ -78,10 +84,18 @@ struct OctPlan {
   bool none;
 };
 
-__device__ __forceinline__ OctPlan od_plan(const OctDecodeArgs& a, int item) {
+// x / d for 0 <= x < 2^24 and by = 1 / d to an ulp.
+__device__ __forceinline__ int od_div(int x, int d, float by) {
+  int k = (int)((float)x * by);
+  k -= k * d > x;
+  return k + ((k + 1) * d <= x);
+}
+
+template <int W>  // waves of a workgroup
+__device__ __forceinline__ OctPlan od_plan(const OctDecodeArgs& a) {
   const int lane = threadIdx.x & 63;
   int n[kODPlanLanes], q0[kODPlanLanes], Q[kODPlanLanes], s0[kODPlanLanes], st[kODPlanLanes], rb[kODPlanLanes];
-  int total = 0;
+  int total = 0, longest = 0, whole = 0;
 #pragma unroll
   for (int i = 0; i < kODPlanLanes; ++i) {
     n[i] = q0[i] = Q[i] = 0;
@@ -93,49 +107,105 @@ __device__ __forceinline__ OctPlan od_plan(const OctDecodeArgs& a, int item) {
   }
 #pragma unroll
   for (int i = 0; i < kODPlanLanes; ++i) {
+    s0[i] = st[i] = rb[i] = 0;
+    if (64 * i >= a.num_reqs) continue;
     const int nn = min(max(n[i], 0), a.max_seq), qq = min(max(Q[i], 0), a.max_q), p0 = nn - Q[i];
     s0[i] = a.window && p0 >= a.window ? (p0 - a.window + 1) / kODStep : 0;
     st[i] = p0 >= 0 && qq > 0 ? (p0 + qq - 1) / kODStep + 1 - s0[i] : 0;
     rb[i] = (qq * a.G + kODRows - 1) / kODRows;
     total += st[i] * rb[i];
+    longest = max(longest, st[i]);
+    whole += rb[i];
   }
-  // (a lane has less than 2^28 of them)
-  const int64_t all = ((int64_t)wave_sum_i(total >> 12) * 4096 + wave_sum_i(total & 4095)) * a.H;
-  // whole rounds of the four waves
-  const int per = all < 0x40000000 ? (int)(((uint32_t)all + a.target - 1) / a.target)
-                                   : (int)fminf((float)all / (float)a.target * 1.00001f, 1e8f) + 1;
-  const int C = max(1, (per + kODWaves - 1) / kODWaves) * kODWaves;
+  // (a lane has less than 2^28 steps, and its sums below fp32's 2^24 are whole)
+  float all = (float)wave_sum_i(total & 4095);
+  if (__builtin_amdgcn_ballot_w64(total >> 12)) all += 4096.f * (float)wave_sum_i(total >> 12);
+  whole = wave_sum_i(whole);
+  // whole rounds of the four waves. (Never shorter than the batch's share: the grid and the workspace are
+  // made for that; fp32 is off by less than the factor.)
+  all *= (float)a.H * 1.000001f;
+  int C = (max(1, (int)ceilf(all * a.by_target)) + W - 1) / W * W;
+  // A step costs its chunk's wave about a, a chunk its join about b per row and dim: the two together are
+  // least at sqrt(4 steps b / a) steps.
+  C = max(C, (int)(sqrtf((float)wave_max_i(longest) * a.join) / W + 0.5f) * W);
+  // Never more than steps / C rounded up; and two rounds of the waves longer rather than a chunk more, whose
+  // hand-over costs as much (24 x 256 keys: 10.2 us with it, 7.0 so; 1 x 300 7.6, 6.8; 61 of 70 to 2,900 39.2, 36.6).
+  float by_C;
+  auto length = [&](int c) {
+    C = c;
+    by_C = __builtin_amdgcn_rcpf((float)c) * 0.9999995f;
+  };
+  auto chunks = [&](int steps) { return max(1, (int)((float)(steps + C - 1 - 2 * W) * by_C)); };
+  length(C);
+  // Longer chunks rather than a second round of workgroups, where the batch has not more blocks anyway (6 x 5
+  // queries, d = 256: 45.2 us, 32.1 so). There are at most `whole` chunks more than the steps have lengths of C.
+  if (whole * a.H <= a.resident && (float)(whole * a.H) + all * by_C * 1.000001f > (float)a.resident) {
+    while (true) {
+      int items = 0;
+#pragma unroll
+      for (int i = 0; i < kODPlanLanes; ++i)
+        if (64 * i < a.num_reqs) items += rb[i] * chunks(st[i]);
+      if (wave_sum_i(items) * a.H <= a.resident) break;
+      length(C + max(1, C / (16 * W)) * W);
+    }
+  }
   OctPlan P{};
-  P.h = item % a.H;
+  P.h = blockIdx.x;
   P.none = true;
-  const int it = item / a.H;
-  int carry = 0, blocks = 0, parts = 0;
+  const int it = blockIdx.y;
+  // Long chunks first, so that a compute unit's workgroups are not all long (64 of 100 to 3,000 keys: 46.2 us in
+  // the batch's order, 43.6 so): classes by the chunk's eighth of C, in the batch's order within each. Not where
+  // chunks are short or requests many, whose scans cost more (200 of 50 to 600: 34.3, 40.5).
+  const int classes = a.num_reqs > 64 || C <= 8 ? 1 : kODClasses;
+  int nch[kODPlanLanes], cls[kODPlanLanes];
 #pragma unroll
   for (int i = 0; i < kODPlanLanes; ++i) {
-    if (64 * i >= a.num_reqs || !P.none) break;
-    const int nch = max(1, (st[i] + C - 1) / C), items = rb[i] * nch, split = nch > 1 ? items : 0;
-    const int incl = nib_scan(items), bincl = nib_scan(rb[i]), pincl = nib_scan(split);
-    const int ex = carry + incl - items;
-    const uint64_t hit = __builtin_amdgcn_ballot_w64(ex <= it && it < ex + items);
-    if (hit) {
-      const int ln = __builtin_ctzll(hit);
-      P.none = false;
-      P.r = 64 * i + ln;
-      P.n = __builtin_amdgcn_readlane(n[i], ln);
-      P.Q = __builtin_amdgcn_readlane(Q[i], ln);
-      P.q0 = __builtin_amdgcn_readlane(q0[i], ln);
-      P.s0 = __builtin_amdgcn_readlane(s0[i], ln);
-      P.steps = __builtin_amdgcn_readlane(st[i], ln);
-      P.nch = __builtin_amdgcn_readlane(nch, ln);
-      const int local = it - __builtin_amdgcn_readlane(ex, ln);
-      P.rb = local / P.nch;
-      P.c = local - P.rb * P.nch;
-      P.part = __builtin_amdgcn_readlane(parts + pincl - split, ln) + P.rb * P.nch;
-      P.block = __builtin_amdgcn_readlane(blocks + bincl - rb[i], ln) + P.rb;
+    nch[i] = cls[i] = 0;
+    if (64 * i >= a.num_reqs) continue;
+    nch[i] = chunks(st[i]);
+    if (classes > 1) {
+      const float eighths = (float)st[i] * __builtin_amdgcn_rcpf((float)nch[i]) * by_C * kODClasses;
+      cls[i] = kODClasses - 1 - min(kODClasses - 1, (int)eighths);
     }
-    carry += __builtin_amdgcn_readlane(incl, 63);
-    blocks += __builtin_amdgcn_readlane(bincl, 63);
-    parts += __builtin_amdgcn_readlane(pincl, 63);
+  }
+  int carry = 0, ln = 0;
+  for (int k = 0; k < classes && P.none; ++k) {
+#pragma unroll
+    for (int i = 0; i < kODPlanLanes; ++i) {
+      if (64 * i >= a.num_reqs) break;
+      const int items = cls[i] == k ? rb[i] * nch[i] : 0;
+      if (!__builtin_amdgcn_ballot_w64(items > 0)) continue;
+      const int incl = nib_scan(items), ex = carry + incl - items;
+      const uint64_t hit = __builtin_amdgcn_ballot_w64(ex <= it && it < ex + items);
+      if (hit) {
+        ln = __builtin_ctzll(hit);
+        P.none = false;
+        P.r = 64 * i + ln;
+        P.n = __builtin_amdgcn_readlane(n[i], ln);
+        P.Q = __builtin_amdgcn_readlane(Q[i], ln);
+        P.q0 = __builtin_amdgcn_readlane(q0[i], ln);
+        P.s0 = __builtin_amdgcn_readlane(s0[i], ln);
+        P.steps = __builtin_amdgcn_readlane(st[i], ln);
+        P.nch = __builtin_amdgcn_readlane(nch[i], ln);
+        const int local = it - __builtin_amdgcn_readlane(ex, ln);
+        P.rb = od_div(local, P.nch, __builtin_amdgcn_rcpf((float)P.nch));
+        P.c = local - P.rb * P.nch;
+        break;
+      }
+      carry += __builtin_amdgcn_readlane(incl, 63);
+    }
+  }
+  // the blocks, and the split ones' items, of the requests before
+  if (P.nch > 1) {
+    int blocks = 0, parts = 0;
+#pragma unroll
+    for (int i = 0; i < kODPlanLanes; ++i)
+      if (64 * i + lane < P.r) {
+        blocks += rb[i];
+        parts += nch[i] > 1 ? rb[i] * nch[i] : 0;
+      }
+    P.block = wave_sum_i(blocks) + P.rb;
+    P.part = wave_sum_i(parts) + P.rb * P.nch;
   }
   return P;
 }
@@ -156,18 +226,19 @@ __device__ __forceinline__ uint32_t od_high(bf16x2 a, bf16x2 b) {
   return __builtin_amdgcn_perm(__builtin_bit_cast(uint32_t, b), __builtin_bit_cast(uint32_t, a), 0x07060302u);
 }
 
-template <int D, int QDT, bool CHUNK>
-__global__ __launch_bounds__(kODThreads, D == 256 ? 1 : 2) void octet_decode_kernel(OctDecodeArgs a) {
+template <int D, int W, int QDT, bool CHUNK>
+__global__ __launch_bounds__(64 * W, W > 4 ? W / 4 : D == 256 ? 1 : D == 128 ? 2 : 4) void octet_decode_kernel(OctDecodeArgs a) {
   using F = Oct<D>;
   constexpr int N = F::kDims, KS = D / 32, PIECES = D / 64, PARTS = QDT == TTKV_DTYPE_F16 ? 2 : 1;
+  constexpr int kThreads = 64 * W;
   constexpr int RS = D + 4;  // floats of a row in LDS: the rows' columns start in different banks
   extern __shared__ __align__(16) float red_all[];  // [waves][rows][RS]: the waves' results, then the join's
   float(*red_o)[kODRows][RS] = (float(*)[kODRows][RS])red_all;
-  __shared__ float red_m[kODWaves][kODRows], red_l[kODWaves][kODRows];
+  __shared__ float red_m[W][kODRows], red_l[W][kODRows];
   __shared__ int last_sh;
   const int tid = threadIdx.x, lane = tid & 63;
   const int wv = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const OctPlan P = od_plan(a, blockIdx.x);
+  const OctPlan P = od_plan<W>(a);
   if (P.none) return;
   const int h = P.h, G = a.G, HQ = a.H * a.G;
   const int n = min(max(P.n, 0), a.max_seq), Q = min(P.Q, a.max_q);
@@ -202,7 +273,7 @@ __global__ __launch_bounds__(kODThreads, D == 256 ? 1 : 2) void octet_decode_ker
       a.lse[((int64_t)P.q0 + j) * HQ + hq] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
   };
   if (p0 < 0) {  // an empty request's rows are 0; fewer keys than queries are refused
-    for (int i = tid; i < nrow * (D / 4); i += kODThreads)
+    for (int i = tid; i < nrow * (D / 4); i += kThreads)
       finish(i / (D / 4), i % (D / 4) * 4, float4v{}, kODNone, n > 0 ? NAN : 0.f);
     return;
   }
@@ -240,21 +311,23 @@ __global__ __launch_bounds__(kODThreads, D == 256 ? 1 : 2) void octet_decode_ker
 #pragma unroll
   for (int e = 0; e < N; ++e) acc[e] = float4v{};
 
-  // the block's steps in equal parts
-  const int s0 = P.s0 + (int)((int64_t)P.steps * P.c / P.nch);
-  const int s1 = P.s0 + (int)((int64_t)P.steps * (P.c + 1) / P.nch);
+  // the block's steps in equal parts, the first ones a step longer
+  const int each = od_div(P.steps, P.nch, __builtin_amdgcn_rcpf((float)P.nch)), more = P.steps - each * P.nch;
+  const int s0 = P.s0 + each * P.c + min(P.c, more);
+  const int s1 = s0 + each + (P.c < more);
   const int first_tile = a.window ? max(p0 - a.window + 1, 0) / kOctTile : 0;
   bool bad = false;
 
   const uint8_t* base = a.page + (int64_t)h * F::kRecord;
   const int32_t* bt = a.bt + (int64_t)P.r * a.bt_row_stride;
   // tile ids of this wave's next 64 steps, one step per lane (-1: a block outside the cache)
+  const float by_tpb = __builtin_amdgcn_rcpf((float)a.tpb);
   int tid0 = 0, tid1 = 0;
   auto fetch_ids = [&](int s) {
-    const int mine = min(s + kODWaves * lane, s1 - 1);  // (past the chunk: its last step's again)
+    const int mine = min(s + W * lane, s1 - 1);  // (past the chunk: its last step's again)
     // (no tile outside the keys that some row sees: a window's past blocks may be gone)
     const int t0 = max(2 * mine, first_tile), t1 = min(max(2 * mine + 1, first_tile), (n - 1) / kOctTile);
-    const int b0 = t0 / a.tpb, b1 = t1 / a.tpb;
+    const int b0 = od_div(t0, a.tpb, by_tpb), b1 = od_div(t1, a.tpb, by_tpb);
     const int i0 = bt[b0], i1 = bt[b1];
     tid0 = (uint32_t)i0 < (uint32_t)a.num_blocks ? i0 * a.tpb + t0 - b0 * a.tpb : -1;
     tid1 = (uint32_t)i1 < (uint32_t)a.num_blocks ? i1 * a.tpb + t1 - b1 * a.tpb : -1;
@@ -415,21 +488,21 @@ __global__ __launch_bounds__(kODThreads, D == 256 ? 1 : 2) void octet_decode_ker
 
   for (int s = s0 + wv; s < s1;) {
     fetch_ids(s);
-    const int cnt = min(64, (s1 - s + kODWaves - 1) / kODWaves);  // steps of this wave in the set
+    const int cnt = min(64, (s1 - s + W - 1) / W);  // steps of this wave in the set
     OctStep<D> xa, xb;
     load(0, xa);
     int k = 0;
     while (true) {
       load(min(k + 1, cnt - 1), xb);
       __builtin_amdgcn_sched_barrier(0);
-      step(s + kODWaves * k, xa);
+      step(s + W * k, xa);
       if (++k >= cnt) break;
       load(min(k + 1, cnt - 1), xa);
       __builtin_amdgcn_sched_barrier(0);
-      step(s + kODWaves * k, xb);
+      step(s + W * k, xb);
       if (++k >= cnt) break;
     }
-    s += kODWaves * 64;
+    s += W * 64;
   }
   if (bad && lane == 0) atomicOr(a.err, TTKV_ERR_BAD_BLOCK);
   l = bad ? NAN : cross_row_sum(l);
@@ -443,7 +516,7 @@ __global__ __launch_bounds__(kODThreads, D == 256 ? 1 : 2) void octet_decode_ker
   {
     float M = kODNone;
 #pragma unroll
-    for (int w = 0; w < kODWaves; ++w) M = fmaxf(M, red_m[w][col]);
+    for (int w = 0; w < W; ++w) M = fmaxf(M, red_m[w][col]);
     const float f = exp2f(m - M);
 #pragma unroll
     for (int i = 0; i < 4; ++i)
@@ -455,14 +528,14 @@ __global__ __launch_bounds__(kODThreads, D == 256 ? 1 : 2) void octet_decode_ker
   __syncthreads();
   const int PR = a.part_rows;
   const int64_t part = ((int64_t)P.part + P.c) * a.H + h;  // (where the block is split)
-  for (int i = tid; i < nrow * (D / 4); i += kODThreads) {
+  for (int i = tid; i < nrow * (D / 4); i += kThreads) {
     const int r = i / (D / 4), d = i % (D / 4) * 4;
     float mm = kODNone, ll = 0.f;
     float4v o = {};
 #pragma unroll
-    for (int w = 0; w < kODWaves; ++w) mm = fmaxf(mm, red_m[w][r]);
+    for (int w = 0; w < W; ++w) mm = fmaxf(mm, red_m[w][r]);
 #pragma unroll
-    for (int w = 0; w < kODWaves; ++w) {
+    for (int w = 0; w < W; ++w) {
       ll += red_l[w][r] * exp2f(red_m[w][r] - mm);
       o += *(const float4v*)&red_o[w][r][d];
     }
@@ -479,7 +552,7 @@ __global__ __launch_bounds__(kODThreads, D == 256 ? 1 : 2) void octet_decode_ker
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   __syncthreads();
   if (tid == 0) {
-    int* cnt = a.ws_cnt + P.block * a.H + h;
+    int* cnt = a.ws_cnt + (P.block * a.H + h) * a.cnt_stride;
     const int prev = arrive(cnt);
     last_sh = prev == P.nch - 1;
     if (last_sh) __hip_atomic_store(cnt, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
@@ -488,7 +561,7 @@ __global__ __launch_bounds__(kODThreads, D == 256 ? 1 : 2) void octet_decode_ker
   if (!last_sh) return;
   // d / 4 lanes take a row, four dims each, chunk after chunk with a running maximum; where rows are few,
   // 2^share such teams take every 2^share-th chunk of a row and are joined in LDS.
-  constexpr int LPR = D / 4, TEAMS = kODThreads / LPR, AHEAD = 8;
+  constexpr int LPR = D / 4, TEAMS = kThreads / LPR, AHEAD = 8;
   const int team = tid / LPR, d4 = tid % LPR * 4;
   int share = 0;
   while (nrow << (share + 1) <= TEAMS && 2 << share <= P.nch) ++share;
@@ -526,7 +599,7 @@ __global__ __launch_bounds__(kODThreads, D == 256 ? 1 : 2) void octet_decode_ker
         at[D + 1] = ll;
       }
       __syncthreads();
-      if (sub) return;
+      if (sub || r >= nrow) return;
       for (int u = 1; u < 1 << share; ++u) {
         const float* y = at + u * (D + 8);
         const float mn = fmaxf(mm, y[D]), f = exp2f(mm - mn), g = exp2f(y[D] - mn);
@@ -539,8 +612,22 @@ __global__ __launch_bounds__(kODThreads, D == 256 ? 1 : 2) void octet_decode_ker
   }
 }
 
-// The plan's item target: workgroups that are resident.
-static int od_target(int d) { return (d == 256 ? 1 : 2) * device_cu_count(); }
+// The plan's item target: two workgroups per compute unit, one of the larger ones. Three of the smaller would
+// fit, but shorter chunks pay their prologue and their join more often (8 x 14,402 tokens: 45.3 us with two,
+// 50 with three; 8 x 5 queries over 3,000 keys 21, 25).
+static int od_target(int d, int waves) { return (d == 256 || waves > 4 ? 1 : 2) * device_cu_count(); }
+
+// Waves of a workgroup: four, or eight where the (block, head) pairs are about as many as the compute units,
+// so that few are split, and their keys of a middle length. Measured with four and with eight (us, eight KV
+// heads of 128 and 64 dims): 24 x 700 keys 13.8 and 11.9, 10.8 and 8.5; 24 x 3,000 35.6 and 29.0, 22.2 and
+// 22.4; 32 x 2,000 28.6 and 27.2, 17.9 and 15.7; but 24 x 512 9.0 and 10.1, 7.1 and 7.4; 32 of 600 to 11,000
+// 72.8 and 79.0, 42.6 and 47.8; 8 x 1,024 10.1 and 11.5; 16 x 1,024 11.9 and 12.6, 9.6 and 9.0. (Heads of 256
+// dims have registers for four.)
+static int od_waves(int d, int64_t pairs, int max_seq, int max_q, int window) {
+  const int span = window ? std::min(max_seq, window + max_q - 1) : max_seq, steps = (span + kODStep - 1) / kODStep;
+  const int cus = device_cu_count();
+  return d < 256 && 8 * pairs > 5 * cus && pairs <= cus && steps > 16 && steps <= 96 ? 8 : 4;
+}
 
 // Requests per launch, of `blocks` row blocks each: the plan's lanes, and a counter per (block, head).
 static int od_slice(int H, int blocks, int num_reqs) {
@@ -551,11 +638,11 @@ static int od_slice(int H, int blocks, int num_reqs) {
 // steps, and a split block of st steps has less than st / C + 1 < 2 st / C chunks: less than 2 target of
 // them in all; and whole rounds of the four waves of a request.
 static int64_t od_max_chunks(int max_seq) {
-  const int64_t round = kODStep * kODWaves;
+  const int64_t round = kODStep * 4;
   return std::max<int64_t>(1, (max_seq + round - 1) / round + 1);  // (a window's first step may be cut)
 }
 static int64_t od_parts(int d, int64_t pairs, int max_seq) {
-  return std::min<int64_t>(2 * od_target(d), pairs * od_max_chunks(max_seq));
+  return std::min<int64_t>(2 * od_target(d, 4), pairs * od_max_chunks(max_seq));
 }
 
 int64_t octet_decode_workspace_bytes(int H, int HQ, int d, int num_reqs, int max_q, int max_seq) {
@@ -564,20 +651,35 @@ int64_t octet_decode_workspace_bytes(int H, int HQ, int d, int num_reqs, int max
   return kCounterBytes + (int64_t)2 * 2 * device_cu_count() * kODRows * (d + 2) * 4;
 }
 
-template <int D>
-static int od_launch(const OctDecodeArgs& a, unsigned grid, int q_dtype, bool chunk, hipStream_t st) {
-  constexpr int smem = kODWaves * kODRows * (D + 4) * 4;
-  auto kernel = q_dtype == TTKV_DTYPE_F16
-                    ? chunk ? octet_decode_kernel<D, TTKV_DTYPE_F16, true> : octet_decode_kernel<D, TTKV_DTYPE_F16, false>
-                : chunk ? octet_decode_kernel<D, TTKV_DTYPE_BF16, true>
-                        : octet_decode_kernel<D, TTKV_DTYPE_BF16, false>;
+static int od_resident[3][2][2][2];  // workgroups per CU, by kernel (the same on every device of a process)
+
+template <int D, int W>
+static int od_launch(OctDecodeArgs a, unsigned grid, int q_dtype, bool chunk, hipStream_t st) {
+  constexpr int smem = W * kODRows * (D + 4) * 4;
+  auto kernel =
+      q_dtype == TTKV_DTYPE_F16
+          ? chunk ? octet_decode_kernel<D, W, TTKV_DTYPE_F16, true> : octet_decode_kernel<D, W, TTKV_DTYPE_F16, false>
+      : chunk ? octet_decode_kernel<D, W, TTKV_DTYPE_BF16, true>
+              : octet_decode_kernel<D, W, TTKV_DTYPE_BF16, false>;
   if (smem > 65536 - 4096)
     if (int rc = raise_smem_limit((const void*)kernel, smem)) return rc;
-  hipLaunchKernelGGL(kernel, dim3(grid), dim3(kODThreads), smem, st, a);
+  int& resident = od_resident[D / 128][W > 4][q_dtype == TTKV_DTYPE_F16][chunk];
+  if (!resident) {
+    int per = 0;
+    if (hipOccupancyMaxActiveBlocksPerMultiprocessor(&per, kernel, 64 * W, smem) != hipSuccess) per = 1;
+    resident = std::max(per, 1);
+  }
+  a.resident = std::max(resident * device_cu_count(), od_target(D, W));
+  hipLaunchKernelGGL(kernel, dim3(a.H, grid), dim3(64 * W), smem, st, a);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess)
     return host_fail(TTKV_E_LAUNCH, std::string("octet decode launch: ") + hipGetErrorString(e));
   return TTKV_OK;
+}
+template <int D>
+static int od_launch(const OctDecodeArgs& a, int waves, unsigned grid, int q_dtype, bool chunk, hipStream_t st) {
+  if (waves == 4) return od_launch<D, 4>(a, grid, q_dtype, chunk, st);
+  return od_launch<D, D == 256 ? 4 : 8>(a, grid, q_dtype, chunk, st);
 }
 
 int octet_decode_paged(int H, int HQ, int d, float scale, const void* q, int q_dtype, int64_t q_row_stride,
@@ -634,7 +736,7 @@ int octet_decode_paged(int H, int HQ, int d, float scale, const void* q, int q_d
   a.ws_o = (float*)((char*)ws + kCounterBytes);
   a.ws_ml = a.ws_o + parts * a.part_rows * d;
   a.o_bytes = (uint32_t)(parts * a.part_rows * d * 4);
-  a.target = od_target(d);
+  a.join = (float)(a.part_rows * d) * kODJoin;
   a.err = err;
   for (int r0 = 0; r0 < num_reqs; r0 += slice) {
     a.num_reqs = std::min(slice, num_reqs - r0);
@@ -643,10 +745,13 @@ int octet_decode_paged(int H, int HQ, int d, float scale, const void* q, int q_d
     a.bt = bt + (int64_t)r0 * bt_row_stride;
     // an item per (block, head), and what the split ones have more
     const int64_t pairs = (int64_t)a.num_reqs * H * blocks;
-    const unsigned grid = (unsigned)std::min(pairs + a.target, pairs * od_max_chunks(max_seq));
-    const int rc = d == 64    ? od_launch<64>(a, grid, q_dtype, max_q > 1, st)
-                   : d == 128 ? od_launch<128>(a, grid, q_dtype, max_q > 1, st)
-                              : od_launch<256>(a, grid, q_dtype, max_q > 1, st);
+    a.cnt_stride = (int)std::max<int64_t>(1, std::min<int64_t>(32, kMaxCounters / pairs));
+    const int waves = od_waves(d, pairs, max_seq, max_q, window), target = od_target(d, waves);
+    a.by_target = 1.f / (float)target;
+    const unsigned grid = (unsigned)((std::min(pairs + target, pairs * od_max_chunks(max_seq)) + H - 1) / H);
+    const int rc = d == 64    ? od_launch<64>(a, waves, grid, q_dtype, max_q > 1, st)
+                   : d == 128 ? od_launch<128>(a, waves, grid, q_dtype, max_q > 1, st)
+                              : od_launch<256>(a, waves, grid, q_dtype, max_q > 1, st);
     if (rc != TTKV_OK) return rc;
   }
   return TTKV_OK;
