@@ -482,6 +482,52 @@ def test_decode_long(d, H, G, lens):
     _check(st, q, counts, out, None, at, window=1500)
 
 
+@pytest.mark.parametrize("d,H,G,R", [(64, 8, 4, 36), (128, 8, 4, 36), (256, 4, 3, 44)])
+@pytest.mark.parametrize("window", [0, 30])
+def test_decode_drafts_of_large_batches(d, H, G, R, window):
+    """More than 16 rows per KV head in batches that share a block's keys between two groups of rows; a
+    NaN in a value stays with the rows that see it."""
+    g = _gen(d + window)
+    lens = [8 + int(torch.randint(0, 150, (1,), generator=g)) for _ in range(R)]
+    st = Store(lens, H, d, seed=6, dtype=torch.bfloat16)
+    v = st.v.clone()
+    sick = sum(lens[:5]) + lens[5] - 4                     # the fourth last token of request 5
+    v[sick, H - 1, d - 1] = float("nan")
+    kernels.octet_write_paged(st.lay, st.k.cuda(), v.cuda(), st.slots.cuda(), st.page)
+    counts = [8 if i % 4 else 5 + i % 3 for i in range(R)]
+    q = torch.randn(sum(counts), H * G, d, generator=g).bfloat16().cuda()
+    lse = torch.zeros(q.shape[:2], device="cuda")
+    out, err, at = _decode(st, q, counts, max_q_len=8, lse=lse, window=window)
+    assert err == 0
+    last, heads = counts[5] - 4, slice((H - 1) * G, H * G)
+    sees = out[at[5]:at[6]][last:, heads]                  # the queries from that token's on
+    assert bool(torch.isnan(sees[..., d - 32:]).all()) and bool(torch.isfinite(sees[..., :d - 32]).all())
+    for r in range(R):
+        rows = slice(at[r], at[r + 1])
+        if r == 5:
+            rows = slice(at[5], at[5] + last)
+            K, V = (x[:lens[5] - 4] for x in st.kv(5))
+            _close(out[rows], lse[rows], q[rows].cpu(), K, V, d ** -0.5, r, window=window)
+        else:
+            _close(out[rows], lse[rows], q[rows].cpu(), *st.kv(r), d ** -0.5, r, window=window)
+
+
+@pytest.mark.parametrize("d,H,R,window,Q", [(64, 8, 24, 0, 1), (128, 8, 24, 0, 1), (64, 8, 32, 640, 2),
+                                            (128, 8, 21, 600, 3), (128, 4, 60, 0, 1)])
+def test_decode_pairs_that_fill_the_chip(d, H, R, window, Q):
+    """About as many (request, KV head) pairs as compute units, keys of a middle length."""
+    g = _gen(R)
+    lens = [int(torch.randint(3, 900 if R < 40 else 700, (1,), generator=g)) for _ in range(R)]
+    lens[1] = 1700
+    st = Store(lens, H, d, 32, seed=6, dtype=torch.float16)
+    q = torch.randn(R * Q, H * 3, d, generator=g).half().cuda()
+    sinks = torch.randn(H * 3, generator=g)
+    lse = torch.zeros(q.shape[:2], device="cuda")
+    out, err, at = _decode(st, q, [Q] * R, lse=lse, window=window, sinks=sinks.cuda())
+    assert err == 0
+    _check(st, q, None, out, lse, at, window=window, sinks=sinks)
+
+
 def test_decode_many_requests():
     """More requests than one launch plans for, some of them waiting, one per group long."""
     lens = [1 + 7 * i % 90 for i in range(600)]

@@ -23,6 +23,8 @@
 //     the rescale is a lane's factor.
 #include <math.h>
 
+#include <type_traits>
+
 #include "ttkv_host.h"
 #include "ttkv_nibble.h"
 #include "ttkv_octet.h"
@@ -91,7 +93,7 @@ __device__ __forceinline__ int od_div(int x, int d, float by) {
   return k + ((k + 1) * d <= x);
 }
 
-template <int W>  // waves of a workgroup
+template <int W, int RB>  // waves of a workgroup, rows of a block
 __device__ __forceinline__ OctPlan od_plan(const OctDecodeArgs& a) {
   const int lane = threadIdx.x & 63;
   int n[kODPlanLanes], q0[kODPlanLanes], Q[kODPlanLanes], s0[kODPlanLanes], st[kODPlanLanes], rb[kODPlanLanes];
@@ -112,7 +114,7 @@ __device__ __forceinline__ OctPlan od_plan(const OctDecodeArgs& a) {
     const int nn = min(max(n[i], 0), a.max_seq), qq = min(max(Q[i], 0), a.max_q), p0 = nn - Q[i];
     s0[i] = a.window && p0 >= a.window ? (p0 - a.window + 1) / kODStep : 0;
     st[i] = p0 >= 0 && qq > 0 ? (p0 + qq - 1) / kODStep + 1 - s0[i] : 0;
-    rb[i] = (qq * a.G + kODRows - 1) / kODRows;
+    rb[i] = (qq * a.G + RB - 1) / RB;
     total += st[i] * rb[i];
     longest = max(longest, st[i]);
     whole += rb[i];
@@ -226,24 +228,24 @@ __device__ __forceinline__ uint32_t od_high(bf16x2 a, bf16x2 b) {
   return __builtin_amdgcn_perm(__builtin_bit_cast(uint32_t, b), __builtin_bit_cast(uint32_t, a), 0x07060302u);
 }
 
-template <int D, int W, int QDT, bool CHUNK>
-__global__ __launch_bounds__(64 * W, W > 4 ? W / 4 : D == 256 ? 1 : D == 128 ? 2 : 4) void octet_decode_kernel(OctDecodeArgs a) {
+template <int D, int W, int QDT, bool CHUNK, int RG>
+__global__ __launch_bounds__(64 * W, W > 4 ? W / 4 : D == 256 ? 3 - RG : D == 128 ? 2 : 5 - RG) void octet_decode_kernel(OctDecodeArgs a) {
   using F = Oct<D>;
   constexpr int N = F::kDims, KS = D / 32, PIECES = D / 64, PARTS = QDT == TTKV_DTYPE_F16 ? 2 : 1;
-  constexpr int kThreads = 64 * W;
+  constexpr int kThreads = 64 * W, RB = kODRows * RG;
   constexpr int RS = D + 4;  // floats of a row in LDS: the rows' columns start in different banks
   extern __shared__ __align__(16) float red_all[];  // [waves][rows][RS]: the waves' results, then the join's
-  float(*red_o)[kODRows][RS] = (float(*)[kODRows][RS])red_all;
-  __shared__ float red_m[W][kODRows], red_l[W][kODRows];
+  float(*red_o)[RB][RS] = (float(*)[RB][RS])red_all;
+  __shared__ float red_m[W][RB], red_l[W][RB];
   __shared__ int last_sh;
   const int tid = threadIdx.x, lane = tid & 63;
   const int wv = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const OctPlan P = od_plan<W>(a);
+  const OctPlan P = od_plan<W, RB>(a);
   if (P.none) return;
   const int h = P.h, G = a.G, HQ = a.H * a.G;
   const int n = min(max(P.n, 0), a.max_seq), Q = min(P.Q, a.max_q);
   const int p0 = n - P.Q;  // position of query 0
-  const int row0 = P.rb * kODRows, nrow = min(kODRows, Q * G - row0);  // the block's rows
+  const int row0 = P.rb * RB, nrow = min(RB, Q * G - row0);  // the block's rows
   const bool outside = P.q0 < 0 || (int64_t)P.q0 + Q > a.num_tokens;
   if (tid == 0 && h == 0 && P.c == 0 && P.rb == 0 &&
       (P.n > a.max_seq || P.Q > a.max_q || (n > 0 && p0 < 0) || outside))
@@ -279,37 +281,41 @@ __global__ __launch_bounds__(64 * W, W > 4 ? W / 4 : D == 256 ? 1 : D == 128 ? 2
   }
   const int col = lane & 15, q4 = lane >> 4;
 
-  // The queries, row `col`, as the B operand of the score products: dims q4 D / 4 + 8 s + (0..7)
-  bf16x8 qf[PARTS][KS];
-  const int my = min(col, nrow - 1);
-  {
-    const bool on = col < nrow && has(my);
+  // The queries, row 16 g + `col` of group g, as the B operand of the score products: dims q4 D / 4 + 8 s + (0..7)
+  bf16x8 qf[RG][PARTS][KS];
+  float m[RG], l[RG];
+  int lim[RG], low[RG];  // last key the lane's row sees, and the one before its first
+  float4v acc[RG][N];    // [g][e][i]: dim (4 q4 + i) N + e of the lane's row
+#pragma unroll
+  for (int g = 0; g < RG; ++g) {
+    const int my = min(kODRows * g + col, nrow - 1);
+    const bool on = kODRows * g + col < nrow && has(my);
     const uint16_t* src = a.q + row_at(my, a.q_row_stride) + q4 * (D / 4);
 #pragma unroll
     for (int s = 0; s < KS; ++s) {
       u32x4 raw = {};
       if (on) raw = *gbl((const u32x4*)(src + 8 * s));
       if constexpr (QDT == TTKV_DTYPE_BF16) {
-        qf[0][s] = __builtin_bit_cast(bf16x8, raw);
+        qf[g][0][s] = __builtin_bit_cast(bf16x8, raw);
       } else {
         const half8 x = __builtin_bit_cast(half8, raw);
 #pragma unroll
         for (int j = 0; j < 8; ++j) {  // 11 bits are 8 and the 3 that they leave
           const __bf16 hi = (__bf16)(float)x[j];
-          qf[0][s][j] = hi;
-          qf[PARTS - 1][s][j] = (__bf16)((float)x[j] - (float)hi);
+          qf[g][0][s][j] = hi;
+          qf[g][PARTS - 1][s][j] = (__bf16)((float)x[j] - (float)hi);
         }
       }
     }
-  }
-  const int lim = p0 + (CHUNK ? (row0 + my) / G : 0);  // last key the lane's row sees
-  const int low = a.window ? lim - a.window : -1;      // and the one before its first
-  const int see_all = p0 + (CHUNK ? row0 / G : 0);     // no row of the block sees less than to here
-  const int low_all = a.window ? p0 + (CHUNK ? (row0 + nrow - 1) / G : 0) - a.window : -1;  // and from behind here
-  float m = kODNone, l = 0.f;
-  float4v acc[N];  // [e][i]: dim (4 q4 + i) N + e of the lane's row
+    lim[g] = p0 + (CHUNK ? (row0 + my) / G : 0);
+    low[g] = a.window ? lim[g] - a.window : -1;
+    m[g] = kODNone;
+    l[g] = 0.f;
 #pragma unroll
-  for (int e = 0; e < N; ++e) acc[e] = float4v{};
+    for (int e = 0; e < N; ++e) acc[g][e] = float4v{};
+  }
+  const int see_all = p0 + (CHUNK ? row0 / G : 0);  // no row of the block sees less than to here
+  const int low_all = a.window ? p0 + (CHUNK ? (row0 + nrow - 1) / G : 0) - a.window : -1;  // and from behind here
 
   // the block's steps in equal parts, the first ones a step longer
   const int each = od_div(P.steps, P.nch, __builtin_amdgcn_rcpf((float)P.nch)), more = P.steps - each * P.nch;
@@ -332,11 +338,15 @@ __global__ __launch_bounds__(64 * W, W > 4 ? W / 4 : D == 256 ? 1 : D == 128 ? 2
     tid0 = (uint32_t)i0 < (uint32_t)a.num_blocks ? i0 * a.tpb + t0 - b0 * a.tpb : -1;
     tid1 = (uint32_t)i1 < (uint32_t)a.num_blocks ? i1 * a.tpb + t1 - b1 * a.tpb : -1;
   };
-  auto load = [&](int k, OctStep<D>& x) {  // the wave's k-th step since fetch_ids
+  auto record = [&](int k, int t) {  // of the wave's k-th step since fetch_ids
+    const int id = __builtin_amdgcn_readlane(t ? tid1 : tid0, k);
+    bad |= id < 0;
+    return base + (int64_t)max(id, 0) * a.tile_stride;
+  };
+  auto load_keys = [&](int k, OctStep<D>& x) {
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
-      const int id = __builtin_amdgcn_readlane(t ? tid1 : tid0, k);
-      const uint8_t* rec = base + (int64_t)max(id, 0) * a.tile_stride;
+      const uint8_t* rec = record(k, t);
 #pragma unroll
       for (int p = 0; p < PIECES; ++p)
         x.k[t][p] = __builtin_nontemporal_load(gbl((const u32x4*)(rec + 1024 * p + 16 * lane)));
@@ -344,18 +354,28 @@ __global__ __launch_bounds__(64 * W, W > 4 ? W / 4 : D == 256 ? 1 : D == 128 ? 2
         x.kp[t] = __builtin_nontemporal_load(gbl((const uint16_t*)(rec + F::kKp) + lane));
       else
         x.kp[t] = __builtin_nontemporal_load(gbl(rec + F::kKp + (D == 64 ? (lane >> 5) * 16 + col : lane)));
+    }
+  };
+  auto load_values = [&](int k, OctStep<D>& x) {
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      const uint8_t* rec = record(k, t);
 #pragma unroll
       for (int p = 0; p < PIECES; ++p)
         x.v[t][p] = __builtin_nontemporal_load(gbl((const u32x4*)(rec + F::kV + 1024 * p + 16 * lane)));
       x.vp[t] = __builtin_nontemporal_load(gbl((const uint32_t*)(rec + F::kVp + col * N / 32 * 16) + q4));
-      bad |= id < 0;
     }
   };
-  auto step = [&](int s, OctStep<D>& x) {
-    float4v sc[2];
+  auto load = [&](int k, OctStep<D>& x) {
+    load_keys(k, x);
+    load_values(k, x);
+  };
+  auto step = [&](int s, OctStep<D>& x, auto&& keys_done) {
+    float4v sc[RG][2];
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
-      sc[t] = float4v{};
+#pragma unroll
+      for (int g = 0; g < RG; ++g) sc[g][t] = float4v{};
       const float pw[2] = {oct_power(x.kp[t] & 0xffu), oct_power(x.kp[t] >> 8)};
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) {
@@ -371,11 +391,15 @@ __global__ __launch_bounds__(64 * W, W > 4 ? W / 4 : D == 256 ? 1 : D == 128 ? 2
           kf[4 * w + 3] = hi[1];
         }
 #pragma unroll
-        for (int part = 0; part < PARTS; ++part)
-          sc[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, qf[part][ks], sc[t], 0, 0, 0);
+        for (int g = 0; g < RG; ++g)
+#pragma unroll
+          for (int part = 0; part < PARTS; ++part)
+            sc[g][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, qf[g][part][ks], sc[g][t], 0, 0, 0);
       }
-      sc[t] *= a.scale_log2;
+#pragma unroll
+      for (int g = 0; g < RG; ++g) sc[g][t] *= a.scale_log2;
     }
+    keys_done();
     const int tok = s * kODStep + 4 * q4;
     uint32_t note = 0;  // bit 4 t + i: the lane's dims of that token are NaN
     if ((s + 1) * kODStep - 1 > see_all || s * kODStep <= low_all) {
@@ -387,10 +411,12 @@ __global__ __launch_bounds__(64 * W, W > 4 ? W / 4 : D == 256 ? 1 : D == 128 ? 2
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const int tk = tok + 16 * t + i;
-          if (tk > lim || tk <= low) sc[t][i] = -INFINITY;
-          bool drop = CHUNK ? tk >= n || tk <= p0 - a.window : tk > lim || tk <= low;
-          if (CHUNK && !a.window) drop = tk >= n;
+#pragma unroll
+          for (int g = 0; g < RG; ++g)
+            if (tk > lim[g] || tk <= low[g]) sc[g][t][i] = -INFINITY;
+          bool drop = tk > lim[0] || tk <= low[0];
           if constexpr (CHUNK) {
+            drop = tk >= n || (a.window && tk <= p0 - a.window);
             const uint32_t c = x.v[t][i * N / 16][i * N % 16 / 4] & 0x7fu;  // (a group is NaN as a whole)
             if (!drop && c == kOctNanCode) {
               note |= 1u << (4 * t + i);
@@ -406,38 +432,49 @@ __global__ __launch_bounds__(64 * W, W > 4 ? W / 4 : D == 256 ? 1 : D == 128 ? 2
     }
     // Weights against the maximum as it stands; it moves where a lane's sum of eight is large (or NaN). A
     // score's product with the scale is rounded by itself, so that equal scores weigh the same.
-    float p[8], sum;
-    auto weights = [&]() {
+    float p[RG][8], sum[RG];
+    auto weights = [&](int g) {
 #pragma clang fp contract(off)
-      sum = 0.f;
+      sum[g] = 0.f;
 #pragma unroll
       for (int t = 0; t < 2; ++t)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          p[4 * t + i] = fast_exp2(sc[t][i] - m);
-          sum += p[4 * t + i];
+          p[g][4 * t + i] = fast_exp2(sc[g][t][i] - m[g]);
+          sum[g] += p[g][4 * t + i];
         }
     };
-    weights();
-    if (__builtin_amdgcn_ballot_w64(!(sum <= kODMost))) {
-      float mt = kODNone;
+    bool fits = true;
 #pragma unroll
-      for (int t = 0; t < 2; ++t)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) mt = fmaxf(mt, sc[t][i]);
-      const float mn = fmaxf(m, cross_row_max(mt)), f = exp2f(m - mn);
-      m = mn;
-      l *= f;
-#pragma unroll
-      for (int e = 0; e < N; ++e) acc[e] *= f;
-      weights();
+    for (int g = 0; g < RG; ++g) {
+      weights(g);
+      fits &= sum[g] <= kODMost;
     }
-    l += sum;
-    bf16x8 ph, pl;  // 16 bits of each weight, in two parts
+    if (__builtin_amdgcn_ballot_w64(!fits)) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      ph[i] = (__bf16)p[i];
-      pl[i] = (__bf16)(p[i] - (float)ph[i]);
+      for (int g = 0; g < RG; ++g) {
+        float mt = kODNone;
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) mt = fmaxf(mt, sc[g][t][i]);
+        const float mn = fmaxf(m[g], cross_row_max(mt)), f = exp2f(m[g] - mn);
+        m[g] = mn;
+        l[g] *= f;
+#pragma unroll
+        for (int e = 0; e < N; ++e) acc[g][e] *= f;
+        weights(g);
+      }
+    }
+    bf16x8 ph[RG], pl[RG];  // 16 bits of each weight, in two parts
+#pragma unroll
+    for (int g = 0; g < RG; ++g) {
+      l[g] += sum[g];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        ph[g][i] = (__bf16)p[g][i];
+        pl[g][i] = (__bf16)(p[g][i] - (float)ph[g][i]);
+      }
     }
     float vp[2][4];
 #pragma unroll
@@ -462,10 +499,13 @@ __global__ __launch_bounds__(64 * W, W > 4 ? W / 4 : D == 256 ? 1 : D == 128 ? 2
         hi[2 * t + 1] = od_high(pr[2], pr[3]);
       }
       const bf16x8 v0 = __builtin_bit_cast(bf16x8, lo), v1 = __builtin_bit_cast(bf16x8, hi);
-      acc[e] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v0, ph, acc[e], 0, 0, 0);
-      acc[e + 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v1, ph, acc[e + 1], 0, 0, 0);
-      acc[e] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v0, pl, acc[e], 0, 0, 0);
-      acc[e + 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v1, pl, acc[e + 1], 0, 0, 0);
+#pragma unroll
+      for (int g = 0; g < RG; ++g) {
+        acc[g][e] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v0, ph[g], acc[g][e], 0, 0, 0);
+        acc[g][e + 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v1, ph[g], acc[g][e + 1], 0, 0, 0);
+        acc[g][e] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v0, pl[g], acc[g][e], 0, 0, 0);
+        acc[g][e + 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v1, pl[g], acc[g][e + 1], 0, 0, 0);
+      }
     }
     if (CHUNK && __builtin_amdgcn_ballot_w64(note != 0)) {
 #pragma unroll
@@ -475,12 +515,13 @@ __global__ __launch_bounds__(64 * W, W > 4 ? W / 4 : D == 256 ? 1 : D == 128 ? 2
         for (int b = 0; b < 4; ++b) {
           const uint32_t lanes = (uint32_t)(of >> (16 * b)) & 0xffffu;
           const int tk = s * kODStep + 16 * (k / 4) + 4 * b + k % 4;
-          if (tk > lim || tk <= low) continue;
 #pragma unroll
-          for (int i = 0; i < 4; ++i)
-            if ((lanes >> (4 * q4 + i)) & 1)
+          for (int g = 0; g < RG; ++g)
 #pragma unroll
-              for (int e = 0; e < N; ++e) acc[e][i] = NAN;
+            for (int i = 0; i < 4; ++i)
+              if (tk <= lim[g] && tk > low[g] && ((lanes >> (4 * q4 + i)) & 1))
+#pragma unroll
+                for (int e = 0; e < N; ++e) acc[g][e][i] = NAN;
         }
       }
     }
@@ -489,41 +530,66 @@ __global__ __launch_bounds__(64 * W, W > 4 ? W / 4 : D == 256 ? 1 : D == 128 ? 2
   for (int s = s0 + wv; s < s1;) {
     fetch_ids(s);
     const int cnt = min(64, (s1 - s + W - 1) / W);  // steps of this wave in the set
-    OctStep<D> xa, xb;
-    load(0, xa);
-    int k = 0;
-    while (true) {
-      load(min(k + 1, cnt - 1), xb);
-      __builtin_amdgcn_sched_barrier(0);
-      step(s + W * k, xa);
-      if (++k >= cnt) break;
-      load(min(k + 1, cnt - 1), xa);
-      __builtin_amdgcn_sched_barrier(0);
-      step(s + W * k, xb);
-      if (++k >= cnt) break;
+    if constexpr (D == 256 || (D == 128 && CHUNK)) {
+      // One register set: the next step's keys are asked for once the scores are formed, a step's values when it
+      // begins. Fewer registers, so heads of 256 dims have two waves per SIMD (24 x 1,000 keys 16.8 us with two
+      // sets, 14.7 so; 6 x 5 queries over 4,000 30.5, 28.6; of 128 dims 22.9, 21.6; single queries of 128 dims gain
+      // nothing, 64 of 100 to 3,000 43.4, 45.3).
+      OctStep<D> x;
+      load_keys(0, x);
+      for (int k = 0; k < cnt; ++k) {
+        load_values(k, x);
+        __builtin_amdgcn_sched_barrier(0);
+        step(s + W * k, x, [&]() {
+          __builtin_amdgcn_sched_barrier(0);
+          load_keys(min(k + 1, cnt - 1), x);
+          __builtin_amdgcn_sched_barrier(0);
+        });
+      }
+    } else {
+      OctStep<D> xa, xb;
+      auto none = []() {};
+      load(0, xa);
+      int k = 0;
+      while (true) {
+        load(min(k + 1, cnt - 1), xb);
+        __builtin_amdgcn_sched_barrier(0);
+        step(s + W * k, xa, none);
+        if (++k >= cnt) break;
+        load(min(k + 1, cnt - 1), xa);
+        __builtin_amdgcn_sched_barrier(0);
+        step(s + W * k, xb, none);
+        if (++k >= cnt) break;
+      }
     }
     s += W * 64;
   }
   if (bad && lane == 0) atomicOr(a.err, TTKV_ERR_BAD_BLOCK);
-  l = bad ? NAN : cross_row_sum(l);
+#pragma unroll
+  for (int g = 0; g < RG; ++g) l[g] = bad ? NAN : cross_row_sum(l[g]);
 
-  // ---- the four waves' results, joined in LDS
+  // ---- the waves' results, joined in LDS
   if (q4 == 0) {
-    red_m[wv][col] = m;
-    red_l[wv][col] = l;
+#pragma unroll
+    for (int g = 0; g < RG; ++g) {
+      red_m[wv][kODRows * g + col] = m[g];
+      red_l[wv][kODRows * g + col] = l[g];
+    }
   }
   __syncthreads();
-  {
+#pragma unroll
+  for (int g = 0; g < RG; ++g) {
+    const int r = kODRows * g + col;
     float M = kODNone;
 #pragma unroll
-    for (int w = 0; w < W; ++w) M = fmaxf(M, red_m[w][col]);
-    const float f = exp2f(m - M);
+    for (int w = 0; w < W; ++w) M = fmaxf(M, red_m[w][r]);
+    const float f = exp2f(m[g] - M);
 #pragma unroll
     for (int i = 0; i < 4; ++i)
 #pragma unroll
       for (int e = 0; e < N; e += 4)
-        *(float4v*)&red_o[wv][col][(4 * q4 + i) * N + e] =
-            float4v{acc[e][i] * f, acc[e + 1][i] * f, acc[e + 2][i] * f, acc[e + 3][i] * f};
+        *(float4v*)&red_o[wv][r][(4 * q4 + i) * N + e] =
+            float4v{acc[g][e][i] * f, acc[g][e + 1][i] * f, acc[g][e + 2][i] * f, acc[g][e + 3][i] * f};
   }
   __syncthreads();
   const int PR = a.part_rows;
@@ -623,10 +689,20 @@ static int od_target(int d, int waves) { return (d == 256 || waves > 4 ? 1 : 2) 
 // 22.4; 32 x 2,000 28.6 and 27.2, 17.9 and 15.7; but 24 x 512 9.0 and 10.1, 7.1 and 7.4; 32 of 600 to 11,000
 // 72.8 and 79.0, 42.6 and 47.8; 8 x 1,024 10.1 and 11.5; 16 x 1,024 11.9 and 12.6, 9.6 and 9.0. (Heads of 256
 // dims have registers for four.)
-static int od_waves(int d, int64_t pairs, int max_seq, int max_q, int window) {
+static int od_waves(int d, int64_t pairs, int max_seq, int max_q, int window, int groups) {
   const int span = window ? std::min(max_seq, window + max_q - 1) : max_seq, steps = (span + kODStep - 1) / kODStep;
   const int cus = device_cu_count();
-  return d < 256 && 8 * pairs > 5 * cus && pairs <= cus && steps > 16 && steps <= 96 ? 8 : 4;
+  return d < 256 && groups == 1 && 8 * pairs > 5 * cus && pairs <= cus && steps > 16 && steps <= 96 ? 8 : 4;
+}
+
+// Groups of 16 rows in a block: one, or two where blocks of one are more than the plan aims at; both share the
+// keys' and values' conversion, but a small call waits longer for its larger join (us, with one and two, eight
+// KV heads of 128 dims: 60 x 8 queries over 1,500 keys 45.2, 38.1; 30 x 5 over 1,500 25.5, 27.8; 6 x 5 over
+// 4,000 20.8, 25.3; four of 256 dims: 60 x 8 62.6, 43.9; 30 x 5 32.9, 33.4). Of fp16 queries of 256 dims there
+// are registers for one.
+static int od_groups(int H, int d, int q_dtype, int num_reqs, int rows) {
+  if (rows <= kODRows || (d == 256 && q_dtype == TTKV_DTYPE_F16)) return 1;
+  return (int64_t)num_reqs * H * ((rows + kODRows - 1) / kODRows) > od_target(d, 4) ? 2 : 1;
 }
 
 // Requests per launch, of `blocks` row blocks each: the plan's lanes, and a counter per (block, head).
@@ -648,22 +724,26 @@ static int64_t od_parts(int d, int64_t pairs, int max_seq) {
 int64_t octet_decode_workspace_bytes(int H, int HQ, int d, int num_reqs, int max_q, int max_seq) {
   if (num_reqs == 0 || max_q == 0) return 256;
   // (sizes that grow with every argument: layers of unlike heads share a workspace)
-  return kCounterBytes + (int64_t)2 * 2 * device_cu_count() * kODRows * (d + 2) * 4;
+  return kCounterBytes + (int64_t)2 * 2 * device_cu_count() * 2 * kODRows * (d + 2) * 4;
 }
 
-static int od_resident[3][2][2][2];  // workgroups per CU, by kernel (the same on every device of a process)
+static int od_resident[3][2][2][3];  // workgroups per CU, by kernel (the same on every device of a process)
 
 template <int D, int W>
-static int od_launch(OctDecodeArgs a, unsigned grid, int q_dtype, bool chunk, hipStream_t st) {
-  constexpr int smem = W * kODRows * (D + 4) * 4;
-  auto kernel =
-      q_dtype == TTKV_DTYPE_F16
-          ? chunk ? octet_decode_kernel<D, W, TTKV_DTYPE_F16, true> : octet_decode_kernel<D, W, TTKV_DTYPE_F16, false>
-      : chunk ? octet_decode_kernel<D, W, TTKV_DTYPE_BF16, true>
-              : octet_decode_kernel<D, W, TTKV_DTYPE_BF16, false>;
+static int od_launch(OctDecodeArgs a, unsigned grid, int q_dtype, int groups, hipStream_t st) {
+  constexpr bool F16 = true;
+  auto pick = [&](auto f16) {
+    constexpr int DT = decltype(f16)::value ? TTKV_DTYPE_F16 : TTKV_DTYPE_BF16;
+    if constexpr (W == 4)
+      if (groups == 2 && !(D == 256 && DT == TTKV_DTYPE_F16))
+        return octet_decode_kernel<D, W, DT, true, D == 256 && DT == TTKV_DTYPE_F16 ? 1 : 2>;
+    return groups ? octet_decode_kernel<D, W, DT, true, 1> : octet_decode_kernel<D, W, DT, false, 1>;
+  };
+  auto kernel = q_dtype == TTKV_DTYPE_F16 ? pick(std::bool_constant<F16>{}) : pick(std::bool_constant<!F16>{});
+  const int smem = W * kODRows * std::max(groups, 1) * (D + 4) * 4;
   if (smem > 65536 - 4096)
     if (int rc = raise_smem_limit((const void*)kernel, smem)) return rc;
-  int& resident = od_resident[D / 128][W > 4][q_dtype == TTKV_DTYPE_F16][chunk];
+  int& resident = od_resident[D / 128][W > 4][q_dtype == TTKV_DTYPE_F16][groups];
   if (!resident) {
     int per = 0;
     if (hipOccupancyMaxActiveBlocksPerMultiprocessor(&per, kernel, 64 * W, smem) != hipSuccess) per = 1;
@@ -676,10 +756,11 @@ static int od_launch(OctDecodeArgs a, unsigned grid, int q_dtype, bool chunk, hi
     return host_fail(TTKV_E_LAUNCH, std::string("octet decode launch: ") + hipGetErrorString(e));
   return TTKV_OK;
 }
+// groups: of 16 rows in a block; 0 where a request has one query.
 template <int D>
-static int od_launch(const OctDecodeArgs& a, int waves, unsigned grid, int q_dtype, bool chunk, hipStream_t st) {
-  if (waves == 4) return od_launch<D, 4>(a, grid, q_dtype, chunk, st);
-  return od_launch<D, D == 256 ? 4 : 8>(a, grid, q_dtype, chunk, st);
+static int od_launch(const OctDecodeArgs& a, int waves, unsigned grid, int q_dtype, int groups, hipStream_t st) {
+  if (waves == 4) return od_launch<D, 4>(a, grid, q_dtype, groups, st);
+  return od_launch<D, D == 256 ? 4 : 8>(a, grid, q_dtype, groups, st);
 }
 
 int octet_decode_paged(int H, int HQ, int d, float scale, const void* q, int q_dtype, int64_t q_row_stride,
@@ -708,7 +789,8 @@ int octet_decode_paged(int H, int HQ, int d, float scale, const void* q, int q_d
     return host_fail(TTKV_E_WORKSPACE, "decode workspace needs " + std::to_string(need) + " bytes, 256-aligned");
   if (num_reqs == 0 || num_tokens == 0 || max_q == 0) return TTKV_OK;
   if (window >= max_seq) window = 0;  // no window
-  const int rows = HQ / H * max_q, blocks = (rows + kODRows - 1) / kODRows;
+  const int rows = HQ / H * max_q, groups = od_groups(H, d, q_dtype, num_reqs, rows);
+  const int blocks = (rows + kODRows * groups - 1) / (kODRows * groups);
   const int slice = od_slice(H, blocks, num_reqs);
   const int64_t parts = od_parts(d, (int64_t)slice * H * blocks, max_seq);
   OctDecodeArgs a{};
@@ -731,7 +813,7 @@ int octet_decode_paged(int H, int HQ, int d, float scale, const void* q, int q_d
   a.out_dtype = out_dtype;
   a.out_row_stride = out_row_stride;
   a.lse = lse;
-  a.part_rows = std::min(rows, kODRows);
+  a.part_rows = std::min(rows, kODRows * groups);
   a.ws_cnt = (int*)ws;
   a.ws_o = (float*)((char*)ws + kCounterBytes);
   a.ws_ml = a.ws_o + parts * a.part_rows * d;
@@ -746,12 +828,12 @@ int octet_decode_paged(int H, int HQ, int d, float scale, const void* q, int q_d
     // an item per (block, head), and what the split ones have more
     const int64_t pairs = (int64_t)a.num_reqs * H * blocks;
     a.cnt_stride = (int)std::max<int64_t>(1, std::min<int64_t>(32, kMaxCounters / pairs));
-    const int waves = od_waves(d, pairs, max_seq, max_q, window), target = od_target(d, waves);
+    const int waves = od_waves(d, pairs, max_seq, max_q, window, groups), target = od_target(d, waves);
     a.by_target = 1.f / (float)target;
     const unsigned grid = (unsigned)((std::min(pairs + target, pairs * od_max_chunks(max_seq)) + H - 1) / H);
-    const int rc = d == 64    ? od_launch<64>(a, waves, grid, q_dtype, max_q > 1, st)
-                   : d == 128 ? od_launch<128>(a, waves, grid, q_dtype, max_q > 1, st)
-                              : od_launch<256>(a, waves, grid, q_dtype, max_q > 1, st);
+    const int rc = d == 64    ? od_launch<64>(a, waves, grid, q_dtype, max_q > 1 ? groups : 0, st)
+                   : d == 128 ? od_launch<128>(a, waves, grid, q_dtype, max_q > 1 ? groups : 0, st)
+                              : od_launch<256>(a, waves, grid, q_dtype, max_q > 1 ? groups : 0, st);
     if (rc != TTKV_OK) return rc;
   }
   return TTKV_OK;
