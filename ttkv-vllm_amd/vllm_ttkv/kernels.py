@@ -737,7 +737,7 @@ def nibble_prefill_paged(lay: NibbleLayout, query: torch.Tensor, page: torch.Ten
 # ---------------------------------------------------------------- the 8-bit cache
 def _turns(rotary, d, device_index, positions, N):
     """(positions, turns, rotary_dim, amplitude, adjacent) as the C entries take them."""
-    turns = rotary.turns
+    turns, amplitude, adjacent = rotary
     if turns.dtype != torch.float64 or turns.dim() != 1 or not turns.is_contiguous():
         raise ValueError("rotary.turns must be a contiguous fp64 tensor, one per pair")
     if turns.get_device() != device_index:
@@ -749,8 +749,25 @@ def _turns(rotary, d, device_index, positions, N):
     if positions is None or positions.dtype != torch.int64 or positions.dim() != 1 \
             or positions.numel() < N or not positions.is_contiguous():
         raise ValueError(f"positions must be contiguous int64, one per token ({N})")
-    return positions.data_ptr(), turns.data_ptr(), rot, float(rotary.amplitude), \
-        int(bool(rotary.adjacent))
+    return positions.data_ptr(), turns.data_ptr(), rot, float(amplitude), bool(adjacent)
+
+
+def _octet_page(page, lay):
+    """(pointer, slots, bytes per slot) of an 8-bit cache."""
+    if not page.is_contiguous():
+        raise ValueError("the cache page must be contiguous")
+    return _page_args(page, lay.compressed_bytes_per_token())
+
+
+def _row_stride(t, shape, dtype, what):
+    """The row stride of a tensor that must have this shape [N, heads, d] and dtype, rows contiguous
+    within a token; each thing is looked at once, since small calls are bound by their host time."""
+    if t.shape != shape or t.dtype != dtype:
+        raise ValueError(f"{what} must be {list(shape)} of dtype {dtype}, got {t.dtype} {list(t.shape)}")
+    if t.is_contiguous():
+        return shape[1] * shape[2]
+    _rows(t, shape[1], shape[2], what)
+    return t.stride(0)
 
 
 def rotary_scaled(query: torch.Tensor, key: torch.Tensor | None, positions: torch.Tensor,
@@ -760,32 +777,30 @@ def rotary_scaled(query: torch.Tensor, key: torch.Tensor | None, positions: torc
     `rotary`'s frequencies; returns (query_out, key_out), each of which may be its input. See
     `ttkv_rotary_scaled` in include/ttkv_hip.h."""
     index = _one_device(query, key, positions, query_out, key_out, error_word)
-    if query.dim() != 3:
-        raise ValueError(f"query must be [N, heads, d], got {tuple(query.shape)}")
-    N, HQ, d = query.shape
+    shape, dtype = query.shape, query.dtype
+    if len(shape) != 3:
+        raise ValueError(f"query must be [N, heads, d], got {tuple(shape)}")
+    N, HQ, d = shape
     turned = _turns(rotary, d, index, positions, N)
-    if query.dtype not in _hip.DTYPE_CODE:
+    code = _hip.DTYPE_CODE.get(dtype)
+    if code is None:
         raise ValueError("query dtype must be fp32, fp16 or bf16")
     query_out = torch.empty_like(query) if query_out is None else query_out
-    H = 0
+    q_stride = _row_stride(query, shape, dtype, "query")
+    qo_stride = _row_stride(query_out, shape, dtype, "query_out")
+    H = k = ko = k_stride = ko_stride = 0
     if key is not None:
-        H = key.shape[1] if key.dim() == 3 else 0
         key_out = torch.empty_like(key) if key_out is None else key_out
-    dtype = query.dtype
-    for t, heads, what in ((query, HQ, "query"), (query_out, HQ, "query_out"), (key, H, "key"),
-                           (key_out, H, "key_out")):
-        if t is None:
-            continue
-        _rows(t, heads, d, what)
-        if t.shape[0] != N or t.dtype != dtype:
-            raise ValueError(f"{what} must have the query's {N} tokens and dtype")
+        H = key.shape[1] if key.dim() == 3 else 0
+        k_stride = _row_stride(key, (N, H, d), dtype, "key")
+        ko_stride = _row_stride(key_out, (N, H, d), dtype, "key_out")
+        k, ko = key.data_ptr(), key_out.data_ptr()
     err = _error_word(error_word, query.device)
-    rc = _on_device(
-        index, _hip.lib().ttkv_rotary_scaled, query.data_ptr(), _hip.ptr(key),
-        query_out.data_ptr(), _hip.ptr(key_out), _hip.DTYPE_CODE[dtype], N, HQ, H, d,
-        query.stride(0), 0 if key is None else key.stride(0), query_out.stride(0),
-        0 if key is None else key_out.stride(0), *turned, err.data_ptr(), _stream(index))
-    _hip.check(rc, "ttkv_rotary_scaled")
+    rc = _on_device(index, _hip.lib().ttkv_rotary_scaled, query.data_ptr(), k, query_out.data_ptr(),
+                    ko, code, N, HQ, H, d, q_stride, k_stride, qo_stride, ko_stride, *turned,
+                    err.data_ptr(), _stream(index))
+    if rc:
+        _hip.check(rc, "ttkv_rotary_scaled")
     return query_out, key_out
 
 
@@ -804,50 +819,45 @@ def octet_write_paged(lay: OctetLayout, key: torch.Tensor, value: torch.Tensor,
     [N, H, d], contiguous) receive what the slots then stand for. See `ttkv_octet_write_paged`."""
     index = _one_device(key, value, slot_mapping, page, positions, query, query_out, key_out,
                         value_out, error_word)
-    shape = key.shape
-    _rows(key, lay.H, lay.d, "key")
-    _rows(value, lay.H, lay.d, "value")
-    N = shape[0]
-    if value.shape[0] != N:
-        raise ValueError(f"{N} keys and {value.shape[0]} values")
-    k_code, v_code = _hip.DTYPE_CODE.get(key.dtype), _hip.DTYPE_CODE.get(value.dtype)
+    H, d = lay.H, lay.d
+    N = key.shape[0] if key.dim() else 0
+    shape, k_dtype, v_dtype = (N, H, d), key.dtype, value.dtype
+    k_code, v_code = _hip.DTYPE_CODE.get(k_dtype), _hip.DTYPE_CODE.get(v_dtype)
     if k_code is None or v_code is None:
         raise ValueError("key / value dtype must be fp32, fp16 or bf16")
+    k_stride = _row_stride(key, shape, k_dtype, "key")
+    v_stride = _row_stride(value, shape, v_dtype, "value")
     for t, what in ((key_out, "key_out"), (value_out, "value_out")):
         if t is not None and (t.shape != shape or t.dtype != torch.bfloat16
                               or not t.is_contiguous()):
-            raise ValueError(f"{what} must be contiguous bf16 [{N}, {lay.H}, {lay.d}]")
+            raise ValueError(f"{what} must be contiguous bf16 [{N}, {H}, {d}]")
     if slot_mapping.dtype != torch.int64 or slot_mapping.numel() < N \
             or not slot_mapping.is_contiguous():
         raise ValueError("slot_mapping must be contiguous int64 with one id per token")
-    if not page.is_contiguous():
-        raise ValueError("the cache page must be contiguous")
     turned, q_args = (0, 0, 0, 1.0, 0), (0, 0, 0, 0, 0, 0)
     if rotary is not None:
-        turned = _turns(rotary, lay.d, index, positions, N)
+        turned = _turns(rotary, d, index, positions, N)
     elif query is not None:
         raise ValueError("queries are taken to be rotated: they need `rotary`")
     if query is not None:
-        HQ = query.shape[1] if query.dim() == 3 else 0
-        query_out = torch.empty_like(query) if query_out is None else query_out
-        q_code = _hip.DTYPE_CODE.get(query.dtype)
+        q_dtype = query.dtype
+        q_code = _hip.DTYPE_CODE.get(q_dtype)
         if q_code is None:
             raise ValueError("query dtype must be fp32, fp16 or bf16")
-        for t, what in ((query, "query"), (query_out, "query_out")):
-            _rows(t, HQ, lay.d, what)
-            if t.shape[0] != N or t.dtype != query.dtype:
-                raise ValueError(f"{what} must have the {N} tokens and the query's dtype")
-        q_args = (query.data_ptr(), q_code, query.stride(0), HQ, query_out.data_ptr(),
-                  query_out.stride(0))
+        HQ = query.shape[1] if query.dim() == 3 else 0
+        query_out = torch.empty_like(query) if query_out is None else query_out
+        q_args = (query.data_ptr(), q_code, _row_stride(query, (N, HQ, d), q_dtype, "query"), HQ,
+                  query_out.data_ptr(), _row_stride(query_out, (N, HQ, d), q_dtype, "query_out"))
     elif query_out is not None:
         raise ValueError("query_out without a query")
     err = _error_word(error_word, key.device)
     rc = _on_device(
-        index, _hip.lib().ttkv_octet_write_paged, lay.H, lay.d, key.data_ptr(), k_code,
-        key.stride(0), value.data_ptr(), v_code, value.stride(0), slot_mapping.data_ptr(), N,
-        *_page_args(page, lay.compressed_bytes_per_token()), _hip.ptr(key_out),
-        _hip.ptr(value_out), *turned, *q_args, err.data_ptr(), _stream(index))
-    _hip.check(rc, "ttkv_octet_write_paged")
+        index, _hip.lib().ttkv_octet_write_paged, H, d, key.data_ptr(), k_code, k_stride,
+        value.data_ptr(), v_code, v_stride, slot_mapping.data_ptr(), N,
+        *_octet_page(page, lay), _hip.ptr(key_out), _hip.ptr(value_out), *turned, *q_args,
+        err.data_ptr(), _stream(index))
+    if rc:
+        _hip.check(rc, "ttkv_octet_write_paged")
     return query_out
 
 
@@ -871,30 +881,29 @@ def octet_read_paged(lay: OctetLayout, page: torch.Tensor, block_size: int,
     W, stride = _table(block_table, "[requests, max_blocks]")
     if block_table.shape[0] < B:
         raise ValueError(f"{B} requests need as many block table rows")
-    for t in (key_out, value_out):
-        if t is not None:
-            num_rows, dtype = t.shape[0], t.dtype
+    given = key_out if key_out is not None else value_out
+    if given is not None:
+        num_rows, dtype = given.shape[0], given.dtype
     if num_rows is None:
         raise ValueError("num_rows or an output must say how many rows there are")
-    key_out, value_out = (page.new_empty(num_rows, lay.H, lay.d, dtype=dtype) if t is None else t
-                          for t in (key_out, value_out))
     code = _hip.DTYPE_CODE.get(dtype)
     if code is None:
         raise ValueError("key_out / value_out dtype must be fp32, fp16 or bf16")
-    for t, what in ((key_out, "key_out"), (value_out, "value_out")):
-        _rows(t, lay.H, lay.d, what)
-        if t.shape[0] != num_rows or t.dtype != dtype:
-            raise ValueError("key_out and value_out must have the same rows and dtype")
-    if not page.is_contiguous():
-        raise ValueError("the cache page must be contiguous")
+    shape = (num_rows, lay.H, lay.d)
+    if key_out is None:
+        key_out = page.new_empty(shape, dtype=dtype)
+    if value_out is None:
+        value_out = page.new_empty(shape, dtype=dtype)
+    k_stride = _row_stride(key_out, shape, dtype, "key_out")
+    v_stride = _row_stride(value_out, shape, dtype, "value_out")
     err = _error_word(error_word, page.device)
     rc = _on_device(
-        index, _hip.lib().ttkv_octet_read_paged, lay.H, lay.d,
-        *_page_args(page, lay.compressed_bytes_per_token()), int(block_size),
-        block_table.data_ptr(), stride, W, row_start_loc.data_ptr(), _hip.ptr(first), B,
-        int(max_seq_len), num_rows, key_out.data_ptr(), key_out.stride(0), value_out.data_ptr(),
-        value_out.stride(0), code, err.data_ptr(), _stream(index))
-    _hip.check(rc, "ttkv_octet_read_paged")
+        index, _hip.lib().ttkv_octet_read_paged, lay.H, lay.d, *_octet_page(page, lay),
+        int(block_size), block_table.data_ptr(), stride, W, row_start_loc.data_ptr(),
+        _hip.ptr(first), B, int(max_seq_len), num_rows, key_out.data_ptr(), k_stride,
+        value_out.data_ptr(), v_stride, code, err.data_ptr(), _stream(index))
+    if rc:
+        _hip.check(rc, "ttkv_octet_read_paged")
     return key_out, value_out
 
 
@@ -924,10 +933,18 @@ def octet_decode_paged(lay: OctetLayout, query: torch.Tensor, page: torch.Tensor
     [N, HQ, d] with the requests' rows written."""
     index = _one_device(query, page, block_table, seq_lens, query_start_loc, sinks, out, lse,
                         workspace, error_word)
-    out, q_args, bt_args, out_args = _nibble_read(lay, query, page, block_table, seq_lens,
-                                                  query_start_loc, out)
-    N, HQ = query.shape[:2]
-    B = seq_lens.numel()
+    shape, q_dtype = query.shape, query.dtype
+    N, HQ = (shape[0], shape[1]) if len(shape) == 3 else (0, 0)
+    d, B = lay.d, seq_lens.numel()
+    q_stride = _row_stride(query, (N, HQ, d), q_dtype, "query")
+    out = torch.empty_like(query) if out is None else out
+    out_stride = _row_stride(out, shape, out.dtype, "out")
+    q_code, out_code = _NIBBLE_DTYPES.get(q_dtype), _NIBBLE_DTYPES.get(out.dtype)
+    if q_code is None or out_code is None:
+        raise ValueError(f"{'out' if q_code else 'query'} dtype must be fp16 or bf16")
+    W, bt_stride = _table(block_table, "[requests, max_blocks]")
+    _i32(seq_lens, "seq_lens")
+    _i32(query_start_loc, "query_start_loc")
     if block_table.shape[0] < B or query_start_loc.numel() < B + 1:
         raise ValueError(f"{B} sequence lengths need as many block table rows and one more "
                          f"query start")
@@ -937,15 +954,18 @@ def octet_decode_paged(lay: OctetLayout, query: torch.Tensor, page: torch.Tensor
     if lse is not None and (lse.dtype != torch.float32 or lse.shape != (N, HQ)
                             or not lse.is_contiguous()):
         raise ValueError(f"lse must be contiguous fp32 [{N}, {HQ}]")
+    page_args = _octet_page(page, lay)
     if N == 0:                                  # every request waits
         return out
     if workspace is None:
         workspace = octet_decode_workspace(lay, HQ, B, max_q_len, max_seq_len, query.device)
     err = _error_word(error_word, query.device)
     rc = _on_device(
-        index, _hip.lib().ttkv_octet_decode_paged, lay.H, HQ, lay.d, float(scale), *q_args[:3], N,
-        *q_args[3:], int(block_size), *bt_args, seq_lens.data_ptr(), query_start_loc.data_ptr(), B,
-        int(max_q_len), int(max_seq_len), min(int(window), 2 ** 31 - 1), _hip.ptr(sinks), *out_args, _hip.ptr(lse),
-        workspace.data_ptr(), workspace.numel(), err.data_ptr(), _stream(index))
-    _hip.check(rc, "ttkv_octet_decode_paged")
+        index, _hip.lib().ttkv_octet_decode_paged, lay.H, HQ, d, float(scale), query.data_ptr(), q_code,
+        q_stride, N, *page_args, int(block_size), block_table.data_ptr(), bt_stride, W,
+        seq_lens.data_ptr(), query_start_loc.data_ptr(), B, int(max_q_len), int(max_seq_len),
+        min(int(window), 2 ** 31 - 1), _hip.ptr(sinks), out.data_ptr(), out_code, out_stride,
+        _hip.ptr(lse), workspace.data_ptr(), workspace.numel(), err.data_ptr(), _stream(index))
+    if rc:
+        _hip.check(rc, "ttkv_octet_decode_paged")
     return out
