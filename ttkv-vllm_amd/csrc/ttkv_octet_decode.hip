@@ -71,6 +71,7 @@ struct OctDecodeArgs {
   float* ws_ml;      // [split items][part_rows][2]
   uint32_t o_bytes;  // size of ws_o
   int part_rows;     // rows of an item's partials
+  float by_H;            // 1 / H
   float by_target;       // 1 / the items that the plan aims at
   int resident;          // what the chip holds at once
   float join;            // what a chunk's join costs against a step
@@ -152,9 +153,8 @@ __device__ __forceinline__ OctPlan od_plan(const OctDecodeArgs& a) {
     }
   }
   OctPlan P{};
-  P.h = blockIdx.x;
   P.none = true;
-  const int it = blockIdx.y;
+  const int it = blockIdx.x;
   // Long chunks first, so that a compute unit's workgroups are not all long (64 of 100 to 3,000 keys: 46.2 us in
   // the batch's order, 43.6 so): classes by the chunk's eighth of C, in the batch's order within each. Not where
   // chunks are short or requests many, whose scans cost more (200 of 50 to 600: 34.3, 40.5).
@@ -175,7 +175,7 @@ __device__ __forceinline__ OctPlan od_plan(const OctDecodeArgs& a) {
 #pragma unroll
     for (int i = 0; i < kODPlanLanes; ++i) {
       if (64 * i >= a.num_reqs) break;
-      const int items = cls[i] == k ? rb[i] * nch[i] : 0;
+      const int items = cls[i] == k ? rb[i] * nch[i] * a.H : 0;
       if (!__builtin_amdgcn_ballot_w64(items > 0)) continue;
       const int incl = nib_scan(items), ex = carry + incl - items;
       const uint64_t hit = __builtin_amdgcn_ballot_w64(ex <= it && it < ex + items);
@@ -189,9 +189,19 @@ __device__ __forceinline__ OctPlan od_plan(const OctDecodeArgs& a) {
         P.s0 = __builtin_amdgcn_readlane(s0[i], ln);
         P.steps = __builtin_amdgcn_readlane(st[i], ln);
         P.nch = __builtin_amdgcn_readlane(nch[i], ln);
-        const int local = it - __builtin_amdgcn_readlane(ex, ln);
-        P.rb = od_div(local, P.nch, __builtin_amdgcn_rcpf((float)P.nch));
-        P.c = local - P.rb * P.nch;
+        const int local = it - __builtin_amdgcn_readlane(ex, ln), blocks = __builtin_amdgcn_readlane(rb[i], ln);
+        // Workgroups go to the eight XCDs in turn: the row blocks of a (chunk, KV head) lie eight items apart, so
+        // that they share its bytes in one L2 (of up to eight such units the last ones lie closer).
+        int unit = local;
+        if (blocks > 1) {
+          const int units = P.nch * a.H;
+          const int group = od_div(local, 8 * blocks, __builtin_amdgcn_rcpf(8.f * (float)blocks));
+          const int rest = local - group * 8 * blocks, wide = min(8, units - group * 8);
+          P.rb = od_div(rest, wide, __builtin_amdgcn_rcpf((float)wide));
+          unit = group * 8 + rest - P.rb * wide;
+        }
+        P.c = od_div(unit, a.H, a.by_H);
+        P.h = unit - P.c * a.H;
         break;
       }
       carry += __builtin_amdgcn_readlane(incl, 63);
@@ -750,7 +760,7 @@ static int od_launch(OctDecodeArgs a, unsigned grid, int q_dtype, int groups, hi
     resident = std::max(per, 1);
   }
   a.resident = std::max(resident * device_cu_count(), od_target(D, W));
-  hipLaunchKernelGGL(kernel, dim3(a.H, grid), dim3(64 * W), smem, st, a);
+  hipLaunchKernelGGL(kernel, dim3(grid), dim3(64 * W), smem, st, a);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess)
     return host_fail(TTKV_E_LAUNCH, std::string("octet decode launch: ") + hipGetErrorString(e));
@@ -830,7 +840,8 @@ int octet_decode_paged(int H, int HQ, int d, float scale, const void* q, int q_d
     a.cnt_stride = (int)std::max<int64_t>(1, std::min<int64_t>(32, kMaxCounters / pairs));
     const int waves = od_waves(d, pairs, max_seq, max_q, window, groups), target = od_target(d, waves);
     a.by_target = 1.f / (float)target;
-    const unsigned grid = (unsigned)((std::min(pairs + target, pairs * od_max_chunks(max_seq)) + H - 1) / H);
+    a.by_H = 1.f / (float)H;
+    const unsigned grid = (unsigned)std::min(pairs + target, pairs * od_max_chunks(max_seq));
     const int rc = d == 64    ? od_launch<64>(a, waves, grid, q_dtype, max_q > 1 ? groups : 0, st)
                    : d == 128 ? od_launch<128>(a, waves, grid, q_dtype, max_q > 1 ? groups : 0, st)
                               : od_launch<256>(a, waves, grid, q_dtype, max_q > 1 ? groups : 0, st);

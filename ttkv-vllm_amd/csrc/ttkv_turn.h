@@ -55,6 +55,20 @@ __device__ __forceinline__ float2v turn_at(const double* turns, int j, int64_t p
   return turn_place(p) ? float2v{c * amplitude, s * amplitude} : float2v{NAN, NAN};
 }
 
+// Eight consecutive elements, rounded once.
+template <int DT>
+__device__ __forceinline__ void turn_store8(void* p, int64_t i, const float v[8]) {
+  if constexpr (DT == TTKV_DTYPE_BF16) {  // (one conversion per pair; store_act8 rounds by integer operations)
+    typedef __bf16 bf8 __attribute__((ext_vector_type(8)));
+    bf8 w;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) w[k] = (__bf16)v[k];
+    *gblw((u32x4*)((uint16_t*)p + i)) = __builtin_bit_cast(u32x4, w);
+  } else {
+    store_act8<DT>(p, i, v);
+  }
+}
+
 // One token's rows in pieces of 8 elements: rows whose pieces are 16-byte aligned, pairs that lie in one
 // piece (adjacent) or in two. A thread keeps its piece's frequencies from head to head; kTurnBatch heads'
 // loads are in flight at a time, the first ones asked for before the angles are formed. Two of them (four:
@@ -120,8 +134,8 @@ __device__ __forceinline__ void turn_pieces(const TurnArgs& a, int64_t tok, int 
             v[i] = ok ? yi : NAN;
           }
         }
-        store_act8<DT>(dst, at + e0, u);
-        if (!ADJ) store_act8<DT>(dst, at + e1, v);
+        turn_store8<DT>(dst, at + e0, u);
+        if (!ADJ) turn_store8<DT>(dst, at + e1, v);
       }
     }
     fetch(h0 + kTurnBatch * slots);
