@@ -23,7 +23,7 @@
 //     the rescale is a lane's factor.
 #include <math.h>
 
-#include <type_traits>
+#include <atomic>
 
 #include "ttkv_host.h"
 #include "ttkv_nibble.h"
@@ -38,6 +38,10 @@ constexpr int kODClasses = 8;          // of chunk lengths, for the items' order
 constexpr int kODRows = 16;            // rows of a block: a matrix product's columns
 constexpr float kODNone = -3.402823466e38f;  // the maximum before the first visible key
 constexpr float kODMost = 0x1p10f;     // a lane's sum of eight weights before the maximum moves
+// One query per request; several, whose rows are one block; or more blocks, whose bytes stay in the caches for
+// each other (6 x 5 queries of four query heads over 4,000 keys, d = 256: 25.1 us with loads that do not stay,
+// 23.3; where there is one block they cost: 30 x 3 over 200 to 4,000 30.1, 32.6).
+enum { kODSingle = 0, kODOwn = 1, kODShared = 2 };
 // What a chunk's join costs per row and dim against a step (1 x 14,000 tokens: 16.4 us with 6e-4, 14.1 so; 1 x
 // 60,000 of one KV head of eight query heads 70 without it, 19.4 so).
 constexpr float kODJoin = 9e-4f;
@@ -230,6 +234,12 @@ struct OctStep {
   uint32_t kp[2], vp[2];
 };
 
+// STREAM: a load that does not stay in the caches.
+template <bool STREAM, typename T>
+__device__ __forceinline__ T od_load(const T* p) {
+  return STREAM ? __builtin_nontemporal_load(gbl(p)) : *gbl(p);
+}
+
 // Four tokens' values of one dim, and of the next, from the tokens' pairs of those dims.
 __device__ __forceinline__ uint32_t od_low(bf16x2 a, bf16x2 b) {
   return __builtin_amdgcn_perm(__builtin_bit_cast(uint32_t, b), __builtin_bit_cast(uint32_t, a), 0x05040100u);
@@ -238,10 +248,11 @@ __device__ __forceinline__ uint32_t od_high(bf16x2 a, bf16x2 b) {
   return __builtin_amdgcn_perm(__builtin_bit_cast(uint32_t, b), __builtin_bit_cast(uint32_t, a), 0x07060302u);
 }
 
-template <int D, int W, int QDT, bool CHUNK, int RG>
+template <int D, int W, int QDT, int MODE, int RG>
 __global__ __launch_bounds__(64 * W, W > 4 ? W / 4 : D == 256 ? 3 - RG : D == 128 ? 2 : 5 - RG) void octet_decode_kernel(OctDecodeArgs a) {
   using F = Oct<D>;
   constexpr int N = F::kDims, KS = D / 32, PIECES = D / 64, PARTS = QDT == TTKV_DTYPE_F16 ? 2 : 1;
+  constexpr bool CHUNK = MODE != kODSingle;
   constexpr int kThreads = 64 * W, RB = kODRows * RG;
   constexpr int RS = D + 4;  // floats of a row in LDS: the rows' columns start in different banks
   extern __shared__ __align__(16) float red_all[];  // [waves][rows][RS]: the waves' results, then the join's
@@ -359,11 +370,11 @@ __global__ __launch_bounds__(64 * W, W > 4 ? W / 4 : D == 256 ? 3 - RG : D == 12
       const uint8_t* rec = record(k, t);
 #pragma unroll
       for (int p = 0; p < PIECES; ++p)
-        x.k[t][p] = __builtin_nontemporal_load(gbl((const u32x4*)(rec + 1024 * p + 16 * lane)));
+        x.k[t][p] = od_load<MODE != kODShared>((const u32x4*)(rec + 1024 * p + 16 * lane));
       if constexpr (D == 256)
-        x.kp[t] = __builtin_nontemporal_load(gbl((const uint16_t*)(rec + F::kKp) + lane));
+        x.kp[t] = od_load<MODE != kODShared>((const uint16_t*)(rec + F::kKp) + lane);
       else
-        x.kp[t] = __builtin_nontemporal_load(gbl(rec + F::kKp + (D == 64 ? (lane >> 5) * 16 + col : lane)));
+        x.kp[t] = od_load<MODE != kODShared>(rec + F::kKp + (D == 64 ? (lane >> 5) * 16 + col : lane));
     }
   };
   auto load_values = [&](int k, OctStep<D>& x) {
@@ -372,8 +383,8 @@ __global__ __launch_bounds__(64 * W, W > 4 ? W / 4 : D == 256 ? 3 - RG : D == 12
       const uint8_t* rec = record(k, t);
 #pragma unroll
       for (int p = 0; p < PIECES; ++p)
-        x.v[t][p] = __builtin_nontemporal_load(gbl((const u32x4*)(rec + F::kV + 1024 * p + 16 * lane)));
-      x.vp[t] = __builtin_nontemporal_load(gbl((const uint32_t*)(rec + F::kVp + col * N / 32 * 16) + q4));
+        x.v[t][p] = od_load<MODE != kODShared>((const u32x4*)(rec + F::kV + 1024 * p + 16 * lane));
+      x.vp[t] = od_load<MODE != kODShared>((const uint32_t*)(rec + F::kVp + col * N / 32 * 16) + q4);
     }
   };
   auto load = [&](int k, OctStep<D>& x) {
@@ -737,40 +748,42 @@ int64_t octet_decode_workspace_bytes(int H, int HQ, int d, int num_reqs, int max
   return kCounterBytes + (int64_t)2 * 2 * device_cu_count() * 2 * kODRows * (d + 2) * 4;
 }
 
-static int od_resident[3][2][2][3];  // workgroups per CU, by kernel (the same on every device of a process)
+template <int D, int W, int QDT>
+static auto od_kernel(int mode, int groups) {
+  if constexpr (W == 4 && !(D == 256 && QDT == TTKV_DTYPE_F16))
+    if (groups == 2) return octet_decode_kernel<D, W, QDT, kODOwn, 2>;
+  return mode == kODSingle ? octet_decode_kernel<D, W, QDT, kODSingle, 1>
+         : mode == kODOwn  ? octet_decode_kernel<D, W, QDT, kODOwn, 1>
+                           : octet_decode_kernel<D, W, QDT, kODShared, 1>;
+}
 
 template <int D, int W>
-static int od_launch(OctDecodeArgs a, unsigned grid, int q_dtype, int groups, hipStream_t st) {
-  constexpr bool F16 = true;
-  auto pick = [&](auto f16) {
-    constexpr int DT = decltype(f16)::value ? TTKV_DTYPE_F16 : TTKV_DTYPE_BF16;
-    if constexpr (W == 4)
-      if (groups == 2 && !(D == 256 && DT == TTKV_DTYPE_F16))
-        return octet_decode_kernel<D, W, DT, true, D == 256 && DT == TTKV_DTYPE_F16 ? 1 : 2>;
-    return groups ? octet_decode_kernel<D, W, DT, true, 1> : octet_decode_kernel<D, W, DT, false, 1>;
-  };
-  auto kernel = q_dtype == TTKV_DTYPE_F16 ? pick(std::bool_constant<F16>{}) : pick(std::bool_constant<!F16>{});
-  const int smem = W * kODRows * std::max(groups, 1) * (D + 4) * 4;
+static int od_launch(OctDecodeArgs a, unsigned grid, int q_dtype, int mode, int groups, hipStream_t st) {
+  auto kernel = q_dtype == TTKV_DTYPE_F16 ? od_kernel<D, W, TTKV_DTYPE_F16>(mode, groups)
+                                          : od_kernel<D, W, TTKV_DTYPE_BF16>(mode, groups);
+  const int smem = W * kODRows * groups * (D + 4) * 4;
   if (smem > 65536 - 4096)
     if (int rc = raise_smem_limit((const void*)kernel, smem)) return rc;
-  int& resident = od_resident[D / 128][W > 4][q_dtype == TTKV_DTYPE_F16][groups];
-  if (!resident) {
-    int per = 0;
-    if (hipOccupancyMaxActiveBlocksPerMultiprocessor(&per, kernel, 64 * W, smem) != hipSuccess) per = 1;
-    resident = std::max(per, 1);
+  // workgroups per CU, by kernel (the same on every device of a process; a race writes the same number)
+  static std::atomic<int> fit[2][4];
+  std::atomic<int>& known = fit[q_dtype == TTKV_DTYPE_F16][groups == 2 ? 3 : mode];
+  int per = known.load(std::memory_order_relaxed);
+  if (!per) {
+    if (hipOccupancyMaxActiveBlocksPerMultiprocessor(&per, kernel, 64 * W, smem) != hipSuccess || per < 1) per = 1;
+    known.store(per, std::memory_order_relaxed);
   }
-  a.resident = std::max(resident * device_cu_count(), od_target(D, W));
+  a.resident = std::max(per * device_cu_count(), od_target(D, W));
   hipLaunchKernelGGL(kernel, dim3(grid), dim3(64 * W), smem, st, a);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess)
     return host_fail(TTKV_E_LAUNCH, std::string("octet decode launch: ") + hipGetErrorString(e));
   return TTKV_OK;
 }
-// groups: of 16 rows in a block; 0 where a request has one query.
 template <int D>
-static int od_launch(const OctDecodeArgs& a, int waves, unsigned grid, int q_dtype, int groups, hipStream_t st) {
-  if (waves == 4) return od_launch<D, 4>(a, grid, q_dtype, groups, st);
-  return od_launch<D, D == 256 ? 4 : 8>(a, grid, q_dtype, groups, st);
+static int od_launch(const OctDecodeArgs& a, int waves, unsigned grid, int q_dtype, int mode, int groups,
+                     hipStream_t st) {
+  if (waves == 4) return od_launch<D, 4>(a, grid, q_dtype, mode, groups, st);
+  return od_launch<D, D == 256 ? 4 : 8>(a, grid, q_dtype, mode, groups, st);
 }
 
 int octet_decode_paged(int H, int HQ, int d, float scale, const void* q, int q_dtype, int64_t q_row_stride,
@@ -801,6 +814,7 @@ int octet_decode_paged(int H, int HQ, int d, float scale, const void* q, int q_d
   if (window >= max_seq) window = 0;  // no window
   const int rows = HQ / H * max_q, groups = od_groups(H, d, q_dtype, num_reqs, rows);
   const int blocks = (rows + kODRows * groups - 1) / (kODRows * groups);
+  const int mode = max_q == 1 ? kODSingle : blocks == 1 ? kODOwn : kODShared;
   const int slice = od_slice(H, blocks, num_reqs);
   const int64_t parts = od_parts(d, (int64_t)slice * H * blocks, max_seq);
   OctDecodeArgs a{};
@@ -842,9 +856,9 @@ int octet_decode_paged(int H, int HQ, int d, float scale, const void* q, int q_d
     a.by_target = 1.f / (float)target;
     a.by_H = 1.f / (float)H;
     const unsigned grid = (unsigned)std::min(pairs + target, pairs * od_max_chunks(max_seq));
-    const int rc = d == 64    ? od_launch<64>(a, waves, grid, q_dtype, max_q > 1 ? groups : 0, st)
-                   : d == 128 ? od_launch<128>(a, waves, grid, q_dtype, max_q > 1 ? groups : 0, st)
-                              : od_launch<256>(a, waves, grid, q_dtype, max_q > 1 ? groups : 0, st);
+    const int rc = d == 64    ? od_launch<64>(a, waves, grid, q_dtype, mode, groups, st)
+                   : d == 128 ? od_launch<128>(a, waves, grid, q_dtype, mode, groups, st)
+                              : od_launch<256>(a, waves, grid, q_dtype, mode, groups, st);
     if (rc != TTKV_OK) return rc;
   }
   return TTKV_OK;

@@ -79,11 +79,10 @@ constexpr int kTurnBatch = 2;
 template <int DT, bool ADJ, bool STREAM>
 __device__ __forceinline__ void turn_pieces(const TurnArgs& a, int64_t tok, int tid, int threads, float2v* cs) {
   constexpr int kFreqs = ADJ ? 4 : 8;  // of an item: a piece, or a pair of pieces
-  const int items = a.d / (ADJ ? 8 : 16), turned = a.half / kFreqs;
-  const int slots = threads / items, heads = a.heads[0] + a.heads[1];
-  const int slot = tid / items, p = tid - slot * items;
-  const bool copy = p >= turned;
-  const int e0 = ADJ ? 8 * p : copy ? 2 * a.half + 16 * (p - turned) : 8 * p, e1 = e0 + (copy ? 8 : a.half);
+  const int items = a.half / kFreqs, heads = a.heads[0] + a.heads[1];
+  const int slots = threads / items, slot = tid / items, p = tid - slot * items;
+  const int e0 = 8 * p, e1 = e0 + a.half;
+  const int rest = (a.d - 2 * a.half) >> 3;  // pieces of a head that are copied
   auto place = [&](int head, bool out, int64_t& at) -> const void* {
     const int set = head >= a.heads[0];
     at = tok * (out ? a.y_stride : a.x_stride)[set] + (int64_t)(set ? head - a.heads[0] : head) * a.d;
@@ -105,13 +104,40 @@ __device__ __forceinline__ void turn_pieces(const TurnArgs& a, int64_t tok, int 
   fetch(0);
   const int64_t pos = *gbl(a.pos + tok);
   const bool ok = turn_place(pos);
+  // Pieces that are copied, bit by bit (NaN where the position is refused), while the first ones to be turned
+  // and the frequencies arrive.
+  for (int i0 = tid; i0 < heads * rest; i0 += kTurnBatch * threads) {
+    Act8<DT> z[kTurnBatch];
+#pragma unroll
+    for (int b = 0; b < kTurnBatch; ++b) {
+      const int i = i0 + b * threads, head = i / rest;
+      int64_t at;
+      if (i < heads * rest) {
+        const void* src = place(head, false, at);
+        z[b] = load_act8<DT, STREAM>(src, at + 2 * a.half + (i - head * rest) * 8);
+      }
+    }
+#pragma unroll
+    for (int b = 0; b < kTurnBatch; ++b) {
+      const int i = i0 + b * threads, head = i / rest;
+      int64_t at;
+      if (i < heads * rest) {
+        char* dst = (char*)const_cast<void*>(place(head, true, at));
+        at += 2 * a.half + (i - head * rest) * 8;
+#pragma unroll
+        for (int j = 0; j < (DT == TTKV_DTYPE_F32 ? 2 : 1); ++j)
+          *gblw((u32x4*)(dst + at * (DT == TTKV_DTYPE_F32 ? 4 : 2)) + j) =
+              ok ? z[b].raw[j] : u32x4{0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu};
+      }
+    }
+  }
   for (int j = tid; j < a.half; j += threads) cs[j] = turn_at(a.turns, j, pos, a.amplitude);
   if (!ok && tid == 0) atomicOr(a.err, TTKV_ERR_BAD_POSITION);
   __syncthreads();
   float c[kFreqs], s[kFreqs];
 #pragma unroll
   for (int i = 0; i < kFreqs; ++i) {
-    const float2v w = cs[copy || slot >= slots ? 0 : kFreqs * p + i];
+    const float2v w = cs[kFreqs * p + i];
     c[i] = w[0];
     s[i] = w[1];
   }
@@ -129,10 +155,6 @@ __device__ __forceinline__ void turn_pieces(const TurnArgs& a, int64_t tok, int 
           const float ci = c[ADJ ? i / 2 : i], si = s[ADJ ? i / 2 : i];
           u[i] = ADJ && (i & 1) ? xi * ci + yi * si : xi * ci - yi * si;
           v[i] = yi * ci + xi * si;
-          if (copy) {
-            u[i] = ok ? xi : NAN;
-            v[i] = ok ? yi : NAN;
-          }
         }
         turn_store8<DT>(dst, at + e0, u);
         if (!ADJ) turn_store8<DT>(dst, at + e1, v);
