@@ -496,7 +496,8 @@ int ttkv_rotary_scaled(const void* query, const void* key, void* query_out, void
  * there are no queries. slot_mapping as for ttkv_write_paged: entries < 0 are padded tokens (not stored;
  * their queries are rotated and their positions looked at all the same), entries past the cache set
  * TTKV_ERR_BAD_SLOT; the slots of one call are distinct. key_out / value_out (optional, bf16 [N, H, d])
- * receive the values that the slots then stand for; rows of tokens that are not stored are left alone.
+ * receive the values that the slots then stand for (key_out may be the key, value_out the value, as they
+ * stand; outputs overlap nothing else); rows of tokens that are not stored are left alone.
  * A position outside [0, 2^31) sets TTKV_ERR_BAD_POSITION; its key is stored as NaN. */
 int ttkv_octet_write_paged(int32_t H, int32_t d, const void* key, int32_t k_dtype,
                            int64_t k_row_stride, const void* value, int32_t v_dtype,
@@ -509,7 +510,7 @@ int ttkv_octet_write_paged(int32_t H, int32_t d, const void* key, int32_t k_dtyp
 
 /* Stored keys and values back as rows, for dense attention over a stored prefix or another worker's
  * cache. Rows row_start_loc[r] .. [r + 1] - 1 of key_out / value_out [num_rows, H, d] (fp32, fp16 or
- * bf16; the stored value rounded once, exact in bf16) receive request r's tokens first[r], first[r] + 1,
+ * bf16; the stored value rounded once, exact in bf16; the two do not overlap) receive request r's tokens first[r], first[r] + 1,
  * ... (first null: from 0). Rows that no request has are left alone. A token outside [0, max_seq_len) or
  * a row outside [0, num_rows) sets TTKV_ERR_SEQ_LEN, a block id outside the cache TTKV_ERR_BAD_BLOCK;
  * such a token's row becomes NaN, such a row is not written. */
@@ -526,16 +527,18 @@ int ttkv_octet_read_paged(int32_t H, int32_t d, const uint8_t* page, int64_t n_s
  * the end of its n = seq_lens[r] stored keys, their own included. Query j, at position p = n - Q + j, sees
  * the keys t <= p and, with a window > 0, t > p - window:
  *   out[j] = sum_t softmax_t(scale * q[j] . K[t]) * V[t]
- * With sinks [num_heads] fp32 the softmax has one more term, exp(sinks[head]), that carries no value; lse
+ * With sinks [num_heads] fp32 (finite or -infinity) the softmax has one more term, exp(sinks[head]), that carries no value; lse
  * [num_tokens, num_heads] fp32 (optional) receives the logarithm of the softmax's sum, by which results
  * over parts of a context are joined. query and out [num_tokens, num_heads, d] fp16 or bf16, up to 16
- * query heads per KV head; `out` may be the query. Rows that no request has are left alone.
+ * query heads per KV head; `out` may be the query as it stands and otherwise does not overlap it. Rows that
+ * no request has are left alone.
  * A request with n == 0 has rows of 0 and an lse of -infinity, or the sink. One with 0 < n < Q sets
  * TTKV_ERR_SEQ_LEN and its rows become NaN; one with Q > max_q_len or n > max_seq_len sets it and has its
  * first max_q_len queries, or its first max_seq_len keys, taken; rows outside [0, num_tokens) set it and
  * are not taken. A block id outside the cache sets TTKV_ERR_BAD_BLOCK; rows that see the block become NaN,
- * and others of the request may. Keys, values and queries enter the products exactly, sums are in 32
- * bits; a score beyond fp32 makes its row NaN.
+ * and others of the request may. Keys, values and queries enter the products exactly (bf16
+ * queries below 2^-126 may count as 0), a softmax weight with 16 bits, sums are in 32 bits. A score beyond
+ * fp32 makes its row NaN; values beyond 2^100 may sum up beyond fp32.
  * max_seq_len at most 2^26 and at most the tokens that max_blocks hold; the page at most 2^31 tiles.
  *
  * Workspace: as for the 4-bit reads, and one buffer may serve them all, in stream order: 256-byte

@@ -191,6 +191,13 @@ def test_write_refusals():
         _refused(_write(**{a: 0}), 1, "null")
     _refused(_write(ko=8), 1, "key_out")
     _refused(_write(vo=24), 1, "value_out")
+    # outputs: bf16 rows of 2,048 bytes, four of them; the inputs are fp16 rows of as many
+    _refused(_write(ko=65536 + 2048), 1, "key_out or value_out overlaps")
+    _refused(_write(ko=65536, kt=0), 1, "key_out or value_out overlaps")
+    _refused(_write(ko=131072), 1, "key_out or value_out overlaps")
+    _refused(_write(vo=65536), 1, "key_out or value_out overlaps")
+    _refused(_write(vo=131072 - 16), 1, "key_out or value_out overlaps")
+    _refused(_write(ko=1 << 18, vo=(1 << 18) + 4096), 1, "key_out or value_out overlaps")
     rotated = dict(pos=64, turns=64, rot=128)
     _refused(_write(**dict(rotated, rot=130)), 1, "rotary dims")
     _refused(_write(**dict(rotated, rot=-2)), 1, "rotary dims")
@@ -202,12 +209,14 @@ def test_write_refusals():
     _refused(_write(**dict(asked, qo=(1 << 20) + 256)), 1, "overlaps the query")
     _refused(_write(**dict(asked, qo=65536)), 1, "overlaps the keys")
     _refused(_write(**dict(asked, qo=131072 + 512)), 1, "overlaps the keys")
+    _refused(_write(**dict(asked, ko=1 << 20)), 1, "overlaps the keys")
+    _refused(_write(**dict(asked, qo=1 << 21, vo=(1 << 20) + 2048)), 1, "overlaps the keys")
     assert _write(n=0) == 0
 
 
 def _read(**kw):
     a = dict(H=8, d=128, page=4096, n_slots=64, stride=2112, bs=16, bt=16, bts=4, mb=4, starts=16,
-             first=0, reqs=1, max_seq=64, rows=8, ko=16, ks=1024, vo=16, vs=1024, dt=2, err=16)
+             first=0, reqs=1, max_seq=64, rows=8, ko=1 << 16, ks=1024, vo=1 << 17, vs=1024, dt=2, err=16)
     a.update(kw)
     return _hip.lib().ttkv_octet_read_paged(*a.values(), None)
 
@@ -225,6 +234,8 @@ def test_read_refusals():
     _refused(_read(dt=3), 1, "dtype")
     for a in ("bt", "starts", "ko", "vo", "err"):
         _refused(_read(**{a: 0}), 1, "null")
+    _refused(_read(ko=1 << 16, vo=(1 << 16) + 2046), 1, "overlap")
+    _refused(_read(ko=1 << 16, vo=(1 << 16) - 16), 1, "overlap")
     assert _read(rows=0) == 0 and _read(reqs=0) == 0
 
 
@@ -253,6 +264,9 @@ def test_decode_refusals():
     _refused(_decode(q=24), 1, "16-byte")
     _refused(_decode(out=8), 1, "16-byte")
     _refused(_decode(qs=4100), 1, "16-byte")
+    _refused(_decode(q=65536, out=65536 + 8192), 1, "overlaps the query")
+    _refused(_decode(q=65536, out=65536, os=8192), 1, "overlaps the query")
+    _refused(_decode(q=65536, out=65536 - 16), 1, "overlaps the query")
     _refused(_decode(ws=0), 4, "workspace")
     _refused(_decode(ws=128), 4, "workspace")
     _refused(_decode(wsb=16), 4, "workspace")

@@ -263,6 +263,14 @@ def test_write_in_place_queries_and_waiting():
     out = kernels.octet_write_paged(lay, k, v, torch.arange(6).cuda(), page, rotary=r, positions=pos,
                                     query=q, query_out=q)
     assert out is q and torch.equal(q, want)
+    ko, vo = k.clone(), v.clone()                       # the stored values in the inputs' place
+    for rotary in (r, None):
+        want = torch.empty_like(k)
+        kw = dict(rotary=rotary, positions=pos) if rotary else {}
+        kernels.octet_write_paged(lay, k, v, torch.arange(6).cuda(), page, key_out=want, **kw)
+        ko.copy_(k), vo.copy_(v)
+        kernels.octet_write_paged(lay, ko, vo, torch.arange(6).cuda(), page, key_out=ko, value_out=vo, **kw)
+        assert torch.equal(ko, want) and torch.equal(vo.cpu().double(), oo.values(v.cpu()))
     before = page.clone()
     kernels.octet_write_paged(lay, k[:0], v[:0], torch.arange(0).cuda(), page)
     assert torch.equal(page, before)

@@ -807,6 +807,9 @@ int octet_decode_paged(int H, int HQ, int d, float scale, const void* q, int q_d
     return host_fail(TTKV_E_INVALID, "null pointer argument");
   if (((uintptr_t)q | (uintptr_t)out) % 16 || q_row_stride % 8 || out_row_stride % 8)
     return host_fail(TTKV_E_INVALID, "query / out rows must be 16-byte aligned");
+  if (q && out && !(out == q && (out_row_stride == q_row_stride || num_tokens == 1)) &&
+      rows_meet(out, 2 * out_row_stride, 2ll * HQ * d, q, 2 * q_row_stride, 2ll * HQ * d, num_tokens))
+    return host_fail(TTKV_E_INVALID, "out overlaps the query without being it");
   const int64_t need = octet_decode_workspace_bytes(H, HQ, d, num_reqs, max_q, max_seq);
   if (!ws || ws_bytes < need || (uintptr_t)ws % 256)
     return host_fail(TTKV_E_WORKSPACE, "decode workspace needs " + std::to_string(need) + " bytes, 256-aligned");

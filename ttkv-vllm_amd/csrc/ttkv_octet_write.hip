@@ -276,17 +276,32 @@ int octet_write_paged(int H, int d, const void* key, int k_dtype, int64_t k_row_
     return host_fail(TTKV_E_INVALID, "key_out / value_out must be 16-byte aligned");
   if (rot)
     if (int rc = turn_check(pos, turns, rot, d)) return rc;
+  // Rows are read while others are written: key_out may be the key as it stands, value_out the value, and
+  // nothing else overlaps.
+  const int64_t kb = k_dtype == TTKV_DTYPE_F32 ? 4 : 2, vb = v_dtype == TTKV_DTYPE_F32 ? 4 : 2, row = (int64_t)H * d;
+  auto meets = [&](const void* y, int64_t ys, int64_t width, const void* x, int64_t xs, int64_t xw) {
+    return rows_meet(y, ys, width, x, xs, xw, num_tokens);
+  };
+  auto same = [&](const void* y, const void* x, int64_t xs, int64_t xb) {
+    return y == x && xb == 2 && (xs == row || num_tokens == 1);
+  };
+  if ((k_out && !same(k_out, key, k_row_stride, kb) && meets(k_out, 2 * row, 2 * row, key, k_row_stride * kb, row * kb)) ||
+      (v_out && !same(v_out, val, v_row_stride, vb) && meets(v_out, 2 * row, 2 * row, val, v_row_stride * vb, row * vb)) ||
+      meets(k_out, 2 * row, 2 * row, val, v_row_stride * vb, row * vb) ||
+      meets(v_out, 2 * row, 2 * row, key, k_row_stride * kb, row * kb) ||
+      meets(k_out, 2 * row, 2 * row, v_out, 2 * row, 2 * row))
+    return host_fail(TTKV_E_INVALID, "key_out or value_out overlaps the keys, the values or the other");
   if (HQ) {
     if (!act_dtype(q_dtype)) return host_fail(TTKV_E_INVALID, "query dtype must be fp32, fp16 or bf16");
     if (!q || !qo) return host_fail(TTKV_E_INVALID, "null pointer argument");
     const int64_t eb = q_dtype == TTKV_DTYPE_F32 ? 4 : 2, qw = (int64_t)HQ * d * eb;
     if (turn_clash(q, q_stride, qo, qo_stride, qw, eb, num_tokens))
       return host_fail(TTKV_E_INVALID, "query_out overlaps the query without being it");
-    // (keys and values are read while queries are written)
-    const int64_t kb = k_dtype == TTKV_DTYPE_F32 ? 4 : 2, vb = v_dtype == TTKV_DTYPE_F32 ? 4 : 2;
-    if (rows_meet(qo, qo_stride * eb, qw, key, k_row_stride * kb, (int64_t)H * d * kb, num_tokens) ||
-        rows_meet(qo, qo_stride * eb, qw, val, v_row_stride * vb, (int64_t)H * d * vb, num_tokens))
-      return host_fail(TTKV_E_INVALID, "query_out overlaps the keys or values");
+    if (meets(qo, qo_stride * eb, qw, key, k_row_stride * kb, row * kb) ||
+        meets(qo, qo_stride * eb, qw, val, v_row_stride * vb, row * vb) ||
+        meets(qo, qo_stride * eb, qw, k_out, 2 * row, 2 * row) || meets(qo, qo_stride * eb, qw, v_out, 2 * row, 2 * row) ||
+        meets(q, q_stride * eb, qw, k_out, 2 * row, 2 * row) || meets(q, q_stride * eb, qw, v_out, 2 * row, 2 * row))
+      return host_fail(TTKV_E_INVALID, "query_out overlaps the keys or values, or the query their outputs");
   }
   const int64_t tokens = 1024 / d, blocks = (num_tokens + tokens - 1) / tokens * H;
   if (blocks > 0x3fffffff) return host_fail(TTKV_E_INVALID, "too many tokens for one call");
