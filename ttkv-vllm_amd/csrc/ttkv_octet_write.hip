@@ -3,7 +3,14 @@
 //
 // A workgroup of 256 threads takes the keys and values of 1024 / d tokens of one head, 8 dims a thread:
 // a group of 32 dims is 4 neighbouring lanes. Tokens of one workgroup that follow each other in a tile
-// write whole 128-byte lines of its record.
+// write whole 128-byte lines of its record. Rotated keys go from the turn into the quantisation in 32 bits,
+// and the queries' workgroups run beside the others in the same launch: a decode step needs one call for both.
+//
+// Kernels in graph replays: 8 tokens of 8 KV and 32 query heads, rotated, 3.5 us (a launch that does nothing
+// 2.0); 2,048 tokens of 8 heads that come rotated, stored values returned, 21 MB, 5.8 us, one chain of slot, row
+// and store over a full chip; 3,321 tokens of 4 heads of 256 dims and 16 query heads, rotated, 75 MB, 18.5 us,
+// 4.1 TB/s with vector issue at 67 %. The kernel without a rotation is one of its own: it has 20 registers where
+// the queries' code takes 84 (2,048 tokens 6.7 us with it).
 #include <math.h>
 
 #include "ttkv_host.h"
@@ -56,7 +63,8 @@ __global__ __launch_bounds__(256) void octet_write_kernel(OctWriteArgs a) {
   const int64_t stride = val ? a.v_row_stride : a.k_row_stride, at = tok * stride + (int64_t)h * D;
   const bool vec = act_rows_aligned(src, dt, stride);
   const int half = TURN ? a.turn.half : 0;
-  // a lane's dims and the others of their pairs, in a piece of 8 where the halves are made of such
+  // a lane's dims and, in a piece of 8 where the halves are made of such, the others of their pairs: a second
+  // load, asked for with the first (through LDS and a token's table at a time 8 x 1 tokens took 6.2 us, 3.5 so)
   const bool whole = a.turn.adjacent || half % 8 == 0, mated = !val && !a.turn.adjacent && whole && 8 * i < 2 * half;
   const int mate = 8 * i < half ? 8 * i + half : 8 * i - half;
   float x[8] = {}, y[8] = {};
