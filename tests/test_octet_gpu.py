@@ -104,7 +104,7 @@ def test_rotary_strides_and_in_place(dtype, pad, shift):
     q = flat[shift:].as_strided((N, HQ, d), (HQ * d + pad, d, 1))
     before = flat.clone()
     pos = torch.randint(0, 5000, (N,), generator=g)
-    for adjacent, rot in ((False, 128), (True, 64), (False, 48)):
+    for adjacent, rot in ((False, 128), (True, 64), (False, 48), (False, 64)):
         r = scaled_rotary(rot, adjacent=adjacent)
         dev = r._replace(turns=r.turns.cuda())
         x = q.cpu().clone()

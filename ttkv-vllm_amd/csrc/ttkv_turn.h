@@ -106,8 +106,9 @@ __device__ __forceinline__ void turn_pieces(const TurnArgs& a, int64_t tok, int 
   const int64_t pos = *gbl(a.pos + tok);
   const bool ok = turn_place(pos);
   // Pieces that are copied, bit by bit (NaN where the position is refused), while the first ones to be turned
-  // and the frequencies arrive.
-  for (int i0 = tid; i0 < heads * rest; i0 += kTurnBatch * threads) {
+  // and the frequencies arrive; none in place.
+  const bool in_place = ok && a.x[0] == a.y[0] && a.x[1] == a.y[1];
+  for (int i0 = in_place ? heads * rest : tid; i0 < heads * rest; i0 += kTurnBatch * threads) {
     Act8<DT> z[kTurnBatch];
 #pragma unroll
     for (int b = 0; b < kTurnBatch; ++b) {

@@ -756,7 +756,12 @@ def _octet_page(page, lay):
     """(pointer, slots, bytes per slot) of an 8-bit cache."""
     if not page.is_contiguous():
         raise ValueError("the cache page must be contiguous")
-    return _page_args(page, lay.compressed_bytes_per_token())
+    last = page.shape[-1] if page.dim() > 1 else 0
+    row = last * page.element_size()
+    if row < lay.compressed_bytes_per_token():
+        raise ValueError(f"the cache row is {row} bytes but the layout needs "
+                         f"{lay.compressed_bytes_per_token()}")
+    return page.data_ptr(), page.numel() // last, row
 
 
 def _row_stride(t, shape, dtype, what):

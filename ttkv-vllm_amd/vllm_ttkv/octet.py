@@ -26,6 +26,7 @@ class OctetLayout:
             raise ValueError(f"H={self.H} KV heads")
         if self.d not in (64, 128, 256):
             raise ValueError(f"head dim {self.d}: the 8-bit cache is built for 64, 128 and 256")
+        object.__setattr__(self, "_slot", 2 * self.H * self.row_bytes)   # (asked for by every call)
 
     @property
     def row_bytes(self) -> int:
@@ -33,7 +34,7 @@ class OctetLayout:
         return self.d + self.d // GROUP
 
     def compressed_bytes_per_token(self) -> int:
-        return 2 * self.H * self.row_bytes
+        return self._slot
 
     def dense_bytes_per_token(self) -> int:
         return 2 * self.H * self.d * 2
