@@ -527,9 +527,9 @@ int ttkv_octet_read_paged(int32_t H, int32_t d, const uint8_t* page, int64_t n_s
  * the end of its n = seq_lens[r] stored keys, their own included. Query j, at position p = n - Q + j, sees
  * the keys t <= p and, with a window > 0, t > p - window:
  *   out[j] = sum_t softmax_t(scale * q[j] . K[t]) * V[t]
- * With sinks [num_heads] fp32 (finite or -infinity) the softmax has one more term, exp(sinks[head]), that carries no value; lse
- * [num_tokens, num_heads] fp32 (optional) receives the logarithm of the softmax's sum, by which results
- * over parts of a context are joined. query and out [num_tokens, num_heads, d] fp16 or bf16, up to 16
+ * With sinks [num_heads] fp32 (finite or -infinity) the softmax has one more term, exp(sinks[head]), that
+ * carries no value; lse [num_tokens, num_heads] fp32 (optional) receives the logarithm of the softmax's sum,
+ * by which results over parts of a context are joined. query and out [num_tokens, num_heads, d] fp16 or bf16, up to 16
  * query heads per KV head; `out` may be the query as it stands and otherwise does not overlap it. Rows that
  * no request has are left alone.
  * A request with n == 0 has rows of 0 and an lse of -infinity, or the sink. One with 0 < n < Q sets
@@ -542,8 +542,8 @@ int ttkv_octet_read_paged(int32_t H, int32_t d, const uint8_t* page, int64_t n_s
  * max_seq_len at most 2^26 and at most the tokens that max_blocks hold; the page at most 2^31 tiles.
  *
  * Workspace: as for the 4-bit reads, and one buffer may serve them all, in stream order: 256-byte
- * aligned, its first 64 KiB zero before its first call and left zero by every call; the size grows with
- * every argument but H, whose largest counts. Results do not depend on what it held, and repeat bit for bit. */
+ * aligned, its first 64 KiB zero before its first call and left zero by every call; its size grows with
+ * every argument; calls that may overlap take one each. Results do not depend on what it held, and repeat bit for bit. */
 int64_t ttkv_octet_decode_workspace_bytes(int32_t H, int32_t num_heads, int32_t d,
                                           int32_t num_reqs, int32_t max_q_len,
                                           int32_t max_seq_len);

@@ -336,6 +336,24 @@ def test_read_rows(dtype, d, H, block, pad):
         assert torch.equal(out[i].cpu(), want[i].to(dtype))
 
 
+@pytest.mark.parametrize("H,d", [(1, 64), (3, 128)])
+def test_read_many_requests(H, d):
+    """More requests than a wave looks at together, many of them empty; heads that share no wave evenly."""
+    lens = [(7 * i) % 53 if i % 3 else 0 for i in range(200)]
+    st = Store(lens, H, d, seed=4)
+    starts = [0]
+    for n in lens:
+        starts.append(starts[-1] + n)
+    k, v = kernels.octet_read_paged(st.lay, st.page, 16, st.bt, _i32(starts), max(lens), num_rows=starts[-1])
+    assert torch.equal(k.cpu().double(), oo.values(st.k)) and torch.equal(v.cpu().double(), oo.values(st.v))
+    # two requests that name the same rows, more than the rows' own number: in bounds, and one of them is there
+    err = _err()
+    k, _ = kernels.octet_read_paged(st.lay, st.page, 16, st.bt[[1, 2, 4]], _i32([0, 7, 0, 14]), 53, num_rows=14,
+                                    error_word=err)
+    assert int(err) == 8
+    assert torch.equal(k[7:].cpu().double(), st.kv(4)[0][7:14])
+
+
 def test_read_strides_and_defaults():
     st = Store([70, 5], 2, 128)
     k, v = kernels.octet_read_paged(st.lay, st.page, 16, st.bt, _i32([0, 70, 75]), 70, num_rows=75)
