@@ -5,8 +5,8 @@
 // of at most one revolution is off by 2^-53 of itself, 2^-22 of a revolution at worst and less than fp32
 // resolves where frequencies are those of a model (1 / (2 pi) at most). Whole and quarter revolutions are
 // taken off exactly; what is left, at most an eighth, goes to radians and to fp32 and into the Taylor
-// series of the sine and the cosine. Bound by memory: 8,192 tokens of 40 heads of 128 in bf16, 168 MB, 31 us,
-// 5.4 TB/s; 8 tokens 2.8 us in a graph, where a launch that does nothing takes 2.0.
+// series of the sine and the cosine. Bound by memory: 8,192 tokens of 40 heads of 128 in bf16, 168 MB, 31 us
+// (pairs in two halves; adjacent 32), 5.4 TB/s; 8 tokens 2.8 us in a graph, where a launch that does nothing takes 2.0.
 #pragma once
 
 #include <type_traits>
@@ -56,8 +56,9 @@ __device__ __forceinline__ float2v turn_at(const double* turns, int j, int64_t p
   return turn_place(p) ? float2v{c * amplitude, s * amplitude} : float2v{NAN, NAN};
 }
 
-// 16 bytes of a row, by a store that does not stay in the cache: rows are whole lines, and drain while others are
-// turned (40 heads of 128 in bf16: 512 tokens 3.8 us with stores that stay, 3.5 so; 4,096 15.8, 15.0).
+// 16 bytes of a row, by a store that does not stay in the caches: rows are whole lines, and drain while others
+// are turned (40 heads of 128 in bf16: 512 tokens 3.8 us with stores that stay, 3.5 so; 4,096 15.8, 15.0;
+// adjacent pairs, 8,192 tokens: 31.5, 31.8).
 __device__ __forceinline__ void turn_store16(void* p, u32x4 w) { __builtin_nontemporal_store(w, gblw((u32x4*)p)); }
 
 // Eight consecutive elements, rounded once by the hardware's conversions.
