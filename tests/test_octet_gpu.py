@@ -403,6 +403,29 @@ def test_read_refused_places():
     assert torch.equal(out[0][:10].cpu().double(), st.kv(0)[0][5:15]) and bool((out[0][10:] == 7).all())
 
 
+@pytest.mark.parametrize("starts,rows", [
+    ([-2 ** 31, -2 ** 31 + 1], (0, 0)), ([-2 ** 31, -5], (0, 0)), ([-2 ** 31, 3], (0, 3)),
+    ([3, -2 ** 31], (0, 0)), ([2 ** 31 - 1, -5], (0, 0)), ([5, 2 ** 31 - 1], (5, 8)),
+    ([2 ** 30, 2 ** 31 - 1], (0, 0)), ([-2 ** 31, 2 ** 31 - 1], (0, 8))])
+def test_read_row_starts_at_the_ends_of_their_type(starts, rows):
+    """Only rows of the outputs are written; of tokens past the call's lengths, as NaN."""
+    st = Store([40], 1, 64)
+    out = [torch.full((24, 1, 64), 7.0, device="cuda") for _ in range(2)]
+    err = _err()
+    kernels.octet_read_paged(st.lay, st.page, 16, st.bt, _i32(starts), 40, key_out=out[0][8:16],
+                             value_out=out[1][8:16], error_word=err)
+    assert int(err) == 8
+    lo, hi = rows
+    for x, kept in zip(out, st.kv(0)):
+        got = x[8:16].cpu()
+        assert bool((x[:8] == 7).all()) and bool((x[16:] == 7).all())
+        assert bool((got[:lo] == 7).all()) and bool((got[hi:] == 7).all())
+        if starts[0] >= 0:
+            assert torch.equal(got[lo:hi].double(), kept[:hi - lo])
+        else:
+            assert bool(torch.isnan(got[lo:hi]).all())
+
+
 # ------------------------------------------------------------------------------------ decode
 def _close(got, lse, q, K, V, scale, what, **kw):
     want, wlse, spread, score = oo.attend(q, K, V, scale, **kw)

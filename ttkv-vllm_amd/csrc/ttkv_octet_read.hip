@@ -31,18 +31,18 @@ struct OctReadArgs {
 
 // A request's rows that the outputs hold, and the tiles of their tokens.
 struct OctReadRows {
-  int64_t t0;      // token of row k is t0 + k, in row row0 + k
+  int64_t t0;        // output row k holds token t0 + k,
   int row0, lo, hi;  // k in [lo, hi)
   int tile, tiles;
 };
 __device__ __forceinline__ OctReadRows oct_read_rows(const OctReadArgs& a, int r, bool& clipped) {
   OctReadRows x;
   x.row0 = a.starts[r];
-  const int64_t rows = (int64_t)a.starts[r + 1] - x.row0;
-  x.t0 = a.first ? a.first[r] : 0;
-  x.lo = max(0, -x.row0);
-  x.hi = (int)min(rows, (int64_t)a.num_rows - x.row0);
-  clipped = rows < 0 || (rows > 0 && (x.lo > 0 || x.hi < rows));
+  const int end = a.starts[r + 1];
+  x.t0 = (int64_t)(a.first ? a.first[r] : 0) - x.row0;
+  x.lo = max(0, x.row0);
+  x.hi = min(end, a.num_rows);
+  clipped = end < x.row0 || (end > x.row0 && (x.row0 < 0 || end > a.num_rows));
   x.tile = (int)((x.t0 + x.lo) >> 4);
   x.tiles = x.hi > x.lo ? (int)((x.t0 + x.hi - 1) >> 4) - x.tile + 1 : 0;
   return x;
@@ -98,7 +98,7 @@ __global__ __launch_bounds__(256) void octet_read_kernel(OctReadArgs a) {
         rq.row0 = __builtin_amdgcn_readlane(mine.row0, ln);
         rq.lo = __builtin_amdgcn_readlane(mine.lo, ln);
         rq.hi = __builtin_amdgcn_readlane(mine.hi, ln);
-        rq.t0 = a.first ? a.first[r] : 0;
+        rq.t0 = (int64_t)(a.first ? a.first[r] : 0) - rq.row0;
         rq.tile = __builtin_amdgcn_readlane(mine.tile, ln) + (int)at - __builtin_amdgcn_readlane(incl - mine.tiles, ln);
       }
       before += __builtin_amdgcn_readlane(incl, 63);
@@ -149,7 +149,7 @@ __global__ __launch_bounds__(256) void octet_read_kernel(OctReadArgs a) {
         const float p = oct_power(pw[kv][k]);
         bf16x2 o[4] = {oct_pair<false>(c[kv][k][0], p), oct_pair<true>(c[kv][k][0], p),
                        oct_pair<false>(c[kv][k][1], p), oct_pair<true>(c[kv][k][1], p)};
-        const int64_t to = (rq.row0 + at) * (kv ? a.v_stride : a.k_stride) + (int64_t)h * D + x;
+        const int64_t to = at * (kv ? a.v_stride : a.k_stride) + (int64_t)h * D + x;
         void* out = kv ? a.v_out : a.k_out;
         float f[8];
 #pragma unroll
