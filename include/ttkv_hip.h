@@ -457,7 +457,7 @@ int ttkv_nibble_prefill_paged(int32_t H, int32_t num_heads, int32_t d, float sca
 /* Rotary positions without a table of angles, for contexts that a table does not reach and for models
  * whose pairs are adjacent elements. query [N, num_heads, d] and key [N, H, d] (same dtype; either may
  * be absent with 0 heads) are rotated into query_out / key_out (which may be query and key at the same
- * strides; otherwise outputs overlap nothing): for j < rotary_dim / 2, with the angle
+ * strides; otherwise outputs, and their rows, overlap nothing): for j < rotary_dim / 2, with the angle
  * 2 pi positions[i] turns[j] of token i and (cos, sin) both times `amplitude`,
  *   y[u] = x[u] cos - x[v] sin,   y[v] = x[v] cos + x[u] sin
  * of the pair (u, v) = (j, j + rotary_dim / 2) or, adjacent, (2 j, 2 j + 1); dims past rotary_dim are
@@ -479,6 +479,7 @@ int ttkv_rotary_scaled(const void* query, const void* key, void* query_out, void
  *   2^e the smallest power of two with max |x| <= 448 * 2^e, e >= -117   (x clamped to +-1.75 * 2^127)
  *   code = e4m3(x / 2^e), to the nearest, ties to even;  byte = e + 127;  value = code * 2^e
  * (exact in bf16); a group that holds a NaN or an infinity reads back as NaN.
+ * Rows that a call writes do not overlap one another.
  *
  * Page: slot s of block b, b * block_size + offset, at 33 d H / 16 bytes per slot (slot_stride may be
  * larger); block sizes are multiples of 16. Sixteen slots from a multiple of 16 make a tile of H records

@@ -273,6 +273,17 @@ def test_decode_refusals():
     assert _decode(reqs=0) == 0 and _decode(n=0) == 0 and _decode(max_q=0) == 0
 
 
+def test_output_rows_that_overlap_one_another_are_refused():
+    for kw in (dict(q=1 << 20, qos=248), dict(q=1 << 20, qos=0), dict(k=1 << 20, kos=-120)):
+        _refused(_rotary(**kw), 1, "rows of an output")
+    _refused(_write(pos=64, turns=64, rot=128, HQ=8, q=1 << 20, qo=1 << 21, qt=1, qs=1024, qos=1016), 1,
+             "rows of query_out")
+    for kw in (dict(ks=1016), dict(vs=0)):
+        _refused(_read(**kw), 1, "rows of an output")
+    for stride in (4088, 0):
+        _refused(_decode(q=1 << 20, out=1 << 21, os=stride), 1, "rows of out")
+
+
 def test_workspace_sizes_grow_with_every_argument():
     f = _hip.lib().ttkv_octet_decode_workspace_bytes
     for bad in ((0, 8, 128, 1, 1, 64), (8, 12, 128, 1, 1, 64), (8, 8, 96, 1, 1, 64),

@@ -39,6 +39,9 @@ inline bool rows_meet(const void* a, int64_t sa, int64_t wa, const void* b, int6
   return false;
 }
 
+// Whether n rows of w bytes, s bytes apart, overlap one another.
+inline bool rows_fold(int64_t s, int64_t w, int64_t n) { return n > 1 && (s < 0 ? -s : s) < w; }
+
 // Every workspace starts with a fixed region of arrival counters: zero before first use (a fresh
 // zero-filled buffer), left zero by every call. It sits at the same offset with the same size
 // whatever the call's shape, so one buffer can serve calls of any shape in turn: a call's data

@@ -814,6 +814,8 @@ int octet_decode_paged(int H, int HQ, int d, float scale, const void* q, int q_d
   if (q && out && !(out == q && (out_row_stride == q_row_stride || num_tokens == 1)) &&
       rows_meet(out, 2 * out_row_stride, 2ll * HQ * d, q, 2 * q_row_stride, 2ll * HQ * d, num_tokens))
     return host_fail(TTKV_E_INVALID, "out overlaps the query without being it");
+  if (rows_fold(out_row_stride, (int64_t)HQ * d, num_tokens))
+    return host_fail(TTKV_E_INVALID, "rows of out overlap one another");
   const int64_t need = octet_decode_workspace_bytes(H, HQ, d, num_reqs, max_q, max_seq);
   if (!ws || ws_bytes < need || (uintptr_t)ws % 256)
     return host_fail(TTKV_E_WORKSPACE, "decode workspace needs " + std::to_string(need) + " bytes, 256-aligned");

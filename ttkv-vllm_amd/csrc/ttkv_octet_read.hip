@@ -206,6 +206,8 @@ int octet_read_paged(int H, int d, const uint8_t* page, int64_t n_slots, int64_t
   const int64_t eb = out_dtype == TTKV_DTYPE_F32 ? 4 : 2;
   if (rows_meet(k_out, k_stride * eb, H * d * eb, v_out, v_stride * eb, H * d * eb, num_rows))
     return host_fail(TTKV_E_INVALID, "key_out and value_out overlap");
+  if (rows_fold(k_stride, H * d, num_rows) || rows_fold(v_stride, H * d, num_rows))
+    return host_fail(TTKV_E_INVALID, "rows of an output overlap one another");
   // wide stores where every row starts 16-byte aligned; else an element at a time
   const bool vec = ((uintptr_t)k_out | (uintptr_t)v_out) % 16 == 0 && (k_stride * eb | v_stride * eb) % 16 == 0;
   OctReadArgs a{H,     num_reqs, page,    kOctTile * slot_stride, (int)(n_slots / bs), bs / kOctTile, bt, bt_row_stride,

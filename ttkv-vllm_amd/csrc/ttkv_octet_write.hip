@@ -230,6 +230,8 @@ int rotary_scaled(const void* q, const void* k, void* qo, void* ko, int dtype, i
       rows_meet(ko, ko_stride * eb, kw, q, q_stride * eb, qw, N) ||
       rows_meet(qo, qo_stride * eb, qw, ko, ko_stride * eb, kw, N))
     return host_fail(TTKV_E_INVALID, "one of query and key overlaps the other's output");
+  if (rows_fold(qo_stride * eb, qw, N) || rows_fold(ko_stride * eb, kw, N))
+    return host_fail(TTKV_E_INVALID, "rows of an output overlap one another");
   TurnArgs a{{q, k}, {qo, ko}, {HQ, H}, {q_stride, k_stride}, {qo_stride, ko_stride}, dtype, d, rot / 2, adjacent != 0,
              0,      pos,      turns,   amplitude,            err};
   a.pieces = turn_pieces_apply(a);
@@ -310,6 +312,8 @@ int octet_write_paged(int H, int d, const void* key, int k_dtype, int64_t k_row_
         meets(qo, qo_stride * eb, qw, k_out, 2 * row, 2 * row) || meets(qo, qo_stride * eb, qw, v_out, 2 * row, 2 * row) ||
         meets(q, q_stride * eb, qw, k_out, 2 * row, 2 * row) || meets(q, q_stride * eb, qw, v_out, 2 * row, 2 * row))
       return host_fail(TTKV_E_INVALID, "query_out overlaps the keys or values, or the query their outputs");
+    if (rows_fold(qo_stride * eb, qw, num_tokens))
+      return host_fail(TTKV_E_INVALID, "rows of query_out overlap one another");
   }
   const int64_t tokens = 1024 / d, blocks = (num_tokens + tokens - 1) / tokens * H;
   if (blocks > 0x3fffffff) return host_fail(TTKV_E_INVALID, "too many tokens for one call");
