@@ -604,6 +604,48 @@ def test_decode_scores_and_values_of_any_size(factor):
         _close(got, None, q.cpu(), *st.kv(0), scale, scale)
 
 
+def _cancelling(d, H, n, Q, seed):
+    """Whole-number keys [n, H, d] and a query [H, d], whose scores are exact in 32 bits, with values of 8 to 15
+    in size whose weighted sum nearly cancels for the last of Q queries: (q, k, v)."""
+    g = _gen(seed)
+    q, k = (torch.randint(-1, 2, s, generator=g).float() for s in ((H, d), (n, H, d)))
+    v = torch.empty(n, H, d)
+    for h in range(H):
+        s = (k[:, h] @ q[h]).double() / 64
+        assert float(s.abs().max()) <= 1
+        tries = torch.randint(8, 16, (n, 40000), generator=g) * (2 * torch.randint(0, 2, (n, 40000), generator=g) - 1)
+        left = (torch.softmax(s, 0) @ tries.double()).abs()
+        v[:, h] = tries[:, left.argsort()[:d]].float()
+    return q, k, v
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("d,H,G,Q,R", [(64, 4, 1, 1, 3), (128, 4, 4, 1, 3), (256, 4, 2, 1, 3), (64, 2, 16, 2, 130),
+                                       (128, 2, 6, 3, 130), (256, 2, 4, 5, 65), (256, 1, 16, 3, 2)])
+def test_decode_weights_are_not_rounded_to_fewer_bits(d, H, G, Q, R, dtype):
+    """Where values cancel, an output shows what its softmax weights are off by. In units of 2^-24 of the
+    spread sum p |v|: a score's product with the scale and that scale's own rounding, at most 1.5 after the
+    exponential; its difference to the maximum, at most 2 in size, 1.4; the exponential 2; the additions of six
+    products in three parts 8: 12.9 in all, 2^-20.3. The sum of weights and the division scale what is left of
+    the values. Weights of 16 bits are off by up to 2^-18 each and fail here (2^-18.7 of the spread)."""
+    n = 6
+    q, k, v = _cancelling(d, H, n, Q, d + G)
+    st = Store([n] * R, H, d, seed=1)
+    st.k, st.v = k.half().repeat(R, 1, 1), v.half().repeat(R, 1, 1)
+    kernels.octet_write_paged(st.lay, st.k.cuda(), st.v.cuda(), st.slots.cuda(), st.page)
+    rows = q.repeat_interleave(G, 0).to(dtype).repeat(R * Q, 1, 1).cuda()
+    err, at = _err(), _i32([Q * r for r in range(R + 1)])
+    out = kernels.octet_decode_paged(st.lay, rows, st.page, st.block, st.bt, st.seq, at, Q, n, 1 / 64,
+                                     out=torch.empty_like(rows, dtype=torch.float16), error_word=err)
+    assert int(err) == 0
+    want, _, spread, _ = oo.attend(rows[:Q].cpu(), *st.kv(0), 1 / 64)
+    last = want[-1].abs()
+    assert float((last / spread[-1]).max()) < 2.0 ** -7                  # (they do cancel)
+    tol = 2.0 ** -20.25 * spread + 2.0 ** -11 * want.abs() + 2.0 ** -25
+    e = (out.cpu().double().reshape(R, Q, H * G, d) - want).abs()
+    assert bool((e <= tol).all()), (float((e / spread).max()), float((e / tol).max()))
+
+
 def test_decode_bad_blocks_and_lengths():
     st = Store([40, 40, 40, 40, 2], 2, 128)
     bt = st.bt.clone()

@@ -16,7 +16,7 @@
 //   softmax in the result's own registers: lane column = row, 8 tokens of it. Weights are taken against
 //     the maximum as it stands, which moves only when their sum is large, so most steps need no maximum
 //     and no exchange between lanes; the sum stays per lane until the end. bf16 has fp32's range, so no
-//     weight leaves it; two parts of a weight keep 16 bits of it.
+//     weight leaves it; three parts of a weight keep its 24 bits.
 //   O^T [dim, row] += V^T P^T, a product per dim of a lane's d / 16 and weight part: the scores' layout is
 //     the B operand's as it stands. A lane holds dims of four tokens per tile; their bf16 pairs of two dims
 //     become pairs of two tokens by one byte permutation each. The result's column is the row again, so
@@ -49,6 +49,10 @@ enum { kODSingle = 0, kODOwn = 1, kODShared = 2 };
 // What a chunk's join costs per row and dim against a step (1 x 14,000 tokens: 16.4 us with 6e-4, 14.1 so; 1 x
 // 60,000 of one KV head of eight query heads 70 without it, 19.4 so).
 constexpr float kODJoin = 9e-4f;
+// bf16 parts of a weight: its 24 bits, as where values cancel an output shows what the weights are off by. Two, of
+// 16 bits, take 1 to 4 % less (8 x 14,402 tokens 45.7 and 45.9 us, 61 of 70 to 2,900 37.0 and 37.3, 6 x 5 queries
+// of 256 dims 26.3 and 27.3), 9 % where 64 rows share a KV head (60 x 8 over 1,500 keys 66.1 and 72.3).
+constexpr int kODParts = 3;
 constexpr float kLog2e = 1.4426950408889634f;
 
 struct OctDecodeArgs {
@@ -491,15 +495,17 @@ __global__ __launch_bounds__(64 * W, W > 4 ? W / 4 : D == 256 ? 3 - RG : D == 12
         weights(g);
       }
     }
-    bf16x8 ph[RG], pl[RG];  // 16 bits of each weight, in two parts
+    bf16x8 part[RG][kODParts];  // the weights' 24 bits
 #pragma unroll
     for (int g = 0; g < RG; ++g) {
       l[g] += sum[g];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        ph[g][i] = (__bf16)p[g][i];
-        pl[g][i] = (__bf16)(p[g][i] - (float)ph[g][i]);
-      }
+      for (int k = 0; k < kODParts; ++k)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          part[g][k][i] = (__bf16)p[g][i];
+          p[g][i] -= (float)part[g][k][i];
+        }
     }
     float vp[2][4];
 #pragma unroll
@@ -525,12 +531,12 @@ __global__ __launch_bounds__(64 * W, W > 4 ? W / 4 : D == 256 ? 3 - RG : D == 12
       }
       const bf16x8 v0 = __builtin_bit_cast(bf16x8, lo), v1 = __builtin_bit_cast(bf16x8, hi);
 #pragma unroll
-      for (int g = 0; g < RG; ++g) {
-        acc[g][e] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v0, ph[g], acc[g][e], 0, 0, 0);
-        acc[g][e + 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v1, ph[g], acc[g][e + 1], 0, 0, 0);
-        acc[g][e] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v0, pl[g], acc[g][e], 0, 0, 0);
-        acc[g][e + 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v1, pl[g], acc[g][e + 1], 0, 0, 0);
-      }
+      for (int g = 0; g < RG; ++g)
+#pragma unroll
+        for (int k = 0; k < kODParts; ++k) {
+          acc[g][e] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v0, part[g][k], acc[g][e], 0, 0, 0);
+          acc[g][e + 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v1, part[g][k], acc[g][e + 1], 0, 0, 0);
+        }
     }
     if (CHUNK && __builtin_amdgcn_ballot_w64(note != 0)) {
 #pragma unroll
