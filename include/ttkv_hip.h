@@ -538,8 +538,9 @@ int ttkv_octet_read_paged(int32_t H, int32_t d, const uint8_t* page, int64_t n_s
  * first max_q_len queries, or its first max_seq_len keys, taken; rows outside [0, num_tokens) set it and
  * are not taken. A block id outside the cache sets TTKV_ERR_BAD_BLOCK; rows that see the block become NaN,
  * and others of the request may. Keys, values and queries enter the products exactly (bf16
- * queries below 2^-126 may count as 0), softmax weights with 24 bits, sums are in 32 bits. A score beyond
- * fp32 makes its row NaN; values beyond 2^100 may sum up beyond fp32.
+ * queries below 2^-126 may count as 0), softmax weights with 24 bits, sums are in 32 bits. A score above
+ * fp32's range makes its row NaN, one below it weighs 0 (a row of such alone, without a sink, is NaN); values
+ * beyond 2^100 may sum up beyond fp32.
  * max_seq_len at most 2^26 and at most the tokens that max_blocks hold; the page at most 2^31 tiles.
  *
  * Workspace: as for the 4-bit reads, and one buffer may serve them all, in stream order: 256-byte

@@ -646,6 +646,51 @@ def test_decode_weights_are_not_rounded_to_fewer_bits(d, H, G, Q, R, dtype):
     assert bool((e <= tol).all()), (float((e / spread).max()), float((e / tol).max()))
 
 
+@pytest.mark.parametrize("d,H,G,n,Q", [(64, 1, 2, 40, 1), (128, 2, 4, 40, 3), (256, 1, 3, 70, 1), (64, 1, 16, 50, 2),
+                                       (128, 1, 2, 3000, 1), (256, 2, 2, 2500, 2)])
+@pytest.mark.parametrize("sinks", [False, True])
+def test_decode_scores_beyond_their_type(d, H, G, n, Q, sinks):
+    """Scores of +-2^130 in size: one above the type makes its row NaN, those below weigh nothing, and a row
+    that has no other is NaN, or its sink's."""
+    g = _gen(n + d)
+    for some in (-1.0, 1.0, None):     # the sign of the scores beyond, of about half the keys; None: all, below
+        k = torch.randint(-2, 3, (n, H, d), generator=g).float()
+        v = torch.randint(-8, 9, (n, H, d), generator=g).float()
+        k[..., :32] = 0
+        k[..., 0] = torch.where(torch.rand(n, H, generator=g) < 0.5, 2.0 ** 30, 0.0)
+        k[n // 2, :, 0] = 2.0 ** 30
+        if some is None:
+            k[..., 0] = 2.0 ** 30
+        st = Store([n], H, d, seed=2)
+        st.k, st.v = k, v
+        kernels.octet_write_paged(st.lay, k.cuda(), v.cuda(), st.slots.cuda(), st.page)
+        assert torch.equal(st.kv(0)[0], k.double())
+        q = torch.randint(-1, 2, (Q, H * G, d), generator=g).float()
+        q[..., 0] = (some or -1.0) * 2.0 ** 100
+        q = q.bfloat16().cuda()
+        s = (torch.arange(H * G).float() / 4).cuda() if sinks else None
+        lse = torch.full((Q, H * G), 7.0, device="cuda")
+        out, err, _ = _decode(st, q, [Q], sinks=s, lse=lse)
+        assert err == 0
+        if some == 1.0:
+            assert bool(torch.isnan(out).all()) and bool(torch.isnan(lse).all())
+        elif some is None and not sinks:
+            assert bool(torch.isnan(out).all()) and bool(torch.isnan(lse).all())
+        elif some is None:
+            assert bool((out == 0).all())
+            assert bool(((lse - s).abs() <= 2.0 ** -22 * (1 + s)).all())
+        else:
+            plain = q.clone()
+            plain[..., 0] = 0
+            for h in range(H):
+                kept, heads = k[:, h, 0] == 0, slice(h * G, h * G + G)
+                for j in range(Q):
+                    seen = kept & (torch.arange(n) <= n - Q + j)
+                    _close(out[j:j + 1, heads], lse[j:j + 1, heads], plain[j:j + 1, heads].cpu(),
+                           k[seen, h:h + 1].double(), v[seen, h:h + 1].double(), d ** -0.5, (h, j),
+                           sinks=s if s is None else s[heads].cpu())
+
+
 def test_decode_bad_blocks_and_lengths():
     st = Store([40, 40, 40, 40, 2], 2, 128)
     bt = st.bt.clone()

@@ -298,10 +298,11 @@ __global__ __launch_bounds__(64 * W, W > 4 ? W / 4 : D == 256 ? 3 - RG : D == 12
       o *= f;
       m = mn;
     }
-    const float by = l == 0.f ? 0.f : 1.f / l;
+    // no weight: no key, or keys whose scores all lie below fp32, which leave nothing to go by
+    const float by = l == 0.f ? (n > 0 ? NAN : 0.f) : 1.f / l;
     store_act4(a.out, a.out_dtype, row_at(r, a.out_row_stride) + d, o * by, true);
     if (a.lse && d == 0)
-      a.lse[((int64_t)P.q0 + j) * HQ + hq] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
+      a.lse[((int64_t)P.q0 + j) * HQ + hq] = l == 0.f ? (n > 0 ? NAN : -INFINITY) : (m + log2f(l)) * 0.6931471805599453f;
   };
   if (p0 < 0) {  // an empty request's rows are 0; fewer keys than queries are refused
     for (int i = tid; i < nrow * (D / 4); i += kThreads)
