@@ -284,6 +284,47 @@ def test_output_rows_that_overlap_one_another_are_refused():
         _refused(_decode(q=1 << 20, out=1 << 21, os=stride), 1, "rows of out")
 
 
+def test_outputs_that_overlap_rows_of_another_stride_are_refused():
+    """Rows of unlike strides whose first ones lie apart: packed rows, and an output's at twice their stride from
+    the second one on; a packed output behind a strided input's first row."""
+    q = 1 << 20
+    _refused(_rotary(q=q, qo=q + 512, qos=512), 1, "overlaps its input")
+    _refused(_rotary(q=q, qs=512, qo=q + 512, n=4), 1, "overlaps its input")
+    _refused(_rotary(q=q, qs=0, qo=q - 512), 1, "overlaps its input")
+    _refused(_rotary(q=q, k=q + 512, ks=256, ko=q + 3 * 512, kos=512, n=4), 1, "overlaps")
+    asked = dict(pos=64, turns=64, rot=128, HQ=8, q=q, qo=1 << 21, qt=1, qs=1024, qos=1024)
+    _refused(_write(**dict(asked, qo=q + 2048, qos=2048)), 1, "overlaps the query")
+    _refused(_write(**dict(asked, qo=65536 + 2048, qos=2048)), 1, "overlaps the keys")
+    _refused(_write(ko=65536 + 2048, ks=2048), 1, "key_out or value_out overlaps")
+    _refused(_write(vo=131072 + 2048, vs=1536), 1, "key_out or value_out overlaps")
+    _refused(_read(ko=1 << 16, vo=(1 << 16) + 2048, vs=2048), 1, "overlap")
+    _refused(_decode(q=1 << 20, out=(1 << 20) + 8192, os=8192), 1, "overlaps the query")
+    _refused(_decode(q=1 << 20, qs=8192, out=(1 << 20) + 8192), 1, "overlaps the query")
+
+
+def test_overlap_is_found_exactly():
+    """Against the rows' bytes one by one, for strides of any sign; a later refusal (keys' output rows that
+    overlap one another) takes the calls whose queries lie apart, so that nothing is launched."""
+    g = torch.Generator().manual_seed(3)
+
+    def pick(lo, hi):
+        return int(torch.randint(lo, hi + 1, (1,), generator=g))
+
+    seen = [0, 0]
+    for _ in range(6000):
+        n, w, q = pick(2, 7), 2 * pick(1, 4), 1 << 20
+        qs, qos = (pick(-12, 12) for _ in range(2))
+        if pick(0, 3) == 0:
+            qos = qs
+        qo = q + 2 * pick(-60, 60)
+        rows = [{a + 2 * s * i + b for i in range(n) for b in range(2 * w)} for a, s in ((q, qs), (qo, qos))]
+        meets = bool(rows[0] & rows[1]) and not (q == qo and qs == qos)
+        seen[meets] += 1
+        _refused(_rotary(q=q, qo=qo, qs=qs, qos=qos, n=n, HQ=1, H=1, d=w, rot=2, k=1 << 24, ks=64, ko=1 << 25,
+                         kos=0), 1, "overlaps its input" if meets else "rows of an output")
+    assert min(seen) > 1000
+
+
 def test_workspace_sizes_grow_with_every_argument():
     f = _hip.lib().ttkv_octet_decode_workspace_bytes
     for bad in ((0, 8, 128, 1, 1, 64), (8, 12, 128, 1, 1, 64), (8, 8, 96, 1, 1, 64),

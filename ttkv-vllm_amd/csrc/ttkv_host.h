@@ -25,17 +25,33 @@ inline int check_dec_pool(const int8_t* dec_q, const float* dec_scale) {
   return TTKV_OK;
 }
 
-// Whether rows of `a` and of `b` share bytes: n rows each, of wa and wb bytes at strides sa and sb. Rows
-// of unlike strides are only looked at where they begin.
-inline bool rows_meet(const void* a, int64_t sa, int64_t wa, const void* b, int64_t sb, int64_t wb,
-                          int64_t n) {
-  if (!wa || !wb || !a || !b) return false;
-  const int64_t off = (int64_t)((uintptr_t)b - (uintptr_t)a);
-  auto meet = [&](int64_t o) { return o < wa && -o < wb; };
-  if (n == 1 || sa != sb || sa <= 0) return meet(off);
-  const int64_t k0 = -off / sa;  // row i + k of b lies nearest to row i of a
-  for (int64_t k = k0 - 1; k <= k0 + 1; ++k)
-    if (k > -n && k < n && meet(off + k * sa)) return true;
+// Whether rows of `a` and of `b` share bytes: n rows each, of wa and wb bytes at strides sa and sb (of any sign;
+// 0: one row). Row i of a and row j of b do where -wb < off + j sb - i sa < wa. Of equal strides that is a range
+// of j - i; of unlike ones, whose spans meet, each row of a in b's span names a range of j.
+inline bool rows_meet(const void* a, int64_t sa, int64_t wa, const void* b, int64_t sb, int64_t wb, int64_t n) {
+  if (!wa || !wb || !a || !b || n <= 0) return false;
+  int64_t off = (int64_t)((uintptr_t)b - (uintptr_t)a);
+  if (sa < 0) off -= (n - 1) * sa, sa = -sa;  // the rows from the other end
+  if (sb < 0) off += (n - 1) * sb, sb = -sb;
+  int64_t na = sa ? n : 1, nb = sb ? n : 1;
+  if (nb == 1) {  // b has more rows than one, where any has
+    off = -off;
+    std::swap(sa, sb);
+    std::swap(wa, wb);
+    std::swap(na, nb);
+  }
+  if (nb == 1) return off < wa && -off < wb;
+  auto down = [](int64_t x, int64_t by) { return x / by - (x % by < 0); };
+  // whether some j in [lo, hi] has -wb < at + j sb < wa
+  auto meet = [&](int64_t at, int64_t lo, int64_t hi) {
+    return std::max(lo, down(-at - wb, sb) + 1) <= std::min(hi, down(wa - at - 1, sb));
+  };
+  if (na > 1 && sa == sb) return meet(off, 1 - n, n - 1);
+  const int64_t end = off + (nb - 1) * sb + wb;  // of b
+  const int64_t i0 = na > 1 ? std::max<int64_t>(0, down(off - wa, sa) + 1) : 0;
+  const int64_t i1 = na > 1 ? std::min(na - 1, down(end - 1, sa)) : 0;
+  for (int64_t i = i0; i <= i1; ++i)
+    if (meet(off - i * sa, 0, nb - 1)) return true;
   return false;
 }
 
