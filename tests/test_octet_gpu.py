@@ -276,6 +276,34 @@ def test_write_in_place_queries_and_waiting():
     assert torch.equal(page, before)
 
 
+def test_more_tokens_than_a_launch_has_threads():
+    """2^24 tokens and some: each as in a small call of its neighbours."""
+    N = 2 ** 24 + 37
+    spans = [slice(a, a + 300) for a in (0, 2 ** 22 - 100, 2 ** 23 - 150, 2 ** 23 + 4000, N - 300)]
+    gen = torch.Generator(device="cuda").manual_seed(1)
+    x = torch.randn(N, 1, 2, generator=gen, device="cuda").bfloat16()
+    pos = torch.arange(N, device="cuda") % 100003
+    r, err = scaled_rotary(2, device="cuda"), _err()
+    out, _ = kernels.rotary_scaled(x, None, pos, r, error_word=err)
+    assert int(err) == 0
+    for s in spans:
+        assert torch.equal(out[s], kernels.rotary_scaled(x[s], None, pos[s], r)[0])
+    del x, out
+    lay, r = OctetLayout(1, 64), scaled_rotary(64, device="cuda")
+    q = torch.randn(N, 1, 64, generator=gen, device="cuda", dtype=torch.bfloat16)
+    slots = torch.full((N,), -1, dtype=torch.int64, device="cuda")
+    for i, s in enumerate(spans):
+        slots[s] = torch.arange(i * 300, i * 300 + 300, device="cuda")
+    pages = [torch.zeros(94, 16, lay.compressed_bytes_per_token(), dtype=torch.uint8, device="cuda") for _ in range(2)]
+    out = kernels.octet_write_paged(lay, q, q, slots, pages[0], rotary=r, positions=pos, query=q, error_word=err)
+    assert int(err) == 0
+    for s in spans:
+        small = kernels.octet_write_paged(lay, q[s], q[s], slots[s], pages[1], rotary=r, positions=pos[s],
+                                          query=q[s])
+        assert torch.equal(out[s], small)
+    assert torch.equal(pages[0], pages[1])
+
+
 # ------------------------------------------------------------------------------------- store
 class Store:
     """An 8-bit store of requests of `lens` tokens in a shuffled paged cache, written by the kernel

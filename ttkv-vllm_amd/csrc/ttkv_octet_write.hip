@@ -183,6 +183,21 @@ __global__ __launch_bounds__(256) void rotary_scaled_kernel(TurnArgs a) {
 // 128: 8,192 tokens, 168 MB, 36.0 us so and 37.5 with loads that stay; 4,096 tokens, 84 MB, 21.3 and 17.9).
 constexpr int64_t kTurnStream = 128 << 20;
 
+// Workgroups of a launch at most: of 256 threads, whose number is below 2^32.
+constexpr int64_t kTurnGrid = 1 << 23;
+
+// The rows from token t on.
+static TurnArgs turn_from(TurnArgs a, int64_t t) {
+  const int64_t eb = a.dtype == TTKV_DTYPE_F32 ? 4 : 2;
+  for (int i = 0; i < 2; ++i)
+    if (a.heads[i]) {
+      a.x[i] = (const char*)a.x[i] + t * a.x_stride[i] * eb;
+      a.y[i] = (char*)a.y[i] + t * a.y_stride[i] * eb;
+    }
+  a.pos += t;
+  return a;
+}
+
 // Whether rows go in pieces of 8 elements: aligned, and pairs that lie in one or two of them.
 static bool turn_pieces_apply(const TurnArgs& a) {
   const int64_t eb = a.dtype == TTKV_DTYPE_F32 ? 4 : 2;
@@ -236,10 +251,12 @@ int rotary_scaled(const void* q, const void* k, void* qo, void* ko, int dtype, i
              0,      pos,      turns,   amplitude,            err};
   a.pieces = turn_pieces_apply(a);
   auto kernel = 2 * (qw + kw) * N > kTurnStream ? rotary_scaled_kernel<true> : rotary_scaled_kernel<false>;
-  hipLaunchKernelGGL(kernel, dim3(N), dim3(256), 0, st, a);
-  const hipError_t e = hipGetLastError();
-  if (e != hipSuccess)
-    return host_fail(TTKV_E_LAUNCH, std::string("scaled rotary launch: ") + hipGetErrorString(e));
+  for (int64_t t = 0; t < N; t += kTurnGrid) {
+    hipLaunchKernelGGL(kernel, dim3((unsigned)std::min(N - t, kTurnGrid)), dim3(256), 0, st, turn_from(a, t));
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess)
+      return host_fail(TTKV_E_LAUNCH, std::string("scaled rotary launch: ") + hipGetErrorString(e));
+  }
   return TTKV_OK;
 }
 
@@ -315,21 +332,40 @@ int octet_write_paged(int H, int d, const void* key, int k_dtype, int64_t k_row_
     if (rows_fold(qo_stride * eb, qw, num_tokens))
       return host_fail(TTKV_E_INVALID, "rows of query_out overlap one another");
   }
-  const int64_t tokens = 1024 / d, blocks = (num_tokens + tokens - 1) / tokens * H;
-  if (blocks > 0x3fffffff) return host_fail(TTKV_E_INVALID, "too many tokens for one call");
-  OctWriteArgs a{key,  val,     k_dtype,     v_dtype,          k_row_stride,     v_row_stride, slots,      num_tokens, H,
-                 page, n_slots, slot_stride, (uint16_t*)k_out, (uint16_t*)v_out, err,          (int)blocks};
-  a.turn = TurnArgs{{q, nullptr},  {qo, nullptr}, {HQ, 0}, {q_stride, 0}, {qo_stride, 0}, q_dtype, d, rot / 2,
-                    adjacent != 0, 0,             pos,     turns,         amplitude,      err};
-  a.turn.pieces = HQ && turn_pieces_apply(a.turn);
-  const int64_t grid = blocks + (HQ ? num_tokens : 0);  // those of the queries: a token each
+  TurnArgs turn{{q, nullptr},  {qo, nullptr}, {HQ, 0}, {q_stride, 0}, {qo_stride, 0}, q_dtype, d, rot / 2,
+                adjacent != 0, 0,             pos,     turns,         amplitude,      err};
+  turn.pieces = HQ && turn_pieces_apply(turn);
   const int dt = k_dtype == v_dtype ? k_dtype : -1;
-  if (d == 64) oct_write_launch<64>(a, (unsigned)grid, dt, st);
-  else if (d == 128) oct_write_launch<128>(a, (unsigned)grid, dt, st);
-  else oct_write_launch<256>(a, (unsigned)grid, dt, st);
-  const hipError_t e = hipGetLastError();
-  if (e != hipSuccess)
-    return host_fail(TTKV_E_LAUNCH, std::string("octet write launch: ") + hipGetErrorString(e));
+  // of `tokens` tokens and a head each, and one per token for the queries
+  const int64_t tokens = 1024 / d, most = std::max<int64_t>(1, kTurnGrid / (H + tokens)) * tokens;
+  for (int64_t t = 0; t < num_tokens; t += most) {
+    const int n = (int)std::min(num_tokens - t, most);
+    const int64_t blocks = (n + tokens - 1) / tokens * H;
+    OctWriteArgs a{(const char*)key + t * k_row_stride * kb,
+                   (const char*)val + t * v_row_stride * vb,
+                   k_dtype,
+                   v_dtype,
+                   k_row_stride,
+                   v_row_stride,
+                   slots + t,
+                   n,
+                   H,
+                   page,
+                   n_slots,
+                   slot_stride,
+                   k_out ? (uint16_t*)k_out + t * row : nullptr,
+                   v_out ? (uint16_t*)v_out + t * row : nullptr,
+                   err,
+                   (int)blocks,
+                   turn_from(turn, t)};
+    const unsigned grid = (unsigned)(blocks + (HQ ? n : 0));
+    if (d == 64) oct_write_launch<64>(a, grid, dt, st);
+    else if (d == 128) oct_write_launch<128>(a, grid, dt, st);
+    else oct_write_launch<256>(a, grid, dt, st);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess)
+      return host_fail(TTKV_E_LAUNCH, std::string("octet write launch: ") + hipGetErrorString(e));
+  }
   return TTKV_OK;
 }
 
