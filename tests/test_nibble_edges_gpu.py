@@ -315,3 +315,19 @@ def test_a_step_without_tokens():
         assert p.query_start_loc.tolist() == [0, 0, 0] and p.seq_lens.tolist() == [40, 700]
     step()
     assert torch.equal(st.page, page)
+
+
+# -------------------------------------------------------- more tokens than a launch has threads
+def test_rotary_of_more_tokens_than_a_launch_has_threads():
+    """2^24 tokens and some: each as in a small call of its neighbours."""
+    N = 2 ** 24 + 37
+    gen = torch.Generator(device="cuda").manual_seed(1)
+    x = torch.randn(N, 1, 2, generator=gen, device="cuda").bfloat16()
+    pos = torch.arange(N, device="cuda") % 4001
+    cs = torch.rand(4001, 2, generator=gen, device="cuda")
+    err = _err()
+    out, _ = kernels.rotary_axes(x, None, pos, cs, (1,), error_word=err)
+    assert int(err) == 0
+    for a in (0, 2 ** 23 - 150, 2 ** 23 + 4000, N - 300):
+        s = slice(a, a + 300)
+        assert bool((out[s] == kernels.rotary_axes(x[s], None, pos[s], cs, (1,))[0]).all())

@@ -12,6 +12,10 @@ namespace ttkv {
 int host_fail(int code, const std::string& msg);
 int device_cu_count();
 
+// Workgroups of a launch at most, of up to 256 threads: the runtime counts a launch's threads in 32 bits and cuts
+// off what lies beyond without an error.
+constexpr int64_t kMaxGrid = 1 << 23;
+
 // Raise a kernel's dynamic LDS limit to `smem` bytes on the current device, once per (kernel,
 // device): the attribute is per device.
 int raise_smem_limit(const void* kfn, size_t smem);

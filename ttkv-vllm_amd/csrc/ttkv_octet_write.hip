@@ -183,9 +183,6 @@ __global__ __launch_bounds__(256) void rotary_scaled_kernel(TurnArgs a) {
 // 128: 8,192 tokens, 168 MB, 36.0 us so and 37.5 with loads that stay; 4,096 tokens, 84 MB, 21.3 and 17.9).
 constexpr int64_t kTurnStream = 128 << 20;
 
-// Workgroups of a launch at most: of 256 threads, whose number is below 2^32.
-constexpr int64_t kTurnGrid = 1 << 23;
-
 // The rows from token t on.
 static TurnArgs turn_from(TurnArgs a, int64_t t) {
   const int64_t eb = a.dtype == TTKV_DTYPE_F32 ? 4 : 2;
@@ -251,8 +248,8 @@ int rotary_scaled(const void* q, const void* k, void* qo, void* ko, int dtype, i
              0,      pos,      turns,   amplitude,            err};
   a.pieces = turn_pieces_apply(a);
   auto kernel = 2 * (qw + kw) * N > kTurnStream ? rotary_scaled_kernel<true> : rotary_scaled_kernel<false>;
-  for (int64_t t = 0; t < N; t += kTurnGrid) {
-    hipLaunchKernelGGL(kernel, dim3((unsigned)std::min(N - t, kTurnGrid)), dim3(256), 0, st, turn_from(a, t));
+  for (int64_t t = 0; t < N; t += kMaxGrid) {
+    hipLaunchKernelGGL(kernel, dim3((unsigned)std::min(N - t, kMaxGrid)), dim3(256), 0, st, turn_from(a, t));
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess)
       return host_fail(TTKV_E_LAUNCH, std::string("scaled rotary launch: ") + hipGetErrorString(e));
@@ -337,7 +334,7 @@ int octet_write_paged(int H, int d, const void* key, int k_dtype, int64_t k_row_
   turn.pieces = HQ && turn_pieces_apply(turn);
   const int dt = k_dtype == v_dtype ? k_dtype : -1;
   // of `tokens` tokens and a head each, and one per token for the queries
-  const int64_t tokens = 1024 / d, most = std::max<int64_t>(1, kTurnGrid / (H + tokens)) * tokens;
+  const int64_t tokens = 1024 / d, most = std::max<int64_t>(1, kMaxGrid / (H + tokens)) * tokens;
   for (int64_t t = 0; t < num_tokens; t += most) {
     const int n = (int)std::min(num_tokens - t, most);
     const int64_t blocks = (n + tokens - 1) / tokens * H;

@@ -427,17 +427,23 @@ int rotary_axes(const void* q, const void* k, void* qo, void* ko, int dtype, int
   bool rows = rot % 16 == 0 && d % 8 == 0 && rot / 2 <= kRotHalf;
   for (const void* p : {q, k, (const void*)qo, (const void*)ko}) rows &= (uintptr_t)p % 16 == 0;
   for (int64_t s : {q_stride, k_stride, qo_stride, ko_stride}) rows &= s * eb % 16 == 0;
-  if (!rows)
-    hipLaunchKernelGGL(rotary_axes_kernel, dim3(N), dim3(256), 0, st, a);
-  else if (dtype == TTKV_DTYPE_F32)
-    hipLaunchKernelGGL(rotary_rows_kernel<TTKV_DTYPE_F32>, dim3(N), dim3(64), 0, st, a);
-  else if (dtype == TTKV_DTYPE_F16)
-    hipLaunchKernelGGL(rotary_rows_kernel<TTKV_DTYPE_F16>, dim3(N), dim3(64), 0, st, a);
-  else
-    hipLaunchKernelGGL(rotary_rows_kernel<TTKV_DTYPE_BF16>, dim3(N), dim3(64), 0, st, a);
-  const hipError_t e = hipGetLastError();
-  if (e != hipSuccess)
-    return host_fail(TTKV_E_LAUNCH, std::string("rotary launch: ") + hipGetErrorString(e));
+  auto kernel = !rows                      ? rotary_axes_kernel
+                : dtype == TTKV_DTYPE_F32 ? rotary_rows_kernel<TTKV_DTYPE_F32>
+                : dtype == TTKV_DTYPE_F16 ? rotary_rows_kernel<TTKV_DTYPE_F16>
+                                          : rotary_rows_kernel<TTKV_DTYPE_BF16>;
+  for (int64_t t = 0; t < N; t += kMaxGrid) {
+    RotArgs b = a;
+    b.q = (const char*)q + t * qs;
+    b.k = (const char*)k + t * ks;
+    b.qo = (char*)qo + t * qos;
+    b.ko = (char*)ko + t * kos;
+    b.pos = pos + t;
+    b.N = (int)std::min(N - t, kMaxGrid);
+    hipLaunchKernelGGL(kernel, dim3(b.N), dim3(rows ? 64 : 256), 0, st, b);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess)
+      return host_fail(TTKV_E_LAUNCH, std::string("rotary launch: ") + hipGetErrorString(e));
+  }
   return TTKV_OK;
 }
 
