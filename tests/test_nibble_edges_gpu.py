@@ -331,3 +331,22 @@ def test_rotary_of_more_tokens_than_a_launch_has_threads():
     for a in (0, 2 ** 23 - 150, 2 ** 23 + 4000, N - 300):
         s = slice(a, a + 300)
         assert bool((out[s] == kernels.rotary_axes(x[s], None, pos[s], cs, (1,))[0]).all())
+
+
+def test_write_of_more_tokens_than_a_launch_has_threads():
+    """2^23 tokens of 16 heads and some, all of one key and value row; a few, the last ones among them, have a
+    slot."""
+    H, N = 16, 2 ** 23 + 40
+    lay = NibbleLayout(H)
+    row = torch.randn(1, H, D, generator=_gen(5)).bfloat16().cuda()
+    x = row.expand(N, H, D)
+    at = torch.tensor([0, 1, 2 ** 22 + 3, 2 ** 23 - 1, 2 ** 23, 2 ** 23 + 9, N - 1]).cuda()
+    slots = torch.full((N,), -1, dtype=torch.int64, device="cuda")
+    slots[at] = torch.arange(at.numel(), device="cuda") * 3
+    pages = [torch.zeros(2, 16, lay.compressed_bytes_per_token(), dtype=torch.uint8, device="cuda") for _ in range(2)]
+    err = _err()
+    kernels.nibble_write_paged(lay, x, x, slots, pages[0], error_word=err)
+    assert int(err) == 0
+    few = row.expand(at.numel(), H, D).contiguous()
+    kernels.nibble_write_paged(lay, few, few, slots[at], pages[1])
+    assert bool((pages[0] == pages[1]).all()) and bool((pages[0].reshape(32, -1)[18] != 0).any())

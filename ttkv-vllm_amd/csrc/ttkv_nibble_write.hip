@@ -158,18 +158,34 @@ int nibble_write_paged(int H, int d, const void* key, int k_dtype, int64_t k_row
   if (!key || !val || !slots || !err) return host_fail(TTKV_E_INVALID, "null pointer argument");
   if ((uintptr_t)k_out % 16 || (uintptr_t)v_out % 16)
     return host_fail(TTKV_E_INVALID, "key_out / value_out must be 16-byte aligned");
-  const int64_t grid = ((int64_t)num_tokens + 7) / 8 * H;
-  if (grid > 0x7fffffff) return host_fail(TTKV_E_INVALID, "too many tokens for one call");
-  NibWriteArgs a{key,   val,  k_dtype, v_dtype,     k_row_stride,     v_row_stride,     slots, num_tokens,
-                 H,     page, n_slots, slot_stride, (_Float16*)k_out, (_Float16*)v_out, err};
   auto kernel = k_dtype != v_dtype               ? nibble_write_kernel<-1>
                 : k_dtype == TTKV_DTYPE_F32 ? nibble_write_kernel<TTKV_DTYPE_F32>
                 : k_dtype == TTKV_DTYPE_F16 ? nibble_write_kernel<TTKV_DTYPE_F16>
                                             : nibble_write_kernel<TTKV_DTYPE_BF16>;
-  hipLaunchKernelGGL(kernel, dim3((unsigned)grid), dim3(256), 0, st, a);
-  const hipError_t e = hipGetLastError();
-  if (e != hipSuccess)
-    return host_fail(TTKV_E_LAUNCH, std::string("nibble write launch: ") + hipGetErrorString(e));
+  const int64_t kb = k_dtype == TTKV_DTYPE_F32 ? 4 : 2, vb = v_dtype == TTKV_DTYPE_F32 ? 4 : 2, row = (int64_t)H * kD;
+  const int64_t most = std::max<int64_t>(1, kMaxGrid / H) * 8;  // tokens of a launch: eight and a head a workgroup
+  for (int64_t t = 0; t < num_tokens; t += most) {
+    const int n = (int)std::min(num_tokens - t, most);
+    NibWriteArgs a{(const char*)key + t * k_row_stride * kb,
+                   (const char*)val + t * v_row_stride * vb,
+                   k_dtype,
+                   v_dtype,
+                   k_row_stride,
+                   v_row_stride,
+                   slots + t,
+                   n,
+                   H,
+                   page,
+                   n_slots,
+                   slot_stride,
+                   k_out ? (_Float16*)k_out + t * row : nullptr,
+                   v_out ? (_Float16*)v_out + t * row : nullptr,
+                   err};
+    hipLaunchKernelGGL(kernel, dim3((unsigned)((n + 7) / 8 * H)), dim3(256), 0, st, a);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess)
+      return host_fail(TTKV_E_LAUNCH, std::string("nibble write launch: ") + hipGetErrorString(e));
+  }
   return TTKV_OK;
 }
 
