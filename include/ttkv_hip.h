@@ -536,7 +536,8 @@ int ttkv_octet_read_paged(int32_t H, int32_t d, const uint8_t* page, int64_t n_s
  * A request with n == 0 has rows of 0 and an lse of -infinity, or the sink. One with 0 < n < Q sets
  * TTKV_ERR_SEQ_LEN and its rows become NaN; one with Q > max_q_len or n > max_seq_len sets it and has its
  * first max_q_len queries, or its first max_seq_len keys, taken; rows outside [0, num_tokens) set it and
- * are not taken. A block id outside the cache sets TTKV_ERR_BAD_BLOCK; rows that see the block become NaN,
+ * are not taken; one with n < 0 or Q < 0 sets it and counts as empty, or has no queries (a call whose
+ * num_reqs, num_tokens or max_q_len is 0 looks at none of them). A block id outside the cache sets TTKV_ERR_BAD_BLOCK; rows that see the block become NaN,
  * and others of the request may. Keys, values and queries enter the products exactly (bf16
  * queries below 2^-126 may count as 0), softmax weights with 24 bits, sums are in 32 bits. A score above
  * fp32's range makes its row NaN, one below it weighs 0 (a row of such alone, without a sink, is NaN); values

@@ -771,6 +771,57 @@ def test_decode_lengths_beyond_the_call():
     assert bool((got[0] == 0).all())
 
 
+def test_decode_rows_partly_outside_the_query():
+    """Of a request whose rows begin before the query's or end behind them, those inside are its own."""
+    st = Store([50, 20], 1, 64)
+    q = torch.randn(5, 2, 64, generator=_gen(1)).half().cuda()
+    for window in (0, 7):
+        out, err = torch.full_like(q, 7.0), _err()
+        kernels.octet_decode_paged(st.lay, q, st.page, 16, st.bt, st.seq, _i32([-1, 1, 7]), 6, 50, 0.125,
+                                   window=window, out=out, error_word=err)
+        assert int(err) == 8
+        # row 0 is the second of request 0's two queries, rows 1 .. 4 the first of request 1's six
+        K, V = st.kv(0)
+        _close(out[:1], None, q[:1].cpu(), K, V, 0.125, "second of two", window=window)
+        K, V = st.kv(1)
+        _close(out[1:], None, q[1:].cpu(), K[:18], V[:18], 0.125, "four of six", window=window)
+
+
+@pytest.mark.parametrize("R", [3, 300])
+def test_decode_negative_lengths_and_falling_starts(R):
+    """Said so; a length below 0 counts as none, starts that fall as a request that waits."""
+    st = Store([20] * R, 1, 64)
+    q = torch.randn(R, 2, 64, generator=_gen(2)).half().cuda()
+    for r in (0, R - 1):
+        seq, err, out = st.seq.clone(), _err(), torch.full_like(q, 7.0)
+        seq[r] = -2 ** 31 if r else -5
+        lse = torch.full((R, 2), 7.0, device="cuda")
+        starts = torch.arange(R + 1, dtype=torch.int32, device="cuda")
+        kernels.octet_decode_paged(st.lay, q, st.page, 16, st.bt, seq, starts, 1, 20, 0.125, out=out, lse=lse,
+                                   error_word=err)
+        assert int(err) == 8
+        assert bool((out[r] == 0).all()) and bool((lse[r] == -math.inf).all())
+        for i in {0, 1, R - 2, R - 1} - {r}:
+            _close(out[i:i + 1], lse[i:i + 1], q[i:i + 1].cpu(), *st.kv(i), 0.125, i)
+    # queries of row i + 1 for request i; request R - 2's end before they begin, the last one's is row 0 or none
+    for low in (0, -2 ** 31):
+        starts, err, out = torch.arange(1, R + 2, dtype=torch.int32, device="cuda"), _err(), torch.full_like(q, 7.0)
+        starts[R - 1], starts[R] = low, low + 1
+        kernels.octet_decode_paged(st.lay, q, st.page, 16, st.bt, st.seq, starts, 1, 20, 0.125, out=out,
+                                   error_word=err)
+        assert int(err) == 8
+        for i in {0, R - 3}:
+            _close(out[i + 1:i + 2], None, q[i + 1:i + 2].cpu(), *st.kv(i), 0.125, i)
+        if low == 0:
+            _close(out[:1], None, q[:1].cpu(), *st.kv(R - 1), 0.125, "last")
+        assert bool((out[R - 1:] == 7).all()) and (low == 0 or bool((out[0] == 7).all()))
+    # from one end of the type to the other: more than max_q_len, all of its first ones outside
+    err, out = _err(), torch.full_like(q, 7.0)
+    kernels.octet_decode_paged(st.lay, q, st.page, 16, st.bt[:1], st.seq[:1], _i32([-2 ** 31, 2 ** 31 - 1]), 1, 20,
+                               0.125, out=out, error_word=err)
+    assert int(err) == 8 and bool((out == 7).all())
+
+
 def test_decode_nan_keys_stay_with_the_rows_that_see_them():
     """A NaN in a stored key or value reaches the rows that see it; behind the last key, in a draft's
     future or before the window it reaches nobody."""

@@ -111,6 +111,7 @@ __device__ __forceinline__ OctPlan od_plan(const OctDecodeArgs& a) {
   const int lane = threadIdx.x & 63;
   int n[kODPlanLanes], q0[kODPlanLanes], Q[kODPlanLanes], s0[kODPlanLanes], st[kODPlanLanes], rb[kODPlanLanes];
   int total = 0, longest = 0, whole = 0;
+  bool falls = false;  // a request's queries end before they begin: none are taken
 #pragma unroll
   for (int i = 0; i < kODPlanLanes; ++i) {
     n[i] = q0[i] = Q[i] = 0;
@@ -118,8 +119,11 @@ __device__ __forceinline__ OctPlan od_plan(const OctDecodeArgs& a) {
     if (64 * i >= a.num_reqs || r >= a.num_reqs) continue;
     n[i] = a.seq_lens[r];
     q0[i] = a.qsl[r];
-    Q[i] = a.qsl[r + 1] - q0[i];
+    const int q1 = a.qsl[r + 1];
+    falls |= q1 < q0[i];
+    Q[i] = q1 < q0[i] ? -1 : (int)min((uint32_t)q1 - (uint32_t)q0[i], 0x7fffffffu);
   }
+  if (blockIdx.x == 0 && threadIdx.x < 64 && falls) atomicOr(a.err, TTKV_ERR_SEQ_LEN);
 #pragma unroll
   for (int i = 0; i < kODPlanLanes; ++i) {
     s0[i] = st[i] = rb[i] = 0;
@@ -277,7 +281,7 @@ __global__ __launch_bounds__(64 * W, W > 4 ? W / 4 : D == 256 ? 3 - RG : D == 12
   const int row0 = P.rb * RB, nrow = min(RB, Q * G - row0);  // the block's rows
   const bool outside = P.q0 < 0 || (int64_t)P.q0 + Q > a.num_tokens;
   if (tid == 0 && h == 0 && P.c == 0 && P.rb == 0 &&
-      (P.n > a.max_seq || P.Q > a.max_q || (n > 0 && p0 < 0) || outside))
+      (P.n < 0 || P.n > a.max_seq || P.Q > a.max_q || (n > 0 && p0 < 0) || outside))
     atomicOr(a.err, TTKV_ERR_SEQ_LEN);
   // row `r` of the block in the query and the output, and whether it has a place there
   auto row_at = [&](int r, int64_t stride) -> int64_t {
