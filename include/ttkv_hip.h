@@ -528,7 +528,7 @@ int ttkv_octet_read_paged(int32_t H, int32_t d, const uint8_t* page, int64_t n_s
  * the end of its n = seq_lens[r] stored keys, their own included. Query j, at position p = n - Q + j, sees
  * the keys t <= p and, with a window > 0, t > p - window:
  *   out[j] = sum_t softmax_t(scale * q[j] . K[t]) * V[t]
- * With sinks [num_heads] fp32 (finite or -infinity) the softmax has one more term, exp(sinks[head]), that
+ * With sinks [num_heads] fp32 (at most 2^127 in size, or -infinity) the softmax has one more term, exp(sinks[head]), that
  * carries no value; lse [num_tokens, num_heads] fp32 (optional) receives the logarithm of the softmax's sum,
  * by which results over parts of a context are joined. query and out [num_tokens, num_heads, d] fp16 or bf16, up to 16
  * query heads per KV head; `out` may be the query as it stands and otherwise does not overlap it. Rows that
@@ -539,9 +539,9 @@ int ttkv_octet_read_paged(int32_t H, int32_t d, const uint8_t* page, int64_t n_s
  * are not taken; one with n < 0 or Q < 0 sets it and counts as empty, or has no queries (a call whose
  * num_reqs, num_tokens or max_q_len is 0 looks at none of them). A block id outside the cache sets TTKV_ERR_BAD_BLOCK; rows that see the block become NaN,
  * and others of the request may. Keys, values and queries enter the products exactly (bf16
- * queries below 2^-126 may count as 0), softmax weights with 24 bits, sums are in 32 bits. A score above
- * fp32's range makes its row NaN, one below it weighs 0 (a row of such alone, without a sink, is NaN); values
- * beyond 2^100 may sum up beyond fp32.
+ * queries below 2^-126 may count as 0), softmax weights with 24 bits, sums are in 32 bits. A score
+ * beyond 2^127 in size may count as infinite: one above makes its row NaN, one below weighs 0 (a row of such
+ * alone, without a sink, is NaN); values beyond 2^100 may sum up beyond fp32.
  * max_seq_len at most 2^26 and at most the tokens that max_blocks hold; the page at most 2^31 tiles.
  *
  * Workspace: as for the 4-bit reads, and one buffer may serve them all, in stream order: 256-byte

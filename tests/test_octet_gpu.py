@@ -117,6 +117,25 @@ def test_rotary_strides_and_in_place(dtype, pad, shift):
     assert torch.equal(flat[mask], before[mask])
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("adjacent,rot", [(False, 128), (True, 128), (False, 48), (True, 24)])
+def test_rotary_of_rows_beyond_the_caches(dtype, adjacent, rot):
+    """Past 128 MB of rows read and written: bit for bit as in calls of a few of them."""
+    N = 6600 if dtype == torch.float32 else 13200
+    gen = torch.Generator(device="cuda").manual_seed(rot)
+    q, k = (torch.randn(N, h, 128, generator=gen, device="cuda").to(dtype) for h in (16, 4))
+    assert 2 * (q.numel() + k.numel()) * q.element_size() > 128 << 20
+    pos = torch.arange(N, device="cuda") * 7
+    r = scaled_rotary(rot, rule="yarn", factor=4.0, adjacent=adjacent, device="cuda")
+    qo, ko = kernels.rotary_scaled(q, k, pos, r)
+    for a in range(0, N, 1100):
+        s = slice(a, a + 1100)
+        few = kernels.rotary_scaled(q[s], k[s], pos[s], r)
+        assert torch.equal(qo[s], few[0]) and torch.equal(ko[s], few[1])
+    kernels.rotary_scaled(q, k, pos, r, query_out=q, key_out=k)
+    assert torch.equal(q, qo) and torch.equal(k, ko)
+
+
 def test_rotary_refused_positions_and_values():
     q = torch.randn(5, 2, 64, generator=_gen(3)).half().cuda()
     q[1, 0, 7], q[1, 1, 40] = float("nan"), float("inf")
@@ -235,6 +254,48 @@ def test_write_rotates(dtype, d, rot, adjacent):
     slack = off.reshape(*kb.shape, 32).amax(-1)
     assert bool((top - slack <= 448 * power).all()) and bool((top + slack > 224 * power).all())
     assert torch.equal(oo.combine(vc, vb), oo.values(v)[kept])
+
+
+@pytest.mark.parametrize("d,rot,adjacent", [(64, 64, True), (128, 128, False), (128, 50, False), (256, 64, True),
+                                            (256, 256, False)])
+@pytest.mark.parametrize("kt,vt,qt,pad", [(torch.float32, torch.bfloat16, torch.float16, 3),
+                                          (torch.float16, torch.float32, torch.float32, 8),
+                                          (torch.bfloat16, torch.bfloat16, torch.float32, 1)])
+def test_write_rotates_rows_of_any_type_and_stride(d, rot, adjacent, kt, vt, qt, pad):
+    """Keys, values and queries of their own types, in rows of odd strides that start off 16 bytes: the bytes,
+    and the stored values of contiguous rows of the same types, which the same kernel takes."""
+    g = _gen(d + rot + pad)
+    n, H, HQ = 21, 2, 3
+    lay = OctetLayout(H, d)
+
+    def rows(h, t):
+        flat = torch.randn(n * (h * d + pad) + 1, generator=g).to(t).cuda()
+        return flat[1:].as_strided((n, h, d), (h * d + pad, d, 1))
+
+    k, v, q = rows(H, kt), rows(H, vt), rows(HQ, qt)
+    pos, slots = torch.arange(n).cuda() * 31 + 5000, torch.arange(n).cuda() + 9
+    slots[4] = -1
+    r = scaled_rotary(rot, rule="linear", factor=2.0, adjacent=adjacent, device="cuda")
+    pages = [torch.zeros(2, 16, lay.compressed_bytes_per_token(), dtype=torch.uint8, device="cuda") for _ in range(2)]
+    kept = [torch.zeros(n, H, d, dtype=torch.bfloat16, device="cuda") for _ in range(4)]
+    err = _err()
+    qo = kernels.octet_write_paged(lay, k, v, slots, pages[0], rotary=r, positions=pos, query=q, key_out=kept[0],
+                                   value_out=kept[1], error_word=err)
+    assert int(err) == 0
+    host = r._replace(turns=r.turns.cpu())
+    _turn_close(qo, q.cpu(), pos.cpu(), host)
+    alone = kernels.octet_write_paged(lay, k.contiguous(), v.contiguous(), slots, pages[1], rotary=r, positions=pos,
+                                      query=q.contiguous(), key_out=kept[2], value_out=kept[3])
+    _turn_close(alone, q.cpu(), pos.cpu(), host)
+    assert torch.equal(pages[0], pages[1])
+    assert torch.equal(kept[0], kept[2]) and torch.equal(kept[1], kept[3])
+    on = slots.cpu() >= 0
+    (kc, kb), _ = oo.fields(pages[0], lay.compressed_bytes_per_token(), slots.cpu()[on], H, d)
+    want = oo.turn(k.cpu(), pos.cpu(), host.turns.tolist(), 1.0, adjacent)[on]
+    off = _turn_tol(k.cpu(), pos.cpu(), host, rot // 2, kt)[on]
+    step = torch.maximum(want.abs() / 16, 2.0 ** (kb.double() - 137).repeat_interleave(32, -1))
+    assert bool(((oo.combine(kc, kb) - want).abs() <= (step + off) * 1.001).all())
+    assert torch.equal(kept[1].cpu().double()[on], oo.values(v.cpu())[on])
 
 
 def test_write_rotates_by_refused_positions():
@@ -380,6 +441,15 @@ def test_read_many_requests(H, d):
                                     error_word=err)
     assert int(err) == 8
     assert torch.equal(k[7:].cpu().double(), st.kv(4)[0][7:14])
+
+
+def test_read_rows_that_two_requests_name():
+    """Each head's row is one request's or the other's as a whole; rows past them are the second's."""
+    st = Store([9, 20], 3, 128, seed=4)
+    k, v = kernels.octet_read_paged(st.lay, st.page, 16, st.bt[[0, 1, 1]], _i32([0, 7, 0, 14]), 20, num_rows=14)
+    for x, i in ((k.cpu().double(), 0), (v.cpu().double(), 1)):
+        one, two = ((x[:7] == st.kv(r)[i][:7]).all(-1) for r in (0, 1))
+        assert bool((one | two).all()) and torch.equal(x[7:], st.kv(1)[i][7:14])
 
 
 def test_read_strides_and_defaults():
@@ -589,6 +659,41 @@ def test_decode_drafts_of_large_batches(d, H, G, R, window):
             _close(out[rows], lse[rows], q[rows].cpu(), *st.kv(r), d ** -0.5, r, window=window)
 
 
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("d,H,G,Q,R,window", [(128, 8, 8, 5, 24, 0), (64, 8, 8, 8, 20, 0), (128, 4, 16, 3, 48, 9),
+                                              (256, 4, 12, 4, 24, 0), (64, 2, 16, 16, 20, 25)])
+def test_decode_drafts_of_several_blocks_in_large_batches(d, H, G, Q, R, window, dtype):
+    """More than 32 rows per KV head in batches that give a block two groups of rows: blocks that are partly
+    filled, requests of fewer queries and waiting ones, keys that are split and that are not."""
+    g = _gen(d + Q)
+    assert G * Q > 32 and R * H * -(-G * Q // 16) > (256 if d == 256 else 512)
+    lens = [Q + int(torch.randint(0, 120, (1,), generator=g)) for _ in range(R)]
+    lens[3] = 900
+    st = Store(lens, H, d, 32, seed=4, dtype=dtype)
+    counts = [Q if i % 3 else i // 3 % (Q + 1) for i in range(R)]
+    q = torch.randn(sum(counts) + 1, H * G, d, generator=g).to(dtype).cuda()
+    out, lse = torch.full_like(q, 7.0), torch.full(q.shape[:2], 7.0, device="cuda")
+    _, err, at = _decode(st, q, counts, max_q_len=Q, out=out, lse=lse, window=window)
+    assert err == 0
+    _check(st, q, counts, out, lse, at, window=window)
+    assert bool((out[-1] == 7).all()) and bool((lse[-1] == 7).all())
+
+
+@pytest.mark.parametrize("d,R", [(64, 150), (128, 140)])
+def test_decode_batches_beyond_the_counters(d, R):
+    """8 KV heads of 16 query heads and 16 drafts: more (block, head) pairs than counters, so several launches."""
+    g = _gen(R)
+    lens = [1 + int(torch.randint(0, 40, (1,), generator=g)) for _ in range(R)]
+    lens[R - 2], lens[2] = 600, 500
+    counts = [min(n, 16 if i % 9 == 0 else 1 + i % 2) for i, n in enumerate(lens)]
+    st = Store(lens, 8, d, seed=5)
+    q = torch.randn(sum(counts), 128, d, generator=g).half().cuda()
+    ws = kernels.octet_decode_workspace(st.lay, 128, R, 16, 600, "cuda")
+    out, err, at = _decode(st, q, counts, max_q_len=16, workspace=ws)
+    assert err == 0 and bool((ws[:65536] == 0).all())
+    _check(st, q, counts, out, None, at)
+
+
 @pytest.mark.parametrize("d,H,R,window,Q", [(64, 8, 24, 0, 1), (128, 8, 24, 0, 1), (64, 8, 32, 640, 2),
                                             (128, 8, 21, 600, 3), (128, 4, 60, 0, 1)])
 def test_decode_pairs_that_fill_the_chip(d, H, R, window, Q):
@@ -717,6 +822,21 @@ def test_decode_scores_beyond_their_type(d, H, G, n, Q, sinks):
                     _close(out[j:j + 1, heads], lse[j:j + 1, heads], plain[j:j + 1, heads].cpu(),
                            k[seen, h:h + 1].double(), v[seen, h:h + 1].double(), d ** -0.5, (h, j),
                            sinks=s if s is None else s[heads].cpu())
+
+
+@pytest.mark.parametrize("size", [1e4, 2.0 ** 100, 2.0 ** 127])
+def test_decode_sinks_of_any_size(size):
+    """A large sink takes all the weight, a low one none; an empty request's lse is its sink."""
+    st = Store([40, 0], 1, 64, seed=3)
+    q = torch.randn(2, 4, 64, generator=_gen(3)).half().cuda()
+    sinks, lse = torch.tensor([size, -size, -math.inf, 0.0]), torch.zeros(2, 4, device="cuda")
+    out, err, _ = _decode(st, q, sinks=sinks.cuda(), lse=lse)
+    assert err == 0
+    _close(out[:1, 1:], lse[:1, 1:], q[:1, 1:].cpu(), *st.kv(0), 0.125, "low", sinks=sinks[1:])
+    assert bool((out[0, 0] == 0).all()) and bool((out[1] == 0).all())
+    assert float(lse[1, 2]) == -math.inf
+    got, want = torch.cat([lse[:1, 0], lse[1, [0, 1, 3]]]).cpu().double(), sinks[[0, 0, 1, 3]].double()
+    assert bool(((got - want).abs() <= 2.0 ** -22 * want.abs()).all()), got
 
 
 def test_decode_bad_blocks_and_lengths():
