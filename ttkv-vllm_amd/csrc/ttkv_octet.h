@@ -24,7 +24,6 @@
 namespace ttkv {
 
 constexpr int kOctTile = 16;   // slots per tile
-constexpr int kOctGroup = 32;  // dims per power of two
 constexpr int kOctMinByte = 127 - 117;
 constexpr uint32_t kOctNanCode = 0x7f, kOctNanByte = 127;
 constexpr float kOctMax = 0x1.cp127f;
@@ -33,8 +32,6 @@ template <int D>
 struct Oct {
   static_assert(D == 64 || D == 128 || D == 256, "head dims of 64, 128 and 256");
   static constexpr int kRecord = 33 * D;       // bytes of a tile's record of one head
-  static constexpr int kSlot = kRecord / 16;   // bytes per slot and head, rounded down
-  static constexpr int kGroups = D / kOctGroup;
   static constexpr int kPair = D >= 128 ? D / 128 : 1;  // key exponents of a lane
   static constexpr int kDims = D / 16;         // a lane's value dims per token
   static constexpr int kV = 16 * D;            // record offsets: value codes,

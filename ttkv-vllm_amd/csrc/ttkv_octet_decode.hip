@@ -2,8 +2,8 @@
 // drafts. gfx950 / CDNA4.
 //
 // The rows of a (request, KV head) are its (query, query head) pairs, row = j G + p. Work item = (request,
-// block of 16 rows, chunk of the request's 32-token steps, KV head), one workgroup of 4 waves that take the
-// chunk's steps in turn. The chunk length comes from a plan that every workgroup computes alike from the
+// block of RG groups of 16 rows, chunk of the request's 32-token steps, KV head), one workgroup of W waves that
+// take the chunk's steps in turn: W is 4 or 8 (od_waves), RG 1 or 2 (od_groups). The chunk length comes from a plan that every workgroup computes alike from the
 // batch's lengths: the shortest that spreads the batch's steps over the resident workgroups, so a ragged
 // batch fills the chip by its total work. Items of a (block, head) leave unnormalised partials in the
 // workspace; the last to arrive joins them.
@@ -22,9 +22,9 @@
 //     become pairs of two tokens by one byte permutation each. The result's column is the row again, so
 //     the rescale is a lane's factor.
 // A step is 66 d bytes. Bound by memory where calls are large: 8 x 14,402 tokens of 8 heads of 128, 243 MB,
-// 45.4 us, of which a prologue takes 5 and the join 3: 6.5 TB/s between them (vector issue 36 %, matrix units
-// 15 %); 61 requests of 70 to 2,900 36.8 us for 178 MB. Smaller calls are a chain of round trips: one key tile
-// 5.1 us, a split and its join 2.3 to 4 more; 1 x 1,082 8.4 us.
+// 46.1 us, of which a prologue takes 5 and the join 3: 6.4 TB/s between them (vector issue 40 %, matrix units
+// 19 %); 61 requests of 70 to 2,900 37.3 us for 178 MB. Smaller calls are a chain of round trips: one key tile
+// 5.3 us, a split and its join 2.3 to 4 more; 1 x 1,082 8.8 us.
 #include <math.h>
 
 #include <atomic>
@@ -39,12 +39,15 @@ constexpr int kODMaxQ = 16;  // queries per request
 constexpr int kODStep = 2 * kOctTile;  // tokens per wave step
 constexpr int kODPlanLanes = 4;        // requests per lane in the plan: 256 per launch
 constexpr int kODClasses = 8;          // of chunk lengths, for the items' order
-constexpr int kODRows = 16;            // rows of a block: a matrix product's columns
+constexpr int kODRows = 16;            // rows of a group: a matrix product's columns
 constexpr float kODNone = -3.402823466e38f;  // the maximum before the first visible key
 constexpr float kODMost = 0x1p10f;     // a lane's sum of eight weights before the maximum moves
 // One query per request; several, whose rows are one block; or more blocks, whose bytes stay in the caches for
 // each other (6 x 5 queries of four query heads over 4,000 keys, d = 256: 25.1 us with loads that do not stay,
-// 23.3; where there is one block they cost: 30 x 3 over 200 to 4,000 30.1, 32.6).
+// 23.3; where there is one block they cost: 30 x 3 over 200 to 4,000 30.1, 32.6). Blocks of two groups of rows
+// take loads that do not stay however many there are (with such and with ones that stay, 60 x 8 queries of eight
+// query heads over 1,500 keys: of 128 dims 76.4 us and 74.2, of 256 90.3 and 85.9, of 64 48.2 and 49.2; 40 x 16
+// of four over 2,000 70.3 and 71.4).
 enum { kODSingle = 0, kODOwn = 1, kODShared = 2 };
 // What a chunk's join costs per row and dim against a step (1 x 14,000 tokens: 16.4 us with 6e-4, 14.1 so; 1 x
 // 60,000 of one KV head of eight query heads 70 without it, 19.4 so).
@@ -140,7 +143,7 @@ __device__ __forceinline__ OctPlan od_plan(const OctDecodeArgs& a) {
   float all = (float)wave_sum_i(total & 4095);
   if (__builtin_amdgcn_ballot_w64(total >> 12)) all += 4096.f * (float)wave_sum_i(total >> 12);
   whole = wave_sum_i(whole);
-  // whole rounds of the four waves. (Never shorter than the batch's share: the grid and the workspace are
+  // whole rounds of the workgroup's waves. (Never shorter than the batch's share: the grid and the workspace are
   // made for that; fp32 is off by less than the factor.)
   all *= (float)a.H * 1.000001f;
   int C = (max(1, (int)ceilf(all * a.by_target)) + W - 1) / W * W;
@@ -748,7 +751,7 @@ static int od_slice(int H, int blocks, int num_reqs) {
 
 // Items of split blocks, at most, of `pairs` (block, head) pairs. A chunk has at least total / target
 // steps, and a split block of st steps has less than st / C + 1 < 2 st / C chunks: less than 2 target of
-// them in all; and whole rounds of the four waves of a request.
+// them in all; and whole rounds of a request's waves, four where they are fewest.
 static int64_t od_max_chunks(int max_seq) {
   const int64_t round = kODStep * 4;
   return std::max<int64_t>(1, (max_seq + round - 1) / round + 1);  // (a window's first step may be cut)
