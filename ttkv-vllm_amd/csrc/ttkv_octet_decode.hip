@@ -54,7 +54,8 @@ enum { kODSingle = 0, kODOwn = 1, kODShared = 2 };
 constexpr float kODJoin = 9e-4f;
 // bf16 parts of a weight: its 24 bits, as where values cancel an output shows what the weights are off by. Two, of
 // 16 bits, take 1 to 4 % less (8 x 14,402 tokens 45.7 and 45.9 us, 61 of 70 to 2,900 37.0 and 37.3, 6 x 5 queries
-// of 256 dims 26.3 and 27.3), 9 % where 64 rows share a KV head (60 x 8 over 1,500 keys 66.1 and 72.3).
+// of 256 dims 26.3 and 27.3), 9 % where 64 rows share a KV head (60 x 8 over 1,500 keys 66.1 and 72.3); the pairs of figures elsewhere in this
+// file compare variants of two parts.
 constexpr int kODParts = 3;
 constexpr float kLog2e = 1.4426950408889634f;
 
