@@ -1070,6 +1070,26 @@ def test_wrapper_refusals():
             kernels.octet_read_paged(st.lay, st.page, 16, st.bt, one, 20, **kw)
 
 
+def test_wrappers_refuse_numbers_beyond_32_bits():
+    """(Cut to 32 bits each of these would be a call that runs.)"""
+    st = Store([20], 2, 64)
+    q, at = torch.zeros(1, 4, 64, dtype=torch.float16, device="cuda"), _i32([0, 1])
+    for block, longest, most in ((16, 2 ** 32 + 20, 1), (16, 20, 2 ** 32 + 1), (2 ** 32 + 16, 20, 1), (16, 2 ** 31, 1)):
+        with pytest.raises(ValueError, match="2.31"):
+            kernels.octet_decode_paged(st.lay, q, st.page, block, st.bt, st.seq, at, most, longest, 0.1)
+    for block, longest, rows in ((2 ** 32 + 16, 20, 20), (16, 2 ** 32 + 20, 20), (16, 20, 2 ** 32 + 20)):
+        with pytest.raises(ValueError, match="2.31"):
+            kernels.octet_read_paged(st.lay, st.page, block, st.bt, _i32([0, 20]), longest, num_rows=rows)
+    with pytest.raises(ValueError, match="2.31"):
+        kernels.octet_decode_workspace(st.lay, 4, 1, 1, 2 ** 32 + 20, "cuda")
+    N = 2 ** 32 + 1                                    # rows that are one row, so no memory
+    x, ids = q[:, :2].expand(N, 2, 64), torch.zeros(1, dtype=torch.int64, device="cuda")
+    with pytest.raises(ValueError, match="2.31"):
+        kernels.rotary_scaled(x, None, ids, scaled_rotary(64, device="cuda"))
+    with pytest.raises(ValueError, match="2.31"):
+        kernels.octet_write_paged(st.lay, x, x, ids, st.page)
+
+
 # ----------------------------------------------------------------------------------- together
 class Serving:
     """A server's layer over the 8-bit cache: each step plans its addresses, rotates and stores its

@@ -735,6 +735,13 @@ def nibble_prefill_paged(lay: NibbleLayout, query: torch.Tensor, page: torch.Ten
 
 
 # ---------------------------------------------------------------- the 8-bit cache
+def _in_32_bits(numbers):
+    """Refuse counts and lengths that the C entries' 32 bits do not hold (ctypes would cut them); given
+    or-ed together, a negative one is theirs to refuse."""
+    if numbers >> 31 > 0:
+        raise ValueError("counts and lengths must be below 2^31")
+
+
 def _turns(rotary, d, device_index, positions, N):
     """(positions, turns, rotary_dim, amplitude, adjacent) as the C entries take them."""
     turns, amplitude, adjacent = rotary
@@ -786,6 +793,7 @@ def rotary_scaled(query: torch.Tensor, key: torch.Tensor | None, positions: torc
     if len(shape) != 3:
         raise ValueError(f"query must be [N, heads, d], got {tuple(shape)}")
     N, HQ, d = shape
+    _in_32_bits(N)
     turned = _turns(rotary, d, index, positions, N)
     code = _hip.DTYPE_CODE.get(dtype)
     if code is None:
@@ -826,6 +834,7 @@ def octet_write_paged(lay: OctetLayout, key: torch.Tensor, value: torch.Tensor,
                         value_out, error_word)
     H, d = lay.H, lay.d
     N = key.shape[0] if key.dim() else 0
+    _in_32_bits(N)
     shape, k_dtype, v_dtype = (N, H, d), key.dtype, value.dtype
     k_code, v_code = _hip.DTYPE_CODE.get(k_dtype), _hip.DTYPE_CODE.get(v_dtype)
     if k_code is None or v_code is None:
@@ -894,6 +903,7 @@ def octet_read_paged(lay: OctetLayout, page: torch.Tensor, block_size: int,
     code = _hip.DTYPE_CODE.get(dtype)
     if code is None:
         raise ValueError("key_out / value_out dtype must be fp32, fp16 or bf16")
+    _in_32_bits(num_rows | int(max_seq_len) | int(block_size))
     shape = (num_rows, lay.H, lay.d)
     if key_out is None:
         key_out = page.new_empty(shape, dtype=dtype)
@@ -916,6 +926,7 @@ def octet_decode_workspace(lay: OctetLayout, num_heads: int, num_reqs: int, max_
                            max_seq_len: int, device) -> torch.Tensor:
     """A workspace for `octet_decode_paged` over batches of up to this shape (see
     `nibble_decode_workspace`; one buffer may serve the reads of both caches, in stream order)."""
+    _in_32_bits(num_reqs | max_q_len | max_seq_len)
     n = _hip.lib().ttkv_octet_decode_workspace_bytes(lay.H, num_heads, lay.d, num_reqs, max_q_len,
                                                      max_seq_len)
     if n < 0:
@@ -959,6 +970,7 @@ def octet_decode_paged(lay: OctetLayout, query: torch.Tensor, page: torch.Tensor
     if lse is not None and (lse.dtype != torch.float32 or lse.shape != (N, HQ)
                             or not lse.is_contiguous()):
         raise ValueError(f"lse must be contiguous fp32 [{N}, {HQ}]")
+    _in_32_bits(N | int(max_q_len) | int(max_seq_len) | int(block_size))
     page_args = _octet_page(page, lay)
     if N == 0:                                  # every request waits
         return out
